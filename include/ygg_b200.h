@@ -189,6 +189,37 @@ YGG_API void ygg_ffree(ygg_fmodel *m);
 /* Free the device memory of a model; NULL is a no-op. */
 YGG_API void ygg_free(ygg_model *m);
 
+/* ---- what a step's answer is worth: log-probabilities, entropy, alternatives --------------------------------------
+ * Additions of this library (the reference sums the bits of a row: yggdrasil/inference.py:82-90). The calls below take
+ * no model: `device` is the CUDA device of the pointers. */
+#define YGG_DTYPE_FLOAT 0
+#define YGG_DTYPE_HALF 1
+#define YGG_DTYPE_BFLOAT 2
+#define YGG_TOP_MAX 64          /* most alternatives of a call */
+
+/* For each row of logits (dtype, `row_stride` entries apart, the entries of a row side by side):
+ *   d_logprob  float [rows]  log softmax(row)[token]; 0 where the token is negative (padding), NaN where it is >= vocab
+ *   d_entropy  float [rows]  -sum p log p         d_lse  float [rows]  log sum exp
+ *   d_top_ids int32 [rows][top], d_top_logprobs float [rows][top]: the largest entries, descending, ties by the lower
+ *                            index; 0 <= top <= min(vocab, YGG_TOP_MAX)
+ *   d_stats    float [rows][4], 16-byte aligned: what ygg_token_logprobs_backward needs; or NULL
+ *   d_tokens   int32 or int64 (token_bytes 4 or 8) [rows]
+ * -inf entries have probability 0; a row of -inf alone gives logprob and lse -inf and entropy 0; a row that holds NaN or
+ * +inf gives NaN values (NaN ranks as -inf among the alternatives). */
+YGG_API int ygg_token_logprobs(int device, int dtype, int64_t rows, int64_t vocab, const void *d_logits,
+                               int64_t row_stride, const void *d_tokens, int token_bytes, int top, float *d_logprob,
+                               float *d_entropy, float *d_lse, int32_t *d_top_ids, float *d_top_logprobs,
+                               float *d_stats, void *stream);
+
+/* The gradient of ygg_token_logprobs with respect to the logits (same dtype, rows `grad_stride` entries apart; may not
+ * overlap the logits), from the gradients that arrive at its outputs (float [rows], d_grad_top float [rows][top]; each
+ * may be NULL: zero) and the d_stats and d_top_ids that it wrote. Empty rows get zeros. */
+YGG_API int ygg_token_logprobs_backward(int device, int dtype, int64_t rows, int64_t vocab, const void *d_logits,
+                                        int64_t row_stride, const void *d_tokens, int token_bytes, int top,
+                                        const int32_t *d_top_ids, const float *d_stats, const float *d_grad_logprob,
+                                        const float *d_grad_entropy, const float *d_grad_lse, const float *d_grad_top,
+                                        void *d_grad, int64_t grad_stride, void *stream);
+
 /* Text of an error code. */
 YGG_API const char *ygg_strerror(int code);
 

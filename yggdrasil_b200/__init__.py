@@ -5,4 +5,15 @@ Python host side, shaped as the reference's inference API (``Yggdrasil.load(path
 """
 from .inference import B200Yggdrasil, Yggdrasil  # noqa: F401
 
-__all__ = ["Yggdrasil", "B200Yggdrasil"]
+__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs"]
+
+_OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs"}
+
+
+def __getattr__(name):   # the operators import torch; the package itself does not
+    if name in _OPERATORS:
+        from importlib import import_module
+        value = getattr(import_module("." + _OPERATORS[name], __name__), name)
+        globals()[name] = value
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

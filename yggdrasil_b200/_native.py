@@ -12,7 +12,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libygg_b200.so"
 
 EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "ygg_score_grouped_workspace",
            "ygg_score_grouped", "ygg_score_grouped_noalloc", "ygg_status", "ygg_selftest_wait", "ygg_free",
-           "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree")
+           "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree",
+           "ygg_token_logprobs", "ygg_token_logprobs_backward")
 
 YGG_OK = 0
 YGG_E_ARG, YGG_E_FORMAT, YGG_E_UNSUPPORTED, YGG_E_MISSING, YGG_E_CUDA, YGG_E_OOM, YGG_E_TOKEN, YGG_E_TIMEOUT, \
@@ -87,6 +88,23 @@ def flib() -> ctypes.CDLL:
         for f in (l.ygg_fload, l.ygg_fstep, l.ygg_fstep_stats, l.ygg_fstatus):
             f.restype = ctypes.c_int
         _float_bound = True
+    return l
+
+
+_ops_bound = False
+
+
+def ops() -> ctypes.CDLL:
+    """The loaded library with the entry points of the operators (no model handle) bound."""
+    global _ops_bound
+    l = lib()
+    if not _ops_bound:
+        vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+        l.ygg_token_logprobs.argtypes = [i32, i32, i64, i64, vp, i64, vp, i32, i32] + [vp] * 7
+        l.ygg_token_logprobs_backward.argtypes = [i32, i32, i64, i64, vp, i64, vp, i32, i32] + [vp] * 7 + [i64, vp]
+        for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward):
+            f.restype = i32
+        _ops_bound = True
     return l
 
 
