@@ -220,6 +220,33 @@ YGG_API int ygg_token_logprobs_backward(int device, int dtype, int64_t rows, int
                                         const float *d_grad_entropy, const float *d_grad_lse, const float *d_grad_top,
                                         void *d_grad, int64_t grad_stride, void *stream);
 
+/* ---- linear layers in 8-bit integers -------------------------------------------------------------------------------
+ * Row m of x has the scale max|x_m| / 127 and the codes rint(x 127 / max|x_m|); y = (codes . weight row) row_scale scale
+ * + bias, the sum exact in int32. A row of zeros has scale 0; a row that holds NaN or infinity has scale NaN (its
+ * outputs are NaN). Codes and weights are rows of bytes, their base and stride multiples of 16; bytes of a row past k
+ * are ignored. k is at most YGG_LINEAR_MAX_K. */
+#define YGG_LINEAR_MAX_K 131072
+
+/* d_codes int8 [rows][code_stride], zeros written from k up to the next multiple of 16; d_scale float [rows]. */
+YGG_API int ygg_quantize_rows(int device, int dtype, int64_t rows, int64_t k, const void *d_x, int64_t row_stride,
+                              int8_t *d_codes, int64_t code_stride, float *d_scale, void *stream);
+
+/* d_out (out_dtype) [rows], out_stride entries apart: the product of quantised rows with a weight int8 [n]
+ * [weight_stride], d_scale float [n], d_bias float [n] or NULL. */
+YGG_API int ygg_linear_quantized(int device, int64_t rows, int64_t k, int64_t n, const int8_t *d_codes,
+                                 int64_t code_stride, const float *d_row_scale, const int8_t *d_weight,
+                                 int64_t weight_stride, const float *d_scale, const float *d_bias, int out_dtype,
+                                 void *d_out, int64_t out_stride, void *stream);
+
+/* Bytes of device workspace ygg_linear needs; 0 for sizes that it refuses. */
+YGG_API size_t ygg_linear_workspace(int64_t rows, int64_t k);
+
+/* ygg_quantize_rows and ygg_linear_quantized in one call; d_workspace: ygg_linear_workspace bytes, 16-byte aligned. */
+YGG_API int ygg_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, const void *d_x, int64_t row_stride,
+                       const int8_t *d_weight, int64_t weight_stride, const float *d_scale, const float *d_bias,
+                       int out_dtype, void *d_out, int64_t out_stride, void *d_workspace, size_t workspace_bytes,
+                       void *stream);
+
 /* Text of an error code. */
 YGG_API const char *ygg_strerror(int code);
 

@@ -5,9 +5,10 @@ Python host side, shaped as the reference's inference API (``Yggdrasil.load(path
 """
 from .inference import B200Yggdrasil, Yggdrasil  # noqa: F401
 
-__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs"]
+__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs", "int8_linear", "quantize_rows"]
 
-_OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs"}
+_OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs",
+              "int8_linear": "linear", "quantize_rows": "linear", "QuantizedRows": "linear"}
 
 
 def __getattr__(name):   # the operators import torch; the package itself does not

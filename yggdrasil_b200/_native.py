@@ -13,7 +13,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libygg_b200.so"
 EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "ygg_score_grouped_workspace",
            "ygg_score_grouped", "ygg_score_grouped_noalloc", "ygg_status", "ygg_selftest_wait", "ygg_free",
            "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree",
-           "ygg_token_logprobs", "ygg_token_logprobs_backward")
+           "ygg_token_logprobs", "ygg_token_logprobs_backward", "ygg_quantize_rows", "ygg_linear_workspace",
+           "ygg_linear_quantized", "ygg_linear")
 
 YGG_OK = 0
 YGG_E_ARG, YGG_E_FORMAT, YGG_E_UNSUPPORTED, YGG_E_MISSING, YGG_E_CUDA, YGG_E_OOM, YGG_E_TOKEN, YGG_E_TIMEOUT, \
@@ -102,7 +103,14 @@ def ops() -> ctypes.CDLL:
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
         l.ygg_token_logprobs.argtypes = [i32, i32, i64, i64, vp, i64, vp, i32, i32] + [vp] * 7
         l.ygg_token_logprobs_backward.argtypes = [i32, i32, i64, i64, vp, i64, vp, i32, i32] + [vp] * 7 + [i64, vp]
-        for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward):
+        l.ygg_quantize_rows.argtypes = [i32, i32, i64, i64, vp, i64, vp, i64, vp, vp]
+        l.ygg_linear_workspace.argtypes = [i64, i64]
+        l.ygg_linear_workspace.restype = ctypes.c_size_t
+        l.ygg_linear_quantized.argtypes = [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, vp]
+        l.ygg_linear.argtypes = [i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64, vp, ctypes.c_size_t,
+                                 vp]
+        for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward, l.ygg_quantize_rows, l.ygg_linear_quantized,
+                  l.ygg_linear):
             f.restype = i32
         _ops_bound = True
     return l

@@ -11,17 +11,16 @@
 // Edge rules: -inf entries have probability 0 and add nothing; a row of -inf alone is empty (logprob and lse -inf,
 // entropy 0, gradient 0); NaN or +inf anywhere makes the row's values NaN, and NaN ranks as -inf among the
 // alternatives. A negative token is padding (logprob 0, no gradient), a token >= V gives NaN.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
 
-#include "ygg_b200.h"
+#include "ygg_ops.cuh"
 
 namespace {
+
+using namespace ygg;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -200.0f;   // e^-200 is 0 in 32 bits: y below it only has to stay finite
@@ -48,13 +47,6 @@ struct Grad {
     void *grad;
     int64_t grad_stride;
 };
-
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_f(float v, float &o) { o = v; }
-__device__ __forceinline__ void from_f(float v, __half &o) { o = __float2half_rn(v); }
-__device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -191,27 +183,6 @@ template <typename T> __global__ void __launch_bounds__(256) logprobs_grad_kerne
                     if (p.top_ids[row * p.top + k] == j) more += p.g_top[row * p.top + k];
             from_f(dense(to_f(x[j]), st.x, st.y, A, B) + more, g[j]);
         }
-    }
-}
-
-struct OnDevice {   // the calling thread's device for the length of a call
-    int prev = -1;
-    bool ok;
-    explicit OnDevice(int device) {
-        ok = cudaGetDevice(&prev) == cudaSuccess && (prev == device || cudaSetDevice(device) == cudaSuccess);
-        if (prev == device) prev = -1;
-    }
-    ~OnDevice() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
-
-template <typename F> int by_type(int dtype, F f) {
-    switch (dtype) {
-        case YGG_DTYPE_FLOAT: f(float()); return YGG_OK;
-        case YGG_DTYPE_HALF: f(__half()); return YGG_OK;
-        case YGG_DTYPE_BFLOAT: f(__nv_bfloat16()); return YGG_OK;
-        default: return YGG_E_UNSUPPORTED;
     }
 }
 
