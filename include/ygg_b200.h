@@ -247,6 +247,57 @@ YGG_API int ygg_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n
                        int out_dtype, void *d_out, int64_t out_stride, void *d_workspace, size_t workspace_bytes,
                        void *stream);
 
+/* ---- the pages of a cache of stream states -------------------------------------------------------------------------
+ * A page is one stream's state; a stream holds the pages table[s][0 .. length[s]) (-1 beyond), the last of them its live
+ * state, its own; the ones before are snapshots that streams may share. refs[p] counts the table entries that hold page
+ * p. Sources and counts of one call are those of its beginning; new pages are the free ones in ascending order, given
+ * in the order of the call's list. Negative stream and page indices are padding and skipped. What cannot be done is left
+ * undone and sets a status word to 1: status[YGG_CACHE_BAD_INDEX] (an index beyond its range, a child that holds pages, a
+ * child named twice: its first fork counts), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row). Calls
+ * on one cache are ordered by the caller (one stream, or events). */
+#define YGG_CACHE_BAD_INDEX 0
+#define YGG_CACHE_NO_ROOM 1
+
+typedef struct {
+    void *pages;             /* page_count pages of page_bytes */
+    int64_t page_count, page_bytes;
+    int32_t *table;          /* [streams][per_stream] */
+    int64_t streams;
+    int32_t per_stream;
+    int32_t *length;         /* [streams] */
+    int32_t *refs;           /* [page_count] */
+    int32_t *status;         /* two words, on the device or mapped host memory (pinned); the caller clears them */
+} ygg_cache_t;
+
+/* Bytes of device workspace of ygg_cache_fork with n entries, and of ygg_cache_compact (any n). */
+YGG_API size_t ygg_cache_workspace(const ygg_cache_t *cache, int64_t n);
+
+/* d_children != NULL: the empty stream d_children[i] becomes a copy of d_parents[i] (of its first d_depth[i] pages, all
+ * of them where d_depth is NULL): all pages but the last shared, the last copied into a new page. A parent without pages
+ * gives a child without pages. d_children == NULL: stream d_parents[i] gets one more page, a copy of its last one (zeros
+ * for its first). */
+YGG_API int ygg_cache_fork(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_parents,
+                           const int32_t *d_children, const int32_t *d_depth, void *d_workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* The streams let go of their pages. */
+YGG_API int ygg_cache_free(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_streams,
+                           void *stream);
+
+/* Moves the live pages to the front, [0, *d_live): the k-th free page below takes over from the k-th live page above.
+ * Tables and counts follow. */
+YGG_API int ygg_cache_compact(int device, const ygg_cache_t *cache, int32_t *d_live, void *d_workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* The live states of streams into a batch [n][page_bytes] (zeros for a stream without pages) and back (skipped for
+ * such a stream). */
+YGG_API int ygg_cache_read(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_streams, void *d_batch, void *stream);
+YGG_API int ygg_cache_write(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_streams,
+                            const void *d_batch, void *stream);
+
+/* Page d_to[i] = page d_from[i]. No page may be named as a destination and anywhere else. */
+YGG_API int ygg_cache_copy(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_from, const int32_t *d_to, void *stream);
+
 /* Text of an error code. */
 YGG_API const char *ygg_strerror(int code);
 

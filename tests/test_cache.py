@@ -1,0 +1,367 @@
+"""StateCache against a plain cache of Python lists, bit for bit: pages, tables, lengths and counts after each call."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from yggdrasil_b200 import _native
+
+
+def cache_class():
+    from yggdrasil_b200 import StateCache
+    return StateCache
+
+
+class Plain:
+    """The definition: a list of page contents, tables, and counts; new pages are the lowest free ones in order."""
+
+    def __init__(self, pages, streams, per_stream):
+        self.pages = pages.cpu().numpy().copy()
+        self.table, self.m = [[] for _ in range(streams)], per_stream
+        self.bad = self.full = False
+
+    def refs(self):
+        r = [0] * len(self.pages)
+        for row in self.table:
+            for p in row:
+                r[p] += 1
+        return r
+
+    def free_pages(self):
+        return [p for p, r in enumerate(self.refs()) if r == 0]
+
+    def known(self, *streams):
+        if any(s < 0 for s in streams):
+            return False
+        if any(s >= len(self.table) for s in streams):
+            self.bad = True
+            return False
+        return True
+
+    def fork(self, parents, children, depth=None):
+        before, spare, taken = [list(r) for r in self.table], self.free_pages(), set()
+        for i, (p, c) in enumerate(zip(parents, children)):
+            if not self.known(p, c):
+                continue
+            row = before[p] if depth is None else before[p][:max(0, depth[i])]
+            if not row:
+                continue
+            if before[c] or c in taken:
+                self.bad = True
+                continue
+            taken.add(c)
+            if not spare:
+                self.full = True
+                continue
+            new = spare.pop(0)
+            self.pages[new] = self.pages[row[-1]]
+            self.table[c] = row[:-1] + [new]
+
+    def grow(self, streams):
+        before, spare, taken = [list(r) for r in self.table], self.free_pages(), set()
+        for s in streams:
+            if not self.known(s):
+                continue
+            if len(before[s]) >= self.m:
+                self.full = True
+                continue
+            if s in taken:
+                self.bad = True
+                continue
+            taken.add(s)
+            if not spare:
+                self.full = True
+                continue
+            new = spare.pop(0)
+            self.pages[new] = self.pages[before[s][-1]] if before[s] else 0
+            self.table[s] = before[s] + [new]
+
+    def free(self, streams):
+        for s in streams:
+            if self.known(s):
+                self.table[s] = []
+
+    def compact(self):
+        r = self.refs()
+        n = sum(v > 0 for v in r)
+        high = [p for p in range(n, len(r)) if r[p] > 0]
+        new = dict(zip(high, [p for p in range(n) if r[p] == 0]))
+        for p, q in new.items():
+            self.pages[q] = self.pages[p]
+        self.table = [[new.get(p, p) for p in row] for row in self.table]
+        return n
+
+    def read(self, streams):
+        rows = [self.table[s] if self.known(s) else [] for s in streams]
+        return np.stack([self.pages[r[-1]] if r else np.zeros_like(self.pages[0]) for r in rows])
+
+    def write(self, streams, batch):
+        for s, b in zip(streams, batch):
+            if self.known(s) and self.table[s]:
+                self.pages[self.table[s][-1]] = b
+
+
+def pair(pages, streams, per_stream, shape=(4, 8), dtype=torch.int8, seed=0):
+    cache = cache_class().empty(pages, streams, per_stream, shape=shape, dtype=dtype, device="cuda")
+    g = torch.Generator().manual_seed(seed)
+    data = torch.randint(-100, 100, (pages, *shape), generator=g).to(dtype)
+    cache.pages.copy_(data)
+    return cache, Plain(data, streams, per_stream)
+
+
+def same(cache, plain):
+    want = torch.full((len(plain.table), plain.m), -1, dtype=torch.int32)
+    for s, row in enumerate(plain.table):
+        want[s, :len(row)] = torch.tensor(row, dtype=torch.int32)
+    assert torch.equal(cache.table.cpu(), want)
+    assert cache.length.tolist() == [len(r) for r in plain.table]
+    assert cache.refs.tolist() == plain.refs()
+    assert np.array_equal(cache.pages.cpu().numpy(), plain.pages)
+    raised = None
+    try:
+        cache.status()
+    except (ValueError, RuntimeError) as e:
+        raised = e
+    assert isinstance(raised, ValueError) == plain.bad
+    assert isinstance(raised, RuntimeError) == (plain.full and not plain.bad)
+    plain.bad = plain.full = False
+
+
+SHAPES = [((4, 128), torch.int8), ((5, 256), torch.float32), ((3, 96), torch.bfloat16), ((1, 1), torch.int8),
+          ((3, 7), torch.int8), ((5, 3), torch.float16), ((1, 5), torch.float32), ((2, 64), torch.float64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dtype", SHAPES)
+@pytest.mark.parametrize("streams,per_stream,pages", [(1, 1, 1), (3, 2, 5), (40, 3, 70), (1500, 2, 2500)])
+def test_random_calls(streams, per_stream, pages, shape, dtype):
+    cache, plain = pair(pages, streams, per_stream, shape, dtype)
+    rng = np.random.default_rng(streams)
+    some = lambda: rng.integers(-1, streams, rng.integers(0, streams + 2)).tolist()  # noqa: E731 (repeats among them)
+    for step in range(14):
+        what = ["grow", "fork", "deep", "free", "compact", "write", "read"][step % 7 if step < 7 else rng.integers(0, 7)]
+        a = some()
+        if what == "grow":
+            cache.grow(a), plain.grow(a)
+        elif what in ("fork", "deep"):
+            b = rng.integers(-1, streams, len(a)).tolist()
+            d = rng.integers(0, per_stream + 2, len(a)).tolist() if what == "deep" else None
+            cache.fork(a, b, d), plain.fork(a, b, d)
+        elif what == "free":
+            a = a[:len(a) // 2]
+            cache.free(a), plain.free(a)
+        elif what == "compact":
+            live = plain.compact()
+            assert int(cache.compact()) == live
+            assert not any(plain.refs()[live:]) and all(plain.refs()[:live])
+        elif what == "write":
+            a = list(dict.fromkeys(s for s in a if s >= 0))
+            batch = torch.randint(-50, 50, (len(a), *shape)).to(dtype)
+            cache.write(a, batch.cuda()), plain.write(a, batch.float().numpy() if dtype == torch.bfloat16 else
+                                                      batch.numpy())
+        else:
+            got = cache.read(a).cpu()
+            if a:
+                assert np.array_equal(_np(got), plain.read(a))
+        same_any(cache, plain)
+
+
+def _np(t):
+    return t.float().numpy() if t.dtype == torch.bfloat16 else t.numpy()
+
+
+def same_any(cache, plain):
+    if cache.pages.dtype == torch.bfloat16:
+        view = type("View", (), dict(table=cache.table, length=cache.length, refs=cache.refs, pages=cache.pages.float(),
+                                     status=cache.status))
+        return same(view, plain)
+    return same(cache, plain)
+
+
+@pytest.fixture(autouse=True)
+def _bfloat16_as_float(monkeypatch):
+    keep = Plain.__init__
+
+    def init(self, pages, streams, per_stream):
+        keep(self, pages.float() if pages.dtype == torch.bfloat16 else pages, streams, per_stream)
+    monkeypatch.setattr(Plain, "__init__", init)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("streams", [8, 1023, 1025, 5000])
+def test_fork_shares_the_snapshots_and_copies_the_last_page(streams):
+    cache, plain = pair(streams * 4, streams * 2, 3, seed=2)
+    a = list(range(streams))
+    for c in (cache, plain):
+        c.grow(a)
+        c.grow(a[::2])
+        c.grow(a[::4])
+        c.fork([x % 7 for x in a], [streams + x for x in a])
+    same(cache, plain)
+    for c in (cache, plain):
+        c.free(a[1::2] + [0, 0, 1])
+    same(cache, plain)
+    assert int(cache.compact()) == plain.compact()
+    same(cache, plain)
+
+
+@pytest.mark.gpu
+def test_a_pool_without_room_serves_the_first_and_reports():
+    cache, plain = pair(6, 10, 1)
+    for c in (cache, plain):
+        c.grow([0, 1, 2, 3])
+        c.fork([0, 1, 2, 3, 0], [4, 5, 6, 7, 8])
+    same(cache, plain)
+    assert cache.length.tolist() == [1] * 6 + [0] * 4
+    for c in (cache, plain):
+        c.grow([0, 7])
+    same(cache, plain)
+
+
+@pytest.mark.gpu
+def test_what_cannot_be_done_is_left_undone():
+    cache, plain = pair(20, 6, 2)
+    for c in (cache, plain):
+        c.grow([0, 1])
+    same(cache, plain)
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for parents, children in (([0, 1], [1, 2]), ([0, 1], [3, 3]), ([0, 4], [4, 5]), ([7, 0], [4, 6]), ([-1, 0], [5, -3])):
+        cache.fork(dev(parents), dev(children))
+        plain.fork(parents, children)
+        same(cache, plain)
+    cache.free(dev([9, -1, 2, 2])), plain.free([9, -1, 2, 2])
+    same(cache, plain)
+    cache.grow(dev([0, 0, 6])), plain.grow([0, 0, 6])
+    same(cache, plain)
+    assert np.array_equal(cache.read(dev([6, 0, -1])).cpu().numpy(), plain.read([6, 0, -1]))
+    same(cache, plain)
+
+
+@pytest.mark.gpu
+def test_copy_of_pages():
+    cache, plain = pair(50, 1, 1, shape=(3, 5))
+    cache.copy([0, 1, 2, -1, 5], [10, 11, 12, 13, -1])
+    for a, b in ((0, 10), (1, 11), (2, 12)):
+        plain.pages[b] = plain.pages[a]
+    same(cache, plain)
+    cache.copy(torch.tensor([3, 60], device="cuda"), torch.tensor([14, 15], device="cuda"))
+    plain.pages[14] = plain.pages[3]
+    plain.bad = True
+    same(cache, plain)
+
+
+@pytest.mark.gpu
+def test_compact_of_none_all_and_the_far_end():
+    cache, plain = pair(3000, 3000, 1)
+    assert int(cache.compact()) == plain.compact() == 0
+    same(cache, plain)
+    for c in (cache, plain):
+        c.grow(list(range(3000)))
+    assert int(cache.compact()) == plain.compact() == 3000
+    same(cache, plain)
+    for c in (cache, plain):
+        c.free(list(range(2999)))
+    assert int(cache.compact()) == plain.compact() == 1
+    same(cache, plain)
+
+
+@pytest.mark.gpu
+def test_pages_beyond_32_bits_of_bytes():
+    """A pool of 5 GB: the copies go beyond byte 2^32."""
+    shape, pages = (1024, 1280), 4096
+    cache = cache_class().empty(pages, 4100, 1, shape=shape, dtype=torch.int8, device="cuda")
+    cache.grow(np.arange(pages - 1))
+    cache.write([pages - 2], torch.full((1, *shape), 7, dtype=torch.int8, device="cuda"))
+    cache.fork([pages - 2], [4099])
+    assert cache.table[4099].item() == pages - 1 and bool((cache.pages[pages - 1] == 7).all())
+    cache.free(np.arange(pages - 1))
+    assert int(cache.compact()) == 1 and bool((cache.pages[0] == 7).all()) and cache.table[4099].item() == 0
+    cache.status()
+
+
+@pytest.mark.gpu
+def test_around_tensors_on_another_stream_and_in_a_graph():
+    cls = cache_class()
+    made = cls.empty(400, 300, 2, shape=(4, 128), dtype=torch.int8, device="cuda")
+    made.pages.random_(-100, 100)
+    made.grow(np.arange(100))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache = cls(made.pages, made.table, made.length, made.refs)
+        cache.fork(np.arange(100), np.arange(100, 200))
+        cache.status()
+    assert torch.equal(cache.read(np.arange(100)), cache.read(np.arange(100, 200)))
+    # a graph of a step's housekeeping, replayed: fork, free, compact
+    parents = torch.arange(50, dtype=torch.int32, device="cuda")
+    children = parents + 200
+    cache.fork(parents, children)
+    cache.free(children)
+    cache.compact()
+    keep = [t.clone() for t in (cache.table, cache.length, cache.refs)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.fork(parents, children)
+        cache.free(children)
+        live = cache.compact()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert int(live) == 200
+    for a, b in zip(keep, (cache.table, cache.length, cache.refs)):
+        assert torch.equal(a, b)
+    cache.status()
+
+
+@pytest.mark.gpu
+def test_refusals():
+    cls = cache_class()
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages = torch.zeros(8, 4, 16, dtype=torch.int8, device="cuda")
+    cls(pages, ints(3, 2), ints(3), ints(8))
+    for bad in ((pages.cpu(), ints(3, 2), ints(3), ints(8)), (pages[:, :, 1:], ints(3, 2), ints(3), ints(8)),
+                (pages, ints(3), ints(3), ints(8)), (pages, ints(3, 2).long(), ints(3), ints(8)),
+                (pages, ints(3, 2), ints(4), ints(8)), (pages, ints(3, 2), ints(3), ints(7)),
+                (pages, ints(2, 3).T, ints(3), ints(8)), (pages, ints(3, 2), ints(3), ints(8).cpu())):
+        with pytest.raises(ValueError):
+            cls(*bad)
+    with pytest.raises(ValueError):
+        cls.empty(0, 3, shape=(2,), device="cuda")
+    with pytest.raises(ValueError):
+        cls.empty(4, 3, shape=(2,), device="cpu")
+    cache = cls.empty(8, 4, 1, shape=(2, 3), dtype=torch.int8, device="cuda")
+    for call in (lambda: cache.fork([0], [1, 2]), lambda: cache.fork([0], [4]), lambda: cache.grow([4]),
+                 lambda: cache.grow([[0]]), lambda: cache.free([0.5]), lambda: cache.free(torch.zeros(2, device="cuda")),
+                 lambda: cache.write([0], torch.zeros(1, 2, 4, dtype=torch.int8, device="cuda")),
+                 lambda: cache.write([0], torch.zeros(1, 2, 3, device="cuda")), lambda: cache.copy([0], [8]),
+                 lambda: cache.copy([0, 1], [2])):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_c_entry_refuses_bad_arguments():
+    """Checked before any CUDA call."""
+    lib, E, p = _native.ops(), _native, 4096
+    good = lambda: _native.YggCache(p, 8, 16, p, 4, 2, p, p, p)  # noqa: E731
+    size = lib.ygg_cache_workspace(ctypes.byref(good()), 5)
+    assert size > 0 and lib.ygg_cache_workspace(None, 5) == 0 and lib.ygg_cache_workspace(ctypes.byref(good()), -1) == 0
+    assert lib.ygg_cache_fork(0, None, 1, p, p, None, p, size, None) == E.YGG_E_ARG
+    for field, value in (("pages", None), ("page_count", 0), ("page_count", 1 << 31), ("page_bytes", 0), ("table", None),
+                         ("streams", 0), ("per_stream", 0), ("length", None), ("refs", None), ("status", None)):
+        c = good()
+        setattr(c, field, value)
+        assert lib.ygg_cache_free(0, ctypes.byref(c), 1, p, None) == E.YGG_E_ARG
+        assert lib.ygg_cache_compact(0, ctypes.byref(c), p, p, 1 << 20, None) == E.YGG_E_ARG
+    c = ctypes.byref(good())
+    assert lib.ygg_cache_fork(0, c, -1, p, p, None, p, size, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_fork(0, c, 1, None, p, None, p, size, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_fork(0, c, 1, p, p, None, None, size, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_fork(0, c, 5, p, p, None, p, 8, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_fork(0, c, 0, None, None, None, None, 0, None) == E.YGG_OK
+    assert lib.ygg_cache_free(0, c, 1, None, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_compact(0, c, None, p, size, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_read(0, c, 1, None, p, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_write(0, c, 1, p, None, None) == E.YGG_E_ARG
+    assert lib.ygg_cache_copy(0, c, 1, p, None, None) == E.YGG_E_ARG

@@ -5,10 +5,11 @@ Python host side, shaped as the reference's inference API (``Yggdrasil.load(path
 """
 from .inference import B200Yggdrasil, Yggdrasil  # noqa: F401
 
-__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs", "int8_linear", "quantize_rows"]
+__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs", "int8_linear", "quantize_rows", "StateCache"]
 
 _OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs",
-              "int8_linear": "linear", "quantize_rows": "linear", "QuantizedRows": "linear"}
+              "int8_linear": "linear", "quantize_rows": "linear", "QuantizedRows": "linear",
+              "StateCache": "cache"}
 
 
 def __getattr__(name):   # the operators import torch; the package itself does not

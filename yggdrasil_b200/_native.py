@@ -14,7 +14,8 @@ EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "y
            "ygg_score_grouped", "ygg_score_grouped_noalloc", "ygg_status", "ygg_selftest_wait", "ygg_free",
            "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree",
            "ygg_token_logprobs", "ygg_token_logprobs_backward", "ygg_quantize_rows", "ygg_linear_workspace",
-           "ygg_linear_quantized", "ygg_linear")
+           "ygg_linear_quantized", "ygg_linear", "ygg_cache_workspace", "ygg_cache_fork", "ygg_cache_free",
+           "ygg_cache_compact", "ygg_cache_read", "ygg_cache_write", "ygg_cache_copy")
 
 YGG_OK = 0
 YGG_E_ARG, YGG_E_FORMAT, YGG_E_UNSUPPORTED, YGG_E_MISSING, YGG_E_CUDA, YGG_E_OOM, YGG_E_TOKEN, YGG_E_TIMEOUT, \
@@ -27,6 +28,12 @@ class YggInfo(ctypes.Structure):
         "router_token_dim", "input_rank", "shift", "n_experts", "vocab_pad", "factored", "group_scales")] + [
         ("file_array_bytes", ctypes.c_int64), ("device_bytes", ctypes.c_int64), ("record_bytes", ctypes.c_int32),
         ("warps_per_block", ctypes.c_int32), ("slots_per_block", ctypes.c_int32)]
+
+
+class YggCache(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("page_count", ctypes.c_int64), ("page_bytes", ctypes.c_int64),
+                ("table", ctypes.c_void_p), ("streams", ctypes.c_int64), ("per_stream", ctypes.c_int32),
+                ("length", ctypes.c_void_p), ("refs", ctypes.c_void_p), ("status", ctypes.c_void_p)]
 
 
 class YggError(RuntimeError):
@@ -109,8 +116,18 @@ def ops() -> ctypes.CDLL:
         l.ygg_linear_quantized.argtypes = [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, vp]
         l.ygg_linear.argtypes = [i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64, vp, ctypes.c_size_t,
                                  vp]
+        size, cache = ctypes.c_size_t, ctypes.POINTER(YggCache)
+        l.ygg_cache_workspace.argtypes = [cache, i64]
+        l.ygg_cache_workspace.restype = size
+        l.ygg_cache_fork.argtypes = [i32, cache, i64, vp, vp, vp, vp, size, vp]
+        l.ygg_cache_free.argtypes = [i32, cache, i64, vp, vp]
+        l.ygg_cache_compact.argtypes = [i32, cache, vp, vp, size, vp]
+        l.ygg_cache_read.argtypes = [i32, cache, i64, vp, vp, vp]
+        l.ygg_cache_write.argtypes = [i32, cache, i64, vp, vp, vp]
+        l.ygg_cache_copy.argtypes = [i32, cache, i64, vp, vp, vp]
         for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward, l.ygg_quantize_rows, l.ygg_linear_quantized,
-                  l.ygg_linear):
+                  l.ygg_linear, l.ygg_cache_fork, l.ygg_cache_free, l.ygg_cache_compact, l.ygg_cache_read,
+                  l.ygg_cache_write, l.ygg_cache_copy):
             f.restype = i32
         _ops_bound = True
     return l

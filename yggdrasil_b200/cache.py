@@ -1,0 +1,183 @@
+"""A cache of stream states in pages: streams branch, end and move together without copying more than they must.
+
+    from yggdrasil_b200 import StateCache
+    cache = StateCache.empty(pages=4096, streams=1024, like=model.init_state(1))   # a page: one stream's state
+    cache.grow([0, 1])                    # streams 0 and 1 get their first page (zeros)
+    cache.fork([0, 0, 1], [2, 3, 4])      # 2 and 3 go on from 0, 4 from 1
+    state = cache.read([2, 3, 4])         # (3, layers, n), for model.step
+    cache.write([2, 3, 4], new_state)
+    cache.free([0, 1])
+    live = cache.compact()                # the live pages are cache.pages[:live] now
+    cache.status()                        # raises if a call met a bad index or had no room
+
+`table[s, :length[s]]` are the pages of stream s (-1 beyond). The last one is its live state, its own; those before are
+snapshots (`grow` leaves one behind), which forks share: `refs[p]` counts the table entries that hold page p. A fork may
+go back to a snapshot (`depth`). Everything stays on the device, on the current stream; the kernels are
+csrc/ygg_pages.cu. Calls on one cache are ordered by their stream; a cache used on several streams at once is the
+caller's to order.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _native
+from ._native import YggCache, check, ops
+from .inference import _raw_stream
+from .logprobs import _nothing
+
+_SLOTS = 1024
+_status: list = [None, _SLOTS]   # pinned words not handed out yet, and how many were
+
+
+def _status_words():
+    """Two zeroed int32 words that the device can write: pinned host memory, each handed out once."""
+    if _status[1] >= _SLOTS:
+        _status[:] = [torch.zeros((_SLOTS, 2), dtype=torch.int32).pin_memory(), 0]
+    words = _status[0][_status[1]]
+    _status[1] += 1
+    return words
+
+
+class StateCache:
+    def __init__(self, pages, table, length, refs):
+        """Around tensors that hold a cache already (updated in place): pages (P, ...) of any type, table (S, M), length
+        (S,) and refs (P,) int32, contiguous, on one CUDA device."""
+        if not isinstance(pages, torch.Tensor) or not pages.is_cuda or pages.dim() < 2 or not pages.is_contiguous() \
+                or pages.numel() == 0:
+            raise ValueError("pages must be a contiguous CUDA tensor (P, ...)")
+        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.numel() == 0:
+            raise ValueError("table must be an int32 tensor (streams, pages of a stream)")
+        count, (streams, m) = pages.shape[0], table.shape
+        for name, t, shape in (("table", table, (streams, m)), ("length", length, (streams,)), ("refs", refs, (count,))):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != shape \
+                    or t.device != pages.device or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {pages.device}")
+        self.pages, self.table, self.length, self.refs = pages, table, length, refs
+        self.device = pages.device
+        self._words = _status_words()
+        self._page_bytes = pages.numel() // count * pages.element_size()
+        self._c = YggCache(pages.data_ptr(), count, self._page_bytes, table.data_ptr(), streams, m, length.data_ptr(),
+                           refs.data_ptr(), self._words.data_ptr())
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, pages, streams, per_stream=1, like=None, shape=None, dtype=None, device=None):
+        """A cache without live pages. A page has `shape` and `dtype` (on `device`), or those of a state `like`
+        (1, layers, n) as model.init_state(1) gives it."""
+        if like is not None:
+            shape, dtype, device = like.shape[1:], like.dtype, like.device
+        if pages < 1 or streams < 1 or per_stream < 1 or shape is None:
+            raise ValueError("a cache needs pages, streams, a table row and the shape of a page")
+        device = torch.device(device if device is not None else "cuda")
+        if device.type != "cuda":
+            raise ValueError(f"device {device}: the cache lives on a CUDA device")
+        ints = lambda *size, v=0: torch.full(size, v, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(torch.empty((pages, *shape), dtype=dtype, device=device), ints(streams, per_stream, v=-1),
+                   ints(streams), ints(pages))
+
+    def _ids(self, ids, what, limit):
+        """Indices as a contiguous int32 tensor on the device; host indices are range-checked (negative: padding)."""
+        if isinstance(ids, torch.Tensor) and ids.is_cuda:
+            if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64) or ids.device != self.device:
+                raise ValueError(f"{what} must be a row of int32 or int64 on {self.device}")
+            return (ids if ids.dtype == torch.int32 else ids.clamp(-1, 2 ** 31 - 1).int()).contiguous()
+        host = np.asarray(ids)
+        if host.ndim != 1 or (host.size and host.dtype.kind not in "iu"):
+            raise ValueError(f"{what} must be a row of integers")
+        if host.size and host.max() >= limit:
+            raise ValueError(f"{what}: {int(host.max())} out of range [0, {limit})")
+        return torch.as_tensor(np.ascontiguousarray(host, np.int32)).to(self.device)
+
+    def _on(self):
+        return torch.cuda.device(self.device) if self.device.index != torch.cuda.current_device() else _nothing
+
+    def _workspace(self, n):
+        size = ops().ygg_cache_workspace(self._ref, n)
+        return torch.empty(size, dtype=torch.uint8, device=self.device), size
+
+    def _plan(self, parents, children, depth):
+        with self._on():
+            n = parents.shape[0]
+            ws, size = self._workspace(n)
+            check(ops().ygg_cache_fork(self.device.index, self._ref, n, parents.data_ptr(),
+                                       None if children is None else children.data_ptr(),
+                                       None if depth is None else depth.data_ptr(), ws.data_ptr(), size,
+                                       _raw_stream(self.device.index)), "ygg_cache_fork")
+
+    def fork(self, parents, children, depth=None):
+        """Stream children[i], which must hold no pages, goes on from parents[i]: it shares the parent's pages but the
+        last, which is copied into a new page. depth[i]: only the parent's first depth[i] pages (at least 1), so that
+        the child goes on from an earlier snapshot. A parent without pages leaves its child without."""
+        p = self._ids(parents, "parents", self._c.streams)
+        c = self._ids(children, "children", self._c.streams)
+        d = None if depth is None else self._ids(depth, "depth", 1 << 31)
+        if p.shape != c.shape or (d is not None and d.shape != p.shape):
+            raise ValueError("one child, and one depth, for each parent")
+        self._plan(p, c, d)
+
+    def grow(self, streams):
+        """Each stream gets one more page, a copy of its last (zeros for its first); the page before it stays as a
+        snapshot."""
+        self._plan(self._ids(streams, "streams", self._c.streams), None, None)
+
+    def free(self, streams):
+        """The streams let go of their pages; pages that nothing holds any more are free."""
+        s = self._ids(streams, "streams", self._c.streams)
+        with self._on():
+            check(ops().ygg_cache_free(self.device.index, self._ref, s.shape[0], s.data_ptr(),
+                                       _raw_stream(self.device.index)), "ygg_cache_free")
+
+    def compact(self):
+        """Moves the live pages to the front and renumbers the tables. Returns their number as an int32 tensor () on the
+        device: pages[:live] is one contiguous batch."""
+        with self._on():
+            live = torch.empty((), dtype=torch.int32, device=self.device)
+            ws, size = self._workspace(0)
+            check(ops().ygg_cache_compact(self.device.index, self._ref, live.data_ptr(), ws.data_ptr(), size,
+                                          _raw_stream(self.device.index)), "ygg_cache_compact")
+        return live
+
+    def read(self, streams):
+        """The live states of streams as a new batch (len(streams), ...); zeros for a stream without pages."""
+        s = self._ids(streams, "streams", self._c.streams)
+        with self._on():
+            batch = torch.empty((s.shape[0], *self.pages.shape[1:]), dtype=self.pages.dtype, device=self.device)
+            check(ops().ygg_cache_read(self.device.index, self._ref, s.shape[0], s.data_ptr(), batch.data_ptr(),
+                                       _raw_stream(self.device.index)), "ygg_cache_read")
+        return batch
+
+    def write(self, streams, batch):
+        """batch[i] becomes the live state of streams[i], a stream that holds pages; no stream named twice."""
+        s = self._ids(streams, "streams", self._c.streams)
+        if not isinstance(batch, torch.Tensor) or batch.dtype != self.pages.dtype or batch.device != self.device \
+                or batch.shape != (s.shape[0], *self.pages.shape[1:]):
+            raise ValueError(f"batch must be {self.pages.dtype} {(s.shape[0], *self.pages.shape[1:])} on {self.device}")
+        b = batch.contiguous()
+        with self._on():
+            check(ops().ygg_cache_write(self.device.index, self._ref, s.shape[0], s.data_ptr(), b.data_ptr(),
+                                        _raw_stream(self.device.index)), "ygg_cache_write")
+
+    def copy(self, source, target):
+        """Page target[i] becomes a copy of page source[i]; a target is named once, and is no source of the call."""
+        a = self._ids(source, "source", self._c.page_count)
+        b = self._ids(target, "target", self._c.page_count)
+        if a.shape != b.shape:
+            raise ValueError("one target for each source")
+        with self._on():
+            check(ops().ygg_cache_copy(self.device.index, self._ref, a.shape[0], a.data_ptr(), b.data_ptr(),
+                                       _raw_stream(self.device.index)), "ygg_cache_copy")
+
+    def status(self, clear=True):
+        """Raise if a call since the last clear met a bad index (ValueError) or had no page or table entry left
+        (RuntimeError); what such a call could do it did. Waits for the current stream."""
+        torch.cuda.current_stream(self.device).synchronize()
+        bad, full = self._words.tolist()
+        if clear:
+            self._words.zero_()
+        if bad:
+            raise ValueError("a stream or page was out of range, or a child held pages or was named twice")
+        if full:
+            raise _native.YggError(_native.YGG_E_CAPACITY, "StateCache: no free page, or a full table row")
