@@ -247,6 +247,10 @@ YGG_API int ygg_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n
                        int out_dtype, void *d_out, int64_t out_stride, void *d_workspace, size_t workspace_bytes,
                        void *stream);
 
+/* YGG_E_TIMEOUT if a bounded wait of a product on this device gave up since the last call (its outputs are not to be
+ * used), else YGG_OK; the record is then cleared. Synchronises `stream`. */
+YGG_API int ygg_linear_status(int device, void *stream, int *status_out);
+
 /* ---- the pages of a cache of stream states -------------------------------------------------------------------------
  * A page is one stream's state; a stream holds the pages table[s][0 .. length[s]) (-1 beyond), the last of them its live
  * state, its own; the ones before are snapshots that streams may share. refs[p] counts the table entries that hold page

@@ -14,7 +14,7 @@ EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "y
            "ygg_score_grouped", "ygg_score_grouped_noalloc", "ygg_status", "ygg_selftest_wait", "ygg_free",
            "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree",
            "ygg_token_logprobs", "ygg_token_logprobs_backward", "ygg_quantize_rows", "ygg_linear_workspace",
-           "ygg_linear_quantized", "ygg_linear", "ygg_cache_workspace", "ygg_cache_fork", "ygg_cache_free",
+           "ygg_linear_quantized", "ygg_linear", "ygg_linear_status", "ygg_cache_workspace", "ygg_cache_fork", "ygg_cache_free",
            "ygg_cache_compact", "ygg_cache_read", "ygg_cache_write", "ygg_cache_copy")
 
 YGG_OK = 0
@@ -116,6 +116,7 @@ def ops() -> ctypes.CDLL:
         l.ygg_linear_quantized.argtypes = [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, vp]
         l.ygg_linear.argtypes = [i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64, vp, ctypes.c_size_t,
                                  vp]
+        l.ygg_linear_status.argtypes = [i32, vp, ctypes.POINTER(i32)]
         size, cache = ctypes.c_size_t, ctypes.POINTER(YggCache)
         l.ygg_cache_workspace.argtypes = [cache, i64]
         l.ygg_cache_workspace.restype = size
@@ -126,7 +127,7 @@ def ops() -> ctypes.CDLL:
         l.ygg_cache_write.argtypes = [i32, cache, i64, vp, vp, vp]
         l.ygg_cache_copy.argtypes = [i32, cache, i64, vp, vp, vp]
         for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward, l.ygg_quantize_rows, l.ygg_linear_quantized,
-                  l.ygg_linear, l.ygg_cache_fork, l.ygg_cache_free, l.ygg_cache_compact, l.ygg_cache_read,
+                  l.ygg_linear, l.ygg_linear_status, l.ygg_cache_fork, l.ygg_cache_free, l.ygg_cache_compact, l.ygg_cache_read,
                   l.ygg_cache_write, l.ygg_cache_copy):
             f.restype = i32
         _ops_bound = True

@@ -9,6 +9,7 @@ there is no gradient.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -120,6 +121,16 @@ def int8_linear(x, weight, scale, bias=None, out_dtype=None):
         if code:
             check(code, "ygg_linear")
     return out if len(lead) == 1 else out.view(*lead, n)
+
+
+def linear_status(device="cuda"):
+    """Raise YggError if a bounded wait of an int8 product on the device gave up since the last call: outputs since then
+    are not to be used. Waits for the current stream."""
+    device = torch.device(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    out = ctypes.c_int(0)
+    check(ops().ygg_linear_status(index, _raw_stream(index), ctypes.byref(out)), "ygg_linear_status")
+    check(out.value, "int8 product")
 
 
 def _laid_out(codes):
