@@ -359,3 +359,35 @@ def test_c_entry_refuses_bad_arguments():
 def test_host_tensors_are_refused():
     with pytest.raises(ValueError):
         op()(torch.zeros(2, 5), [0, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [17, 64, 256, 700, 1024, 1100, 2600, 9000, 70001])
+def test_sorted_rows_and_few_open_tokens(vocab, dtype):
+    """Rows whose best entries lie side by side, and rows with fewer open tokens than alternatives."""
+    x, t = make(8, vocab, dtype, seed=31)
+    x[0] = x[0].sort()[0]
+    x[1] = x[1].sort(descending=True)[0]
+    for row, open_ in ((2, 1), (3, 3), (4, min(vocab, 40))):
+        at = torch.randperm(vocab, generator=torch.Generator().manual_seed(row))[:open_].cuda()
+        keep = x[row, at]
+        x[row] = -INF
+        x[row, at] = keep
+    x[5, : vocab // 2] = x[5].max()
+    x[6, vocab // 3:] = x[6].max() + 1
+    for top in {1, min(5, vocab), min(32, vocab), min(33, vocab), min(64, vocab)}:
+        check_values(x, t, top, op()(x, t, top=top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(1, 600001), (2, 1 << 20), (1, 3000000)])
+def test_very_wide_rows(rows, vocab):
+    """Rows cut into segments of more than one run."""
+    for dtype in (torch.float32, torch.float16):
+        x, t = make(rows, vocab, dtype, "coarse", seed=37)
+        for top in (0, 3, 64):
+            check_values(x, t, top, op()(x, t, top=top))
+    x[0] = -INF
+    x[0, vocab - 2] = 0.5
+    check_values(x, t, 20, op()(x, t, top=20))

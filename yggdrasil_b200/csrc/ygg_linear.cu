@@ -267,15 +267,6 @@ bool map_rows(CUtensorMap *map, const int8_t *base, int64_t rows, int64_t stride
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-    static int counts[kMaxDevices];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
-    if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
-    return counts[dev];
-}
-
 template <int CTAS, typename T> int launch_tc(const Linear &q, int tn, cudaStream_t st) {
     static SmemLimits limits;
     const size_t smem = kRing + sizeof(TcShared);

@@ -82,69 +82,540 @@ __device__ __forceinline__ void join(Sums &a, Sums b) {
     a.s += b.s;
     a.t += b.t;
 }
-__device__ __forceinline__ void add(Sums &a, float x) {
-    if (x > a.m) raise(a, x);
-    const float y = x - (a.m == -INFINITY ? 0.0f : a.m), e = exp2_approx(y * kLog2e);
-    a.s += e;
-    a.t = fmaf(e, fmaxf(y, kFloor), a.t);
-}
 
 __device__ __forceinline__ int64_t token_of(const void *tokens, int bytes, int64_t row) {
     return bytes == 8 ? ((const int64_t *)tokens)[row] : (int64_t)((const int32_t *)tokens)[row];
 }
 
-template <typename T> __global__ void __launch_bounds__(256) logprobs_kernel(const Rows p) {
-    __shared__ Sums part[8];
-    __shared__ unsigned long long best[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T *x = (const T *)p.logits + row * p.stride;
-        Sums a = none();
-        for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x) add(a, to_f(x[j]));
+// A vector of 16 bytes as floats.
+template <typename T> constexpr int kPer = 16 / sizeof(T);
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[4], float) {
+    v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
+}
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __nv_bfloat16) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int o = 16; o; o >>= 1)
-            join(a, Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)});
-        if (lane == 0) part[warp] = a;
-        __syncthreads();
-        a = part[0];
-        for (int w = 1; w < 8; w++) join(a, part[w]);
-        const bool empty = a.s == 0.0f;
-        const float m = empty ? 0.0f : a.m, ls = empty ? -INFINITY : logf(a.s);
-        const float H = empty ? 0.0f : ls - a.t / a.s;
-        if (threadIdx.x == 0) {
-            const int64_t t = token_of(p.tokens, p.token_bytes, row);
-            float lp = 0.0f;
-            if (t >= p.vocab) lp = NAN;
-            else if (t >= 0) lp = empty ? -INFINITY : (to_f(x[t]) - m) - ls;
-            p.logprob[row] = lp;
-            p.entropy[row] = H;
-            p.lse[row] = m + ls;
-            if (p.stats) p.stats[row] = make_float4(m, empty ? 0.0f : 1.0f / a.s, empty ? 0.0f : ls, H);
-        }
-        // the k-th best is the best key below the last: value above, then the lower index
-        unsigned long long last = ~0ull;
-        for (int k = 0; k < p.top; k++) {
-            unsigned long long mine = 0;
-            for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x) {
-                const unsigned long long key =
-                    ((unsigned long long)((unsigned)order(to_f(x[j])) ^ 0x80000000u) << 32) | (unsigned)~(unsigned)j;
-                if (key < last && key > mine) mine = key;
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) mine = max(mine, __shfl_xor_sync(~0u, mine, o));
-            __syncthreads();
-            if (lane == 0) best[warp] = mine;
-            __syncthreads();
-            for (int w = 0; w < 8; w++) mine = max(mine, best[w]);
-            last = mine;
-            if (threadIdx.x == 0) {
-                const float v = unorder((int)((unsigned)(mine >> 32) ^ 0x80000000u));
-                p.top_ids[row * p.top + k] = (int32_t)~(unsigned)mine;
-                p.top_logprobs[row * p.top + k] = empty ? -INFINITY : (v - m) - ls;
-            }
-        }
-        __syncthreads();
+    for (int i = 0; i < 4; i++) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
+}
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __half) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*(const __half2 *)&w[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint4 load_stream(const void *p) {
+    uint4 v;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// A warp's run of 32 kPer entries from j0 on: lane l holds entries j0 + l kPer .. (VEC: one 16-byte load; entries past
+// the row's end lie in the same 16 bytes as one of its own) or j0 + l, j0 + 32 + l, .. (single loads). -inf past the end.
+template <typename T, bool VEC> __device__ __forceinline__ int64_t entry(int64_t j0, int lane, int i) {
+    return VEC ? j0 + lane * kPer<T> + i : j0 + i * 32 + lane;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_run(const T *x, int64_t j0, int64_t vocab, int lane, float (&v)[kPer<T>]) {
+    if constexpr (VEC) {
+        const int64_t j = j0 + lane * kPer<T>;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (j < vocab) q = load_stream(x + j);
+        unpack(q, v, T());
+        if (j + kPer<T> > vocab) {
+#pragma unroll
+            for (int i = 0; i < kPer<T>; i++)
+                if (j + i >= vocab) v[i] = -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer<T>; i++) {
+            const int64_t j = j0 + i * 32 + lane;
+            v[i] = j < vocab ? to_f(x[j]) : -INFINITY;
+        }
+    }
+}
+
+using Key = unsigned long long;   // orders entries: value above, then the lower index
+__device__ __forceinline__ Key key_of(float x, int64_t j) {
+    return ((Key)((unsigned)order(x) ^ 0x80000000u) << 32) | (unsigned)~(unsigned)j;
+}
+__device__ __forceinline__ float value_of(Key k) { return unorder((int)((unsigned)(k >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ int32_t index_of(Key k) { return (int32_t)~(unsigned)k; }
+__device__ __forceinline__ Key warp_max(Key k) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) k = max(k, __shfl_xor_sync(~0u, k, o));
+    return k;
+}
+
+// What a row's sums say.
+struct Ends {
+    float m, ls, h;
+    bool empty;
+    __device__ __forceinline__ explicit Ends(const Sums &a) {
+        empty = a.s == 0.0f;
+        m = empty ? 0.0f : a.m;
+        ls = empty ? -INFINITY : logf(a.s);
+        h = empty ? 0.0f : ls - a.t / a.s;
+    }
+    __device__ __forceinline__ float logprob(float x) const { return empty ? -INFINITY : (x - m) - ls; }
+};
+template <typename T> __device__ __forceinline__ void write_row(const Rows &p, int64_t row, const T *x, const Sums &a, const Ends &e) {
+    const int64_t t = token_of(p.tokens, p.token_bytes, row);
+    float lp = 0.0f;
+    if (t >= p.vocab) lp = NAN;
+    else if (t >= 0) lp = e.logprob(to_f(x[t]));
+    p.logprob[row] = lp;
+    p.entropy[row] = e.h;
+    p.lse[row] = e.m + e.ls;
+    if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? 0.0f : 1.0f / a.s, e.empty ? 0.0f : e.ls, e.h);
+}
+__device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, Key key, const Ends &e) {
+    p.top_ids[row * p.top + k] = index_of(key);
+    p.top_logprobs[row * p.top + k] = e.logprob(value_of(key));
+}
+
+// The k-th largest of the lanes' values (k <= 32), a lower bound of the k-th largest entry that the lanes hold.
+__device__ __forceinline__ int kth_of_lanes(int mine, int k, int lane) {
+    int best = 0;
+    for (int i = 0; i < k; i++) {
+        best = __reduce_max_sync(~0u, mine);
+        const unsigned who = __ballot_sync(~0u, mine == best);
+        if (lane == __ffs(who) - 1) mine = INT32_MIN;
+    }
+    return best;
+}
+
+// Short rows: a warp holds a row in registers, RUNS runs of 32 kPer entries. Alternatives: the k-th largest of the lanes'
+// maxima bounds the k-th largest entry from below, so the few entries at or above it are the candidates, and they are
+// ranked by counting. Where ties make them more than 32, the equal ones that come too late are left out; where entries
+// above the bound are more than 32, or alternatives are, they are taken one at a time.
+template <typename T, bool VEC, int RUNS> __global__ void __launch_bounds__(128) short_kernel(const Rows p) {
+    constexpr int N = kPer<T>;
+    __shared__ Key lists[4][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * 4 + warp;
+    if (row >= p.rows) return;
+    const T *x = (const T *)p.logits + row * p.stride;
+    float v[RUNS][N];
+    float most = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < RUNS; r++) load_run<T, VEC>(x, r * 32 * N, p.vocab, lane, v[r]);
+#pragma unroll
+    for (int r = 0; r < RUNS; r++)
+#pragma unroll
+        for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
+    const int mine = order(most);
+    const float top1 = unorder(__reduce_max_sync(~0u, mine)), m = top1 == -INFINITY ? 0.0f : top1;
+    Sums a{top1, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < RUNS; r++)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float y = v[r][i] - m, e = exp2_approx(y * kLog2e);
+            a.s += e;
+            a.t = fmaf(e, fmaxf(y, kFloor), a.t);
+        }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a.s += __shfl_xor_sync(~0u, a.s, o);
+        a.t += __shfl_xor_sync(~0u, a.t, o);
+    }
+    const Ends e(a);
+    if (lane == 0) write_row(p, row, x, a, e);
+    if (p.top == 0) return;
+    int n = 33;
+    if (p.top <= 32) {
+        const float bound = unorder(kth_of_lanes(mine, p.top, lane));
+        n = 0;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
+                const bool in = !(v[r][i] < bound) && j < p.vocab;
+                const unsigned who = __ballot_sync(~0u, in);
+                const int at = n + __popc(who & ((1u << lane) - 1));
+                if (in && at < 32) lists[warp][at] = key_of(v[r][i], j);
+                n += __popc(who);
+            }
+        if (n > 32) {   // ties at the bound: the entries above it, and as many equal ones as are still wanted
+            __syncwarp();
+            n = 0;
+#pragma unroll
+            for (int r = 0; r < RUNS; r++)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
+                    const bool in = v[r][i] > bound && j < p.vocab;
+                    const unsigned who = __ballot_sync(~0u, in);
+                    const int at = n + __popc(who & ((1u << lane) - 1));
+                    if (in && at < 32) lists[warp][at] = key_of(v[r][i], j);
+                    n += __popc(who);
+                }
+            // the equal ones in the order of their indices: with VEC a lane's entries of a run lie side by side, else
+            // the lanes' i-th entries do
+#pragma unroll
+            for (int r = 0; r < RUNS; r++) {
+                if (n >= p.top) break;
+                if constexpr (VEC) {
+                    int own = 0;
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        own += !(v[r][i] < bound) && !(v[r][i] > bound) && entry<T, VEC>(r * 32 * N, lane, i) < p.vocab;
+                    int upto = own;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int y = __shfl_up_sync(~0u, upto, o);
+                        if (lane >= o) upto += y;
+                    }
+                    int at = n + upto - own;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
+                        if (!(v[r][i] < bound) && !(v[r][i] > bound) && j < p.vocab) {
+                            if (at < p.top) lists[warp][at] = key_of(v[r][i], j);
+                            at++;
+                        }
+                    }
+                    n = min(p.top, n + __shfl_sync(~0u, upto, 31));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
+                        const bool in = !(v[r][i] < bound) && !(v[r][i] > bound) && j < p.vocab;
+                        const unsigned who = __ballot_sync(~0u, in);
+                        const int at = n + __popc(who & ((1u << lane) - 1));
+                        if (in && at < p.top) lists[warp][at] = key_of(v[r][i], j);
+                        n = max(n, min(p.top, n + __popc(who)));
+                    }
+                }
+            }
+        }
+    }
+    if (n <= 32) {
+        __syncwarp();
+        const Key key = lane < n ? lists[warp][lane] : 0;
+        int rank = 0;
+        for (int i = 0; i < n; i++) rank += lists[warp][i] > key;
+        if (lane < n && rank < p.top) write_top(p, row, rank, key, e);
+        return;
+    }
+    Key last = ~0ull;
+    for (int k = 0; k < p.top; k++) {
+        Key best = 0;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
+                const Key key = j < p.vocab ? key_of(v[r][i], j) : 0;
+                if (key < last && key > best) best = key;
+            }
+        last = warp_max(best);
+        if (lane == 0) write_top(p, row, k, last, e);
+    }
+}
+
+// Long rows: a cluster of up to 8 blocks a row. The row is cut into segments of 32 kPer << shift entries, given to the
+// warps of the cluster in turn; a warp keeps its running sums and leaves the largest value of each segment. The first
+// block joins the sums. Alternatives: the k largest segments by (largest value, lower segment) hold the k best entries,
+// since any other entry has k better ones, one in each of them. They are read again, and the entries at or above the
+// k-th segment's largest value are ranked by counting. If they are more than a block has threads (ties, masks, sorted
+// rows), a second bound from the threads' best entries leaves fewer; if those are still more, they are taken one at a
+// time.
+constexpr int kLongThreads = 256, kLongWarps = kLongThreads / 32, kMaxSegments = 4096, kMaxCluster = 8, kBatch = 4;
+
+struct LongShared {
+    Sums part[kMaxCluster * kLongWarps];   // in the first block
+    int picked[YGG_TOP_MAX];               // segments
+    Key keys[kLongThreads];
+    Key best[kLongWarps];
+    int count, bound;
+    int segment[];                         // order() of the segments' largest values; in the first block of all
+};
+
+__device__ __forceinline__ uint32_t shared_at(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void put_remote(uint32_t at, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cluster, int shift, int segments) {
+    constexpr int N = kPer<T>;
+    extern __shared__ __align__(16) uint8_t raw[];
+    LongShared &sh = *(LongShared *)raw;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x / cluster;
+    const int rank = blockIdx.x - (int)row * cluster;
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // the first block runs
+    const T *x = (const T *)p.logits + row * p.stride;
+    const int64_t span = (int64_t)(32 * N) << shift;
+    Sums a = none();
+    const int w = rank * kLongWarps + warp, warps = cluster * kLongWarps;
+    // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
+    const int steps = shift ? 1 << (shift - 2) : 1;
+    for (int g0 = w * (shift ? 1 : kBatch); g0 < segments; g0 += warps * (shift ? 1 : kBatch)) {
+        float top_of[kBatch];
+        for (int q = 0; q < steps; q++) {
+            float v[kBatch][N], most = -INFINITY;
+            const int64_t j0 = g0 * span + (int64_t)q * kBatch * 32 * N;
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) load_run<T, VEC>(x, j0 + (int64_t)b * 32 * N, p.vocab, lane, v[b]);
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                float t = v[b][0];
+#pragma unroll
+                for (int i = 1; i < N; i++) t = fmaxf(t, v[b][i]);
+                top_of[b] = shift && q ? fmaxf(top_of[b], t) : t;
+                most = fmaxf(most, t);
+            }
+            if (most > a.m) raise(a, most);
+            const float m = a.m == -INFINITY ? 0.0f : a.m;
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float y = v[b][i] - m, e = exp2_approx(y * kLog2e);
+                    a.s += e;
+                    a.t = fmaf(e, fmaxf(y, kFloor), a.t);
+                }
+        }
+        if (p.top) {
+            if (shift) {
+                const float t = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+                const int best = __reduce_max_sync(~0u, order(t));
+                if (lane == 0) sh.segment[g0] = best;
+            } else {
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) {
+                    const int best = __reduce_max_sync(~0u, order(top_of[b]));
+                    if (lane == 0 && g0 + b < segments) sh.segment[g0 + b] = best;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        join(a, Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)});
+    if (rank == 0 && lane == 0) sh.part[warp] = a;
+    if (cluster > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (rank) {
+            if (lane == 0) {
+                const uint32_t at = shared_at(&sh.part[w], 0);
+                put_remote(at, __float_as_uint(a.m));
+                put_remote(at + 4, __float_as_uint(a.s));
+                put_remote(at + 8, __float_as_uint(a.t));
+            }
+            if (p.top) {   // the warp's own segments
+                const int per = shift ? 1 : kBatch;
+                __syncwarp();
+                for (int g0 = w * per; g0 < segments; g0 += warps * per)
+                    if (lane < per && g0 + lane < segments)
+                        put_remote(shared_at(&sh.segment[g0 + lane], 0), (uint32_t)sh.segment[g0 + lane]);
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank) return;
+    }
+    __syncthreads();
+    a = sh.part[0];
+    for (int i = 1; i < warps; i++) join(a, sh.part[i]);
+    const Ends e(a);
+    if (threadIdx.x == 0) write_row(p, row, x, a, e);
+    if (p.top == 0) return;
+
+    // the best segments, by one warp; fewer segments than alternatives: all of them
+    const int picks = min(p.top, segments);
+    if (warp == 0) {
+        // the k-th largest of 64 bins' maxima bounds the k-th largest segment from below
+        int b0 = INT32_MIN, b1 = INT32_MIN;
+        for (int g = lane; g < segments; g += 64) {
+            b0 = max(b0, sh.segment[g]);
+            if (g + 32 < segments) b1 = max(b1, sh.segment[g + 32]);
+        }
+        int bound = 0;
+        for (int i = 0; i < picks; i++) {
+            bound = __reduce_max_sync(~0u, max(b0, b1));
+            const unsigned who = __ballot_sync(~0u, max(b0, b1) == bound);
+            if (lane == __ffs(who) - 1) (b0 >= b1 ? b0 : b1) = INT32_MIN;
+        }
+        int n = 0;
+        for (int g0 = 0; g0 < segments; g0 += 32) {
+            const int g = g0 + lane;
+            const bool in = g < segments && sh.segment[g] >= bound;
+            const unsigned who = __ballot_sync(~0u, in);
+            const int at = n + __popc(who & ((1u << lane) - 1));
+            if (in && at < kLongThreads) sh.keys[at] = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
+            n += __popc(who);
+        }
+        if (lane == 0) sh.count = n;
+    }
+    __syncthreads();
+    const int found = sh.count;
+    if (found <= kLongThreads) {
+        const Key key = threadIdx.x < found ? sh.keys[threadIdx.x] : 0;
+        int above = 0;
+        for (int i = 0; i < found; i++) above += sh.keys[i] > key;
+        if (threadIdx.x < found && above < picks) {
+            sh.picked[above] = index_of(key);
+            if (above == picks - 1) sh.bound = order(value_of(key));
+        }
+    } else {   // many equal segments
+        Key last = ~0ull;
+        for (int k = 0; k < picks; k++) {
+            Key best = 0;
+            for (int g = threadIdx.x; g < segments; g += kLongThreads) {
+                const Key key = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
+                if (key < last && key > best) best = key;
+            }
+            best = warp_max(best);
+            if (lane == 0) sh.best[warp] = best;
+            __syncthreads();
+            for (int i = 0; i < kLongWarps; i++) best = max(best, sh.best[i]);
+            last = best;
+            if (threadIdx.x == 0) {
+                sh.picked[k] = index_of(last);
+                sh.bound = order(value_of(last));
+            }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    // with fewer segments than alternatives every entry is a candidate
+    const float bound = picks < p.top ? -INFINITY : unorder(sh.bound);
+    const int runs = picks << shift;   // runs of 32 N entries in the picked segments
+    for (int q = warp; q < runs; q += kLongWarps) {
+        const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+        float v[N];
+        load_run<T, VEC>(x, j0, p.vocab, lane, v);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int64_t j = entry<T, VEC>(j0, lane, i);
+            if (!(v[i] < bound) && j < p.vocab) {
+                const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
+                if (at < kLongThreads) sh.keys[at] = key_of(v[i], j);
+            }
+        }
+    }
+    __syncthreads();
+    int n = sh.count;
+    if (n > kLongThreads) {
+        // ties, masks, sorted rows, or fewer segments than alternatives: the k-th best of the threads' best entries (by
+        // value and index) is a better bound
+        Key mine = 0;
+        for (int q = warp; q < runs; q += kLongWarps) {
+            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            float v[N];
+            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int64_t j = entry<T, VEC>(j0, lane, i);
+                if (j < p.vocab) mine = max(mine, key_of(v[i], j));
+            }
+        }
+        __syncthreads();
+        sh.keys[threadIdx.x] = mine;
+        __syncthreads();
+        int above = 0;
+        for (int i = 0; i < kLongThreads; i++) above += sh.keys[i] > mine;
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = 0;
+        if (mine && above == p.top - 1) sh.best[0] = mine;
+        __syncthreads();
+        const Key least = sh.best[0];
+        for (int q = warp; q < runs; q += kLongWarps) {
+            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            float v[N];
+            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int64_t j = entry<T, VEC>(j0, lane, i);
+                const Key key = j < p.vocab ? key_of(v[i], j) : 0;
+                if (key && key >= least) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kLongThreads) sh.keys[at] = key;
+                }
+            }
+        }
+        __syncthreads();
+        n = sh.count;
+    }
+    if (n <= kLongThreads) {
+        const Key key = threadIdx.x < n ? sh.keys[threadIdx.x] : 0;
+        int above = 0;
+        for (int i = 0; i < n; i++) above += sh.keys[i] > key;
+        if (threadIdx.x < n && above < p.top) write_top(p, row, above, key, e);
+        return;
+    }
+    Key last = ~0ull;
+    for (int k = 0; k < p.top; k++) {
+        Key best = 0;
+        for (int q = warp; q < runs; q += kLongWarps) {
+            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            float v[N];
+            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int64_t j = entry<T, VEC>(j0, lane, i);
+                const Key key = j < p.vocab ? key_of(v[i], j) : 0;
+                if (key < last && key > best) best = key;
+            }
+        }
+        best = warp_max(best);
+        __syncthreads();
+        if (lane == 0) sh.best[warp] = best;
+        __syncthreads();
+        for (int i = 0; i < kLongWarps; i++) best = max(best, sh.best[i]);
+        last = best;
+        if (threadIdx.x == 0) write_top(p, row, k, last, e);
+    }
+}
+
+// Blocks a row for the long kernel: as many as it takes to give the SMs work, up to 8, while each keeps a batch a warp.
+int cluster_for(int64_t rows, int64_t runs, int sms) {
+    int c = 1;
+    while (c < kMaxCluster && rows * c < 2 * sms && runs >= 2 * c * kLongWarps * kBatch) c *= 2;
+    return c;
+}
+
+template <typename T, bool VEC> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
+    constexpr int N = kPer<T>;
+    const int64_t runs = (p.vocab + 32 * N - 1) / (32 * N);
+    if (runs <= 32 / N) {   // at most 32 entries a lane
+        const unsigned grid = (unsigned)((p.rows + 3) / 4);
+        if (runs <= 1) short_kernel<T, VEC, 1><<<grid, 128, 0, st>>>(p);
+        else if (runs <= 2) short_kernel<T, VEC, 2><<<grid, 128, 0, st>>>(p);
+        else short_kernel<T, VEC, 32 / N><<<grid, 128, 0, st>>>(p);
+        return cudaGetLastError();
+    }
+    int shift = 0;
+    while ((runs >> shift) >= kMaxSegments) shift = shift ? shift + 1 : 2;
+    const int segments = (int)((runs + (1ll << shift) - 1) >> shift);
+    const int cluster = cluster_for(p.rows, runs, sm_count());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * cluster));
+    cfg.blockDim = dim3(kLongThreads);
+    cfg.dynamicSmemBytes = sizeof(LongShared) + (p.top ? segments : 0) * sizeof(int);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1;
+    return cudaLaunchKernelEx(&cfg, long_kernel<T, VEC>, p, cluster, shift, segments);
 }
 
 // The gradient of one entry, less the terms of the row's given tokens: p (A + B y).
@@ -204,12 +675,24 @@ int ygg_token_logprobs(int device, int dtype, int64_t rows, int64_t vocab, const
     if (!on.ok) return YGG_E_DEVICE;
     const Rows p{d_logits, rows, vocab, row_stride, d_tokens, token_bytes, top, d_logprob, d_entropy, d_lse, d_top_ids,
                  d_top_logprobs, (float4 *)d_stats};
-    const int grid = (int)std::min<int64_t>(rows, 148 * 8);
-    const int rc = by_type(dtype, [&](auto t) {
-        logprobs_kernel<decltype(t)><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    });
-    if (rc != YGG_OK) return rc;
-    return cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    cudaError_t e = cudaSuccess;
+    const int64_t step = (int64_t)1 << 26;   // rows of a launch: its grid stays below 2^31 blocks
+    for (int64_t r = 0; r < rows && e == cudaSuccess; r += step) {
+        Rows q = p;
+        q.rows = std::min(step, rows - r);
+        q.tokens = (const char *)d_tokens + r * token_bytes;
+        q.logprob += r, q.entropy += r, q.lse += r;
+        if (top) q.top_ids += r * top, q.top_logprobs += r * top;
+        if (q.stats) q.stats += r;
+        const int rc = by_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            q.logits = (const T *)d_logits + r * row_stride;
+            const bool vec = ((uintptr_t)q.logits & 15) == 0 && (row_stride * sizeof(T)) % 16 == 0;
+            e = vec ? launch_rows<T, true>(q, (cudaStream_t)stream) : launch_rows<T, false>(q, (cudaStream_t)stream);
+        });
+        if (rc != YGG_OK) return rc;
+    }
+    return e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 int ygg_token_logprobs_backward(int device, int dtype, int64_t rows, int64_t vocab, const void *d_logits,

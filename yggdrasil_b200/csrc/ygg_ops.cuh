@@ -31,6 +31,16 @@ struct OnDevice {   // makes `device` the calling thread's for the length of a c
     OnDevice &operator=(const OnDevice &) = delete;
 };
 
+// The SMs of the calling thread's device.
+inline int sm_count() {
+    static int counts[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return counts[dev];
+}
+
 // f of a value of the type that a YGG_DTYPE_ number names.
 template <typename F> int by_type(int dtype, F f) {
     switch (dtype) {
