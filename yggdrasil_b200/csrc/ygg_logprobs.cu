@@ -114,29 +114,21 @@ __device__ __forceinline__ uint4 load_stream(const void *p) {
     return v;
 }
 
-// A warp's run of 32 kPer entries from j0 on: lane l holds entries j0 + l kPer .. (VEC: one 16-byte load; entries past
-// the row's end lie in the same 16 bytes as one of its own) or j0 + l, j0 + 32 + l, .. (single loads). -inf past the end.
-template <typename T, bool VEC> __device__ __forceinline__ int64_t entry(int64_t j0, int lane, int i) {
-    return VEC ? j0 + lane * kPer<T> + i : j0 + i * 32 + lane;
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_run(const T *x, int64_t j0, int64_t vocab, int lane, float (&v)[kPer<T>]) {
-    if constexpr (VEC) {
-        const int64_t j = j0 + lane * kPer<T>;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (j < vocab) q = load_stream(x + j);
-        unpack(q, v, T());
-        if (j + kPer<T> > vocab) {
+// Rows may begin anywhere: a row is read from the 16-byte boundary at or before it, `off` entries early, and place u of
+// what is read holds the entry u - off. The places outside the row lie in the same 16 bytes as one of its own entries.
+template <typename T> __device__ __forceinline__ int offset_of(const T *x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+
+// A warp's run of 32 kPer places from u0 on, lane l those from u0 + l kPer on; -inf outside the row's places [off, end).
+template <typename T>
+__device__ __forceinline__ void load_run(const T *from, int64_t u0, int off, int64_t end, int lane, float (&v)[kPer<T>]) {
+    const int64_t u = u0 + lane * kPer<T>;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (u < end) q = load_stream(from + u);
+    unpack(q, v, T());
+    if (u + kPer<T> > end || u < off) {
 #pragma unroll
-            for (int i = 0; i < kPer<T>; i++)
-                if (j + i >= vocab) v[i] = -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer<T>; i++) {
-            const int64_t j = j0 + i * 32 + lane;
-            v[i] = j < vocab ? to_f(x[j]) : -INFINITY;
-        }
+        for (int i = 0; i < kPer<T>; i++)
+            if (u + i >= end || u + i < off) v[i] = -INFINITY;
     }
 }
 
@@ -194,17 +186,18 @@ __device__ __forceinline__ int kth_of_lanes(int mine, int k, int lane) {
 // maxima bounds the k-th largest entry from below, so the few entries at or above it are the candidates, and they are
 // ranked by counting. Where ties make them more than 32, the equal ones that come too late are left out; where entries
 // above the bound are more than 32, or alternatives are, they are taken one at a time.
-template <typename T, bool VEC, int RUNS> __global__ void __launch_bounds__(128) short_kernel(const Rows p) {
+template <typename T, int RUNS> __global__ void __launch_bounds__(128) short_kernel(const Rows p) {
     constexpr int N = kPer<T>;
     __shared__ Key lists[4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * 4 + warp;
     if (row >= p.rows) return;
     const T *x = (const T *)p.logits + row * p.stride;
+    const int off = offset_of(x), end = (int)p.vocab + off;
     float v[RUNS][N];
     float most = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < RUNS; r++) load_run<T, VEC>(x, r * 32 * N, p.vocab, lane, v[r]);
+    for (int r = 0; r < RUNS; r++) load_run<T>(x - off, r * 32 * N, off, end, lane, v[r]);
 #pragma unroll
     for (int r = 0; r < RUNS; r++)
 #pragma unroll
@@ -236,11 +229,11 @@ template <typename T, bool VEC, int RUNS> __global__ void __launch_bounds__(128)
         for (int r = 0; r < RUNS; r++)
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
-                const bool in = !(v[r][i] < bound) && j < p.vocab;
+                const int u = (r * 32 + lane) * N + i;
+                const bool in = !(v[r][i] < bound) && u >= off && u < end;
                 const unsigned who = __ballot_sync(~0u, in);
                 const int at = n + __popc(who & ((1u << lane) - 1));
-                if (in && at < 32) lists[warp][at] = key_of(v[r][i], j);
+                if (in && at < 32) lists[warp][at] = key_of(v[r][i], u - off);
                 n += __popc(who);
             }
         if (n > 32) {   // ties at the bound: the entries above it, and as many equal ones as are still wanted
@@ -250,50 +243,39 @@ template <typename T, bool VEC, int RUNS> __global__ void __launch_bounds__(128)
             for (int r = 0; r < RUNS; r++)
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
-                    const bool in = v[r][i] > bound && j < p.vocab;
+                    const int u = (r * 32 + lane) * N + i;
+                    const bool in = v[r][i] > bound && u >= off && u < end;
                     const unsigned who = __ballot_sync(~0u, in);
                     const int at = n + __popc(who & ((1u << lane) - 1));
-                    if (in && at < 32) lists[warp][at] = key_of(v[r][i], j);
+                    if (in && at < 32) lists[warp][at] = key_of(v[r][i], u - off);
                     n += __popc(who);
                 }
-            // the equal ones in the order of their indices: with VEC a lane's entries of a run lie side by side, else
-            // the lanes' i-th entries do
+            // the equal ones in the order of their indices: a lane's entries of a run lie side by side
 #pragma unroll
             for (int r = 0; r < RUNS; r++) {
                 if (n >= p.top) break;
-                if constexpr (VEC) {
-                    int own = 0;
+                int own = 0;
 #pragma unroll
-                    for (int i = 0; i < N; i++)
-                        own += !(v[r][i] < bound) && !(v[r][i] > bound) && entry<T, VEC>(r * 32 * N, lane, i) < p.vocab;
-                    int upto = own;
+                for (int i = 0; i < N; i++) {
+                    const int u = (r * 32 + lane) * N + i;
+                    own += !(v[r][i] < bound) && !(v[r][i] > bound) && u >= off && u < end;
+                }
+                int upto = own;
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int y = __shfl_up_sync(~0u, upto, o);
-                        if (lane >= o) upto += y;
-                    }
-                    int at = n + upto - own;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(~0u, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                int at = n + upto - own;
 #pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
-                        if (!(v[r][i] < bound) && !(v[r][i] > bound) && j < p.vocab) {
-                            if (at < p.top) lists[warp][at] = key_of(v[r][i], j);
-                            at++;
-                        }
-                    }
-                    n = min(p.top, n + __shfl_sync(~0u, upto, 31));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
-                        const bool in = !(v[r][i] < bound) && !(v[r][i] > bound) && j < p.vocab;
-                        const unsigned who = __ballot_sync(~0u, in);
-                        const int at = n + __popc(who & ((1u << lane) - 1));
-                        if (in && at < p.top) lists[warp][at] = key_of(v[r][i], j);
-                        n = max(n, min(p.top, n + __popc(who)));
+                for (int i = 0; i < N; i++) {
+                    const int u = (r * 32 + lane) * N + i;
+                    if (!(v[r][i] < bound) && !(v[r][i] > bound) && u >= off && u < end) {
+                        if (at < p.top) lists[warp][at] = key_of(v[r][i], u - off);
+                        at++;
                     }
                 }
+                n = min(p.top, n + __shfl_sync(~0u, upto, 31));
             }
         }
     }
@@ -312,8 +294,8 @@ template <typename T, bool VEC, int RUNS> __global__ void __launch_bounds__(128)
         for (int r = 0; r < RUNS; r++)
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t j = entry<T, VEC>(r * 32 * N, lane, i);
-                const Key key = j < p.vocab ? key_of(v[r][i], j) : 0;
+                const int u = (r * 32 + lane) * N + i;
+                const Key key = u >= off && u < end ? key_of(v[r][i], u - off) : 0;
                 if (key < last && key > best) best = key;
             }
         last = warp_max(best);
@@ -348,7 +330,7 @@ __device__ __forceinline__ void put_remote(uint32_t at, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cluster, int shift, int segments) {
     constexpr int N = kPer<T>;
     extern __shared__ __align__(16) uint8_t raw[];
@@ -358,7 +340,9 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const int rank = blockIdx.x - (int)row * cluster;
     if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // the first block runs
     const T *x = (const T *)p.logits + row * p.stride;
-    const int64_t span = (int64_t)(32 * N) << shift;
+    const int off = offset_of(x);
+    const int64_t span = (int64_t)(32 * N) << shift, end = p.vocab + off;
+    const T *from = x - off;
     Sums a = none();
     const int w = rank * kLongWarps + warp, warps = cluster * kLongWarps;
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
@@ -367,9 +351,9 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         float top_of[kBatch];
         for (int q = 0; q < steps; q++) {
             float v[kBatch][N], most = -INFINITY;
-            const int64_t j0 = g0 * span + (int64_t)q * kBatch * 32 * N;
+            const int64_t u0 = g0 * span + (int64_t)q * kBatch * 32 * N;
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) load_run<T, VEC>(x, j0 + (int64_t)b * 32 * N, p.vocab, lane, v[b]);
+            for (int b = 0; b < kBatch; b++) load_run<T>(from, u0 + (int64_t)b * 32 * N, off, end, lane, v[b]);
 #pragma unroll
             for (int b = 0; b < kBatch; b++) {
                 float t = v[b][0];
@@ -497,15 +481,15 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const float bound = picks < p.top ? -INFINITY : unorder(sh.bound);
     const int runs = picks << shift;   // runs of 32 N entries in the picked segments
     for (int q = warp; q < runs; q += kLongWarps) {
-        const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+        const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
         float v[N];
-        load_run<T, VEC>(x, j0, p.vocab, lane, v);
+        load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int64_t j = entry<T, VEC>(j0, lane, i);
-            if (!(v[i] < bound) && j < p.vocab) {
+            const int64_t u = u0 + lane * N + i;
+            if (!(v[i] < bound) && u >= off && u < end) {
                 const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
-                if (at < kLongThreads) sh.keys[at] = key_of(v[i], j);
+                if (at < kLongThreads) sh.keys[at] = key_of(v[i], u - off);
             }
         }
     }
@@ -516,13 +500,13 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         // value and index) is a better bound
         Key mine = 0;
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
-            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+            load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t j = entry<T, VEC>(j0, lane, i);
-                if (j < p.vocab) mine = max(mine, key_of(v[i], j));
+                const int64_t u = u0 + lane * N + i;
+                if (u >= off && u < end) mine = max(mine, key_of(v[i], u - off));
             }
         }
         __syncthreads();
@@ -536,13 +520,13 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         __syncthreads();
         const Key least = sh.best[0];
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
-            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+            load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t j = entry<T, VEC>(j0, lane, i);
-                const Key key = j < p.vocab ? key_of(v[i], j) : 0;
+                const int64_t u = u0 + lane * N + i;
+                const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
                 if (key && key >= least) {
                     const int at = atomicAdd(&sh.count, 1);
                     if (at < kLongThreads) sh.keys[at] = key;
@@ -563,13 +547,13 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     for (int k = 0; k < p.top; k++) {
         Key best = 0;
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t j0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
-            load_run<T, VEC>(x, j0, p.vocab, lane, v);
+            load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t j = entry<T, VEC>(j0, lane, i);
-                const Key key = j < p.vocab ? key_of(v[i], j) : 0;
+                const int64_t u = u0 + lane * N + i;
+                const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
                 if (key < last && key > best) best = key;
             }
         }
@@ -590,14 +574,15 @@ int cluster_for(int64_t rows, int64_t runs, int sms) {
     return c;
 }
 
-template <typename T, bool VEC> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
+template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
     constexpr int N = kPer<T>;
-    const int64_t runs = (p.vocab + 32 * N - 1) / (32 * N);
-    if (runs <= 32 / N) {   // at most 32 entries a lane
+    const bool even = ((uintptr_t)p.logits & 15) == 0 && (p.rows == 1 || p.stride % N == 0);   // every row on a boundary
+    const int64_t runs = (p.vocab + (even ? 0 : N - 1) + 32 * N - 1) / (32 * N);
+    if (runs <= 32 / N) {   // at most 32 places a lane
         const unsigned grid = (unsigned)((p.rows + 3) / 4);
-        if (runs <= 1) short_kernel<T, VEC, 1><<<grid, 128, 0, st>>>(p);
-        else if (runs <= 2) short_kernel<T, VEC, 2><<<grid, 128, 0, st>>>(p);
-        else short_kernel<T, VEC, 32 / N><<<grid, 128, 0, st>>>(p);
+        if (runs <= 1) short_kernel<T, 1><<<grid, 128, 0, st>>>(p);
+        else if (runs <= 2) short_kernel<T, 2><<<grid, 128, 0, st>>>(p);
+        else short_kernel<T, 32 / N><<<grid, 128, 0, st>>>(p);
         return cudaGetLastError();
     }
     int shift = 0;
@@ -615,46 +600,119 @@ template <typename T, bool VEC> cudaError_t launch_rows(const Rows &p, cudaStrea
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1;
-    return cudaLaunchKernelEx(&cfg, long_kernel<T, VEC>, p, cluster, shift, segments);
+    return cudaLaunchKernelEx(&cfg, long_kernel<T>, p, cluster, shift, segments);
 }
 
-// The gradient of one entry, less the terms of the row's given tokens: p (A + B y).
-__device__ __forceinline__ float dense(float x, float m, float inv_s, float A, float B) {
-    const float y = x - m;
-    return exp2_approx(y * kLog2e) * inv_s * fmaf(B, fmaxf(y, kFloor), A);
-}
-
-// A warp per (row, chunk of kChunk entries).
-constexpr int kChunk = 1024;
-template <typename T> __global__ void __launch_bounds__(256) logprobs_grad_kernel(const Grad p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t chunks = (p.vocab + kChunk - 1) / kChunk, items = p.rows * chunks;
-    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
-        const int64_t row = it / chunks, j0 = (it - row * chunks) * kChunk, j1 = min(j0 + (int64_t)kChunk, p.vocab);
-        const T *x = (const T *)p.logits + row * p.stride;
-        T *g = (T *)p.grad + row * p.grad_stride;
+// What the gradient of a row needs: p (A + B y) everywhere, and more at the given token and the alternatives.
+struct RowGrad {
+    float m, inv_s, A, B, given;
+    int64_t token;   // -1: none
+    __device__ __forceinline__ RowGrad(const Grad &p, int64_t row) {
         const float4 st = p.stats[row];
-        const int64_t t = token_of(p.tokens, p.token_bytes, row);
-        const bool given = t >= 0 && t < p.vocab;
-        const float gl = p.g_logprob && given ? p.g_logprob[row] : 0.0f, gh = p.g_entropy ? p.g_entropy[row] : 0.0f;
-        float c = (p.g_lse ? p.g_lse[row] : 0.0f) - gl;
+        token = token_of(p.tokens, p.token_bytes, row);
+        if (token >= p.vocab) token = -1;
+        given = p.g_logprob && token >= 0 ? p.g_logprob[row] : 0.0f;
+        const float gh = p.g_entropy ? p.g_entropy[row] : 0.0f;
+        float c = (p.g_lse ? p.g_lse[row] : 0.0f) - given;
         if (p.g_top)
             for (int k = 0; k < p.top; k++) c -= p.g_top[row * p.top + k];
-        const float A = c - gh * (st.w - st.z), B = -gh;
-        for (int64_t j = j0 + lane; j < j1; j += 32) from_f(dense(to_f(x[j]), st.x, st.y, A, B), g[j]);
-        __syncwarp();
-        // the given token and the alternatives: written again, whole, so that they are rounded once
-        const bool live = st.y != 0.0f;
-        for (int q = lane; q <= (p.g_top ? p.top : 0); q += 32) {
-            const int64_t j = q == 0 ? (given ? t : -1) : p.top_ids[row * p.top + q - 1];
-            if (j < j0 || j >= j1 || !live || (q > 0 && given && j == t)) continue;
-            float more = q == 0 ? gl : p.g_top[row * p.top + q - 1];
-            if (q == 0 && p.g_top)
-                for (int k = 0; k < p.top; k++)
-                    if (p.top_ids[row * p.top + k] == j) more += p.g_top[row * p.top + k];
-            from_f(dense(to_f(x[j]), st.x, st.y, A, B) + more, g[j]);
+        m = st.x, inv_s = st.y, A = c - gh * (st.w - st.z), B = -gh;
+    }
+    __device__ __forceinline__ float dense(float x) const {
+        const float y = x - m;
+        return exp2_approx(y * kLog2e) * inv_s * fmaf(B, fmaxf(y, kFloor), A);
+    }
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[4], float) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[8], T t) {
+    return make_uint4(pack2(v[0], v[1], t), pack2(v[2], v[3], t), pack2(v[4], v[5], t), pack2(v[6], v[7], t));
+}
+__device__ __forceinline__ void store_stream(void *p, const uint4 &v) {
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A warp per (row, chunk of kGradRuns runs of 32 kPer places). SAME: the logits and the gradient of a row lie alike to
+// the 16-byte boundary, so that both move 16 bytes at a time.
+constexpr int kGradRuns = 4;
+template <typename T, bool SAME> __global__ void __launch_bounds__(256) grad_kernel(const Grad p, unsigned chunks) {
+    constexpr int N = kPer<T>;
+    const int lane = threadIdx.x & 31;
+    const int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row = it < ((int64_t)1 << 32) ? (unsigned)it / chunks : it / chunks;
+    if (row >= p.rows) return;
+    const int64_t u0 = (it - row * chunks) * (kGradRuns * 32 * N);
+    const T *x = (const T *)p.logits + row * p.stride;
+    T *g = (T *)p.grad + row * p.grad_stride;
+    const int off = offset_of(x);
+    const int64_t end = p.vocab + off;
+    float v[kGradRuns][N];
+#pragma unroll
+    for (int r = 0; r < kGradRuns; r++) load_run<T>(x - off, u0 + r * 32 * N, off, end, lane, v[r]);
+    const RowGrad d(p, row);
+#pragma unroll
+    for (int r = 0; r < kGradRuns; r++) {
+        const int64_t u = u0 + (r * 32 + lane) * N;
+        if (u >= end) break;
+#pragma unroll
+        for (int i = 0; i < N; i++) v[r][i] = d.dense(v[r][i]);
+        if (SAME && u >= off && u + N <= end) {
+            store_stream(g - off + u, pack(v[r], T()));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (u + i >= off && u + i < end) from_f(v[r][i], g[u + i - off]);
         }
     }
+    __syncwarp();
+    // the given token and the alternatives: written again, whole, so that they are rounded once
+    if (d.inv_s == 0.0f) return;
+    const int64_t j0 = u0 - off, j1 = min(j0 + kGradRuns * 32 * N, p.vocab);
+    for (int q = lane; q <= (p.g_top ? p.top : 0); q += 32) {
+        const int64_t j = q == 0 ? d.token : p.top_ids[row * p.top + q - 1];
+        if (j < 0 || j < j0 || j >= j1 || (q > 0 && j == d.token)) continue;
+        float more = q == 0 ? d.given : p.g_top[row * p.top + q - 1];
+        if (q == 0 && p.g_top)
+            for (int k = 0; k < p.top; k++)
+                if (p.top_ids[row * p.top + k] == j) more += p.g_top[row * p.top + k];
+        from_f(d.dense(to_f(x[j])) + more, g[j]);
+    }
+}
+
+template <typename T> cudaError_t launch_grad(const Grad &p, cudaStream_t st) {
+    constexpr int N = kPer<T>;
+    const bool even = ((uintptr_t)p.logits & 15) == 0 && (p.rows == 1 || p.stride % N == 0);
+    const bool same = (((uintptr_t)p.logits ^ (uintptr_t)p.grad) & 15) == 0 &&
+                      (p.rows == 1 || (p.stride - p.grad_stride) % N == 0);
+    const int64_t places = p.vocab + (even ? 0 : N - 1), chunk = kGradRuns * 32 * N, chunks = (places + chunk - 1) / chunk;
+    const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 33) / chunks);   // rows a launch: its grid is below 2^31
+    for (int64_t r = 0; r < p.rows; r += step) {
+        Grad q = p;
+        q.rows = std::min(step, p.rows - r);
+        q.logits = (const T *)p.logits + r * p.stride;
+        q.grad = (T *)p.grad + r * p.grad_stride;
+        q.tokens = (const char *)p.tokens + r * p.token_bytes;
+        q.stats += r;
+        if (q.top_ids) q.top_ids += r * p.top;
+        if (q.g_logprob) q.g_logprob += r;
+        if (q.g_entropy) q.g_entropy += r;
+        if (q.g_lse) q.g_lse += r;
+        if (q.g_top) q.g_top += r * p.top;
+        const unsigned grid = (unsigned)((q.rows * chunks + 7) / 8);
+        if (same) grad_kernel<T, true><<<grid, 256, 0, st>>>(q, (unsigned)chunks);
+        else grad_kernel<T, false><<<grid, 256, 0, st>>>(q, (unsigned)chunks);
+    }
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -687,8 +745,7 @@ int ygg_token_logprobs(int device, int dtype, int64_t rows, int64_t vocab, const
         const int rc = by_type(dtype, [&](auto t) {
             using T = decltype(t);
             q.logits = (const T *)d_logits + r * row_stride;
-            const bool vec = ((uintptr_t)q.logits & 15) == 0 && (row_stride * sizeof(T)) % 16 == 0;
-            e = vec ? launch_rows<T, true>(q, (cudaStream_t)stream) : launch_rows<T, false>(q, (cudaStream_t)stream);
+            e = launch_rows<T>(q, (cudaStream_t)stream);
         });
         if (rc != YGG_OK) return rc;
     }
@@ -710,13 +767,10 @@ int ygg_token_logprobs_backward(int device, int dtype, int64_t rows, int64_t voc
     if (!on.ok) return YGG_E_DEVICE;
     const Grad p{d_logits, rows, vocab, row_stride, d_tokens, token_bytes, top, d_top_ids, (const float4 *)d_stats,
                  d_grad_logprob, d_grad_entropy, d_grad_lse, d_grad_top, d_grad, grad_stride};
-    const int64_t items = rows * ((vocab + kChunk - 1) / kChunk);
-    const int grid = (int)std::min<int64_t>((items + 7) / 8, 148 * 16);
-    const int rc = by_type(dtype, [&](auto t) {
-        logprobs_grad_kernel<decltype(t)><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    });
+    cudaError_t e = cudaSuccess;
+    const int rc = by_type(dtype, [&](auto t) { e = launch_grad<decltype(t)>(p, (cudaStream_t)stream); });
     if (rc != YGG_OK) return rc;
-    return cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    return e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 }  // extern "C"

@@ -69,14 +69,17 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, _, g_top):
         logits, tokens, stats, ids = ctx.saved_tensors
         rows, vocab = logits.shape
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        # rows that lie to the 16-byte boundary as the logits' do move 16 bytes at a time
+        per = 16 // logits.element_size()
+        wide = -(-vocab // per) * per if logits.stride(0) % per == 0 else vocab
+        grad = torch.empty((rows, wide), dtype=logits.dtype, device=logits.device)[:, :vocab]
         # what arrives may be expanded (a sum's gradient) or of another type
         arriving = [None if g is None else g.float().contiguous() for g in (g_logprob, g_entropy, g_lse, g_top)]
         dev = logits.device.index
         code = ops().ygg_token_logprobs_backward(
             dev, DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
             tokens.element_size(), ctx.top, ids.data_ptr() if ids is not None else None, stats.data_ptr(),
-            *[None if g is None else g.data_ptr() for g in arriving], grad.data_ptr(), vocab, _raw_stream(dev))
+            *[None if g is None else g.data_ptr() for g in arriving], grad.data_ptr(), wide, _raw_stream(dev))
         if code:
             check(code, "ygg_token_logprobs_backward")
         return grad, None, None
