@@ -48,29 +48,121 @@ __device__ __forceinline__ Factors factors(float most) {
     if (scale == 0.0f || inverse == INFINITY) return {0.0f, 0.0f};
     return {inverse, scale};
 }
-__device__ __forceinline__ int code(float x, float inverse) {
-    if (inverse == 0.0f) return 0;
-    return max(-127, min(127, __float2int_rn(__fmul_rn(x, inverse))));
-}
-// max that keeps NaN
-__device__ __forceinline__ float most_of(float a, float b) { return (a > b || a != a) ? a : b; }
+// Magnitudes compare as the integers of their bits, with NaN above infinity above the numbers.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-template <typename T> __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
-    __shared__ float part[8];
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T *x = (const T *)p.x + row * p.stride;
-        float most = 0.0f;
-        for (int j = threadIdx.x; j < p.k; j += 256) most = most_of(fabsf(to_f(x[j])), most);
+// The code of x as the low byte: the product rounds once, and adding 1.5 2^23 rounds it to the nearest integer, ties to
+// even. |x| inverse is at most 127 (1 + 2^-22), so no code is beyond 127.
+__device__ __forceinline__ uint32_t code(float x, float inverse) {
+    return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
+}
+__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float inverse) {
+    return __byte_perm(__byte_perm(code(a, inverse), code(b, inverse), 0x0040),
+                       __byte_perm(code(c, inverse), code(d, inverse), 0x0040), 0x5410);
+}
+__device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[4], float inverse) {
+    *(uint32_t *)p = inverse == 0.0f ? 0u : code4(v[0], v[1], v[2], v[3], inverse);
+}
+__device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[8], float inverse) {
+    *(uint2 *)p = inverse == 0.0f ? make_uint2(0, 0)
+                                  : make_uint2(code4(v[0], v[1], v[2], v[3], inverse), code4(v[4], v[5], v[6], v[7], inverse));
+}
+
+// THREADS threads a row (32: eight rows a block, or the whole block of 256), the row in registers as VECS vectors of 16
+// bytes a thread. Rows on 16-byte boundaries; what lies past k in a row's last vector is not the row's.
+template <typename T, int THREADS, int VECS>
+__global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
+    constexpr int N = kPer<T>;
+    __shared__ uint32_t part[8];
+    const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    const int t = threadIdx.x & (THREADS - 1);
+    let_next_begin();
+    if (row >= p.rows) return;
+    const T *x = (const T *)p.x + row * p.stride;
+    uint4 q[VECS];
+    uint32_t most = 0;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) most = most_of(__shfl_xor_sync(~0u, most, o), most);
+    for (int i = 0; i < VECS; i++) {
+        const int j = (i * THREADS + t) * N;
+        q[i] = make_uint4(0, 0, 0, 0);
+        if (j < p.k) q[i] = load_stream(x + j);
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int j = (i * THREADS + t) * N;
+        float v[N];
+        unpack(q[i], v, T());
+#pragma unroll
+        for (int e = 0; e < N; e++) most = max(most, j + e < p.k ? magnitude(v[e]) : 0u);
+    }
+    most = __reduce_max_sync(~0u, most);
+    if (THREADS > 32) {
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
         __syncthreads();
-        for (int w = 0; w < 8; w++) most = most_of(part[w], most);
+#pragma unroll
+        for (int w = 0; w < 8; w++) most = max(most, part[w]);
+    }
+    const Factors f = factors(__uint_as_float(most));
+    int8_t *codes = p.codes + row * p.code_stride;
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int j = (i * THREADS + t) * N;
+        if (j >= p.padded) continue;
+        float v[N];
+        unpack(q[i], v, T());
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (j + e >= p.k) v[e] = 0.0f;
+        store_codes(codes + j, v, f.inverse);
+    }
+    if (t == 0) p.scale[row] = f.scale;
+}
+
+// Any k and any alignment: the row is read twice.
+template <typename T> __global__ void __launch_bounds__(256) quantize_any_kernel(const Quantize p) {
+    __shared__ uint32_t part[8];
+    let_next_begin();
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T *x = (const T *)p.x + row * p.stride;
+        uint32_t most = 0;
+#pragma unroll 8
+        for (int j = threadIdx.x; j < p.k; j += 256) most = max(most, magnitude(to_f(x[j])));
+        most = __reduce_max_sync(~0u, most);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
         __syncthreads();
-        const Factors f = factors(most);
-        for (int j = threadIdx.x; j < p.padded; j += 256)
-            p.codes[row * p.code_stride + j] = j < p.k ? (int8_t)code(to_f(x[j]), f.inverse) : (int8_t)0;
+        for (int w = 0; w < 8; w++) most = max(most, part[w]);
+        __syncthreads();
+        const Factors f = factors(__uint_as_float(most));
+        int8_t *codes = p.codes + row * p.code_stride;
+#pragma unroll 4
+        for (int j = 4 * threadIdx.x; j < p.padded; j += 1024) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = j + e < p.k ? to_f(x[j + e]) : 0.0f;
+            store_codes(codes + j, v, f.inverse);
+        }
         if (threadIdx.x == 0) p.scale[row] = f.scale;
+    }
+}
+
+template <typename T> void launch_quantize(const Quantize &p, cudaStream_t st) {
+    constexpr int N = kPer<T>;
+    const bool even = ((uintptr_t)p.x & 15) == 0 && (p.rows == 1 || p.stride % N == 0);
+    const int vecs = (p.k + N - 1) / N;
+    if (!even || vecs > 2048 || p.rows > INT32_MAX) {
+        quantize_any_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 8 * sm_count()), 256, 0, st>>>(p);
+    } else if (vecs <= 256 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
+        const unsigned grid = (unsigned)((p.rows + 7) / 8);
+        if (vecs <= 32) quantize_kernel<T, 32, 1><<<grid, 256, 0, st>>>(p);
+        else if (vecs <= 64) quantize_kernel<T, 32, 2><<<grid, 256, 0, st>>>(p);
+        else if (vecs <= 128) quantize_kernel<T, 32, 4><<<grid, 256, 0, st>>>(p);
+        else quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
+    } else {
+        const unsigned grid = (unsigned)p.rows;
+        if (vecs <= 256) quantize_kernel<T, 256, 1><<<grid, 256, 0, st>>>(p);
+        else if (vecs <= 512) quantize_kernel<T, 256, 2><<<grid, 256, 0, st>>>(p);
+        else if (vecs <= 1024) quantize_kernel<T, 256, 4><<<grid, 256, 0, st>>>(p);
+        else quantize_kernel<T, 256, 8><<<grid, 256, 0, st>>>(p);
     }
 }
 
@@ -148,6 +240,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) {
             int s = 0;
             uint32_t phase = 1;
+            wait_for_previous();   // the codes
             for (int t = first; t < tiles && ok; t += step) {
                 int cb, rb;
                 tile_at(p, t, cb, rb);
@@ -191,6 +284,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int quad = warp & 3, half = warp >> 2;
         float *rs = sh.row_scale[warp];
         int it = 0;
+        wait_for_previous();       // the rows' scales
         for (int t = first; t < tiles; t += step, it++) {
             int cb, rb;
             tile_at(p, t, cb, rb);
@@ -240,6 +334,122 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == kEpilogueWarps) tmem_free<CTAS>(tmem, p.tmem_cols);
 }
 
+// Few tiles: the K of a tile is cut among the CTAs of a cluster (CTAS 1, one tile a cluster). Each sums its part in
+// tensor memory; then the columns go round in chunks of 16, chunk q to CTA q mod the cluster's size, through distributed
+// shared memory (the rings, once every CTA's products are done), and each CTA adds up and writes its chunks. Integer sums:
+// the result does not depend on the cut.
+struct SplitShared {
+    uint64_t full[kMaxStages], empty[kMaxStages], done;
+    uint32_t tmem;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Tiles p,
+                 int ring_bytes, int parts) {
+    extern __shared__ __align__(1024) uint8_t ring[];
+    SplitShared &sh = *(SplitShared *)(ring + ring_bytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = (int)cluster_rank();
+    const int tile = blockIdx.x / parts, cb = tile % p.channel_blocks, rb = tile / p.channel_blocks;
+    const int k0 = (int)((int64_t)p.k_blocks * part / parts), k1 = (int)((int64_t)p.k_blocks * (part + 1) / parts);
+    const int stage_bytes = 128 * kStageK + p.tn * kStageK;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_addr(&sh.full[s]), 1);
+            mbar_init(smem_addr(&sh.empty[s]), 1);
+        }
+        mbar_init(smem_addr(&sh.done), 1);
+        fence_mbar_init();
+    }
+    if (warp == kEpilogueWarps) tmem_alloc<1>(smem_addr(&sh.tmem), p.tmem_cols);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    bool ok = true;
+    if (warp == kEpilogueWarps) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 1;
+            wait_for_previous();
+            for (int kb = k0; kb < k1; kb++) {
+                if (!(ok = mbar_wait_bounded(smem_addr(&sh.empty[s]), phase))) break;
+                const uint32_t bar = smem_addr(&sh.full[s]), at = smem_addr(ring + s * stage_bytes);
+                mbar_expect_tx(bar, stage_bytes);
+                tma_load<1>(at, &wmap, kb * kStageK, cb * 128, bar);
+                tma_load<1>(at + 128 * kStageK, &xmap, kb * kStageK, rb * p.tn, bar);
+                if (++s == p.stages) s = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == kEpilogueWarps + 1) {
+        if (lane == 0) {
+            const uint32_t shape = product_s8(128, p.tn);
+            int s = 0;
+            uint32_t phase = 0;
+            for (int kb = k0; kb < k1; kb++) {
+                if (!(ok = mbar_wait_bounded(smem_addr(&sh.full[s]), phase))) break;
+                tmem_fence_after();
+                const uint32_t at = smem_addr(ring + s * stage_bytes);
+                const uint64_t a = operand_128b(at), b = operand_128b(at + 128 * kStageK);
+#pragma unroll
+                for (int j = 0; j < kStageK / 32; j++) mma_s8<1>(tmem, a + 2 * j, b + 2 * j, shape, kb > k0 || j > 0);
+                mma_commit<1>(smem_addr(&sh.empty[s]));
+                if (++s == p.stages) s = 0, phase ^= 1;
+            }
+            if (ok) mma_commit<1>(smem_addr(&sh.done));
+        }
+    } else {
+        wait_for_previous();
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done), 0));
+        tmem_fence_after();
+    }
+    __syncwarp();
+    cluster_sync();   // every ring is free
+    const int quad = warp & 3, half = warp >> 2, chunks = p.tn / 16;
+    const uint32_t mine = smem_addr(ring);
+    if (warp < kEpilogueWarps) {
+        for (int q = half; q < chunks; q += 2) {
+            uint32_t v[16];
+            tmem_load16(tmem + q * 16 + ((uint32_t)(quad * 32) << 16), v);
+            tmem_loaded();
+            const uint32_t to = at_rank(mine + ((q / parts) * parts + part) * 8192 + (quad * 32 + lane) * 4, q % parts);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * 512), "r"(v[j]) : "memory");
+        }
+    }
+    tmem_fence_before();
+    __syncwarp();
+    cluster_sync();
+    if (warp < kEpilogueWarps && ok) {
+        const int64_t row0 = (int64_t)rb * p.tn, ch = (int64_t)cb * 128 + quad * 32 + lane;
+        const bool live = ch < p.n;
+        const float sn = live ? p.scale[ch] : 0.0f, bn = live && p.bias ? p.bias[ch] : 0.0f;
+        T *out = (T *)p.out + row0 * p.out_stride + ch;
+        const int rows = (int)min((int64_t)p.tn, p.rows - row0);
+        for (int q = part; q < chunks && live; q += parts) {
+            const int *from = (const int *)(ring + (q / parts) * parts * 8192) + quad * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int c = half * 8 + j, r = q * 16 + c;
+                if (r >= rows) break;
+                int sum = 0;
+                for (int i = 0; i < parts; i++) sum += from[i * 2048 + c * 128];
+                const float y = __int2float_rn(sum) * sn * p.row_scale[row0 + r];
+                from_f(p.bias ? y + bn : y, out[(int64_t)r * p.out_stride]);
+            }
+        }
+    }
+    if (!ok) {
+        *(volatile int *)&g_fault = 1;
+        const long long t0 = clock64();
+        while (clock64() - t0 < 50000000LL) {}
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == kEpilogueWarps) tmem_free<1>(tmem, p.tmem_cols);
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -267,31 +477,222 @@ bool map_rows(CUtensorMap *map, const int8_t *base, int64_t rows, int64_t stride
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The launch attributes of the tensor-core kernels: a cluster, and leave to begin under the launch before it.
+struct Launch {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    Launch(int64_t blocks, int cluster, size_t smem, cudaStream_t st) {
+        cfg.gridDim = dim3((unsigned)blocks);
+        cfg.blockDim = dim3(kTcThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+    }
+};
+
+Tiles tiles_of(const Linear &q, int ctas, int tn, int accumulators) {
+    Tiles p{q.rows, q.n, (q.k + kStageK - 1) / kStageK, tn, 0, (int)((q.n + 128 * ctas - 1) / (128 * ctas)),
+            (int)((q.rows + tn - 1) / tn), 32, q.row_scale, q.scale, q.bias, q.out, q.out_stride};
+    while (p.tmem_cols < accumulators * tn) p.tmem_cols *= 2;
+    return p;
+}
+
 template <int CTAS, typename T> int launch_tc(const Linear &q, int tn, cudaStream_t st) {
     static SmemLimits limits;
     const size_t smem = kRing + sizeof(TcShared);
-    Tiles p{q.rows, q.n, (q.k + kStageK - 1) / kStageK, tn, 0, (int)((q.n + 128 * CTAS - 1) / (128 * CTAS)),
-            (int)((q.rows + tn - 1) / tn), 32, q.row_scale, q.scale, q.bias, q.out, q.out_stride};
+    Tiles p = tiles_of(q, CTAS, tn, 2);
     p.stages = std::min(kMaxStages, kRing / ((128 + tn / CTAS) * kStageK));
-    while (p.tmem_cols < 2 * tn) p.tmem_cols *= 2;
     CUtensorMap wmap, xmap;
     if (!map_rows(&wmap, q.weight, q.n, q.weight_stride, q.k, 128) ||
         !map_rows(&xmap, q.codes, q.rows, q.code_stride, q.k, tn / CTAS) ||
         raise_smem_limit((const void *)tc_kernel<CTAS, T>, smem, limits) != cudaSuccess)
         return YGG_E_CUDA;
     const int64_t tiles = (int64_t)p.channel_blocks * p.row_blocks;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, sm_count() / CTAS) * CTAS);
-    cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tc_kernel<CTAS, T>, wmap, xmap, p) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    Launch l(std::min<int64_t>(tiles, sm_count() / CTAS) * CTAS, CTAS, smem, st);
+    return cudaLaunchKernelEx(&l.cfg, tc_kernel<CTAS, T>, wmap, xmap, p) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+}
+
+template <typename T> int launch_split(const Linear &q, int tn, int parts, cudaStream_t st) {
+    static SmemLimits limits;
+    Tiles p = tiles_of(q, 1, tn, 1);
+    const int stage = (128 + tn) * kStageK, k_blocks = (p.k_blocks + parts - 1) / parts;
+    // two CTAs an SM where a few stages fit half of its shared memory, else the whole ring
+    p.stages = std::min(std::min(kMaxStages, k_blocks), (tn <= 128 ? kRing / 2 : kRing) / stage);
+    const int chunks = (tn / 16 + parts - 1) / parts, ring = std::max(p.stages * stage, chunks * parts * 8192);
+    const size_t smem = ring + sizeof(SplitShared);
+    CUtensorMap wmap, xmap;
+    if (!map_rows(&wmap, q.weight, q.n, q.weight_stride, q.k, 128) ||
+        !map_rows(&xmap, q.codes, q.rows, q.code_stride, q.k, tn) ||
+        raise_smem_limit((const void *)split_kernel<T>, smem, limits) != cudaSuccess)
+        return YGG_E_CUDA;
+    Launch l((int64_t)p.channel_blocks * p.row_blocks * parts, parts, smem, st);
+    return cudaLaunchKernelEx(&l.cfg, split_kernel<T>, wmap, xmap, p, ring, parts) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+}
+
+// ---------------------------------------------------------------------------------------------------- few rows
+//
+// Up to 8 rows: the weights are read once and nothing else counts. A warp (or `split` warps, each a part of K) takes two
+// channels at a time, 2048 bytes of each, the next ones loaded while dp4a sums the last; the codes of the rows lie in
+// shared memory. Short rows are quantised by every block itself, under the first loads of its weights.
+constexpr int kFewRows = 8, kFewBlock = 2048, kFewFused = 16384;   // kFewFused: values that each block quantises itself
+
+struct Few {
+    Linear q;
+    const void *x;          // what to quantise, or null: q.codes
+    int64_t x_stride;
+    int out_dtype, split, k_room;   // k_room: bytes of a row in shared memory, a multiple of kFewBlock
+    bool early;             // the weights may be read before the launch before this one ends
+};
+
+struct FewLoad { uint4 w[2][4]; };
+
+__device__ __forceinline__ void few_load(FewLoad &l, const Linear &q, int64_t ch, int kb, int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = kb * kFewBlock + i * 512 + lane * 16;
+            l.w[c][i] = make_uint4(0, 0, 0, 0);
+            if (at < q.k && ch + c < q.n) l.w[c][i] = load_stream(q.weight + (ch + c) * q.weight_stride + at);
+        }
+}
+
+__device__ __forceinline__ void store_as(int dtype, void *out, int64_t at, float v) {
+    if (dtype == YGG_DTYPE_FLOAT) ((float *)out)[at] = v;
+    else if (dtype == YGG_DTYPE_HALF) ((__half *)out)[at] = __float2half_rn(v);
+    else ((__nv_bfloat16 *)out)[at] = __float2bfloat16_rn(v);
+}
+
+// X: the type of the rows to quantise, or int8_t: codes.
+template <typename X, int ROWS> __global__ void __launch_bounds__(256, 2) few_kernel(const Few p) {
+    extern __shared__ __align__(16) uint8_t room[];   // [ROWS][k_room] codes
+    __shared__ uint32_t most[ROWS][8];
+    __shared__ float row_scale[ROWS];
+    __shared__ int sums[2][8][2 * ROWS];
+    const Linear &q = p.q;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = (int)q.rows;
+    const int teams = 8 / p.split, team = warp / p.split, part = warp - team * p.split;
+    const int64_t groups = (q.n + 1) / 2, all = (int64_t)gridDim.x * teams, id = (int64_t)blockIdx.x * teams + team;
+    const int64_t g0 = groups * id / all, g1 = groups * (id + 1) / all;
+    const int blocks = p.k_room / kFewBlock;
+    FewLoad cur, next;
+    if (!p.early) wait_for_previous();
+    if (g0 < g1) few_load(cur, q, 2 * g0, part, lane);
+    if constexpr (sizeof(X) > 1) {
+        const X *x = (const X *)p.x;
+        for (int r = 0; r < rows; r++) {
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int j = threadIdx.x; j < q.k; j += 256) m = max(m, magnitude(to_f(x[r * p.x_stride + j])));
+            m = __reduce_max_sync(~0u, m);
+            if (lane == 0) most[r][warp] = m;
+        }
+        __syncthreads();
+        for (int r = 0; r < rows; r++) {
+            uint32_t m = 0;
+            for (int w = 0; w < 8; w++) m = max(m, most[r][w]);
+            const Factors f = factors(__uint_as_float(m));
+            if (threadIdx.x == 0) row_scale[r] = f.scale;
+#pragma unroll 2
+            for (int j = 4 * threadIdx.x; j < p.k_room; j += 1024) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = j + e < q.k ? to_f(x[r * p.x_stride + j + e]) : 0.0f;
+                store_codes((int8_t *)room + r * p.k_room + j, v, f.inverse);
+            }
+        }
+    } else {
+        if (p.early) wait_for_previous();
+        for (int i = threadIdx.x; i < rows * (p.k_room / 16); i += 256) {
+            const int r = i / (p.k_room / 16), at = (i - r * (p.k_room / 16)) * 16;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (at < q.k) v = *(const uint4 *)(q.codes + r * q.code_stride + at);
+            if (at + 16 > q.k) {   // bytes past k are not the row's
+                uint32_t *w = (uint32_t *)&v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int left = q.k - at - 4 * e;
+                    if (left < 4) w[e] = left <= 0 ? 0u : w[e] & ((1u << (8 * left)) - 1);
+                }
+            }
+            *(uint4 *)(room + r * p.k_room + at) = v;
+        }
+        if (threadIdx.x < rows) row_scale[threadIdx.x] = q.row_scale[threadIdx.x];
+    }
+    __syncthreads();
+    int turn = 0;
+    for (int64_t g = g0; g < g1; g++, turn ^= 1) {
+        int acc[2][ROWS] = {};
+        for (int kb = part; kb < blocks; kb += p.split) {
+            if (kb + p.split < blocks) few_load(next, q, 2 * g, kb + p.split, lane);
+            else if (g + 1 < g1) few_load(next, q, 2 * (g + 1), part, lane);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint8_t *at = room + kb * kFewBlock + i * 512 + lane * 16;
+#pragma unroll
+                for (int r = 0; r < ROWS; r++) {
+                    if (r >= rows) break;
+                    const uint4 c = *(const uint4 *)(at + r * p.k_room);
+#pragma unroll
+                    for (int ch = 0; ch < 2; ch++) acc[ch][r] = dot16(cur.w[ch][i], c, acc[ch][r]);
+                }
+            }
+            cur = next;
+        }
+        int mine = 0;   // lane ch ROWS + r keeps the sum of channel ch and row r
+#pragma unroll
+        for (int ch = 0; ch < 2; ch++)
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const int sum = __reduce_add_sync(~0u, acc[ch][r]);
+                if (lane == ch * ROWS + r) mine = sum;
+            }
+        if (p.split > 1) {
+            if (lane < 2 * ROWS) sums[turn][warp][lane] = mine;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.split * 32) : "memory");
+            if (part) continue;
+            mine = 0;
+            if (lane < 2 * ROWS)
+                for (int w = 0; w < p.split; w++) mine += sums[turn][warp + w][lane];
+        }
+        const int64_t ch = 2 * g + lane / ROWS;
+        const int r = lane % ROWS;
+        if (lane < 2 * ROWS && r < rows && ch < q.n) {
+            const float y = __int2float_rn(mine) * q.scale[ch] * row_scale[r];
+            store_as(p.out_dtype, q.out, r * q.out_stride + ch, q.bias ? y + q.bias[ch] : y);
+        }
+    }
+}
+
+int few_room(int k) { return (k + kFewBlock - 1) / kFewBlock * kFewBlock; }
+bool is_few(int64_t rows, int k) { return rows <= kFewRows && rows * few_room(k) <= 192 * 1024; }
+
+template <typename X, int ROWS> cudaError_t launch_few_rows(Few p, cudaStream_t st) {
+    static SmemLimits limits;
+    const size_t smem = (size_t)p.q.rows * p.k_room;
+    cudaError_t e = raise_smem_limit((const void *)few_kernel<X, ROWS>, smem, limits);
+    if (e != cudaSuccess) return e;
+    const int64_t groups = (p.q.n + 1) / 2, warps = 16 * sm_count();
+    const int blocks = p.k_room / kFewBlock;
+    p.split = 1;
+    while (p.split < 8 && 2 * p.split <= blocks && 2 * p.split * groups <= warps) p.split *= 2;
+    Launch l(std::min<int64_t>((groups * p.split + 7) / 8, 2 * sm_count()), 1, smem, st);
+    l.cfg.blockDim = dim3(256);
+    if (sizeof(X) > 1) l.cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&l.cfg, few_kernel<X, ROWS>, p);
+}
+
+template <typename X> int launch_few(const Few &p, cudaStream_t st) {
+    const int64_t rows = p.q.rows;
+    const cudaError_t e = rows == 1 ? launch_few_rows<X, 1>(p, st) : rows == 2 ? launch_few_rows<X, 2>(p, st)
+                          : rows <= 4 ? launch_few_rows<X, 4>(p, st) : launch_few_rows<X, 8>(p, st);
+    return e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 int padded_of(int64_t k) { return (int)((k + 15) / 16 * 16); }
@@ -299,11 +700,24 @@ int padded_of(int64_t k) { return (int)((k + 15) / 16 * 16); }
 bool rows_ok(int64_t rows, int64_t k) { return rows >= 0 && rows < ((int64_t)1 << 40) && k >= 1; }
 
 int quantize(int dtype, const Quantize &p, cudaStream_t st) {
-    const int grid = (int)std::min<int64_t>(p.rows, 148 * 8);
-    return by_type(dtype, [&](auto t) { quantize_kernel<decltype(t)><<<grid, 256, 0, st>>>(p); });
+    return by_type(dtype, [&](auto t) { launch_quantize<decltype(t)>(p, st); });
 }
 
-int linear(int out_dtype, const Linear &p, cudaStream_t st) {
+struct Shape { int ctas, tn, parts; };
+Shape shape_for(int64_t rows, int64_t n, int k) {
+    const int sms = sm_count(), k_blocks = (k + kStageK - 1) / kStageK;
+    const int64_t row_blocks = (rows + 255) / 256;
+    int tn = (int)((rows + row_blocks - 1) / row_blocks + 15) / 16 * 16;
+    const int64_t tiles = (n + 127) / 128 * ((rows + tn - 1) / tn);
+    if (rows > 256 && tiles >= 2 * sms) return {2, 256, 1};
+    int parts = 1;
+    while (parts < 8 && 2 * parts * tiles <= sms && 2 * parts <= k_blocks) parts *= 2;
+    return {1, tn, parts};
+}
+
+// early: the launch before this one wrote the codes and nothing else that the product reads.
+int linear(int out_dtype, const Linear &p, bool early, cudaStream_t st) {
+    if (is_few(p.rows, p.k)) return launch_few<int8_t>({p, nullptr, 0, out_dtype, 1, few_room(p.k), early}, st);
     const int64_t step = (int64_t)1 << 24;   // rows a launch counts its tiles over
     for (int64_t m = 0; m < p.rows; m += step) {
         Linear q = p;
@@ -314,8 +728,10 @@ int linear(int out_dtype, const Linear &p, cudaStream_t st) {
         int done = YGG_OK;
         const int rc = by_type(out_dtype, [&](auto t) {
             using T = decltype(t);
-            if (q.rows > 256) done = launch_tc<2, T>(q, 256, st);
-            else done = launch_tc<1, T>(q, (int)(q.rows + 15) / 16 * 16, st);
+            const Shape s = shape_for(q.rows, q.n, q.k);
+            done = s.ctas == 2    ? launch_tc<2, T>(q, s.tn, st)
+                   : s.parts == 1 ? launch_tc<1, T>(q, s.tn, st)
+                                  : launch_split<T>(q, s.tn, s.parts, st);
         });
         if (rc != YGG_OK) return rc;
         if (done != YGG_OK) return done;
@@ -352,7 +768,7 @@ int ygg_linear_quantized(int device, int64_t rows, int64_t k, int64_t n, const i
                          const float *d_scale, const float *d_bias, int out_dtype, void *d_out, int64_t out_stride,
                          void *stream) {
     if (!rows_ok(rows, k) || n < 1 || n > INT32_MAX) return YGG_E_ARG;
-    if (k > YGG_LINEAR_MAX_K) return YGG_E_UNSUPPORTED;
+    if (k > YGG_LINEAR_MAX_K || out_dtype < YGG_DTYPE_FLOAT || out_dtype > YGG_DTYPE_BFLOAT) return YGG_E_UNSUPPORTED;
     if (rows == 0) return YGG_OK;
     if (!d_codes || !d_row_scale || !d_weight || !d_scale || !d_out || !aligned16(d_codes, code_stride) ||
         !aligned16(d_weight, weight_stride) || code_stride < k || weight_stride < k)
@@ -360,7 +776,7 @@ int ygg_linear_quantized(int device, int64_t rows, int64_t k, int64_t n, const i
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
     const int rc = linear(out_dtype, {d_codes, d_weight, code_stride, weight_stride, d_row_scale, d_scale, d_bias, rows,
-                                      n, (int)k, d_out, out_stride}, (cudaStream_t)stream);
+                                      n, (int)k, d_out, out_stride}, false, (cudaStream_t)stream);
     return rc != YGG_OK ? rc : cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
@@ -384,16 +800,30 @@ int ygg_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, const 
                const int8_t *d_weight, int64_t weight_stride, const float *d_scale, const float *d_bias, int out_dtype,
                void *d_out, int64_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream) {
     if (!rows_ok(rows, k) || n < 1 || n > INT32_MAX) return YGG_E_ARG;
-    if (k > YGG_LINEAR_MAX_K) return YGG_E_UNSUPPORTED;
+    if (k > YGG_LINEAR_MAX_K || out_dtype < YGG_DTYPE_FLOAT || out_dtype > YGG_DTYPE_BFLOAT) return YGG_E_UNSUPPORTED;
     if (rows == 0) return YGG_OK;
     if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < ygg_linear_workspace(rows, k)) return YGG_E_ARG;
+    if (!d_x || !d_weight || !d_scale || !d_out || !aligned16(d_weight, weight_stride) || weight_stride < k)
+        return YGG_E_ARG;
+    OnDevice on(device);
+    if (!on.ok) return YGG_E_DEVICE;
+    const cudaStream_t st = (cudaStream_t)stream;
     const int64_t padded = padded_of(k);
     int8_t *codes = (int8_t *)d_workspace;
     float *scale = (float *)(codes + rows * padded);
-    const int rc = ygg_quantize_rows(device, dtype, rows, k, d_x, row_stride, codes, padded, scale, stream);
-    if (rc != YGG_OK) return rc;
-    return ygg_linear_quantized(device, rows, k, n, codes, padded, scale, d_weight, weight_stride, d_scale, d_bias,
-                                out_dtype, d_out, out_stride, stream);
+    const Linear q{codes, d_weight, padded, weight_stride, scale, d_scale, d_bias, rows, n, (int)k, d_out, out_stride};
+    int rc;
+    if (rows * k <= kFewFused && is_few(rows, (int)k)) {
+        int done = YGG_OK;
+        rc = by_type(dtype, [&](auto t) {
+            done = launch_few<decltype(t)>({q, d_x, row_stride, out_dtype, 1, few_room((int)k), true}, st);
+        });
+        if (rc == YGG_OK) rc = done;
+    } else {
+        rc = quantize(dtype, {d_x, rows, row_stride, (int)k, (int)padded, codes, padded, scale}, st);
+        if (rc == YGG_OK) rc = linear(out_dtype, q, true, st);
+    }
+    return rc != YGG_OK ? rc : cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 }  // extern "C"

@@ -87,33 +87,6 @@ __device__ __forceinline__ int64_t token_of(const void *tokens, int bytes, int64
     return bytes == 8 ? ((const int64_t *)tokens)[row] : (int64_t)((const int32_t *)tokens)[row];
 }
 
-// A vector of 16 bytes as floats.
-template <typename T> constexpr int kPer = 16 / sizeof(T);
-__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[4], float) {
-    v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
-}
-__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __nv_bfloat16) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-}
-__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __half) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*(const __half2 *)&w[i]);
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ uint4 load_stream(const void *p) {
-    uint4 v;
-    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
 // Rows may begin anywhere: a row is read from the 16-byte boundary at or before it, `off` entries early, and place u of
 // what is read holds the entry u - off. The places outside the row lie in the same 16 bytes as one of its own entries.
 template <typename T> __device__ __forceinline__ int offset_of(const T *x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }

@@ -17,6 +17,40 @@ __device__ __forceinline__ void from_f(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f(float v, __half &o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
+// A vector of 16 bytes as floats.
+template <typename T> constexpr int kPer = 16 / sizeof(T);
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[4], float) {
+    v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
+}
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __nv_bfloat16) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8], __half) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*(const __half2 *)&w[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+// 16 bytes that this launch reads once. volatile: a load in plain asm counts as free of side effects, so that the compiler
+// may issue it before the branch that guards its address.
+__device__ __forceinline__ uint4 load_stream(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// A launch that follows another in its stream may begin before that one ends; it waits here before it reads what the
+// other wrote. The other says when it may begin.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 struct OnDevice {   // makes `device` the calling thread's for the length of a call
     int prev = -1;
     bool ok;
