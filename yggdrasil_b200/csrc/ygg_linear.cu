@@ -151,12 +151,13 @@ template <typename T> void launch_quantize(const Quantize &p, cudaStream_t st) {
     const int vecs = (p.k + N - 1) / N;
     if (!even || vecs > 2048 || p.rows > INT32_MAX) {
         quantize_any_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 8 * sm_count()), 256, 0, st>>>(p);
-    } else if (vecs <= 256 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
+    } else if (vecs <= 512 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
         const unsigned grid = (unsigned)((p.rows + 7) / 8);
         if (vecs <= 32) quantize_kernel<T, 32, 1><<<grid, 256, 0, st>>>(p);
         else if (vecs <= 64) quantize_kernel<T, 32, 2><<<grid, 256, 0, st>>>(p);
         else if (vecs <= 128) quantize_kernel<T, 32, 4><<<grid, 256, 0, st>>>(p);
-        else quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
+        else if (vecs <= 256) quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
+        else quantize_kernel<T, 32, 16><<<grid, 256, 0, st>>>(p);
     } else {
         const unsigned grid = (unsigned)p.rows;
         if (vecs <= 256) quantize_kernel<T, 256, 1><<<grid, 256, 0, st>>>(p);
@@ -195,7 +196,7 @@ struct Tiles {
 
 struct TcShared {   // at the end of dynamic shared memory
     uint64_t full[kMaxStages], empty[kMaxStages], done[2], drained[2];
-    float row_scale[kEpilogueWarps][256];   // each warp its own: no barrier among them
+    alignas(16) float row_scale[kEpilogueWarps][256];   // each warp its own: no barrier among them
     uint32_t tmem;
 };
 
@@ -206,6 +207,24 @@ __device__ __forceinline__ void tile_at(const Tiles &p, int t, int &cb, int &rb)
     t %= band;
     cb = first + t % left;
     rb = t / left;
+}
+
+// 16 sums of one channel, of the rows whose scales are rs[0..16) (16-byte aligned): row j goes to out + j stride.
+template <typename T>
+__device__ __forceinline__ void write_rows(const uint32_t (&v)[16], const float *rs, float sn, float bn, T *out,
+                                           int64_t stride, int rows) {
+    float4 f[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[j] = ((const float4 *)rs)[j];
+    const float *r = (const float *)f;
+    if (rows >= 16) {
+#pragma unroll
+        for (int j = 0; j < 16; j++, out += stride) from_f(fmaf(__int2float_rn((int)v[j]) * sn, r[j], bn), *out);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++, out += stride)
+            if (j < rows) from_f(fmaf(__int2float_rn((int)v[j]) * sn, r[j], bn), *out);
+    }
 }
 
 template <int CTAS, typename T>
@@ -292,25 +311,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int64_t row0 = (int64_t)rb * p.tn, ch = (int64_t)(cb * CTAS + rank) * 128 + quad * 32 + lane;
             const int rows = (int)min((int64_t)p.tn, p.rows - row0);
             __syncwarp();
-            for (int c = lane; c < rows; c += 32) rs[c] = p.row_scale[row0 + c];
+            for (int c = lane; c < p.tn; c += 32) rs[c] = c < rows ? p.row_scale[row0 + c] : 0.0f;
             const bool live = ch < p.n;
             const float sn = live ? p.scale[ch] : 0.0f, bn = live && p.bias ? p.bias[ch] : 0.0f;
             if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[acc]), (it >> 1) & 1)))) break;
             tmem_fence_after();
             const uint32_t d = tmem + acc * (p.tmem_cols / 2) + ((uint32_t)(quad * 32) << 16);
             T *out = (T *)p.out + row0 * p.out_stride + ch;
-            for (int c = half * 16; c < p.tn; c += 32) {
-                uint32_t v[16];
+            const int span = p.tn >= 64 ? 32 : 16;   // columns a turn; small tiles give each half of the warps some
+            for (int c = half * span; c < p.tn; c += 2 * span) {
+                uint32_t v[16], w[16];
+                const bool two = span == 32 && c + 16 < p.tn;
                 __syncwarp();
                 tmem_load16(d + c, v);
+                if (two) tmem_load16(d + c + 16, w);
                 tmem_loaded();
                 if (live) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (c + j < rows) {
-                            const float y = __int2float_rn((int)v[j]) * sn * rs[c + j];
-                            from_f(p.bias ? y + bn : y, out[(int64_t)(c + j) * p.out_stride]);
-                        }
+                    write_rows(v, rs + c, sn, bn, out + c * p.out_stride, p.out_stride, rows - c);
+                    if (two) write_rows(w, rs + c + 16, sn, bn, out + (c + 16) * p.out_stride, p.out_stride, rows - c - 16);
                 }
             }
             tmem_fence_before();
@@ -537,10 +555,11 @@ template <typename T> int launch_split(const Linear &q, int tn, int parts, cudaS
 
 // ---------------------------------------------------------------------------------------------------- few rows
 //
-// Up to 8 rows: the weights are read once and nothing else counts. A warp (or `split` warps, each a part of K) takes two
+// Up to 4 rows (from 5 on the tensor cores are faster: 5 x 4096 x 32768 in 26.3 us there, 27.8 us here; 4 rows in 26.6 and
+// 25.0): the weights are read once and nothing else counts. A warp (or `split` warps, each a part of K) takes two
 // channels at a time, 2048 bytes of each, the next ones loaded while dp4a sums the last; the codes of the rows lie in
-// shared memory. Short rows are quantised by every block itself, under the first loads of its weights.
-constexpr int kFewRows = 8, kFewBlock = 2048, kFewFused = 16384;   // kFewFused: values that each block quantises itself
+// shared memory. Short rows before few weights are quantised by every block itself, under its first loads.
+constexpr int kFewRows = 4, kFewBlock = 2048;
 
 struct Few {
     Linear q;
@@ -691,7 +710,7 @@ template <typename X, int ROWS> cudaError_t launch_few_rows(Few p, cudaStream_t 
 template <typename X> int launch_few(const Few &p, cudaStream_t st) {
     const int64_t rows = p.q.rows;
     const cudaError_t e = rows == 1 ? launch_few_rows<X, 1>(p, st) : rows == 2 ? launch_few_rows<X, 2>(p, st)
-                          : rows <= 4 ? launch_few_rows<X, 4>(p, st) : launch_few_rows<X, 8>(p, st);
+                                                                               : launch_few_rows<X, 4>(p, st);
     return e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
@@ -703,16 +722,38 @@ int quantize(int dtype, const Quantize &p, cudaStream_t st) {
     return by_type(dtype, [&](auto t) { launch_quantize<decltype(t)>(p, st); });
 }
 
+// How a product is cut: CTAs a product, rows a tile, CTAs that share the K of a tile. The least of what the cuts are
+// expected to take, in ns, by a model fitted to sweeps on a B200 (us, measured):
+//   a launch costs 3200; 128 bytes of K of a tile 240, or its bytes at 115 a ns where those take longer (a pair of
+//   256 x 256: 410, bound by the tensor cores); the epilogue 8 a column, hidden under the next tile's products.
+//   512 x 4096 x 4096: tn 128 12.1, 256 15.6; 1024 x 4096 x 4096: tn 256 16.0, 128 20.5;
+//   8192 x 4096 x 16384: pair 370, one CTA 410.
+//   Sharing K costs 2200 and 25 a column: 16 x 4096 x 4096 8.0 with 4 parts, 11.0 with one; 512 x 1024 x 4096 (tn 256) 15.5
+//   with two, 7.2 with one.
 struct Shape { int ctas, tn, parts; };
 Shape shape_for(int64_t rows, int64_t n, int k) {
-    const int sms = sm_count(), k_blocks = (k + kStageK - 1) / kStageK;
+    const int64_t sms = sm_count(), k_blocks = (k + kStageK - 1) / kStageK, channel_blocks = (n + 127) / 128;
+    Shape best{1, 16, 1};
+    int64_t least = INT64_MAX;
+    auto consider = [&](int ctas, int tn, int parts) {
+        const int64_t tiles = (channel_blocks + ctas - 1) / ctas * ((rows + tn - 1) / tn);
+        if (parts > 1 && tiles * parts > sms) return;
+        const int64_t waves = (tiles * ctas * parts + sms - 1) / sms;
+        const int64_t block = ctas == 2 ? 410 : std::max(240, (128 + tn) * kStageK / 115), epilogue = 8 * tn;
+        int64_t t = 3200 + (k_blocks + parts - 1) / parts * block + epilogue + (parts > 1 ? 2200 + 17 * tn : 0);
+        t += (waves - 1) * std::max(k_blocks * block, epilogue);
+        if (t < least) {
+            least = t;
+            best = {ctas, tn, parts};
+        }
+    };
     const int64_t row_blocks = (rows + 255) / 256;
-    int tn = (int)((rows + row_blocks - 1) / row_blocks + 15) / 16 * 16;
-    const int64_t tiles = (n + 127) / 128 * ((rows + tn - 1) / tn);
-    if (rows > 256 && tiles >= 2 * sms) return {2, 256, 1};
-    int parts = 1;
-    while (parts < 8 && 2 * parts * tiles <= sms && 2 * parts <= k_blocks) parts *= 2;
-    return {1, tn, parts};
+    const int even = (int)((rows + row_blocks - 1) / row_blocks + 15) / 16 * 16;   // the rows in equal tiles
+    for (const int tn : {even, 16, 32, 64, 128, 192, 256})
+        if (tn == even || tn < even || rows > 256)
+            for (int parts = 1; parts <= 8 && parts <= k_blocks; parts *= 2) consider(1, tn, parts);
+    if (rows > 256) consider(2, 256, 1);
+    return best;
 }
 
 // early: the launch before this one wrote the codes and nothing else that the product reads.
@@ -813,7 +854,9 @@ int ygg_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, const 
     float *scale = (float *)(codes + rows * padded);
     const Linear q{codes, d_weight, padded, weight_stride, scale, d_scale, d_bias, rows, n, (int)k, d_out, out_stride};
     int rc;
-    if (rows * k <= kFewFused && is_few(rows, (int)k)) {
+    // one launch: 1 x 1280 x 256 in 3.7 us against 4.1, 1 x 4096 x 4096 in 6.7 against 6.4 but 3 us less on the host, which
+    // larger weights would hide (1 x 4096 x 32768: 24.5 against 24.1)
+    if (rows * k <= 4096 && n * k <= (1 << 25) && is_few(rows, (int)k)) {
         int done = YGG_OK;
         rc = by_type(dtype, [&](auto t) {
             done = launch_few<decltype(t)>({q, d_x, row_stride, out_dtype, 1, few_room((int)k), true}, st);
