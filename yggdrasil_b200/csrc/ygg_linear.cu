@@ -51,14 +51,35 @@ __device__ __forceinline__ Factors factors(float most) {
 // Magnitudes compare as the integers of their bits, with NaN above infinity above the numbers.
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-// The code of x as the low byte: the product rounds once, and adding 1.5 2^23 rounds it to the nearest integer, ties to
-// even. |x| inverse is at most 127 (1 + 2^-22), so no code is beyond 127.
-__device__ __forceinline__ uint32_t code(float x, float inverse) {
-    return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
+// The largest magnitude of a vector; 16-bit types compare in pairs.
+__device__ __forceinline__ uint32_t magnitude_of(const uint4 &q, float) {
+    return max(max(q.x & 0x7FFFFFFFu, q.y & 0x7FFFFFFFu), max(q.z & 0x7FFFFFFFu, q.w & 0x7FFFFFFFu));
+}
+__device__ __forceinline__ uint32_t magnitude_16(const uint4 &q) {
+    const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu), __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFFu, m >> 16);
+}
+__device__ __forceinline__ uint32_t magnitude_of(const uint4 &q, __half) {
+    const uint32_t m = magnitude_16(q);
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+__device__ __forceinline__ uint32_t magnitude_of(const uint4 &q, __nv_bfloat16) { return magnitude_16(q) << 16; }
+
+// A code is the low byte of the sum: the product rounds once, and adding 1.5 2^23 rounds it to the nearest integer, ties
+// to even. |x| inverse is at most 127 (1 + 2^-22), so no code is beyond 127.
+// The sums are single instructions on purpose: as a pair (add.rn.f32x2) after the paired product they came out as if
+// fused with it, rounded once, and codes at halves went the other way.
+__device__ __forceinline__ uint2 code2(float a, float b, float inverse) {
+    float x, y;
+    asm("{\n\t.reg .b64 v, f;\n\t"
+        "mov.b64 v, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "f"(a), "f"(b), "f"(inverse));
+    return make_uint2(__float_as_uint(__fadd_rn(x, 12582912.0f)), __float_as_uint(__fadd_rn(y, 12582912.0f)));
 }
 __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float inverse) {
-    return __byte_perm(__byte_perm(code(a, inverse), code(b, inverse), 0x0040),
-                       __byte_perm(code(c, inverse), code(d, inverse), 0x0040), 0x5410);
+    const uint2 x = code2(a, b, inverse), y = code2(c, d, inverse);
+    return __byte_perm(__byte_perm(x.x, x.y, 0x0040), __byte_perm(y.x, y.y, 0x0040), 0x5410);
 }
 __device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[4], float inverse) {
     *(uint32_t *)p = inverse == 0.0f ? 0u : code4(v[0], v[1], v[2], v[3], inverse);
@@ -90,10 +111,13 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
         const int j = (i * THREADS + t) * N;
-        float v[N];
-        unpack(q[i], v, T());
+        if (j < p.k && j + N > p.k) {   // the vector that holds the row's end
+            uint32_t *w = (uint32_t *)&q[i];
 #pragma unroll
-        for (int e = 0; e < N; e++) most = max(most, j + e < p.k ? magnitude(v[e]) : 0u);
+            for (int e = 0; e < N; e++)
+                if (j + e >= p.k) w[e * 4 / N] &= N == 4 ? 0u : 0xFFFFu << (e & 1 ? 0 : 16);
+        }
+        most = max(most, magnitude_of(q[i], T()));
     }
     most = __reduce_max_sync(~0u, most);
     if (THREADS > 32) {
@@ -110,9 +134,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
         if (j >= p.padded) continue;
         float v[N];
         unpack(q[i], v, T());
-#pragma unroll
-        for (int e = 0; e < N; e++)
-            if (j + e >= p.k) v[e] = 0.0f;
         store_codes(codes + j, v, f.inverse);
     }
     if (t == 0) p.scale[row] = f.scale;
@@ -145,13 +166,17 @@ template <typename T> __global__ void __launch_bounds__(256) quantize_any_kernel
     }
 }
 
+#ifndef WV
+#define WV 512
+#endif
+constexpr int kWarpVecs = WV;
 template <typename T> void launch_quantize(const Quantize &p, cudaStream_t st) {
     constexpr int N = kPer<T>;
     const bool even = ((uintptr_t)p.x & 15) == 0 && (p.rows == 1 || p.stride % N == 0);
     const int vecs = (p.k + N - 1) / N;
     if (!even || vecs > 2048 || p.rows > INT32_MAX) {
         quantize_any_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 8 * sm_count()), 256, 0, st>>>(p);
-    } else if (vecs <= 512 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
+    } else if (vecs <= kWarpVecs && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
         const unsigned grid = (unsigned)((p.rows + 7) / 8);
         if (vecs <= 32) quantize_kernel<T, 32, 1><<<grid, 256, 0, st>>>(p);
         else if (vecs <= 64) quantize_kernel<T, 32, 2><<<grid, 256, 0, st>>>(p);

@@ -33,7 +33,7 @@ struct Rows {
     float *logprob, *entropy, *lse;
     int32_t *top_ids;
     float *top_logprobs;
-    float4 *stats;        // m, 1 / s, log s, H: what the gradient needs; or null
+    float4 *stats;        // m, log2 s (inf for an empty row), log s, H: what the gradient needs; or null
 };
 
 struct Grad {
@@ -48,9 +48,10 @@ struct Grad {
     int64_t grad_stride;
 };
 
+// 2^x, results below 2^-126 as 0 (keeping them costs three instructions more, and no sum of a row would show them).
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -88,26 +89,117 @@ __device__ __forceinline__ int64_t token_of(const void *tokens, int bytes, int64
 }
 
 // Rows may begin anywhere: a row is read from the 16-byte boundary at or before it, `off` entries early, and place u of
-// what is read holds the entry u - off. The places outside the row lie in the same 16 bytes as one of its own entries.
-template <typename T> __device__ __forceinline__ int offset_of(const T *x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+// what is read holds the entry u - off (32 bits: a row has less than 2^31 entries). The places outside the row lie in the same 16 bytes as one of its own entries.
+template <typename T> __device__ __forceinline__ uint32_t offset_of(const T *x) { return ((uint32_t)(uintptr_t)x & 15) / sizeof(T); }
+
+template <typename T> constexpr uint32_t kMinusInf = 0;
+template <> constexpr uint32_t kMinusInf<float> = 0xFF800000u;
+template <> constexpr uint32_t kMinusInf<__half> = 0xFC00u;
+template <> constexpr uint32_t kMinusInf<__nv_bfloat16> = 0xFF80u;
 
 // A warp's run of 32 kPer places from u0 on, lane l those from u0 + l kPer on; -inf outside the row's places [off, end).
 template <typename T>
-__device__ __forceinline__ void load_run(const T *from, int64_t u0, int off, int64_t end, int lane, float (&v)[kPer<T>]) {
-    const int64_t u = u0 + lane * kPer<T>;
+__device__ __forceinline__ uint4 load_run(const T *from, uint32_t u0, uint32_t off, uint32_t end, int lane) {
+    constexpr int N = kPer<T>;
+    const uint32_t u = u0 + lane * N;
     uint4 q = make_uint4(0, 0, 0, 0);
     if (u < end) q = load_stream(from + u);
-    unpack(q, v, T());
-    if (u + kPer<T> > end || u < off) {
+    if (u + N > end || u < off) {
+        uint32_t *w = (uint32_t *)&q;
 #pragma unroll
-        for (int i = 0; i < kPer<T>; i++)
-            if (u + i >= end || u + i < off) v[i] = -INFINITY;
+        for (int i = 0; i < N; i++)
+            if (u + i >= end || u + i < off) {
+                if (N == 4) w[i] = kMinusInf<T>;
+                else w[i / 2] = (w[i / 2] & (0xFFFFu << (i & 1 ? 0 : 16))) | kMinusInf<T> << (i & 1 ? 16 : 0);
+            }
     }
+    return q;
+}
+template <typename T>
+__device__ __forceinline__ void load_run(const T *from, uint32_t u0, uint32_t off, uint32_t end, int lane, float (&v)[kPer<T>]) {
+    unpack(load_run(from, u0, off, end, lane), v, T());
+}
+
+// The largest of a vector, NaN left out. 16-bit types compare in pairs.
+__device__ __forceinline__ float largest(const uint4 &q, float) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ float largest(const uint4 &q, __half) {
+    const __half2 *h = (const __half2 *)&q;
+    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float largest(const uint4 &q, __nv_bfloat16) {
+    const __nv_bfloat162 *h = (const __nv_bfloat162 *)&q;
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+}
+
+// Two floats to an instruction.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split(Pair v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair exp2_approx(Pair v) {
+    const float2 f = split(v);
+    return pair(exp2_approx(f.x), exp2_approx(f.y));
+}
+
+// Adds entries to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN; it is rare, so
+// the sum says whether there was one, and only then the products are formed again with y cut off.
+template <int N, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const float (&v)[RUNS][N]) {
+    const float m = a.m == -INFINITY ? 0.0f : a.m;
+    const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e);
+    Pair s = 0, t = 0;
+#pragma unroll
+    for (int r = 0; r < RUNS; r++)
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const Pair y = add(pair(v[r][i], v[r][i + 1]), minus), e = exp2_approx(mul(y, l));
+            s = add(s, e);
+            t = fma(e, y, t);
+        }
+    const float2 sf = split(s), tf = split(t);
+    float sum = tf.x + tf.y;
+    if (sum != sum) {
+        sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float y = v[r][i] - m;
+                sum = fmaf(exp2_approx(y * kLog2e), fmaxf(y, kFloor), sum);
+            }
+    }
+    a.s += sf.x + sf.y;
+    a.t += sum;
 }
 
 using Key = unsigned long long;   // orders entries: value above, then the lower index
-__device__ __forceinline__ Key key_of(float x, int64_t j) {
-    return ((Key)((unsigned)order(x) ^ 0x80000000u) << 32) | (unsigned)~(unsigned)j;
+__device__ __forceinline__ Key key_of(float x, uint32_t j) {
+    return ((Key)((unsigned)order(x) ^ 0x80000000u) << 32) | ~j;
 }
 __device__ __forceinline__ float value_of(Key k) { return unorder((int)((unsigned)(k >> 32) ^ 0x80000000u)); }
 __device__ __forceinline__ int32_t index_of(Key k) { return (int32_t)~(unsigned)k; }
@@ -129,7 +221,8 @@ struct Ends {
     }
     __device__ __forceinline__ float logprob(float x) const { return empty ? -INFINITY : (x - m) - ls; }
 };
-template <typename T> __device__ __forceinline__ void write_row(const Rows &p, int64_t row, const T *x, const Sums &a, const Ends &e) {
+template <typename T>
+__device__ __forceinline__ void write_row(const Rows &p, int64_t row, const T *x, const Sums &a, const Ends &e) {
     const int64_t t = token_of(p.tokens, p.token_bytes, row);
     float lp = 0.0f;
     if (t >= p.vocab) lp = NAN;
@@ -137,7 +230,7 @@ template <typename T> __device__ __forceinline__ void write_row(const Rows &p, i
     p.logprob[row] = lp;
     p.entropy[row] = e.h;
     p.lse[row] = e.m + e.ls;
-    if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? 0.0f : 1.0f / a.s, e.empty ? 0.0f : e.ls, e.h);
+    if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? INFINITY : log2f(a.s), e.empty ? 0.0f : e.ls, e.h);
 }
 __device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, Key key, const Ends &e) {
     p.top_ids[row * p.top + k] = index_of(key);
@@ -154,125 +247,226 @@ __device__ __forceinline__ int kth_of_lanes(int mine, int k, int lane) {
     }
     return best;
 }
+// The same over four values a lane (k <= 128): a closer bound.
+__device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k, int lane) {
+    const auto order2 = [](int &x, int &y) {
+        const int t = min(x, y);
+        x = max(x, y);
+        y = t;
+    };
+    order2(a, b), order2(c, d), order2(a, c), order2(b, d), order2(b, c);
+    int best = 0;
+    for (int i = 0; i < k; i++) {
+        best = __reduce_max_sync(~0u, a);
+        const unsigned who = __ballot_sync(~0u, a == best);
+        if (lane == __ffs(who) - 1) a = b, b = c, c = d, d = INT32_MIN;
+    }
+    return best;
+}
 
-// Short rows: a warp holds a row in registers, RUNS runs of 32 kPer entries. Alternatives: the k-th largest of the lanes'
-// maxima bounds the k-th largest entry from below, so the few entries at or above it are the candidates, and they are
-// ranked by counting. Where ties make them more than 32, the equal ones that come too late are left out; where entries
-// above the bound are more than 32, or alternatives are, they are taken one at a time.
-template <typename T, int RUNS> __global__ void __launch_bounds__(128) short_kernel(const Rows p) {
-    constexpr int N = kPer<T>;
-    __shared__ Key lists[4][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * 4 + warp;
+// Up to 8 entries: a thread a row.
+template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const Rows p) {
+    const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
     if (row >= p.rows) return;
     const T *x = (const T *)p.logits + row * p.stride;
-    const int off = offset_of(x), end = (int)p.vocab + off;
-    float v[RUNS][N];
-    float most = -INFINITY;
+    float v[1][8];
+    Sums a = none();
 #pragma unroll
-    for (int r = 0; r < RUNS; r++) load_run<T>(x - off, r * 32 * N, off, end, lane, v[r]);
-#pragma unroll
-    for (int r = 0; r < RUNS; r++)
-#pragma unroll
-        for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
-    const int mine = order(most);
-    const float top1 = unorder(__reduce_max_sync(~0u, mine)), m = top1 == -INFINITY ? 0.0f : top1;
-    Sums a{top1, 0.0f, 0.0f};
-#pragma unroll
-    for (int r = 0; r < RUNS; r++)
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float y = v[r][i] - m, e = exp2_approx(y * kLog2e);
-            a.s += e;
-            a.t = fmaf(e, fmaxf(y, kFloor), a.t);
-        }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        a.s += __shfl_xor_sync(~0u, a.s, o);
-        a.t += __shfl_xor_sync(~0u, a.t, o);
+    for (int i = 0; i < 8; i++) {
+        v[0][i] = i < p.vocab ? to_f(x[i]) : -INFINITY;
+        a.m = fmaxf(a.m, v[0][i]);
     }
+    add_entries(a, v);
     const Ends e(a);
-    if (lane == 0) write_row(p, row, x, a, e);
+    write_row(p, row, x, a, e);
     if (p.top == 0) return;
-    int n = 33;
-    if (p.top <= 32) {
-        const float bound = unorder(kth_of_lanes(mine, p.top, lane));
-        n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j != i) above += order(v[0][j]) + (j < i) > order(v[0][i]);
+        if (i < p.vocab && above < p.top) write_top(p, row, above, key_of(v[0][i], i), e);
+    }
+}
+
+// Short rows: a warp holds a row in registers, RUNS runs of 32 kPer places, and takes R rows one after another, so that
+// what a row needs only once (the sums over the lanes, the logarithm, the token, the writes) is done for R rows by
+// different lanes at once. Alternatives: the k-th largest of the lanes' maxima (of four maxima a lane for more than 8
+// alternatives: 20 of 128 bins leave about 22 candidates, 20 of 32 about 31, 64 of 128 about 89) bounds the k-th largest
+// entry from below, so the few entries at or above it are the candidates, and they are ranked by counting. Where ties
+// make them more than the list holds, the equal ones that come too late are left out; where entries above the bound are
+// too many, they are taken one at a time.
+constexpr int kShortWarps = 4, kCandidates = 128, kList = kCandidates + 1;   // an odd pitch: lists begin in unlike banks
+template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
+    constexpr int N = kPer<T>;
+    __shared__ Key lists[kShortWarps][R][kList];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row0 = ((int64_t)blockIdx.x * kShortWarps + warp) * R;
+    if (row0 >= p.rows) return;
+    const unsigned below = (1u << lane) - 1;
+    float ms[R], sums[2 * R];
+    int found[R];
+#pragma unroll
+    for (int w = 0; w < R; w++) {
+        const int64_t row = min(row0 + w, p.rows - 1);   // rows past the last are the last once more, unseen
+        const T *x = (const T *)p.logits + row * p.stride;
+        const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
+        const T *from = x - off;
+        float v[RUNS][N];
+        float most = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++) load_run<T>(from, r * 32 * N, off, end, lane, v[r]);
 #pragma unroll
         for (int r = 0; r < RUNS; r++)
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int u = (r * 32 + lane) * N + i;
-                const bool in = !(v[r][i] < bound) && u >= off && u < end;
-                const unsigned who = __ballot_sync(~0u, in);
-                const int at = n + __popc(who & ((1u << lane) - 1));
-                if (in && at < 32) lists[warp][at] = key_of(v[r][i], u - off);
-                n += __popc(who);
+            for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
+        const int mine = order(most);
+        Sums a{unorder(__reduce_max_sync(~0u, mine)), 0.0f, 0.0f};
+        add_entries(a, v);
+        ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
+        found[w] = 0;
+        if (p.top == 0) continue;
+        Key *list = lists[warp][w];
+        int n;
+        {
+            int kth;
+            if (p.top <= 8) {
+                kth = kth_of_lanes(mine, p.top, lane);
+            } else {
+                float bin[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) bin[k] = v[0][k];
+#pragma unroll
+                for (int r = 0; r < RUNS; r++)
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        if (r || i >= 4) bin[i & 3] = fmaxf(bin[i & 3], v[r][i]);
+                kth = kth_of_lanes(order(bin[0]), order(bin[1]), order(bin[2]), order(bin[3]), p.top, lane);
             }
-        if (n > 32) {   // ties at the bound: the entries above it, and as many equal ones as are still wanted
-            __syncwarp();
-            n = 0;
+            const float bound = unorder(kth);
+            unsigned in = 0;
 #pragma unroll
             for (int r = 0; r < RUNS; r++)
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const int u = (r * 32 + lane) * N + i;
-                    const bool in = v[r][i] > bound && u >= off && u < end;
-                    const unsigned who = __ballot_sync(~0u, in);
-                    const int at = n + __popc(who & ((1u << lane) - 1));
-                    if (in && at < 32) lists[warp][at] = key_of(v[r][i], u - off);
-                    n += __popc(who);
-                }
-            // the equal ones in the order of their indices: a lane's entries of a run lie side by side
+                for (int i = 0; i < N; i++) in |= v[r][i] >= bound ? 1u << (r * N + i) : 0u;
+            if (bound == -INFINITY) {   // every entry, NaN too, but not the places outside the row
+                in = ~0u;
 #pragma unroll
-            for (int r = 0; r < RUNS; r++) {
-                if (n >= p.top) break;
-                int own = 0;
+                for (int r = 0; r < RUNS; r++)
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const int u = (r * 32 + lane) * N + i;
-                    own += !(v[r][i] < bound) && !(v[r][i] > bound) && u >= off && u < end;
-                }
-                int upto = own;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(~0u, upto, o);
-                    if (lane >= o) upto += y;
-                }
-                int at = n + upto - own;
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const int u = (r * 32 + lane) * N + i;
-                    if (!(v[r][i] < bound) && !(v[r][i] > bound) && u >= off && u < end) {
-                        if (at < p.top) lists[warp][at] = key_of(v[r][i], u - off);
-                        at++;
+                    for (int i = 0; i < N; i++) {
+                        const uint32_t u = (r * 32 + lane) * N + i;
+                        if (u < off || u >= end) in &= ~(1u << (r * N + i));
+                    }
+                if (RUNS * N < 32) in &= (1u << (RUNS * N & 31)) - 1;
+            }
+            n = __reduce_add_sync(~0u, __popc(in));
+            if (n <= kCandidates) {
+                unsigned who;
+                for (int done = 0; (who = __ballot_sync(~0u, in != 0)) != 0; done += __popc(who)) {
+                    if (in) {
+                        const int bit = __ffs(in) - 1, u = (bit / N * 32 + lane) * N + bit % N;
+                        list[done + __popc(who & below)] = key_of(to_f(from[u]), u - off);
+                        in &= in - 1;
                     }
                 }
-                n = min(p.top, n + __shfl_sync(~0u, upto, 31));
+            } else {   // ties at the bound: the entries above it, and as many equal ones as are still wanted
+                n = 0;
+#pragma unroll
+                for (int r = 0; r < RUNS; r++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const bool more = v[r][i] > bound;
+                        const unsigned who = __ballot_sync(~0u, more);
+                        const int at = n + __popc(who & below);
+                        if (more && at < kCandidates) list[at] = key_of(v[r][i], (r * 32 + lane) * N + i - off);
+                        n += __popc(who);
+                    }
+                // in the order of their indices: a lane's entries of a run lie side by side
+#pragma unroll
+                for (int r = 0; r < RUNS; r++) {
+                    if (n >= p.top) break;
+                    const unsigned mask = (N == 32 ? ~0u : (1u << N) - 1) << (r * N);
+                    unsigned equal = in & mask;
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        if (v[r][i] > bound) equal &= ~(1u << (r * N + i));
+                    const int own = __popc(equal);
+                    int upto = own;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int y = __shfl_up_sync(~0u, upto, o);
+                        if (lane >= o) upto += y;
+                    }
+                    int at = n + upto - own;
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        if (equal >> (r * N + i) & 1) {
+                            if (at < p.top) list[at] = key_of(v[r][i], (r * 32 + lane) * N + i - off);
+                            at++;
+                        }
+                    n = min(p.top, n + __shfl_sync(~0u, upto, 31));
+                }
             }
         }
-    }
-    if (n <= 32) {
-        __syncwarp();
-        const Key key = lane < n ? lists[warp][lane] : 0;
-        int rank = 0;
-        for (int i = 0; i < n; i++) rank += lists[warp][i] > key;
-        if (lane < n && rank < p.top) write_top(p, row, rank, key, e);
-        return;
-    }
-    Key last = ~0ull;
-    for (int k = 0; k < p.top; k++) {
-        Key best = 0;
+        if (n > kCandidates) {
+            Key last = ~0ull;
+            for (int k = 0; k < p.top; k++) {
+                Key best = 0;
 #pragma unroll
-        for (int r = 0; r < RUNS; r++)
+                for (int r = 0; r < RUNS; r++)
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int u = (r * 32 + lane) * N + i;
-                const Key key = u >= off && u < end ? key_of(v[r][i], u - off) : 0;
-                if (key < last && key > best) best = key;
+                    for (int i = 0; i < N; i++) {
+                        const uint32_t u = (r * 32 + lane) * N + i;
+                        const Key key = u >= off && u < end ? key_of(v[r][i], u - off) : 0;
+                        if (key < last && key > best) best = key;
+                    }
+                last = warp_max(best);
+                if (lane == 0) list[k] = last;
             }
-        last = warp_max(best);
-        if (lane == 0) write_top(p, row, k, last, e);
+            n = p.top;
+        }
+        found[w] = n;
+    }
+    // lane l serves row l mod R: the sums of 2 R values over the lanes, halved with the values while there are several
+#pragma unroll
+    for (int half = R, o = 16; o; o >>= 1, half = half > 1 ? half / 2 : 0) {
+        if (half) {
+#pragma unroll
+            for (int i = 0; i < half; i++) {
+                const bool upper = lane & o;
+                const float give = upper ? sums[i] : sums[half + i];
+                sums[i] = (upper ? sums[half + i] : sums[i]) + __shfl_xor_sync(~0u, give, o);
+            }
+        } else {
+            sums[0] += __shfl_xor_sync(~0u, sums[0], o);
+        }
+    }
+    // value i of the 2 R is now in the lanes whose upper bits, first bit first, spell i
+    const int mine = lane & (R - 1);
+    constexpr int kStep = 16 / R;   // lanes of one value: t of a row lies 16 lanes above its s
+    Sums a;
+    a.m = ms[0];
+    int n = found[0], most = found[0];
+#pragma unroll
+    for (int w = 1; w < R; w++) {
+        if (mine == w) a.m = ms[w], n = found[w];
+        most = max(most, found[w]);
+    }
+    a.s = __shfl_sync(~0u, sums[0], mine * kStep);
+    a.t = __shfl_sync(~0u, sums[0], 16 + mine * kStep);
+    const Ends e(a);
+    const int64_t row = row0 + mine;
+    if (row >= p.rows) n = 0;
+    if (lane < R && row < p.rows) write_row(p, row, (const T *)p.logits + row * p.stride, a, e);
+    __syncwarp();
+    const Key *list = lists[warp][mine];
+    for (int slot = lane / R; slot < most; slot += 32 / R) {
+        const Key key = slot < n ? list[slot] : ~0ull;
+        int above = 0;
+        for (int i = 0; i < n; i++) above += list[i] > key;
+        if (slot < n && above < p.top) write_top(p, row, above, key, e);
     }
 }
 
@@ -313,8 +507,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const int rank = blockIdx.x - (int)row * cluster;
     if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // the first block runs
     const T *x = (const T *)p.logits + row * p.stride;
-    const int off = offset_of(x);
-    const int64_t span = (int64_t)(32 * N) << shift, end = p.vocab + off;
+    const uint32_t off = offset_of(x), span = (32u * N) << shift, end = (uint32_t)p.vocab + off;
     const T *from = x - off;
     Sums a = none();
     const int w = rank * kLongWarps + warp, warps = cluster * kLongWarps;
@@ -322,29 +515,22 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const int steps = shift ? 1 << (shift - 2) : 1;
     for (int g0 = w * (shift ? 1 : kBatch); g0 < segments; g0 += warps * (shift ? 1 : kBatch)) {
         float top_of[kBatch];
-        for (int q = 0; q < steps; q++) {
+        for (int step = 0; step < steps; step++) {
+            uint4 q[kBatch];
             float v[kBatch][N], most = -INFINITY;
-            const int64_t u0 = g0 * span + (int64_t)q * kBatch * 32 * N;
+            const uint32_t u0 = g0 * span + step * kBatch * 32 * N;
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) load_run<T>(from, u0 + (int64_t)b * 32 * N, off, end, lane, v[b]);
+            for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
 #pragma unroll
             for (int b = 0; b < kBatch; b++) {
-                float t = v[b][0];
-#pragma unroll
-                for (int i = 1; i < N; i++) t = fmaxf(t, v[b][i]);
-                top_of[b] = shift && q ? fmaxf(top_of[b], t) : t;
+                const float t = largest(q[b], T());
+                top_of[b] = shift && step ? fmaxf(top_of[b], t) : t;
                 most = fmaxf(most, t);
             }
             if (most > a.m) raise(a, most);
-            const float m = a.m == -INFINITY ? 0.0f : a.m;
 #pragma unroll
-            for (int b = 0; b < kBatch; b++)
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float y = v[b][i] - m, e = exp2_approx(y * kLog2e);
-                    a.s += e;
-                    a.t = fmaf(e, fmaxf(y, kFloor), a.t);
-                }
+            for (int b = 0; b < kBatch; b++) unpack(q[b], v[b], T());
+            add_entries(a, v);
         }
         if (p.top) {
             if (shift) {
@@ -454,12 +640,12 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const float bound = picks < p.top ? -INFINITY : unorder(sh.bound);
     const int runs = picks << shift;   // runs of 32 N entries in the picked segments
     for (int q = warp; q < runs; q += kLongWarps) {
-        const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+        const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
         float v[N];
         load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int64_t u = u0 + lane * N + i;
+            const uint32_t u = u0 + lane * N + i;
             if (!(v[i] < bound) && u >= off && u < end) {
                 const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
                 if (at < kLongThreads) sh.keys[at] = key_of(v[i], u - off);
@@ -473,12 +659,12 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         // value and index) is a better bound
         Key mine = 0;
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t u = u0 + lane * N + i;
+                const uint32_t u = u0 + lane * N + i;
                 if (u >= off && u < end) mine = max(mine, key_of(v[i], u - off));
             }
         }
@@ -493,12 +679,12 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         __syncthreads();
         const Key least = sh.best[0];
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t u = u0 + lane * N + i;
+                const uint32_t u = u0 + lane * N + i;
                 const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
                 if (key && key >= least) {
                     const int at = atomicAdd(&sh.count, 1);
@@ -520,12 +706,12 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     for (int k = 0; k < p.top; k++) {
         Key best = 0;
         for (int q = warp; q < runs; q += kLongWarps) {
-            const int64_t u0 = sh.picked[q >> shift] * span + (int64_t)(q & ((1 << shift) - 1)) * 32 * N;
+            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int64_t u = u0 + lane * N + i;
+                const uint32_t u = u0 + lane * N + i;
                 const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
                 if (key < last && key > best) best = key;
             }
@@ -547,15 +733,27 @@ int cluster_for(int64_t rows, int64_t runs, int sms) {
     return c;
 }
 
+// Four rows a warp as soon as they fill the SMs.
+template <typename T, int RUNS> void launch_short(const Rows &p, cudaStream_t st) {
+    const bool many = p.rows >= (int64_t)sm_count() * 64;
+    const int64_t per = kShortWarps * (many ? 4 : 1);
+    const unsigned grid = (unsigned)((p.rows + per - 1) / per);
+    if (many) short_kernel<T, RUNS, 4><<<grid, kShortWarps * 32, 0, st>>>(p);
+    else short_kernel<T, RUNS, 1><<<grid, kShortWarps * 32, 0, st>>>(p);
+}
+
 template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
     constexpr int N = kPer<T>;
     const bool even = ((uintptr_t)p.logits & 15) == 0 && (p.rows == 1 || p.stride % N == 0);   // every row on a boundary
     const int64_t runs = (p.vocab + (even ? 0 : N - 1) + 32 * N - 1) / (32 * N);
+    if (p.vocab <= 8) {
+        tiny_kernel<T><<<(unsigned)((p.rows + 127) / 128), 128, 0, st>>>(p);
+        return cudaGetLastError();
+    }
     if (runs <= 32 / N) {   // at most 32 places a lane
-        const unsigned grid = (unsigned)((p.rows + 3) / 4);
-        if (runs <= 1) short_kernel<T, 1><<<grid, 128, 0, st>>>(p);
-        else if (runs <= 2) short_kernel<T, 2><<<grid, 128, 0, st>>>(p);
-        else short_kernel<T, 32 / N><<<grid, 128, 0, st>>>(p);
+        if (runs <= 1) launch_short<T, 1>(p, st);
+        else if (runs <= 2) launch_short<T, 2>(p, st);
+        else launch_short<T, 32 / N>(p, st);
         return cudaGetLastError();
     }
     int shift = 0;
@@ -576,9 +774,10 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, long_kernel<T>, p, cluster, shift, segments);
 }
 
-// What the gradient of a row needs: p (A + B y) everywhere, and more at the given token and the alternatives.
+// What the gradient of a row needs: p (A + B y) everywhere, p = 2^(y log2 e - log2 s), and more at the given token and
+// the alternatives.
 struct RowGrad {
-    float m, inv_s, A, B, given;
+    float m, l2, A, B, given;
     int64_t token;   // -1: none
     __device__ __forceinline__ RowGrad(const Grad &p, int64_t row) {
         const float4 st = p.stats[row];
@@ -589,11 +788,33 @@ struct RowGrad {
         float c = (p.g_lse ? p.g_lse[row] : 0.0f) - given;
         if (p.g_top)
             for (int k = 0; k < p.top; k++) c -= p.g_top[row * p.top + k];
-        m = st.x, inv_s = st.y, A = c - gh * (st.w - st.z), B = -gh;
+        m = st.x, l2 = st.y, A = c - gh * (st.w - st.z), B = -gh;
     }
     __device__ __forceinline__ float dense(float x) const {
         const float y = x - m;
-        return exp2_approx(y * kLog2e) * inv_s * fmaf(B, fmaxf(y, kFloor), A);
+        return exp2_approx(fmaf(y, kLog2e, -l2)) * fmaf(B, fmaxf(y, kFloor), A);
+    }
+    // The same for a vector, in pairs. An entry of -inf gives NaN (p = 0 times infinity): then once more, with y cut off.
+    template <int N> __device__ __forceinline__ void dense(float (&v)[N]) const {
+        const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e), s = pair(-l2, -l2), a = pair(A, A), b = pair(B, B);
+        Pair sum = 0, g[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const Pair y = add(pair(v[2 * i], v[2 * i + 1]), minus);
+            g[i] = mul(exp2_approx(fma(y, l, s)), fma(b, y, a));
+            sum = add(sum, g[i]);
+        }
+        const float2 f = split(sum);
+        if (f.x + f.y != f.x + f.y) {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = dense(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                const float2 h = split(g[i]);
+                v[2 * i] = h.x, v[2 * i + 1] = h.y;
+            }
+        }
     }
 };
 
@@ -624,33 +845,33 @@ template <typename T, bool SAME> __global__ void __launch_bounds__(256) grad_ker
     const int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t row = it < ((int64_t)1 << 32) ? (unsigned)it / chunks : it / chunks;
     if (row >= p.rows) return;
-    const int64_t u0 = (it - row * chunks) * (kGradRuns * 32 * N);
+    const uint32_t u0 = (uint32_t)(it - row * chunks) * (kGradRuns * 32 * N);
     const T *x = (const T *)p.logits + row * p.stride;
     T *g = (T *)p.grad + row * p.grad_stride;
-    const int off = offset_of(x);
-    const int64_t end = p.vocab + off;
-    float v[kGradRuns][N];
+    const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
+    uint4 q[kGradRuns];
 #pragma unroll
-    for (int r = 0; r < kGradRuns; r++) load_run<T>(x - off, u0 + r * 32 * N, off, end, lane, v[r]);
+    for (int r = 0; r < kGradRuns; r++) q[r] = load_run<T>(x - off, u0 + r * 32 * N, off, end, lane);
     const RowGrad d(p, row);
 #pragma unroll
     for (int r = 0; r < kGradRuns; r++) {
-        const int64_t u = u0 + (r * 32 + lane) * N;
+        const uint32_t u = u0 + (r * 32 + lane) * N;
         if (u >= end) break;
-#pragma unroll
-        for (int i = 0; i < N; i++) v[r][i] = d.dense(v[r][i]);
+        float v[N];
+        unpack(q[r], v, T());
+        d.dense(v);
         if (SAME && u >= off && u + N <= end) {
-            store_stream(g - off + u, pack(v[r], T()));
+            store_stream(g + (int64_t)u - off, pack(v, T()));
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (u + i >= off && u + i < end) from_f(v[r][i], g[u + i - off]);
+                if (u + i >= off && u + i < end) from_f(v[i], g[u + i - off]);
         }
     }
     __syncwarp();
     // the given token and the alternatives: written again, whole, so that they are rounded once
-    if (d.inv_s == 0.0f) return;
-    const int64_t j0 = u0 - off, j1 = min(j0 + kGradRuns * 32 * N, p.vocab);
+    if (d.l2 == INFINITY) return;   // an empty row
+    const int64_t j0 = (int64_t)u0 - off, j1 = min(j0 + kGradRuns * 32 * N, p.vocab);
     for (int q = lane; q <= (p.g_top ? p.top : 0); q += 32) {
         const int64_t j = q == 0 ? d.token : p.top_ids[row * p.top + q - 1];
         if (j < 0 || j < j0 || j >= j1 || (q > 0 && j == d.token)) continue;
