@@ -257,10 +257,12 @@ YGG_API int ygg_linear_status(int device, void *stream, int *status_out);
  * p. Sources and counts of one call are those of its beginning; new pages are the free ones in ascending order, given
  * in the order of the call's list. Negative stream and page indices are padding and skipped. What cannot be done is left
  * undone and sets a status word to 1: status[YGG_CACHE_BAD_INDEX] (an index beyond its range, a child that holds pages, a
- * child named twice: its first fork counts), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row). Calls
- * on one cache are ordered by the caller (one stream, or events). */
+ * child named twice: its first fork counts), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row),
+ * status[YGG_CACHE_TIMEOUT] (a bounded wait of a call's blocks for each other gave up: the cache is not to be used any
+ * more). Calls on one cache are ordered by the caller (one stream, or events). */
 #define YGG_CACHE_BAD_INDEX 0
 #define YGG_CACHE_NO_ROOM 1
+#define YGG_CACHE_TIMEOUT 2
 
 typedef struct {
     void *pages;             /* page_count pages of page_bytes */
@@ -270,7 +272,8 @@ typedef struct {
     int32_t per_stream;
     int32_t *length;         /* [streams] */
     int32_t *refs;           /* [page_count] */
-    int32_t *status;         /* two words, on the device or mapped host memory (pinned); the caller clears them */
+    int32_t *status;         /* three words, on the device or mapped host memory (pinned); the caller clears them */
+    uint32_t *sync;          /* two words of device memory, zero before the cache's first call */
 } ygg_cache_t;
 
 /* Bytes of device workspace of ygg_cache_fork with n entries, and of ygg_cache_compact (any n). */

@@ -344,12 +344,13 @@ def test_refusals():
 def test_c_entry_refuses_bad_arguments():
     """Checked before any CUDA call."""
     lib, E, p = _native.ops(), _native, 4096
-    good = lambda: _native.YggCache(p, 8, 16, p, 4, 2, p, p, p)  # noqa: E731
+    good = lambda: _native.YggCache(p, 8, 16, p, 4, 2, p, p, p, p)  # noqa: E731
     size = lib.ygg_cache_workspace(ctypes.byref(good()), 5)
     assert size > 0 and lib.ygg_cache_workspace(None, 5) == 0 and lib.ygg_cache_workspace(ctypes.byref(good()), -1) == 0
     assert lib.ygg_cache_fork(0, None, 1, p, p, None, p, size, None) == E.YGG_E_ARG
     for field, value in (("pages", None), ("page_count", 0), ("page_count", 1 << 31), ("page_bytes", 0), ("table", None),
-                         ("streams", 0), ("per_stream", 0), ("length", None), ("refs", None), ("status", None)):
+                         ("streams", 0), ("per_stream", 0), ("length", None), ("refs", None), ("status", None),
+                         ("sync", None)):
         c = good()
         setattr(c, field, value)
         assert lib.ygg_cache_free(0, ctypes.byref(c), 1, p, None) == E.YGG_E_ARG

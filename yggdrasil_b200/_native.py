@@ -33,7 +33,7 @@ class YggInfo(ctypes.Structure):
 class YggCache(ctypes.Structure):
     _fields_ = [("pages", ctypes.c_void_p), ("page_count", ctypes.c_int64), ("page_bytes", ctypes.c_int64),
                 ("table", ctypes.c_void_p), ("streams", ctypes.c_int64), ("per_stream", ctypes.c_int32),
-                ("length", ctypes.c_void_p), ("refs", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+                ("length", ctypes.c_void_p), ("refs", ctypes.c_void_p), ("status", ctypes.c_void_p), ("sync", ctypes.c_void_p)]
 
 
 class YggError(RuntimeError):

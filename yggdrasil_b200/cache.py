@@ -29,16 +29,21 @@ from .inference import _raw_stream
 from .logprobs import _nothing
 
 _SLOTS = 1024
-_status: list = [None, _SLOTS]   # pinned words not handed out yet, and how many were
+_slots: dict = {}   # device index -> [status words, sync words, how many of them are handed out]
 
 
-def _status_words():
-    """Two zeroed int32 words that the device can write: pinned host memory, each handed out once."""
-    if _status[1] >= _SLOTS:
-        _status[:] = [torch.zeros((_SLOTS, 2), dtype=torch.int32).pin_memory(), 0]
-    words = _status[0][_status[1]]
-    _status[1] += 1
-    return words
+def _words(index):
+    """A cache's own words, each handed out once: three of status (pinned host memory, which the device can write) and
+    two for its blocks' barriers (device memory), all zero."""
+    got = _slots.get(index)
+    if got is None or got[2] == _SLOTS:
+        got = [torch.zeros((_SLOTS, 4), dtype=torch.int32).pin_memory(),
+               torch.zeros((_SLOTS, 2), dtype=torch.int32, device=torch.device("cuda", index)), 0]
+        torch.cuda.current_stream(index).synchronize()   # zero for a cache on any stream
+        _slots[index] = got
+    status, sync, at = got
+    got[2] = at + 1
+    return status, sync, at
 
 
 class StateCache:
@@ -57,10 +62,10 @@ class StateCache:
                 raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {pages.device}")
         self.pages, self.table, self.length, self.refs = pages, table, length, refs
         self.device = pages.device
-        self._words = _status_words()
-        self._page_bytes = pages.numel() // count * pages.element_size()
-        self._c = YggCache(pages.data_ptr(), count, self._page_bytes, table.data_ptr(), streams, m, length.data_ptr(),
-                           refs.data_ptr(), self._words.data_ptr())
+        self._status, self._sync, self._at = _words(pages.device.index)
+        self._c = YggCache(pages.data_ptr(), count, pages.numel() // count * pages.element_size(), table.data_ptr(),
+                           streams, m, length.data_ptr(), refs.data_ptr(), self._status.data_ptr() + 16 * self._at,
+                           self._sync.data_ptr() + 8 * self._at)
         self._ref = ctypes.byref(self._c)
 
     @classmethod
@@ -174,9 +179,12 @@ class StateCache:
         """Raise if a call since the last clear met a bad index (ValueError) or had no page or table entry left
         (RuntimeError); what such a call could do it did. Waits for the current stream."""
         torch.cuda.current_stream(self.device).synchronize()
-        bad, full = self._words.tolist()
+        words = self._status[self._at]
+        bad, full, late, _ = words.tolist()
         if clear:
-            self._words.zero_()
+            words.zero_()
+        if late:
+            raise _native.YggError(_native.YGG_E_TIMEOUT, "StateCache: not to be used any more")
         if bad:
             raise ValueError("a stream or page was out of range, or a child held pages or was named twice")
         if full:

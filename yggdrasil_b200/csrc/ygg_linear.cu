@@ -166,23 +166,18 @@ template <typename T> __global__ void __launch_bounds__(256) quantize_any_kernel
     }
 }
 
-#ifndef WV
-#define WV 512
-#endif
-constexpr int kWarpVecs = WV;
 template <typename T> void launch_quantize(const Quantize &p, cudaStream_t st) {
     constexpr int N = kPer<T>;
     const bool even = ((uintptr_t)p.x & 15) == 0 && (p.rows == 1 || p.stride % N == 0);
     const int vecs = (p.k + N - 1) / N;
     if (!even || vecs > 2048 || p.rows > INT32_MAX) {
         quantize_any_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 8 * sm_count()), 256, 0, st>>>(p);
-    } else if (vecs <= kWarpVecs && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
+    } else if (vecs <= 256 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
         const unsigned grid = (unsigned)((p.rows + 7) / 8);
         if (vecs <= 32) quantize_kernel<T, 32, 1><<<grid, 256, 0, st>>>(p);
         else if (vecs <= 64) quantize_kernel<T, 32, 2><<<grid, 256, 0, st>>>(p);
         else if (vecs <= 128) quantize_kernel<T, 32, 4><<<grid, 256, 0, st>>>(p);
-        else if (vecs <= 256) quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
-        else quantize_kernel<T, 32, 16><<<grid, 256, 0, st>>>(p);
+        else quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
     } else {
         const unsigned grid = (unsigned)p.rows;
         if (vecs <= 256) quantize_kernel<T, 256, 1><<<grid, 256, 0, st>>>(p);

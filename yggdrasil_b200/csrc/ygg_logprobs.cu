@@ -232,35 +232,40 @@ __device__ __forceinline__ void write_row(const Rows &p, int64_t row, const T *x
     p.lse[row] = e.m + e.ls;
     if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? INFINITY : log2f(a.s), e.empty ? 0.0f : e.ls, e.h);
 }
+__device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, int value, uint32_t index, const Ends &e) {
+    p.top_ids[row * p.top + k] = (int32_t)index;
+    p.top_logprobs[row * p.top + k] = e.logprob(unorder(value));
+}
 __device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, Key key, const Ends &e) {
-    p.top_ids[row * p.top + k] = index_of(key);
-    p.top_logprobs[row * p.top + k] = e.logprob(value_of(key));
+    write_top(p, row, k, (int)((unsigned)(key >> 32) ^ 0x80000000u), (uint32_t)index_of(key), e);
 }
 
 // The k-th largest of the lanes' values (k <= 32), a lower bound of the k-th largest entry that the lanes hold.
-__device__ __forceinline__ int kth_of_lanes(int mine, int k, int lane) {
-    int best = 0;
-    for (int i = 0; i < k; i++) {
+__device__ __forceinline__ int kth_of_lanes(int mine, int k) {
+    int best;
+    do {
         best = __reduce_max_sync(~0u, mine);
-        const unsigned who = __ballot_sync(~0u, mine == best);
-        if (lane == __ffs(who) - 1) mine = INT32_MIN;
-    }
+        const bool it = mine == best;
+        k -= __popc(__ballot_sync(~0u, it));
+        if (it) mine = INT32_MIN;
+    } while (k > 0);
     return best;
 }
 // The same over four values a lane (k <= 128): a closer bound.
-__device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k, int lane) {
+__device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k) {
     const auto order2 = [](int &x, int &y) {
         const int t = min(x, y);
         x = max(x, y);
         y = t;
     };
     order2(a, b), order2(c, d), order2(a, c), order2(b, d), order2(b, c);
-    int best = 0;
-    for (int i = 0; i < k; i++) {
+    int best;
+    do {
         best = __reduce_max_sync(~0u, a);
-        const unsigned who = __ballot_sync(~0u, a == best);
-        if (lane == __ffs(who) - 1) a = b, b = c, c = d, d = INT32_MIN;
-    }
+        const bool it = a == best;
+        k -= __popc(__ballot_sync(~0u, it));
+        if (it) a = b, b = c, c = d, d = INT32_MIN;
+    } while (k > 0);
     return best;
 }
 
@@ -298,9 +303,17 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
 // make them more than the list holds, the equal ones that come too late are left out; where entries above the bound are
 // too many, they are taken one at a time.
 constexpr int kShortWarps = 4, kCandidates = 128, kList = kCandidates + 1;   // an odd pitch: lists begin in unlike banks
-template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
+// WHOLE: rows of exactly RUNS runs, all on 16-byte boundaries.
+struct List {
+    int value[kList];        // order() of the candidates
+    uint32_t index[kList];
+    __device__ __forceinline__ void put(int at, float x, uint32_t j) { value[at] = order(x), index[at] = j; }
+    __device__ __forceinline__ void put(int at, Key k) { put(at, value_of(k), (uint32_t)index_of(k)); }
+};
+template <typename T, int RUNS, int R, bool WHOLE>
+__global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     constexpr int N = kPer<T>;
-    __shared__ Key lists[kShortWarps][R][kList];
+    __shared__ List lists[kShortWarps][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row0 = ((int64_t)blockIdx.x * kShortWarps + warp) * R;
     if (row0 >= p.rows) return;
@@ -311,12 +324,15 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
     for (int w = 0; w < R; w++) {
         const int64_t row = min(row0 + w, p.rows - 1);   // rows past the last are the last once more, unseen
         const T *x = (const T *)p.logits + row * p.stride;
-        const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
+        const uint32_t off = WHOLE ? 0 : offset_of(x), end = WHOLE ? RUNS * 32 * N : (uint32_t)p.vocab + off;
         const T *from = x - off;
         float v[RUNS][N];
         float most = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < RUNS; r++) load_run<T>(from, r * 32 * N, off, end, lane, v[r]);
+        for (int r = 0; r < RUNS; r++) {
+            if (WHOLE) unpack(load_stream(x + (r * 32 + lane) * N), v[r], T());
+            else load_run<T>(from, r * 32 * N, off, end, lane, v[r]);
+        }
 #pragma unroll
         for (int r = 0; r < RUNS; r++)
 #pragma unroll
@@ -327,12 +343,12 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
         ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
         found[w] = 0;
         if (p.top == 0) continue;
-        Key *list = lists[warp][w];
+        List &list = lists[warp][w];
         int n;
         {
             int kth;
             if (p.top <= 8) {
-                kth = kth_of_lanes(mine, p.top, lane);
+                kth = kth_of_lanes(mine, p.top);
             } else {
                 float bin[4];
 #pragma unroll
@@ -342,7 +358,7 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
 #pragma unroll
                     for (int i = 0; i < N; i++)
                         if (r || i >= 4) bin[i & 3] = fmaxf(bin[i & 3], v[r][i]);
-                kth = kth_of_lanes(order(bin[0]), order(bin[1]), order(bin[2]), order(bin[3]), p.top, lane);
+                kth = kth_of_lanes(order(bin[0]), order(bin[1]), order(bin[2]), order(bin[3]), p.top);
             }
             const float bound = unorder(kth);
             unsigned in = 0;
@@ -357,7 +373,7 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
 #pragma unroll
                     for (int i = 0; i < N; i++) {
                         const uint32_t u = (r * 32 + lane) * N + i;
-                        if (u < off || u >= end) in &= ~(1u << (r * N + i));
+                        if (u - off >= end - off) in &= ~(1u << (r * N + i));
                     }
                 if (RUNS * N < 32) in &= (1u << (RUNS * N & 31)) - 1;
             }
@@ -367,7 +383,7 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
                 for (int done = 0; (who = __ballot_sync(~0u, in != 0)) != 0; done += __popc(who)) {
                     if (in) {
                         const int bit = __ffs(in) - 1, u = (bit / N * 32 + lane) * N + bit % N;
-                        list[done + __popc(who & below)] = key_of(to_f(from[u]), u - off);
+                        list.put(done + __popc(who & below), to_f(from[u]), u - off);
                         in &= in - 1;
                     }
                 }
@@ -380,7 +396,7 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
                         const bool more = v[r][i] > bound;
                         const unsigned who = __ballot_sync(~0u, more);
                         const int at = n + __popc(who & below);
-                        if (more && at < kCandidates) list[at] = key_of(v[r][i], (r * 32 + lane) * N + i - off);
+                        if (more && at < kCandidates) list.put(at, v[r][i], (r * 32 + lane) * N + i - off);
                         n += __popc(who);
                     }
                 // in the order of their indices: a lane's entries of a run lie side by side
@@ -403,7 +419,7 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
 #pragma unroll
                     for (int i = 0; i < N; i++)
                         if (equal >> (r * N + i) & 1) {
-                            if (at < p.top) list[at] = key_of(v[r][i], (r * 32 + lane) * N + i - off);
+                            if (at < p.top) list.put(at, v[r][i], (r * 32 + lane) * N + i - off);
                             at++;
                         }
                     n = min(p.top, n + __shfl_sync(~0u, upto, 31));
@@ -419,11 +435,11 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
 #pragma unroll
                     for (int i = 0; i < N; i++) {
                         const uint32_t u = (r * 32 + lane) * N + i;
-                        const Key key = u >= off && u < end ? key_of(v[r][i], u - off) : 0;
+                        const Key key = u - off < end - off ? key_of(v[r][i], u - off) : 0;
                         if (key < last && key > best) best = key;
                     }
                 last = warp_max(best);
-                if (lane == 0) list[k] = last;
+                if (lane == 0) list.put(k, last);
             }
             n = p.top;
         }
@@ -461,12 +477,27 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
     if (row >= p.rows) n = 0;
     if (lane < R && row < p.rows) write_row(p, row, (const T *)p.logits + row * p.stride, a, e);
     __syncwarp();
-    const Key *list = lists[warp][mine];
+    if (p.top == 0) return;
+    // ranks by the values alone; ties give ranks twice, which shows in the ranks' sum, and then the indices count too
+    const List &list = lists[warp][mine];
+    int wrong = 0;
     for (int slot = lane / R; slot < most; slot += 32 / R) {
-        const Key key = slot < n ? list[slot] : ~0ull;
+        if (slot >= n) continue;
+        const int value = list.value[slot];
         int above = 0;
-        for (int i = 0; i < n; i++) above += list[i] > key;
-        if (slot < n && above < p.top) write_top(p, row, above, key, e);
+        for (int i = 0; i < n; i++) above += list.value[i] > value;
+        wrong += slot - above;   // a row's slots and ranks have one sum
+        if (above < p.top) write_top(p, row, above, value, list.index[slot], e);
+    }
+    // (the rows' sums are looked at together: ranks are never above the true ones, so that no row makes up for another)
+    if (__reduce_add_sync(~0u, wrong) == 0) return;
+    for (int slot = lane / R; slot < n; slot += 32 / R) {
+        const int value = list.value[slot];
+        const uint32_t index = list.index[slot];
+        int above = 0;
+        for (int i = 0; i < n; i++)
+            above += list.value[i] > value || (list.value[i] == value && list.index[i] < index);
+        if (above < p.top) write_top(p, row, above, value, index, e);
     }
 }
 
@@ -477,10 +508,14 @@ template <typename T, int RUNS, int R> __global__ void __launch_bounds__(kShortW
 // k-th segment's largest value are ranked by counting. If they are more than a block has threads (ties, masks, sorted
 // rows), a second bound from the threads' best entries leaves fewer; if those are still more, they are taken one at a
 // time.
+// AHEAD: a warp's next batch is loaded while one is added up. Rows that share an SM hide their loads behind each other, and
+// the registers cost a block an SM (8192 x 32768 bf16: 124 us without, 136 with); few rows wait for each load in turn
+// (7 x 100003 bf16: 12.8 us without, 9.5 with).
 constexpr int kLongThreads = 256, kLongWarps = kLongThreads / 32, kMaxSegments = 4096, kMaxCluster = 8, kBatch = 4;
 
 struct LongShared {
     Sums part[kMaxCluster * kLongWarps];   // in the first block
+    Sums all;
     int picked[YGG_TOP_MAX];               // segments
     Key keys[kLongThreads];
     Key best[kLongWarps];
@@ -497,7 +532,7 @@ __device__ __forceinline__ void put_remote(uint32_t at, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-template <typename T>
+template <typename T, bool AHEAD>
 __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cluster, int shift, int segments) {
     constexpr int N = kPer<T>;
     extern __shared__ __align__(16) uint8_t raw[];
@@ -512,24 +547,29 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     Sums a = none();
     const int w = rank * kLongWarps + warp, warps = cluster * kLongWarps;
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
-    const int steps = shift ? 1 << (shift - 2) : 1;
-    for (int g0 = w * (shift ? 1 : kBatch); g0 < segments; g0 += warps * (shift ? 1 : kBatch)) {
+    const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
+    const auto load = [&](uint4(&q)[kBatch], uint32_t u0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
+    };
+    uint4 q[kBatch];
+    if (AHEAD && w * per < segments) load(q, w * per * span);
+    for (int g0 = w * per; g0 < segments; g0 += warps * per) {
         float top_of[kBatch];
         for (int step = 0; step < steps; step++) {
-            uint4 q[kBatch];
             float v[kBatch][N], most = -INFINITY;
-            const uint32_t u0 = g0 * span + step * kBatch * 32 * N;
-#pragma unroll
-            for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
+            if (!AHEAD) load(q, g0 * span + step * kBatch * 32 * N);
 #pragma unroll
             for (int b = 0; b < kBatch; b++) {
                 const float t = largest(q[b], T());
                 top_of[b] = shift && step ? fmaxf(top_of[b], t) : t;
                 most = fmaxf(most, t);
+                unpack(q[b], v[b], T());
             }
+            const bool on = step + 1 < steps;
+            if (AHEAD && (on || g0 + warps * per < segments))
+                load(q, (on ? g0 : g0 + warps * per) * span + (on ? step + 1 : 0) * kBatch * 32 * N);
             if (most > a.m) raise(a, most);
-#pragma unroll
-            for (int b = 0; b < kBatch; b++) unpack(q[b], v[b], T());
             add_entries(a, v);
         }
         if (p.top) {
@@ -560,7 +600,6 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
                 put_remote(at + 8, __float_as_uint(a.t));
             }
             if (p.top) {   // the warp's own segments
-                const int per = shift ? 1 : kBatch;
                 __syncwarp();
                 for (int g0 = w * per; g0 < segments; g0 += warps * per)
                     if (lane < per && g0 + lane < segments)
@@ -571,10 +610,17 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         if (rank) return;
     }
     __syncthreads();
-    a = sh.part[0];
-    for (int i = 1; i < warps; i++) join(a, sh.part[i]);
-    const Ends e(a);
-    if (threadIdx.x == 0) write_row(p, row, x, a, e);
+    if (warp == 1) {   // the sums, while the first warp looks for the best segments
+        a = lane < warps ? sh.part[lane] : none();
+        if (lane + 32 < warps) join(a, sh.part[lane + 32]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            join(a, Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)});
+        if (lane == 0) {
+            write_row(p, row, x, a, Ends(a));
+            sh.all = a;
+        }
+    }
     if (p.top == 0) return;
 
     // the best segments, by one warp; fewer segments than alternatives: all of them
@@ -604,6 +650,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         if (lane == 0) sh.count = n;
     }
     __syncthreads();
+    const Ends e(sh.all);
     const int found = sh.count;
     if (found <= kLongThreads) {
         const Key key = threadIdx.x < found ? sh.keys[threadIdx.x] : 0;
@@ -646,7 +693,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const uint32_t u = u0 + lane * N + i;
-            if (!(v[i] < bound) && u >= off && u < end) {
+            if (!(v[i] < bound) && u - off < end - off) {
                 const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
                 if (at < kLongThreads) sh.keys[at] = key_of(v[i], u - off);
             }
@@ -665,7 +712,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const uint32_t u = u0 + lane * N + i;
-                if (u >= off && u < end) mine = max(mine, key_of(v[i], u - off));
+                if (u - off < end - off) mine = max(mine, key_of(v[i], u - off));
             }
         }
         __syncthreads();
@@ -685,7 +732,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const uint32_t u = u0 + lane * N + i;
-                const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
+                const Key key = u - off < end - off ? key_of(v[i], u - off) : 0;
                 if (key && key >= least) {
                     const int at = atomicAdd(&sh.count, 1);
                     if (at < kLongThreads) sh.keys[at] = key;
@@ -712,7 +759,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const uint32_t u = u0 + lane * N + i;
-                const Key key = u >= off && u < end ? key_of(v[i], u - off) : 0;
+                const Key key = u - off < end - off ? key_of(v[i], u - off) : 0;
                 if (key < last && key > best) best = key;
             }
         }
@@ -734,12 +781,13 @@ int cluster_for(int64_t rows, int64_t runs, int sms) {
 }
 
 // Four rows a warp as soon as they fill the SMs.
-template <typename T, int RUNS> void launch_short(const Rows &p, cudaStream_t st) {
-    const bool many = p.rows >= (int64_t)sm_count() * 64;
+template <typename T, int RUNS> void launch_short(const Rows &p, bool even, cudaStream_t st) {
+    const bool many = p.rows >= (int64_t)sm_count() * 64, whole = even && p.vocab == RUNS * 32 * kPer<T>;
     const int64_t per = kShortWarps * (many ? 4 : 1);
     const unsigned grid = (unsigned)((p.rows + per - 1) / per);
-    if (many) short_kernel<T, RUNS, 4><<<grid, kShortWarps * 32, 0, st>>>(p);
-    else short_kernel<T, RUNS, 1><<<grid, kShortWarps * 32, 0, st>>>(p);
+    if (!many) short_kernel<T, RUNS, 1, false><<<grid, kShortWarps * 32, 0, st>>>(p);
+    else if (whole) short_kernel<T, RUNS, 4, true><<<grid, kShortWarps * 32, 0, st>>>(p);
+    else short_kernel<T, RUNS, 4, false><<<grid, kShortWarps * 32, 0, st>>>(p);
 }
 
 template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
@@ -751,9 +799,10 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
         return cudaGetLastError();
     }
     if (runs <= 32 / N) {   // at most 32 places a lane
-        if (runs <= 1) launch_short<T, 1>(p, st);
-        else if (runs <= 2) launch_short<T, 2>(p, st);
-        else launch_short<T, 32 / N>(p, st);
+        if (runs <= 1) launch_short<T, 1>(p, even, st);
+        else if (runs <= 2) launch_short<T, 2>(p, even, st);
+        else if (runs <= 4) launch_short<T, 4>(p, even, st);
+        else launch_short<T, 32 / N>(p, even, st);
         return cudaGetLastError();
     }
     int shift = 0;
@@ -771,7 +820,8 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1;
-    return cudaLaunchKernelEx(&cfg, long_kernel<T>, p, cluster, shift, segments);
+    return cluster > 1 ? cudaLaunchKernelEx(&cfg, long_kernel<T, true>, p, cluster, shift, segments)
+                       : cudaLaunchKernelEx(&cfg, long_kernel<T, false>, p, cluster, shift, segments);
 }
 
 // What the gradient of a row needs: p (A + B y) everywhere, p = 2^(y log2 e - log2 s), and more at the given token and

@@ -25,7 +25,7 @@ namespace {
 
 using namespace ygg;
 
-enum : int { kBadIndex = 0, kNoRoom = 1 };   // the words of Cache::status
+enum : int { kBadIndex = 0, kNoRoom = 1, kTimeout = 2 };   // the words of Cache::status
 
 struct Cache {
     char *pages;
@@ -34,7 +34,8 @@ struct Cache {
     int64_t streams;
     int per_stream;
     int32_t *length, *refs;
-    int32_t *status;             // two words, set to 1 by plain stores: they may lie in mapped host memory
+    int32_t *status;             // three words, set to 1 by plain stores: they may lie in mapped host memory
+    unsigned *sync;              // two words of device memory: blocks that have arrived, barriers passed
 };
 
 // One page copy: source page (or none: zeros), destination page (or none: nothing to do).
@@ -42,7 +43,42 @@ struct Move { int32_t from, to; };
 
 __device__ __forceinline__ void report(int32_t *status, int what) { *(volatile int32_t *)(status + what) = 1; }
 
-constexpr int kPlan = 1024;
+constexpr int kPlan = 1024, kWarps = kPlan / 32, kMaxBlocks = 256;
+
+__device__ __forceinline__ unsigned acquire(const unsigned *p) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
+// All blocks of a cooperative launch. The count is back at 0 when it is done, so that the words serve the cache's next call.
+// The wait is bounded (false: it ran out, and the cache is reported as unusable).
+__device__ __forceinline__ bool all_blocks(const Cache &c) {
+    __shared__ int fine;
+    __syncthreads();
+    if (gridDim.x == 1) return true;
+    if (threadIdx.x == 0) {
+        fine = 1;
+        __threadfence();
+        const unsigned now = acquire(c.sync + 1);
+        if (atomicAdd(c.sync, 1u) == gridDim.x - 1) {
+            *(volatile unsigned *)c.sync = 0;
+            __threadfence();
+            atomicAdd(c.sync + 1, 1u);
+        } else {
+            const long long t0 = clock64();
+            while (acquire(c.sync + 1) == now)
+                if (clock64() - t0 > 2000000000LL) {
+                    fine = 0;
+                    report(c.status, kTimeout);
+                    break;
+                }
+        }
+        __threadfence();
+    }
+    __syncthreads();
+    return fine;
+}
 
 // Exclusive prefix sum over the block's threads of v; `total` receives the sum.
 __device__ __forceinline__ int block_scan(int v, int *scratch, int &total) {
@@ -56,13 +92,47 @@ __device__ __forceinline__ int block_scan(int v, int *scratch, int &total) {
     __syncthreads();
     if (lane == 31) scratch[warp] = x;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int w = 0; w < kPlan / 32; w++) {
-        if (w == warp) before = total;
-        total += scratch[w];
+    int w = scratch[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, w, o);
+        if (lane >= o) w += y;
     }
-    return before + x - v;
+    total = __shfl_sync(~0u, w, 31);
+    return x - v + (warp ? __shfl_sync(~0u, w, warp - 1) : 0);
+}
+// How many of the block's threads have it set, and how many before this one.
+__device__ __forceinline__ int block_count(bool v, int *scratch, int &before) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned who = __ballot_sync(~0u, v);
+    __syncthreads();
+    if (lane == 0) scratch[warp] = __popc(who);
+    __syncthreads();
+    int w = scratch[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, w, o);
+        if (lane >= o) w += y;
+    }
+    before = __popc(who & ((1u << lane) - 1)) + (warp ? __shfl_sync(~0u, w, warp - 1) : 0);
+    return __shfl_sync(~0u, w, 31);
+}
+// The sum of the blocks' counts, and of those before this block. Counts come from other blocks: past the L1.
+__device__ __forceinline__ int over_blocks(const int *counts, int *scratch, int &before) {
+    int total;
+    const int mine = threadIdx.x < gridDim.x ? __ldcg(counts + threadIdx.x) : 0;
+    const int at = block_scan(mine, scratch, total);
+    __shared__ int here;
+    if (threadIdx.x == blockIdx.x) here = at;
+    __syncthreads();
+    before = here;
+    return total;
+}
+
+// The block's share of n things, side by side.
+struct Range { int64_t from, to; };
+__device__ __forceinline__ Range share(int64_t n) {
+    return {n * blockIdx.x / gridDim.x, n * (blockIdx.x + 1) / gridDim.x};
 }
 
 __device__ __forceinline__ int length_of(const Cache &c, int64_t s) {
@@ -70,118 +140,145 @@ __device__ __forceinline__ int length_of(const Cache &c, int64_t s) {
 }
 __device__ __forceinline__ bool is_page(const Cache &c, int p) { return p >= 0 && p < c.count; }
 
-// What a grow or a fork does, before room is looked for: the pages taken over and whether it can be done at all.
-struct Wish { int64_t parent, child; int taken; bool ok; };
-
-__device__ __forceinline__ Wish wish(const Cache &c, const int32_t *parents, const int32_t *children,
-                                     const int32_t *depth, int64_t i) {
-    Wish w{parents[i], children ? children[i] : parents[i], 0, false};
-    if (w.parent < 0 || w.child < 0) return w;
-    if (w.parent >= c.streams || w.child >= c.streams) {
-        report(c.status, kBadIndex);
-        return w;
+// Whole pages in units of V, `n` of them from the i-th thread of `all` on; move(i) says which.
+template <typename V, typename F>
+__device__ __forceinline__ void copy_moves(const Cache &c, int64_t n, int64_t thread, int64_t all, F move) {
+    const int64_t units = c.page_bytes / (int64_t)sizeof(V), total = n * units;
+    const bool narrow = total + 4 * all < ((int64_t)1 << 32);
+    for (int64_t u0 = thread; u0 < total; u0 += 4 * all) {
+        V v[4];
+        char *to[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t u = u0 + k * all;
+            to[k] = nullptr;
+            v[k] = V{};
+            if (u >= total) continue;
+            const int64_t i = narrow ? (uint32_t)u / (uint32_t)units : u / units, at = (u - i * units) * sizeof(V);
+            const Move m = move(i);
+            if (m.to < 0 || m.to >= c.count || m.from >= c.count) continue;
+            to[k] = c.pages + m.to * c.page_bytes + at;
+            if (m.from >= 0) v[k] = *(const V *)(c.pages + m.from * c.page_bytes + at);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (to[k]) *(V *)to[k] = v[k];
     }
-    const int n = length_of(c, w.parent);
-    if (!children) {
-        w.taken = n;
-        w.ok = true;
-        return w;
-    }
-    w.taken = depth ? min(depth[i], n) : n;
-    if (w.taken <= 0) return w;   // an empty parent: the child stays empty
-    w.ok = true;
-    return w;
 }
 
 constexpr int32_t kClaim = INT32_MIN;
 
-// fork: the first of a child's forks claims it by the smallest index in its (empty) table row, -1 before.
-// grow: likewise in the slot after its last page.
-__device__ __forceinline__ int32_t *claim_slot(const Cache &c, const Wish &w, bool grow) {
-    return c.table + w.child * c.per_stream + (grow ? w.taken : 0);
-}
-
-__global__ void __launch_bounds__(kPlan) plan_kernel(const Cache c, const int32_t *parents, const int32_t *children,
-                                                     const int32_t *depth, int64_t n, int32_t *order, Move *moves) {
-    __shared__ int scratch[kPlan / 32];
-    __shared__ int found;
+// grow and fork, in three parts between barriers:
+//   claims: a fork claims its (empty) child by the smallest index of the list in the child's first table entry, a grow its
+//           stream in the entry after its last page (-1 before); the blocks count the free pages of their shares
+//   order:  the free pages in ascending order, as many as may be wanted; the blocks count the claims that held
+//   pages:  the k-th claim that held takes the k-th free page; table rows, counts, and the page's copy
+// info[i]: the pages that entry i takes over, or -1: nothing to do.
+template <typename V>
+__global__ void __launch_bounds__(kPlan, 1)
+    fork_kernel(const Cache c, const int32_t *parents, const int32_t *children, const int32_t *depth, int64_t n,
+                int32_t *info, int32_t *order, Move *moves, int *counts) {
+    __shared__ int scratch[kWarps];
     const bool grow = children == nullptr;
-    int total;
-    // the free pages in ascending order, as many as may be wanted
-    int free_before = 0;
-    for (int64_t p0 = 0; p0 < c.count && free_before < n; p0 += kPlan) {
+    const Range mine = share(n), pages = share(c.count);
+    int *const free_counts = counts, *const held_counts = counts + kMaxBlocks;
+    const auto slot = [&](int64_t child, int taken) { return c.table + child * c.per_stream + (grow ? taken : 0); };
+    const auto child_of = [&](int64_t i) { return grow ? parents[i] : children[i]; };
+
+    for (int64_t i = mine.from + threadIdx.x; i < mine.to; i += kPlan) {
+        const int64_t parent = parents[i], child = child_of(i);
+        int taken = -1;
+        if (parent >= 0 && child >= 0) {
+            if (parent >= c.streams || child >= c.streams) {
+                report(c.status, kBadIndex);
+            } else {
+                const int held = length_of(c, parent);
+                if (grow) {
+                    taken = held;
+                    if (held >= c.per_stream) {
+                        report(c.status, kNoRoom);
+                        taken = -1;
+                    }
+                } else {
+                    taken = depth ? min(depth[i], held) : held;
+                    if (taken <= 0) {   // a parent without pages: a child without
+                        taken = -1;
+                    } else if (length_of(c, child) != 0) {
+                        report(c.status, kBadIndex);
+                        taken = -1;
+                    }
+                }
+            }
+        }
+        info[i] = taken;
+        if (taken >= 0) atomicMin(slot(child, taken), kClaim + (int32_t)i);
+    }
+    int free_here = 0, before;
+    for (int64_t p0 = pages.from; p0 < pages.to; p0 += kPlan) {
         const int64_t p = p0 + threadIdx.x;
-        const bool is_free = p < c.count && c.refs[p] == 0;
-        const int at = free_before + block_scan(is_free, scratch, total);
-        if (is_free && at < n) order[at] = (int32_t)p;
-        free_before += total;
+        free_here += __syncthreads_count(p < pages.to && c.refs[p] == 0);
     }
-    const int available = (int)min((int64_t)free_before, n);
-    if (threadIdx.x == 0) found = available;
-    // claims
-    for (int64_t i = threadIdx.x; i < n; i += kPlan) {
-        const Wish w = wish(c, parents, children, depth, i);
-        if (!w.ok) continue;
-        if (grow ? w.taken >= c.per_stream : length_of(c, w.child) != 0) {
-            report(c.status, grow ? kNoRoom : kBadIndex);
-            continue;
-        }
-        atomicMin(claim_slot(c, w, grow), kClaim + (int32_t)i);
+    if (threadIdx.x == 0) free_counts[blockIdx.x] = free_here;
+    if (!all_blocks(c)) return;
+
+    int free_before;
+    const int available = over_blocks(free_counts, scratch, free_before);
+    for (int64_t p0 = pages.from; p0 < pages.to && free_before < n; p0 += kPlan) {
+        const int64_t p = p0 + threadIdx.x;
+        const bool is_free = p < pages.to && c.refs[p] == 0;
+        const int here = block_count(is_free, scratch, before);
+        if (is_free && free_before + before < n) order[free_before + before] = (int32_t)p;
+        free_before += here;
     }
-    __syncthreads();
-    // pages in the order of the list
-    int given = 0;
-    for (int64_t i0 = 0; i0 < n; i0 += kPlan) {
+    int held = 0;
+    for (int64_t i0 = mine.from; i0 < mine.to; i0 += kPlan) {
         const int64_t i = i0 + threadIdx.x;
-        Wish w{};
-        bool mine = false;
-        if (i < n) {
-            w = wish(c, parents, children, depth, i);
-            if (w.ok && !(grow ? w.taken >= c.per_stream : length_of(c, w.child) != 0)) {
-                mine = *(volatile int32_t *)claim_slot(c, w, grow) == kClaim + (int32_t)i;
-                if (!mine) report(c.status, kBadIndex);   // named twice
+        bool holds = false;
+        if (i < mine.to && info[i] >= 0) {
+            holds = __ldcg(slot(child_of(i), info[i])) == kClaim + (int32_t)i;
+            if (!holds) {   // named twice
+                report(c.status, kBadIndex);
+                info[i] = -1;
             }
         }
-        const int at = given + block_scan(mine, scratch, total);
-        given += total;
-        if (i < n) {
-            Move m{-1, -1};
-            if (mine && at < found) {
-                m.to = order[at];
-                m.from = w.taken > 0 ? c.table[w.parent * c.per_stream + w.taken - 1] : -1;
-            } else if (mine) {
+        held += __syncthreads_count(holds);
+    }
+    if (threadIdx.x == 0) held_counts[blockIdx.x] = held;
+    if (!all_blocks(c)) return;
+
+    int given;
+    over_blocks(held_counts, scratch, given);
+    for (int64_t i0 = mine.from; i0 < mine.to; i0 += kPlan) {
+        const int64_t i = i0 + threadIdx.x;
+        const int taken = i < mine.to ? info[i] : -1;
+        const int here = block_count(taken >= 0, scratch, before);
+        Move m{-1, -1};
+        if (taken >= 0) {
+            const int64_t child = child_of(i);
+            int32_t *row = c.table + child * c.per_stream;
+            if (given + before < available) {
+                const int32_t *from = c.table + parents[i] * (int64_t)c.per_stream;
+                m.to = __ldcg(order + given + before);
+                m.from = taken > 0 ? from[taken - 1] : -1;
+                if (!grow)
+                    for (int j = 0; j < taken - 1; j++) {
+                        row[j] = from[j];
+                        if (is_page(c, from[j])) atomicAdd(&c.refs[from[j]], 1);
+                    }
+                row[grow ? taken : taken - 1] = m.to;
+                c.refs[m.to] = 1;
+                c.length[child] = grow ? taken + 1 : taken;
+            } else {   // the claim is taken back
                 report(c.status, kNoRoom);
+                *slot(child, taken) = -1;
             }
-            moves[i] = m;
         }
+        if (i < mine.to) moves[i] = m;
+        given += here;
     }
     __syncthreads();
-    // the claims that got no page are taken back; the others become table rows
-    for (int64_t i = threadIdx.x; i < n; i += kPlan) {
-        const Move m = moves[i];
-        const int64_t child = children ? children[i] : parents[i], parent = parents[i];
-        if (child < 0 || parent < 0 || child >= c.streams || parent >= c.streams) continue;
-        int32_t *row = c.table + child * c.per_stream;
-        if (m.to < 0) {
-            const Wish w = wish(c, parents, children, depth, i);
-            if (w.ok && (grow ? w.taken < c.per_stream : true)) {
-                int32_t *slot = claim_slot(c, w, grow);
-                if (*slot == kClaim + (int32_t)i) *slot = -1;
-            }
-            continue;
-        }
-        const Wish w = wish(c, parents, children, depth, i);
-        if (!grow) {
-            const int32_t *from = c.table + parent * c.per_stream;
-            for (int j = 0; j < w.taken - 1; j++) {
-                row[j] = from[j];
-                if (is_page(c, from[j])) atomicAdd(&c.refs[from[j]], 1);
-            }
-        }
-        row[grow ? w.taken : w.taken - 1] = m.to;
-        c.refs[m.to] = 1;
-        c.length[child] = grow ? w.taken + 1 : w.taken;
-    }
+    const Move *own = moves + mine.from;
+    copy_moves<V>(c, mine.to - mine.from, threadIdx.x, kPlan, [&](int64_t i) { return own[i]; });
 }
 
 __global__ void __launch_bounds__(256) free_kernel(const Cache c, const int32_t *streams, int64_t n) {
@@ -201,48 +298,56 @@ __global__ void __launch_bounds__(256) free_kernel(const Cache c, const int32_t 
     }
 }
 
-// compact: the moves, and renumber[p] for each page.
-__global__ void __launch_bounds__(kPlan) compact_plan_kernel(const Cache c, int32_t *live, int32_t *moved,
-                                                             int32_t *renumber, Move *moves) {
-    __shared__ int scratch[kPlan / 32];
-    int total, n = 0;
-    for (int64_t p0 = 0; p0 < c.count; p0 += kPlan) {
+// compact, in three parts between barriers. rank(p): the live pages before p.
+//   count:  the live pages of the blocks' shares, n in all
+//   lists:  holes[k], the k-th free page below n (k = p - rank(p)); movers[rank(p)] = p and ranks[p] = rank(p) for the live
+//           pages at or above n, whose k is rank(p) less the live pages below n
+//   moves:  tables, counts and pages
+template <typename V>
+__global__ void __launch_bounds__(kPlan, 1)
+    compact_kernel(const Cache c, int32_t *live, int32_t *holes, int32_t *movers, int32_t *ranks, int *counts) {
+    __shared__ int scratch[kWarps];
+    const Range pages = share(c.count);
+    int here = 0, before, rank0;
+    for (int64_t p0 = pages.from; p0 < pages.to; p0 += kPlan) {
         const int64_t p = p0 + threadIdx.x;
-        block_scan(p < c.count && c.refs[p] > 0, scratch, total);
-        n += total;
+        here += __syncthreads_count(p < pages.to && c.refs[p] > 0);
     }
-    int holes = 0, movers = 0;
-    for (int64_t p0 = 0; p0 < c.count; p0 += kPlan) {
-        const int64_t p = p0 + threadIdx.x;
-        const bool used = p < c.count && c.refs[p] > 0;
-        const bool hole = p < n && !used, mover = p >= n && used;
-        int at = holes + block_scan(hole, scratch, total);
-        holes += total;
-        if (hole) moves[at].to = (int32_t)p;
-        at = movers + block_scan(mover, scratch, total);
-        movers += total;
-        if (mover) moves[at].from = (int32_t)p;
-        if (p < c.count) renumber[p] = (int32_t)p;
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < movers; k += kPlan) {
-        const Move m = moves[k];
-        renumber[m.from] = m.to;
-        c.refs[m.to] = c.refs[m.from];
-        c.refs[m.from] = 0;
-    }
-    if (threadIdx.x == 0) {
-        *live = n;
-        *moved = movers;
-    }
-}
+    if (threadIdx.x == 0) counts[blockIdx.x] = here;
+    if (!all_blocks(c)) return;
 
-__global__ void __launch_bounds__(256) renumber_kernel(const Cache c, const int32_t *renumber) {
-    const int64_t n = c.streams * c.per_stream;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int32_t p = c.table[i];
-        if (is_page(c, p) && renumber[p] != p) c.table[i] = renumber[p];
+    const int n = over_blocks(counts, scratch, rank0);
+    int *const below = counts + kMaxBlocks;   // the live pages below n
+    if (threadIdx.x == 0 && n == c.count && blockIdx.x == 0) *below = n;
+    for (int64_t p0 = pages.from; p0 < pages.to; p0 += kPlan) {
+        const int64_t p = p0 + threadIdx.x;
+        const bool used = p < pages.to && c.refs[p] > 0;
+        const int count = block_count(used, scratch, before);
+        const int rank = rank0 + before;
+        if (p < pages.to) {
+            if (p == n) *below = rank;
+            if (p < n && !used) holes[p - rank] = (int32_t)p;
+            if (p >= n && used) movers[rank] = (int32_t)p, ranks[p] = rank;
+        }
+        rank0 += count;
     }
+    if (!all_blocks(c)) return;
+
+    const int low = __ldcg(below), moving = n - low;
+    const int64_t thread = (int64_t)blockIdx.x * kPlan + threadIdx.x, all = (int64_t)gridDim.x * kPlan;
+    if (thread == 0) *live = n;
+    if (moving == 0) return;
+    const int64_t entries = c.streams * c.per_stream;
+    for (int64_t i = thread; i < entries; i += all) {
+        const int32_t p = c.table[i];
+        if (p >= n && p < c.count) c.table[i] = __ldcg(holes + __ldcg(ranks + p) - low);
+    }
+    for (int64_t k = thread; k < moving; k += all) {
+        const int32_t from = __ldcg(movers + low + k), to = __ldcg(holes + k);
+        c.refs[to] = c.refs[from];
+        c.refs[from] = 0;
+    }
+    copy_moves<V>(c, moving, thread, all, [&](int64_t k) { return Move{__ldcg(movers + low + k), __ldcg(holes + k)}; });
 }
 
 // Copies of whole pages in units of V. Where from[i] and to[i] are is what Where says: pages outside their pool are
@@ -251,22 +356,15 @@ struct Where {
     const char *src;
     char *dst;
     int64_t src_count, dst_count;
-    const Move *moves;              // or
     const int32_t *src_ids, *dst_ids;   // null: page i
     const int32_t *streams, *table, *length;   // the last pages of streams, on the side that `last` names
     int64_t stream_count;
     int per_stream, last;           // 0: none, 1: source, 2: destination
-    const int32_t *n_of;            // the number of copies on the device, or null
     int64_t n;
     int32_t *status;
 };
 
 __device__ __forceinline__ bool resolve(const Where &w, int64_t i, bool first, int64_t &from, int64_t &to) {
-    if (w.moves) {
-        from = w.moves[i].from;
-        to = w.moves[i].to;
-        return to >= 0 && to < w.dst_count && from < w.src_count;   // from < 0: zeros
-    }
     from = w.src_ids ? w.src_ids[i] : i;
     to = w.dst_ids ? w.dst_ids[i] : i;
     if (w.last) {
@@ -286,7 +384,7 @@ __device__ __forceinline__ bool resolve(const Where &w, int64_t i, bool first, i
 }
 
 template <typename V> __global__ void __launch_bounds__(256) copy_kernel(const Where w, int64_t page_bytes) {
-    const int64_t units = page_bytes / sizeof(V), n = w.n_of ? *w.n_of : w.n, all = n * units;
+    const int64_t units = page_bytes / sizeof(V), all = w.n * units;
     for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < all; u += (int64_t)gridDim.x * 256) {
         const int64_t i = u / units, at = u - i * units;
         int64_t from, to;
@@ -299,20 +397,42 @@ template <typename V> __global__ void __launch_bounds__(256) copy_kernel(const W
 
 int blocks_for(int64_t threads) { return (int)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 148 * 16)); }
 
-void copy_pages(const Where &w, int64_t page_bytes, int64_t most, cudaStream_t st) {
-    const uintptr_t mix = (uintptr_t)w.src | (uintptr_t)w.dst | (uintptr_t)page_bytes;
-    if (mix % 16 == 0) copy_kernel<uint4><<<blocks_for(most * (page_bytes / 16)), 256, 0, st>>>(w, page_bytes);
-    else if (mix % 4 == 0) copy_kernel<uint32_t><<<blocks_for(most * (page_bytes / 4)), 256, 0, st>>>(w, page_bytes);
-    else copy_kernel<uint8_t><<<blocks_for(most * page_bytes), 256, 0, st>>>(w, page_bytes);
+// f of a unit that pages at `mix` (addresses and sizes, or'ed) can be copied in.
+template <typename F> auto by_unit(uintptr_t mix, F f) {
+    return mix % 16 == 0 ? f(uint4()) : mix % 4 == 0 ? f(uint32_t()) : f(uint8_t());
+}
+
+int copy_pages(const Where &w, int64_t page_bytes, cudaStream_t st) {
+    return by_unit((uintptr_t)w.src | (uintptr_t)w.dst | (uintptr_t)page_bytes, [&](auto v) {
+        using V = decltype(v);
+        copy_kernel<V><<<blocks_for(w.n * (page_bytes / (int64_t)sizeof(V))), 256, 0, st>>>(w, page_bytes);
+        return cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    });
+}
+
+// One block where its own work is short, else a block an SM that meet at barriers.
+template <typename... P, typename... A>
+int launch_plan(void (*kernel)(P...), int64_t things, int64_t bytes, cudaStream_t st, A... args) {
+    const bool small = things <= 4096 && bytes <= (128 << 10);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(small ? 1 : std::min(kMaxBlocks, sm_count()));
+    cfg.blockDim = dim3(kPlan);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = small ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 int cache_of(const ygg_cache_t *h, Cache &c) {
-    if (!h || !h->pages || !h->table || !h->length || !h->refs || !h->status || h->page_bytes < 1 || h->page_count < 1 ||
+    if (!h || !h->pages || !h->table || !h->length || !h->refs || !h->status || !h->sync || h->page_bytes < 1 || h->page_count < 1 ||
         h->page_count > INT32_MAX || h->streams < 1 || h->streams > INT32_MAX || h->per_stream < 1 ||
         h->page_bytes > ((int64_t)1 << 40))
         return YGG_E_ARG;
     c = {(char *)h->pages, h->page_count, h->page_bytes, h->table, h->streams, h->per_stream, h->length, h->refs,
-         h->status};
+         h->status, h->sync};
     return YGG_OK;
 }
 
@@ -326,8 +446,8 @@ extern "C" {
 
 size_t ygg_cache_workspace(const ygg_cache_t *h, int64_t n) {
     if (!h || n < 0 || h->page_count < 1) return 0;
-    // fork and grow: order [n], moves [n]; compact: renumber [count], moves [count]
-    return sizeof(int32_t) * (size_t)(3 * rounded(std::max(n, h->page_count)) + 4);
+    // counts; fork and grow: info [n], order [n], moves [n]; compact: holes, movers, ranks [count]
+    return sizeof(int32_t) * (2 * kMaxBlocks + 4 * (size_t)rounded(std::max(n, h->page_count)));
 }
 
 int ygg_cache_fork(int device, const ygg_cache_t *h, int64_t n, const int32_t *d_parents, const int32_t *d_children,
@@ -340,16 +460,13 @@ int ygg_cache_fork(int device, const ygg_cache_t *h, int64_t n, const int32_t *d
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
     const cudaStream_t st = (cudaStream_t)stream;
-    int32_t *order = (int32_t *)d_workspace;
+    int *counts = (int *)d_workspace;
+    int32_t *info = counts + 2 * kMaxBlocks, *order = info + rounded(n);
     Move *moves = (Move *)(order + rounded(n));
-    plan_kernel<<<1, kPlan, 0, st>>>(c, d_parents, d_children, d_depth, n, order, moves);
-    Where w{};
-    w.src = w.dst = c.pages;
-    w.src_count = w.dst_count = c.count;
-    w.moves = moves;
-    w.n = n;
-    copy_pages(w, c.page_bytes, n, st);
-    return done();
+    return by_unit((uintptr_t)c.pages | (uintptr_t)c.page_bytes, [&](auto v) {
+        return launch_plan(fork_kernel<decltype(v)>, std::max(n, c.count), n * c.page_bytes, st, c, d_parents, d_children,
+                           d_depth, n, info, order, moves, counts);
+    });
 }
 
 int ygg_cache_free(int device, const ygg_cache_t *h, int64_t n, const int32_t *d_streams, void *stream) {
@@ -372,17 +489,12 @@ int ygg_cache_compact(int device, const ygg_cache_t *h, int32_t *d_live, void *d
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
     const cudaStream_t st = (cudaStream_t)stream;
-    int32_t *counts = (int32_t *)d_workspace, *renumber = counts + 4;
-    Move *moves = (Move *)(renumber + rounded(c.count));
-    compact_plan_kernel<<<1, kPlan, 0, st>>>(c, d_live, counts, renumber, moves);
-    renumber_kernel<<<blocks_for(c.streams * c.per_stream), 256, 0, st>>>(c, renumber);
-    Where w{};
-    w.src = w.dst = c.pages;
-    w.src_count = w.dst_count = c.count;
-    w.moves = moves;
-    w.n_of = counts;
-    copy_pages(w, c.page_bytes, c.count / 2 + 1, st);
-    return done();
+    int *counts = (int *)d_workspace;
+    int32_t *holes = counts + 2 * kMaxBlocks, *movers = holes + rounded(c.count), *ranks = movers + rounded(c.count);
+    return by_unit((uintptr_t)c.pages | (uintptr_t)c.page_bytes, [&](auto v) {
+        return launch_plan(compact_kernel<decltype(v)>, std::max(c.count, c.streams * c.per_stream),
+                           c.count / 4 * c.page_bytes, st, c, d_live, holes, movers, ranks, counts);
+    });
 }
 
 int ygg_cache_read(int device, const ygg_cache_t *h, int64_t n, const int32_t *d_streams, void *d_batch, void *stream) {
@@ -392,10 +504,9 @@ int ygg_cache_read(int device, const ygg_cache_t *h, int64_t n, const int32_t *d
     if (!d_streams || !d_batch) return YGG_E_ARG;
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
-    Where w{c.pages, (char *)d_batch, c.count, n, nullptr, nullptr, nullptr, d_streams, c.table, c.length, c.streams,
-            c.per_stream, 1, nullptr, n, c.status};
-    copy_pages(w, c.page_bytes, n, (cudaStream_t)stream);
-    return done();
+    Where w{c.pages, (char *)d_batch, c.count, n, nullptr, nullptr, d_streams, c.table, c.length, c.streams, c.per_stream, 1,
+            n, c.status};
+    return copy_pages(w, c.page_bytes, (cudaStream_t)stream);
 }
 
 int ygg_cache_write(int device, const ygg_cache_t *h, int64_t n, const int32_t *d_streams, const void *d_batch,
@@ -406,10 +517,9 @@ int ygg_cache_write(int device, const ygg_cache_t *h, int64_t n, const int32_t *
     if (!d_streams || !d_batch) return YGG_E_ARG;
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
-    Where w{(const char *)d_batch, c.pages, n, c.count, nullptr, nullptr, nullptr, d_streams, c.table, c.length,
-            c.streams, c.per_stream, 2, nullptr, n, c.status};
-    copy_pages(w, c.page_bytes, n, (cudaStream_t)stream);
-    return done();
+    Where w{(const char *)d_batch, c.pages, n, c.count, nullptr, nullptr, d_streams, c.table, c.length, c.streams,
+            c.per_stream, 2, n, c.status};
+    return copy_pages(w, c.page_bytes, (cudaStream_t)stream);
 }
 
 int ygg_cache_copy(int device, const ygg_cache_t *h, int64_t n, const int32_t *d_from, const int32_t *d_to, void *stream) {
@@ -419,10 +529,8 @@ int ygg_cache_copy(int device, const ygg_cache_t *h, int64_t n, const int32_t *d
     if (!d_from || !d_to) return YGG_E_ARG;
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
-    Where w{c.pages, c.pages, c.count, c.count, nullptr, d_from, d_to, nullptr, nullptr, nullptr, 0, 0, 0, nullptr, n,
-            c.status};
-    copy_pages(w, c.page_bytes, n, (cudaStream_t)stream);
-    return done();
+    Where w{c.pages, c.pages, c.count, c.count, d_from, d_to, nullptr, nullptr, nullptr, 0, 0, 0, n, c.status};
+    return copy_pages(w, c.page_bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"
