@@ -55,14 +55,15 @@ class StateCache:
             raise ValueError("pages must be a contiguous CUDA tensor (P, ...)")
         if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.numel() == 0:
             raise ValueError("table must be an int32 tensor (streams, pages of a stream)")
-        count, (streams, m) = pages.shape[0], table.shape
-        for name, t, shape in (("table", table, (streams, m)), ("length", length, (streams,)), ("refs", refs, (count,))):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != shape \
-                    or t.device != pages.device or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {pages.device}")
+        count, (streams, m), index = pages.shape[0], table.shape, pages.get_device()
+        for t, shape in ((table, (streams, m)), (length, (streams,)), (refs, (count,))):
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != shape \
+                    or t.get_device() != index or not t.is_contiguous():
+                raise ValueError(f"table, length and refs must be contiguous int32 tensors ({streams}, {m}), "
+                                 f"({streams},) and ({count},) on {pages.device}")
         self.pages, self.table, self.length, self.refs = pages, table, length, refs
-        self.device = pages.device
-        self._status, self._sync, self._at = _words(pages.device.index)
+        self.device, self._dix, self._sizes = pages.device, index, {}
+        self._status, self._sync, self._at = _words(index)
         self._c = YggCache(pages.data_ptr(), count, pages.numel() // count * pages.element_size(), table.data_ptr(),
                            streams, m, length.data_ptr(), refs.data_ptr(), self._status.data_ptr() + 16 * self._at,
                            self._sync.data_ptr() + 8 * self._at)
@@ -86,6 +87,8 @@ class StateCache:
     def _ids(self, ids, what, limit):
         """Indices as a contiguous int32 tensor on the device; host indices are range-checked (negative: padding)."""
         if isinstance(ids, torch.Tensor) and ids.is_cuda:
+            if ids.dtype is torch.int32 and ids.dim() == 1 and ids.get_device() == self._dix and ids.is_contiguous():
+                return ids
             if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64) or ids.device != self.device:
                 raise ValueError(f"{what} must be a row of int32 or int64 on {self.device}")
             return (ids if ids.dtype == torch.int32 else ids.clamp(-1, 2 ** 31 - 1).int()).contiguous()
@@ -97,20 +100,24 @@ class StateCache:
         return torch.as_tensor(np.ascontiguousarray(host, np.int32)).to(self.device)
 
     def _on(self):
-        return torch.cuda.device(self.device) if self.device.index != torch.cuda.current_device() else _nothing
+        return _nothing if self._dix == torch.cuda.current_device() else torch.cuda.device(self._dix)
 
     def _workspace(self, n):
-        size = ops().ygg_cache_workspace(self._ref, n)
+        size = self._sizes.get(n)
+        if size is None:
+            size = self._sizes[n] = ops().ygg_cache_workspace(self._ref, n)
         return torch.empty(size, dtype=torch.uint8, device=self.device), size
 
     def _plan(self, parents, children, depth):
         with self._on():
             n = parents.shape[0]
             ws, size = self._workspace(n)
-            check(ops().ygg_cache_fork(self.device.index, self._ref, n, parents.data_ptr(),
-                                       None if children is None else children.data_ptr(),
-                                       None if depth is None else depth.data_ptr(), ws.data_ptr(), size,
-                                       _raw_stream(self.device.index)), "ygg_cache_fork")
+            code = ops().ygg_cache_fork(self._dix, self._ref, n, parents.data_ptr(),
+                                        None if children is None else children.data_ptr(),
+                                        None if depth is None else depth.data_ptr(), ws.data_ptr(), size,
+                                        _raw_stream(self._dix))
+            if code:
+                check(code, "ygg_cache_fork")
 
     def fork(self, parents, children, depth=None):
         """Stream children[i], which must hold no pages, goes on from parents[i]: it shares the parent's pages but the
@@ -132,8 +139,8 @@ class StateCache:
         """The streams let go of their pages; pages that nothing holds any more are free."""
         s = self._ids(streams, "streams", self._c.streams)
         with self._on():
-            check(ops().ygg_cache_free(self.device.index, self._ref, s.shape[0], s.data_ptr(),
-                                       _raw_stream(self.device.index)), "ygg_cache_free")
+            check(ops().ygg_cache_free(self._dix, self._ref, s.shape[0], s.data_ptr(),
+                                       _raw_stream(self._dix)), "ygg_cache_free")
 
     def compact(self):
         """Moves the live pages to the front and renumbers the tables. Returns their number as an int32 tensor () on the
@@ -141,8 +148,10 @@ class StateCache:
         with self._on():
             live = torch.empty((), dtype=torch.int32, device=self.device)
             ws, size = self._workspace(0)
-            check(ops().ygg_cache_compact(self.device.index, self._ref, live.data_ptr(), ws.data_ptr(), size,
-                                          _raw_stream(self.device.index)), "ygg_cache_compact")
+            code = ops().ygg_cache_compact(self._dix, self._ref, live.data_ptr(), ws.data_ptr(), size,
+                                           _raw_stream(self._dix))
+            if code:
+                check(code, "ygg_cache_compact")
         return live
 
     def read(self, streams):
@@ -150,8 +159,8 @@ class StateCache:
         s = self._ids(streams, "streams", self._c.streams)
         with self._on():
             batch = torch.empty((s.shape[0], *self.pages.shape[1:]), dtype=self.pages.dtype, device=self.device)
-            check(ops().ygg_cache_read(self.device.index, self._ref, s.shape[0], s.data_ptr(), batch.data_ptr(),
-                                       _raw_stream(self.device.index)), "ygg_cache_read")
+            check(ops().ygg_cache_read(self._dix, self._ref, s.shape[0], s.data_ptr(), batch.data_ptr(),
+                                       _raw_stream(self._dix)), "ygg_cache_read")
         return batch
 
     def write(self, streams, batch):
@@ -162,8 +171,8 @@ class StateCache:
             raise ValueError(f"batch must be {self.pages.dtype} {(s.shape[0], *self.pages.shape[1:])} on {self.device}")
         b = batch.contiguous()
         with self._on():
-            check(ops().ygg_cache_write(self.device.index, self._ref, s.shape[0], s.data_ptr(), b.data_ptr(),
-                                        _raw_stream(self.device.index)), "ygg_cache_write")
+            check(ops().ygg_cache_write(self._dix, self._ref, s.shape[0], s.data_ptr(), b.data_ptr(),
+                                        _raw_stream(self._dix)), "ygg_cache_write")
 
     def copy(self, source, target):
         """Page target[i] becomes a copy of page source[i]; a target is named once, and is no source of the call."""
@@ -172,8 +181,8 @@ class StateCache:
         if a.shape != b.shape:
             raise ValueError("one target for each source")
         with self._on():
-            check(ops().ygg_cache_copy(self.device.index, self._ref, a.shape[0], a.data_ptr(), b.data_ptr(),
-                                       _raw_stream(self.device.index)), "ygg_cache_copy")
+            check(ops().ygg_cache_copy(self._dix, self._ref, a.shape[0], a.data_ptr(), b.data_ptr(),
+                                       _raw_stream(self._dix)), "ygg_cache_copy")
 
     def status(self, clear=True):
         """Raise if a call since the last clear met a bad index (ValueError) or had no page or table entry left

@@ -10,6 +10,7 @@ there is no gradient.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -33,7 +34,7 @@ def _rows(x, what):
     k = x.shape[-1]
     if not 1 <= k <= MAX_K:
         raise ValueError(f"{what}: K {k}: 1 to {MAX_K}")
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and torch.is_grad_enabled():   # the weights are frozen
         raise NotImplementedError("the int8 product has no gradient: use detach() or torch.no_grad()")
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     return x2 if x2.stride(1) == 1 or k == 1 else x2.contiguous()
@@ -43,8 +44,9 @@ def _on(device):
     return torch.cuda.device(device) if device.index != torch.cuda.current_device() else _nothing
 
 
-def _aligned(t):
-    return t.stride(-1) == 1 and t.stride(-2) % 16 == 0 and t.stride(-2) >= t.shape[-1] and t.data_ptr() % 16 == 0
+def _aligned(t):   # (rows, K) bytes
+    step, one = t.stride()
+    return one == 1 and step % 16 == 0 and step >= t.shape[1] and t.data_ptr() % 16 == 0
 
 
 def quantize_rows(x):
@@ -76,51 +78,58 @@ def int8_linear(x, weight, scale, bias=None, out_dtype=None):
         if codes.dtype != torch.int8 or not codes.is_cuda or codes.dim() < 1 or row_scale.dtype != torch.float32 \
                 or row_scale.shape != codes.shape[:-1] or row_scale.device != codes.device:
             raise ValueError("QuantizedRows: int8 codes (..., K) and a float32 scale (...) on one CUDA device")
-        lead, k, device = codes.shape[:-1], codes.shape[-1], codes.device
+        lead, k, index = codes.shape[:-1], codes.shape[-1], codes.get_device()
         if not 1 <= k <= MAX_K:
             raise ValueError(f"codes: K {k}: 1 to {MAX_K}")
-        out_dtype = out_dtype or torch.float32
+        x2, out_dtype = None, out_dtype or torch.float32
     else:
         x2 = _rows(x, "x")
-        lead, k, device = x.shape[:-1], x.shape[-1], x.device
+        shape = x.shape
+        lead, k, index = shape[:-1], shape[-1], x.get_device()
         out_dtype = out_dtype or x.dtype
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype {out_dtype}: float32, float16 or bfloat16")
-    if not isinstance(weight, torch.Tensor) or weight.dtype != torch.int8 or weight.dim() != 2 or weight.shape[1] != k \
-            or weight.device != device or weight.shape[0] < 1:
-        raise ValueError(f"weight must be an int8 tensor (N, {k}) on {device}")
+    if not isinstance(weight, torch.Tensor) or weight.dtype is not torch.int8 or weight.dim() != 2 \
+            or weight.shape[1] != k or weight.get_device() != index or weight.shape[0] < 1:
+        raise ValueError(f"weight must be an int8 tensor (N, {k}) on cuda:{index}")
     n = weight.shape[0]
-    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.shape != (n,) \
-            or scale.device != device:
-        raise ValueError(f"scale must be a float32 tensor ({n},) on {device}")
-    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.device != device
+    if not isinstance(scale, torch.Tensor) or scale.dtype is not torch.float32 or scale.shape != (n,) \
+            or scale.get_device() != index:
+        raise ValueError(f"scale must be a float32 tensor ({n},) on cuda:{index}")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.get_device() != index
                              or bias.dtype not in DTYPES):
-        raise ValueError(f"bias must be a float tensor ({n},) on {device}")
-    with _on(device):
+        raise ValueError(f"bias must be a float tensor ({n},) on cuda:{index}")
+    with _nothing if index == torch.cuda.current_device() else torch.cuda.device(index):
         w = weight if _aligned(weight) else _laid_out(weight)
-        s = scale.contiguous()
-        b = None if bias is None else bias.float().contiguous()
-        dev = device.index
-        if isinstance(x, QuantizedRows):
+        s = scale if scale.is_contiguous() else scale.contiguous()
+        b = bias_at = None
+        if bias is not None:
+            b = bias if bias.dtype is torch.float32 and bias.is_contiguous() else bias.float().contiguous()
+            bias_at = b.data_ptr()
+        if x2 is None:
             c = codes.reshape(-1, k)
             c = c if _aligned(c) else _laid_out(c)
             rows, r = c.shape[0], row_scale.reshape(-1).contiguous()
-            out = torch.empty((rows, n), dtype=out_dtype, device=device)
+            out = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=c.device)
             code = ops().ygg_linear_quantized(
-                dev, rows, k, n, c.data_ptr(), c.stride(0), r.data_ptr(), w.data_ptr(), w.stride(0), s.data_ptr(),
-                None if b is None else b.data_ptr(), DTYPES[out_dtype], out.data_ptr(), n, _raw_stream(dev))
+                index, rows, k, n, c.data_ptr(), c.stride(0), r.data_ptr(), w.data_ptr(), w.stride(0), s.data_ptr(),
+                bias_at, DTYPES[out_dtype], out.data_ptr(), n, _raw_stream(index))
         else:
-            rows = x2.shape[0]
-            out = torch.empty((rows, n), dtype=out_dtype, device=device)
-            nbytes = ops().ygg_linear_workspace(rows, k)
+            rows, device = x2.shape[0], x2.device
+            out = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=device)
+            nbytes = _workspace(rows, k)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             code = ops().ygg_linear(
-                dev, DTYPES[x2.dtype], rows, k, n, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0),
-                s.data_ptr(), None if b is None else b.data_ptr(), DTYPES[out_dtype], out.data_ptr(), n, ws.data_ptr(),
-                nbytes, _raw_stream(dev))
+                index, DTYPES[x2.dtype], rows, k, n, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0),
+                s.data_ptr(), bias_at, DTYPES[out_dtype], out.data_ptr(), n, ws.data_ptr(), nbytes, _raw_stream(index))
         if code:
             check(code, "ygg_linear")
     return out if len(lead) == 1 else out.view(*lead, n)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(rows, k):
+    return ops().ygg_linear_workspace(rows, k)
 
 
 def linear_status(device="cuda"):

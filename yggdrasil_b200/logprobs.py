@@ -14,8 +14,6 @@ a gradient, logprob, entropy, lse and top_logprobs carry one (top_ids does not).
 """
 from __future__ import annotations
 
-from typing import NamedTuple
-
 import numpy as np
 import torch
 
@@ -26,43 +24,60 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 TOP_MAX = 64
 
 
-class TokenLogprobs(NamedTuple):
-    logprob: torch.Tensor
-    entropy: torch.Tensor
-    lse: torch.Tensor
-    top_ids: torch.Tensor | None
-    top_logprobs: torch.Tensor | None
+class TokenLogprobs:
+    """logprob, entropy, lse, top_ids, top_logprobs, by name or in this order."""
+    __slots__ = ("logprob", "entropy", "top_ids", "top_logprobs", "_lse")
+
+    def __init__(self, logprob, entropy, lse, top_ids, top_logprobs):
+        self.logprob, self.entropy, self.top_ids, self.top_logprobs = logprob, entropy, top_ids, top_logprobs
+        self._lse = lse
+
+    @property
+    def lse(self):
+        if type(self._lse) is tuple:   # (buffer of all three, rows, leading shape): a view is made when it is asked for
+            buf, rows, lead = self._lse
+            self._lse = buf[2 * rows:].view(lead)
+        return self._lse
+
+    def __iter__(self):
+        return iter((self.logprob, self.entropy, self.lse, self.top_ids, self.top_logprobs))
 
 
-def _forward(logits, tokens, top, stats):
-    rows, vocab = logits.shape
-    dev = logits.device
-    values = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    ids = tops = None
+def _forward(logits, rows, vocab, tokens, top, stats, index):
+    """logprob and entropy (rows,), the buffer that holds them and lse, and the alternatives."""
+    device = logits.device
+    buf = torch.empty(3 * rows, dtype=torch.float32, device=device)
+    at = buf.data_ptr()
     if top:
-        ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
-        tops = torch.empty((rows, top), dtype=torch.float32, device=dev)
-    at = values.data_ptr()
+        shape, strides = (rows, top), (top, 1)
+        ids = torch.empty_strided(shape, strides, dtype=torch.int32, device=device)
+        tops = torch.empty_strided(shape, strides, dtype=torch.float32, device=device)
+        ids_at, tops_at = ids.data_ptr(), tops.data_ptr()
+    else:
+        ids = tops = ids_at = tops_at = None
     code = ops().ygg_token_logprobs(
-        dev.index, DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
-        tokens.element_size(), top, at, at + 4 * rows, at + 8 * rows, ids.data_ptr() if top else None,
-        tops.data_ptr() if top else None, stats.data_ptr() if stats is not None else None, _raw_stream(dev.index))
+        index, DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
+        tokens.element_size(), top, at, at + 4 * rows, at + 8 * rows, ids_at, tops_at,
+        stats.data_ptr() if stats is not None else None, _raw_stream(index))
     if code:
         check(code, "ygg_token_logprobs")
-    return *values.unbind(0), ids, tops
+    one = (rows,)
+    return buf.as_strided(one, (1,), 0), buf.as_strided(one, (1,), rows), buf, ids, tops
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
         stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=logits.device)
-        out = _forward(logits, tokens, top, stats)
-        ctx.save_for_backward(logits, tokens, stats, out[3])
+        rows = logits.shape[0]
+        logprob, entropy, buf, ids, tops = _forward(logits, rows, logits.shape[1], tokens, top, stats,
+                                                    logits.device.index)
+        ctx.save_for_backward(logits, tokens, stats, ids)
         ctx.top = top
         ctx.set_materialize_grads(False)
         if top:
-            ctx.mark_non_differentiable(out[3])
-        return out
+            ctx.mark_non_differentiable(ids)
+        return logprob, entropy, buf[2 * rows:], ids, tops
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -94,7 +109,8 @@ def token_logprobs(logits, tokens, top=0):
     0, and alternatives by the lower index; a row that holds NaN or +inf has NaN values."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in DTYPES or logits.dim() < 1:
         raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor (..., V)")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    shape = logits.shape
+    lead, vocab, index = shape[:-1], shape[-1], logits.get_device()
     if vocab < 1:
         raise ValueError("logits: the vocabulary is empty")
     if not 0 <= top <= min(vocab, TOP_MAX):
@@ -104,22 +120,27 @@ def token_logprobs(logits, tokens, top=0):
         if host.size and (host.dtype.kind not in "iu" or host.max() >= vocab):
             raise ValueError(f"tokens must be integers below {vocab}")
         tokens = torch.as_tensor(np.array(host, np.int64)).to(logits.device)
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
+    if (tokens.dtype is not torch.int32 and tokens.dtype is not torch.int64) or tokens.get_device() != index:
         raise ValueError(f"tokens must be int32 or int64 on {logits.device}")
     if tokens.shape != lead:
-        raise ValueError(f"tokens {tuple(tokens.shape)} for logits {tuple(logits.shape)}: one token for each row")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    if x.stride(1) != 1 and vocab > 1:
+        raise ValueError(f"tokens {tuple(tokens.shape)} for logits {tuple(shape)}: one token for each row")
+    x = logits if len(shape) == 2 else logits.reshape(-1, vocab)
+    if vocab > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    t = tokens.contiguous()
-    with torch.cuda.device(x.device) if x.device.index != torch.cuda.current_device() else _nothing:
+    t = tokens if tokens.is_contiguous() else tokens.contiguous()
+    rows = x.shape[0]
+    with _nothing if index == torch.cuda.current_device() else torch.cuda.device(index):
         if x.requires_grad and torch.is_grad_enabled():
             out = _TokenLogprobs.apply(x, t, top)
-        else:
-            out = _forward(x, t, top, None)
+            if len(lead) != 1:
+                out = [None if v is None else v.reshape(lead + v.shape[1:]) for v in out]
+            return TokenLogprobs(*out)
+        logprob, entropy, buf, ids, tops = _forward(x, rows, vocab, t, top, None, index)
     if len(lead) != 1:
-        out = [None if v is None else v.reshape(lead + v.shape[1:]) for v in out]
-    return TokenLogprobs(*out)
+        logprob, entropy = logprob.view(lead), entropy.view(lead)
+        if top:
+            ids, tops = ids.view(*lead, top), tops.view(*lead, top)
+    return TokenLogprobs(logprob, entropy, (buf, rows, lead), ids, tops)
 
 
 class _Nothing:
