@@ -98,12 +98,12 @@ template <> constexpr uint32_t kMinusInf<__half> = 0xFC00u;
 template <> constexpr uint32_t kMinusInf<__nv_bfloat16> = 0xFF80u;
 
 // A warp's run of 32 kPer places from u0 on, lane l those from u0 + l kPer on; -inf outside the row's places [off, end).
-template <typename T>
+template <typename T, bool AGAIN = false>
 __device__ __forceinline__ uint4 load_run(const T *from, uint32_t u0, uint32_t off, uint32_t end, int lane) {
     constexpr int N = kPer<T>;
     const uint32_t u = u0 + lane * N;
     uint4 q = make_uint4(0, 0, 0, 0);
-    if (u < end) q = load_stream(from + u);
+    if (u < end) q = AGAIN ? load_again(from + u) : load_stream(from + u);
     if (u + N > end || u < off) {
         uint32_t *w = (uint32_t *)&q;
 #pragma unroll
@@ -330,8 +330,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
         float most = -INFINITY;
 #pragma unroll
         for (int r = 0; r < RUNS; r++) {
-            if (WHOLE) unpack(load_stream(x + (r * 32 + lane) * N), v[r], T());
-            else load_run<T>(from, r * 32 * N, off, end, lane, v[r]);
+            unpack(WHOLE ? load_again(x + (r * 32 + lane) * N) : load_run<T, true>(from, r * 32 * N, off, end, lane), v[r], T());
         }
 #pragma unroll
         for (int r = 0; r < RUNS; r++)
@@ -549,8 +548,13 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
     const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
     const auto load = [&](uint4(&q)[kBatch], uint32_t u0) {
+        if (u0 >= off && u0 + kBatch * 32 * N <= end) {   // inside the row
 #pragma unroll
-        for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
+            for (int b = 0; b < kBatch; b++) q[b] = load_stream(from + u0 + (b * 32 + lane) * N);
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
+        }
     };
     uint4 q[kBatch];
     if (AHEAD && w * per < segments) load(q, w * per * span);

@@ -46,6 +46,13 @@ __device__ __forceinline__ uint4 load_stream(const void *p) {
     return v;
 }
 
+// The same where the launch comes back to some of the bytes soon: they stay in L1.
+__device__ __forceinline__ uint4 load_again(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // A launch that follows another in its stream may begin before that one ends; it waits here before it reads what the
 // other wrote. The other says when it may begin.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

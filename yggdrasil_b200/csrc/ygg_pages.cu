@@ -140,29 +140,33 @@ __device__ __forceinline__ int length_of(const Cache &c, int64_t s) {
 }
 __device__ __forceinline__ bool is_page(const Cache &c, int p) { return p >= 0 && p < c.count; }
 
-// Whole pages in units of V, `n` of them from the i-th thread of `all` on; move(i) says which.
+// Whole pages in units of V, `n` of them, by the threads of `all` from `thread` on; move(i) says which. Eight units a
+// thread at a time: first where they lie, then all loads, then all stores, so that 128 KB of an SM are in flight.
 template <typename V, typename F>
 __device__ __forceinline__ void copy_moves(const Cache &c, int64_t n, int64_t thread, int64_t all, F move) {
+    constexpr int kEach = 8;
     const int64_t units = c.page_bytes / (int64_t)sizeof(V), total = n * units;
-    const bool narrow = total + 4 * all < ((int64_t)1 << 32);
-    for (int64_t u0 = thread; u0 < total; u0 += 4 * all) {
-        V v[4];
-        char *to[4];
+    const bool narrow = total + kEach * all < ((int64_t)1 << 32);
+    for (int64_t u0 = thread; u0 < total; u0 += kEach * all) {
+        V v[kEach];
+        int64_t from[kEach], to[kEach];   // -1: zeros; nothing to do
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int64_t u = u0 + k * all;
-            to[k] = nullptr;
-            v[k] = V{};
-            if (u >= total) continue;
+        for (int k = 0; k < kEach; k++) {
+            const int64_t u = min(u0 + k * all, total - 1);
             const int64_t i = narrow ? (uint32_t)u / (uint32_t)units : u / units, at = (u - i * units) * sizeof(V);
             const Move m = move(i);
-            if (m.to < 0 || m.to >= c.count || m.from >= c.count) continue;
-            to[k] = c.pages + m.to * c.page_bytes + at;
-            if (m.from >= 0) v[k] = *(const V *)(c.pages + m.from * c.page_bytes + at);
+            const bool go = u0 + k * all < total && m.to >= 0 && m.to < c.count && m.from < c.count;
+            to[k] = go ? m.to * c.page_bytes + at : -1;
+            from[k] = go && m.from >= 0 ? m.from * c.page_bytes + at : -1;
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (to[k]) *(V *)to[k] = v[k];
+        for (int k = 0; k < kEach; k++) {
+            v[k] = V{};
+            if (from[k] >= 0) v[k] = *(const V *)(c.pages + from[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; k++)
+            if (to[k] >= 0) *(V *)(c.pages + to[k]) = v[k];
     }
 }
 
@@ -183,16 +187,20 @@ __global__ void __launch_bounds__(kPlan, 1)
     const Range mine = share(n), pages = share(c.count);
     int *const free_counts = counts, *const held_counts = counts + kMaxBlocks;
     const auto slot = [&](int64_t child, int taken) { return c.table + child * c.per_stream + (grow ? taken : 0); };
-    const auto child_of = [&](int64_t i) { return grow ? parents[i] : children[i]; };
+    // a thread's first entry stays in registers (all of them, up to 1024 a block); the others are read again
+    int32_t parent0 = -1, child0 = -1;
+    int taken0 = -1;
 
+    const int64_t first_page = pages.from + threadIdx.x;
+    const bool free0 = first_page < pages.to && c.refs[first_page] == 0;   // its load runs under the claims
     for (int64_t i = mine.from + threadIdx.x; i < mine.to; i += kPlan) {
-        const int64_t parent = parents[i], child = child_of(i);
+        const int32_t parent = parents[i], child = grow ? parent : children[i];
         int taken = -1;
         if (parent >= 0 && child >= 0) {
             if (parent >= c.streams || child >= c.streams) {
                 report(c.status, kBadIndex);
             } else {
-                const int held = length_of(c, parent);
+                const int held = length_of(c, parent), other = grow ? 0 : length_of(c, child);
                 if (grow) {
                     taken = held;
                     if (held >= c.per_stream) {
@@ -203,29 +211,31 @@ __global__ void __launch_bounds__(kPlan, 1)
                     taken = depth ? min(depth[i], held) : held;
                     if (taken <= 0) {   // a parent without pages: a child without
                         taken = -1;
-                    } else if (length_of(c, child) != 0) {
+                    } else if (other != 0) {
                         report(c.status, kBadIndex);
                         taken = -1;
                     }
                 }
             }
         }
-        info[i] = taken;
         if (taken >= 0) atomicMin(slot(child, taken), kClaim + (int32_t)i);
+        if (i < mine.from + kPlan) parent0 = parent, child0 = child, taken0 = taken;
+        else info[i] = taken;
     }
-    int free_here = 0, before;
-    for (int64_t p0 = pages.from; p0 < pages.to; p0 += kPlan) {
+    int free_here = __syncthreads_count(free0), before;
+    for (int64_t p0 = pages.from + kPlan; p0 < pages.to; p0 += kPlan) {
         const int64_t p = p0 + threadIdx.x;
         free_here += __syncthreads_count(p < pages.to && c.refs[p] == 0);
     }
     if (threadIdx.x == 0) free_counts[blockIdx.x] = free_here;
     if (!all_blocks(c)) return;
 
+    const int32_t claim0 = taken0 >= 0 ? __ldcg(slot(child0, taken0)) : 0;   // its load runs under the free pages' list
     int free_before;
     const int available = over_blocks(free_counts, scratch, free_before);
     for (int64_t p0 = pages.from; p0 < pages.to && free_before < n; p0 += kPlan) {
         const int64_t p = p0 + threadIdx.x;
-        const bool is_free = p < pages.to && c.refs[p] == 0;
+        const bool is_free = p0 == pages.from ? free0 : p < pages.to && c.refs[p] == 0;
         const int here = block_count(is_free, scratch, before);
         if (is_free && free_before + before < n) order[free_before + before] = (int32_t)p;
         free_before += here;
@@ -233,37 +243,45 @@ __global__ void __launch_bounds__(kPlan, 1)
     int held = 0;
     for (int64_t i0 = mine.from; i0 < mine.to; i0 += kPlan) {
         const int64_t i = i0 + threadIdx.x;
+        const bool first = i0 == mine.from;
+        const int taken = i >= mine.to ? -1 : first ? taken0 : info[i];
         bool holds = false;
-        if (i < mine.to && info[i] >= 0) {
-            holds = __ldcg(slot(child_of(i), info[i])) == kClaim + (int32_t)i;
+        if (taken >= 0) {
+            const int32_t claim = first ? claim0 : __ldcg(slot(grow ? parents[i] : children[i], taken));
+            holds = claim == kClaim + (int32_t)i;
             if (!holds) {   // named twice
                 report(c.status, kBadIndex);
-                info[i] = -1;
+                if (first) taken0 = -1;
+                else info[i] = -1;
             }
         }
         held += __syncthreads_count(holds);
     }
     if (threadIdx.x == 0) held_counts[blockIdx.x] = held;
+    // what the first entry will copy does not wait for its place
+    const int32_t source0 = taken0 > 0 ? c.table[(int64_t)parent0 * c.per_stream + taken0 - 1] : -1;
     if (!all_blocks(c)) return;
 
     int given;
     over_blocks(held_counts, scratch, given);
     for (int64_t i0 = mine.from; i0 < mine.to; i0 += kPlan) {
         const int64_t i = i0 + threadIdx.x;
-        const int taken = i < mine.to ? info[i] : -1;
+        const bool first = i0 == mine.from;
+        const int taken = i >= mine.to ? -1 : first ? taken0 : info[i];
         const int here = block_count(taken >= 0, scratch, before);
         Move m{-1, -1};
         if (taken >= 0) {
-            const int64_t child = child_of(i);
+            const int64_t parent = first ? parent0 : parents[i], child = first ? child0 : grow ? parent : children[i];
             int32_t *row = c.table + child * c.per_stream;
             if (given + before < available) {
-                const int32_t *from = c.table + parents[i] * (int64_t)c.per_stream;
+                const int32_t *from = c.table + parent * c.per_stream;
                 m.to = __ldcg(order + given + before);
-                m.from = taken > 0 ? from[taken - 1] : -1;
+                m.from = first ? source0 : taken > 0 ? from[taken - 1] : -1;
                 if (!grow)
                     for (int j = 0; j < taken - 1; j++) {
-                        row[j] = from[j];
-                        if (is_page(c, from[j])) atomicAdd(&c.refs[from[j]], 1);
+                        const int32_t page = from[j];
+                        row[j] = page;
+                        if (is_page(c, page)) atomicAdd(&c.refs[page], 1);
                     }
                 row[grow ? taken : taken - 1] = m.to;
                 c.refs[m.to] = 1;
