@@ -167,17 +167,48 @@ __device__ __forceinline__ Pair exp2_approx(Pair v) {
     return pair(exp2_approx(f.x), exp2_approx(f.y));
 }
 
-// Adds entries to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN; it is rare, so
-// the sum says whether there was one, and only then the products are formed again with y cut off.
-template <int N, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const float (&v)[RUNS][N]) {
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[4], float) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[8], T t) {
+    return make_uint4(pack2(v[0], v[1], t), pack2(v[2], v[3], t), pack2(v[4], v[5], t), pack2(v[6], v[7], t));
+}
+
+// The i-th pair of a vector.
+__device__ __forceinline__ Pair pair_of(const uint4 &q, int i, float) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
+__device__ __forceinline__ Pair pair_of(const uint4 &q, int i, __nv_bfloat16) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ Pair pair_of(const uint4 &q, int i, __half) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const float2 f = __half22float2(*(const __half2 *)&w[i]);
+    return pair(f.x, f.y);
+}
+
+// Adds the entries of vectors to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN; it
+// is rare, so the sum says whether there was one, and only then the products are formed again with y cut off.
+template <typename T, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const uint4 (&q)[RUNS]) {
+    constexpr int N = kPer<T>;
     const float m = a.m == -INFINITY ? 0.0f : a.m;
     const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e);
     Pair s = 0, t = 0;
 #pragma unroll
     for (int r = 0; r < RUNS; r++)
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const Pair y = add(pair(v[r][i], v[r][i + 1]), minus), e = exp2_approx(mul(y, l));
+        for (int i = 0; i < N / 2; i++) {
+            const Pair y = add(pair_of(q[r], i, T()), minus), e = exp2_approx(mul(y, l));
             s = add(s, e);
             t = fma(e, y, t);
         }
@@ -186,12 +217,15 @@ template <int N, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, 
     if (sum != sum) {
         sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < RUNS; r++)
+        for (int r = 0; r < RUNS; r++) {
+            float v[N];
+            unpack(q[r], v, T());
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float y = v[r][i] - m;
+                const float y = v[i] - m;
                 sum = fmaf(exp2_approx(y * kLog2e), fmaxf(y, kFloor), sum);
             }
+        }
     }
     a.s += sf.x + sf.y;
     a.t += sum;
@@ -274,14 +308,15 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
     const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
     if (row >= p.rows) return;
     const T *x = (const T *)p.logits + row * p.stride;
-    float v[1][8];
+    float v[8];
     Sums a = none();
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        v[0][i] = i < p.vocab ? to_f(x[i]) : -INFINITY;
-        a.m = fmaxf(a.m, v[0][i]);
+        v[i] = i < p.vocab ? to_f(x[i]) : -INFINITY;
+        a.m = fmaxf(a.m, v[i]);
     }
-    add_entries(a, v);
+    const uint4 q[2] = {pack({v[0], v[1], v[2], v[3]}, 0.0f), pack({v[4], v[5], v[6], v[7]}, 0.0f)};
+    add_entries<float>(a, q);
     const Ends e(a);
     write_row(p, row, x, a, e);
     if (p.top == 0) return;
@@ -290,8 +325,8 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
         int above = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j != i) above += order(v[0][j]) + (j < i) > order(v[0][i]);
-        if (i < p.vocab && above < p.top) write_top(p, row, above, key_of(v[0][i], i), e);
+            if (j != i) above += order(v[j]) + (j < i) > order(v[i]);
+        if (i < p.vocab && above < p.top) write_top(p, row, above, key_of(v[i], i), e);
     }
 }
 
@@ -326,11 +361,13 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
         const T *x = (const T *)p.logits + row * p.stride;
         const uint32_t off = WHOLE ? 0 : offset_of(x), end = WHOLE ? RUNS * 32 * N : (uint32_t)p.vocab + off;
         const T *from = x - off;
+        uint4 q[RUNS];
         float v[RUNS][N];
         float most = -INFINITY;
 #pragma unroll
         for (int r = 0; r < RUNS; r++) {
-            unpack(WHOLE ? load_again(x + (r * 32 + lane) * N) : load_run<T, true>(from, r * 32 * N, off, end, lane), v[r], T());
+            q[r] = (WHOLE ? load_again(x + (r * 32 + lane) * N) : load_run<T, true>(from, r * 32 * N, off, end, lane));
+            unpack(q[r], v[r], T());
         }
 #pragma unroll
         for (int r = 0; r < RUNS; r++)
@@ -338,7 +375,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
             for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
         const int mine = order(most);
         Sums a{unorder(__reduce_max_sync(~0u, mine)), 0.0f, 0.0f};
-        add_entries(a, v);
+        add_entries<T>(a, q);
         ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
         found[w] = 0;
         if (p.top == 0) continue;
@@ -556,25 +593,29 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
             for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
         }
     };
-    uint4 q[kBatch];
-    if (AHEAD && w * per < segments) load(q, w * per * span);
+    uint4 q[kBatch], next[kBatch];
+    if (AHEAD && w * per < segments) load(next, w * per * span);
     for (int g0 = w * per; g0 < segments; g0 += warps * per) {
         float top_of[kBatch];
         for (int step = 0; step < steps; step++) {
-            float v[kBatch][N], most = -INFINITY;
-            if (!AHEAD) load(q, g0 * span + step * kBatch * 32 * N);
+            const bool on = step + 1 < steps;
+            if (AHEAD) {
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) q[b] = next[b];
+                if (on || g0 + warps * per < segments)
+                    load(next, (on ? g0 : g0 + warps * per) * span + (on ? step + 1 : 0) * kBatch * 32 * N);
+            } else {
+                load(q, g0 * span + step * kBatch * 32 * N);
+            }
+            float most = -INFINITY;
 #pragma unroll
             for (int b = 0; b < kBatch; b++) {
                 const float t = largest(q[b], T());
                 top_of[b] = shift && step ? fmaxf(top_of[b], t) : t;
                 most = fmaxf(most, t);
-                unpack(q[b], v[b], T());
             }
-            const bool on = step + 1 < steps;
-            if (AHEAD && (on || g0 + warps * per < segments))
-                load(q, (on ? g0 : g0 + warps * per) * span + (on ? step + 1 : 0) * kBatch * 32 * N);
             if (most > a.m) raise(a, most);
-            add_entries(a, v);
+            add_entries<T>(a, q);
         }
         if (p.top) {
             if (shift) {
@@ -872,20 +913,6 @@ struct RowGrad {
     }
 };
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *(const uint32_t *)&h;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *(const uint32_t *)&h;
-}
-__device__ __forceinline__ uint4 pack(const float (&v)[4], float) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-}
-template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[8], T t) {
-    return make_uint4(pack2(v[0], v[1], t), pack2(v[2], v[3], t), pack2(v[4], v[5], t), pack2(v[6], v[7], t));
-}
 __device__ __forceinline__ void store_stream(void *p, const uint4 &v) {
     asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
