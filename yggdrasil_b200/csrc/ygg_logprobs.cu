@@ -544,19 +544,18 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
 // k-th segment's largest value are ranked by counting. If they are more than a block has threads (ties, masks, sorted
 // rows), a second bound from the threads' best entries leaves fewer; if those are still more, they are taken one at a
 // time.
-// AHEAD: a warp's next batch is loaded while one is added up. Rows that share an SM hide their loads behind each other, and
-// the registers cost a block an SM (8192 x 32768 bf16: 124 us without, 136 with); few rows wait for each load in turn
-// (7 x 100003 bf16: 12.8 us without, 9.5 with).
-constexpr int kLongThreads = 256, kLongWarps = kLongThreads / 32, kMaxSegments = 4096, kMaxCluster = 8, kBatch = 4;
+// (Loading a warp's next batch while one is added up costs the registers of a block an SM and gained nothing: 8192 x 32768
+// bf16 136 us with, 117 without, 7 x 100003 bf16 9.5 and 9.4.)
+constexpr int kMaxSegments = 4096, kMaxCluster = 8, kBatch = 4, kKeys = 256;
 
-struct LongShared {
-    Sums part[kMaxCluster * kLongWarps];   // in the first block
+template <int WARPS> struct LongShared {
+    Sums part[kMaxCluster * WARPS];   // in the first block
     Sums all;
-    int picked[YGG_TOP_MAX];               // segments
-    Key keys[kLongThreads];
-    Key best[kLongWarps];
+    int picked[YGG_TOP_MAX];          // segments
+    Key keys[kKeys];
+    Key best[WARPS];
     int count, bound;
-    int segment[];                         // order() of the segments' largest values; in the first block of all
+    int segment[];                    // order() of the segments' largest values; in the first block of all
 };
 
 __device__ __forceinline__ uint32_t shared_at(const void *p, uint32_t rank) {
@@ -568,11 +567,11 @@ __device__ __forceinline__ void put_remote(uint32_t at, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-template <typename T, bool AHEAD>
-__global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cluster, int shift, int segments) {
-    constexpr int N = kPer<T>;
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int cluster, int shift, int segments) {
+    constexpr int N = kPer<T>, kThreads = WARPS * 32;
     extern __shared__ __align__(16) uint8_t raw[];
-    LongShared &sh = *(LongShared *)raw;
+    LongShared<WARPS> &sh = *(LongShared<WARPS> *)raw;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x / cluster;
     const int rank = blockIdx.x - (int)row * cluster;
@@ -581,7 +580,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     const uint32_t off = offset_of(x), span = (32u * N) << shift, end = (uint32_t)p.vocab + off;
     const T *from = x - off;
     Sums a = none();
-    const int w = rank * kLongWarps + warp, warps = cluster * kLongWarps;
+    const int w = rank * WARPS + warp, warps = cluster * WARPS;
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
     const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
     const auto load = [&](uint4(&q)[kBatch], uint32_t u0) {
@@ -593,20 +592,11 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
             for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
         }
     };
-    uint4 q[kBatch], next[kBatch];
-    if (AHEAD && w * per < segments) load(next, w * per * span);
     for (int g0 = w * per; g0 < segments; g0 += warps * per) {
         float top_of[kBatch];
         for (int step = 0; step < steps; step++) {
-            const bool on = step + 1 < steps;
-            if (AHEAD) {
-#pragma unroll
-                for (int b = 0; b < kBatch; b++) q[b] = next[b];
-                if (on || g0 + warps * per < segments)
-                    load(next, (on ? g0 : g0 + warps * per) * span + (on ? step + 1 : 0) * kBatch * 32 * N);
-            } else {
-                load(q, g0 * span + step * kBatch * 32 * N);
-            }
+            uint4 q[kBatch];
+            load(q, g0 * span + step * kBatch * 32 * N);
             float most = -INFINITY;
 #pragma unroll
             for (int b = 0; b < kBatch; b++) {
@@ -655,7 +645,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         if (rank) return;
     }
     __syncthreads();
-    if (warp == 1) {   // the sums, while the first warp looks for the best segments
+    if (warp == (WARPS > 1)) {   // the sums, while the first warp looks for the best segments
         a = lane < warps ? sh.part[lane] : none();
         if (lane + 32 < warps) join(a, sh.part[lane + 32]);
 #pragma unroll
@@ -689,7 +679,7 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
             const bool in = g < segments && sh.segment[g] >= bound;
             const unsigned who = __ballot_sync(~0u, in);
             const int at = n + __popc(who & ((1u << lane) - 1));
-            if (in && at < kLongThreads) sh.keys[at] = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
+            if (in && at < kKeys) sh.keys[at] = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
             n += __popc(who);
         }
         if (lane == 0) sh.count = n;
@@ -697,26 +687,28 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     __syncthreads();
     const Ends e(sh.all);
     const int found = sh.count;
-    if (found <= kLongThreads) {
-        const Key key = threadIdx.x < found ? sh.keys[threadIdx.x] : 0;
-        int above = 0;
-        for (int i = 0; i < found; i++) above += sh.keys[i] > key;
-        if (threadIdx.x < found && above < picks) {
-            sh.picked[above] = index_of(key);
-            if (above == picks - 1) sh.bound = order(value_of(key));
+    if (found <= kKeys) {
+        for (int k = threadIdx.x; k < found; k += kThreads) {
+            const Key key = sh.keys[k];
+            int above = 0;
+            for (int i = 0; i < found; i++) above += sh.keys[i] > key;
+            if (above < picks) {
+                sh.picked[above] = index_of(key);
+                if (above == picks - 1) sh.bound = order(value_of(key));
+            }
         }
     } else {   // many equal segments
         Key last = ~0ull;
         for (int k = 0; k < picks; k++) {
             Key best = 0;
-            for (int g = threadIdx.x; g < segments; g += kLongThreads) {
+            for (int g = threadIdx.x; g < segments; g += kThreads) {
                 const Key key = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
                 if (key < last && key > best) best = key;
             }
             best = warp_max(best);
             if (lane == 0) sh.best[warp] = best;
             __syncthreads();
-            for (int i = 0; i < kLongWarps; i++) best = max(best, sh.best[i]);
+            for (int i = 0; i < WARPS; i++) best = max(best, sh.best[i]);
             last = best;
             if (threadIdx.x == 0) {
                 sh.picked[k] = index_of(last);
@@ -728,10 +720,9 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    // with fewer segments than alternatives every entry is a candidate
-    const float bound = picks < p.top ? -INFINITY : unorder(sh.bound);
+    const float bound = unorder(sh.bound);
     const int runs = picks << shift;   // runs of 32 N entries in the picked segments
-    for (int q = warp; q < runs; q += kLongWarps) {
+    for (int q = picks < p.top ? runs : warp; q < runs; q += WARPS) {
         const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
         float v[N];
         load_run<T>(from, u0, off, end, lane, v);
@@ -740,17 +731,17 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
             const uint32_t u = u0 + lane * N + i;
             if (!(v[i] < bound) && u - off < end - off) {
                 const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
-                if (at < kLongThreads) sh.keys[at] = key_of(v[i], u - off);
+                if (at < kKeys) sh.keys[at] = key_of(v[i], u - off);
             }
         }
     }
     __syncthreads();
-    int n = sh.count;
-    if (n > kLongThreads) {
+    int n = picks < p.top ? INT32_MAX : sh.count;   // fewer segments than alternatives: any entry may be one
+    if (n > kKeys && p.top <= kThreads) {
         // ties, masks, sorted rows, or fewer segments than alternatives: the k-th best of the threads' best entries (by
         // value and index) is a better bound
         Key mine = 0;
-        for (int q = warp; q < runs; q += kLongWarps) {
+        for (int q = warp; q < runs; q += WARPS) {
             const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
@@ -764,13 +755,13 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         sh.keys[threadIdx.x] = mine;
         __syncthreads();
         int above = 0;
-        for (int i = 0; i < kLongThreads; i++) above += sh.keys[i] > mine;
+        for (int i = 0; i < kThreads; i++) above += sh.keys[i] > mine;
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0;
         if (mine && above == p.top - 1) sh.best[0] = mine;
         __syncthreads();
         const Key least = sh.best[0];
-        for (int q = warp; q < runs; q += kLongWarps) {
+        for (int q = warp; q < runs; q += WARPS) {
             const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
@@ -780,24 +771,26 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
                 const Key key = u - off < end - off ? key_of(v[i], u - off) : 0;
                 if (key && key >= least) {
                     const int at = atomicAdd(&sh.count, 1);
-                    if (at < kLongThreads) sh.keys[at] = key;
+                    if (at < kKeys) sh.keys[at] = key;
                 }
             }
         }
         __syncthreads();
         n = sh.count;
     }
-    if (n <= kLongThreads) {
-        const Key key = threadIdx.x < n ? sh.keys[threadIdx.x] : 0;
-        int above = 0;
-        for (int i = 0; i < n; i++) above += sh.keys[i] > key;
-        if (threadIdx.x < n && above < p.top) write_top(p, row, above, key, e);
+    if (n <= kKeys) {
+        for (int k = threadIdx.x; k < n; k += kThreads) {
+            const Key key = sh.keys[k];
+            int above = 0;
+            for (int i = 0; i < n; i++) above += sh.keys[i] > key;
+            if (above < p.top) write_top(p, row, above, key, e);
+        }
         return;
     }
     Key last = ~0ull;
     for (int k = 0; k < p.top; k++) {
         Key best = 0;
-        for (int q = warp; q < runs; q += kLongWarps) {
+        for (int q = warp; q < runs; q += WARPS) {
             const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
             float v[N];
             load_run<T>(from, u0, off, end, lane, v);
@@ -812,17 +805,34 @@ __global__ void __launch_bounds__(kLongThreads) long_kernel(const Rows p, int cl
         __syncthreads();
         if (lane == 0) sh.best[warp] = best;
         __syncthreads();
-        for (int i = 0; i < kLongWarps; i++) best = max(best, sh.best[i]);
+        for (int i = 0; i < WARPS; i++) best = max(best, sh.best[i]);
         last = best;
         if (threadIdx.x == 0) write_top(p, row, k, last, e);
     }
 }
 
 // Blocks a row for the long kernel: as many as it takes to give the SMs work, up to 8, while each keeps a batch a warp.
+constexpr int kFewWarps = 8;
 int cluster_for(int64_t rows, int64_t runs, int sms) {
     int c = 1;
-    while (c < kMaxCluster && rows * c < 2 * sms && runs >= 2 * c * kLongWarps * kBatch) c *= 2;
+    while (c < kMaxCluster && rows * c < 2 * sms && runs >= 2 * c * kFewWarps * kBatch) c *= 2;
     return c;
+}
+
+template <typename T, int WARPS>
+cudaError_t launch_long(const Rows &p, int cluster, int shift, int segments, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * cluster));
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = sizeof(LongShared<WARPS>) + (p.top ? segments : 0) * sizeof(int);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1;
+    return cudaLaunchKernelEx(&cfg, long_kernel<T, WARPS>, p, cluster, shift, segments);
 }
 
 // Four rows a warp as soon as they fill the SMs.
@@ -854,19 +864,14 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
     while ((runs >> shift) >= kMaxSegments) shift = shift ? shift + 1 : 2;
     const int segments = (int)((runs + (1ll << shift) - 1) >> shift);
     const int cluster = cluster_for(p.rows, runs, sm_count());
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * cluster));
-    cfg.blockDim = dim3(kLongThreads);
-    cfg.dynamicSmemBytes = sizeof(LongShared) + (p.top ? segments : 0) * sizeof(int);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1;
-    return cluster > 1 ? cudaLaunchKernelEx(&cfg, long_kernel<T, true>, p, cluster, shift, segments)
-                       : cudaLaunchKernelEx(&cfg, long_kernel<T, false>, p, cluster, shift, segments);
+    if (cluster > 1) return launch_long<T, kFewWarps>(p, cluster, shift, segments, st);
+    // about 24 warps an SM, with as few to a row as give that: what a row needs once, it needs of each of its warps
+    // (8192 x 32768 bf16: 101 us with one, 117 with eight; 600 x 100003 fp32: 180 and 45)
+    const int64_t wanted = 24 * (int64_t)sm_count();
+    if (p.rows >= wanted) return launch_long<T, 1>(p, 1, shift, segments, st);
+    if (p.rows * 2 >= wanted) return launch_long<T, 2>(p, 1, shift, segments, st);
+    if (p.rows * 4 >= wanted) return launch_long<T, 4>(p, 1, shift, segments, st);
+    return launch_long<T, 8>(p, 1, shift, segments, st);
 }
 
 // What the gradient of a row needs: p (A + B y) everywhere, p = 2^(y log2 e - log2 s), and more at the given token and
