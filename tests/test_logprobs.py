@@ -391,3 +391,24 @@ def test_very_wide_rows(rows, vocab):
     x[0] = -INF
     x[0, vocab - 2] = 0.5
     check_values(x, t, 20, op()(x, t, top=20))
+
+
+@pytest.mark.gpu
+def test_no_second_derivative():
+    x, t = make(3, 40, torch.float32)
+    leaf = x.requires_grad_()
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(op()(leaf, t).logprob.sum(), leaf, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_alternatives_alone_and_of_float64_arrivals():
+    x, t = make(6, 700, torch.bfloat16, seed=41)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    out = op()(a, t, top=3)
+    assert not out.top_ids.requires_grad and out.top_logprobs.requires_grad
+    g = torch.randn(6, 3, device="cuda")
+    out.top_logprobs.backward(g)
+    out = op()(b, t, top=3)
+    (out.top_logprobs.double() * g.double()).sum().backward()
+    assert torch.equal(a.grad, b.grad) and a.grad.shape == x.shape

@@ -66,38 +66,46 @@ def _forward(logits, rows, vocab, tokens, top, stats, index):
 
 
 class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top):
-        stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=logits.device)
-        rows = logits.shape[0]
-        logprob, entropy, buf, ids, tops = _forward(logits, rows, logits.shape[1], tokens, top, stats,
-                                                    logits.device.index)
-        ctx.save_for_backward(logits, tokens, stats, ids)
-        ctx.top = top
-        ctx.set_materialize_grads(False)
-        if top:
-            ctx.mark_non_differentiable(ids)
-        return logprob, entropy, buf[2 * rows:], ids, tops
+    """logprob, entropy, lse and top_logprobs of logits; the ids, which carry no gradient, are put into `box`."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_lse, _, g_top):
-        logits, tokens, stats, ids = ctx.saved_tensors
+    def forward(ctx, logits, tokens, top, box):
         rows, vocab = logits.shape
+        index = logits.get_device()
+        stats = torch.empty_strided((rows, 4), (4, 1), dtype=torch.float32, device=logits.device)
+        logprob, entropy, buf, ids, tops = _forward(logits, rows, vocab, tokens, top, stats, index)
+        ctx.save_for_backward(logits, tokens, stats, ids)
+        ctx.sizes = rows, vocab, top, index
+        ctx.set_materialize_grads(False)
+        box.append(ids)
+        return logprob, entropy, buf.as_strided((rows,), (1,), 2 * rows), tops
+
+    @staticmethod
+    def backward(ctx, g_logprob, g_entropy, g_lse, g_top):
+        if torch.is_grad_enabled():   # create_graph
+            raise NotImplementedError("token_logprobs has no second derivative")
+        logits, tokens, stats, ids = ctx.saved_tensors
+        rows, vocab, top, index = ctx.sizes
+        step, dtype = logits.stride(0), logits.dtype
         # rows that lie to the 16-byte boundary as the logits' do move 16 bytes at a time
         per = 16 // logits.element_size()
-        wide = -(-vocab // per) * per if logits.stride(0) % per == 0 else vocab
-        grad = torch.empty((rows, wide), dtype=logits.dtype, device=logits.device)[:, :vocab]
-        # what arrives may be expanded (a sum's gradient) or of another type
-        arriving = [None if g is None else g.float().contiguous() for g in (g_logprob, g_entropy, g_lse, g_top)]
-        dev = logits.device.index
+        wide = -(-vocab // per) * per if step % per == 0 else vocab
+        grad = torch.empty_strided((rows, vocab), (wide, 1), dtype=dtype, device=logits.device)
+        keep = [_arrived(g) for g in (g_logprob, g_entropy, g_lse, g_top)]
         code = ops().ygg_token_logprobs_backward(
-            dev, DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), logits.stride(0), tokens.data_ptr(),
-            tokens.element_size(), ctx.top, ids.data_ptr() if ids is not None else None, stats.data_ptr(),
-            *[None if g is None else g.data_ptr() for g in arriving], grad.data_ptr(), wide, _raw_stream(dev))
+            index, DTYPES[dtype], rows, vocab, logits.data_ptr(), step, tokens.data_ptr(), tokens.element_size(), top,
+            ids.data_ptr() if top else None, stats.data_ptr(), *[None if g is None else g.data_ptr() for g in keep],
+            grad.data_ptr(), wide, _raw_stream(index))
         if code:
             check(code, "ygg_token_logprobs_backward")
-        return grad, None, None
+        return grad, None, None, None
+
+
+def _arrived(g):
+    """A gradient that arrives, as the kernel reads it: it may be expanded (a sum's) or of another type."""
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.float().contiguous()
 
 
 def token_logprobs(logits, tokens, top=0):
@@ -131,7 +139,9 @@ def token_logprobs(logits, tokens, top=0):
     rows = x.shape[0]
     with _nothing if index == torch.cuda.current_device() else torch.cuda.device(index):
         if x.requires_grad and torch.is_grad_enabled():
-            out = _TokenLogprobs.apply(x, t, top)
+            box = []
+            logprob, entropy, lse, tops = _TokenLogprobs.apply(x, t, top, box)
+            out = logprob, entropy, lse, box[0], tops
             if len(lead) != 1:
                 out = [None if v is None else v.reshape(lead + v.shape[1:]) for v in out]
             return TokenLogprobs(*out)
