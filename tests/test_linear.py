@@ -280,3 +280,42 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.ygg_linear_workspace(-1, 17) == 0
     assert g(0, 0, 3, 17, 4, p, 17, p, 32, p, None, 0, p, 4, p, 8, None) == E.YGG_E_ARG
     assert g(0, 0, 3, 17, 4, p, 17, p, 32, p, None, 0, p, 4, None, 1 << 20, None) == E.YGG_E_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 20, 300])
+def test_weights_written_just_before_the_product(rows):
+    """The product may begin under the launches before it, but reads weights, scales and rows only when they are written:
+    weights quantised, rows computed and both used back to back."""
+    f, q = ops()
+    x = inputs(rows, 2048, torch.bfloat16)
+    w = [torch.randn(3000, 2048, device="cuda", generator=torch.Generator("cuda").manual_seed(k)) for k in range(3)]
+    want = []
+    for v in w:
+        c = q(v)
+        torch.cuda.synchronize()
+        want.append(f(x * 2, c.codes, c.scale))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for v in w:
+            y = x * 2
+            c = q(v)
+            got.append(f(y, c.codes, c.scale))
+            got.append(f(q(y), c.codes, c.scale, out_dtype=torch.bfloat16))
+            c.codes.zero_()   # its memory is free to be used again
+        assert all(torch.equal(got[2 * k], want[k]) and torch.equal(got[2 * k + 1], want[k]) for k in range(3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 4, 16])
+def test_weights_that_end_with_their_allocation(rows):
+    """Weights of 128 MiB to the byte: nothing past them may be read."""
+    f, _ = ops()
+    x = inputs(rows, 4096, torch.bfloat16)
+    w = [torch.randint(-127, 128, (32768, 4096), dtype=torch.int8, device="cuda") for _ in range(3)]
+    s = torch.full((32768,), 0.01, device="cuda")
+    for v in w:
+        y = f(x, v, s)
+        pick = torch.tensor([0, 1, 16383, 32766, 32767], device="cuda")
+        check(y[:, pick], x, v[pick], s[pick], None, torch.bfloat16)

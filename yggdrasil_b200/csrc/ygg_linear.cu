@@ -97,7 +97,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
     __shared__ uint32_t part[8];
     const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     const int t = threadIdx.x & (THREADS - 1);
-    let_next_begin();
+    wait_for_previous();
+    let_next_begin();   // not before the wait: a product may read its weights before its own wait, and whoever wrote them
+                        // has to be done by then
     if (row >= p.rows) return;
     const T *x = (const T *)p.x + row * p.stride;
     uint4 q[VECS];
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
 // Any k and any alignment: the row is read twice.
 template <typename T> __global__ void __launch_bounds__(256) quantize_any_kernel(const Quantize p) {
     __shared__ uint32_t part[8];
+    wait_for_previous();
     let_next_begin();
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = (const T *)p.x + row * p.stride;
@@ -166,25 +169,39 @@ template <typename T> __global__ void __launch_bounds__(256) quantize_any_kernel
     }
 }
 
-template <typename T> void launch_quantize(const Quantize &p, cudaStream_t st) {
+template <typename T> cudaError_t launch_quantize(const Quantize &p, cudaStream_t st) {
     constexpr int N = kPer<T>;
+    cudaError_t e;
+    const auto launch = [&](void (*kernel)(const Quantize), unsigned grid) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];   // it may begin under the launch before it
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, p);
+    };
     const bool even = ((uintptr_t)p.x & 15) == 0 && (p.rows == 1 || p.stride % N == 0);
     const int vecs = (p.k + N - 1) / N;
     if (!even || vecs > 2048 || p.rows > INT32_MAX) {
-        quantize_any_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 8 * sm_count()), 256, 0, st>>>(p);
+        e = launch(quantize_any_kernel<T>, (unsigned)std::min<int64_t>(p.rows, 8 * sm_count()));
     } else if (vecs <= 256 && p.rows >= 8 * sm_count()) {   // enough rows to fill the SMs with a warp each
         const unsigned grid = (unsigned)((p.rows + 7) / 8);
-        if (vecs <= 32) quantize_kernel<T, 32, 1><<<grid, 256, 0, st>>>(p);
-        else if (vecs <= 64) quantize_kernel<T, 32, 2><<<grid, 256, 0, st>>>(p);
-        else if (vecs <= 128) quantize_kernel<T, 32, 4><<<grid, 256, 0, st>>>(p);
-        else quantize_kernel<T, 32, 8><<<grid, 256, 0, st>>>(p);
+        if (vecs <= 32) e = launch(quantize_kernel<T, 32, 1>, grid);
+        else if (vecs <= 64) e = launch(quantize_kernel<T, 32, 2>, grid);
+        else if (vecs <= 128) e = launch(quantize_kernel<T, 32, 4>, grid);
+        else e = launch(quantize_kernel<T, 32, 8>, grid);
     } else {
         const unsigned grid = (unsigned)p.rows;
-        if (vecs <= 256) quantize_kernel<T, 256, 1><<<grid, 256, 0, st>>>(p);
-        else if (vecs <= 512) quantize_kernel<T, 256, 2><<<grid, 256, 0, st>>>(p);
-        else if (vecs <= 1024) quantize_kernel<T, 256, 4><<<grid, 256, 0, st>>>(p);
-        else quantize_kernel<T, 256, 8><<<grid, 256, 0, st>>>(p);
+        if (vecs <= 256) e = launch(quantize_kernel<T, 256, 1>, grid);
+        else if (vecs <= 512) e = launch(quantize_kernel<T, 256, 2>, grid);
+        else if (vecs <= 1024) e = launch(quantize_kernel<T, 256, 4>, grid);
+        else e = launch(quantize_kernel<T, 256, 8>, grid);
     }
+    return e;
 }
 
 // ---------------------------------------------------------------------------------------------------- tensor cores
@@ -577,8 +594,7 @@ template <typename T> int launch_split(const Linear &q, int tn, int parts, cudaS
 //
 // Up to 4 rows (from 5 on the tensor cores are faster: 5 x 4096 x 32768 in 26.3 us there, 27.8 us here; 4 rows in 26.6 and
 // 25.0): the weights are read once and nothing else counts. A warp (or `split` warps, each a part of K) takes two
-// channels at a time, 2048 bytes of each, the next ones loaded while dp4a sums the last; the codes of the rows lie in
-// shared memory. Short rows before few weights are quantised by every block itself, under its first loads.
+// channels at a time, 2048 bytes of each; the codes of the rows lie in shared memory. Short rows before few weights are quantised by every block itself, under its first loads.
 constexpr int kFewRows = 4, kFewBlock = 2048;
 
 struct Few {
@@ -608,8 +624,12 @@ __device__ __forceinline__ void store_as(int dtype, void *out, int64_t at, float
     else ((__nv_bfloat16 *)out)[at] = __float2bfloat16_rn(v);
 }
 
+// Blocks an SM. A warp has 4 KB of weights on their way while it sums nothing, so that the SM's warps cover for each other:
+// 1 x 4096 x 32768 in 22.9 us with four blocks, 23.9 with two whose warps load the next 4 KB while they sum.
+template <int ROWS> constexpr int kFewBlocks = ROWS < 4 ? 4 : 3;
+
 // X: the type of the rows to quantise, or int8_t: codes.
-template <typename X, int ROWS> __global__ void __launch_bounds__(256, 2) few_kernel(const Few p) {
+template <typename X, int ROWS> __global__ void __launch_bounds__(256, kFewBlocks<ROWS>) few_kernel(const Few p) {
     extern __shared__ __align__(16) uint8_t room[];   // [ROWS][k_room] codes
     __shared__ uint32_t most[ROWS][8];
     __shared__ float row_scale[ROWS];
@@ -620,7 +640,7 @@ template <typename X, int ROWS> __global__ void __launch_bounds__(256, 2) few_ke
     const int64_t groups = (q.n + 1) / 2, all = (int64_t)gridDim.x * teams, id = (int64_t)blockIdx.x * teams + team;
     const int64_t g0 = groups * id / all, g1 = groups * (id + 1) / all;
     const int blocks = p.k_room / kFewBlock;
-    FewLoad cur, next;
+    FewLoad cur;
     if (!p.early) wait_for_previous();
     if (g0 < g1) few_load(cur, q, 2 * g0, part, lane);
     if constexpr (sizeof(X) > 1) {
@@ -669,8 +689,6 @@ template <typename X, int ROWS> __global__ void __launch_bounds__(256, 2) few_ke
     for (int64_t g = g0; g < g1; g++, turn ^= 1) {
         int acc[2][ROWS] = {};
         for (int kb = part; kb < blocks; kb += p.split) {
-            if (kb + p.split < blocks) few_load(next, q, 2 * g, kb + p.split, lane);
-            else if (g + 1 < g1) few_load(next, q, 2 * (g + 1), part, lane);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint8_t *at = room + kb * kFewBlock + i * 512 + lane * 16;
@@ -682,7 +700,8 @@ template <typename X, int ROWS> __global__ void __launch_bounds__(256, 2) few_ke
                     for (int ch = 0; ch < 2; ch++) acc[ch][r] = dot16(cur.w[ch][i], c, acc[ch][r]);
                 }
             }
-            cur = next;
+            if (kb + p.split < blocks) few_load(cur, q, 2 * g, kb + p.split, lane);
+            else if (g + 1 < g1) few_load(cur, q, 2 * (g + 1), part, lane);
         }
         int mine = 0;   // lane ch ROWS + r keeps the sum of channel ch and row r
 #pragma unroll
@@ -717,11 +736,11 @@ template <typename X, int ROWS> cudaError_t launch_few_rows(Few p, cudaStream_t 
     const size_t smem = (size_t)p.q.rows * p.k_room;
     cudaError_t e = raise_smem_limit((const void *)few_kernel<X, ROWS>, smem, limits);
     if (e != cudaSuccess) return e;
-    const int64_t groups = (p.q.n + 1) / 2, warps = 16 * sm_count();
+    const int64_t groups = (p.q.n + 1) / 2, fit = (int64_t)kFewBlocks<ROWS> * sm_count();
     const int blocks = p.k_room / kFewBlock;
     p.split = 1;
-    while (p.split < 8 && 2 * p.split <= blocks && 2 * p.split * groups <= warps) p.split *= 2;
-    Launch l(std::min<int64_t>((groups * p.split + 7) / 8, 2 * sm_count()), 1, smem, st);
+    while (p.split < 8 && 2 * p.split <= blocks && 2 * p.split * groups <= 8 * fit) p.split *= 2;
+    Launch l(std::min<int64_t>((groups * p.split + 7) / 8, fit), 1, smem, st);
     l.cfg.blockDim = dim3(256);
     if (sizeof(X) > 1) l.cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&l.cfg, few_kernel<X, ROWS>, p);
@@ -739,7 +758,9 @@ int padded_of(int64_t k) { return (int)((k + 15) / 16 * 16); }
 bool rows_ok(int64_t rows, int64_t k) { return rows >= 0 && rows < ((int64_t)1 << 40) && k >= 1; }
 
 int quantize(int dtype, const Quantize &p, cudaStream_t st) {
-    return by_type(dtype, [&](auto t) { launch_quantize<decltype(t)>(p, st); });
+    cudaError_t e = cudaSuccess;
+    const int rc = by_type(dtype, [&](auto t) { e = launch_quantize<decltype(t)>(p, st); });
+    return rc != YGG_OK ? rc : e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 // How a product is cut: CTAs a product, rows a tile, CTAs that share the K of a tile. The least of what the cuts are
