@@ -273,7 +273,7 @@ typedef struct {
     int32_t *length;         /* [streams] */
     int32_t *refs;           /* [page_count] */
     int32_t *status;         /* three words, on the device or mapped host memory (pinned); the caller clears them */
-    uint32_t *sync;          /* two words of device memory, zero before the cache's first call */
+    uint64_t *sync;          /* one word of device memory, zero before the cache's first call */
 } ygg_cache_t;
 
 /* Bytes of device workspace of ygg_cache_fork with n entries, and of ygg_cache_compact (any n). */

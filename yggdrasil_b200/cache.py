@@ -34,11 +34,11 @@ _slots: dict = {}   # device index -> [status words, sync words, how many of the
 
 def _words(index):
     """A cache's own words, each handed out once: three of status (pinned host memory, which the device can write) and
-    two for its blocks' barriers (device memory), all zero."""
+    a 64-bit one for its blocks' barriers (device memory), all zero."""
     got = _slots.get(index)
     if got is None or got[2] == _SLOTS:
         got = [torch.zeros((_SLOTS, 4), dtype=torch.int32).pin_memory(),
-               torch.zeros((_SLOTS, 2), dtype=torch.int32, device=torch.device("cuda", index)), 0]
+               torch.zeros(_SLOTS, dtype=torch.int64, device=torch.device("cuda", index)), 0]
         torch.cuda.current_stream(index).synchronize()   # zero for a cache on any stream
         _slots[index] = got
     status, sync, at = got
