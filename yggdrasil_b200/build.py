@@ -1,4 +1,5 @@
-"""Build libygg_b200.so in-tree with nvcc for sm_100a (the library travels with the tree; nothing is JIT-compiled).
+"""Build libygg_b200.so in-tree with nvcc for sm_100a, and _ops.so, the operators' calls on torch tensors, with the C++
+compiler against torch's headers (both travel with the tree; nothing is JIT-compiled).
 
     python -m yggdrasil_b200.build [--verbose]
 """
@@ -15,6 +16,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libygg_b200.so"
+OPS = PKG / "_ops.so"
+OPS_SOURCE = CSRC / "ygg_torch.cpp"
 SOURCES = [CSRC / "ygg_load.cu", CSRC / "ygg_step.cu", CSRC / "ygg_coop.cu", CSRC / "ygg_grouped.cu",
            CSRC / "ygg_float.cu", CSRC / "ygg_logprobs.cu", CSRC / "ygg_linear.cu",
            CSRC / "ygg_pages.cu"]
@@ -33,17 +36,23 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def stale() -> bool:
-    if not LIB.exists():
+def stale(target: Path, sources) -> bool:
+    if not target.exists():
         return True
-    t = LIB.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
+    t = target.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in sources)
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile the library if a source is newer than it; returns its path."""
-    if not force and not stale():
-        return LIB
+    """Compile what a source is newer than; returns the library's path."""
+    if force or stale(LIB, SOURCES + HEADERS):
+        build_library(verbose)
+    if force or stale(OPS, [OPS_SOURCE, ROOT / "include" / "ygg_b200.h"]):
+        build_ops()
+    return LIB
+
+
+def build_library(verbose: bool) -> None:
     objs, procs = [], []
     tmp = PKG / "_build"
     tmp.mkdir(exist_ok=True)
@@ -60,11 +69,28 @@ def build(verbose: bool = False, force: bool = False) -> Path:
             raise RuntimeError(f"nvcc failed on {src.name}:\n{out}\n{err}")
         if verbose:
             print(err, file=sys.stderr)
-    cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *objs]
+    run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *objs], "link")
+
+
+def build_ops() -> None:
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    system = [x for d in (home / "include", home / "include" / "torch" / "csrc" / "api" / "include", cuda)
+              for x in ("-isystem", str(d))]
+    run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", str(ROOT / "include"), "-I", sysconfig.get_paths()["include"], *system,
+         str(OPS_SOURCE), "-o", str(OPS), "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+         "-lc10_cuda", "-lc10", "-L", str(PKG), "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN"], "the torch binding")
+
+
+def run(cmd, what: str) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    return LIB
+        raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

@@ -18,15 +18,10 @@ caller's to order.
 """
 from __future__ import annotations
 
-import ctypes
-
 import numpy as np
 import torch
 
-from . import _native
-from ._native import YggCache, check, ops
-from .inference import _raw_stream
-from .logprobs import _nothing
+from . import _native, _ops
 
 _SLOTS = 1024
 _slots: dict = {}   # device index -> [status words, sync words, how many of them are handed out]
@@ -50,24 +45,16 @@ class StateCache:
     def __init__(self, pages, table, length, refs):
         """Around tensors that hold a cache already (updated in place): pages (P, ...) of any type, table (S, M), length
         (S,) and refs (P,) int32, contiguous, on one CUDA device."""
-        if not isinstance(pages, torch.Tensor) or not pages.is_cuda or pages.dim() < 2 or not pages.is_contiguous() \
-                or pages.numel() == 0:
-            raise ValueError("pages must be a contiguous CUDA tensor (P, ...)")
-        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.numel() == 0:
-            raise ValueError("table must be an int32 tensor (streams, pages of a stream)")
-        count, (streams, m), index = pages.shape[0], table.shape, pages.get_device()
-        for t, shape in ((table, (streams, m)), (length, (streams,)), (refs, (count,))):
-            if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != shape \
-                    or t.get_device() != index or not t.is_contiguous():
-                raise ValueError(f"table, length and refs must be contiguous int32 tensors ({streams}, {m}), "
-                                 f"({streams},) and ({count},) on {pages.device}")
+        self._h = None
+        if isinstance(pages, torch.Tensor) and pages.is_cuda:
+            self._status, self._sync, self._at = _words(pages.get_device())
+            self._h = _ops.cache(pages, table, length, refs, self._status.data_ptr() + 16 * self._at,
+                                 self._sync.data_ptr() + 8 * self._at)
+        if self._h is None:
+            raise ValueError("a cache needs contiguous tensors on one CUDA device: pages (P, ...), table (S, M) int32, "
+                             "length (S,) int32 and refs (P,) int32")
         self.pages, self.table, self.length, self.refs = pages, table, length, refs
-        self.device, self._dix, self._sizes = pages.device, index, {}
-        self._status, self._sync, self._at = _words(index)
-        self._c = YggCache(pages.data_ptr(), count, pages.numel() // count * pages.element_size(), table.data_ptr(),
-                           streams, m, length.data_ptr(), refs.data_ptr(), self._status.data_ptr() + 16 * self._at,
-                           self._sync.data_ptr() + 8 * self._at)
-        self._ref = ctypes.byref(self._c)
+        self.device = pages.device
 
     @classmethod
     def empty(cls, pages, streams, per_stream=1, like=None, shape=None, dtype=None, device=None):
@@ -87,8 +74,6 @@ class StateCache:
     def _ids(self, ids, what, limit):
         """Indices as a contiguous int32 tensor on the device; host indices are range-checked (negative: padding)."""
         if isinstance(ids, torch.Tensor) and ids.is_cuda:
-            if ids.dtype is torch.int32 and ids.dim() == 1 and ids.get_device() == self._dix and ids.is_contiguous():
-                return ids
             if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64) or ids.device != self.device:
                 raise ValueError(f"{what} must be a row of int32 or int64 on {self.device}")
             return (ids if ids.dtype == torch.int32 else ids.clamp(-1, 2 ** 31 - 1).int()).contiguous()
@@ -99,90 +84,59 @@ class StateCache:
             raise ValueError(f"{what}: {int(host.max())} out of range [0, {limit})")
         return torch.as_tensor(np.ascontiguousarray(host, np.int32)).to(self.device)
 
-    def _on(self):
-        return _nothing if self._dix == torch.cuda.current_device() else torch.cuda.device(self._dix)
-
-    def _workspace(self, n):
-        size = self._sizes.get(n)
-        if size is None:
-            size = self._sizes[n] = ops().ygg_cache_workspace(self._ref, n)
-        return torch.empty(size, dtype=torch.uint8, device=self.device), size
-
-    def _plan(self, parents, children, depth):
-        with self._on():
-            n = parents.shape[0]
-            ws, size = self._workspace(n)
-            code = ops().ygg_cache_fork(self._dix, self._ref, n, parents.data_ptr(),
-                                        None if children is None else children.data_ptr(),
-                                        None if depth is None else depth.data_ptr(), ws.data_ptr(), size,
-                                        _raw_stream(self._dix))
-            if code:
-                check(code, "ygg_cache_fork")
+    def _streams(self, ids, what="streams"):
+        return self._ids(ids, what, self.table.shape[0])
 
     def fork(self, parents, children, depth=None):
         """Stream children[i], which must hold no pages, goes on from parents[i]: it shares the parent's pages but the
         last, which is copied into a new page. depth[i]: only the parent's first depth[i] pages (at least 1), so that
         the child goes on from an earlier snapshot. A parent without pages leaves its child without."""
-        p = self._ids(parents, "parents", self._c.streams)
-        c = self._ids(children, "children", self._c.streams)
-        d = None if depth is None else self._ids(depth, "depth", 1 << 31)
-        if p.shape != c.shape or (d is not None and d.shape != p.shape):
-            raise ValueError("one child, and one depth, for each parent")
-        self._plan(p, c, d)
+        if children is None or _ops.cache_fork(self._h, parents, children, depth) is None:
+            p, c = self._streams(parents, "parents"), self._streams(children, "children")
+            d = None if depth is None else self._ids(depth, "depth", 1 << 31)
+            if p.shape != c.shape or (d is not None and d.shape != p.shape):
+                raise ValueError("one child, and one depth, for each parent")
+            _ops.cache_fork(self._h, p, c, d)
 
     def grow(self, streams):
         """Each stream gets one more page, a copy of its last (zeros for its first); the page before it stays as a
         snapshot."""
-        self._plan(self._ids(streams, "streams", self._c.streams), None, None)
+        if _ops.cache_fork(self._h, streams, None, None) is None:
+            _ops.cache_fork(self._h, self._streams(streams), None, None)
 
     def free(self, streams):
         """The streams let go of their pages; pages that nothing holds any more are free."""
-        s = self._ids(streams, "streams", self._c.streams)
-        with self._on():
-            check(ops().ygg_cache_free(self._dix, self._ref, s.shape[0], s.data_ptr(),
-                                       _raw_stream(self._dix)), "ygg_cache_free")
+        if _ops.cache_free(self._h, streams) is None:
+            _ops.cache_free(self._h, self._streams(streams))
 
     def compact(self):
         """Moves the live pages to the front and renumbers the tables. Returns their number as an int32 tensor () on the
         device: pages[:live] is one contiguous batch."""
-        with self._on():
-            live = torch.empty((), dtype=torch.int32, device=self.device)
-            ws, size = self._workspace(0)
-            code = ops().ygg_cache_compact(self._dix, self._ref, live.data_ptr(), ws.data_ptr(), size,
-                                           _raw_stream(self._dix))
-            if code:
-                check(code, "ygg_cache_compact")
-        return live
+        return _ops.cache_compact(self._h)
 
     def read(self, streams):
         """The live states of streams as a new batch (len(streams), ...); zeros for a stream without pages."""
-        s = self._ids(streams, "streams", self._c.streams)
-        with self._on():
-            batch = torch.empty((s.shape[0], *self.pages.shape[1:]), dtype=self.pages.dtype, device=self.device)
-            check(ops().ygg_cache_read(self._dix, self._ref, s.shape[0], s.data_ptr(), batch.data_ptr(),
-                                       _raw_stream(self._dix)), "ygg_cache_read")
-        return batch
+        batch = _ops.cache_read(self._h, streams)
+        return batch if batch is not None else _ops.cache_read(self._h, self._streams(streams))
 
     def write(self, streams, batch):
         """batch[i] becomes the live state of streams[i], a stream that holds pages; no stream named twice."""
-        s = self._ids(streams, "streams", self._c.streams)
-        if not isinstance(batch, torch.Tensor) or batch.dtype != self.pages.dtype or batch.device != self.device \
-                or batch.shape != (s.shape[0], *self.pages.shape[1:]):
-            raise ValueError(f"batch must be {self.pages.dtype} {(s.shape[0], *self.pages.shape[1:])} on {self.device}")
-        b = batch.contiguous()
-        with self._on():
-            check(ops().ygg_cache_write(self._dix, self._ref, s.shape[0], s.data_ptr(), b.data_ptr(),
-                                        _raw_stream(self._dix)), "ygg_cache_write")
+        if _ops.cache_write(self._h, streams, batch) is None:
+            s = self._streams(streams)
+            want = (s.shape[0], *self.pages.shape[1:])
+            if not isinstance(batch, torch.Tensor) or batch.dtype != self.pages.dtype or batch.device != self.device \
+                    or batch.shape != want:
+                raise ValueError(f"batch must be {self.pages.dtype} {want} on {self.device}")
+            _ops.cache_write(self._h, s, batch.contiguous())
 
     def copy(self, source, target):
         """Page target[i] becomes a copy of page source[i]; a target is named once, and is no source of the call."""
-        a = self._ids(source, "source", self._c.page_count)
-        b = self._ids(target, "target", self._c.page_count)
-        if a.shape != b.shape:
-            raise ValueError("one target for each source")
-        with self._on():
-            check(ops().ygg_cache_copy(self._dix, self._ref, a.shape[0], a.data_ptr(), b.data_ptr(),
-                                       _raw_stream(self._dix)), "ygg_cache_copy")
+        if _ops.cache_copy(self._h, source, target) is None:
+            count = self.pages.shape[0]
+            a, b = self._ids(source, "source", count), self._ids(target, "target", count)
+            if a.shape != b.shape:
+                raise ValueError("one target for each source")
+            _ops.cache_copy(self._h, a, b)
 
     def status(self, clear=True):
         """Raise if a call since the last clear met a bad index (ValueError) or had no page or table entry left
