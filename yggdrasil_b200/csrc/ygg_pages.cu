@@ -117,8 +117,13 @@ __device__ __forceinline__ int block_count(bool v, int *scratch, int &before) {
     before = __popc(who & ((1u << lane) - 1)) + (warp ? __shfl_sync(~0u, w, warp - 1) : 0);
     return __shfl_sync(~0u, w, 31);
 }
-// The sum of the blocks' counts, and of those before this block. Counts come from other blocks: past the L1.
-__device__ __forceinline__ int over_blocks(const int *counts, int *scratch, int &before) {
+// The sum of the blocks' counts (`own`: this block's), and of those before this block. They come from other blocks: past
+// the L1.
+__device__ __forceinline__ int over_blocks(const int *counts, int own, int *scratch, int &before) {
+    if (gridDim.x == 1) {
+        before = 0;
+        return own;
+    }
     int total;
     const int mine = threadIdx.x < gridDim.x ? __ldcg(counts + threadIdx.x) : 0;
     const int at = block_scan(mine, scratch, total);
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(kPlan, 1)
 
     const int32_t claim0 = taken0 >= 0 ? __ldcg(slot(child0, taken0)) : 0;   // its load runs under the free pages' list
     int free_before;
-    const int available = over_blocks(free_counts, scratch, free_before);
+    const int available = over_blocks(free_counts, free_here, scratch, free_before);
     for (int64_t p0 = pages.from; p0 < pages.to && free_before < n; p0 += kPlan) {
         const int64_t p = p0 + threadIdx.x;
         const bool is_free = p0 == pages.from ? free0 : p < pages.to && c.refs[p] == 0;
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kPlan, 1)
     if (!blocks.meet()) return;
 
     int given;
-    over_blocks(held_counts, scratch, given);
+    over_blocks(held_counts, held, scratch, given);
     for (int64_t i0 = mine.from; i0 < mine.to; i0 += kPlan) {
         const int64_t i = i0 + threadIdx.x;
         const bool first = i0 == mine.from;
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kPlan, 1)
     if (threadIdx.x == 0) counts[blockIdx.x] = here;
     if (!blocks.meet()) return;
 
-    const int n = over_blocks(counts, scratch, rank0);
+    const int n = over_blocks(counts, here, scratch, rank0);
     int *const below = counts + kMaxBlocks;   // the live pages below n
     if (threadIdx.x == 0 && n == c.count && blockIdx.x == 0) *below = n;
     for (int64_t p0 = pages.from; p0 < pages.to; p0 += kPlan) {
