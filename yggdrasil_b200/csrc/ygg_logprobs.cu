@@ -197,38 +197,40 @@ __device__ __forceinline__ Pair pair_of(const uint4 &q, int i, __half) {
     return pair(f.x, f.y);
 }
 
-// Adds the entries of vectors to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN; it
-// is rare, so the sum says whether there was one, and only then the products are formed again with y cut off.
-template <typename T, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const uint4 (&q)[RUNS]) {
+// Adds the entries of vectors to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN. Most
+// rows have none, so that the first NaN of the sum says that this one has (`masked`), and from then on y is cut off.
+template <typename T, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const uint4 (&q)[RUNS], bool &masked) {
     constexpr int N = kPer<T>;
     const float m = a.m == -INFINITY ? 0.0f : a.m;
     const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e);
     Pair s = 0, t = 0;
+    if (!masked) {
 #pragma unroll
-    for (int r = 0; r < RUNS; r++)
+        for (int r = 0; r < RUNS; r++)
 #pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const Pair y = add(pair_of(q[r], i, T()), minus), e = exp2_approx(mul(y, l));
-            s = add(s, e);
-            t = fma(e, y, t);
-        }
-    const float2 sf = split(s), tf = split(t);
-    float sum = tf.x + tf.y;
-    if (sum != sum) {
-        sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < RUNS; r++) {
-            float v[N];
-            unpack(q[r], v, T());
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float y = v[i] - m;
-                sum = fmaf(exp2_approx(y * kLog2e), fmaxf(y, kFloor), sum);
+            for (int i = 0; i < N / 2; i++) {
+                const Pair y = add(pair_of(q[r], i, T()), minus), e = exp2_approx(mul(y, l));
+                s = add(s, e);
+                t = fma(e, y, t);
             }
-        }
+        const float2 f = split(t);
+        masked = f.x + f.y != f.x + f.y;
     }
+    if (masked) {
+        s = 0, t = 0;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++)
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                const float2 f = split(add(pair_of(q[r], i, T()), minus));
+                const Pair e = exp2_approx(mul(pair(f.x, f.y), l));   // of y itself, which keeps NaN
+                s = add(s, e);
+                t = fma(e, pair(fmaxf(f.x, kFloor), fmaxf(f.y, kFloor)), t);
+            }
+    }
+    const float2 sf = split(s), tf = split(t);
     a.s += sf.x + sf.y;
-    a.t += sum;
+    a.t += tf.x + tf.y;
 }
 
 using Key = unsigned long long;   // orders entries: value above, then the lower index
@@ -316,7 +318,8 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
         a.m = fmaxf(a.m, v[i]);
     }
     const uint4 q[2] = {pack({v[0], v[1], v[2], v[3]}, 0.0f), pack({v[4], v[5], v[6], v[7]}, 0.0f)};
-    add_entries<float>(a, q);
+    bool masked = false;
+    add_entries<float>(a, q, masked);
     const Ends e(a);
     write_row(p, row, x, a, e);
     if (p.top == 0) return;
@@ -353,6 +356,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     const int64_t row0 = ((int64_t)blockIdx.x * kShortWarps + warp) * R;
     if (row0 >= p.rows) return;
     const unsigned below = (1u << lane) - 1;
+    bool masked = false;
     float ms[R], sums[2 * R];
     int found[R];
 #pragma unroll
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
             for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
         const int mine = order(most);
         Sums a{unorder(__reduce_max_sync(~0u, mine)), 0.0f, 0.0f};
-        add_entries<T>(a, q);
+        add_entries<T>(a, q, masked);
         ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
         found[w] = 0;
         if (p.top == 0) continue;
@@ -580,6 +584,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     const uint32_t off = offset_of(x), span = (32u * N) << shift, end = (uint32_t)p.vocab + off;
     const T *from = x - off;
     Sums a = none();
+    bool masked = false;
     const int w = rank * WARPS + warp, warps = cluster * WARPS;
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
     const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
@@ -605,7 +610,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
                 most = fmaxf(most, t);
             }
             if (most > a.m) raise(a, most);
-            add_entries<T>(a, q);
+            add_entries<T>(a, q, masked);
         }
         if (p.top) {
             if (shift) {
