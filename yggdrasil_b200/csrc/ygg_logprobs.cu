@@ -197,37 +197,22 @@ __device__ __forceinline__ Pair pair_of(const uint4 &q, int i, __half) {
     return pair(f.x, f.y);
 }
 
-// Adds the entries of vectors to sums whose m is at least the largest of them. An entry of -inf has e = 0 and e y = NaN. Most
-// rows have none, so that the first NaN of the sum says that this one has (`masked`), and from then on y is cut off.
-template <typename T, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const uint4 (&q)[RUNS], bool &masked) {
+// Adds the entries of vectors to sums whose m is at least the largest of them. y is cut off for the product alone: an entry of
+// -inf has e = 0, and 0 times its y would be NaN (looking for NaN and going back instead cost 4 to 16 % more).
+template <typename T, int RUNS> __device__ __forceinline__ void add_entries(Sums &a, const uint4 (&q)[RUNS]) {
     constexpr int N = kPer<T>;
     const float m = a.m == -INFINITY ? 0.0f : a.m;
     const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e);
     Pair s = 0, t = 0;
-    if (!masked) {
 #pragma unroll
-        for (int r = 0; r < RUNS; r++)
+    for (int r = 0; r < RUNS; r++)
 #pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-                const Pair y = add(pair_of(q[r], i, T()), minus), e = exp2_approx(mul(y, l));
-                s = add(s, e);
-                t = fma(e, y, t);
-            }
-        const float2 f = split(t);
-        masked = f.x + f.y != f.x + f.y;
-    }
-    if (masked) {
-        s = 0, t = 0;
-#pragma unroll
-        for (int r = 0; r < RUNS; r++)
-#pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-                const float2 f = split(add(pair_of(q[r], i, T()), minus));
-                const Pair e = exp2_approx(mul(pair(f.x, f.y), l));   // of y itself, which keeps NaN
-                s = add(s, e);
-                t = fma(e, pair(fmaxf(f.x, kFloor), fmaxf(f.y, kFloor)), t);
-            }
-    }
+        for (int i = 0; i < N / 2; i++) {
+            const Pair y = add(pair_of(q[r], i, T()), minus), e = exp2_approx(mul(y, l));
+            const float2 f = split(y);
+            s = add(s, e);
+            t = fma(e, pair(fmaxf(f.x, kFloor), fmaxf(f.y, kFloor)), t);
+        }
     const float2 sf = split(s), tf = split(t);
     a.s += sf.x + sf.y;
     a.t += tf.x + tf.y;
@@ -257,13 +242,18 @@ struct Ends {
     }
     __device__ __forceinline__ float logprob(float x) const { return empty ? -INFINITY : (x - m) - ls; }
 };
-template <typename T>
-__device__ __forceinline__ void write_row(const Rows &p, int64_t row, const T *x, const Sums &a, const Ends &e) {
-    const int64_t t = token_of(p.tokens, p.token_bytes, row);
-    float lp = 0.0f;
-    if (t >= p.vocab) lp = NAN;
-    else if (t >= 0) lp = e.logprob(to_f(x[t]));
-    p.logprob[row] = lp;
+// The given token of a row and its logit; loaded before the row's sums are known, so that they do not wait for it.
+struct Given {
+    float x = 0.0f;
+    int kind = 0;   // 0: padding, 1: a token, 2: one beyond the vocabulary
+    template <typename T> __device__ __forceinline__ void load(const Rows &p, int64_t row, const T *logits) {
+        const int64_t t = token_of(p.tokens, p.token_bytes, row);
+        kind = t >= p.vocab ? 2 : t >= 0;
+        if (kind == 1) x = to_f(logits[t]);
+    }
+};
+__device__ __forceinline__ void write_row(const Rows &p, int64_t row, const Given &given, const Sums &a, const Ends &e) {
+    p.logprob[row] = given.kind == 0 ? 0.0f : given.kind == 1 ? e.logprob(given.x) : NAN;
     p.entropy[row] = e.h;
     p.lse[row] = e.m + e.ls;
     if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? INFINITY : log2f(a.s), e.empty ? 0.0f : e.ls, e.h);
@@ -318,10 +308,11 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
         a.m = fmaxf(a.m, v[i]);
     }
     const uint4 q[2] = {pack({v[0], v[1], v[2], v[3]}, 0.0f), pack({v[4], v[5], v[6], v[7]}, 0.0f)};
-    bool masked = false;
-    add_entries<float>(a, q, masked);
+    add_entries<float>(a, q);
     const Ends e(a);
-    write_row(p, row, x, a, e);
+    Given given;
+    given.load(p, row, x);
+    write_row(p, row, given, a, e);
     if (p.top == 0) return;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -356,9 +347,10 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     const int64_t row0 = ((int64_t)blockIdx.x * kShortWarps + warp) * R;
     if (row0 >= p.rows) return;
     const unsigned below = (1u << lane) - 1;
-    bool masked = false;
     float ms[R], sums[2 * R];
     int found[R];
+    Given given;   // lane l serves row l mod R
+    if (lane < R && row0 + lane < p.rows) given.load(p, row0 + lane, (const T *)p.logits + (row0 + lane) * p.stride);
 #pragma unroll
     for (int w = 0; w < R; w++) {
         const int64_t row = min(row0 + w, p.rows - 1);   // rows past the last are the last once more, unseen
@@ -379,7 +371,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
             for (int i = 0; i < N; i++) most = fmaxf(most, v[r][i]);
         const int mine = order(most);
         Sums a{unorder(__reduce_max_sync(~0u, mine)), 0.0f, 0.0f};
-        add_entries<T>(a, q, masked);
+        add_entries<T>(a, q);
         ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
         found[w] = 0;
         if (p.top == 0) continue;
@@ -515,7 +507,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     const Ends e(a);
     const int64_t row = row0 + mine;
     if (row >= p.rows) n = 0;
-    if (lane < R && row < p.rows) write_row(p, row, (const T *)p.logits + row * p.stride, a, e);
+    if (lane < R && row < p.rows) write_row(p, row, given, a, e);
     __syncwarp();
     if (p.top == 0) return;
     // ranks by the values alone; ties give ranks twice, which shows in the ranks' sum, and then the indices count too
@@ -583,8 +575,10 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     const T *x = (const T *)p.logits + row * p.stride;
     const uint32_t off = offset_of(x), span = (32u * N) << shift, end = (uint32_t)p.vocab + off;
     const T *from = x - off;
+    constexpr int kJoin = WARPS > 1;   // the warp that joins the sums
+    Given given;
+    if (rank == 0 && warp == kJoin && lane == 0) given.load(p, row, x);
     Sums a = none();
-    bool masked = false;
     const int w = rank * WARPS + warp, warps = cluster * WARPS;
     // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
     const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
@@ -610,7 +604,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
                 most = fmaxf(most, t);
             }
             if (most > a.m) raise(a, most);
-            add_entries<T>(a, q, masked);
+            add_entries<T>(a, q);
         }
         if (p.top) {
             if (shift) {
@@ -650,15 +644,15 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
         if (rank) return;
     }
     __syncthreads();
-    if (warp == (WARPS > 1)) {   // the sums, while the first warp looks for the best segments
+    if (warp == kJoin) {   // the sums, while the first warp looks for the best segments
         a = lane < warps ? sh.part[lane] : none();
         if (lane + 32 < warps) join(a, sh.part[lane + 32]);
 #pragma unroll
         for (int o = 16; o; o >>= 1)
             join(a, Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)});
         if (lane == 0) {
-            write_row(p, row, x, a, Ends(a));
             sh.all = a;
+            write_row(p, row, given, a, Ends(a));
         }
     }
     if (p.top == 0) return;
@@ -735,7 +729,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
         for (int i = 0; i < N; i++) {
             const uint32_t u = u0 + lane * N + i;
             if (!(v[i] < bound) && u - off < end - off) {
-                const int at = atomicAdd(&sh.count, 1);   // the order in the list does not matter: the keys rank
+                const int at = atomicAdd(&sh.count, 1);
                 if (at < kKeys) sh.keys[at] = key_of(v[i], u - off);
             }
         }
@@ -884,7 +878,7 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
 struct RowGrad {
     float m, l2, A, B, given;
     int64_t token;   // -1: none
-    __device__ __forceinline__ RowGrad(const Grad &p, int64_t row) {
+    __device__ __forceinline__ void load(const Grad &p, int64_t row) {
         const float4 st = p.stats[row];
         token = token_of(p.tokens, p.token_bytes, row);
         if (token >= p.vocab) token = -1;
@@ -899,26 +893,15 @@ struct RowGrad {
         const float y = x - m;
         return exp2_approx(fmaf(y, kLog2e, -l2)) * fmaf(B, fmaxf(y, kFloor), A);
     }
-    // The same for a vector, in pairs. An entry of -inf gives NaN (p = 0 times infinity): then once more, with y cut off.
+    // The same for a vector, in pairs.
     template <int N> __device__ __forceinline__ void dense(float (&v)[N]) const {
         const Pair minus = pair(-m, -m), l = pair(kLog2e, kLog2e), s = pair(-l2, -l2), a = pair(A, A), b = pair(B, B);
-        Pair sum = 0, g[N / 2];
 #pragma unroll
         for (int i = 0; i < N / 2; i++) {
             const Pair y = add(pair(v[2 * i], v[2 * i + 1]), minus);
-            g[i] = mul(exp2_approx(fma(y, l, s)), fma(b, y, a));
-            sum = add(sum, g[i]);
-        }
-        const float2 f = split(sum);
-        if (f.x + f.y != f.x + f.y) {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = dense(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-                const float2 h = split(g[i]);
-                v[2 * i] = h.x, v[2 * i + 1] = h.y;
-            }
+            const float2 f = split(y);
+            const float2 g = split(mul(exp2_approx(fma(y, l, s)), fma(b, pair(fmaxf(f.x, kFloor), fmaxf(f.y, kFloor)), a)));
+            v[2 * i] = g.x, v[2 * i + 1] = g.y;
         }
     }
 };
@@ -927,50 +910,89 @@ __device__ __forceinline__ void store_stream(void *p, const uint4 &v) {
     asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// A warp per (row, chunk of kGradRuns runs of 32 kPer places). SAME: the logits and the gradient of a row lie alike to
-// the 16-byte boundary, so that both move 16 bytes at a time.
-constexpr int kGradRuns = 4;
-template <typename T, bool SAME> __global__ void __launch_bounds__(256) grad_kernel(const Grad p, unsigned chunks) {
-    constexpr int N = kPer<T>;
-    const int lane = threadIdx.x & 31;
-    const int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t row = it < ((int64_t)1 << 32) ? (unsigned)it / chunks : it / chunks;
+// Up to 8 entries: a thread a row.
+template <typename T> __global__ void __launch_bounds__(128) tiny_grad_kernel(const Grad p) {
+    const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
     if (row >= p.rows) return;
-    const uint32_t u0 = (uint32_t)(it - row * chunks) * (kGradRuns * 32 * N);
     const T *x = (const T *)p.logits + row * p.stride;
     T *g = (T *)p.grad + row * p.grad_stride;
-    const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
-    uint4 q[kGradRuns];
+    RowGrad d;
+    d.load(p, row);
+    float more[8] = {};
+    if (p.g_top)
+        for (int k = 0; k < p.top; k++) {
+            const int j = p.top_ids[row * p.top + k];
+            const float v = p.g_top[row * p.top + k];
 #pragma unroll
-    for (int r = 0; r < kGradRuns; r++) q[r] = load_run<T>(x - off, u0 + r * 32 * N, off, end, lane);
-    const RowGrad d(p, row);
-#pragma unroll
-    for (int r = 0; r < kGradRuns; r++) {
-        const uint32_t u = u0 + (r * 32 + lane) * N;
-        if (u >= end) break;
-        float v[N];
-        unpack(q[r], v, T());
-        d.dense(v);
-        if (SAME && u >= off && u + N <= end) {
-            store_stream(g + (int64_t)u - off, pack(v, T()));
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (u + i >= off && u + i < end) from_f(v[i], g[u + i - off]);
+            for (int i = 0; i < 8; i++) more[i] += i == j ? v : 0.0f;
         }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < p.vocab) {
+            const float v = d.dense(to_f(x[i]));
+            from_f(d.l2 == INFINITY ? 0.0f : v + (i == d.token ? d.given : 0.0f) + more[i], g[i]);
+        }
+}
+
+// A warp takes kGradRuns runs of 32 kPer places: a chunk of one row, or ROWS short rows whole. SAME: the logits and the
+// gradient of a row lie alike to the 16-byte boundary, so that both move 16 bytes at a time.
+constexpr int kGradRuns = 4;
+template <typename T, bool SAME, int ROWS>
+__global__ void __launch_bounds__(256) grad_kernel(const Grad p, unsigned chunks) {
+    constexpr int N = kPer<T>, RUNS = kGradRuns / ROWS;
+    const int lane = threadIdx.x & 31;
+    const int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row0 = ROWS > 1 ? it * ROWS : it < ((int64_t)1 << 32) ? (unsigned)it / chunks : it / chunks;
+    if (row0 >= p.rows) return;
+    const uint32_t u0 = ROWS > 1 ? 0 : (uint32_t)(it - row0 * chunks) * (kGradRuns * 32 * N);
+    uint4 q[ROWS][RUNS];
+#pragma unroll
+    for (int w = 0; w < ROWS; w++) {
+        const int64_t row = min(row0 + w, p.rows - 1);
+        const T *x = (const T *)p.logits + row * p.stride;
+        const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++) q[w][r] = load_run<T>(x - off, u0 + r * 32 * N, off, end, lane);
     }
-    __syncwarp();
-    // the given token and the alternatives: written again, whole, so that they are rounded once
-    if (d.l2 == INFINITY) return;   // an empty row
-    const int64_t j0 = (int64_t)u0 - off, j1 = min(j0 + kGradRuns * 32 * N, p.vocab);
-    for (int q = lane; q <= (p.g_top ? p.top : 0); q += 32) {
-        const int64_t j = q == 0 ? d.token : p.top_ids[row * p.top + q - 1];
-        if (j < 0 || j < j0 || j >= j1 || (q > 0 && j == d.token)) continue;
-        float more = q == 0 ? d.given : p.g_top[row * p.top + q - 1];
-        if (q == 0 && p.g_top)
-            for (int k = 0; k < p.top; k++)
-                if (p.top_ids[row * p.top + k] == j) more += p.g_top[row * p.top + k];
-        from_f(d.dense(to_f(x[j])) + more, g[j]);
+    RowGrad ds[ROWS];
+#pragma unroll
+    for (int w = 0; w < ROWS; w++) ds[w].load(p, min(row0 + w, p.rows - 1));
+#pragma unroll
+    for (int w = 0; w < ROWS; w++) {
+        const int64_t row = row0 + w;
+        if (row >= p.rows) break;
+        const RowGrad &d = ds[w];
+        const T *x = (const T *)p.logits + row * p.stride;
+        T *g = (T *)p.grad + row * p.grad_stride;
+        const uint32_t off = offset_of(x), end = (uint32_t)p.vocab + off;
+#pragma unroll
+        for (int r = 0; r < RUNS; r++) {
+            const uint32_t u = u0 + (r * 32 + lane) * N;
+            if (u >= end) break;
+            float v[N];
+            unpack(q[w][r], v, T());
+            d.dense(v);
+            if (SAME && u >= off && u + N <= end) {
+                store_stream(g + (int64_t)u - off, pack(v, T()));
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (u + i - off < end - off) from_f(v[i], g[u + i - off]);
+            }
+        }
+        __syncwarp();
+        // the given token and the alternatives: written again, whole, so that they are rounded once
+        if (d.l2 == INFINITY) continue;   // an empty row
+        const int64_t j0 = (int64_t)u0 - off, j1 = min(j0 + RUNS * 32 * N, p.vocab);
+        for (int k = lane; k <= (p.g_top ? p.top : 0); k += 32) {
+            const int64_t j = k == 0 ? d.token : p.top_ids[row * p.top + k - 1];
+            if (j < 0 || j < j0 || j >= j1 || (k > 0 && j == d.token)) continue;
+            float more = k == 0 ? d.given : p.g_top[row * p.top + k - 1];
+            if (k == 0 && p.g_top)
+                for (int i = 0; i < p.top; i++)
+                    if (p.top_ids[row * p.top + i] == j) more += p.g_top[row * p.top + i];
+            from_f(d.dense(to_f(x[j])) + more, g[j]);
+        }
     }
 }
 
@@ -993,9 +1015,17 @@ template <typename T> cudaError_t launch_grad(const Grad &p, cudaStream_t st) {
         if (q.g_entropy) q.g_entropy += r;
         if (q.g_lse) q.g_lse += r;
         if (q.g_top) q.g_top += r * p.top;
-        const unsigned grid = (unsigned)((q.rows * chunks + 7) / 8);
-        if (same) grad_kernel<T, true><<<grid, 256, 0, st>>>(q, (unsigned)chunks);
-        else grad_kernel<T, false><<<grid, 256, 0, st>>>(q, (unsigned)chunks);
+        if (p.vocab <= 8) {
+            tiny_grad_kernel<T><<<(unsigned)((q.rows + 127) / 128), 128, 0, st>>>(q);
+            continue;
+        }
+        const int64_t runs = (places + 32 * N - 1) / (32 * N);
+        const int each = runs <= 1 ? 4 : runs <= 2 ? 2 : 1;   // rows a warp
+        const unsigned grid = (unsigned)(((q.rows + each - 1) / each * chunks + 7) / 8);
+        const auto launch = [&](auto k) { k<<<grid, 256, 0, st>>>(q, (unsigned)chunks); };
+        if (each == 4) launch(same ? grad_kernel<T, true, 4> : grad_kernel<T, false, 4>);
+        else if (each == 2) launch(same ? grad_kernel<T, true, 2> : grad_kernel<T, false, 2>);
+        else launch(same ? grad_kernel<T, true, 1> : grad_kernel<T, false, 1>);
     }
     return cudaGetLastError();
 }
