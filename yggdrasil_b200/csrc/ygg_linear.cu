@@ -765,12 +765,13 @@ int quantize(int dtype, const Quantize &p, cudaStream_t st) {
 
 // How a product is cut: CTAs a product, rows a tile, CTAs that share the K of a tile. The least of what the cuts are
 // expected to take, in ns, by a model fitted to sweeps on a B200 (us, measured):
-//   a launch costs 3200; 128 bytes of K of a tile 240, or its bytes at 115 a ns where those take longer (a pair of
-//   256 x 256: 410, bound by the tensor cores); the epilogue 8 a column, hidden under the next tile's products.
+//   a launch costs 2500; 128 bytes of K of a tile 240, or its bytes at 115 a ns where those take longer (a pair of
+//   256 x 256: 410, bound by the tensor cores); the epilogue 550 and 9 a column (a pair 3600), bound by its stores, under
+//   the next tile's products.
 //   512 x 4096 x 4096: tn 128 12.1, 256 15.6; 1024 x 4096 x 4096: tn 256 16.0, 128 20.5;
-//   8192 x 4096 x 16384: pair 370, one CTA 410.
-//   Sharing K costs 2200 and 25 a column: 16 x 4096 x 4096 8.0 with 4 parts, 11.0 with one; 512 x 1024 x 4096 (tn 256) 15.5
-//   with two, 7.2 with one.
+//   8192 x 4096 x 16384: pair 345, one CTA 393; 4096 x 64 x 16384: tn 256 42.1, 128 49.7, 32 105.9, pair 51.2.
+//   Sharing K costs 1650 and 16 a column more: 16 x 4096 x 4096 8.0 with 4 parts, 11.0 with one; 512 x 1024 x 4096
+//   (tn 256) 15.5 with two, 7.2 with one.
 struct Shape { int ctas, tn, parts; };
 Shape shape_for(int64_t rows, int64_t n, int k) {
     const int64_t sms = sm_count(), k_blocks = (k + kStageK - 1) / kStageK, channel_blocks = (n + 127) / 128;
@@ -780,8 +781,9 @@ Shape shape_for(int64_t rows, int64_t n, int k) {
         const int64_t tiles = (channel_blocks + ctas - 1) / ctas * ((rows + tn - 1) / tn);
         if (parts > 1 && tiles * parts > sms) return;
         const int64_t waves = (tiles * ctas * parts + sms - 1) / sms;
-        const int64_t block = ctas == 2 ? 410 : std::max(240, (128 + tn) * kStageK / 115), epilogue = 8 * tn;
-        int64_t t = 3200 + (k_blocks + parts - 1) / parts * block + epilogue + (parts > 1 ? 2200 + 17 * tn : 0);
+        const int64_t block = ctas == 2 ? 410 : std::max(240, (128 + tn) * kStageK / 115);
+        const int64_t epilogue = ctas == 2 ? 3600 : 550 + 9 * tn;
+        int64_t t = 2500 + (k_blocks + parts - 1) / parts * block + epilogue + (parts > 1 ? 1650 + 16 * tn : 0);
         t += (waves - 1) * std::max(k_blocks * block, epilogue);
         if (t < least) {
             least = t;
@@ -790,7 +792,7 @@ Shape shape_for(int64_t rows, int64_t n, int k) {
     };
     const int64_t row_blocks = (rows + 255) / 256;
     const int even = (int)((rows + row_blocks - 1) / row_blocks + 15) / 16 * 16;   // the rows in equal tiles
-    for (const int tn : {even, 16, 32, 64, 128, 192, 256})
+    for (const int tn : {even, 16, 32, 64, 128, 256})
         if (tn == even || tn < even || rows > 256)
             for (int parts = 1; parts <= 8 && parts <= k_blocks; parts *= 2) consider(1, tn, parts);
     if (rows > 256) consider(2, 256, 1);
