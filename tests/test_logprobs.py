@@ -412,3 +412,15 @@ def test_gradient_of_the_alternatives_alone_and_of_float64_arrivals():
     out = op()(b, t, top=3)
     (out.top_logprobs.double() * g.double()).sum().backward()
     assert torch.equal(a.grad, b.grad) and a.grad.shape == x.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,step", [(1100, 128), (8192, 512), (8192, 1024), (32768, 1024), (32768, 4096), (120000, 16384)])
+def test_best_entries_a_fixed_step_apart(vocab, step, dtype):
+    """The best entries lie `step` apart, in few of the bins that a bound is taken from, alone or with a tie of most others."""
+    x, t = make(6, vocab, dtype, seed=41)
+    x = torch.where(torch.arange(vocab, device="cuda") % step < 8, x + 50, x)
+    x[3:] = torch.where(x[3:] > 30, x[3:], torch.tensor(1.0, device="cuda", dtype=dtype))
+    for top in (1, 9, 20, 33, 64):
+        check_values(x, t, top, op()(x, t, top=top))

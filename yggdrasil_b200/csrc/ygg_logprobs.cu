@@ -533,25 +533,28 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     }
 }
 
-// Long rows: a cluster of up to 8 blocks a row. The row is cut into segments of 32 kPer << shift entries, given to the
-// warps of the cluster in turn; a warp keeps its running sums and leaves the largest value of each segment. The first
-// block joins the sums. Alternatives: the k largest segments by (largest value, lower segment) hold the k best entries,
-// since any other entry has k better ones, one in each of them. They are read again, and the entries at or above the
-// k-th segment's largest value are ranked by counting. If they are more than a block has threads (ties, masks, sorted
-// rows), a second bound from the threads' best entries leaves fewer; if those are still more, they are taken one at a
-// time.
+// Long rows: a cluster of up to 8 blocks a row. The row is cut into segments of 2^lg vectors of 16 bytes, 512 to 1024 of
+// them (fewer in rows of fewer vectors), and the warps of the cluster take runs of 32 vectors in turn; a warp keeps its
+// running sums and leaves the largest value of each segment. The first block joins the sums. Alternatives: the k-th
+// largest of 128 bins' maxima (bin b: the segments b mod 128) bounds the k-th best entry from below, so the segments that
+// reach it hold the k best entries: about 22 for 20, which are read again, and the entries that reach it are ranked by
+// counting. Where ties at the bound make the segments too many, the equal ones beyond the k-th are left out, in the order
+// of their indices. If the entries are too many (ties, masks, sorted rows), a second bound from the threads' best entries
+// leaves fewer; if those are still more, they are taken one at a time.
 // (Loading a warp's next batch while one is added up costs the registers of a block an SM and gained nothing: 8192 x 32768
 // bf16 136 us with, 117 without, 7 x 100003 bf16 9.5 and 9.4.)
-constexpr int kMaxSegments = 4096, kMaxCluster = 8, kBatch = 4, kKeys = 256;
+constexpr int kMaxSegments = 1024, kBins = 128, kMaxCluster = 8, kBatch = 4, kKeys = 256;
+// segments above the bound: at most 63 bins' worth
+constexpr int kMost = (YGG_TOP_MAX - 1) * (kMaxSegments / kBins);
 
 template <int WARPS> struct LongShared {
     Sums part[kMaxCluster * WARPS];   // in the first block
     Sums all;
-    int picked[YGG_TOP_MAX];          // segments
+    uint16_t picked[kMost];           // segments
     Key keys[kKeys];
     Key best[WARPS];
-    int count, bound;
-    int segment[];                    // order() of the segments' largest values; in the first block of all
+    int count, picks, bound;
+    alignas(16) int segment[];        // order() of the segments' largest values; in the first block of all
 };
 
 __device__ __forceinline__ uint32_t shared_at(const void *p, uint32_t rank) {
@@ -564,7 +567,7 @@ __device__ __forceinline__ void put_remote(uint32_t at, uint32_t v) {
 }
 
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int cluster, int shift, int segments) {
+__global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int cluster, int lg, int segments) {
     constexpr int N = kPer<T>, kThreads = WARPS * 32;
     extern __shared__ __align__(16) uint8_t raw[];
     LongShared<WARPS> &sh = *(LongShared<WARPS> *)raw;
@@ -573,6 +576,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     const int rank = blockIdx.x - (int)row * cluster;
     if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // the first block runs
     const T *x = (const T *)p.logits + row * p.stride;
+    const int shift = max(lg - 5, 0);
     const uint32_t off = offset_of(x), span = (32u * N) << shift, end = (uint32_t)p.vocab + off;
     const T *from = x - off;
     constexpr int kJoin = WARPS > 1;   // the warp that joins the sums
@@ -580,8 +584,9 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     if (rank == 0 && warp == kJoin && lane == 0) given.load(p, row, x);
     Sums a = none();
     const int w = rank * WARPS + warp, warps = cluster * WARPS;
-    // batches of runs: with shift 0 of kBatch segments, else of kBatch runs of one segment (2^shift is then >= kBatch)
-    const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch;
+    // batches of kBatch runs: with shift of one segment (2^shift is then >= kBatch), else of 2^(5 - lg) segments a run
+    const int steps = shift ? 1 << (shift - 2) : 1, per = shift ? 1 : kBatch, cut = shift ? 0 : 5 - lg;
+    const int units = segments >> cut;
     const auto load = [&](uint4(&q)[kBatch], uint32_t u0) {
         if (u0 >= off && u0 + kBatch * 32 * N <= end) {   // inside the row
 #pragma unroll
@@ -591,7 +596,7 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
             for (int b = 0; b < kBatch; b++) q[b] = load_run<T>(from, u0 + b * 32 * N, off, end, lane);
         }
     };
-    for (int g0 = w * per; g0 < segments; g0 += warps * per) {
+    for (int g0 = w * per; g0 < units; g0 += warps * per) {
         float top_of[kBatch];
         for (int step = 0; step < steps; step++) {
             uint4 q[kBatch];
@@ -606,18 +611,27 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
             if (most > a.m) raise(a, most);
             add_entries<T>(a, q);
         }
-        if (p.top) {
-            if (shift) {
-                const float t = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
-                const int best = __reduce_max_sync(~0u, order(t));
-                if (lane == 0) sh.segment[g0] = best;
-            } else {
+        if (p.top == 0) continue;
+        if (shift) {
+            const float t = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+            const int best = __reduce_max_sync(~0u, order(t));
+            if (lane == 0) sh.segment[g0] = best;
+        } else if (lg == 5) {
 #pragma unroll
-                for (int b = 0; b < kBatch; b++) {
-                    const int best = __reduce_max_sync(~0u, order(top_of[b]));
-                    if (lane == 0 && g0 + b < segments) sh.segment[g0 + b] = best;
-                }
+            for (int b = 0; b < kBatch; b++) {
+                const int best = __reduce_max_sync(~0u, order(top_of[b]));
+                if (lane == 0) sh.segment[g0 + b] = best;
             }
+        } else {
+            int best[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) best[b] = order(top_of[b]);
+            for (int o = 1; o < 1 << lg; o <<= 1)
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) best[b] = max(best[b], __shfl_xor_sync(~0u, best[b], o));
+            if ((lane & ((1 << lg) - 1)) == 0)
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) sh.segment[((g0 + b) << cut) + (lane >> lg)] = best[b];
         }
     }
 #pragma unroll
@@ -635,9 +649,10 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
             }
             if (p.top) {   // the warp's own segments
                 __syncwarp();
-                for (int g0 = w * per; g0 < segments; g0 += warps * per)
-                    if (lane < per && g0 + lane < segments)
-                        put_remote(shared_at(&sh.segment[g0 + lane], 0), (uint32_t)sh.segment[g0 + lane]);
+                for (int g0 = w * per; g0 < units; g0 += warps * per)
+                    for (int g = g0 << cut; g < (g0 + per) << cut; g += 32)
+                        if (g + lane < (g0 + per) << cut)
+                            put_remote(shared_at(&sh.segment[g + lane], 0), (uint32_t)sh.segment[g + lane]);
             }
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -657,123 +672,86 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     }
     if (p.top == 0) return;
 
-    // the best segments, by one warp; fewer segments than alternatives: all of them
-    const int picks = min(p.top, segments);
+    // the best segments, by one warp
     if (warp == 0) {
-        // the k-th largest of 64 bins' maxima bounds the k-th largest segment from below
-        int b0 = INT32_MIN, b1 = INT32_MIN;
-        for (int g = lane; g < segments; g += 64) {
-            b0 = max(b0, sh.segment[g]);
-            if (g + 32 < segments) b1 = max(b1, sh.segment[g + 32]);
+        int4 bin = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+        const auto each = [&](auto f) {   // four segments a lane
+            for (int g = lane * 4; g < segments; g += kBins) f(*(const int4 *)(sh.segment + g), g);
+        };
+        each([&](int4 v, int) {
+            bin = make_int4(max(bin.x, v.x), max(bin.y, v.y), max(bin.z, v.z), max(bin.w, v.w));
+        });
+        const int bound = kth_of_lanes(bin.x, bin.y, bin.z, bin.w, p.top);
+        if (lane == 0) sh.picks = sh.count = 0, sh.bound = bound;
+        __syncwarp();
+        const auto pick = [&](int least) {
+            const auto put = [&](int v, int g) {
+                if (v < least) return;
+                const int at = atomicAdd(&sh.picks, 1);
+                if (at < kMost) sh.picked[at] = (uint16_t)g;
+            };
+            each([&](int4 v, int g) { put(v.x, g), put(v.y, g + 1), put(v.z, g + 2), put(v.w, g + 3); });
+            __syncwarp();
+        };
+        pick(bound);
+        if (sh.picks > kMost) {
+            __syncwarp();
+            if (lane == 0) sh.picks = 0;
+            __syncwarp();
+            if (bound < INT32_MAX) pick(bound + 1);
+            int n = sh.picks;
+            for (int g0 = 0; g0 < segments && n < p.top; g0 += 32) {
+                const bool equal = g0 + lane < segments && sh.segment[g0 + lane] == bound;
+                const unsigned who = __ballot_sync(~0u, equal);
+                const int at = n + __popc(who & ((1u << lane) - 1));
+                if (equal && at < p.top) sh.picked[at] = (uint16_t)(g0 + lane);
+                n = min(p.top, n + __popc(who));
+            }
+            __syncwarp();
+            if (lane == 0) sh.picks = n;
         }
-        int bound = 0;
-        for (int i = 0; i < picks; i++) {
-            bound = __reduce_max_sync(~0u, max(b0, b1));
-            const unsigned who = __ballot_sync(~0u, max(b0, b1) == bound);
-            if (lane == __ffs(who) - 1) (b0 >= b1 ? b0 : b1) = INT32_MIN;
-        }
-        int n = 0;
-        for (int g0 = 0; g0 < segments; g0 += 32) {
-            const int g = g0 + lane;
-            const bool in = g < segments && sh.segment[g] >= bound;
-            const unsigned who = __ballot_sync(~0u, in);
-            const int at = n + __popc(who & ((1u << lane) - 1));
-            if (in && at < kKeys) sh.keys[at] = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
-            n += __popc(who);
-        }
-        if (lane == 0) sh.count = n;
     }
     __syncthreads();
     const Ends e(sh.all);
-    const int found = sh.count;
-    if (found <= kKeys) {
-        for (int k = threadIdx.x; k < found; k += kThreads) {
-            const Key key = sh.keys[k];
-            int above = 0;
-            for (int i = 0; i < found; i++) above += sh.keys[i] > key;
-            if (above < picks) {
-                sh.picked[above] = index_of(key);
-                if (above == picks - 1) sh.bound = order(value_of(key));
-            }
-        }
-    } else {   // many equal segments
-        Key last = ~0ull;
-        for (int k = 0; k < picks; k++) {
-            Key best = 0;
-            for (int g = threadIdx.x; g < segments; g += kThreads) {
-                const Key key = ((Key)((unsigned)sh.segment[g] ^ 0x80000000u) << 32) | (unsigned)~(unsigned)g;
-                if (key < last && key > best) best = key;
-            }
-            best = warp_max(best);
-            if (lane == 0) sh.best[warp] = best;
-            __syncthreads();
-            for (int i = 0; i < WARPS; i++) best = max(best, sh.best[i]);
-            last = best;
-            if (threadIdx.x == 0) {
-                sh.picked[k] = index_of(last);
-                sh.bound = order(value_of(last));
-            }
-            __syncthreads();
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
     const float bound = unorder(sh.bound);
-    const int runs = picks << shift;   // runs of 32 N entries in the picked segments
-    for (int q = picks < p.top ? runs : warp; q < runs; q += WARPS) {
-        const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
-        float v[N];
-        load_run<T>(from, u0, off, end, lane, v);
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t u = u0 + lane * N + i;
-            if (!(v[i] < bound) && u - off < end - off) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kKeys) sh.keys[at] = key_of(v[i], u - off);
-            }
-        }
-    }
-    __syncthreads();
-    int n = picks < p.top ? INT32_MAX : sh.count;   // fewer segments than alternatives: any entry may be one
-    if (n > kKeys && p.top <= kThreads) {
-        // ties, masks, sorted rows, or fewer segments than alternatives: the k-th best of the threads' best entries (by
-        // value and index) is a better bound
-        Key mine = 0;
-        for (int q = warp; q < runs; q += WARPS) {
-            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
+    const int vectors = sh.picks << lg;   // in the picked segments
+    // f(entry, its place) for the entries of the picked segments
+    const auto entries = [&](auto f) {
+        for (int q = threadIdx.x; q < vectors; q += kThreads) {
+            const uint32_t u0 = (((uint32_t)sh.picked[q >> lg] << lg) + (q & ((1 << lg) - 1))) * N;
             float v[N];
-            load_run<T>(from, u0, off, end, lane, v);
+            load_run<T>(from, u0, off, end, 0, v);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t u = u0 + lane * N + i;
-                if (u - off < end - off) mine = max(mine, key_of(v[i], u - off));
-            }
+            for (int i = 0; i < N; i++)
+                if (u0 + i - off < end - off) f(v[i], u0 + i - off);
         }
+    };
+    const auto keep = [&](Key key) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kKeys) sh.keys[at] = key;
+    };
+    entries([&](float v, uint32_t j) {
+        if (!(v < bound)) keep(key_of(v, j));
+    });
+    __syncthreads();
+    int n = sh.count;
+    if (n > kKeys && p.top <= kThreads) {
+        // ties, masks, sorted rows: the k-th best of the threads' best entries (by value and index) is a better bound
+        Key mine = 0;
+        entries([&](float v, uint32_t j) { mine = max(mine, key_of(v, j)); });
         __syncthreads();
         sh.keys[threadIdx.x] = mine;
+        if (threadIdx.x == 0) sh.count = 0, sh.best[0] = 0;
         __syncthreads();
         int above = 0;
         for (int i = 0; i < kThreads; i++) above += sh.keys[i] > mine;
-        __syncthreads();
-        if (threadIdx.x == 0) sh.count = 0;
         if (mine && above == p.top - 1) sh.best[0] = mine;
         __syncthreads();
         const Key least = sh.best[0];
-        for (int q = warp; q < runs; q += WARPS) {
-            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
-            float v[N];
-            load_run<T>(from, u0, off, end, lane, v);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t u = u0 + lane * N + i;
-                const Key key = u - off < end - off ? key_of(v[i], u - off) : 0;
-                if (key && key >= least) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kKeys) sh.keys[at] = key;
-                }
-            }
-        }
+        entries([&](float v, uint32_t j) {
+            const Key key = key_of(v, j);
+            if (key >= least) keep(key);
+        });
         __syncthreads();
         n = sh.count;
     }
@@ -789,17 +767,10 @@ __global__ void __launch_bounds__(WARPS * 32) long_kernel(const Rows p, int clus
     Key last = ~0ull;
     for (int k = 0; k < p.top; k++) {
         Key best = 0;
-        for (int q = warp; q < runs; q += WARPS) {
-            const uint32_t u0 = sh.picked[q >> shift] * span + (q & ((1 << shift) - 1)) * 32 * N;
-            float v[N];
-            load_run<T>(from, u0, off, end, lane, v);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t u = u0 + lane * N + i;
-                const Key key = u - off < end - off ? key_of(v[i], u - off) : 0;
-                if (key < last && key > best) best = key;
-            }
-        }
+        entries([&](float v, uint32_t j) {
+            const Key key = key_of(v, j);
+            if (key < last && key > best) best = key;
+        });
         best = warp_max(best);
         __syncthreads();
         if (lane == 0) sh.best[warp] = best;
@@ -819,7 +790,7 @@ int cluster_for(int64_t rows, int64_t runs, int sms) {
 }
 
 template <typename T, int WARPS>
-cudaError_t launch_long(const Rows &p, int cluster, int shift, int segments, cudaStream_t st) {
+cudaError_t launch_long(const Rows &p, int cluster, int lg, int segments, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p.rows * cluster));
     cfg.blockDim = dim3(WARPS * 32);
@@ -831,7 +802,7 @@ cudaError_t launch_long(const Rows &p, int cluster, int shift, int segments, cud
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1;
-    return cudaLaunchKernelEx(&cfg, long_kernel<T, WARPS>, p, cluster, shift, segments);
+    return cudaLaunchKernelEx(&cfg, long_kernel<T, WARPS>, p, cluster, lg, segments);
 }
 
 // Four rows a warp as soon as they fill the SMs.
@@ -859,18 +830,26 @@ template <typename T> cudaError_t launch_rows(const Rows &p, cudaStream_t st) {
         else launch_short<T, 32 / N>(p, even, st);
         return cudaGetLastError();
     }
-    int shift = 0;
-    while ((runs >> shift) >= kMaxSegments) shift = shift ? shift + 1 : 2;
-    const int segments = (int)((runs + (1ll << shift) - 1) >> shift);
+    int lg = 0;
+    while (runs * 32 > (int64_t)kMaxSegments << lg) lg = lg == 3 ? 5 : lg == 5 ? 7 : lg + 1;   // a run's part, a run, or batches of runs
+    // whole batches, and four segments a read: the last may lie beyond the row
+    const int cut = 5 - std::min(lg, 5);
+    const int segments = (int)(((lg > 5 ? (runs + (1 << (lg - 5)) - 1) >> (lg - 5) : runs) + kBatch - 1) / kBatch * kBatch) << cut;
     const int cluster = cluster_for(p.rows, runs, sm_count());
-    if (cluster > 1) return launch_long<T, kFewWarps>(p, cluster, shift, segments, st);
-    // about 24 warps an SM, with as few to a row as give that: what a row needs once, it needs of each of its warps
-    // (8192 x 32768 bf16: 101 us with one, 117 with eight; 600 x 100003 fp32: 180 and 45)
-    const int64_t wanted = 24 * (int64_t)sm_count();
-    if (p.rows >= wanted) return launch_long<T, 1>(p, 1, shift, segments, st);
-    if (p.rows * 2 >= wanted) return launch_long<T, 2>(p, 1, shift, segments, st);
-    if (p.rows * 4 >= wanted) return launch_long<T, 4>(p, 1, shift, segments, st);
-    return launch_long<T, 8>(p, 1, shift, segments, st);
+    if (cluster > 1) return launch_long<T, kFewWarps>(p, cluster, lg, segments, st);
+    // about 20 warps an SM, with as few to a row as give that: what a row needs once, it needs of each of its warps
+    // (8192 x 32768 bf16: 101 us with one, 117 with eight; 800 x 32768: 15.5 with four, 17.2 with eight, 20.5 with two;
+    // 600 x 100003 fp32: 180 with one, 45 with eight), and no more warps than batches (600 x 2600 bf16: 6.8 with eight,
+    // 4.4 with four). Long rows that would leave most of a second round of 32 warps an SM empty are shared by two
+    // (5000 x 32768 bf16 65.6, 77.7 with one; 8192 x 32768 101.2 and 102.5).
+    const int64_t sms = sm_count(), batches = (runs + kBatch - 1) / kBatch;
+    int warps = 1;
+    while (warps < kFewWarps && warps < batches && p.rows * warps < 20 * sms) warps *= 2;
+    if (warps == 1 && batches >= 16 && p.rows > 32 * sms && p.rows < 48 * sms) warps = 2;
+    if (warps == 1) return launch_long<T, 1>(p, 1, lg, segments, st);
+    if (warps == 2) return launch_long<T, 2>(p, 1, lg, segments, st);
+    if (warps == 4) return launch_long<T, 4>(p, 1, lg, segments, st);
+    return launch_long<T, kFewWarps>(p, 1, lg, segments, st);
 }
 
 // What the gradient of a row needs: p (A + B y) everywhere, p = 2^(y log2 e - log2 s), and more at the given token and
