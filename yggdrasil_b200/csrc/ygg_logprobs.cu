@@ -258,12 +258,12 @@ __device__ __forceinline__ void write_row(const Rows &p, int64_t row, const Give
     p.lse[row] = e.m + e.ls;
     if (p.stats) p.stats[row] = make_float4(e.m, e.empty ? INFINITY : log2f(a.s), e.empty ? 0.0f : e.ls, e.h);
 }
-__device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, int value, uint32_t index, const Ends &e) {
+__device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, float x, uint32_t index, const Ends &e) {
     p.top_ids[row * p.top + k] = (int32_t)index;
-    p.top_logprobs[row * p.top + k] = e.logprob(unorder(value));
+    p.top_logprobs[row * p.top + k] = e.logprob(x);
 }
 __device__ __forceinline__ void write_top(const Rows &p, int64_t row, int k, Key key, const Ends &e) {
-    write_top(p, row, k, (int)((unsigned)(key >> 32) ^ 0x80000000u), (uint32_t)index_of(key), e);
+    write_top(p, row, k, value_of(key), (uint32_t)index_of(key), e);
 }
 
 // The k-th largest of the lanes' values (k <= 32), a lower bound of the k-th largest entry that the lanes hold.
@@ -277,14 +277,17 @@ __device__ __forceinline__ int kth_of_lanes(int mine, int k) {
     } while (k > 0);
     return best;
 }
-// The same over four values a lane (k <= 128): a closer bound.
-__device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k) {
+__device__ __forceinline__ void order_down(int &a, int &b, int &c, int &d) {
     const auto order2 = [](int &x, int &y) {
         const int t = min(x, y);
         x = max(x, y);
         y = t;
     };
     order2(a, b), order2(c, d), order2(a, c), order2(b, d), order2(b, c);
+}
+// The same over four values a lane (k <= 128): a closer bound.
+__device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k) {
+    order_down(a, b, c, d);
     int best;
     do {
         best = __reduce_max_sync(~0u, a);
@@ -293,6 +296,25 @@ __device__ __forceinline__ int kth_of_lanes(int a, int b, int c, int d, int k) {
         if (it) a = b, b = c, c = d, d = INT32_MIN;
     } while (k > 0);
     return best;
+}
+// A bound that k to 1.25 k of four values a lane reach (k <= 64; more only where they tie), by halving the range between
+// the largest and one that 32 or 64 reach: some 5 rounds for logits, where the k-th itself takes k.
+__device__ __forceinline__ int about_kth_of_lanes(int a, int b, int c, int d, int k, int largest) {
+    order_down(a, b, c, d);
+    int low = __reduce_min_sync(~0u, k <= 32 ? a : b);
+    unsigned range = (unsigned)largest - (unsigned)low;   // the k-th lies in [low, low + range]
+    while (range) {
+        const unsigned half = range - range / 2;
+        const int at = (int)((unsigned)low + half);
+        const int n = __reduce_add_sync(~0u, (a >= at) + (b >= at) + (c >= at) + (d >= at));
+        if (n < k) {
+            range = half - 1;
+        } else {
+            low = at, range -= half;
+            if (n <= k + k / 4) break;
+        }
+    }
+    return low;
 }
 
 // Up to 8 entries: a thread a row.
@@ -320,29 +342,65 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (j != i) above += order(v[j]) + (j < i) > order(v[i]);
-        if (i < p.vocab && above < p.top) write_top(p, row, above, key_of(v[i], i), e);
+        if (i < p.vocab && above < p.top) write_top(p, row, above, v[i], i, e);
     }
 }
 
 // Short rows: a warp holds a row in registers, RUNS runs of 32 kPer places, and takes R rows one after another, so that
 // what a row needs only once (the sums over the lanes, the logarithm, the token, the writes) is done for R rows by
-// different lanes at once. Alternatives: the k-th largest of the lanes' maxima (of four maxima a lane for more than 8
-// alternatives: 20 of 128 bins leave about 22 candidates, 20 of 32 about 31, 64 of 128 about 89) bounds the k-th largest
-// entry from below, so the few entries at or above it are the candidates, and they are ranked by counting. Where ties
-// make them more than the list holds, the equal ones that come too late are left out; where entries above the bound are
+// different lanes at once. Alternatives: the k-th largest of the lanes' maxima, or for more than 8 a value that about k
+// of four maxima a lane reach (20 of 128 bins leave about 22 candidates, 20 of 32 about 31, 64 of 128 about 89), bounds
+// the k-th largest entry from below, so the few entries at or above it are the candidates, and they are ranked by
+// counting (65536 x 256 with 32 alternatives: fp32 70 us, 86 with the k-th of the bins itself; bf16 65, 128 with values
+// and indices apart). Where ties make them more than the list holds, the equal ones that come too late are left out; where entries above the bound are
 // too many, they are taken one at a time.
 constexpr int kShortWarps = 4, kCandidates = 128, kList = kCandidates + 1;   // an odd pitch: lists begin in unlike banks
 // WHOLE: rows of exactly RUNS runs, all on 16-byte boundaries.
-struct List {
+template <typename T> struct List {
     int value[kList];        // order() of the candidates
     uint32_t index[kList];
     __device__ __forceinline__ void put(int at, float x, uint32_t j) { value[at] = order(x), index[at] = j; }
-    __device__ __forceinline__ void put(int at, Key k) { put(at, value_of(k), (uint32_t)index_of(k)); }
 };
+// 16-bit entries tie often: value and index in one word, the lower index above
+struct HalfList {
+    int value[kList];
+    __device__ __forceinline__ uint32_t index_at(int i) const { return ~value[i] & 0xFFFF; }
+};
+template <> struct List<__nv_bfloat16> : HalfList {
+    __device__ __forceinline__ void put(int at, float x, uint32_t j) { value[at] = (order(x) & 0xFFFF0000) | (~j & 0xFFFF); }
+    __device__ __forceinline__ float value_at(int i) const {
+        const int high = value[i] & 0xFFFF0000;
+        return unorder(high < 0 ? high | 0xFFFF : high);
+    }
+};
+template <> struct List<__half> : HalfList {
+    __device__ __forceinline__ void put(int at, float x, uint32_t j) {
+        const int b = (int16_t)__half_as_ushort(__float2half_rn(isnan(x) ? -INFINITY : x + 0.0f));
+        value[at] = (int)((unsigned)(b >= 0 ? b : b ^ 0x7FFF) << 16 | (~j & 0xFFFF));
+    }
+    __device__ __forceinline__ float value_at(int i) const {
+        const int b = value[i] >> 16;
+        return __half2float(__ushort_as_half((unsigned short)(b >= 0 ? b : b ^ 0x7FFF)));
+    }
+};
+// Place `bit` of a lane's, by selects.
+template <int RUNS, int N> __device__ __forceinline__ float entry_at(const float (&v)[RUNS][N], int bit) {
+    float w[RUNS * N];
+#pragma unroll
+    for (int i = 0; i < RUNS * N; i++) w[i] = v[i / N][i % N];
+#pragma unroll
+    for (int h = RUNS * N / 2; h; h /= 2)
+#pragma unroll
+        for (int i = 0; i < h; i++) w[i] = bit & h ? w[i + h] : w[i];
+    return w[0];
+}
+
+// Blocks an SM for so many places a lane: the registers that keep the loads of enough rows in flight.
+constexpr int blocks_for(int places) { return places <= 4 ? 11 : places <= 8 ? 10 : places <= 16 ? 8 : 5; }
 template <typename T, int RUNS, int R, bool WHOLE>
-__global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
+__global__ void __launch_bounds__(kShortWarps * 32, blocks_for(RUNS * kPer<T>)) short_kernel(const Rows p) {
     constexpr int N = kPer<T>;
-    __shared__ List lists[kShortWarps][R];
+    __shared__ List<T> lists[kShortWarps][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row0 = ((int64_t)blockIdx.x * kShortWarps + warp) * R;
     if (row0 >= p.rows) return;
@@ -375,7 +433,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
         ms[w] = a.m, sums[w] = a.s, sums[R + w] = a.t;
         found[w] = 0;
         if (p.top == 0) continue;
-        List &list = lists[warp][w];
+        List<T> &list = lists[warp][w];
         int n;
         {
             int kth;
@@ -390,7 +448,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
 #pragma unroll
                     for (int i = 0; i < N; i++)
                         if (r || i >= 4) bin[i & 3] = fmaxf(bin[i & 3], v[r][i]);
-                kth = kth_of_lanes(order(bin[0]), order(bin[1]), order(bin[2]), order(bin[3]), p.top);
+                kth = about_kth_of_lanes(order(bin[0]), order(bin[1]), order(bin[2]), order(bin[3]), p.top, order(a.m));
             }
             const float bound = unorder(kth);
             unsigned in = 0;
@@ -415,7 +473,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
                 for (int done = 0; (who = __ballot_sync(~0u, in != 0)) != 0; done += __popc(who)) {
                     if (in) {
                         const int bit = __ffs(in) - 1, u = (bit / N * 32 + lane) * N + bit % N;
-                        list.put(done + __popc(who & below), to_f(from[u]), u - off);
+                        // up to 8 places by selects: 28.3 us against 29.5 for 65536 x 256 fp32 with 5 alternatives
+                        list.put(done + __popc(who & below), RUNS * N <= 8 ? entry_at(v, bit) : to_f(from[u]), u - off);
                         in &= in - 1;
                     }
                 }
@@ -471,7 +530,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
                         if (key < last && key > best) best = key;
                     }
                 last = warp_max(best);
-                if (lane == 0) list.put(k, last);
+                if (lane == 0) list.put(k, value_of(last), (uint32_t)index_of(last));
             }
             n = p.top;
         }
@@ -510,26 +569,35 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const Rows p) {
     if (lane < R && row < p.rows) write_row(p, row, given, a, e);
     __syncwarp();
     if (p.top == 0) return;
-    // ranks by the values alone; ties give ranks twice, which shows in the ranks' sum, and then the indices count too
-    const List &list = lists[warp][mine];
-    int wrong = 0;
-    for (int slot = lane / R; slot < most; slot += 32 / R) {
-        if (slot >= n) continue;
-        const int value = list.value[slot];
-        int above = 0;
-        for (int i = 0; i < n; i++) above += list.value[i] > value;
-        wrong += slot - above;   // a row's slots and ranks have one sum
-        if (above < p.top) write_top(p, row, above, value, list.index[slot], e);
-    }
-    // (the rows' sums are looked at together: ranks are never above the true ones, so that no row makes up for another)
-    if (__reduce_add_sync(~0u, wrong) == 0) return;
-    for (int slot = lane / R; slot < n; slot += 32 / R) {
-        const int value = list.value[slot];
-        const uint32_t index = list.index[slot];
-        int above = 0;
-        for (int i = 0; i < n; i++)
-            above += list.value[i] > value || (list.value[i] == value && list.index[i] < index);
-        if (above < p.top) write_top(p, row, above, value, index, e);
+    const List<T> &list = lists[warp][mine];
+    if constexpr (sizeof(T) == 2) {
+        for (int slot = lane / R; slot < n; slot += 32 / R) {
+            const int value = list.value[slot];
+            int above = 0;
+            for (int i = 0; i < n; i++) above += list.value[i] > value;
+            if (above < p.top) write_top(p, row, above, list.value_at(slot), list.index_at(slot), e);
+        }
+    } else {
+        // ranks by the values alone; ties give ranks twice, which shows in the ranks' sum, and then the indices count too
+        int wrong = 0;
+        for (int slot = lane / R; slot < most; slot += 32 / R) {
+            if (slot >= n) continue;
+            const int value = list.value[slot];
+            int above = 0;
+            for (int i = 0; i < n; i++) above += list.value[i] > value;
+            wrong += slot - above;   // a row's slots and ranks have one sum
+            if (above < p.top) write_top(p, row, above, unorder(value), list.index[slot], e);
+        }
+        // (the rows' sums are looked at together: ranks are never above the true ones, so that no row makes up for another)
+        if (__reduce_add_sync(~0u, wrong) == 0) return;
+        for (int slot = lane / R; slot < n; slot += 32 / R) {
+            const int value = list.value[slot];
+            const uint32_t index = list.index[slot];
+            int above = 0;
+            for (int i = 0; i < n; i++)
+                above += list.value[i] > value || (list.value[i] == value && list.index[i] < index);
+            if (above < p.top) write_top(p, row, above, unorder(value), index, e);
+        }
     }
 }
 
