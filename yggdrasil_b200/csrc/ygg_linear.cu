@@ -90,7 +90,8 @@ __device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[8], floa
 }
 
 // THREADS threads a row (32: eight rows a block, or the whole block of 256), the row in registers as VECS vectors of 16
-// bytes a thread. Rows on 16-byte boundaries; what lies past k in a row's last vector is not the row's.
+// bytes a thread. Rows on 16-byte boundaries; what lies past k in a row's last vector is not the row's. Bound by HBM: 8192
+// x 4096 bf16 16 us, 6.3 TB/s read and written; small calls by the launch (1.7 us).
 template <typename T, int THREADS, int VECS>
 __global__ void __launch_bounds__(256) quantize_kernel(const Quantize p) {
     constexpr int N = kPer<T>;
@@ -215,6 +216,10 @@ template <typename T> cudaError_t launch_quantize(const Quantize &p, cudaStream_
 // accumulators (two, so that a tile's epilogue runs under the next one's products). In a pair each CTA holds its own 128
 // channels and half of the rows of x; the leader issues the products of both.
 //
+// Large products are bound by the tensor cores: 8192 x 4096 x 16384 bf16 342 us, 0.98 of the rate of a burst (393 with one
+// CTA a tile), fewer rows by the weights (64 x 4096 x 16384 14 us, 4.8 TB/s), a small K by the epilogue (4096 x 64 x 16384
+// bf16 41.6 us, twice its floor; fp32 51, 1.2 times).
+//
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in
 // flight time to land and leaves.
 
@@ -246,6 +251,7 @@ __device__ __forceinline__ void tile_at(const Tiles &p, int t, int &cb, int &rb)
     rb = t / left;
 }
 
+// (Rows staged in shared memory and written in whole lines were slower: 4096 x 64 x 16384 bf16 47 to 52 us, 41.6 so.)
 // 16 sums of one channel, of the rows whose scales are rs[0..16) (16-byte aligned): row j goes to out + j stride.
 template <typename T>
 __device__ __forceinline__ void write_rows(const uint32_t (&v)[16], const float *rs, float sn, float bn, T *out,
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // Few tiles: the K of a tile is cut among the CTAs of a cluster (CTAS 1, one tile a cluster). Each sums its part in
 // tensor memory; then the columns go round in chunks of 16, chunk q to CTA q mod the cluster's size, through distributed
 // shared memory (the rings, once every CTA's products are done), and each CTA adds up and writes its chunks. Integer sums:
-// the result does not depend on the cut.
+// the result does not depend on the cut. 16 x 4096 x 4096: 8.0 us with four parts, 11.0 with one; bound by latency.
 struct SplitShared {
     uint64_t full[kMaxStages], empty[kMaxStages], done;
     uint32_t tmem;
@@ -594,7 +600,8 @@ template <typename T> int launch_split(const Linear &q, int tn, int parts, cudaS
 //
 // Up to 4 rows (from 5 on the tensor cores are faster: 5 x 4096 x 32768 in 26.3 us there, 27.8 us here; 4 rows in 26.6 and
 // 25.0): the weights are read once and nothing else counts. A warp (or `split` warps, each a part of K) takes two
-// channels at a time, 2048 bytes of each; the codes of the rows lie in shared memory. Short rows before few weights are quantised by every block itself, under its first loads.
+// channels at a time, 2048 bytes of each; the codes of the rows lie in shared memory. Short rows before few weights are
+// quantised by every block itself, under its first loads.
 constexpr int kFewRows = 4, kFewBlock = 2048;
 
 struct Few {
@@ -766,8 +773,8 @@ int quantize(int dtype, const Quantize &p, cudaStream_t st) {
 // How a product is cut: CTAs a product, rows a tile, CTAs that share the K of a tile. The least of what the cuts are
 // expected to take, in ns, by a model fitted to sweeps on a B200 (us, measured):
 //   a launch costs 2500; 128 bytes of K of a tile 240, or its bytes at 115 a ns where those take longer (a pair of
-//   256 x 256: 410, bound by the tensor cores); the epilogue 550 and 9 a column (a pair 3600), bound by its stores, under
-//   the next tile's products.
+//   256 x 256: 410, bound by the tensor cores); the epilogue 550 and 9 a column (a pair 3600), under the next tile's
+//   products.
 //   512 x 4096 x 4096: tn 128 12.1, 256 15.6; 1024 x 4096 x 4096: tn 256 16.0, 128 20.5;
 //   8192 x 4096 x 16384: pair 345, one CTA 393; 4096 x 64 x 16384: tn 256 42.1, 128 49.7, 32 105.9, pair 51.2.
 //   Sharing K costs 1650 and 16 a column more: 16 x 4096 x 4096 8.0 with 4 parts, 11.0 with one; 512 x 1024 x 4096

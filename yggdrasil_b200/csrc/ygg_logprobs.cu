@@ -317,7 +317,7 @@ __device__ __forceinline__ int about_kth_of_lanes(int a, int b, int c, int d, in
     return low;
 }
 
-// Up to 8 entries: a thread a row.
+// Up to 8 entries: a thread a row (65536 x 5 fp32 2.1 us, a launch's time; a warp a row takes 12 for 65536 x 20).
 template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const Rows p) {
     const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
     if (row >= p.rows) return;
@@ -351,9 +351,11 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_kernel(const R
 // different lanes at once. Alternatives: the k-th largest of the lanes' maxima, or for more than 8 a value that about k
 // of four maxima a lane reach (20 of 128 bins leave about 22 candidates, 20 of 32 about 31, 64 of 128 about 89), bounds
 // the k-th largest entry from below, so the few entries at or above it are the candidates, and they are ranked by
-// counting (65536 x 256 with 32 alternatives: fp32 70 us, 86 with the k-th of the bins itself; bf16 65, 128 with values
-// and indices apart). Where ties make them more than the list holds, the equal ones that come too late are left out; where entries above the bound are
-// too many, they are taken one at a time.
+// counting (65536 x 256 with 32 alternatives: fp32 69 us, 86 with the k-th of the bins itself; bf16 64, 128 with values
+// and indices apart). Where ties make them more than the list holds, the equal ones that come too late are left out;
+// where entries above the bound are too many, they are taken one at a time.
+// Bound by instructions and the latency of the selection's chain: 65536 x 256 fp32 16.3 us (4.1 TB/s), 27.8 with 5
+// alternatives; issue slots 58 % full, 40 warps an SM.
 constexpr int kShortWarps = 4, kCandidates = 128, kList = kCandidates + 1;   // an odd pitch: lists begin in unlike banks
 // WHOLE: rows of exactly RUNS runs, all on 16-byte boundaries.
 template <typename T> struct List {
@@ -609,6 +611,8 @@ __global__ void __launch_bounds__(kShortWarps * 32, blocks_for(RUNS * kPer<T>)) 
 // counting. Where ties at the bound make the segments too many, the equal ones beyond the k-th are left out, in the order
 // of their indices. If the entries are too many (ties, masks, sorted rows), a second bound from the threads' best entries
 // leaves fewer; if those are still more, they are taken one at a time.
+// Bound by issue slots and the exponentials' pipe, then by waves of rows that end unevenly: 8192 x 32768 bf16 103 us (5.2
+// TB/s, 0.8 of a copy's rate), 136 with 20 alternatives; fp32 4096 x 32768 82 us, a copy's rate.
 // (Loading a warp's next batch while one is added up costs the registers of a block an SM and gained nothing: 8192 x 32768
 // bf16 136 us with, 117 without, 7 x 100003 bf16 9.5 and 9.4.)
 constexpr int kMaxSegments = 1024, kBins = 128, kMaxCluster = 8, kBatch = 4, kKeys = 256;
@@ -982,7 +986,8 @@ template <typename T> __global__ void __launch_bounds__(128) tiny_grad_kernel(co
 }
 
 // A warp takes kGradRuns runs of 32 kPer places: a chunk of one row, or ROWS short rows whole. SAME: the logits and the
-// gradient of a row lie alike to the 16-byte boundary, so that both move 16 bytes at a time.
+// gradient of a row lie alike to the 16-byte boundary, so that both move 16 bytes at a time. Bound by HBM: 8192 x 32768
+// bf16 188 us, 5.7 TB/s read and written, 0.87 of a copy's rate.
 constexpr int kGradRuns = 4;
 template <typename T, bool SAME, int ROWS>
 __global__ void __launch_bounds__(256) grad_kernel(const Grad p, unsigned chunks) {
