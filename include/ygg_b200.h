@@ -257,7 +257,8 @@ YGG_API int ygg_linear_status(int device, void *stream, int *status_out);
  * p. Sources and counts of one call are those of its beginning; new pages are the free ones in ascending order, given
  * in the order of the call's list. Negative stream and page indices are padding and skipped. What cannot be done is left
  * undone and sets a status word to 1: status[YGG_CACHE_BAD_INDEX] (an index beyond its range, a child that holds pages, a
- * child named twice: its first fork counts), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row),
+ * child named twice: its first fork counts, a table entry that names a page beyond the pool or, where compact looks for its
+ * new place, one of no count: such a page reads as zeros and its entry stays), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row),
  * status[YGG_CACHE_TIMEOUT] (a bounded wait of a call's blocks for each other gave up: the cache is not to be used any
  * more). Calls on one cache are ordered by the caller (one stream, or events). */
 #define YGG_CACHE_BAD_INDEX 0

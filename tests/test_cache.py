@@ -366,3 +366,34 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.ygg_cache_read(0, c, 1, None, p, None) == E.YGG_E_ARG
     assert lib.ygg_cache_write(0, c, 1, p, None, None) == E.YGG_E_ARG
     assert lib.ygg_cache_copy(0, c, 1, p, None, None) == E.YGG_E_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [20, 6000])
+def test_tables_that_do_not_fit_their_counts_are_reported(pages):
+    """A cache around tensors of the caller's: entries of pages beyond the pool, and of pages that nothing counts, at or
+    beyond the number of live pages. compact moves what is counted, leaves those entries and reports them."""
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    data = torch.arange(pages, dtype=torch.int32, device="cuda")[:, None].repeat(1, 3) + 1
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[pages - 2] = 1
+    table = ints([[pages - 2, -1], [pages - 1, -1], [pages, -1], [2 ** 31 - 1, -1], [5, -1]])
+    cache = cache_class()(data, table, ints([1] * 5), refs)
+    assert int(cache.compact()) == 1
+    assert cache.table[:, 0].tolist() == [0, pages - 1, pages, 2 ** 31 - 1, 5]
+    assert refs[0].item() == 1 and int(refs.sum()) == 1 and data[0].tolist() == [pages - 1] * 3
+    with pytest.raises(ValueError):
+        cache.status()
+    assert cache.read([0, 2, 3]).tolist() == [[pages - 1] * 3, [0] * 3, [0] * 3]
+    with pytest.raises(ValueError):
+        cache.status()
+    keep = data.clone()
+    cache.write([2, 3], torch.ones(2, 3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(data, keep)
+    with pytest.raises(ValueError):
+        cache.status()
+    cache.grow([0, 2])
+    assert cache.table[0].tolist() == [0, 1] and cache.table[2].tolist() == [pages, 2]
+    assert data[1].tolist() == [pages - 1] * 3 and data[2].tolist() == [0] * 3
+    with pytest.raises(ValueError):
+        cache.status()

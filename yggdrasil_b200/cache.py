@@ -149,6 +149,7 @@ class StateCache:
         if late:
             raise _native.YggError(_native.YGG_E_TIMEOUT, "StateCache: not to be used any more")
         if bad:
-            raise ValueError("a stream or page was out of range, or a child held pages or was named twice")
+            raise ValueError("a stream or page was out of range, a child held pages or was named twice, or a table named a "
+                             "page that is not the cache's")
         if full:
             raise _native.YggError(_native.YGG_E_CAPACITY, "StateCache: no free page, or a full table row")

@@ -11,7 +11,8 @@
 // result depends on nothing else. Parents are read as they were before the call, children must be empty. What cannot
 // be done is left undone and reported in the status word: an index at or beyond the number of streams, a child that
 // holds pages or is named twice (the first one counts), a pool or a table row without room. Negative indices are
-// padding.
+// padding. Tables and counts come from the caller and need not fit together: a page beyond the pool, or one to be moved
+// that nothing counts, is reported and never used as an address.
 //
 // Sources and destinations of one call's page copies never overlap: grow and fork write pages that were free, compact
 // writes below n and reads at or above it.
@@ -299,6 +300,10 @@ __global__ void __launch_bounds__(kPlan, 1)
                 const int32_t *from = c.table + parent * c.per_stream;
                 m.to = __ldcg(order + given + before);
                 m.from = first ? source0 : taken > 0 ? from[taken - 1] : -1;
+                if (m.from >= c.count) {   // a table that names a page beyond the pool
+                    report(c.status, kBadIndex);
+                    m.from = -1;
+                }
                 if (!grow)
                     for (int j = 0; j < taken - 1; j++) {
                         const int32_t page = from[j];
@@ -343,7 +348,8 @@ __global__ void __launch_bounds__(256) free_kernel(const Cache c, const int32_t 
 // compact, in three parts between barriers. rank(p): the live pages before p.
 //   count:  the live pages of the blocks' shares, n in all
 //   lists:  holes[k], the k-th free page below n (k = p - rank(p)); movers[rank(p)] = p and ranks[p] = rank(p) for the live
-//           pages at or above n, whose k is rank(p) less the live pages below n
+//           pages at or above n, whose k is rank(p) less the live pages below n (ranks[p] = -1 for the free ones: a table
+//           that names one is reported, and nothing is looked up for it)
 //   moves:  tables, counts and pages
 // Bound by the copies: 30 000 moves of 5 KB among 65 536 streams 60 us, 47 of them the copies; few streams 8.5 us, latency.
 template <typename V>
@@ -371,7 +377,8 @@ __global__ void __launch_bounds__(kPlan, 1)
         if (p < pages.to) {
             if (p == n) *below = rank;
             if (p < n && !used) holes[p - rank] = (int32_t)p;
-            if (p >= n && used) movers[rank] = (int32_t)p, ranks[p] = rank;
+            if (p >= n) ranks[p] = used ? rank : -1;
+            if (p >= n && used) movers[rank] = (int32_t)p;
         }
         rank0 += count;
     }
@@ -384,7 +391,10 @@ __global__ void __launch_bounds__(kPlan, 1)
     const int64_t entries = c.streams * c.per_stream;
     for (int64_t i = thread; i < entries; i += all) {
         const int32_t p = c.table[i];
-        if (p >= n && p < c.count) c.table[i] = __ldcg(holes + __ldcg(ranks + p) - low);
+        if (p < n) continue;
+        const int rank = p < c.count ? __ldcg(ranks + p) : -1;
+        if (rank >= 0) c.table[i] = __ldcg(holes + rank - low);
+        else report(c.status, kBadIndex);   // a page beyond the pool, or one that nothing counts
     }
     for (int64_t k = thread; k < moving; k += all) {
         const int32_t from = __ldcg(movers + low + k), to = __ldcg(holes + k);
@@ -421,8 +431,12 @@ __device__ __forceinline__ WideMove resolve(const Where &w, int64_t i) {
             const int n = min(w.length[s], w.per_stream);
             if (n > 0) p = w.table[s * w.per_stream + n - 1];
         }
+        if (p >= (w.last == 1 ? w.src_count : w.dst_count)) {   // a table that names a page beyond the pool
+            report(w.status, kBadIndex);
+            p = -1;
+        }
         (w.last == 1 ? from : to) = p;
-        if (w.last == 1) return from < w.src_count ? WideMove{from, to} : none;   // a stream without pages reads as zeros
+        if (w.last == 1) return {from, to};   // a stream without pages reads as zeros
     } else if (from >= w.src_count || to >= w.dst_count) {
         report(w.status, kBadIndex);
     }
