@@ -397,3 +397,62 @@ def test_tables_that_do_not_fit_their_counts_are_reported(pages):
     assert data[1].tolist() == [pages - 1] * 3 and data[2].tolist() == [0] * 3
     with pytest.raises(ValueError):
         cache.status()
+
+
+def words_by_two(monkeypatch):
+    """Words of caches two at a time, and whatever a first call of each kind waits for behind us."""
+    from yggdrasil_b200 import cache as module
+    monkeypatch.setattr(module, "_SLOTS", 2)
+    monkeypatch.setattr(module, "_pools", {})
+    made = [cache_class().empty(4, 4, shape=(4,), dtype=torch.int8, device="cuda") for _ in range(30)]
+    made[0].grow([0, 1])
+    torch.cuda._sleep(100)
+    torch.cuda.synchronize()
+    del made
+    module._pools.clear()
+
+
+@pytest.mark.gpu
+def test_words_of_a_cache_that_is_gone_serve_no_other_before_its_calls_are_done(monkeypatch):
+    """A call that will report waits on a stream of its own, its cache goes, and others are made: none gets the report."""
+    words_by_two(monkeypatch)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    held = torch.zeros(1, 4, dtype=torch.int8, device="cuda"), ints([[-1], [-1]]), ints([0, 0]), ints([0])
+    ids = ints([0, 1])
+    first, cache = cache_class()(*held), cache_class()(*held)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)
+        cache.grow(ids)   # one page for two streams
+    assert not side.query()
+    del first, cache
+    made = [cache_class().empty(4, 4, shape=(4,), dtype=torch.int8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    assert held[2].sum().item() == 1
+    for c in made:
+        c.status()
+    assert len({c._status[c._at].data_ptr() for c in made}) == len({c._sync[c._at].data_ptr() for c in made}) == 8
+
+
+@pytest.mark.gpu
+def test_words_are_used_again_and_a_cache_can_be_made_in_a_capture(monkeypatch):
+    from yggdrasil_b200 import cache as module
+    words_by_two(monkeypatch)
+    make = lambda: cache_class().empty(4, 4, shape=(4,), dtype=torch.int8, device="cuda")  # noqa: E731
+    seen = set()
+    for _ in range(100):
+        c = make()
+        seen.add(c._status[c._at].data_ptr())
+    assert len(seen) <= 8   # memory does not grow with the caches that were
+    module._pools.clear()
+    kept = [make(), make()]   # the second: half are out, the next two are got ready
+    kept[0].grow([0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = cache_class()(kept[0].pages, kept[0].table, kept[0].length, kept[0].refs)
+        inside.fork(kept[0].refs[:1] * 0, kept[0].refs[:1] * 0 + 1)
+    graph.replay()
+    inside.status()
+    assert kept[0].length.tolist() == [1, 1, 0, 0]

@@ -14,9 +14,12 @@
 snapshots (`grow` leaves one behind), which forks share: `refs[p]` counts the table entries that hold page p. A fork may
 go back to a snapshot (`depth`). Everything stays on the device, on the current stream; the kernels are
 csrc/ygg_pages.cu. Calls on one cache are ordered by their stream; a cache used on several streams at once is the
-caller's to order.
+caller's to order. A cache has to live as long as the CUDA graphs that captured calls on it.
 """
 from __future__ import annotations
+
+import threading
+import weakref
 
 import numpy as np
 import torch
@@ -24,21 +27,69 @@ import torch
 from . import _native, _ops
 
 _SLOTS = 1024
-_slots: dict = {}   # device index -> [status words, sync words, how many of them are handed out]
+_lock = threading.Lock()
+_pools: dict = {}   # device index -> _Pool
+
+
+class _Chunk:
+    """The words of _SLOTS caches, each handed out once: three of status (pinned host memory, which the device can write) and
+    a 64-bit one for a cache's barriers (device memory), all zero."""
+
+    def __init__(self, index):
+        self.status = torch.zeros((_SLOTS, 4), dtype=torch.int32).pin_memory()
+        self.sync = torch.zeros(_SLOTS, dtype=torch.int64, device=torch.device("cuda", index))
+        self.begin(index)
+
+    def begin(self, index):
+        self.used, self.hold = 0, _Hold()   # `hold`: kept by the caches too, so that it tells whether any is left
+        self.held = weakref.ref(self.hold)
+        torch.cuda.current_stream(index).synchronize()   # zero for a cache on any stream
+
+
+class _Hold:
+    pass
+
+
+class _Pool:
+    """A device's chunks. A cache may go while calls on it are on their way, on whatever stream: its words stay, and serve
+    again only when no cache of their chunk is left and the device has been waited for (once in _SLOTS caches at most). The
+    next chunk is got ready early, outside graph captures, so that a cache can be made inside one."""
+
+    def __init__(self, index):
+        self.index, self.current, self.spare, self.old = index, None, None, []
+
+    def fresh(self):
+        for chunk in self.old:
+            if chunk.held() is None:
+                self.old.remove(chunk)
+                torch.cuda.synchronize(self.index)
+                chunk.status.zero_()
+                chunk.sync.zero_()
+                chunk.begin(self.index)
+                return chunk
+        return _Chunk(self.index)
+
+    def take(self):
+        now = self.current
+        if now is None or now.used == _SLOTS:
+            self.current, self.spare = self.spare or self.fresh(), None
+            if now is not None:
+                now.hold = None
+                self.old.append(now)
+            now = self.current
+        elif self.spare is None and 2 * now.used >= _SLOTS and not torch.cuda.is_current_stream_capturing():
+            self.spare = self.fresh()
+        now.used += 1
+        return now.status, now.sync, now.used - 1, now.hold
 
 
 def _words(index):
-    """A cache's own words, each handed out once: three of status (pinned host memory, which the device can write) and
-    a 64-bit one for its blocks' barriers (device memory), all zero."""
-    got = _slots.get(index)
-    if got is None or got[2] == _SLOTS:
-        got = [torch.zeros((_SLOTS, 4), dtype=torch.int32).pin_memory(),
-               torch.zeros(_SLOTS, dtype=torch.int64, device=torch.device("cuda", index)), 0]
-        torch.cuda.current_stream(index).synchronize()   # zero for a cache on any stream
-        _slots[index] = got
-    status, sync, at = got
-    got[2] = at + 1
-    return status, sync, at
+    """Words of a cache's own: (status, sync, which row of theirs, what to keep as long as the cache lives)."""
+    with _lock:
+        pool = _pools.get(index)
+        if pool is None:
+            pool = _pools[index] = _Pool(index)
+        return pool.take()
 
 
 class StateCache:
@@ -47,7 +98,7 @@ class StateCache:
         (S,) and refs (P,) int32, contiguous, on one CUDA device."""
         self._h = None
         if isinstance(pages, torch.Tensor) and pages.is_cuda:
-            self._status, self._sync, self._at = _words(pages.get_device())
+            self._status, self._sync, self._at, self._hold = _words(pages.get_device())
             self._h = _ops.cache(pages, table, length, refs, self._status.data_ptr() + 16 * self._at,
                                  self._sync.data_ptr() + 8 * self._at)
         if self._h is None:
