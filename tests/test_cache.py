@@ -456,3 +456,27 @@ def test_words_are_used_again_and_a_cache_can_be_made_in_a_capture(monkeypatch):
     graph.replay()
     inside.status()
     assert kept[0].length.tolist() == [1, 1, 0, 0]
+
+
+@pytest.mark.gpu
+def test_a_cache_whose_barrier_gave_up_stays_unusable():
+    """What a wait that ran out leaves behind (the barrier's top bit and the status word): later calls give up at their first
+    barrier, nothing is handed out or moved, and status() says so each time, cleared or not."""
+    cache = cache_class().empty(6000, 6000, shape=(4,), dtype=torch.int8, device="cuda")
+    cache.pages.fill_(3)
+    cache.grow(np.arange(0, 6000, 2))
+    cache.status()
+    cache._sync[cache._at] |= -2 ** 63
+    cache.grow(np.arange(1, 6000, 2))
+    for _ in range(2):
+        with pytest.raises(_native.YggError) as e:
+            cache.status()
+        assert e.value.code == _native.YGG_E_TIMEOUT
+    assert cache.length[1::2].sum().item() == 0 and cache.refs.sum().item() == 3000
+    cache._status[cache._at].zero_()
+    cache.free(np.arange(1000))
+    cache.compact()
+    assert cache.refs.sum().item() == 2500 and int(cache.refs[2500:].sum()) > 0
+    for _ in range(2):
+        with pytest.raises(_native.YggError):
+            cache.status(clear=False)

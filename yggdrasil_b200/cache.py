@@ -191,12 +191,13 @@ class StateCache:
 
     def status(self, clear=True):
         """Raise if a call since the last clear met a bad index (ValueError) or had no page or table entry left
-        (RuntimeError); what such a call could do it did. Waits for the current stream."""
+        (RuntimeError); what such a call could do it did. Waits for the current stream. A cache whose blocks once gave up
+        waiting for each other (YggError with YGG_E_TIMEOUT) stays unusable: clear does not clear that."""
         torch.cuda.current_stream(self.device).synchronize()
         words = self._status[self._at]
         bad, full, late, _ = words.tolist()
         if clear:
-            words.zero_()
+            words[:2].zero_()
         if late:
             raise _native.YggError(_native.YGG_E_TIMEOUT, "StateCache: not to be used any more")
         if bad:

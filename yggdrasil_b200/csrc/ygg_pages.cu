@@ -55,7 +55,10 @@ constexpr int kPlan = 1024, kWarps = kPlan / 32, kMaxBlocks = 256;
 
 // A barrier of all blocks of a cooperative launch. The cache's counter goes up by the number of blocks at each barrier and is
 // never reset (its calls are ordered and their launches have one size), so that one look before the first barrier tells
-// how far it will have come at each. The wait is bounded (false: it ran out, and the cache is reported as unusable).
+// how far it will have come at each. The wait is bounded (false: it ran out, and the cache is reported as unusable). After
+// one that ran out the counter no longer tells how many came, and a later barrier would open too early: its top bit is set
+// then, at which every barrier gives up, this call's and those of the calls behind it.
+constexpr unsigned long long kDead = 1ull << 63;
 struct AllBlocks {
     unsigned long long *count, target = 0;
     int32_t *status;
@@ -72,16 +75,14 @@ struct AllBlocks {
         __syncthreads();
         if (gridDim.x == 1) return true;
         if (threadIdx.x == 0) {
-            fine = 1;
             target += gridDim.x;
             asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(count) : "memory");
             const long long t0 = clock64();
-            while (look() < target)
-                if (clock64() - t0 > 2000000000LL) {
-                    fine = 0;
-                    report(status, kTimeout);
-                    break;
-                }
+            unsigned long long v;
+            while (!((v = look()) & kDead) && v < target)
+                if (clock64() - t0 > 2000000000LL) atomicOr(count, kDead);
+            fine = !(v & kDead);
+            if (!fine) report(status, kTimeout);
         }
         __syncthreads();
         return fine;
