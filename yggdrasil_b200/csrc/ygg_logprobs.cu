@@ -520,6 +520,7 @@ __global__ void __launch_bounds__(kShortWarps * 32, blocks_for(RUNS * kPer<T>)) 
             }
         }
         if (n > kCandidates) {
+            __syncwarp();   // other lanes wrote to the list
             Key last = ~0ull;
             for (int k = 0; k < p.top; k++) {
                 Key best = 0;
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(kShortWarps * 32, blocks_for(RUNS * kPer<T>)) 
         }
         // (the rows' sums are looked at together: ranks are never above the true ones, so that no row makes up for another)
         if (__reduce_add_sync(~0u, wrong) == 0) return;
+        __syncwarp();   // the ranks that tied are written over, by other lanes
         for (int slot = lane / R; slot < n; slot += 32 / R) {
             const int value = list.value[slot];
             const uint32_t index = list.index[slot];
