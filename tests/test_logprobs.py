@@ -424,3 +424,26 @@ def test_best_entries_a_fixed_step_apart(vocab, step, dtype):
     x[3:] = torch.where(x[3:] > 30, x[3:], torch.tensor(1.0, device="cuda", dtype=dtype))
     for top in (1, 9, 20, 33, 64):
         check_values(x, t, top, op()(x, t, top=top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5, 8, 9, 20, 200, 5000])
+def test_empty_rows_have_no_gradient_whatever_arrives(vocab, dtype):
+    """What arrives at a row of -inf alone is often not finite (its logprob is -inf, a difference of two such NaN)."""
+    x, t = make(9, vocab, dtype, "empty", seed=43)
+    t = t.abs() % vocab
+    empty = torch.arange(9, device="cuda") % 3 == 0
+    for bad in (math.nan, INF, -INF):
+        for which in ("logprob", "entropy", "lse", "top_logprobs"):
+            leaf = x.clone().requires_grad_()
+            out = op()(leaf, t, top=4)
+            g = torch.where(empty, bad, 0.5)
+            o = getattr(out, which)
+            got, = torch.autograd.grad(o, leaf, g if o.dim() == 1 else g[:, None].expand(o.shape))
+            assert not bool(got[empty].any()), (bad, which)
+            g = torch.where(empty, 0.0, 0.5)
+            out = op()(leaf, t, top=4)
+            o = getattr(out, which)
+            want, = torch.autograd.grad(o, leaf, g if o.dim() == 1 else g[:, None].expand(o.shape))
+            assert torch.equal(got, want)

@@ -941,6 +941,7 @@ struct RowGrad {
         if (p.g_top)
             for (int k = 0; k < p.top; k++) c -= p.g_top[row * p.top + k];
         m = st.x, l2 = st.y, A = c - gh * (st.w - st.z), B = -gh;
+        if (l2 == INFINITY) A = B = given = 0.0f;   // an empty row's gradient is 0 whatever arrives: 0 times NaN is not
     }
     __device__ __forceinline__ float dense(float x) const {
         const float y = x - m;
