@@ -221,9 +221,11 @@ YGG_API int ygg_token_logprobs_backward(int device, int dtype, int64_t rows, int
                                         void *d_grad, int64_t grad_stride, void *stream);
 
 /* ---- linear layers in 8-bit integers -------------------------------------------------------------------------------
- * Row m of x has the scale max|x_m| / 127 and the codes rint(x 127 / max|x_m|); y = (codes . weight row) row_scale scale
- * + bias, the sum exact in int32. A row of zeros has scale 0; a row that holds NaN or infinity has scale NaN (its
- * outputs are NaN). Codes and weights are rows of bytes, their base and stride multiples of 16; bytes of a row past k
+ * Row m of x has the scale max|x_m| / 127 and the codes rint(x 127 / max|x_m|); y = (codes . weight row) scale row_scale
+ * + bias, the sum exact in int32, rounded to float and after each factor, the row's together with the bias: a row's outputs
+ * have the same bits alone and among any number of rows. A row of zeros, or of magnitudes below 3.73e-37, has scale 0; a row
+ * that holds NaN or infinity has scale NaN (its outputs are NaN). Codes are -127 to 127 (-128 is one too many for sums of
+ * k = YGG_LINEAR_MAX_K). Codes and weights are rows of bytes, their base and stride multiples of 16; bytes of a row past k
  * are ignored. k is at most YGG_LINEAR_MAX_K. */
 #define YGG_LINEAR_MAX_K 131072
 

@@ -319,3 +319,33 @@ def test_weights_that_end_with_their_allocation(rows):
         y = f(x, v, s)
         pick = torch.tensor([0, 1, 16383, 32766, 32767], device="cuda")
         check(y[:, pick], x, v[pick], s[pick], None, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("k,n", [(1280, 1300), (4000, 7000)])
+def test_a_row_has_the_same_bits_in_any_batch(k, n, bias):
+    """Few rows, shared K, one CTA a tile and (3000 rows) a pair: every cut of the product rounds alike."""
+    f, q = ops()
+    w, s, b = weights(n, k, seed=5)
+    if not bias:
+        b = None
+    x = inputs(3000, k, torch.float32, seed=7)
+    whole, codes = f(x, w, s, b), q(x)
+    assert torch.equal(f(codes, w, s, b), whole)
+    for rows in (1, 2, 3, 4, 5, 16, 33, 64, 100, 256, 300, 1000, 2047):
+        assert torch.equal(f(x[:rows], w, s, b), whole[:rows]), rows
+        assert torch.equal(f(x[-rows:], w, s, b), whole[-rows:]), rows
+        assert torch.equal(f(type(codes)(codes.codes[:rows], codes.scale[:rows]), w, s, b), whole[:rows]), rows
+
+
+@pytest.mark.gpu
+def test_rows_of_magnitudes_below_the_inverse_of_the_range_count_as_zeros():
+    """127 / 3.7e-37 is infinite in float32, 127 / 3.8e-37 is not."""
+    f, q = ops()
+    x = torch.zeros(4, 20, device="cuda")
+    x[0, 3], x[1, 3], x[2, 3], x[3, 3] = 3.7e-37, 3.8e-37, -1e-38, 1e-44
+    got = q(x)
+    codes, scale = codes_of(x)
+    assert np.array_equal(got.codes.cpu().numpy(), codes) and np.array_equal(got.scale.cpu().numpy(), scale)
+    assert got.codes[:, 3].tolist() == [0, 127, 0, 0] and (got.scale > 0).tolist() == [False, True, False, False]

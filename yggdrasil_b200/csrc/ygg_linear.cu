@@ -4,10 +4,11 @@
 // a weight row n (one output channel) has codes w and its scale s_n. Then
 //   y[m][n] = (sum_k c[m][k] w[n][k]) s_m s_n + b[n],
 // (the channel's factor first: a row's scale may be near the end of the type's range, where only a result beyond it may
-// overflow), with the sum exact in int32 (K <= 131072 keeps |sum| below 127 127 2^17 < 2^31), one rounding to float, one for each
-// factor and the bias, and one to the output's type. Integer sums have no order: results repeat bit for bit.
-// A row of zeros (or so small that its scale rounds to 0) has scale 0 and codes 0; a row that holds NaN or infinity has
-// scale NaN and codes 0, so that its outputs are NaN.
+// overflow), with the sum exact in int32 (K <= 131072 keeps |sum| below 127 127 2^17 < 2^31), one rounding to float, one for
+// the channel's factor, one for the row's factor and the bias together, and one to the output's type. Integer sums have no
+// order: a row's results repeat bit for bit, alone or among others.
+// A row of zeros (or one so small that 127 / max|x_m| is beyond the type's range: below 3.73e-37) has scale 0 and codes 0; a row
+// that holds NaN or infinity has scale NaN and codes 0, so that its outputs are NaN.
 #include <math.h>
 #include <stdint.h>
 
@@ -87,6 +88,12 @@ __device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[4], floa
 __device__ __forceinline__ void store_codes(int8_t *p, const float (&v)[8], float inverse) {
     *(uint2 *)p = inverse == 0.0f ? make_uint2(0, 0)
                                   : make_uint2(code4(v[0], v[1], v[2], v[3], inverse), code4(v[4], v[5], v[6], v[7], inverse));
+}
+
+// The output of a sum: one expression for all kernels, so that a row's outputs have the same bits however many rows go with
+// it and however the product is cut. (Rounded apart, product and bias gave other last bits in one of four float32 outputs.)
+__device__ __forceinline__ float value_of(int sum, float scale, float row_scale, float bias) {
+    return fmaf(__int2float_rn(sum) * scale, row_scale, bias);
 }
 
 // THREADS threads a row (32: eight rows a block, or the whole block of 256), the row in registers as VECS vectors of 16
@@ -262,11 +269,11 @@ __device__ __forceinline__ void write_rows(const uint32_t (&v)[16], const float 
     const float *r = (const float *)f;
     if (rows >= 16) {
 #pragma unroll
-        for (int j = 0; j < 16; j++, out += stride) from_f(fmaf(__int2float_rn((int)v[j]) * sn, r[j], bn), *out);
+        for (int j = 0; j < 16; j++, out += stride) from_f(value_of((int)v[j], sn, r[j], bn), *out);
     } else {
 #pragma unroll
         for (int j = 0; j < 16; j++, out += stride)
-            if (j < rows) from_f(fmaf(__int2float_rn((int)v[j]) * sn, r[j], bn), *out);
+            if (j < rows) from_f(value_of((int)v[j], sn, r[j], bn), *out);
     }
 }
 
@@ -496,8 +503,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (r >= rows) break;
                 int sum = 0;
                 for (int i = 0; i < parts; i++) sum += from[i * 2048 + c * 128];
-                const float y = __int2float_rn(sum) * sn * p.row_scale[row0 + r];
-                from_f(p.bias ? y + bn : y, out[(int64_t)r * p.out_stride]);
+                from_f(value_of(sum, sn, p.row_scale[row0 + r], bn), out[(int64_t)r * p.out_stride]);
             }
         }
     }
@@ -729,8 +735,8 @@ template <typename X, int ROWS> __global__ void __launch_bounds__(256, kFewBlock
         const int64_t ch = 2 * g + lane / ROWS;
         const int r = lane % ROWS;
         if (lane < 2 * ROWS && r < rows && ch < q.n) {
-            const float y = __int2float_rn(mine) * q.scale[ch] * row_scale[r];
-            store_as(p.out_dtype, q.out, r * q.out_stride + ch, q.bias ? y + q.bias[ch] : y);
+            store_as(p.out_dtype, q.out, r * q.out_stride + ch,
+                     value_of(mine, q.scale[ch], row_scale[r], q.bias ? q.bias[ch] : 0.0f));
         }
     }
 }

@@ -4,8 +4,8 @@
     head = quantize_rows(weight)                        # once: (N, K) floats -> codes and a scale for each channel
     y = int8_linear(x, head.codes, head.scale, bias)    # (..., K) -> (..., N) in x's type
 
-y = (codes(x) . codes(w)) scale_x scale_w + bias, the sums exact in int32 (csrc/ygg_linear.cu). The weights are frozen:
-there is no gradient.
+y = (codes(x) . codes(w)) scale_w scale_x + bias, the sums exact in int32 (csrc/ygg_linear.cu): a row's outputs have the same
+bits alone and in any batch. The weights are frozen: there is no gradient.
 """
 from __future__ import annotations
 
@@ -29,8 +29,8 @@ class QuantizedRows(NamedTuple):
 
 def quantize_rows(x):
     """x (..., K) float32, float16 or bfloat16 -> QuantizedRows. The scale of a row is its largest magnitude / 127, a
-    code the nearest integer (ties to even) of the value times 127 / that magnitude. A row of zeros has scale 0; a row
-    that holds NaN or infinity has scale NaN."""
+    code the nearest integer (ties to even) of the value times 127 / that magnitude. A row of zeros, or of magnitudes
+    below 3.73e-37, has scale 0; a row that holds NaN or infinity has scale NaN."""
     out = _ops.quantize_rows(x)
     if out is None:
         codes, scale = _ops.quantize_rows(_rows(x))
