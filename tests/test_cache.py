@@ -480,3 +480,27 @@ def test_a_cache_whose_barrier_gave_up_stays_unusable():
     for _ in range(2):
         with pytest.raises(_native.YggError):
             cache.status(clear=False)
+
+
+FAR = [-2 ** 32 + 5, 2, -2 ** 31 - 1, -2 ** 63, -7]   # low 32 bits: 5, 2, 2^31 - 1, 0, -7
+
+
+@pytest.mark.parametrize("kind", [list, np.array, torch.tensor])
+def test_host_indices_far_below_zero_are_padding(kind):
+    from types import SimpleNamespace
+    ids = cache_class()._ids(SimpleNamespace(device=torch.device("cpu")), kind(FAR), "streams", 8)
+    assert ids.dtype == torch.int32 and ids.tolist() == [-1, 2, -1, -1, -1]
+    for unsigned in (np.uint8, np.uint64):
+        assert cache_class()._ids(SimpleNamespace(device=torch.device("cpu")), np.array([3, 7], unsigned), "x", 8).tolist() == [3, 7]
+    with pytest.raises(ValueError):
+        cache_class()._ids(SimpleNamespace(device=torch.device("cpu")), np.array([2 ** 64 - 1], np.uint64), "streams", 8)
+
+
+@pytest.mark.gpu
+def test_indices_far_below_zero_on_the_host_and_on_the_device():
+    for ids in (FAR, torch.tensor(FAR, device="cuda")):
+        cache, plain = pair(8, 8, 1)
+        cache.grow(list(range(8))), plain.grow(list(range(8)))
+        cache.free(ids), plain.free(FAR)
+        same(cache, plain)
+        assert cache.length.tolist() == [1, 1, 0, 1, 1, 1, 1, 1]

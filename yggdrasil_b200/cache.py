@@ -133,7 +133,8 @@ class StateCache:
             raise ValueError(f"{what} must be a row of integers")
         if host.size and host.max() >= limit:
             raise ValueError(f"{what}: {int(host.max())} out of range [0, {limit})")
-        return torch.as_tensor(np.ascontiguousarray(host, np.int32)).to(self.device)
+        host = np.maximum(host.astype(np.int64), -1)   # as below -2^31 on the device: padding, whatever its low 32 bits say
+        return torch.as_tensor(host.astype(np.int32)).to(self.device)
 
     def _streams(self, ids, what="streams"):
         return self._ids(ids, what, self.table.shape[0])
