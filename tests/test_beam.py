@@ -102,3 +102,24 @@ def test_one_row_no_tokens_and_refusals(models):
                      (([99], 2, 2), {})):
         with pytest.raises(ValueError):
             beam_search(model, *args, **kw)
+
+
+class GaveUp:
+    """The library as after a product that gave up a wait."""
+    def ygg_linear_status(self, index, stream, out):
+        out._obj.value = -8   # YGG_E_TIMEOUT
+        return 0
+
+
+def test_a_head_whose_product_gave_up_is_reported(models, monkeypatch):
+    from yggdrasil_b200 import _native, linear, quantize_rows
+    from yggdrasil_b200.beam import beam_search, state_head
+    model = models["int8"]
+    w = quantize_rows(torch.randn(model.vocab, model.layers * model.n).cuda())
+    head = state_head(w.codes, w.scale)
+    monkeypatch.setattr(linear, "ops", GaveUp)
+    for n in (0, 3):
+        with pytest.raises(_native.YggError) as e:
+            beam_search(model, [1, 2, 3], n, 2, head=head)
+        assert e.value.code == _native.YGG_E_TIMEOUT
+    beam_search(model, [1, 2, 3], 3, 2)   # no product of the operators in it

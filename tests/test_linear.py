@@ -349,3 +349,14 @@ def test_rows_of_magnitudes_below_the_inverse_of_the_range_count_as_zeros():
     codes, scale = codes_of(x)
     assert np.array_equal(got.codes.cpu().numpy(), codes) and np.array_equal(got.scale.cpu().numpy(), scale)
     assert got.codes[:, 3].tolist() == [0, 127, 0, 0] and (got.scale > 0).tolist() == [False, True, False, False]
+
+
+@pytest.mark.gpu
+def test_status_is_clean_after_products_of_each_cut():
+    from yggdrasil_b200.linear import linear_status
+    f, q = ops()
+    w, s, b = weights(7000, 4000)
+    for rows in (1, 4, 5, 100, 3000):
+        f(inputs(rows, 4000, torch.float32), w, s, b)
+        linear_status()
+        linear_status("cuda:0")

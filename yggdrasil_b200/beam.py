@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from .cache import StateCache
-from .linear import QuantizedRows, int8_linear
+from .linear import QuantizedRows, int8_linear, linear_status
 from .logprobs import token_logprobs
 
 
@@ -108,6 +108,8 @@ def beam_search(model, prompt, n, width=4, head=None, end=None):
         cache.status()
         if hasattr(model, "status"):
             model.status()
+        if head is not None:   # its products may have given up a wait: then the logits are not to be used
+            linear_status(dev)
         if n == 0:
             tokens, scores = tokens.expand(rows, width, -1), scores.expand(rows, width)
         tokens, scores = tokens.cpu().numpy(), scores.cpu().numpy()

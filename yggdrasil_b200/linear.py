@@ -110,7 +110,8 @@ def _strides(lead, step):
 
 def linear_status(device="cuda"):
     """Raise YggError if a bounded wait of an int8 product on the device gave up since the last call: outputs since then
-    are not to be used. Waits for the current stream."""
+    are not to be used. Waits for the current stream. The record is one for the device and all of its callers: the first
+    that asks is told, and clears it."""
     device = torch.device(device)
     index = device.index if device.index is not None else torch.cuda.current_device()
     out = ctypes.c_int(0)
