@@ -447,3 +447,26 @@ def test_empty_rows_have_no_gradient_whatever_arrives(vocab, dtype):
             o = getattr(out, which)
             want, = torch.autograd.grad(o, leaf, g if o.dim() == 1 else g[:, None].expand(o.shape))
             assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    """A forward-mode derivative is refused, not lost: of the logits, and of what arrives at the gradient."""
+    import torch.autograd.forward_ad as fw
+    x, t = make(4, 60, torch.float32)
+    one = torch.ones_like(x)
+    with fw.dual_level():
+        dual = fw.make_dual(x, one)
+        for logits in (dual, dual[:, 1:], dual.unflatten(0, (2, 2)), dual.T.contiguous().T, dual.half(),
+                       fw.make_dual(x.clone().requires_grad_(), one)):
+            with pytest.raises(NotImplementedError):
+                op()(logits, t.view(logits.shape[:-1]) % 50, top=2)
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                op()(logits, t.view(logits.shape[:-1]) % 50, top=2)
+        leaf = x.clone().requires_grad_()
+        out = op()(leaf, t)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(out.lse, leaf, fw.make_dual(torch.ones(4, device="cuda"), torch.ones(4, device="cuda")))
+        primal = fw.unpack_dual(dual).primal
+        assert torch.equal(op()(primal, t).logprob, op()(x, t).logprob)
+    assert torch.equal(op()(x, t).logprob, op()(x.clone().requires_grad_(), t).logprob)

@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -66,6 +67,11 @@ bool is_row(const Tensor &t, at::ScalarType type, int64_t n, const at::Device &d
            t.device() == device;
 }
 
+// Whether a forward-mode derivative comes with it (the dual of a tangent), which no kernel here carries on.
+bool has_tangent(const Tensor &t) {
+    return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+
 PyObject *wrap(const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
 
 // ------------------------------------------------------------------------------------------------ token_logprobs
@@ -111,7 +117,8 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list arriving) {
-        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "token_logprobs has no second derivative");
+        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() && std::none_of(arriving.begin(), arriving.end(), has_tangent),
+                                    "token_logprobs has no second derivative");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &tokens = saved[1], &stats = saved[2], &ids = saved[3];
         const int64_t top = ctx->saved_data["top"].toInt(), rows = x.size(0), vocab = x.size(1), step = x.stride(0);
@@ -151,6 +158,7 @@ PyObject *py_token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t n) {
         (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong) || t->dim() != 1 || t->size(0) != x->size(0) ||
         !t->is_contiguous() || t->device() != x->device())
         Py_RETURN_NONE;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*x), "token_logprobs has no forward-mode derivative");
     const c10::cuda::CUDAGuard on(x->device());
     Logprobs o;
     if (x->requires_grad() && at::GradMode::is_enabled()) {

@@ -10,7 +10,8 @@
     out.top_logprobs  # (B, 5) float32
 
 The kernels are csrc/ygg_logprobs.cu; the sums are held in 32 bits whatever the logits' type. With logits that require
-a gradient, logprob, entropy, lse and top_logprobs carry one (top_ids does not).
+a gradient, logprob, entropy, lse and top_logprobs carry one (top_ids does not). There is no second derivative and no
+forward-mode one: logits with a tangent are refused with NotImplementedError.
 """
 from __future__ import annotations
 
