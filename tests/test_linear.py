@@ -360,3 +360,34 @@ def test_status_is_clean_after_products_of_each_cut():
         f(inputs(rows, 4000, torch.float32), w, s, b)
         linear_status()
         linear_status("cuda:0")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 40])
+def test_derivatives_are_refused_of_every_input(rows):
+    """Of the rows, their scales, the channels' scales and the bias, by gradients and by tangents; none is lost."""
+    import torch.autograd.forward_ad as fw
+    f, q = ops()
+    x, (w, s, b) = inputs(rows, 64, torch.float32), weights(32, 64)
+    c = q(x)
+    want = f(x, w, s, b)
+
+    def calls(mark):
+        return [lambda: f(mark(x), w, s, b), lambda: f(mark(x)[None], w, s, b), lambda: q(mark(x)), lambda: q(mark(x).T),
+                lambda: f(x, w, mark(s), b), lambda: f(x, w, s, mark(b)), lambda: f(x, w, s, mark(b.half())),
+                lambda: f(x, w, mark(s.repeat_interleave(2))[::2], b), lambda: f(c, w, mark(s), b),
+                lambda: f(type(c)(c.codes, mark(c.scale)), w, s, b), lambda: f(c, w, s, mark(b))]
+
+    leaf = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    for call in calls(leaf):
+        with pytest.raises(NotImplementedError):
+            call()
+        with torch.no_grad():
+            call()
+    with fw.dual_level():
+        for call in calls(lambda t: fw.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(NotImplementedError):
+                call()
+    with torch.no_grad():
+        assert torch.equal(f(leaf(x), w, leaf(s), leaf(b)), want)
+    assert torch.equal(f(x, w, s, torch.nn.Parameter(b).detach()), want)

@@ -72,6 +72,9 @@ bool has_tangent(const Tensor &t) {
     return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
 }
 
+// Whether a derivative is asked for through it, of either kind.
+bool tracked(const Tensor &t) { return (t.requires_grad() && at::GradMode::is_enabled()) || has_tangent(t); }
+
 PyObject *wrap(const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
 
 // ------------------------------------------------------------------------------------------------ token_logprobs
@@ -195,7 +198,8 @@ std::optional<Weights> weights_of(PyObject *const *args, int64_t k, const at::De
         r.w->size(1) != k || r.w->size(0) < 1 || r.w->device() != device || !aligned_rows(*r.w))
         return std::nullopt;
     const int64_t n = r.w->size(0);
-    if (!is_row(*r.scale, at::kFloat, n, device) || (r.bias && !is_row(*r.bias, at::kFloat, n, device)))
+    if (!is_row(*r.scale, at::kFloat, n, device) || (r.bias && !is_row(*r.bias, at::kFloat, n, device)) ||
+        tracked(*r.scale) || (r.bias && tracked(*r.bias)))
         return std::nullopt;
     return r;
 }
@@ -210,7 +214,7 @@ int type_asked(PyObject *o, at::ScalarType other, at::ScalarType &type) {
 
 bool rows_ok(const Tensor &x) {
     return dtype_of(x.scalar_type()) >= 0 && x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= YGG_LINEAR_MAX_K &&
-           (x.size(1) == 1 || x.stride(1) == 1) && !(x.requires_grad() && at::GradMode::is_enabled());
+           (x.size(1) == 1 || x.stride(1) == 1) && !tracked(x);
 }
 
 // (x, weight, scale, bias or None, out_dtype or None) -> y, or None
@@ -243,7 +247,7 @@ PyObject *py_int8_linear_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const Tensor *c = n == 6 ? cuda_tensor(args[0]) : nullptr, *s = n == 6 ? cuda_tensor(args[1]) : nullptr;
     if (!c || !s || c->scalar_type() != at::kChar || c->dim() != 2 || c->size(1) < 1 || c->size(1) > YGG_LINEAR_MAX_K ||
-        !aligned_rows(*c) || !is_row(*s, at::kFloat, c->size(0), c->device()))
+        !aligned_rows(*c) || !is_row(*s, at::kFloat, c->size(0), c->device()) || tracked(*s))
         Py_RETURN_NONE;
     at::ScalarType type = at::kFloat;
     const int out_dtype = type_asked(args[5], at::kFloat, type);
@@ -283,6 +287,14 @@ PyObject *py_quantize_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
     PyTuple_SET_ITEM(r, 0, wrap(codes));
     PyTuple_SET_ITEM(r, 1, wrap(scale));
     return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// (tensor,) -> whether a derivative is asked for through it
+PyObject *py_tracked(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n == 1 && THPVariable_Check(args[0]) && tracked(THPVariable_Unpack(args[0]))) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
     END_HANDLE_TH_ERRORS
 }
 
@@ -441,8 +453,9 @@ PyObject *py_cache_copy(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(token_logprobs), CALL(int8_linear), CALL(int8_linear_rows), CALL(quantize_rows),
-                           CALL(cache),          CALL(cache_fork),  CALL(cache_free),       CALL(cache_compact),
-                           CALL(cache_read),     CALL(cache_write), CALL(cache_copy),       {nullptr, nullptr, 0, nullptr}};
+                           CALL(tracked),        CALL(cache),       CALL(cache_fork),       CALL(cache_free),
+                           CALL(cache_compact),  CALL(cache_read),  CALL(cache_write),      CALL(cache_copy),
+                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

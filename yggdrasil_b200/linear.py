@@ -5,7 +5,8 @@
     y = int8_linear(x, head.codes, head.scale, bias)    # (..., K) -> (..., N) in x's type
 
 y = (codes(x) . codes(w)) scale_w scale_x + bias, the sums exact in int32 (csrc/ygg_linear.cu): a row's outputs have the same
-bits alone and in any batch. The weights are frozen: there is no gradient.
+bits alone and in any batch. The weights are frozen: there is no gradient, and rows, scales or a bias that ask for one are
+refused with NotImplementedError (detach() them, or call under torch.no_grad()).
 """
 from __future__ import annotations
 
@@ -59,6 +60,7 @@ def _prepared(x, weight, scale, bias, out_dtype):
                 or row_scale.shape != codes.shape[:-1] or row_scale.device != codes.device:
             raise ValueError("QuantizedRows: int8 codes (..., K) and a float32 scale (...) on one CUDA device")
         lead, k, device = codes.shape[:-1], codes.shape[-1], codes.device
+        _frozen(row_scale)
         if not 1 <= k <= MAX_K:
             raise ValueError(f"codes: K {k}: 1 to {MAX_K}")
     else:
@@ -76,7 +78,9 @@ def _prepared(x, weight, scale, bias, out_dtype):
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.device != device or bias.dtype not in DTYPES:
             raise ValueError(f"bias must be a float tensor ({n},) on {device}")
+        _frozen(bias)
         bias = bias.detach().float().contiguous()
+    _frozen(scale)
     with torch.cuda.device(device):
         weights = _laid_out(weight), scale.contiguous(), bias, out_dtype
         if isinstance(x, QuantizedRows):
@@ -93,10 +97,15 @@ def _rows(x):
     k = x.shape[-1]
     if not 1 <= k <= MAX_K:
         raise ValueError(f"x: K {k}: 1 to {MAX_K}")
-    if x.requires_grad and torch.is_grad_enabled():   # the weights are frozen
-        raise NotImplementedError("the int8 product has no gradient: use detach() or torch.no_grad()")
+    _frozen(x)
     rows = x.reshape(-1, k)
     return rows if k == 1 or rows.stride(1) == 1 else rows.contiguous()
+
+
+def _frozen(*tensors):
+    """Refuse tensors through which a gradient, or a forward-mode derivative, is asked for."""
+    if any(_ops.tracked(t) for t in tensors):
+        raise NotImplementedError("the int8 product has no gradient: use detach() or torch.no_grad()")
 
 
 def _strides(lead, step):
