@@ -504,3 +504,26 @@ def test_indices_far_below_zero_on_the_host_and_on_the_device():
         cache.free(ids), plain.free(FAR)
         same(cache, plain)
         assert cache.length.tolist() == [1, 1, 0, 1, 1, 1, 1, 1]
+
+
+@pytest.mark.gpu
+def test_derivatives_are_refused():
+    import torch.autograd.forward_ad as fw
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    make = lambda pages: cache_class()(pages, ints(2, 1) - 1, ints(2), ints(4))  # noqa: E731
+    pages = torch.zeros(4, 3, device="cuda")
+    cache, batch = make(pages), torch.ones(1, 3, device="cuda")
+    cache.grow([0])
+    leaf = batch.clone().requires_grad_()
+    for b in (leaf, leaf.T.contiguous().T, leaf * 2):
+        with pytest.raises(NotImplementedError):
+            cache.write([0], b)
+    with pytest.raises(NotImplementedError):
+        make(pages.clone().requires_grad_())
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError):
+            cache.write([0], fw.make_dual(batch, batch))
+    assert not bool(pages.any())
+    with torch.no_grad():
+        cache.write([0], leaf)
+    assert torch.equal(cache.read([0]), batch)

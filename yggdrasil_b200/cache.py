@@ -14,7 +14,8 @@
 snapshots (`grow` leaves one behind), which forks share: `refs[p]` counts the table entries that hold page p. A fork may
 go back to a snapshot (`depth`). Everything stays on the device, on the current stream; the kernels are
 csrc/ygg_pages.cu. Calls on one cache are ordered by their stream; a cache used on several streams at once is the
-caller's to order. A cache has to live as long as the CUDA graphs that captured calls on it.
+caller's to order. A cache has to live as long as the CUDA graphs that captured calls on it. Pages hold values: a batch or
+pages that ask for a gradient are refused.
 """
 from __future__ import annotations
 
@@ -92,12 +93,19 @@ def _words(index):
         return pool.take()
 
 
+def _valued(t):
+    """Refuse a tensor through which a derivative is asked for: pages hold values, and their copies would lose it."""
+    if _ops.tracked(t):
+        raise NotImplementedError("a cache carries no gradient: use detach() or torch.no_grad()")
+
+
 class StateCache:
     def __init__(self, pages, table, length, refs):
         """Around tensors that hold a cache already (updated in place): pages (P, ...) of any type, table (S, M), length
         (S,) and refs (P,) int32, contiguous, on one CUDA device."""
         self._h = None
         if isinstance(pages, torch.Tensor) and pages.is_cuda:
+            _valued(pages)
             self._status, self._sync, self._at, self._hold = _words(pages.get_device())
             self._h = _ops.cache(pages, table, length, refs, self._status.data_ptr() + 16 * self._at,
                                  self._sync.data_ptr() + 8 * self._at)
@@ -172,13 +180,15 @@ class StateCache:
         return batch if batch is not None else _ops.cache_read(self._h, self._streams(streams))
 
     def write(self, streams, batch):
-        """batch[i] becomes the live state of streams[i], a stream that holds pages; no stream named twice."""
+        """batch[i] becomes the live state of streams[i], a stream that holds pages; no stream named twice, and the batch
+        no part of the pages themselves."""
         if _ops.cache_write(self._h, streams, batch) is None:
             s = self._streams(streams)
             want = (s.shape[0], *self.pages.shape[1:])
             if not isinstance(batch, torch.Tensor) or batch.dtype != self.pages.dtype or batch.device != self.device \
                     or batch.shape != want:
                 raise ValueError(f"batch must be {self.pages.dtype} {want} on {self.device}")
+            _valued(batch)
             _ops.cache_write(self._h, s, batch.contiguous())
 
     def copy(self, source, target):

@@ -426,7 +426,7 @@ PyObject *py_cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Cache &c = *cache_of(args[0]);
     const Tensor *s = ids_of(args[1], c), *b = cuda_tensor(args[2]);
     if (!s || !b || !b->is_contiguous() || b->scalar_type() != c.pages.scalar_type() || b->device() != c.pages.device() ||
-        b->dim() != c.pages.dim() || b->size(0) != s->size(0) || b->sizes().slice(1) != c.pages.sizes().slice(1))
+        b->dim() != c.pages.dim() || b->size(0) != s->size(0) || b->sizes().slice(1) != c.pages.sizes().slice(1) || tracked(*b))
         Py_RETURN_NONE;
     const at::Device device = c.pages.device();
     raise_for(ygg_cache_write(device.index(), &c.c, s->size(0), (const int32_t *)s->data_ptr(), b->data_ptr(),
