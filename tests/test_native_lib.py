@@ -95,3 +95,12 @@ def test_selftest_wait_arguments():
     status = ctypes.c_int(7)
     assert lib.ygg_selftest_wait(0, -1, None, ctypes.byref(status)) == _native.YGG_E_ARG
     assert lib.ygg_selftest_wait(0, 1000, None, None) == _native.YGG_E_ARG
+
+
+def test_importing_the_package_imports_neither_torch_nor_the_operators():
+    import subprocess
+    import sys
+    code = ("import sys\nfrom yggdrasil_b200 import *\nassert Yggdrasil and B200Yggdrasil\n"
+            "assert not {'torch', 'yggdrasil_b200._ops', 'yggdrasil_b200.cache'} & set(sys.modules)\n"
+            "from yggdrasil_b200 import StateCache, int8_linear, quantize_rows, token_logprobs\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)

@@ -5,7 +5,7 @@ Python host side, shaped as the reference's inference API (``Yggdrasil.load(path
 """
 from .inference import B200Yggdrasil, Yggdrasil  # noqa: F401
 
-__all__ = ["Yggdrasil", "B200Yggdrasil", "token_logprobs", "int8_linear", "quantize_rows", "StateCache"]
+__all__ = ["Yggdrasil", "B200Yggdrasil"]   # without the operators: `import *` would import torch and their binding
 
 _OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs",
               "int8_linear": "linear", "quantize_rows": "linear", "QuantizedRows": "linear",
