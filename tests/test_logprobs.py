@@ -470,3 +470,12 @@ def test_tangents_are_refused():
         primal = fw.unpack_dual(dual).primal
         assert torch.equal(op()(primal, t).logprob, op()(x, t).logprob)
     assert torch.equal(op()(x, t).logprob, op()(x.clone().requires_grad_(), t).logprob)
+
+
+@pytest.mark.gpu
+def test_a_number_of_alternatives_is_an_integer():
+    x, t = make(4, 50, torch.float32)
+    for bad in (2.5, 2.0, "2", None, [2]):
+        with pytest.raises(ValueError):
+            op()(x, t, top=bad)
+    assert op()(x, t, top=np.int64(2)).top_ids.shape == (4, 2) and op()(x[None], t[None], top=np.uint8(3)).top_ids.shape == (1, 4, 3)

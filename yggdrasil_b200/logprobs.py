@@ -52,8 +52,8 @@ def _prepared(logits, tokens, top):
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     if vocab < 1:
         raise ValueError("logits: the vocabulary is empty")
-    if not 0 <= top <= min(vocab, TOP_MAX):
-        raise ValueError(f"top {top}: 0 to {min(vocab, TOP_MAX)}")
+    if not hasattr(top, "__index__") or not 0 <= top <= min(vocab, TOP_MAX):   # 2.5 is no number of alternatives
+        raise ValueError(f"top {top}: an integer, 0 to {min(vocab, TOP_MAX)}")
     if not isinstance(tokens, torch.Tensor) or not tokens.is_cuda:
         host = np.asarray(tokens)
         if host.size and (host.dtype.kind not in "iu" or host.max() >= vocab):
