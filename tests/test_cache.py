@@ -527,3 +527,12 @@ def test_derivatives_are_refused():
     with torch.no_grad():
         cache.write([0], leaf)
     assert torch.equal(cache.read([0]), batch)
+
+
+@pytest.mark.gpu
+def test_a_full_pool_says_so():
+    cache = cache_class().empty(1, 2, shape=(4,), dtype=torch.int8, device="cuda")
+    cache.grow([0, 1])
+    with pytest.raises(_native.YggError) as e:
+        cache.status()
+    assert e.value.code == _native.YGG_E_CAPACITY and str(e.value) == "StateCache: no free page, or a full table row (-10)"

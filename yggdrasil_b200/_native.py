@@ -37,9 +37,9 @@ class YggCache(ctypes.Structure):
 
 
 class YggError(RuntimeError):
-    def __init__(self, code: int, what: str):
+    def __init__(self, code: int, what: str, why: str | None = None):
         self.code = code
-        super().__init__(f"{what}: {strerror(code)} ({code})")
+        super().__init__(f"{what}: {why or strerror(code)} ({code})")
 
 
 _lib = None

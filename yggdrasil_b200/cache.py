@@ -215,4 +215,4 @@ class StateCache:
             raise ValueError("a stream or page was out of range, a child held pages or was named twice, or a table named a "
                              "page that is not the cache's")
         if full:
-            raise _native.YggError(_native.YGG_E_CAPACITY, "StateCache: no free page, or a full table row")
+            raise _native.YggError(_native.YGG_E_CAPACITY, "StateCache", "no free page, or a full table row")
