@@ -391,3 +391,48 @@ def test_derivatives_are_refused_of_every_input(rows):
     with torch.no_grad():
         assert torch.equal(f(leaf(x), w, leaf(s), leaf(b)), want)
     assert torch.equal(f(x, w, s, torch.nn.Parameter(b).detach()), want)
+
+
+# CTA pairs over several rounds of tiles (the first two), one CTA over several rounds with bands of channel blocks, and narrow
+# and short K on the tensor cores
+LARGE = [(5001, 2001, 3003), (3000, 4000, 7000), (1025, 4096, 9000), (700, 300, 40000), (20000, 40, 700), (9001, 130, 1100),
+         (20, 1, 40), (20, 5, 130), (300, 3, 70), (300, 15, 2000), (2000, 1, 5)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,n", LARGE)
+def test_values_of_large_and_narrow_products(rows, k, n, dtype):
+    f, _ = ops()
+    x = inputs(rows, k, dtype, seed=k)
+    w, s, b = weights(n, k, seed=n, bias=rows % 2 == 1)
+    check(f(x, w, s, b), x, w, s, b, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [1, 7, 128, 130, 255, 256, 500, 512, 513, 1000, 1024, 1030, 2000, 2048])
+def test_codes_of_many_rows(k, dtype):
+    """A warp a row, in one to eight vectors a lane, where rows fill the SMs; rows that end inside a vector of theirs."""
+    _, q = ops()
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    for x in (inputs(rows, (k + 15) // 16 * 16, dtype, seed=k)[:, :k], inputs(rows, k, dtype, seed=k + 1)):
+        x[5], x[rows - 1, k - 1], x[17, k // 2] = 0, float("inf"), float("nan")
+        got = q(x)
+        codes, scale = codes_of(x)
+        assert np.array_equal(got.codes.cpu().numpy(), codes)
+        assert np.array_equal(got.scale.cpu().numpy(), scale, equal_nan=True)
+        padded = (k + 15) // 16 * 16
+        assert not bool(got.codes.as_strided((rows, padded), (padded, 1))[:, k:].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [1025, 2050, 4100, 8190, 16380, 16400])
+def test_codes_of_long_rows(k, dtype):
+    """A block a row, in one to eight vectors a thread, and beyond."""
+    _, q = ops()
+    x = inputs(9, (k + 15) // 16 * 16, dtype, seed=k)[:, :k]
+    got = q(x)
+    codes, scale = codes_of(x)
+    assert np.array_equal(got.codes.cpu().numpy(), codes) and np.array_equal(got.scale.cpu().numpy(), scale)
