@@ -39,16 +39,18 @@ class _Chunk:
     def __init__(self, index):
         self.status = torch.zeros((_SLOTS, 4), dtype=torch.int32).pin_memory()
         self.sync = torch.zeros(_SLOTS, dtype=torch.int64, device=torch.device("cuda", index))
-        self.begin(index)
-
-    def begin(self, index):
-        self.used, self.hold = 0, _Hold()   # `hold`: kept by the caches too, so that it tells whether any is left
-        self.held = weakref.ref(self.hold)
+        self.status_at, self.sync_at = self.status.data_ptr(), self.sync.data_ptr()
         torch.cuda.current_stream(index).synchronize()   # zero for a cache on any stream
+
+    def renew(self, index):
+        torch.cuda.synchronize(index)
+        self.status.zero_()
+        self.sync.zero_()
+        torch.cuda.current_stream(index).synchronize()
 
 
 class _Hold:
-    pass
+    """Kept by the caches of a chunk: it tells whether any is left."""
 
 
 class _Pool:
@@ -57,46 +59,40 @@ class _Pool:
     next chunk is got ready early, outside graph captures, so that a cache can be made inside one."""
 
     def __init__(self, index):
-        self.index, self.current, self.spare, self.old = index, None, None, []
+        self.index, self.chunk, self.hold, self.spare, self.old = index, None, None, None, []
+        self.used = self.until = 0   # words handed out of the chunk, and up to when without a further look
 
     def fresh(self):
-        for chunk in self.old:
-            if chunk.held() is None:
-                self.old.remove(chunk)
-                torch.cuda.synchronize(self.index)
-                chunk.status.zero_()
-                chunk.sync.zero_()
-                chunk.begin(self.index)
+        for i, (chunk, held) in enumerate(self.old):
+            if held() is None:
+                chunk.renew(self.index)
+                del self.old[i]
                 return chunk
         return _Chunk(self.index)
 
-    def take(self):
-        now = self.current
-        if now is None or now.used == _SLOTS:
-            self.current, self.spare = self.spare or self.fresh(), None
-            if now is not None:
-                now.hold = None
-                self.old.append(now)
-            now = self.current
-        elif self.spare is None and 2 * now.used >= _SLOTS and not torch.cuda.is_current_stream_capturing():
-            self.spare = self.fresh()
-        now.used += 1
-        return now.status, now.sync, now.used - 1, now.hold
+    def look(self):
+        if self.chunk is None or self.used == _SLOTS:
+            chunk = self.spare or self.fresh()
+            if self.chunk is not None:
+                self.old.append((self.chunk, weakref.ref(self.hold)))
+            self.chunk, self.hold, self.spare = chunk, _Hold(), None
+            self.used, self.until = 0, _SLOTS // 2
+        elif torch.cuda.is_current_stream_capturing():
+            self.until = self.used + 1
+        else:
+            self.spare, self.until = self.fresh(), _SLOTS
 
 
 def _words(index):
-    """Words of a cache's own: (status, sync, which row of theirs, what to keep as long as the cache lives)."""
+    """Words of a cache's own: their chunk, which of them, and what to keep as long as the cache lives."""
     with _lock:
         pool = _pools.get(index)
         if pool is None:
             pool = _pools[index] = _Pool(index)
-        return pool.take()
-
-
-def _valued(t):
-    """Refuse a tensor through which a derivative is asked for: pages hold values, and their copies would lose it."""
-    if _ops.tracked(t):
-        raise NotImplementedError("a cache carries no gradient: use detach() or torch.no_grad()")
+        if pool.used >= pool.until:
+            pool.look()
+        pool.used += 1
+        return pool.chunk, pool.used - 1, pool.hold
 
 
 class StateCache:
@@ -105,10 +101,9 @@ class StateCache:
         (S,) and refs (P,) int32, contiguous, on one CUDA device."""
         self._h = None
         if isinstance(pages, torch.Tensor) and pages.is_cuda:
-            _valued(pages)
-            self._status, self._sync, self._at, self._hold = _words(pages.get_device())
-            self._h = _ops.cache(pages, table, length, refs, self._status.data_ptr() + 16 * self._at,
-                                 self._sync.data_ptr() + 8 * self._at)
+            chunk, self._at, self._hold = _words(pages.get_device())
+            self._status, self._sync = chunk.status, chunk.sync
+            self._h = _ops.cache(pages, table, length, refs, chunk.status_at + 16 * self._at, chunk.sync_at + 8 * self._at)
         if self._h is None:
             raise ValueError("a cache needs contiguous tensors on one CUDA device: pages (P, ...), table (S, M) int32, "
                              "length (S,) int32 and refs (P,) int32")
@@ -188,7 +183,6 @@ class StateCache:
             if not isinstance(batch, torch.Tensor) or batch.dtype != self.pages.dtype or batch.device != self.device \
                     or batch.shape != want:
                 raise ValueError(f"batch must be {self.pages.dtype} {want} on {self.device}")
-            _valued(batch)
             _ops.cache_write(self._h, s, batch.contiguous())
 
     def copy(self, source, target):

@@ -306,6 +306,10 @@ struct Cache {
 };
 constexpr const char *kCache = "yggdrasil_b200.cache";
 
+void refuse_derivatives(const Tensor &t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!tracked(t), "a cache carries no gradient: use detach() or torch.no_grad()");
+}
+
 Cache *cache_of(PyObject *o) {
     Cache *c = (Cache *)PyCapsule_GetPointer(o, kCache);
     if (!c) throw python_error();
@@ -325,6 +329,7 @@ PyObject *py_cache(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (pages.dim() < 2 || table.dim() != 2 || t[2]->dim() != 1 || t[2]->size(0) != table.size(0) || t[3]->dim() != 1 ||
         t[3]->size(0) != pages.size(0))
         Py_RETURN_NONE;
+    refuse_derivatives(pages);
     void *status = PyLong_AsVoidPtr(args[4]), *sync = PyLong_AsVoidPtr(args[5]);
     if (PyErr_Occurred()) throw python_error();
     const int64_t count = pages.size(0);
@@ -426,8 +431,9 @@ PyObject *py_cache_write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Cache &c = *cache_of(args[0]);
     const Tensor *s = ids_of(args[1], c), *b = cuda_tensor(args[2]);
     if (!s || !b || !b->is_contiguous() || b->scalar_type() != c.pages.scalar_type() || b->device() != c.pages.device() ||
-        b->dim() != c.pages.dim() || b->size(0) != s->size(0) || b->sizes().slice(1) != c.pages.sizes().slice(1) || tracked(*b))
+        b->dim() != c.pages.dim() || b->size(0) != s->size(0) || b->sizes().slice(1) != c.pages.sizes().slice(1))
         Py_RETURN_NONE;
+    refuse_derivatives(*b);
     const at::Device device = c.pages.device();
     raise_for(ygg_cache_write(device.index(), &c.c, s->size(0), (const int32_t *)s->data_ptr(), b->data_ptr(),
                               stream_of(device.index())),
