@@ -260,9 +260,11 @@ YGG_API int ygg_linear_status(int device, void *stream, int *status_out);
  * in the order of the call's list. Negative stream and page indices are padding and skipped. What cannot be done is left
  * undone and sets a status word to 1: status[YGG_CACHE_BAD_INDEX] (an index beyond its range, a child that holds pages, a
  * child named twice: its first fork counts, a table entry that names a page beyond the pool or, where compact looks for its
- * new place, one of no count: such a page reads as zeros and its entry stays), status[YGG_CACHE_NO_ROOM] (no free page, or no room in the table row),
+ * new place, one of no count: such a page reads as zeros and its entry stays), status[YGG_CACHE_NO_ROOM] (no free page, or
+ * no room in the table row),
  * status[YGG_CACHE_TIMEOUT] (a bounded wait of a call's blocks for each other gave up: the cache is not to be used any
- * more; the top bit of *sync is set, at which the waits of later calls give up too). Calls on one cache are ordered by the caller (one stream, or events). */
+ * more; the top bit of *sync is set, at which the waits of later calls give up too). Calls on one cache are ordered by the
+ * caller (one stream, or events). */
 #define YGG_CACHE_BAD_INDEX 0
 #define YGG_CACHE_NO_ROOM 1
 #define YGG_CACHE_TIMEOUT 2

@@ -782,7 +782,7 @@ int quantize(int dtype, const Quantize &p, cudaStream_t st) {
 //   256 x 256: 410, bound by the tensor cores); the epilogue 550 and 9 a column (a pair 3600), under the next tile's
 //   products.
 //   512 x 4096 x 4096: tn 128 12.1, 256 15.6; 1024 x 4096 x 4096: tn 256 16.0, 128 20.5;
-//   8192 x 4096 x 16384: pair 345, one CTA 393; 4096 x 64 x 16384: tn 256 42.1, 128 49.7, 32 105.9, pair 51.2.
+//   8192 x 4096 x 16384: pair 342, one CTA 393; 4096 x 64 x 16384: tn 256 42.1, 128 49.7, 32 105.9, pair 51.2.
 //   Sharing K costs 1650 and 16 a column more: 16 x 4096 x 4096 8.0 with 4 parts, 11.0 with one; 512 x 1024 x 4096
 //   (tn 256) 15.5 with two, 7.2 with one.
 struct Shape { int ctas, tn, parts; };
