@@ -536,3 +536,23 @@ def test_a_full_pool_says_so():
     with pytest.raises(_native.YggError) as e:
         cache.status()
     assert e.value.code == _native.YGG_E_CAPACITY and str(e.value) == "StateCache: no free page, or a full table row (-10)"
+
+
+@pytest.mark.gpu
+def test_fork_and_free_report_pages_beyond_the_pool():
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    data = torch.ones(8, 3, dtype=torch.int32, device="cuda")
+    table, refs = ints([[9, 0], [-1, -1], [1, -1], [-1, -1]]), ints([1, 1, 0, 0, 0, 0, 0, 0])
+    cache = cache_class()(data, table, ints([2, 0, 1, 0]), refs)
+    cache.fork([2], [3])
+    cache.status()
+    cache.fork([0], [1])   # shares a page 9 of 8
+    assert table[1].tolist() == [9, 3] and refs.tolist() == [1, 1, 1, 1, 0, 0, 0, 0]
+    with pytest.raises(ValueError):
+        cache.status()
+    cache.free([3])
+    cache.status()
+    cache.free([0])
+    assert table[0].tolist() == [-1, -1] and refs.tolist() == [0, 1, 0, 1, 0, 0, 0, 0]
+    with pytest.raises(ValueError):
+        cache.status()

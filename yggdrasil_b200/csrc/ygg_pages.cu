@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(kPlan, 1)
                         const int32_t page = from[j];
                         row[j] = page;
                         if (is_page(c, page)) atomicAdd(&c.refs[page], 1);
+                        else report(c.status, kBadIndex);
                     }
                 row[grow ? taken : taken - 1] = m.to;
                 c.refs[m.to] = 1;
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(256) free_kernel(const Cache c, const int32_t 
         for (int j = 0; j < held; j++) {
             const int32_t p = j ? c.table[s * c.per_stream + j] : first;
             if (is_page(c, p)) atomicSub(&c.refs[p], 1);
+            else report(c.status, kBadIndex);
             c.table[s * c.per_stream + j] = -1;
         }
     }
