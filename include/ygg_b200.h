@@ -310,6 +310,71 @@ YGG_API int ygg_cache_write(int device, const ygg_cache_t *cache, int64_t n, con
 /* Page d_to[i] = page d_from[i]. No page may be named as a destination and anywhere else. */
 YGG_API int ygg_cache_copy(int device, const ygg_cache_t *cache, int64_t n, const int32_t *d_from, const int32_t *d_to, void *stream);
 
+/* ---- linear layers with 4-bit weights ------------------------------------------------------------------------------
+ * y[m][n] = sum over groups g of scale[n][g] (sum over k in g of x[m][k] code[n][k]) + bias[n]; codes -8 to 7, x as it is,
+ * a group's sum and the sum over groups in float. Group g: inputs g group .. g group + group - 1 (the last may be cut off); group is
+ * a power of two from 32 on; k is at most YGG_LINEAR_MAX_K.
+ * Codes: for each channel ceil(k / 128) blocks of 64 bytes, the first at a multiple of 16, codes past k zero (a field of 8).
+ * Of a block's 128 inputs, four runs of 32 with four pieces of 8 each, piece t of run i is the 32-bit word 4 t + i: inputs 0,
+ * 2, 4, 6 of the piece in its fields of 4 bits 0 to 3 (from the lowest), 1, 3, 5, 7 in the fields 4 to 7, each as code + 8.
+ * Scales: [n][ceil(k / group)] of scale_dtype. */
+
+/* Scales (dtype, as the weights): a group's largest magnitude / 7, rounded to the type; a code is the nearest integer of
+ * weight / scale (one division in float, ties to even), kept within -8 to 7. A group whose scale is 0 has codes 0; one that holds NaN or
+ * infinity has scale NaN and codes 0. */
+YGG_API int ygg_fourbit_quantize(int device, int dtype, int64_t n, int64_t k, int64_t group, const void *d_weight,
+                                 int64_t row_stride, uint8_t *d_codes, void *d_scale, void *stream);
+
+/* Codes int8 [n], rows row_stride apart (their four lowest bits count), into that layout. */
+YGG_API int ygg_fourbit_pack(int device, int64_t n, int64_t k, const int8_t *d_in, int64_t row_stride, uint8_t *d_codes,
+                             void *stream);
+
+/* The product. d_bias: float [n], or NULL. */
+YGG_API int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, int64_t group, const void *d_x,
+                               int64_t row_stride, const uint8_t *d_codes, int scale_dtype, const void *d_scale,
+                               const float *d_bias, int out_dtype, void *d_out, int64_t out_stride, void *stream);
+
+/* ---- the choice over beams and vocabulary, and rows in its order ---------------------------------------------------
+ * Beam b of a prompt has scores[prompt][b] and the row of logits at prompt_stride and beam_stride entries. With lse its
+ * log sum exp, its continuation by v is worth score + (x_v - lse), in 64 bits; the best `width` of a prompt's beams x vocab
+ * continuations go on, ties by the lower beam, then the lower token. They are the exact ones: two that are nearer than
+ * float sums tell are told apart in 64 bits.
+ *   d_scores     float or double (score_bytes 4 or 8) [prompts][beams]
+ *   d_done       bytes [prompts][beams], or NULL: a beam that is done goes on with `end` alone, at no cost
+ *   end          the token after which a beam is done, or -1
+ *   d_out_scores [prompts][width] as d_scores;   d_tokens, d_parents int32 [prompts][width]
+ *   d_out_done   bytes [prompts][width], or NULL: the parent was done, or the token is `end`
+ * A beam of -inf logits alone is worth -inf everywhere, one that holds NaN or +inf is worth NaN; NaN ranks as -inf. */
+#define YGG_BEAMS_MAX 64        /* most beams, and most picks, of a prompt */
+YGG_API int ygg_beam_select(int device, int dtype, int64_t prompts, int64_t beams, int64_t vocab, const void *d_logits,
+                            int64_t prompt_stride, int64_t beam_stride, int score_bytes, const void *d_scores,
+                            const uint8_t *d_done, int64_t end, int64_t width, void *d_out_scores, int32_t *d_tokens,
+                            int32_t *d_parents, uint8_t *d_out_done, void *stream);
+
+/* Row prompt width + j of d_to[i] = row prompt beams + d_parents[prompt][j] of d_from[i] (rows of row_bytes[i] bytes, side by
+ * side), zeros where the parent is negative or beyond the beams; for `count` arrays in one launch. parent_bytes 4 or 8. No
+ * array that is read may overlap one that is written. */
+#define YGG_REORDER_MAX 8
+YGG_API int ygg_reorder(int device, int64_t prompts, int64_t beams, int64_t width, const void *d_parents, int parent_bytes,
+                        int count, const void *const *d_from, void *const *d_to, const int64_t *row_bytes, void *stream);
+
+/* ---- layer norm ----------------------------------------------------------------------------------------------------
+ * mu and r = 1 / sqrt(var + eps) of each row of x, y = (x - mu) r weight + bias; weight and bias may be NULL. y has the type
+ * of x, its rows side by side. d_stats: float [rows][2] (mu, r), 8-byte aligned, for the gradient; or NULL. */
+YGG_API int ygg_layer_norm(int device, int dtype, int64_t rows, int64_t dim, const void *d_x, int64_t row_stride,
+                           int weight_dtype, const void *d_weight, int bias_dtype, const void *d_bias, float eps, void *d_y,
+                           float *d_stats, void *stream);
+
+/* Bytes of device workspace that ygg_layer_norm_backward needs for the gradients of weight and bias. */
+YGG_API size_t ygg_layer_norm_workspace(int64_t rows, int64_t dim);
+
+/* The gradients from the one that arrives at y (type of x): d_dx (type of x, rows side by side), d_dweight and d_dbias (their
+ * types); each may be NULL. The sums over rows are joined in an order of their own: results repeat bit for bit. */
+YGG_API int ygg_layer_norm_backward(int device, int dtype, int64_t rows, int64_t dim, const void *d_x, int64_t row_stride,
+                                    int weight_dtype, const void *d_weight, int bias_dtype, const float *d_stats,
+                                    const void *d_grad, int64_t grad_stride, void *d_dx, void *d_dweight, void *d_dbias,
+                                    void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* Text of an error code. */
 YGG_API const char *ygg_strerror(int code);
 

@@ -1,0 +1,304 @@
+"""int4_linear, quantize_int4 and pack_int4 against their definition, at the sizes where the kernels change shape or can go
+wrong, and their refusals.
+
+Tolerances. Codes and scales are compared exactly: one division and one rounding each, here as there. A product of an entry
+and a code is exact or rounds once; sums are in float, in whatever order the kernel takes, which may cut a sum off instead of
+rounding it: each addition of a chain is off by at most 2^-23 of what has been summed, and no chain is longer than 64 + K / 4
+additions. The scale, the bias and the pieces of a long sum add 8 more. So a value is off by at most (72 + K / 4) 2^-23 of the sum of
+the magnitudes of its terms, and by half a spacing of its own type.
+"""
+import math
+
+import pytest
+import torch
+
+from yggdrasil_b200 import _native
+
+STEP = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -7}
+TINY = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}   # half the spacing of the smallest numbers
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def ops():
+    import yggdrasil_b200 as y
+    return y.int4_linear, y.quantize_int4, y.pack_int4
+
+
+def laid_out(codes):
+    """The layout in plain steps: codes (n, k) on the host -> uint8 (n, 64 ceil(k / 128))."""
+    n, k = codes.shape
+    out = torch.zeros(n, -(-k // 128) * 64, dtype=torch.int64)
+    for j in range(-(-k // 128) * 128):
+        block, run, piece, e = j // 128, j % 128 // 32, j % 32 // 8, j % 8
+        field = e // 2 + e % 2 * 4
+        at = block * 64 + (piece * 4 + run) * 4 + field // 2
+        q = codes[:, j].long() if j < k else torch.zeros(n, dtype=torch.int64)
+        out[:, at] |= (q + 8 & 15) << field % 2 * 4
+    return out.to(torch.uint8)
+
+
+def weights(n, k, group, scale_dtype=torch.float32, seed=0, bias=True):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8)
+    scale = (torch.rand(n, -(-k // group), generator=g) * 0.1 + 0.01).to(scale_dtype)
+    b = torch.randn(n, generator=g) if bias else None
+    return codes.cuda(), scale.cuda(), None if b is None else b.cuda()
+
+
+def inputs(rows, k, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + 100)
+    x = torch.randn(rows, k, generator=g) * (torch.rand(rows, 1, generator=g) * 10 + 0.01) + 0.5
+    return x.to(dtype).cuda()
+
+
+def check(y, x, codes, scale, group, bias, dtype):
+    k = codes.shape[1]
+    w = codes.double() * scale.double().repeat_interleave(group, 1)[:, :k]
+    want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    assert y.dtype == dtype and y.shape == want.shape
+    tol = (72 + k / 4) * 2.0 ** -23 * size + STEP[dtype] / 2 * want.abs() * (1 + 2.0 ** -10) + TINY[dtype]
+    edge = {torch.float32: 2.0 ** 128, torch.float16: 65520.0, torch.bfloat16: 2.0 ** 128}[dtype]
+    assert want.abs().max() < edge * 0.9
+    off = ((y.double() - want).abs() / tol).max().item()
+    assert off <= 1, f"off by {off}"
+
+
+SIZES = [(1, 1, 1, 32), (1, 16, 1, 128), (1, 31, 17, 32), (1, 1280, 256, 32), (1, 4096, 1000, 128), (2, 100, 33, 64),
+         (2, 4100, 130, 128), (3, 4097, 257, 64), (4, 512, 256, 512), (5, 1000, 515, 32), (7, 33, 129, 64), (8, 2048, 2047, 256),
+         (9, 96, 128, 32), (11, 2500, 100, 128), (15, 8191, 130, 128), (16, 512, 4099, 64), (17, 64, 300, 32), (24, 1024, 96, 128),
+         (31, 640, 1000, 128), (33, 129, 128, 32), (64, 1000, 257, 64), (77, 1000, 5003, 128), (127, 512, 640, 128),
+         (128, 128, 128, 32), (129, 257, 129, 64), (200, 4096, 16, 128), (256, 384, 256, 2048), (257, 1024, 513, 128),
+         (300, 5000, 1030, 64), (513, 272, 5, 32), (1000, 64, 256, 64), (1025, 1500, 1100, 128), (4099, 512, 256, 32),
+         (65537, 64, 5, 32), (1, 20000, 300, 128), (6, 16384, 260, 64), (12, 9000, 40, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,n,group", SIZES)
+def test_values(rows, k, n, group, dtype):
+    f, _, pack = ops()
+    x = inputs(rows, k, dtype, seed=k)
+    codes, scale, b = weights(n, k, group, dtype, seed=n, bias=n % 2 == 1)
+    if dtype == torch.float16:   # keeps the outputs within its range
+        x = x / 16
+    check(f(x, pack(codes, scale, group), b), x, codes, scale, group, b, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 9, 40, 130])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale_dtype", TYPES)
+@pytest.mark.parametrize("out_dtype", TYPES)
+def test_every_combination_of_types(rows, dtype, scale_dtype, out_dtype):
+    f, _, pack = ops()
+    x = inputs(rows, 700, dtype, seed=rows) / 8
+    codes, scale, b = weights(90, 700, 64, scale_dtype, seed=rows)
+    for bias in (b, b.to(torch.bfloat16)):
+        check(f(x, pack(codes, scale, 64), bias, out_dtype), x, codes, scale, 64, bias, out_dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 131072, 40), (3, 131072, 5), (20, 100003, 300), (130, 65552, 130)])
+def test_long_rows_with_the_largest_codes(rows, k, n):
+    f, _, pack = ops()
+    x = torch.full((rows, k), 3.0, device="cuda")
+    codes, scale, b = weights(n, k, 128)
+    codes.fill_(-8)
+    codes[1::2] = 7
+    check(f(x, pack(codes, scale, 128), b), x, codes, scale, 128, b, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 4, 20, 200])
+def test_entries_of_all_sizes(rows):
+    """float32 rows of magnitudes from 2^-130 to 2^100, each with all its 24 bits."""
+    f, _, pack = ops()
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 300, generator=g).cuda() * torch.linspace(-100, 100, rows).exp2().cuda()[:, None]
+    x[-1] = torch.finfo(torch.float32).max / 2 ** 12 * (torch.arange(300, device="cuda") % 3 - 1)
+    codes, scale, b = weights(50, 300, 32)
+    check(f(x, pack(codes, scale, 32), b), x, codes, scale, 32, b, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 5, 30, 150])
+def test_infinities_and_nan_stay_in_their_rows(rows, dtype):
+    f, _, pack = ops()
+    x = inputs(rows, 300, dtype, seed=1) / 16
+    codes, scale, b = weights(40, 300, 64)
+    codes[:, 7] = torch.tensor([3, -2], dtype=torch.int8, device="cuda").repeat(20)
+    want = f(x, pack(codes, scale, 64), b)
+    x[0, 7] = math.inf
+    got = f(x, pack(codes, scale, 64), b)
+    assert torch.equal(got[0], torch.tensor([math.inf, -math.inf], device="cuda").repeat(20).to(dtype))
+    assert torch.equal(got[1:], want[1:])
+    x[0, 7] = math.nan
+    got = f(x, pack(codes, scale, 64), b)
+    assert got[0].isnan().all() and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 31, 32), (5, 129, 64), (9, 1000, 128), (300, 255, 256), (4, 4096, 32),
+                                       (2, 20001, 131072), (7, 64, 1024)])
+def test_codes_and_scales(n, k, group, dtype):
+    _, quantize, _ = ops()
+    g = torch.Generator().manual_seed(n)
+    w = (torch.randn(n, k, generator=g) * torch.rand(n, 1, generator=g)).to(dtype)
+    if n > 2:
+        w[1] = 0
+        w[2, -1] = math.inf
+    got = quantize(w.cuda(), group)
+    assert (got.k, got.group) == (k, group)
+    groups = -(-k // group)
+    padded = torch.zeros(n, groups * group)
+    padded[:, :k] = w.float()
+    padded = padded.view(n, groups, group)
+    most = padded.abs().amax(-1)
+    scale = torch.where(most.isfinite(), most / torch.full_like(most, 7.0), math.nan).to(dtype)
+    assert torch.equal(got.scale.cpu().view(n, groups).nan_to_num(nan=-1.0), scale.nan_to_num(nan=-1.0))
+    codes = torch.where(scale.float()[:, :, None] > 0, padded / scale.float()[:, :, None], 0.0).round().clamp(-8, 7)
+    codes = codes.nan_to_num(nan=0.0).view(n, -1)[:, :k].to(torch.int8)
+    assert torch.equal(got.codes.cpu(), laid_out(codes))
+
+
+@pytest.mark.gpu
+def test_packed_codes_lie_as_stated():
+    _, _, pack = ops()
+    for n, k in ((1, 1), (3, 127), (5, 128), (2, 1000)):
+        codes, scale, _ = weights(n, k, 64, seed=k)
+        assert torch.equal(pack(codes, scale, 64).codes.cpu(), laid_out(codes.cpu()))
+        wide = torch.zeros(n, 2 * k, dtype=torch.int8, device="cuda")[:, ::2]
+        assert torch.equal(pack(wide.copy_(codes), scale, 64).codes.cpu(), laid_out(codes.cpu()))
+    for value in (8, -9):
+        codes[1, 999] = value
+        with pytest.raises(ValueError):
+            pack(codes, scale, 64)
+
+
+@pytest.mark.gpu
+def test_quantised_weights_are_near():
+    f, quantize, _ = ops()
+    w = torch.randn(200, 700, device="cuda")
+    x = torch.randn(10, 700, device="cuda")
+    y, want = f(x, quantize(w, 32)), x @ w.T
+    assert (y - want).norm() < 0.12 * want.norm()   # a code is off by up to half a step of max / 7 in a group of 32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 6, 50])
+def test_strides_shapes_and_no_rows(rows):
+    f, _, pack = ops()
+    x = inputs(rows, 333, torch.bfloat16)
+    codes, scale, b = weights(70, 333, 64)
+    w = pack(codes, scale, 64)
+    want = f(x, w, b)
+    wide = torch.full((rows, 700), math.nan, dtype=torch.bfloat16, device="cuda")
+    for off in (0, 1, 3, 8):
+        wide[:, off:off + 333] = x
+        assert torch.equal(f(wide[:, off:off + 333], w, b), want)
+    assert torch.equal(f(x.T.contiguous().T, w, b), want)
+    assert torch.equal(f(x[None, :, None], w, b), want[None, :, None])
+    assert torch.equal(f(x[0], w, b), f(x[:1], w, b)[0])
+    assert f(x[:0], w, b).shape == (0, 70)
+    moved = torch.empty(70 * 192 + 1, dtype=torch.uint8, device="cuda")[1:].view(70, 192).copy_(w.codes)
+    assert torch.equal(f(x, w._replace(codes=moved, scale=w.scale.T.contiguous().T), b), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 300, 200), (8, 4096, 1000), (40, 1000, 300), (300, 2000, 600)])
+def test_other_streams_and_graphs(rows, k, n):
+    f, _, pack = ops()
+    x = inputs(rows, k, torch.bfloat16)
+    codes, scale, b = weights(n, k, 128)
+    w = pack(codes, scale, 128)
+    want = f(x, w, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = f(x, w, b)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graphs, outs = [], []
+    for _ in range(2):   # two graphs do not share what they work in
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(f(x, w, b))
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, want) for got in outs)
+
+
+@pytest.mark.gpu
+def test_outputs_stay_in_their_rows():
+    f, _, pack = ops()
+    lib = _native.ops()
+    for rows, k, n in ((1, 100, 77), (5, 100, 77), (50, 100, 77), (200, 300, 259)):
+        x = inputs(rows, k, torch.float32)
+        codes, scale, b = weights(n, k, 32)
+        w = pack(codes, scale, 32)
+        frame = torch.full((rows + 2, n + 9), -5.0, device="cuda")
+        out = frame[1:-1, 4:4 + n]
+        rc = lib.ygg_fourbit_linear(0, 0, rows, k, n, 32, x.data_ptr(), x.stride(0), w.codes.data_ptr(), 0, scale.data_ptr(),
+                                    b.data_ptr(), 0, out.data_ptr(), out.stride(0), torch.cuda.current_stream().cuda_stream)
+        assert rc == _native.YGG_OK
+        assert torch.equal(out, f(x, w, b))
+        keep = frame.clone()
+        keep[1:-1, 4:4 + n] = -5.0
+        assert bool((keep == -5.0).all())
+
+
+@pytest.mark.gpu
+def test_refusals():
+    f, quantize, pack = ops()
+    x = inputs(4, 64, torch.float32)
+    codes, s, b = weights(20, 64, 32)
+    w = pack(codes, s, 32)
+    for bad in (x.double(), x.cpu(), x[:, :63], torch.empty(4, 0, device="cuda"), "x"):
+        with pytest.raises(ValueError):
+            f(bad, w, b)
+    for bad in (w._replace(codes=w.codes[:, :32]), w._replace(codes=w.codes.cpu()), w._replace(codes=codes), w._replace(k=63),
+                w._replace(group=64), w._replace(group=48), w._replace(scale=s.double()), w._replace(scale=s[:19]),
+                w._replace(scale=s.cpu()), w.codes, None, w._replace(codes=w.codes[:0], scale=s[:0])):
+        with pytest.raises(ValueError):
+            f(x, bad, b)
+    for bad in (b[:19], b.double(), b.cpu()):
+        with pytest.raises(ValueError):
+            f(x, w, bad)
+    with pytest.raises(ValueError):
+        f(x, w, b, out_dtype=torch.int32)
+    for bad in ((torch.zeros(1, 131073, device="cuda"), 32), (x, 16), (x, 100), (x, 2.0), (x[0], 32), (x.cpu(), 32), (x[:0], 32)):
+        with pytest.raises(ValueError):
+            quantize(*bad)
+    for bad in ((codes.int(), s, 32), (codes, s, 64), (codes, s.double(), 32), (codes[0], s, 32), (codes.cpu(), s, 32)):
+        with pytest.raises(ValueError):
+            pack(*bad)
+    for args in ((x.clone().requires_grad_(), w, b), (x, w._replace(scale=s.clone().requires_grad_()), b),
+                 (x, w, b.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError):
+            f(*args)
+        with torch.no_grad():
+            f(*args)
+    with pytest.raises(NotImplementedError):
+        quantize(x.clone().requires_grad_(), 32)
+
+
+def test_c_entry_refuses_bad_arguments():
+    lib = _native.ops()
+    linear = lambda rows=1, k=64, n=4, group=32, dtype=0, sd=0, od=0, x=16, codes=16, s=16, out=16: lib.ygg_fourbit_linear(  # noqa: E731
+        0, dtype, rows, k, n, group, x, k, codes, sd, s, None, od, out, n, None)
+    for kw in (dict(rows=-1), dict(k=0), dict(n=0), dict(group=31), dict(group=96), dict(x=None), dict(codes=None), dict(s=None),
+               dict(out=None), dict(codes=24)):
+        assert linear(**kw) == _native.YGG_E_ARG, kw
+    for kw in (dict(k=131073), dict(group=1 << 18), dict(sd=3), dict(od=-1)):
+        assert linear(**kw) == _native.YGG_E_UNSUPPORTED, kw
+    assert linear(rows=0, x=None) == _native.YGG_OK
+    assert lib.ygg_fourbit_quantize(0, 0, 1, 1, 32, None, 1, 16, 16, None) == _native.YGG_E_ARG
+    assert lib.ygg_fourbit_quantize(0, 0, 1, 131073, 32, 16, 1, 16, 16, None) == _native.YGG_E_UNSUPPORTED
+    assert lib.ygg_fourbit_pack(0, 1, 1, None, 1, 16, None) == _native.YGG_E_ARG
+    assert lib.ygg_fourbit_pack(0, 1, 1, 16, 1, 24, None) == _native.YGG_E_ARG

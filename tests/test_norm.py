@@ -1,0 +1,306 @@
+"""layer_norm against its formulas in 64 bits: values and gradients, at the sizes where the kernels change shape or can go
+wrong, and its refusals.
+
+Tolerances, with u = 2^-24 and chains of at most c = 32 + D / 64 additions. The mean is off by dm = c u mean|x|; a difference x - mu
+by dm + u |x - mu|; its square's mean by a relative (c + 3) u (and dm^2, which the mean of the squares then holds too, as all of its
+terms shift together); 1 / sqrt by half of that and 4 u. So h = (x - mu) r is off by dh = r dm (1 + |h|^2 r dm) + |h| (c + 8) u, and
+y = h w + b by |w| dh + 2 u (|h w| + |b|) and half a spacing of its type. With gw = g w, a = mean gw and q = mean gw h, a is off by
+da = (c + 2) u mean|gw|, q by dq = (c + 3) u mean|gw h| + mean(|gw| dh), and dx = r (gw - a - h q) by r (da + |h| dq + |q| dh) +
+(c + 12) u r (|gw| + |a| + |h q|) and half a spacing. A sum over R rows has chains of at most 64 + R / 32 additions: dw is off by
+sum(|g| dh) + (66 + R / 32) u sum|g h|, db by (65 + R / 32) u sum|g|, and half a spacing.
+"""
+import math
+
+import pytest
+import torch
+
+from yggdrasil_b200 import _native
+
+STEP = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -7}
+TINY = {torch.float32: 2.0 ** -150, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+U = 2.0 ** -24
+
+
+def op():
+    from yggdrasil_b200 import layer_norm
+    return layer_norm
+
+
+def make(rows, dim, dtype, seed=0, shift=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, dim, generator=g) * (torch.rand(rows, 1, generator=g) * 3 + 0.1) + shift * torch.randn(rows, 1, generator=g)
+    w, b = 1 + 0.3 * torch.randn(dim, generator=g), torch.randn(dim, generator=g)
+    d = torch.randn(rows, dim, generator=g)
+    return x.to(dtype).cuda(), w.cuda(), b.cuda(), d.to(dtype).cuda()
+
+
+def rounded(want, off, dtype):
+    return off + STEP[dtype] / 2 * (want.abs() + off) + TINY[dtype]
+
+
+def near(got, want, off, dtype, what):
+    assert got.dtype == dtype and got.shape == want.shape
+    far = ((got.double() - want).abs() / rounded(want, off, dtype)).max().item() if want.numel() else 0
+    assert far <= 1, f"{what} off by {far}"
+
+
+def formulas(x, w, b, eps):
+    dim = x.shape[-1]
+    c = 32 + dim / 64
+    x = x.double().reshape(-1, dim)
+    w = torch.ones(dim, device="cuda").double() if w is None else w.double()
+    b = torch.zeros(dim, device="cuda").double() if b is None else b.double()
+    mu = x.mean(-1, keepdim=True)
+    r = 1 / ((x - mu).square().mean(-1, keepdim=True) + eps).sqrt()
+    h = (x - mu) * r
+    dm = c * U * x.abs().mean(-1, keepdim=True)
+    dh = r * dm * (1 + h.square() * r * dm) + h.abs() * (c + 8) * U
+    return c, w, b, r, h, dh
+
+
+def check_values(y, x, w, b, eps):
+    c, w, b, r, h, dh = formulas(x, w, b, eps)
+    want = h * w + b
+    near(y.reshape(want.shape), want, w.abs() * dh + 2 * U * ((h * w).abs() + b.abs()), x.dtype, "y")
+
+
+def check_gradients(grads, types, x, w, b, g, eps):
+    c, w, b, r, h, dh = formulas(x, w, b, eps)
+    g = g.double().reshape(h.shape)
+    rows = len(g)
+    gw = g * w
+    mean = lambda v: v.mean(-1, keepdim=True)  # noqa: E731
+    a, q = mean(gw), mean(gw * h)
+    da, dq = (c + 2) * U * mean(gw.abs()), (c + 3) * U * mean((gw * h).abs()) + mean(gw.abs() * dh)
+    want = [r * (gw - a - h * q), (g * h).sum(0), g.sum(0)]
+    off = [r * (da + h.abs() * dq + q.abs() * dh) + (c + 12) * U * r * (gw.abs() + a.abs() + (h * q).abs()),
+           (g.abs() * dh).sum(0) + (66 + rows / 32) * U * (g * h).abs().sum(0), (65 + rows / 32) * U * g.abs().sum(0)]
+    for got, value, tol, dtype, what in zip(grads, want, off, types, ("dx", "dw", "db")):
+        if got is not None:
+            near(got.reshape(value.shape), value, tol, dtype, what)
+
+
+SIZES = [(1, 1), (1, 2), (3, 5), (2, 31), (5, 32), (4, 33), (7, 100), (1, 1280), (33, 256), (65, 255), (9, 1000), (130, 1024), (17, 1025),
+         (3, 4096), (200, 2048), (5, 4099), (2, 8192), (3, 12000), (1, 16384), (2, 20001), (1, 100003), (1003, 96), (4097, 8), (600, 513),
+         (20000, 3), (300, 4096)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", SIZES)
+def test_values_and_gradients(rows, dim, dtype):
+    f = op()
+    x, w, b, g = make(rows, dim, dtype, seed=dim)
+    for own in (dtype, torch.float32) if dtype != torch.float32 else (dtype,):
+        leaves = [x.clone().requires_grad_(), w.to(own).requires_grad_(), b.to(own).requires_grad_()]
+        y = f(*leaves)
+        check_values(y.detach(), x, leaves[1].detach(), leaves[2].detach(), 1e-5)
+        assert torch.equal(f(x, leaves[1].detach(), leaves[2].detach()), y)
+        grads = torch.autograd.grad(y, leaves, g)
+        check_gradients(grads, (dtype, own, own), x, leaves[1].detach(), leaves[2].detach(), g, 1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_weight", [False, True])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("rows,dim", [(5, 70), (40, 1000), (3, 9000)])
+def test_absent_parts_and_single_gradients(rows, dim, with_weight, with_bias):
+    f = op()
+    x, w, b, g = make(rows, dim, torch.float32, seed=rows)
+    w, b = w if with_weight else None, b if with_bias else None
+    for wanted in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1), (1, 1, 1)):
+        leaves = [None if v is None else v.clone().requires_grad_(bool(n)) for v, n in zip((x, w, b), wanted)]
+        y = f(*leaves, eps=1e-3)
+        check_values(y.detach(), x, w, b, 1e-3)
+        asked = [v for v in leaves if v is not None and v.requires_grad]
+        if not asked:
+            assert not y.requires_grad
+            continue
+        found = iter(torch.autograd.grad(y, asked, g))
+        grads = [next(found) if v is not None and v.requires_grad else None for v in leaves]
+        check_gradients(grads, [torch.float32] * 3, x, w, b, g, 1e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [6, 200, 5000])
+def test_gradients_against_differences(dim):
+    f = op()
+    x, w, b, g = make(2, dim, torch.float32, seed=dim + 1)
+    leaves = [x.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+    grads = torch.autograd.grad(f(*leaves), leaves, g)
+
+    def loss(x, w, b):
+        mu = x.mean(-1, keepdim=True)
+        return (((x - mu) / ((x - mu).square().mean(-1, keepdim=True) + 1e-5).sqrt() * w + b) * g.double()).sum()
+
+    for i, leaf in enumerate(leaves):
+        at = [v.detach().double() for v in leaves]
+        way = torch.randn(leaf.shape, generator=torch.Generator().manual_seed(i)).double().cuda()
+        step = 1e-5   # central differences: off by about step^2, and 2^-53 of the loss / step
+        up = loss(*[v + step * way if j == i else v for j, v in enumerate(at)])
+        down = loss(*[v - step * way if j == i else v for j, v in enumerate(at)])
+        size = (grads[i].double() * way).abs().sum()
+        assert abs((up - down) / (2 * step) - (grads[i].double() * way).sum()) < 1e-5 * size + 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_means_and_equal_rows(dtype):
+    f = op()
+    x, w, b, g = make(6, 700, dtype, seed=3, shift=50.0)
+    x[2] = 3.0        # no variance: r = 1 / sqrt(eps)
+    x[3] = 0.0
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+    y = f(*leaves)
+    check_values(y.detach(), x, w, b, 1e-5)
+    check_gradients(torch.autograd.grad(y, leaves, g), (dtype, torch.float32, torch.float32), x, w, b, g, 1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [100, 1024, 6000])
+def test_nan_and_infinity_stay_in_their_rows(dim):
+    f = op()
+    x, w, b, g = make(5, dim, torch.float32, seed=4)
+    good = x.clone().requires_grad_()
+    want = f(good, w, b)
+    want_dx, = torch.autograd.grad(want, good, g)
+    for value in (math.nan, math.inf):
+        bad = x.clone()
+        bad[1, dim // 2] = value
+        bad.requires_grad_()
+        y = f(bad, w, b)
+        dx, = torch.autograd.grad(y, bad, g)
+        assert y[1].isnan().all() and dx[1].isnan().all()
+        for i in (0, 2, 3, 4):
+            assert torch.equal(y[i], want[i]) and torch.equal(dx[i], want_dx[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [100, 128, 2049])
+def test_strides_shapes_and_no_rows(dim, dtype):
+    f = op()
+    x, w, b, g = make(6, dim, dtype, seed=5)
+    want = f(x, w, b)
+    leaf = x.clone().requires_grad_()
+    want_dx, = torch.autograd.grad(f(leaf, w, b), leaf, g)
+    wide = torch.full((6, dim + 20), math.nan, dtype=dtype, device="cuda")
+    for off in (0, 1, 3, 8):
+        part = wide[:, off:off + dim]
+        part.copy_(x)
+        assert torch.equal(f(part, w, b), want)
+        part = part.detach().requires_grad_()
+        arriving = torch.zeros(6, dim + 9, dtype=dtype, device="cuda")[:, off:off + dim].copy_(g)
+        got, = torch.autograd.grad(f(part, w, b), part, arriving)
+        assert torch.equal(got, want_dx)
+    assert torch.equal(f(x.T.contiguous().T, w, b), want)
+    assert torch.equal(f(x.view(2, 3, dim), w, b), want.view(2, 3, dim))
+    assert torch.equal(f(x.view(2, 3, dim).transpose(0, 1), w, b), want.view(2, 3, dim).transpose(0, 1))
+    assert torch.equal(f(x[0], w, b), want[0])
+    assert torch.equal(f(x, torch.stack([w, w], 1)[:, 0], b), want)
+    turned = leaf.view(2, 3, dim).transpose(0, 1)
+    got, = torch.autograd.grad(f(turned, w, b).transpose(0, 1), leaf, g.view(2, 3, dim))
+    assert torch.equal(got, want_dx)
+    one = x.clone().requires_grad_()
+    a, = torch.autograd.grad(f(one, w, b).sum(), one)   # an expanded gradient arrives
+    one = x.clone().requires_grad_()
+    c, = torch.autograd.grad(f(one, w, b), one, torch.ones_like(x))
+    assert torch.equal(a, c)
+    none = x[:0].clone().requires_grad_()
+    weight = w.clone().requires_grad_()
+    y = f(none, weight, b)
+    dx, dw = torch.autograd.grad(y, [none, weight], g[:0])
+    assert y.shape == dx.shape == (0, dim) and not dw.any()
+    same = x[:1].expand(6, dim)
+    assert torch.equal(f(same, w, b), want[:1].expand(6, dim))
+
+
+@pytest.mark.gpu
+def test_shared_leaves_and_two_uses():
+    """A weight used twice gets both gradients, and x may be the weight's own row."""
+    f = op()
+    x, w, b, g = make(4, 64, torch.float32, seed=6)
+    weight = w.clone().requires_grad_()
+    y = f(f(x, weight, b), weight, b)
+    dw, = torch.autograd.grad(y, weight, g)
+    one, two = w.clone().requires_grad_(), w.clone().requires_grad_()
+    parts = torch.autograd.grad(f(f(x, one, b), two, b), [one, two], g)
+    torch.testing.assert_close(dw, parts[0] + parts[1], rtol=0, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim", [(3, 100), (500, 300), (4, 20000)])
+def test_other_streams_and_graphs(rows, dim):
+    f = op()
+    x, w, b, g = make(rows, dim, torch.bfloat16, seed=7)
+    leaves = [x.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+
+    def both():
+        y = f(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, g)]
+
+    want = both()
+    assert all(torch.equal(a, c) for a, c in zip(both(), want))   # repeats bit for bit
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    with torch.cuda.stream(side):   # an eager graph of the same leaves, alive while another is captured (torch refuses one of
+        alive = f(*leaves)          # the default stream there, whatever the operator)
+    side.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(both())
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for got in outs for a, c in zip(got, want))
+    assert torch.equal(torch.autograd.grad(alive, leaves, g)[1], want[2])
+
+
+@pytest.mark.gpu
+def test_refusals():
+    import torch.autograd.forward_ad as fw
+    f = op()
+    x, w, b, g = make(4, 50, torch.float32)
+    for bad in (x.double(), x.int(), x.cpu(), "x", torch.empty(3, 0, device="cuda"), torch.tensor(1.0, device="cuda")):
+        with pytest.raises(ValueError):
+            f(bad, w, b)
+    for bad in (w[:49], w.double(), w.cpu(), w[None], "w"):
+        with pytest.raises(ValueError):
+            f(x, bad, b)
+        with pytest.raises(ValueError):
+            f(x, w, bad)
+    for eps in (-1.0, math.inf, math.nan, "0", None, True):
+        with pytest.raises(ValueError):
+            f(x, w, b, eps)
+    f(x, w, b, 0)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(f(leaf, w, b), leaf, g, create_graph=True)
+    with fw.dual_level():
+        for args in ((fw.make_dual(x, g), w, b), (x, fw.make_dual(w, w), b), (x.T.contiguous().T, w, fw.make_dual(b, b))):
+            with pytest.raises(NotImplementedError):
+                f(*args)
+
+
+def test_c_entries_refuse_bad_arguments():
+    lib = _native.ops()
+    forward = lambda rows=1, dim=8, dtype=0, wt=0, bt=0, x=16, y=16: lib.ygg_layer_norm(  # noqa: E731
+        0, dtype, rows, dim, x, dim, wt, None, bt, None, 1e-5, y, None, None)
+    for kw in (dict(rows=-1), dict(dim=0), dict(x=None), dict(y=None)):
+        assert forward(**kw) == _native.YGG_E_ARG, kw
+    for kw in (dict(dim=1 << 31), dict(wt=3), dict(bt=-1)):
+        assert forward(**kw) == _native.YGG_E_UNSUPPORTED, kw
+    assert forward(rows=0, x=None) == _native.YGG_OK
+    assert lib.ygg_layer_norm_workspace(-1, 8) == lib.ygg_layer_norm_workspace(4, 0) == 0
+    backward = lambda rows=1, dim=8, dtype=0: lib.ygg_layer_norm_backward(  # noqa: E731
+        0, dtype, rows, dim, 16, dim, 0, None, 0, 16, 16, dim, 16, 16, 16, 16, 0, None)
+    assert backward(rows=-1) == backward(dim=0) == _native.YGG_E_ARG
+    assert backward(dtype=5) == _native.YGG_E_UNSUPPORTED

@@ -1,0 +1,313 @@
+"""beam_select and reorder_states against their definition: the choice in 64 bits, at the sizes and masks where the kernels
+change shape or can go wrong, and their refusals.
+
+Tolerances. Tokens, parents and the done flags are compared exactly. A score in float32 is its 64-bit value rounded once, where that
+value is off by at most (64 + V / 256) 2^-24 from the sum of exponentials and 2^-21 from exp2 and its argument (each only moves
+lse); in float64 it is off by at most V 2^-52 and the roundings of three additions.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from yggdrasil_b200 import _native
+
+INF = math.inf
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def ops():
+    import yggdrasil_b200 as y
+    return y.beam_select, y.reorder_states
+
+
+def plain(logits, scores, width, done=None, end=None):
+    """The definition, prompt by prompt, in float64 on the host."""
+    x, s = logits.double().cpu().numpy(), scores.double().cpu().numpy()
+    prompts, beams, vocab = x.shape
+    was = np.zeros((prompts, beams), bool) if done is None else done.cpu().numpy()
+    with np.errstate(all="ignore"):
+        m = x.max(-1, keepdims=True)
+        bad = np.isnan(x).any(-1) | (m[:, :, 0] == INF)
+        empty = m[:, :, 0] == -INF
+        e = np.exp(x - np.where(np.isfinite(m), m, 0))
+        lse = np.where(np.isfinite(m), m, 0) + np.log(e.sum(-1, keepdims=True))
+        total = s[:, :, None] + np.where(empty[:, :, None], -INF, x - lse)
+        total[bad] = math.nan
+        for p, b in zip(*np.nonzero(was)):
+            total[p, b] = -INF
+            total[p, b, end] = s[p, b]
+    flat = total.reshape(prompts, -1)
+    rank = np.where(np.isnan(flat), -INF, flat)
+    best = np.argsort(-rank, axis=1, kind="stable")[:, :width]
+    parent = best // vocab
+    token = np.where(np.take_along_axis(was, parent, 1), end if end is not None else -1, best % vocab)
+    over = np.take_along_axis(was, parent, 1) | (token == (-1 if end is None else end))
+    return np.take_along_axis(flat, best, 1), token, parent, over
+
+
+def check(out, logits, scores, width, done=None, end=None):
+    value, token, parent, over = plain(logits, scores, width, done, end)
+    assert out.tokens.dtype == out.parents.dtype == torch.int32 and out.scores.dtype == scores.dtype
+    np.testing.assert_array_equal(out.parents.cpu().numpy(), parent)
+    np.testing.assert_array_equal(out.tokens.cpu().numpy(), token)
+    if end is None:
+        assert out.done is None
+    else:
+        np.testing.assert_array_equal(out.done.cpu().numpy(), over)
+    got = out.scores.double().cpu().numpy()
+    vocab = logits.shape[2]
+    fine = np.isfinite(value)
+    np.testing.assert_array_equal(got[~fine], value[~fine])
+    size = np.abs(value[fine]) + float(scores[scores.isfinite()].abs().max() if scores.isfinite().any() else 0.0) + \
+        float(logits[logits.isfinite()].float().abs().clamp(max=1e4).max() if logits.isfinite().any() else 0.0)
+    if scores.dtype == torch.float64:
+        tol = vocab * 2.0 ** -52 + 8 * 2.0 ** -53 * size
+    else:
+        tol = (64 + vocab / 256) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -24 * np.abs(value[fine]) * 1.001
+    assert (np.abs(got[fine] - value[fine]) <= tol).all(), np.max(np.abs(got[fine] - value[fine]) / tol)
+
+
+def make(prompts, beams, vocab, dtype, mask="none", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(prompts, beams, vocab, generator=g) * (torch.rand(prompts, beams, 1, generator=g) * 4 + 0.5)
+    if mask == "half":
+        x[torch.rand(x.shape, generator=g) < 0.5] = -INF
+    elif mask == "lowest":
+        x[torch.rand(x.shape, generator=g) < 0.5] = torch.finfo(dtype).min
+    elif mask == "few":          # a handful of open tokens in all, fewer than some widths
+        keep = torch.rand(x.shape, generator=g) < 2.0 / vocab
+        x[~keep] = -INF
+    elif mask == "rows":         # beams with nothing open
+        x[torch.rand(prompts, beams, generator=g) < 0.5] = -INF
+    elif mask == "wrong":        # NaN and +inf
+        x[torch.rand(x.shape, generator=g) < 0.3 / vocab] = math.nan
+        x[torch.rand(x.shape, generator=g) < 0.3 / vocab] = INF
+        x[torch.rand(x.shape, generator=g) < 0.1] = -INF
+    elif mask == "equal":
+        x.zero_()
+    elif mask == "steps":        # many ties within a beam
+        x = (x * 2).round()
+    scores = -5 * torch.rand(prompts, beams, generator=g) - 1
+    return x.to(dtype).cuda(), scores.cuda()
+
+
+SIZES = [(1, 1, 1, 1), (1, 1, 5, 5), (1, 4, 256, 4), (3, 2, 20, 16), (2, 64, 3, 64), (5, 3, 31, 7), (7, 4, 256, 4), (33, 5, 256, 8),
+         (2, 1, 257, 64), (4, 8, 300, 16), (3, 16, 1000, 12), (1, 1, 4096, 4), (2, 5, 4099, 5), (1, 3, 8192, 64), (9, 2, 2048, 3),
+         (2, 7, 16385, 10), (1, 4, 32768, 8), (3, 5, 50257, 5), (1, 1, 131072, 1), (1, 64, 5000, 64), (2, 2, 100003, 33),
+         (300, 4, 256, 4), (1000, 2, 27, 3), (2000, 1, 9, 2), (130, 8, 1025, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("prompts,beams,vocab,width", SIZES)
+def test_choice(prompts, beams, vocab, width, dtype):
+    f, _ = ops()
+    x, s = make(prompts, beams, vocab, dtype, seed=vocab)
+    check(f(x, s, width), x, s, width)
+    done = torch.rand(prompts, beams, device="cuda") < 0.3
+    check(f(x, s, width, done=done, end=vocab // 2), x, s, width, done, vocab // 2)
+    check(f(x, s.double(), width, end=0), x, s.double(), width, None, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", ["half", "lowest", "few", "rows", "wrong", "equal", "steps"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("prompts,beams,vocab,width", [(1, 4, 256, 4), (40, 4, 256, 16), (5, 3, 33, 40), (2, 5, 5000, 10),
+                                                       (2, 6, 30001, 7), (1, 2, 70000, 64), (300, 2, 100, 5)])
+def test_masks_and_ties(prompts, beams, vocab, width, dtype, mask):
+    f, _ = ops()
+    x, s = make(prompts, beams, vocab, dtype, mask, seed=prompts + vocab)
+    check(f(x, s, width), x, s, width)
+    done = torch.rand(prompts, beams, device="cuda") < 0.3
+    check(f(x, s, width, done=done, end=1), x, s, width, done, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,width", [(256, 4), (2000, 8), (40000, 8), (100003, 5)])
+def test_beams_nearer_than_sums_in_32_bits_tell(vocab, width, dtype):
+    """Beams that hold the same logits in another order, with scores a spacing of 2^-33 apart: their continuations interleave, and
+    sums in 32 bits would put them in any order."""
+    f, _ = ops()
+    for seed in range(6):
+        g = torch.Generator().manual_seed(seed)
+        row = torch.randn(vocab, generator=g) * 3
+        x = torch.stack([row[torch.randperm(vocab, generator=g)] for _ in range(4)])[None].to(dtype).cuda()
+        s = (2.0 ** -10 + torch.randperm(4, generator=g) * 2.0 ** -33)[None].float().cuda()
+        assert len(set(s.flatten().tolist())) == 4
+        check(f(x, s, width), x, s, width)
+        check(f(x, s.double(), width), x, s.double(), width)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,width", [(256, 4), (3000, 9), (60000, 12)])
+def test_equal_beams_by_the_lower_one(vocab, width):
+    f, _ = ops()
+    x, s = make(3, 5, vocab, torch.float32, seed=7)
+    x[:, 3], s[:, 3] = x[:, 1], s[:, 1]
+    x[:, 2], s[:, 2] = x[:, 1], s[:, 1]
+    check(f(x, s, width), x, s, width)
+
+
+@pytest.mark.gpu
+def test_scores_that_are_not_finite():
+    f, _ = ops()
+    x, _ = make(2, 5, 300, torch.float32, "half", seed=2)
+    s = torch.tensor([[-INF, -1.0, INF, math.nan, -2.0], [-INF, -INF, -INF, -INF, -INF]], device="cuda")
+    for width in (3, 60):
+        check(f(x, s, width), x, s, width)
+        done = torch.tensor([[True, False, False, True, True]] * 2, device="cuda")
+        check(f(x, s, width, done=done, end=3), x, s, width, done, 3)
+    first = torch.full((2, 5), -INF, device="cuda")
+    first[:, 0] = 0
+    check(f(x, first, 5), x, first, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [255, 256, 7001, 40001])
+def test_strides(vocab, dtype):
+    f, _ = ops()
+    x, s = make(3, 4, vocab, dtype, seed=5)
+    wide = torch.full((3, 6, vocab + 9), math.nan, dtype=dtype, device="cuda")
+    for off in (0, 1, 5, 8):
+        part = wide[:, 1:5, off:off + vocab]
+        part.copy_(x)
+        check(f(part, s, 6), x, s, 6)
+    turned = x.transpose(0, 1).contiguous().transpose(0, 1)
+    check(f(turned, s.T.contiguous().T, 6), x, s, 6)
+    check(f(x.transpose(1, 2).contiguous().transpose(1, 2), s, 6), x, s, 6)
+    same = x[:1].expand(3, 4, vocab)
+    check(f(same, s, 6), same, s, 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompts,beams,vocab,width", [(1, 4, 256, 4), (20, 4, 256, 4), (2, 5, 50257, 5), (4, 3, 3000, 9)])
+def test_other_streams_and_graphs(prompts, beams, vocab, width):
+    f, reorder = ops()
+    x, s = make(prompts, beams, vocab, torch.bfloat16, seed=1)
+    state = torch.randn(prompts * beams, 3, 70, device="cuda")
+
+    def both():
+        out = f(x, s, width, end=2)
+        return [out.scores, out.tokens, out.parents, out.done, reorder(out.parents, state)]
+
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(both())
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in outs for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_no_prompts():
+    f, reorder = ops()
+    out = f(torch.empty(0, 3, 10, device="cuda"), torch.empty(0, 3, device="cuda"), 2, end=1)
+    assert all(v.shape == (0, 2) for v in out)
+    assert reorder(out.parents, torch.empty(0, 7, device="cuda")).shape == (0, 7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompts,beams,width,shapes", [
+    (1, 1, 1, [(1,)]), (2, 4, 4, [(5, 256), (57,)]), (3, 5, 2, [(3,), (16,), (2, 8), ()]), (7, 3, 9, [(333,), (1, 4)]),
+    (50, 2, 4, [(4096,)]), (300, 4, 4, [(5, 128), (64,), (1,)]), (2, 3, 3, [(0,), (7,)]), (3, 4, 0, [(7,)]), (1, 2, 2, [(300000,)])])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_reordered_rows(prompts, beams, width, shapes, index):
+    _, f = ops()
+    g = torch.Generator().manual_seed(prompts)
+    parents = torch.randint(0, beams, (prompts, width), generator=g).to(index).cuda()
+    types = [torch.float32, torch.int8, torch.bfloat16, torch.int64]
+    tensors = [torch.randint(-100, 100, (prompts * beams, *shape), generator=g).to(types[(i + prompts) % 4]).cuda()
+               for i, shape in enumerate(shapes)]
+    out = f(parents, *tensors)
+    out = [out] if len(tensors) == 1 else out
+    rows = (torch.arange(prompts, device="cuda")[:, None] * beams + parents).flatten()
+    for a, b in zip(out, tensors):
+        assert a.dtype == b.dtype and torch.equal(a, b[rows])
+
+
+@pytest.mark.gpu
+def test_padding_and_layouts_of_reordered_rows():
+    _, f = ops()
+    x = torch.randn(8, 6, 10, device="cuda")
+    parents = torch.tensor([[0, -1, 3], [4, 2, -(2 ** 31)]], dtype=torch.int32, device="cuda")
+    want = x[[0, 0, 3, 0, 6, 0]].clone()
+    want[[1, 3, 5]] = 0
+    assert torch.equal(f(parents, x), want)
+    assert torch.equal(f(parents.long(), x.permute(0, 2, 1).contiguous().permute(0, 2, 1)), want)
+    far = torch.tensor([[2 ** 40, -(2 ** 40), 2 ** 32]], device="cuda")
+    assert not f(far, x).any()
+    odd = torch.randint(0, 255, (8 * 33 + 1,), dtype=torch.uint8, device="cuda")[1:].view(8, 33)
+    assert torch.equal(f(parents[:, :1].contiguous(), odd)[0], odd[0])
+
+
+@pytest.mark.gpu
+def test_refusals():
+    f, reorder = ops()
+    x, s = make(2, 4, 50, torch.float32)
+    for bad in (x.double(), x.int(), x.cpu(), "x", x[0], torch.empty(2, 65, 3, device="cuda"), torch.empty(2, 0, 3, device="cuda"),
+                torch.empty(2, 4, 0, device="cuda")):
+        with pytest.raises(ValueError):
+            f(bad, s if isinstance(bad, str) or bad.dim() != 3 or bad.shape[1] == 4 else torch.empty(bad.shape[:2], device="cuda"), 2)
+    for bad in (s.half(), s.cpu(), s[:, :3], None):
+        with pytest.raises(ValueError):
+            f(x, bad, 2)
+    for width in (0, -1, 65, 2.0):
+        with pytest.raises(ValueError):
+            f(x, s, width)
+    with pytest.raises(ValueError):
+        f(x[:, :, :5], s, 21)
+    done = torch.zeros(2, 4, dtype=torch.bool, device="cuda")
+    for kw in (dict(done=done), dict(done=done[:, :3], end=1), dict(done=done.int(), end=1), dict(done=done.cpu(), end=1), dict(end=50),
+               dict(end=-1), dict(end=1.5)):
+        with pytest.raises(ValueError):
+            f(x, s, 2, **kw)
+    with pytest.raises(NotImplementedError):
+        f(x.clone().requires_grad_(), s, 2)
+    with pytest.raises(NotImplementedError):
+        f(x, s.clone().requires_grad_(), 2)
+    with torch.no_grad():
+        f(x.clone().requires_grad_(), s, 2)
+    parents = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    for bad in ((parents.float(), x[0]), (parents[0], x[0]), (parents.cpu(), x[0]), (parents,), (parents, x[0, :3]), (parents, x[0].cpu()),
+                (parents, x[0], x[0, :2]), (parents, *[x[0]] * 9), (parents, torch.tensor(1.0, device="cuda")), (parents[:0], x[0])):
+        with pytest.raises(ValueError):
+            reorder(*bad)
+    with pytest.raises(NotImplementedError):
+        reorder(parents, x[0].clone().requires_grad_())
+
+
+def test_c_entries_refuse_bad_arguments():
+    lib = _native.ops()
+    choose = lambda prompts=1, beams=2, vocab=9, sb=4, done=None, end=-1, width=2, x=16, s=16, out=16, dtype=0: lib.ygg_beam_select(  # noqa: E731
+        0, dtype, prompts, beams, vocab, x, beams * vocab, vocab, sb, s, done, end, width, out, 16, 16, None, None)
+    for kw in (dict(prompts=-1), dict(beams=0), dict(vocab=0), dict(width=0), dict(sb=2), dict(width=19), dict(end=9), dict(end=-2),
+               dict(done=16), dict(x=None), dict(s=None), dict(out=None)):
+        assert choose(**kw) == _native.YGG_E_ARG, kw
+    for kw in (dict(beams=65), dict(width=65, vocab=100), dict(vocab=1 << 30), dict(prompts=1 << 31)):
+        assert choose(**kw) == _native.YGG_E_UNSUPPORTED, kw
+    assert choose(prompts=0, x=None) == _native.YGG_OK
+    import ctypes
+    one = (ctypes.c_void_p * 1)(16)
+    size = (ctypes.c_int64 * 1)(4)
+    reorder = lambda prompts=1, beams=2, width=2, p=16, pb=4, count=1, a=one, b=one, n=size: lib.ygg_reorder(  # noqa: E731
+        0, prompts, beams, width, p, pb, count, a, b, n, None)
+    for kw in (dict(prompts=-1), dict(beams=-1), dict(width=-1), dict(p=None), dict(pb=2), dict(count=9), dict(count=-1), dict(a=None),
+               dict(b=None), dict(n=None), dict(a=(ctypes.c_void_p * 1)(None))):
+        assert reorder(**kw) == _native.YGG_E_ARG, kw
+    assert reorder(prompts=1 << 20, width=1 << 12) == _native.YGG_E_UNSUPPORTED
+    assert reorder(count=0, p=None) == reorder(width=0, p=None) == _native.YGG_OK

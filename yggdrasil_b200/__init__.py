@@ -9,6 +9,8 @@ __all__ = ["Yggdrasil", "B200Yggdrasil"]   # without the operators: `import *` w
 
 _OPERATORS = {"token_logprobs": "logprobs", "TokenLogprobs": "logprobs",
               "int8_linear": "linear", "quantize_rows": "linear", "QuantizedRows": "linear",
+              "int4_linear": "linear", "quantize_int4": "linear", "pack_int4": "linear", "Int4Weights": "linear",
+              "beam_select": "select", "BeamChoice": "select", "reorder_states": "select", "layer_norm": "norm",
               "StateCache": "cache"}
 
 

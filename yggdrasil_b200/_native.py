@@ -15,7 +15,9 @@ EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "y
            "ygg_strerror", "ygg_version", "ygg_fload", "ygg_fstep", "ygg_fstep_stats", "ygg_fstatus", "ygg_ffree",
            "ygg_token_logprobs", "ygg_token_logprobs_backward", "ygg_quantize_rows", "ygg_linear_workspace",
            "ygg_linear_quantized", "ygg_linear", "ygg_linear_status", "ygg_cache_workspace", "ygg_cache_fork", "ygg_cache_free",
-           "ygg_cache_compact", "ygg_cache_read", "ygg_cache_write", "ygg_cache_copy")
+           "ygg_cache_compact", "ygg_cache_read", "ygg_cache_write", "ygg_cache_copy", "ygg_fourbit_quantize",
+           "ygg_fourbit_pack", "ygg_fourbit_linear", "ygg_beam_select", "ygg_reorder", "ygg_layer_norm",
+           "ygg_layer_norm_workspace", "ygg_layer_norm_backward")
 
 YGG_OK = 0
 YGG_E_ARG, YGG_E_FORMAT, YGG_E_UNSUPPORTED, YGG_E_MISSING, YGG_E_CUDA, YGG_E_OOM, YGG_E_TOKEN, YGG_E_TIMEOUT, \
@@ -126,6 +128,18 @@ def ops() -> ctypes.CDLL:
         l.ygg_cache_read.argtypes = [i32, cache, i64, vp, vp, vp]
         l.ygg_cache_write.argtypes = [i32, cache, i64, vp, vp, vp]
         l.ygg_cache_copy.argtypes = [i32, cache, i64, vp, vp, vp]
+        l.ygg_fourbit_quantize.argtypes = [i32, i32, i64, i64, i64, vp, i64, vp, vp, vp]
+        l.ygg_fourbit_pack.argtypes = [i32, i64, i64, vp, i64, vp, vp]
+        l.ygg_fourbit_linear.argtypes = [i32, i32, i64, i64, i64, i64, vp, i64, vp, i32, vp, vp, i32, vp, i64, vp]
+        l.ygg_beam_select.argtypes = [i32, i32, i64, i64, i64, vp, i64, i64, i32, vp, vp, i64, i64] + [vp] * 5
+        l.ygg_reorder.argtypes = [i32, i64, i64, i64, vp, i32, i32, vp, vp, vp, vp]
+        l.ygg_layer_norm.argtypes = [i32, i32, i64, i64, vp, i64, i32, vp, i32, vp, ctypes.c_float, vp, vp, vp]
+        l.ygg_layer_norm_workspace.argtypes = [i64, i64]
+        l.ygg_layer_norm_workspace.restype = size
+        l.ygg_layer_norm_backward.argtypes = [i32, i32, i64, i64, vp, i64, i32, vp, i32, vp, vp, i64, vp, vp, vp, vp, size, vp]
+        for f in (l.ygg_fourbit_quantize, l.ygg_fourbit_pack, l.ygg_fourbit_linear, l.ygg_beam_select, l.ygg_reorder,
+                  l.ygg_layer_norm, l.ygg_layer_norm_backward):
+            f.restype = i32
         for f in (l.ygg_token_logprobs, l.ygg_token_logprobs_backward, l.ygg_quantize_rows, l.ygg_linear_quantized,
                   l.ygg_linear, l.ygg_linear_status, l.ygg_cache_fork, l.ygg_cache_free, l.ygg_cache_compact, l.ygg_cache_read,
                   l.ygg_cache_write, l.ygg_cache_copy):

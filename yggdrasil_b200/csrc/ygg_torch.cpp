@@ -1,5 +1,6 @@
 // The operators' Python calls on torch tensors, without an interpreter's overhead: checks, outputs from torch's allocator, the
-// current stream, the C-ABI call (include/ygg_b200.h), and the gradient of token_logprobs as a node of torch's autograd.
+// current stream, the C-ABI call (include/ygg_b200.h), and the gradients of token_logprobs and layer_norm as nodes of torch's
+// autograd.
 //
 // Each call takes the plain case (what a loop passes: tensors of the right types and layouts on one device) and returns None
 // for any other; the Python side then checks, converts, and calls again. A call costs the host 5 to 8 us this way, most of
@@ -457,11 +458,278 @@ PyObject *py_cache_copy(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ int4_linear
+
+struct FourBit {
+    Tensor codes, scale;   // uint8 [n][64 blocks], [n][groups]
+    int64_t k, group;
+};
+
+// Int4Weights as the kernels read them.
+std::optional<FourBit> fourbit_of(PyObject *o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return std::nullopt;
+    const Tensor *c = cuda_tensor(PyTuple_GET_ITEM(o, 0)), *s = cuda_tensor(PyTuple_GET_ITEM(o, 1));
+    PyObject *k = PyTuple_GET_ITEM(o, 2), *group = PyTuple_GET_ITEM(o, 3);
+    if (!c || !s || !PyLong_CheckExact(k) || !PyLong_CheckExact(group)) return std::nullopt;
+    FourBit r{*c, *s, PyLong_AsLongLong(k), PyLong_AsLongLong(group)};
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return std::nullopt;
+    }
+    if (r.k < 1 || r.k > YGG_LINEAR_MAX_K || r.group < 32 || r.group > YGG_LINEAR_MAX_K || (r.group & (r.group - 1)) ||
+        c->scalar_type() != at::kByte || c->dim() != 2 || c->size(0) < 1 || c->size(1) != (r.k + 127) / 128 * 64 ||
+        !c->is_contiguous() || (uintptr_t)c->data_ptr() % 16 || dtype_of(s->scalar_type()) < 0 || s->dim() != 2 ||
+        s->size(0) != c->size(0) || s->size(1) != (r.k + r.group - 1) / r.group || !s->is_contiguous() ||
+        s->device() != c->device() || tracked(*s))
+        return std::nullopt;
+    return r;
+}
+
+// (x, Int4Weights, bias or None, out_dtype or None) -> y, or None
+PyObject *py_int4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = n == 4 ? cuda_tensor(args[0]) : nullptr;
+    if (!x || !rows_ok(*x)) Py_RETURN_NONE;
+    const auto w = fourbit_of(args[1]);
+    const at::Device device = x->device();
+    if (!w || x->size(1) != w->k || w->codes.device() != device) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), channels = w->codes.size(0);
+    const Tensor *bias = args[2] == Py_None ? nullptr : cuda_tensor(args[2]);
+    if (args[2] != Py_None && (!bias || !is_row(*bias, at::kFloat, channels, device) || tracked(*bias))) Py_RETURN_NONE;
+    at::ScalarType type = at::kFloat;
+    const int out_dtype = type_asked(args[3], x->scalar_type(), type);
+    if (out_dtype < 0) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard on(device);
+    Tensor out = empty({rows, channels}, type, device);
+    raise_for(ygg_fourbit_linear(device.index(), dtype_of(x->scalar_type()), rows, w->k, channels, w->group, x->data_ptr(),
+                                 x->stride(0), (const uint8_t *)w->codes.data_ptr(), dtype_of(w->scale.scalar_type()),
+                                 w->scale.data_ptr(), bias ? (const float *)bias->data_ptr() : nullptr, out_dtype,
+                                 out.data_ptr(), channels, stream_of(device.index())),
+              "ygg_fourbit_linear");
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// (weight, group) -> (codes, scale), or None
+PyObject *py_quantize_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *w = n == 2 ? cuda_tensor(args[0]) : nullptr;
+    if (!w || !rows_ok(*w) || w->size(0) < 1 || !PyLong_Check(args[1])) Py_RETURN_NONE;
+    const int64_t group = PyLong_AsLongLong(args[1]), channels = w->size(0), k = w->size(1);
+    if (group == -1 && PyErr_Occurred()) throw python_error();
+    const at::Device device = w->device();
+    const c10::cuda::CUDAGuard on(device);
+    const Tensor codes = empty({channels, (k + 127) / 128 * 64}, at::kByte, device);
+    const Tensor scale = empty({channels, (k + group - 1) / group}, w->scalar_type(), device);
+    raise_for(ygg_fourbit_quantize(device.index(), dtype_of(w->scalar_type()), channels, k, group, w->data_ptr(), w->stride(0),
+                                   (uint8_t *)codes.data_ptr(), scale.data_ptr(), stream_of(device.index())),
+              "ygg_fourbit_quantize");
+    PyObject *r = PyTuple_New(2);
+    if (!r) throw python_error();
+    PyTuple_SET_ITEM(r, 0, wrap(codes));
+    PyTuple_SET_ITEM(r, 1, wrap(scale));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// (codes int8 (n, k),) -> codes as they are laid out, or None
+PyObject *py_pack_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *c = n == 1 ? cuda_tensor(args[0]) : nullptr;
+    if (!c || c->scalar_type() != at::kChar || c->dim() != 2 || c->size(0) < 1 || c->size(1) < 1 ||
+        c->size(1) > YGG_LINEAR_MAX_K || (c->size(1) > 1 && c->stride(1) != 1))
+        Py_RETURN_NONE;
+    const at::Device device = c->device();
+    const c10::cuda::CUDAGuard on(device);
+    const Tensor codes = empty({c->size(0), (c->size(1) + 127) / 128 * 64}, at::kByte, device);
+    raise_for(ygg_fourbit_pack(device.index(), c->size(0), c->size(1), (const int8_t *)c->data_ptr(), c->stride(0),
+                               (uint8_t *)codes.data_ptr(), stream_of(device.index())),
+              "ygg_fourbit_pack");
+    return wrap(codes);
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------------ beams
+
+// (logits, scores, width, done or None, end or None) -> (scores, tokens, parents, done or None), or None
+PyObject *py_beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = n == 5 ? cuda_tensor(args[0]) : nullptr, *s = n == 5 ? cuda_tensor(args[1]) : nullptr;
+    if (!x || !s || !PyLong_Check(args[2]) || (args[4] != Py_None && !PyLong_Check(args[4]))) Py_RETURN_NONE;
+    const int64_t width = PyLong_AsLongLong(args[2]), end = args[4] == Py_None ? -1 : PyLong_AsLongLong(args[4]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const Tensor *done = args[3] == Py_None ? nullptr : cuda_tensor(args[3]);
+    if (dtype_of(x->scalar_type()) < 0 || x->dim() != 3 || x->size(1) < 1 || x->size(1) > YGG_BEAMS_MAX || x->size(2) < 1 ||
+        x->size(2) > INT32_MAX / x->size(1) || x->size(0) > INT32_MAX || (x->size(2) > 1 && x->stride(2) != 1) ||
+        (s->scalar_type() != at::kFloat && s->scalar_type() != at::kDouble) || s->dim() != 2 || s->size(0) != x->size(0) ||
+        s->size(1) != x->size(1) || !s->is_contiguous() || s->device() != x->device() || width < 1 || width > YGG_BEAMS_MAX ||
+        width > x->size(1) * x->size(2) || (args[4] != Py_None && (end < 0 || end >= x->size(2))) || tracked(*x) || tracked(*s))
+        Py_RETURN_NONE;
+    if (args[3] != Py_None && (!done || end < 0 || done->scalar_type() != at::kBool || done->sizes() != s->sizes() ||
+                               !done->is_contiguous() || done->device() != x->device()))
+        Py_RETURN_NONE;
+    const at::Device device = x->device();
+    const c10::cuda::CUDAGuard on(device);
+    const int64_t prompts = x->size(0);
+    const Tensor scores = empty({prompts, width}, s->scalar_type(), device), tokens = empty({prompts, width}, at::kInt, device),
+                 parents = empty({prompts, width}, at::kInt, device),
+                 ended = end < 0 ? Tensor() : empty({prompts, width}, at::kBool, device);
+    raise_for(ygg_beam_select(device.index(), dtype_of(x->scalar_type()), prompts, x->size(1), x->size(2), x->data_ptr(),
+                              x->stride(0), x->stride(1), (int)s->element_size(), s->data_ptr(),
+                              done ? (const uint8_t *)done->data_ptr() : nullptr, end, width, scores.data_ptr(),
+                              (int32_t *)tokens.data_ptr(), (int32_t *)parents.data_ptr(),
+                              ended.defined() ? (uint8_t *)ended.data_ptr() : nullptr, stream_of(device.index())),
+              "ygg_beam_select");
+    PyObject *r = PyTuple_New(4);
+    if (!r) throw python_error();
+    PyTuple_SET_ITEM(r, 0, wrap(scores));
+    PyTuple_SET_ITEM(r, 1, wrap(tokens));
+    PyTuple_SET_ITEM(r, 2, wrap(parents));
+    PyTuple_SET_ITEM(r, 3, wrap(ended));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// (parents (prompts, width), tensors...) -> a tuple of their rows, or None
+PyObject *py_reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const int count = (int)n - 1;
+    const Tensor *p = n >= 2 ? cuda_tensor(args[0]) : nullptr;
+    if (!p || count > YGG_REORDER_MAX || (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong) || p->dim() != 2 ||
+        p->size(0) < 1 || !p->is_contiguous())
+        Py_RETURN_NONE;
+    const int64_t prompts = p->size(0), width = p->size(1);
+    const at::Device device = p->device();
+    const Tensor *from[YGG_REORDER_MAX];
+    for (int i = 0; i < count; i++) {
+        from[i] = cuda_tensor(args[i + 1]);
+        if (!from[i] || from[i]->dim() < 1 || from[i]->size(0) != (i ? from[0] : from[i])->size(0) ||
+            from[i]->size(0) % prompts || !from[i]->is_contiguous() || from[i]->device() != device || tracked(*from[i]))
+            Py_RETURN_NONE;
+    }
+    const c10::cuda::CUDAGuard on(device);
+    Tensor to[YGG_REORDER_MAX];
+    const void *source[YGG_REORDER_MAX];
+    void *target[YGG_REORDER_MAX];
+    int64_t bytes[YGG_REORDER_MAX];
+    c10::DimVector size;
+    for (int i = 0; i < count; i++) {
+        size.assign(from[i]->sizes().begin(), from[i]->sizes().end());
+        size[0] = prompts * width;
+        to[i] = empty(size, from[i]->scalar_type(), device);
+        source[i] = from[i]->data_ptr();
+        target[i] = to[i].data_ptr();
+        bytes[i] = from[i]->element_size();
+        for (size_t d = 1; d < size.size(); d++) bytes[i] *= size[d];
+    }
+    raise_for(ygg_reorder(device.index(), prompts, from[0]->size(0) / prompts, width, p->data_ptr(), (int)p->element_size(),
+                          count, source, target, bytes, stream_of(device.index())),
+              "ygg_reorder");
+    PyObject *r = PyTuple_New(count);
+    if (!r) throw python_error();
+    for (int i = 0; i < count; i++) PyTuple_SET_ITEM(r, i, wrap(to[i]));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------------ layer_norm
+
+using MaybeTensor = std::optional<Tensor>;
+
+const void *data_of(const MaybeTensor &t) { return t ? t->data_ptr() : nullptr; }
+int dtype_of(const MaybeTensor &t) { return t ? dtype_of(t->scalar_type()) : YGG_DTYPE_FLOAT; }
+
+// Rows of x (..., D): x is contiguous, or (rows, D) with its entries side by side.
+int64_t row_stride(const Tensor &x) { return x.dim() == 2 && x.size(0) > 1 ? x.stride(0) : x.size(-1); }
+bool plain_rows(const Tensor &x) { return x.is_contiguous() || (x.dim() == 2 && (x.size(1) == 1 || x.stride(1) == 1)); }
+
+Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, double eps, float *stats) {
+    const at::Device device = x.device();
+    const int64_t dim = x.size(-1);
+    Tensor y = empty(x.sizes(), x.scalar_type(), device);
+    raise_for(ygg_layer_norm(device.index(), dtype_of(x.scalar_type()), x.numel() / dim, dim, x.data_ptr(), row_stride(x),
+                             dtype_of(weight), data_of(weight), dtype_of(bias), data_of(bias), (float)eps, y.data_ptr(), stats,
+                             stream_of(device.index())),
+              "ygg_layer_norm");
+    return y;
+}
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const MaybeTensor &weight,
+                          const MaybeTensor &bias, double eps) {
+        const Tensor stats = empty({x.numel() / x.size(-1), 2}, at::kFloat, x.device());
+        const Tensor y = layer_norm(x, weight, bias, eps, (float *)stats.data_ptr());
+        ctx->save_for_backward({x, weight ? *weight : Tensor(), stats});
+        ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : -1;
+        ctx->set_materialize_grads(false);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                   torch::autograd::variable_list arriving) {
+        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() && !has_tangent(arriving[0]), "layer_norm has no second derivative");
+        if (!arriving[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+        const int64_t bias = ctx->saved_data["bias"].toInt(), dim = x.size(-1), rows = x.numel() / dim;
+        const at::Device device = x.device();
+        const c10::cuda::CUDAGuard on(device);
+        Tensor g = arriving[0].scalar_type() == x.scalar_type() ? arriving[0] : arriving[0].to(x.scalar_type());
+        if (!plain_rows(g)) g = g.contiguous();
+        const bool has_weight = weight.defined(), has_bias = bias >= 0;
+        const auto bias_type = has_bias ? (at::ScalarType)bias : at::kFloat;
+        Tensor dx, dw, db, room;
+        if (ctx->needs_input_grad(0)) dx = empty(x.sizes(), x.scalar_type(), device);
+        if (has_weight && ctx->needs_input_grad(1)) dw = empty({dim}, weight.scalar_type(), device);
+        if (has_bias && ctx->needs_input_grad(1 + has_weight)) db = empty({dim}, bias_type, device);
+        int64_t bytes = 0;
+        if (dw.defined() || db.defined()) {
+            bytes = (int64_t)ygg_layer_norm_workspace(rows, dim);
+            room = empty({bytes}, at::kByte, device);
+        }
+        const auto at = [](const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+        raise_for(ygg_layer_norm_backward(
+                      device.index(), dtype_of(x.scalar_type()), rows, dim, x.data_ptr(), row_stride(x),
+                      has_weight ? dtype_of(weight.scalar_type()) : YGG_DTYPE_FLOAT, at(weight), dtype_of(bias_type),
+                      (const float *)stats.data_ptr(), g.data_ptr(), row_stride(g), at(dx), at(dw), at(db), at(room),
+                      (size_t)bytes, stream_of(device.index())),
+                  "ygg_layer_norm_backward");
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+// (x, weight or None, bias or None, eps) -> y, or None
+PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = n == 4 ? cuda_tensor(args[0]) : nullptr;
+    if (!x || dtype_of(x->scalar_type()) < 0 || x->dim() < 1 || x->size(-1) < 1 || !plain_rows(*x) || !PyFloat_CheckExact(args[3]))
+        Py_RETURN_NONE;
+    MaybeTensor a[2];
+    bool wanted = x->requires_grad(), tangent = has_tangent(*x);
+    for (int i = 0; i < 2; i++) {
+        if (args[i + 1] == Py_None) continue;
+        const Tensor *t = cuda_tensor(args[i + 1]);
+        if (!t || dtype_of(t->scalar_type()) < 0 || !is_row(*t, t->scalar_type(), x->size(-1), x->device())) Py_RETURN_NONE;
+        a[i] = *t;
+        wanted |= t->requires_grad();
+        tangent |= has_tangent(*t);
+    }
+    TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "layer_norm has no forward-mode derivative");
+    const double eps = PyFloat_AS_DOUBLE(args[3]);
+    const c10::cuda::CUDAGuard on(x->device());
+    if (wanted && at::GradMode::is_enabled()) return wrap(LayerNormNode::apply(*x, a[0], a[1], eps));
+    return wrap(layer_norm(*x, a[0], a[1], eps, nullptr));
+    END_HANDLE_TH_ERRORS
+}
+
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(token_logprobs), CALL(int8_linear), CALL(int8_linear_rows), CALL(quantize_rows),
                            CALL(tracked),        CALL(cache),       CALL(cache_fork),       CALL(cache_free),
                            CALL(cache_compact),  CALL(cache_read),  CALL(cache_write),      CALL(cache_copy),
-                           {nullptr, nullptr, 0, nullptr}};
+                           CALL(int4_linear),    CALL(quantize_int4), CALL(pack_int4),       CALL(beam_select),
+                           CALL(reorder_states), CALL(layer_norm),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,4 +1,6 @@
-"""Linear layers in 8-bit integers: a scale for each row of activations, found as it comes, and one for each channel.
+"""Linear layers with frozen weights of 8 or 4 bits.
+
+In 8-bit integers: a scale for each row of activations, found as it comes, and one for each channel.
 
     from yggdrasil_b200 import int8_linear, quantize_rows
     head = quantize_rows(weight)                        # once: (N, K) floats -> codes and a scale for each channel
@@ -7,6 +9,15 @@
 y = (codes(x) . codes(w)) scale_w scale_x + bias, the sums exact in int32 (csrc/ygg_linear.cu): a row's outputs have the same
 bits alone and in any batch. The weights are frozen: there is no gradient, and rows, scales or a bias that ask for one are
 refused with NotImplementedError (detach() them, or call under torch.no_grad()).
+
+With weights of 4 bits: a scale for each channel and each group of inputs, the activations as they are.
+
+    from yggdrasil_b200 import int4_linear, quantize_int4
+    head = quantize_int4(weight, group=128)             # once
+    y = int4_linear(x, head, bias)
+
+y = sum over groups of scale (x . codes) + bias, no weight rounded any further, the sums in 32 bits (csrc/ygg_fourbit.cu). For
+few rows it is bound by the bytes of the weights, half of those of 8 bits. Frozen in the same way.
 """
 from __future__ import annotations
 
@@ -75,11 +86,7 @@ def _prepared(x, weight, scale, bias, out_dtype):
     if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.shape != (n,) \
             or scale.device != device:
         raise ValueError(f"scale must be a float32 tensor ({n},) on {device}")
-    if bias is not None:
-        if not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.device != device or bias.dtype not in DTYPES:
-            raise ValueError(f"bias must be a float tensor ({n},) on {device}")
-        _frozen(bias)
-        bias = bias.detach().float().contiguous()
+    bias = _bias(bias, n, device)
     _frozen(scale)
     with torch.cuda.device(device):
         weights = _laid_out(weight), scale.contiguous(), bias, out_dtype
@@ -105,7 +112,7 @@ def _rows(x):
 def _frozen(*tensors):
     """Refuse tensors through which a gradient, or a forward-mode derivative, is asked for."""
     if any(_ops.tracked(t) for t in tensors):
-        raise NotImplementedError("the int8 product has no gradient: use detach() or torch.no_grad()")
+        raise NotImplementedError("products with frozen weights have no gradient: use detach() or torch.no_grad()")
 
 
 def _strides(lead, step):
@@ -115,6 +122,94 @@ def _strides(lead, step):
         out.insert(0, step)
         step *= size
     return out
+
+
+class Int4Weights(NamedTuple):
+    codes: torch.Tensor   # uint8 (N, 64 ceil(K / 128)), as quantize_int4 and pack_int4 lay them out
+    scale: torch.Tensor   # (N, ceil(K / group)) float32, float16 or bfloat16
+    k: int                # inputs
+    group: int            # inputs that share a scale: a power of two, 32 or more
+
+
+def quantize_int4(weight, group=128):
+    """weight (N, K) float32, float16 or bfloat16 -> Int4Weights, the scales in the weight's type. The scale of a group is its
+    largest magnitude / 7, rounded to that type, a code the nearest integer (ties to even) of the value divided by the scale,
+    within -8 to 7. A group of zeros (or whose scale is too small for the type) has scale 0; one that holds NaN or infinity
+    has scale NaN."""
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] < 1:
+        raise ValueError("weight must be a float32, float16 or bfloat16 CUDA tensor (N, K)")
+    group = _group(group)
+    codes, scale = _ops.quantize_int4(_rows(weight), group)
+    return Int4Weights(codes, scale, weight.shape[1], group)
+
+
+def pack_int4(codes, scale, group=128):
+    """Codes that are there already, int8 (N, K) of -8 to 7, with their scales (N, ceil(K / group)) -> Int4Weights. Waits for the
+    device, to look at the codes' range."""
+    group = _group(group)
+    if not isinstance(codes, torch.Tensor) or not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2 \
+            or codes.shape[0] < 1 or not 1 <= codes.shape[1] <= MAX_K:
+        raise ValueError(f"codes must be an int8 CUDA tensor (N, K), K 1 to {MAX_K}")
+    if codes.min() < -8 or codes.max() > 7:
+        raise ValueError("codes must be -8 to 7")
+    n, k = codes.shape
+    if not isinstance(scale, torch.Tensor) or scale.dtype not in DTYPES or scale.shape != (n, -(-k // group)) \
+            or scale.device != codes.device:
+        raise ValueError(f"scale must be a float tensor {(n, -(-k // group))} on {codes.device}")
+    _frozen(scale)
+    return Int4Weights(_ops.pack_int4(codes if k == 1 or codes.stride(1) == 1 else codes.contiguous()), scale.contiguous(), k, group)
+
+
+def int4_linear(x, weight, bias=None, out_dtype=None):
+    """x (..., K) float32, float16 or bfloat16 times Int4Weights of N channels, plus bias (N,) or None. Returns (..., N) in
+    out_dtype, x's type by default."""
+    out = _ops.int4_linear(x, weight, bias, out_dtype)   # (rows, K) and weights as the kernels read them
+    return out if out is not None else _prepared_int4(x, weight, bias, out_dtype)
+
+
+def _prepared_int4(x, weight, bias, out_dtype):
+    """The same with whatever else the arguments may be: checked, and brought into the plain form."""
+    if not isinstance(weight, Int4Weights):
+        raise ValueError("weight must be Int4Weights, as quantize_int4 and pack_int4 give them")
+    codes, scale, k, group = weight
+    group = _group(group)
+    rows = _rows(x)
+    if x.shape[-1] != k:
+        raise ValueError(f"x (..., {x.shape[-1]}) for weights of {k} inputs")
+    if not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[0] < 1 \
+            or codes.shape[1] != -(-k // 128) * 64 or codes.device != x.device:
+        raise ValueError(f"Int4Weights: uint8 codes (N, {-(-k // 128) * 64}) on {x.device}")
+    n = codes.shape[0]
+    if not isinstance(scale, torch.Tensor) or scale.dtype not in DTYPES or scale.shape != (n, -(-k // group)) \
+            or scale.device != x.device:
+        raise ValueError(f"Int4Weights: a float scale {(n, -(-k // group))} on {x.device}")
+    if out_dtype is not None and out_dtype not in DTYPES:
+        raise ValueError(f"out_dtype {out_dtype}: float32, float16 or bfloat16")
+    _frozen(scale)
+    bias = _bias(bias, n, x.device)
+    with torch.cuda.device(x.device):
+        codes = codes.contiguous()
+        if codes.data_ptr() % 16:
+            codes = codes.clone()
+        weight = Int4Weights(codes, scale.contiguous(), int(k), group)
+        out = _ops.int4_linear(rows, weight, bias, out_dtype)
+    return out.view(*x.shape[:-1], n)
+
+
+def _group(group):
+    if not hasattr(group, "__index__") or not 32 <= group <= MAX_K or group & (group - 1):
+        raise ValueError(f"group {group}: a power of two, 32 to {MAX_K}")
+    return int(group)
+
+
+def _bias(bias, n, device):
+    """A bias (n,) as the kernels read it."""
+    if bias is None:
+        return None
+    if not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.device != device or bias.dtype not in DTYPES:
+        raise ValueError(f"bias must be a float tensor ({n},) on {device}")
+    _frozen(bias)
+    return bias.detach().float().contiguous()
 
 
 def linear_status(device="cuda"):

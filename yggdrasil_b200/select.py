@@ -1,0 +1,105 @@
+"""The choice over beams and vocabulary, and states in its order.
+
+    from yggdrasil_b200 import beam_select, reorder_states
+    out = beam_select(logits, scores, width=4)          # logits (prompts, beams, V), scores (prompts, beams)
+    out.scores, out.tokens, out.parents                 # (prompts, 4): best first
+    state, history = reorder_states(out.parents, state, history)   # rows (prompts beams, ...) -> (prompts 4, ...)
+
+The kernels are csrc/ygg_select.cu. Neither carries a gradient: tensors that ask for one are refused with
+NotImplementedError.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _ops
+from .logprobs import DTYPES
+
+BEAMS_MAX = 64
+REORDER_MAX = 8
+
+
+class BeamChoice(NamedTuple):
+    scores: torch.Tensor        # (prompts, width), best first
+    tokens: torch.Tensor        # (prompts, width) int32
+    parents: torch.Tensor       # (prompts, width) int32: the beam that each goes on from
+    done: torch.Tensor | None   # (prompts, width) bool, where an end is given
+
+
+def beam_select(logits, scores, width, done=None, end=None):
+    """The best `width` continuations of each prompt's beams by one token: a beam's score plus the log-probability of the token,
+    in 64 bits, ties by the lower beam, then the lower token. Continuations that are nearer than sums in 32 bits tell
+    are told apart exactly.
+
+    logits (prompts, beams, V) float32, float16 or bfloat16 on a CUDA device, with any strides of prompts and beams; scores
+    (prompts, beams) float32 or float64, and the new ones in their type (float64 ones are exact to 64 bits, at some cost). end: a
+    token after which a beam is done. done: (prompts, beams) bool, the beams that are done before: each goes on with `end` alone, at no cost.
+    At most 64 beams and picks, and beams times V below 2^31.
+
+    -inf logits (closed tokens) are worth -inf; where fewer continuations than `width` are open, closed ones follow in their order. A
+    beam that holds NaN or +inf is worth NaN; NaN ranks as -inf."""
+    out = _ops.beam_select(logits, scores, width, done, end)
+    return tuple.__new__(BeamChoice, out if out is not None else _prepared(logits, scores, width, done, end))
+
+
+def _prepared(logits, scores, width, done, end):
+    """The same with whatever else the arguments may be: checked, and brought into the plain form."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in DTYPES or logits.dim() != 3:
+        raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor (prompts, beams, V)")
+    prompts, beams, vocab = logits.shape
+    if not 1 <= beams <= BEAMS_MAX or vocab < 1 or beams * vocab >= 2 ** 31 or prompts >= 2 ** 31:
+        raise ValueError(f"logits {tuple(logits.shape)}: 1 to {BEAMS_MAX} beams, beams times V from 1 to 2^31 - 1")
+    if not isinstance(scores, torch.Tensor) or scores.dtype not in (torch.float32, torch.float64) \
+            or scores.shape != (prompts, beams) or scores.device != logits.device:
+        raise ValueError(f"scores must be a float32 or float64 tensor {(prompts, beams)} on {logits.device}")
+    most = min(BEAMS_MAX, beams * vocab)
+    if not hasattr(width, "__index__") or not 1 <= width <= most:
+        raise ValueError(f"width {width}: an integer, 1 to {most}")
+    if end is not None and (not hasattr(end, "__index__") or not 0 <= end < vocab):
+        raise ValueError(f"end {end}: a token below {vocab}")
+    if done is not None:
+        if end is None:
+            raise ValueError("beams are done after an end: give one")
+        if not isinstance(done, torch.Tensor) or done.dtype != torch.bool or done.shape != (prompts, beams) \
+                or done.device != logits.device:
+            raise ValueError(f"done must be a bool tensor {(prompts, beams)} on {logits.device}")
+        done = done.contiguous()
+    _no_gradient(logits, scores)
+    return _ops.beam_select(logits if vocab == 1 or logits.stride(2) == 1 else logits.contiguous(), scores.contiguous(), int(width),
+                            done, None if end is None else int(end))
+
+
+def reorder_states(parents, *tensors):
+    """Rows of tensors in the order of a choice: row prompt width + j of a result is row prompt beams + parents[prompt, j]. parents
+    (prompts, width) int32 or int64, as beam_select gives them; tensors (prompts beams, ...) of any types, one to eight,
+    with as many rows each. Returns the one result, or a tuple. A parent that is negative (padding) or no beam gives zeros."""
+    out = _ops.reorder_states(parents, *tensors)
+    if out is None:
+        out = _prepared_reorder(parents, tensors)
+    return out[0] if len(out) == 1 else out
+
+
+def _prepared_reorder(parents, tensors):
+    if not isinstance(parents, torch.Tensor) or not parents.is_cuda or parents.dtype not in (torch.int32, torch.int64) \
+            or parents.dim() != 2:
+        raise ValueError("parents must be an int32 or int64 CUDA tensor (prompts, width)")
+    if not 1 <= len(tensors) <= REORDER_MAX:
+        raise ValueError(f"{len(tensors)} tensors: 1 to {REORDER_MAX}")
+    prompts = parents.shape[0]
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.device != parents.device or t.dim() < 1:
+            raise ValueError(f"tensors must be (prompts beams, ...) on {parents.device}")
+        if t.shape[0] != tensors[0].shape[0] or (t.shape[0] % prompts if prompts else t.shape[0]):
+            raise ValueError(f"{t.shape[0]} rows for {prompts} prompts: as many for each, in every tensor")
+    _no_gradient(*tensors)
+    if prompts == 0:
+        return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors)
+    return _ops.reorder_states(parents.contiguous(), *(t.contiguous() for t in tensors))
+
+
+def _no_gradient(*tensors):
+    """Refuse tensors through which a gradient, or a forward-mode derivative, is asked for."""
+    if any(_ops.tracked(t) for t in tensors):
+        raise NotImplementedError("a choice of beams carries no gradient: use detach() or torch.no_grad()")
