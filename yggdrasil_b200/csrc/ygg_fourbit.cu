@@ -13,8 +13,10 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ygg_ops.cuh"
+#include "ygg_smem.h"
 
 namespace {
 
@@ -144,6 +146,246 @@ template <typename T> cudaError_t launch_plain(const FourBit &p, cudaStream_t st
     return cudaGetLastError();
 }
 
+// ---------------------------------------------------------------------------------------------------- few rows
+//
+// Up to 24 columns of 16-bit entries: the rows of x, or three for a row of floats (its bits cut in three pieces of 8, which are
+// exact and add up to it). A warp multiplies 16 channels by 8 columns and 16 inputs at a time (mma.sync, float sums): lane
+// (g, t) holds channels g and g + 8, and 16 bytes of each bring its piece t of four runs of 32 inputs. The columns lie in
+// shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory.
+constexpr int kFewCols = 24, kFewWarps = 8, kDepth = 4, kColStride = 20;
+
+template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+
+__device__ __forceinline__ uint32_t sub2(uint32_t a, __half) {   // 1024 + code + 8 -> code
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x64086408u));
+    return r;
+}
+__device__ __forceinline__ uint32_t sub2(uint32_t a, __nv_bfloat16) {   // 128 + code + 8 -> code
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x43084308u));
+    return r;
+}
+// The inputs 2 j and 2 j + 1 of a word's piece.
+template <typename E> __device__ __forceinline__ uint32_t codes_of(uint32_t w, int j) {
+    constexpr uint32_t magic = sizeof(E) == 2 && std::is_same<E, __half>::value ? 0x64006400u : 0x43004300u;
+    return sub2(((w >> (4 * j)) & 0x000F000Fu) | magic, E());
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                    __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A float's pieces: cut off, so that the first never overflows; infinities and NaN have one.
+struct Pieces { uint16_t v[3]; };
+__device__ __forceinline__ Pieces pieces_of(float x) {
+    const uint32_t b = __float_as_uint(x);
+    if ((b & 0x7F800000u) == 0x7F800000u) return {{(uint16_t)((b >> 16) | ((b & 0x7FFFFFu) ? 0x40u : 0u)), 0, 0}};
+    const float rest = __fsub_rn(x, __uint_as_float(b & 0xFFFF0000u));
+    const uint32_t m = __float_as_uint(rest);
+    const float last = __fsub_rn(rest, __uint_as_float(m & 0xFFFF0000u));
+    return {{(uint16_t)(b >> 16), (uint16_t)(m >> 16), (uint16_t)(__float_as_uint(last) >> 16)}};
+}
+
+struct Few {
+    FourBit q;
+    int cols, split, shift;   // shift: log2(group / 128) for groups of 128 and more
+};
+
+int col_bytes(int blocks) { return blocks * 256 + 64; }   // 64 beyond a multiple of 128: lanes of two columns meet no bank twice
+
+struct Unit {
+    uint4 a, b;
+    float sa, sb;
+};
+
+// RUNS: runs of 32 inputs that share a scale (4: groups of 128 and more).
+template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWarps * 32, 2) few_kernel(const Few p) {
+    using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+    constexpr int P = kPieces<T>;
+    extern __shared__ __align__(16) uint8_t room[];   // [cols][col_bytes] entries, then the sums that warps exchange
+    const FourBit &q = p.q;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int stride = q.blocks * 256 + 64;
+    float *sums = (float *)(room + p.cols * stride);   // [2][kFewWarps][NT 8][kColStride]
+    const int teams = kFewWarps / p.split, team = warp / p.split, part = warp - team * p.split;
+    const int64_t tiles = (q.n + 15) / 16, all = (int64_t)gridDim.x * teams, id = (int64_t)blockIdx.x * teams + team;
+    const int64_t first = tiles * id / all, last = tiles * (id + 1) / all;
+    const int steps = (q.blocks - part + p.split - 1) / p.split;   // blocks of this warp in a tile
+
+    int64_t next_tile = first;
+    int next_step = 0;
+    const auto load = [&](Unit &u) {
+        if (next_tile >= last) return;
+        const int kb = part + next_step * p.split;
+        const int64_t ca = min(next_tile * 16 + g, q.n - 1), cb = min(next_tile * 16 + g + 8, q.n - 1);
+        const int64_t at = (int64_t)kb * 64 + t * 16, row = (int64_t)q.blocks * 64;
+        u.a = load_stream(q.codes + ca * row + at);
+        u.b = load_stream(q.codes + cb * row + at);
+        int i = RUNS == 4 ? kb >> p.shift : RUNS == 2 ? kb * 2 + (t & 1) : kb * 4 + t;
+        i = min(i, q.groups - 1);   // the last block's runs past k: their codes are zero
+        u.sa = load_as(q.scale_dtype, q.scale, ca * q.groups + i);
+        u.sb = load_as(q.scale_dtype, q.scale, cb * q.groups + i);
+        if (++next_step == steps) next_step = 0, next_tile++;
+    };
+    Unit ring[kDepth];
+#pragma unroll
+    for (int d = 0; d < kDepth; d++) load(ring[d]);
+
+    // the columns
+    const T *x = (const T *)q.x;
+    const int rows = (int)q.rows, padded = q.blocks * 128;
+    constexpr int N = kPer<T>;
+    if (((uintptr_t)x & 15) == 0 && (rows == 1 || q.x_stride % N == 0)) {
+        const int vecs = padded / N;
+        for (int r = 0; r < rows; r++)
+#pragma unroll 4
+            for (int v = threadIdx.x; v < vecs; v += kFewWarps * 32) {
+                uint4 e = make_uint4(0, 0, 0, 0);
+                if (v * N < q.k) e = load_again(x + r * q.x_stride + v * N);
+                if (v * N < q.k && v * N + N > q.k) {   // the vector that holds the row's end
+                    uint32_t *w = (uint32_t *)&e;
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        if (v * N + i >= q.k) w[i * 4 / N] &= N == 4 ? 0u : 0xFFFFu << (i & 1 ? 0 : 16);
+                }
+                if constexpr (P == 1) {
+                    *(uint4 *)(room + r * stride + v * 16) = e;
+                } else {
+                    const uint32_t w[4] = {e.x, e.y, e.z, e.w};
+                    Pieces c[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) c[i] = pieces_of(__uint_as_float(w[i]));
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+                        *(uint2 *)(room + (r * 3 + k) * stride + v * 8) =
+                            make_uint2(c[0].v[k] | (uint32_t)c[1].v[k] << 16, c[2].v[k] | (uint32_t)c[3].v[k] << 16);
+                }
+            }
+    } else {
+        for (int r = 0; r < rows; r++)
+#pragma unroll 4
+            for (int j = threadIdx.x; j < padded; j += kFewWarps * 32) {
+                T e;
+                from_f(0.0f, e);
+                if (j < q.k) e = x[r * q.x_stride + j];
+                if constexpr (P == 1) {
+                    *(T *)(room + r * stride + j * 2) = e;
+                } else {
+                    const Pieces c = pieces_of(e);
+#pragma unroll
+                    for (int k = 0; k < 3; k++) *(uint16_t *)(room + (r * 3 + k) * stride + j * 2) = c.v[k];
+                }
+            }
+    }
+    __syncthreads();
+
+    const uint8_t *col[NT];   // this lane's columns; those past the last are some other one's, and not read from the sums
+#pragma unroll
+    for (int i = 0; i < NT; i++) col[i] = room + min(i * 8 + g, p.cols - 1) * stride + t * 16;
+    float acc[NT][4] = {};
+    int turn = 0, step = 0;
+    for (int64_t tile = first; tile < last;) {
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            if (tile >= last) break;
+            const int kb = part + step * p.split;
+            const uint32_t wa[4] = {ring[d].a.x, ring[d].a.y, ring[d].a.z, ring[d].a.w};
+            const uint32_t wb[4] = {ring[d].b.x, ring[d].b.y, ring[d].b.z, ring[d].b.w};
+            float c[NT][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i % RUNS == 0)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) a[j] = codes_of<E>(wa[i], j), b[j] = codes_of<E>(wb[i], j);
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const uint4 e = *(const uint4 *)(col[j] + kb * 256 + i * 64);
+                    mma(c[j], a[0], b[0], a[1], b[1], e.x, e.y, E());
+                    mma(c[j], a[2], b[2], a[3], b[3], e.z, e.w, E());
+                }
+                if (i % RUNS == RUNS - 1) {
+                    float sa = ring[d].sa, sb = ring[d].sb;
+                    if (RUNS < 4) {
+                        sa = __shfl_sync(~0u, sa, (lane & ~3) | i / RUNS);
+                        sb = __shfl_sync(~0u, sb, (lane & ~3) | i / RUNS);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        acc[j][0] = fmaf(sa, c[j][0], acc[j][0]);
+                        acc[j][1] = fmaf(sa, c[j][1], acc[j][1]);
+                        acc[j][2] = fmaf(sb, c[j][2], acc[j][2]);
+                        acc[j][3] = fmaf(sb, c[j][3], acc[j][3]);
+                    }
+                }
+            }
+            load(ring[d]);
+            if (++step < steps) continue;
+            step = 0;
+            float *mine = sums + (turn * kFewWarps + warp) * (NT * 8 * kColStride);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                float *to = mine + (j * 8 + 2 * t) * kColStride + g;
+                to[0] = acc[j][0], to[kColStride] = acc[j][1], to[8] = acc[j][2], to[kColStride + 8] = acc[j][3];
+                acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+            }
+            if (p.split == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.split * 32) : "memory");
+            const float *from = sums + (turn * kFewWarps + team * p.split) * (NT * 8 * kColStride);
+            for (int o = part * 32 + lane; o < rows * 16; o += p.split * 32) {
+                const int r = o >> 4;
+                const int64_t ch = tile * 16 + (o & 15);
+                float v = 0.0f;
+                for (int w = 0; w < p.split; w++)
+#pragma unroll
+                    for (int k = 0; k < P; k++) v += from[w * (NT * 8 * kColStride) + (r * P + k) * kColStride + (o & 15)];
+                if (ch < q.n) store_as(q.out_dtype, q.out, r * q.out_stride + ch, v + (q.bias ? q.bias[ch] : 0.0f));
+            }
+            if (p.split == 1) __syncwarp();   // (two turns: with a barrier a tile no warp is two tiles ahead)
+            turn ^= 1;
+            tile++;
+        }
+    }
+}
+
+int few_bytes(int cols, int blocks) { return cols * col_bytes(blocks) + 2 * kFewWarps * ((cols + 7) / 8 * 8) * kColStride * 4; }
+template <typename T> bool is_few(int64_t rows, int blocks) {
+    return rows <= kFewCols / kPieces<T> && few_bytes((int)rows * kPieces<T>, blocks) <= 220 * 1024;
+}
+
+template <typename T, int NT, int RUNS> cudaError_t launch_few_as(Few p, cudaStream_t st) {
+    static SmemLimits limits;
+    const size_t smem = few_bytes(p.cols, p.q.blocks);
+    const cudaError_t e = raise_smem_limit((const void *)few_kernel<T, NT, RUNS>, smem, limits);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = (p.q.n + 15) / 16, fit = (int64_t)(smem <= 110 * 1024 ? 2 : 1) * sm_count();
+    // warps a tile: the least of rounds of tiles times what a tile takes a warp, with about a block for the exchange
+    int64_t least = INT64_MAX, grid = 1;
+    for (int split = 1; split <= kFewWarps && split <= p.q.blocks; split *= 2) {
+        const int64_t blocks = std::min<int64_t>((tiles * split + kFewWarps - 1) / kFewWarps, fit), teams = blocks * (kFewWarps / split);
+        const int64_t cost = (tiles + teams - 1) / teams * ((p.q.blocks + split - 1) / split + 1);
+        if (cost < least) least = cost, grid = blocks, p.split = split;
+    }
+    few_kernel<T, NT, RUNS><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p);
+    return cudaGetLastError();
+}
+template <typename T, int NT> cudaError_t launch_few_cols(const Few &p, cudaStream_t st) {
+    return p.q.group == 32 ? launch_few_as<T, NT, 1>(p, st) : p.q.group == 64 ? launch_few_as<T, NT, 2>(p, st) : launch_few_as<T, NT, 4>(p, st);
+}
+template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) {
+    Few p{q, (int)q.rows * kPieces<T>, 1, 0};
+    while (128 << p.shift < q.group) p.shift++;
+    return p.cols <= 8 ? launch_few_cols<T, 1>(p, st) : p.cols <= 16 ? launch_few_cols<T, 2>(p, st) : launch_few_cols<T, 3>(p, st);
+}
+
 bool shape_ok(int64_t n, int64_t k, int64_t group) {
     return n >= 1 && n <= INT32_MAX && k >= 1 && group >= 32 && (group & (group - 1)) == 0;
 }
@@ -194,7 +436,10 @@ int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n
     const FourBit p{d_x, rows, row_stride, n, (int)k, blocks_of(k), (int)group, groups_of(k, group), d_codes, scale_dtype,
                     d_scale, d_bias, out_dtype, d_out, out_stride};
     cudaError_t e = cudaSuccess;
-    const int rc = by_type(dtype, [&](auto t) { e = launch_plain<decltype(t)>(p, (cudaStream_t)stream); });
+    const int rc = by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        e = is_few<T>(rows, p.blocks) ? launch_few<T>(p, (cudaStream_t)stream) : launch_plain<T>(p, (cudaStream_t)stream);
+    });
     return rc != YGG_OK ? rc : e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 

@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <limits>
 #include <optional>
 
 #include "ygg_b200.h"
@@ -706,6 +707,8 @@ PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor *x = n == 4 ? cuda_tensor(args[0]) : nullptr;
     if (!x || dtype_of(x->scalar_type()) < 0 || x->dim() < 1 || x->size(-1) < 1 || !plain_rows(*x) || !PyFloat_CheckExact(args[3]))
         Py_RETURN_NONE;
+    const double eps = PyFloat_AS_DOUBLE(args[3]);
+    if (!(eps >= 0.0 && eps < std::numeric_limits<double>::infinity())) Py_RETURN_NONE;
     MaybeTensor a[2];
     bool wanted = x->requires_grad(), tangent = has_tangent(*x);
     for (int i = 0; i < 2; i++) {
@@ -717,7 +720,6 @@ PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
         tangent |= has_tangent(*t);
     }
     TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "layer_norm has no forward-mode derivative");
-    const double eps = PyFloat_AS_DOUBLE(args[3]);
     const c10::cuda::CUDAGuard on(x->device());
     if (wanted && at::GradMode::is_enabled()) return wrap(LayerNormNode::apply(*x, a[0], a[1], eps));
     return wrap(layer_norm(*x, a[0], a[1], eps, nullptr));
