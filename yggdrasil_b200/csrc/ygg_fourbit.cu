@@ -152,7 +152,9 @@ template <typename T> cudaError_t launch_plain(const FourBit &p, cudaStream_t st
 // exact and add up to it). A warp multiplies 16 channels by 8 columns and 16 inputs at a time (mma.sync, float sums): lane
 // (g, t) holds channels g and g + 8, and 16 bytes of each bring its piece t of four runs of 32 inputs. The columns lie in
 // shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory.
-constexpr int kFewCols = 24, kFewWarps = 8, kDepth = 4, kColStride = 20;
+constexpr int kFewCols = 24, kFewWarps = 8, kColStride = 20;
+// Blocks an SM: a warp's next 2 KB of codes are on their way while it multiplies nothing, so that the SM's warps cover for each other.
+constexpr int few_blocks(int nt) { return nt == 1 ? 4 : 3; }
 
 template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
 
@@ -169,7 +171,9 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, __nv_bfloat16) {   // 128 +
 // The inputs 2 j and 2 j + 1 of a word's piece.
 template <typename E> __device__ __forceinline__ uint32_t codes_of(uint32_t w, int j) {
     constexpr uint32_t magic = sizeof(E) == 2 && std::is_same<E, __half>::value ? 0x64006400u : 0x43004300u;
-    return sub2(((w >> (4 * j)) & 0x000F000Fu) | magic, E());
+    uint32_t v;   // (in one instruction: written in C it took two)
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * j)), "r"(0x000F000Fu), "r"(magic));
+    return sub2(v, E());
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -197,49 +201,74 @@ struct Few {
     int cols, split, shift;   // shift: log2(group / 128) for groups of 128 and more
 };
 
-int col_bytes(int blocks) { return blocks * 256 + 64; }   // 64 beyond a multiple of 128: lanes of two columns meet no bank twice
+// Bytes of a column, zeros past k up to a whole unit; 64 beyond a multiple of 128: lanes of two columns meet no bank twice.
+__host__ __device__ __forceinline__ int col_bytes(int units) { return units * 512 + 64; }
 
-struct Unit {
-    uint4 a, b;
-    float sa, sb;
+// Two blocks of both channels of a lane, and the scales that this lane of the four gets for all.
+template <int RUNS> struct Unit {
+    uint4 a[2], b[2];
+    uint32_t sa[RUNS == 1 ? 2 : 1], sb[RUNS == 1 ? 2 : 1];   // as they are stored
 };
-
+__device__ __forceinline__ float scale_of(uint32_t raw, int dtype) {
+    if (dtype == YGG_DTYPE_HALF) return __half2float(__ushort_as_half((unsigned short)raw));
+    return __uint_as_float(dtype == YGG_DTYPE_FLOAT ? raw : raw << 16);
+}
 // RUNS: runs of 32 inputs that share a scale (4: groups of 128 and more).
-template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWarps * 32, 2) few_kernel(const Few p) {
+template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWarps * 32, few_blocks(NT)) few_kernel(const Few p) {
     using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
     constexpr int P = kPieces<T>;
     extern __shared__ __align__(16) uint8_t room[];   // [cols][col_bytes] entries, then the sums that warps exchange
     const FourBit &q = p.q;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int stride = q.blocks * 256 + 64;
+    const int units = (q.blocks + 1) / 2, stride = col_bytes(units);
     float *sums = (float *)(room + p.cols * stride);   // [2][kFewWarps][NT 8][kColStride]
     const int teams = kFewWarps / p.split, team = warp / p.split, part = warp - team * p.split;
     const int64_t tiles = (q.n + 15) / 16, all = (int64_t)gridDim.x * teams, id = (int64_t)blockIdx.x * teams + team;
     const int64_t first = tiles * id / all, last = tiles * (id + 1) / all;
-    const int steps = (q.blocks - part + p.split - 1) / p.split;   // blocks of this warp in a tile
 
+    // What is loaded next. Rows past the last stand for some row that is there, and are not written; so does the second block
+    // of a row that has none: its inputs are zeros.
+    const bool wide = q.scale_dtype == YGG_DTYPE_FLOAT;
+    const int64_t row_bytes = q.blocks * 64, scale_bytes = (int64_t)q.groups * (wide ? 4 : 2);
+    const uint8_t *at_a = nullptr, *at_b = nullptr, *scale_a = nullptr, *scale_b = nullptr;
     int64_t next_tile = first;
-    int next_step = 0;
-    const auto load = [&](Unit &u) {
-        if (next_tile >= last) return;
-        const int kb = part + next_step * p.split;
-        const int64_t ca = min(next_tile * 16 + g, q.n - 1), cb = min(next_tile * 16 + g + 8, q.n - 1);
-        const int64_t at = (int64_t)kb * 64 + t * 16, row = (int64_t)q.blocks * 64;
-        u.a = load_stream(q.codes + ca * row + at);
-        u.b = load_stream(q.codes + cb * row + at);
-        int i = RUNS == 4 ? kb >> p.shift : RUNS == 2 ? kb * 2 + (t & 1) : kb * 4 + t;
-        i = min(i, q.groups - 1);   // the last block's runs past k: their codes are zero
-        u.sa = load_as(q.scale_dtype, q.scale, ca * q.groups + i);
-        u.sb = load_as(q.scale_dtype, q.scale, cb * q.groups + i);
-        if (++next_step == steps) next_step = 0, next_tile++;
-    };
-    Unit ring[kDepth];
+    int next = units;
+    const auto load = [&](Unit<RUNS> &u) {
+        if (next >= units) {
+            if (next_tile >= last) return;
+            next = part;
+            const int64_t a = min(next_tile * 16 + g, q.n - 1), b = min(next_tile * 16 + g + 8, q.n - 1);
+            at_a = q.codes + a * row_bytes + (part * 128 + t * 16);
+            at_b = q.codes + b * row_bytes + (part * 128 + t * 16);
+            scale_a = (const uint8_t *)q.scale + a * scale_bytes;
+            scale_b = (const uint8_t *)q.scale + b * scale_bytes;
+            next_tile++;
+        }
+        u.a[0] = load_stream(at_a);
+        u.b[0] = load_stream(at_b);
+        if (2 * next + 1 < q.blocks) {
+            u.a[1] = load_stream(at_a + 64);
+            u.b[1] = load_stream(at_b + 64);
+        }
 #pragma unroll
-    for (int d = 0; d < kDepth; d++) load(ring[d]);
+        for (int i = 0; i < (RUNS == 1 ? 2 : 1); i++) {   // scales past the last group: the last one's, on zeros
+            const int group = min(RUNS == 4 ? (2 * next + (t & 1)) >> p.shift : RUNS == 2 ? next * 4 + t : next * 8 + i * 4 + t, q.groups - 1);
+            if (wide) {
+                u.sa[i] = ((const uint32_t *)scale_a)[group];
+                u.sb[i] = ((const uint32_t *)scale_b)[group];
+            } else {
+                u.sa[i] = ((const uint16_t *)scale_a)[group];
+                u.sb[i] = ((const uint16_t *)scale_b)[group];
+            }
+        }
+        at_a += p.split * 128, at_b += p.split * 128, next += p.split;
+    };
+    Unit<RUNS> u = {};
+    load(u);
 
     // the columns
     const T *x = (const T *)q.x;
-    const int rows = (int)q.rows, padded = q.blocks * 128;
+    const int rows = (int)q.rows, padded = units * 256;
     constexpr int N = kPer<T>;
     if (((uintptr_t)x & 15) == 0 && (rows == 1 || q.x_stride % N == 0)) {
         const int vecs = padded / N;
@@ -289,74 +318,73 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
 #pragma unroll
     for (int i = 0; i < NT; i++) col[i] = room + min(i * 8 + g, p.cols - 1) * stride + t * 16;
     float acc[NT][4] = {};
-    int turn = 0, step = 0;
+    int turn = 0, unit = part;
     for (int64_t tile = first; tile < last;) {
+        float sa[RUNS == 1 ? 2 : 1], sb[RUNS == 1 ? 2 : 1], c[NT][4];
 #pragma unroll
-        for (int d = 0; d < kDepth; d++) {
-            if (tile >= last) break;
-            const int kb = part + step * p.split;
-            const uint32_t wa[4] = {ring[d].a.x, ring[d].a.y, ring[d].a.z, ring[d].a.w};
-            const uint32_t wb[4] = {ring[d].b.x, ring[d].b.y, ring[d].b.z, ring[d].b.w};
-            float c[NT][4];
+        for (int i = 0; i < (RUNS == 1 ? 2 : 1); i++)
+            sa[i] = scale_of(u.sa[i], q.scale_dtype), sb[i] = scale_of(u.sb[i], q.scale_dtype);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (i % RUNS == 0)
+        for (int i = 0; i < 8; i++) {   // runs of 32 inputs
+            const uint4 va = u.a[i / 4], vb = u.b[i / 4];
+            const uint32_t wa = i % 4 == 0 ? va.x : i % 4 == 1 ? va.y : i % 4 == 2 ? va.z : va.w;
+            const uint32_t wb = i % 4 == 0 ? vb.x : i % 4 == 1 ? vb.y : i % 4 == 2 ? vb.z : vb.w;
+            if (i % RUNS == 0)
 #pragma unroll
-                    for (int j = 0; j < NT; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-                uint32_t a[4], b[4];
+                for (int j = 0; j < NT; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+            uint32_t a[4], b[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) a[j] = codes_of<E>(wa[i], j), b[j] = codes_of<E>(wb[i], j);
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const uint4 e = *(const uint4 *)(col[j] + kb * 256 + i * 64);
-                    mma(c[j], a[0], b[0], a[1], b[1], e.x, e.y, E());
-                    mma(c[j], a[2], b[2], a[3], b[3], e.z, e.w, E());
-                }
-                if (i % RUNS == RUNS - 1) {
-                    float sa = ring[d].sa, sb = ring[d].sb;
-                    if (RUNS < 4) {
-                        sa = __shfl_sync(~0u, sa, (lane & ~3) | i / RUNS);
-                        sb = __shfl_sync(~0u, sb, (lane & ~3) | i / RUNS);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        acc[j][0] = fmaf(sa, c[j][0], acc[j][0]);
-                        acc[j][1] = fmaf(sa, c[j][1], acc[j][1]);
-                        acc[j][2] = fmaf(sb, c[j][2], acc[j][2]);
-                        acc[j][3] = fmaf(sb, c[j][3], acc[j][3]);
-                    }
-                }
-            }
-            load(ring[d]);
-            if (++step < steps) continue;
-            step = 0;
-            float *mine = sums + (turn * kFewWarps + warp) * (NT * 8 * kColStride);
+            for (int j = 0; j < 4; j++) a[j] = codes_of<E>(wa, j), b[j] = codes_of<E>(wb, j);
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                float *to = mine + (j * 8 + 2 * t) * kColStride + g;
-                to[0] = acc[j][0], to[kColStride] = acc[j][1], to[8] = acc[j][2], to[kColStride + 8] = acc[j][3];
-                acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+                const uint4 e = *(const uint4 *)(col[j] + unit * 512 + i * 64);
+                mma(c[j], a[0], b[0], a[1], b[1], e.x, e.y, E());
+                mma(c[j], a[2], b[2], a[3], b[3], e.z, e.w, E());
             }
-            if (p.split == 1) __syncwarp();
-            else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.split * 32) : "memory");
-            const float *from = sums + (turn * kFewWarps + team * p.split) * (NT * 8 * kColStride);
-            for (int o = part * 32 + lane; o < rows * 16; o += p.split * 32) {
-                const int r = o >> 4;
-                const int64_t ch = tile * 16 + (o & 15);
-                float v = 0.0f;
-                for (int w = 0; w < p.split; w++)
+            if (i % RUNS == RUNS - 1) {
+                const float fa = __shfl_sync(~0u, sa[RUNS == 1 ? i / 4 : 0], (lane & ~3) | (i / RUNS & 3));
+                const float fb = __shfl_sync(~0u, sb[RUNS == 1 ? i / 4 : 0], (lane & ~3) | (i / RUNS & 3));
 #pragma unroll
-                    for (int k = 0; k < P; k++) v += from[w * (NT * 8 * kColStride) + (r * P + k) * kColStride + (o & 15)];
-                if (ch < q.n) store_as(q.out_dtype, q.out, r * q.out_stride + ch, v + (q.bias ? q.bias[ch] : 0.0f));
+                for (int j = 0; j < NT; j++) {
+                    acc[j][0] = fmaf(fa, c[j][0], acc[j][0]);
+                    acc[j][1] = fmaf(fa, c[j][1], acc[j][1]);
+                    acc[j][2] = fmaf(fb, c[j][2], acc[j][2]);
+                    acc[j][3] = fmaf(fb, c[j][3], acc[j][3]);
+                }
             }
-            if (p.split == 1) __syncwarp();   // (two turns: with a barrier a tile no warp is two tiles ahead)
-            turn ^= 1;
-            tile++;
         }
+        load(u);
+        unit += p.split;
+        if (unit < units) continue;
+        unit = part;
+        float *mine = sums + (turn * kFewWarps + warp) * (NT * 8 * kColStride);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            float *to = mine + (j * 8 + 2 * t) * kColStride + g;
+            to[0] = acc[j][0], to[kColStride] = acc[j][1], to[8] = acc[j][2], to[kColStride + 8] = acc[j][3];
+            acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+        }
+        if (p.split == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.split * 32) : "memory");
+        const float *from = sums + (turn * kFewWarps + team * p.split) * (NT * 8 * kColStride);
+        for (int o = part * 32 + lane; o < rows * 16; o += p.split * 32) {
+            const int r = o >> 4;
+            const int64_t ch = tile * 16 + (o & 15);
+            float v = 0.0f;
+            for (int w = 0; w < p.split; w++)
+#pragma unroll
+                for (int k = 0; k < P; k++) v += from[w * (NT * 8 * kColStride) + (r * P + k) * kColStride + (o & 15)];
+            if (ch < q.n) store_as(q.out_dtype, q.out, r * q.out_stride + ch, v + (q.bias ? q.bias[ch] : 0.0f));
+        }
+        if (p.split == 1) __syncwarp();   // (two turns: with a barrier a tile no warp is two tiles ahead)
+        turn ^= 1;
+        tile++;
     }
 }
 
-int few_bytes(int cols, int blocks) { return cols * col_bytes(blocks) + 2 * kFewWarps * ((cols + 7) / 8 * 8) * kColStride * 4; }
+int few_bytes(int cols, int blocks) {
+    return cols * col_bytes((blocks + 1) / 2) + 2 * kFewWarps * ((cols + 7) / 8 * 8) * kColStride * 4;
+}
 template <typename T> bool is_few(int64_t rows, int blocks) {
     return rows <= kFewCols / kPieces<T> && few_bytes((int)rows * kPieces<T>, blocks) <= 220 * 1024;
 }
@@ -366,14 +394,18 @@ template <typename T, int NT, int RUNS> cudaError_t launch_few_as(Few p, cudaStr
     const size_t smem = few_bytes(p.cols, p.q.blocks);
     const cudaError_t e = raise_smem_limit((const void *)few_kernel<T, NT, RUNS>, smem, limits);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = (p.q.n + 15) / 16, fit = (int64_t)(smem <= 110 * 1024 ? 2 : 1) * sm_count();
-    // warps a tile: the least of rounds of tiles times what a tile takes a warp, with about a block for the exchange
-    int64_t least = INT64_MAX, grid = 1;
-    for (int split = 1; split <= kFewWarps && split <= p.q.blocks; split *= 2) {
-        const int64_t blocks = std::min<int64_t>((tiles * split + kFewWarps - 1) / kFewWarps, fit), teams = blocks * (kFewWarps / split);
-        const int64_t cost = (tiles + teams - 1) / teams * ((p.q.blocks + split - 1) / split + 1);
-        if (cost < least) least = cost, grid = blocks, p.split = split;
+    const int64_t tiles = (p.q.n + 15) / 16, units = (p.q.blocks + 1) / 2, resident = std::max<int64_t>(1, std::min<int64_t>(few_blocks(NT), 227 * 1024 / (smem + 1024)));
+    // Warps a tile: as few as keep the SMs' warps busy over whole rounds of tiles, since the exchange costs each of them. 1 x 4096
+    // x 32768 (0.86 of the warps for two or more): two 21.0 us, four 21.8, eight 22.9, one (0.43) 25.5; 1 x 4096 x 4096: eight
+    // 5.7, four 6.8; 16 x 4096 x 32768 (one block an SM): four 51.4, one and two 57.
+    const int64_t warps = resident * sm_count() * kFewWarps;
+    double most = 0.0;
+    for (int split = 1; split <= kFewWarps && split <= units; split *= 2) {
+        const int64_t busy = tiles * split, rounds = (busy + warps - 1) / warps;
+        const double share = (double)busy / (double)(rounds * warps);
+        if (share > most * 1.02) most = share, p.split = split;
     }
+    const int64_t grid = std::min<int64_t>((tiles * p.split + kFewWarps - 1) / kFewWarps, resident * sm_count());
     few_kernel<T, NT, RUNS><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p);
     return cudaGetLastError();
 }
