@@ -346,10 +346,15 @@ YGG_API int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, i
  *   d_out_done   bytes [prompts][width], or NULL: the parent was done, or the token is `end`
  * A beam of -inf logits alone is worth -inf everywhere, one that holds NaN or +inf is worth NaN; NaN ranks as -inf. */
 #define YGG_BEAMS_MAX 64        /* most beams, and most picks, of a prompt */
+
+/* Bytes of device workspace that ygg_beam_select needs, 16-byte aligned; it may be 0. */
+YGG_API size_t ygg_beam_workspace(int dtype, int64_t prompts, int64_t beams, int64_t vocab, int64_t width);
+
 YGG_API int ygg_beam_select(int device, int dtype, int64_t prompts, int64_t beams, int64_t vocab, const void *d_logits,
                             int64_t prompt_stride, int64_t beam_stride, int score_bytes, const void *d_scores,
                             const uint8_t *d_done, int64_t end, int64_t width, void *d_out_scores, int32_t *d_tokens,
-                            int32_t *d_parents, uint8_t *d_out_done, void *stream);
+                            int32_t *d_parents, uint8_t *d_out_done, void *d_workspace, size_t workspace_bytes,
+                            void *stream);
 
 /* Row prompt width + j of d_to[i] = row prompt beams + d_parents[prompt][j] of d_from[i] (rows of row_bytes[i] bytes, side by
  * side), zeros where the parent is negative or beyond the beams; for `count` arrays in one launch. parent_bytes 4 or 8. No

@@ -294,13 +294,15 @@ def test_refusals():
 def test_c_entries_refuse_bad_arguments():
     lib = _native.ops()
     choose = lambda prompts=1, beams=2, vocab=9, sb=4, done=None, end=-1, width=2, x=16, s=16, out=16, dtype=0: lib.ygg_beam_select(  # noqa: E731
-        0, dtype, prompts, beams, vocab, x, beams * vocab, vocab, sb, s, done, end, width, out, 16, 16, None, None)
+        0, dtype, prompts, beams, vocab, x, beams * vocab, vocab, sb, s, done, end, width, out, 16, 16, None, None, 0, None)
     for kw in (dict(prompts=-1), dict(beams=0), dict(vocab=0), dict(width=0), dict(sb=2), dict(width=19), dict(end=9), dict(end=-2),
                dict(done=16), dict(x=None), dict(s=None), dict(out=None)):
         assert choose(**kw) == _native.YGG_E_ARG, kw
     for kw in (dict(beams=65), dict(width=65, vocab=100), dict(vocab=1 << 30), dict(prompts=1 << 31)):
         assert choose(**kw) == _native.YGG_E_UNSUPPORTED, kw
     assert choose(prompts=0, x=None) == _native.YGG_OK
+    assert lib.ygg_beam_workspace(0, 4, 4, 100000, 4) > 0 and choose(beams=8, vocab=100000) == _native.YGG_E_ARG   # no workspace
+    assert lib.ygg_beam_workspace(0, -1, 4, 100, 4) == lib.ygg_beam_workspace(0, 1, 65, 100, 4) == 0
     import ctypes
     one = (ctypes.c_void_p * 1)(16)
     size = (ctypes.c_int64 * 1)(4)

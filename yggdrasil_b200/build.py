@@ -21,7 +21,7 @@ OPS_SOURCE = CSRC / "ygg_torch.cpp"
 SOURCES = [CSRC / "ygg_load.cu", CSRC / "ygg_step.cu", CSRC / "ygg_coop.cu", CSRC / "ygg_grouped.cu",
            CSRC / "ygg_float.cu", CSRC / "ygg_logprobs.cu", CSRC / "ygg_linear.cu",
            CSRC / "ygg_pages.cu", CSRC / "ygg_fourbit.cu", CSRC / "ygg_select.cu", CSRC / "ygg_norm.cu"]
-HEADERS = [CSRC / "ygg_model.h", CSRC / "ygg_smem.h", CSRC / "ygg_device.cuh", CSRC / "ygg_ops.cuh",
+HEADERS = [CSRC / "ygg_model.h", CSRC / "ygg_smem.h", CSRC / "ygg_device.cuh", CSRC / "ygg_ops.cuh", CSRC / "ygg_rows.cuh",
            CSRC / "ygg_tensor.cuh", ROOT / "include" / "ygg_b200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # no --use_fast_math and no FMA contraction: every f32 op of the step is single-rounded as in the reference

@@ -578,11 +578,15 @@ PyObject *py_beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor scores = empty({prompts, width}, s->scalar_type(), device), tokens = empty({prompts, width}, at::kInt, device),
                  parents = empty({prompts, width}, at::kInt, device),
                  ended = end < 0 ? Tensor() : empty({prompts, width}, at::kBool, device);
+    const int64_t bytes = (int64_t)ygg_beam_workspace(dtype_of(x->scalar_type()), prompts, x->size(1), x->size(2), width);
+    Tensor room;
+    if (bytes) room = empty({bytes}, at::kByte, device);
     raise_for(ygg_beam_select(device.index(), dtype_of(x->scalar_type()), prompts, x->size(1), x->size(2), x->data_ptr(),
                               x->stride(0), x->stride(1), (int)s->element_size(), s->data_ptr(),
                               done ? (const uint8_t *)done->data_ptr() : nullptr, end, width, scores.data_ptr(),
                               (int32_t *)tokens.data_ptr(), (int32_t *)parents.data_ptr(),
-                              ended.defined() ? (uint8_t *)ended.data_ptr() : nullptr, stream_of(device.index())),
+                              ended.defined() ? (uint8_t *)ended.data_ptr() : nullptr, bytes ? room.data_ptr() : nullptr,
+                              (size_t)bytes, stream_of(device.index())),
               "ygg_beam_select");
     PyObject *r = PyTuple_New(4);
     if (!r) throw python_error();
