@@ -160,6 +160,9 @@ def test_scores_that_are_not_finite():
         check(f(x, s, width), x, s, width)
         done = torch.tensor([[True, False, False, True, True]] * 2, device="cuda")
         check(f(x, s, width, done=done, end=3), x, s, width, done, 3)
+    far = torch.tensor([[-1e39, -2e39, 3.0, -1.5e39, -1e38], [1e39, 2.0, 1e39, 3e38, -1e300]], dtype=torch.float64, device="cuda")
+    for width in (3, 60):
+        check(f(x, far, width), x, far, width)
     first = torch.full((2, 5), -INF, device="cuda")
     first[:, 0] = 0
     check(f(x, first, 5), x, first, 5)

@@ -41,9 +41,9 @@ struct Select {
 };
 
 // Twice what an lse is off, at most: a term by 2^-22 of exp2 and 2^-23 |y| of its argument (y = x - m, rounded, times log2 e,
-// rounded; weighted by e^y at most log V, 12: 1.4e-6); a chain of 8 + 3 + 4 + 5 additions by 2^-24 each (1.2e-6); three new references by
-// 2^-22 and their argument (1.2e-6).
-constexpr double kNear = 1e-5;
+// rounded; weighted by e^y at most log V, 12: 1.4e-6); a chain of 8 + 3 + 4 + 5 + 6 additions by 2^-24 each (1.6e-6); four new references by
+// 2^-22 and their argument (1.6e-6); log2 by 2^-22.
+constexpr double kNear = 1.2e-5;
 
 // What a beam's continuations are worth: score + (x - lse). m: the row's largest entry.
 struct Beam {
@@ -61,12 +61,7 @@ __device__ __forceinline__ double worth(const Beam &b, float x, int v, int end) 
     return b.score + (b.lse == -INFINITY ? -INFINITY : (double)x - b.lse);
 }
 __device__ __forceinline__ double rank_of(double worth) { return isnan(worth) ? -INFINITY : worth; }
-// Floats at or below the worth, in the order of integers; only what is -inf (or NaN) is kClosed.
-constexpr int kClosed = (int)0x807FFFFF;
-__device__ __forceinline__ int key_of(double worth) {
-    const double r = rank_of(worth);
-    return r == -INFINITY ? kClosed : order(fmaxf(__double2float_rd(r), -3.402823466e38f));
-}
+constexpr int kClosed = (int)0x807FFFFF;   // order() of -inf, and of NaN
 
 __device__ __forceinline__ void write_pick(const Select &p, int64_t prompt, int k, uint32_t at, double value, const Beam *beams) {
     const int64_t to = prompt * p.width + k;
@@ -128,12 +123,14 @@ template <int THREADS> constexpr int kRoom = THREADS == 32 ? 128 : 1024;   // ca
 
 template <int THREADS> struct Team {
     Beam beams[kBeams<THREADS>];
+    float about[kBeams<THREADS>];   // score - lse
     double value[kRoom<THREADS>];
-    uint32_t at[kRoom<THREADS>], list[kRoom<THREADS>];   // list: segments, then the candidates' order
+    uint32_t at[kRoom<THREADS>];
+    uint2 list[kRoom<THREADS>];     // segments and their keys; then, in x, the candidates' order
     double part[THREADS / 32];
     uint32_t part_at[THREADS / 32];
-    int count[3], candidates, segments;
-    unsigned long long near;   // rows whose lse is wanted in 64 bits
+    int bound[THREADS / 32], count[3], candidates, segments;
+    unsigned long long near;        // rows whose lse is wanted in 64 bits
 };
 
 template <int THREADS> __device__ __forceinline__ void sync() {
@@ -212,160 +209,38 @@ template <typename T, int THREADS> __device__ __noinline__ void pick_slowly(cons
     }
 }
 
-// tops [beams][pieces][32] and sums [beams][pieces] of the prompt; keys: room for as many numbers as `tops` has, or kKeys (they may
-// be the same memory where all fit). per: vectors of a segment.
-constexpr int kKeys = 8192;
+// The candidates' order and the picks.
 template <typename T, int THREADS>
-__device__ void choose(const Select &p, int64_t prompt, int t, const float *tops, const float2 *sums, int *keys, int per, Team<THREADS> &sh) {
-    constexpr int N = kPer<T>;
-    const int lane = t & 31, row_segments = p.pieces * 32, segments = p.beams * row_segments;
-    const bool fits = segments <= kKeys;
-    // each row's lse
-    for (int b = t >> 5; b < p.beams; b += THREADS / 32) {
-        const int64_t row = prompt * p.beams + b;
-        const bool done = p.done && p.done[row];
-        float m = -INFINITY;
-        double s = 0.0;
-        if (!done) {
-            for (int i = lane; i < p.pieces; i += 32) m = fmaxf(m, sums[b * p.pieces + i].x);
-            m = unorder(__reduce_max_sync(~0u, order(m)));
-            for (int i = lane; i < p.pieces; i += 32) {
-                const float2 f = sums[b * p.pieces + i];
-                s += p.pieces == 1 ? (double)f.y : f.x == -INFINITY ? (double)f.y : (double)f.y * exp64((double)f.x - (double)m);
-            }
-            s = shuffle_add(s);
-        }
-        if (lane == 0) {
-            const double score = p.wide ? ((const double *)p.scores)[row] : (double)((const float *)p.scores)[row];
-            sh.beams[b] = {score, isnan(s) ? (double)NAN : m == -INFINITY ? -INFINITY : (double)m + log(s), m, done};
-        }
-    }
-    if (t == 0) sh.candidates = sh.segments = 0, sh.count[0] = sh.count[1] = sh.count[2] = 0, sh.near = 0;
-    sync<THREADS>();
-
-    // a bound that at least `width` segments reach
-    const auto value_of = [&](int b, int i) {   // of a segment's largest entry; a done beam is one entry
-        const Beam &beam = sh.beams[b];
-        return beam.done ? (i ? -INFINITY : beam.score) : worth(beam, tops[b * row_segments + i], 0, -1);
-    };
-    int most = kClosed;
-    for (int b = 0, j = t; b < p.beams; b++)
-        for (; j < (b + 1) * row_segments; j += THREADS) {
-            int k = key_of(value_of(b, j - b * row_segments));
-            if (!fits && j >= kKeys) k = max(k, keys[j & (kKeys - 1)]);   // this thread's own: THREADS divides kKeys
-            keys[fits ? j : j & (kKeys - 1)] = k;
-            most = max(most, k);
-        }
-    const int held = min(segments, kKeys);
-    most = __reduce_max_sync(~0u, most);
-    if (THREADS > 32) {
-        if (lane == 0) sh.list[t >> 5] = (uint32_t)most;
-        __syncthreads();
-        for (int w = 0; w < THREADS / 32; w++) most = max(most, (int)sh.list[w]);
-    }
-    sync<THREADS>();
-    int round = 0;
-    const auto reach = [&](int bound) {   // how many keys are at least the bound
-        int n = 0;
-        for (int j = t; j < held; j += THREADS) n += keys[j] >= bound;
-        n = __reduce_add_sync(~0u, n);
-        if (THREADS == 32) return n;
-        if (lane == 0 && n) atomicAdd(&sh.count[round], n);
-        if (t == 0) sh.count[round == 2 ? 0 : round + 1] = 0;
-        __syncthreads();
-        n = sh.count[round];
-        round = round == 2 ? 0 : round + 1;
-        return n;
-    };
-    bool open = false;   // no bound: all that is not closed
-    int bound = kClosed + 1;
-    if (most == kClosed || reach(bound) < p.width) {
-        open = true;
-    } else {
-        int hi = most;
-        const int guess = order(unorder(most) - 32.0f);
-        if (guess > bound && guess < hi) {
-            if (reach(guess) >= p.width) bound = guess;
-            else hi = guess - 1;
-        }
-        while (bound < hi) {
-            const int mid = bound + (int)(((unsigned)hi - (unsigned)bound + 1u) / 2u);
-            const int n = reach(mid);
-            if (n < p.width) {
-                hi = mid - 1;
-            } else {
-                bound = mid;
-                if (n <= p.width + p.width / 4) break;
-            }
-        }
-        open = unorder(bound) < -1e38f;   // beyond what keys tell apart
-    }
-    const double least = open ? -INFINITY : (double)unorder(bound) - kNear;
-    const int least_key = open ? kClosed + 1 : order(__double2float_rd(least));
-
-    // the segments that reach it, and their entries that do
-    const auto push = [&](double value, uint32_t at) {
-        const int i = atomicAdd(&sh.candidates, 1);
-        if (i < kRoom<THREADS>) sh.value[i] = value, sh.at[i] = at;
-    };
-    for (int b = 0, j = t; b < p.beams; b++)
-        for (; j < (b + 1) * row_segments; j += THREADS) {
-            if ((fits ? keys[j] : keys[j & (kKeys - 1)]) < least_key) continue;
-            if (!fits && key_of(value_of(b, j - b * row_segments)) < least_key) continue;
-            if (sh.beams[b].done) {
-                push(sh.beams[b].score, (uint32_t)b * (uint32_t)p.vocab + (uint32_t)p.end);
-            } else {
-                const int i = atomicAdd(&sh.segments, 1);
-                if (i < kRoom<THREADS>) sh.list[i] = (uint32_t)j;
-            }
-        }
-    sync<THREADS>();
-    const int listed = sh.segments;
-    if (listed > kRoom<THREADS>) {
-        pick_slowly<T, THREADS>(p, prompt, t, sh);
-        return;
-    }
-    for (int item = t; item < listed * per; item += THREADS) {
-        const int e = item / per, i = item - e * per, j = (int)sh.list[e], b = j / row_segments;
-        const int piece = (j - b * row_segments) >> 5;
-        const T *x = row_of<T>(p, prompt, b);
-        const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab, u = (uint32_t)(piece * per + i) * (32 * N) + (j & 31) * N;
-        if (u >= end) continue;
-        float v[N];
-        unpack(load_run<T, true>(x - off, u, off, end, 0), v, T());
-        const Beam beam = sh.beams[b];
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            const double w = worth(beam, v[k], 0, -1);
-            if (open ? w > -INFINITY : w >= least) push(w, (uint32_t)b * (uint32_t)p.vocab + (u + k - off));
-        }
-    }
-    sync<THREADS>();
-    const int n = sh.candidates;
-    if (n > kRoom<THREADS>) {
-        pick_slowly<T, THREADS>(p, prompt, t, sh);
-        return;
-    }
-
-    // their order
-    const auto rank = [&] {
-        for (int c = t; c < n; c += THREADS) {
+__device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt, int t, int n, Team<THREADS> &sh) {
+    const int lane = t & 31;
+    // A few of them are a warp's work, and the others wait for whether rows are wanted in 64 bits.
+    const auto rank = [&](int first, int step) {
+        for (int c = first; c < n; c += step) {
             const double v = sh.value[c];
             const uint32_t at = sh.at[c];
             int r = 0;
+#pragma unroll 4
             for (int i = 0; i < n; i++) r += better(sh.value[i], sh.at[i], v, at);
-            sh.list[r] = c;
+            sh.list[r].x = c;
         }
-        sync<THREADS>();
     };
-    rank();
-    const auto beam_of = [&](int r) { return (int)(sh.at[sh.list[r]] / (uint32_t)p.vocab); };
-    for (int r = t + 1; r < n; r += THREADS) {   // with the one before, or, past the last pick, with that
-        const int q = min(r, p.width) - 1, a = beam_of(q), b = beam_of(r);
-        if (p.wide || (a != b && sh.value[sh.list[q]] - sh.value[sh.list[r]] < kNear))
-            atomicOr(&sh.near, (1ull << a) | (1ull << b));
+    const bool few = THREADS == 32 || n <= 64;
+    if (!few || t < 32) rank(few ? lane : t, few ? 32 : THREADS);
+    if (few) __syncwarp();
+    else sync<THREADS>();
+    if (t < 32) {
+        unsigned long long near = 0;
+        for (int r = lane; r < n; r += 32) {   // with the one before, or, past the last pick, with that
+            const int q = max(min(r, p.width) - 1, 0), cq = sh.list[q].x, cr = sh.list[r].x;
+            const uint32_t a = sh.at[cq] / (uint32_t)p.vocab, b = sh.at[cr] / (uint32_t)p.vocab;
+            if (p.wide || (a != b && sh.value[cq] - sh.value[cr] < kNear)) near |= (1ull << a) | (1ull << b);
+        }
+        near = (unsigned long long)__reduce_or_sync(~0u, (unsigned)(near >> 32)) << 32 | __reduce_or_sync(~0u, (unsigned)near);
+        if (THREADS > 32 && t == 0) sh.near = near;
+        if (THREADS == 32) sh.near = near;
+        if (!near)
+            for (int k = lane; k < min(n, p.width); k += 32) write_pick(p, prompt, k, sh.at[sh.list[k].x], sh.value[sh.list[k].x], sh.beams);
     }
-    if (p.wide && t == 0 && n) atomicOr(&sh.near, 1ull << beam_of(0));
     sync<THREADS>();
     const unsigned long long near = sh.near;
     if (near) {
@@ -375,9 +250,10 @@ __device__ void choose(const Select &p, int64_t prompt, int t, const float *tops
             if (near >> b & 1) sh.value[c] = worth(sh.beams[b], to_f(row_of<T>(p, prompt, b)[v]), v, p.end);
         }
         sync<THREADS>();
-        rank();
+        rank(t, THREADS);
+        sync<THREADS>();
+        for (int k = t; k < min(n, p.width); k += THREADS) write_pick(p, prompt, k, sh.at[sh.list[k].x], sh.value[sh.list[k].x], sh.beams);
     }
-    for (int k = t; k < min(n, p.width); k += THREADS) write_pick(p, prompt, k, sh.at[sh.list[k]], sh.value[sh.list[k]], sh.beams);
     if (n >= p.width || t >= 32) return;
     // fewer are open than are wanted: closed ones in their order
     const uint32_t all = (uint32_t)p.beams * (uint32_t)p.vocab;
@@ -395,26 +271,457 @@ __device__ void choose(const Select &p, int64_t prompt, int t, const float *tops
     }
 }
 
-// A prompt to a team, in one launch; the team's warps share its rows' pieces. Dynamic shared memory: for each team [beams][pieces][32] largest entries
-// (then their keys) and [beams][pieces] sums.
-template <typename T, int VECS, int THREADS> __global__ void __launch_bounds__(256) small_kernel(const Select p) {
-    extern __shared__ __align__(16) uint8_t room[];
-    __shared__ Team<THREADS> teams[256 / THREADS];
-    const int team = threadIdx.x / THREADS, t = threadIdx.x % THREADS, lane = t & 31, all = p.beams * p.pieces;
-    const int64_t prompt = (int64_t)blockIdx.x * (256 / THREADS) + team;
-    if (prompt >= p.prompts) return;   // a whole team
-    float *tops = (float *)(room + (size_t)team * all * 136);
-    float2 *sums = (float2 *)(tops + all * 32);
-    for (int i = t >> 5; i < all; i += THREADS / 32) {
-        const int b = i / p.pieces;
-        if (p.done && p.done[prompt * p.beams + b]) continue;
-        float top;
-        const float2 s = sum_piece<T, VECS>(row_of<T>(p, prompt, b), p.vocab, i - b * p.pieces, 1, lane, top);
-        tops[i * 32 + lane] = top;
-        if (lane == 0) sums[i] = s;
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ Beam beam_of(const Select &p, int64_t row, bool done, float m, float s) {
+    const double score = p.wide ? ((const double *)p.scores)[row] : (double)((const float *)p.scores)[row];
+    const double lse = isnan(s) ? (double)NAN : m == -INFINITY ? -INFINITY : fma((double)log2_approx(s), 0.693147180559945309, (double)m);
+    return {score, lse, m, done};
+}
+
+// score - lse in a float; a finite one stays finite.
+__device__ __forceinline__ float about_of(const Beam &b) {
+    if (!b.done && b.lse == -INFINITY) return -INFINITY;
+    const double v = b.done ? b.score : b.score - b.lse;
+    return isfinite(v) ? (float)fmin(fmax(v, -3.402823466e38), 3.402823466e38) : (float)v;
+}
+
+// What a segment's largest entry is worth, in a float: -inf (or NaN) only where it is that in 64 bits.
+__device__ __forceinline__ float worth_of(float top, float about) {
+    const float v = top + about;
+    return top == -INFINITY ? top : v == -INFINITY && about > -INFINITY ? -3.402823466e38f : v;
+}
+
+// The largest bound that `width` lanes (at least; a quarter more at most, where the search finds one) reach; kClosed if there is none.
+__device__ __forceinline__ int bound_of_lanes(int mine, int width) {
+    const int most = __reduce_max_sync(~0u, mine);
+    if (width > 32 || __popc(__ballot_sync(~0u, mine > kClosed)) < width) return kClosed;
+    int lo = __reduce_min_sync(~0u, mine), hi = most;   // lo: all lanes reach it, or it is kClosed
+    lo = max(lo, kClosed + 1);
+    const int guess = order(unorder(most) - 32.0f);
+    if (guess > lo && guess < hi) {
+        if (__popc(__ballot_sync(~0u, mine >= guess)) >= width) lo = guess;
+        else hi = guess - 1;
+    }
+    while (lo < hi) {
+        const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
+        const int n = __popc(__ballot_sync(~0u, mine >= mid));
+        if (n < width) {
+            hi = mid - 1;
+        } else {
+            lo = mid;
+            if (n <= width + width / 4) break;
+        }
+    }
+    return lo;
+}
+
+// tops [beams][pieces][32] (of a done beam: 0, then -inf) and sums [beams][pieces] of the prompt; keys: room for as many numbers as `tops` has, or kKeys (they may
+// be the same memory where all fit). per_log: log2 of the vectors of a segment.
+constexpr int kKeys = 8192;
+template <typename T, int THREADS>
+__device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, const float *tops, const float2 *sums, int *keys, int per_log, Team<THREADS> &sh) {
+    constexpr int N = kPer<T>;
+    const int lane = t & 31, row_segments = p.pieces * 32, segments = p.beams * row_segments;
+    const bool fits = segments <= kKeys;
+    // each row's lse: a thread a row, or a warp where a row has more pieces
+    if (THREADS == 32 || p.pieces <= 4) {
+        if (t < p.beams) {
+            const int64_t row = prompt * p.beams + t;
+            const bool done = p.done && p.done[row];
+            float m = -INFINITY, s = 0.0f;
+            if (!done) {
+                for (int i = 0; i < p.pieces; i++) m = fmaxf(m, sums[t * p.pieces + i].x);
+                for (int i = 0; i < p.pieces; i++) {
+                    const float2 f = sums[t * p.pieces + i];
+                    s += f.x == m || f.x == -INFINITY ? f.y : f.y * exp2_approx((f.x - m) * kLog2e);
+                }
+            }
+            const Beam beam = beam_of(p, row, done, m, s);
+            sh.beams[t] = beam;
+            sh.about[t] = about_of(beam);
+        }
+    } else {
+        for (int b = t >> 5; b < p.beams; b += THREADS / 32) {
+            const int64_t row = prompt * p.beams + b;
+            const bool done = p.done && p.done[row];
+            float m = -INFINITY, s = 0.0f;
+            if (!done) {
+                for (int i = lane; i < p.pieces; i += 32) m = fmaxf(m, sums[b * p.pieces + i].x);
+                m = unorder(__reduce_max_sync(~0u, order(m)));
+                for (int i = lane; i < p.pieces; i += 32) {
+                    const float2 f = sums[b * p.pieces + i];
+                    s += f.x == m || f.x == -INFINITY ? f.y : f.y * exp2_approx((f.x - m) * kLog2e);
+                }
+#pragma unroll
+                for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+            }
+            if (lane == 0) {
+                const Beam beam = beam_of(p, row, done, m, s);
+                sh.beams[b] = beam;
+                sh.about[b] = about_of(beam);
+            }
+        }
+    }
+    if (t == 0) sh.candidates = sh.segments = 0, sh.count[0] = sh.count[1] = sh.count[2] = 0, sh.near = 0;
+    sync<THREADS>();
+
+    // A bound that at least `width` segments reach, in floats: a segment's key is its largest entry's worth, off by two roundings.
+    int mine = kClosed;
+    float far = 0.0f;   // the largest magnitude that a key was rounded from
+    for (int b = 0; b < p.beams; b++) {
+        const float about = fabsf(sh.about[b]);
+        if (about < INFINITY) far = fmaxf(far, about);
+    }
+    for (int j = t; j < segments; j += 8 * THREADS) {
+        float top[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) top[i] = j + i * THREADS < segments ? tops[j + i * THREADS] : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int at = j + i * THREADS;
+            if (at >= segments) break;
+            int k = order(worth_of(top[i], sh.about[(unsigned)at / (unsigned)row_segments]));
+            mine = max(mine, k);
+            if (!fits && at >= kKeys) k = max(k, keys[at & (kKeys - 1)]);   // this thread's own: THREADS divides kKeys
+            keys[fits ? at : at & (kKeys - 1)] = k;
+        }
+    }
+    const int held = min(segments, kKeys);
+    int bound = bound_of_lanes(mine, p.width);
+    if (THREADS > 32) {
+        if (lane == 0) sh.bound[t >> 5] = bound;
+        __syncthreads();
+        for (int w = 0; w < THREADS / 32; w++) bound = max(bound, sh.bound[w]);
+    } else {
+        __syncwarp();
+    }
+    bool open = false;   // no bound: all that is not closed
+    if (bound == kClosed) {   // too few threads have something open, or the picks are more than a warp's lanes
+        int round = 0;
+        const auto reach = [&](int bound) {   // how many keys are at least the bound
+            int n = 0;
+            for (int j = t; j < held; j += THREADS) n += keys[j] >= bound;
+            n = __reduce_add_sync(~0u, n);
+            if (THREADS == 32) return n;
+            if (lane == 0 && n) atomicAdd(&sh.count[round], n);
+            if (t == 0) sh.count[round == 2 ? 0 : round + 1] = 0;
+            __syncthreads();
+            n = sh.count[round];
+            round = round == 2 ? 0 : round + 1;
+            return n;
+        };
+        bound = kClosed + 1;
+        if (reach(bound) < p.width) {
+            open = true;
+        } else {
+            int hi = order(INFINITY);
+            while (bound < hi) {
+                const int mid = bound + (int)(((unsigned)hi - (unsigned)bound + 1u) / 2u);
+                const int n = reach(mid);
+                if (n < p.width) {
+                    hi = mid - 1;
+                } else {
+                    bound = mid;
+                    if (n <= p.width + p.width / 4) break;
+                }
+            }
+        }
+    }
+    open |= unorder(bound) < -1e38f;   // beyond what keys tell apart
+    double least;
+    float least_f;
+    int least_key;
+    const auto set_bound = [&] {
+        const float f = unorder(bound), slack = 0x1p-22f * (far + fabsf(f)) + (float)kNear * 1.01f;
+        least = open ? -INFINITY : f == INFINITY ? INFINITY : (double)f - (double)slack;
+        least_f = open ? -3.402823466e38f : f == INFINITY ? INFINITY : __double2float_rd(least - (double)slack);
+        least_key = open ? kClosed + 1 : order(least_f);
+    };
+    set_bound();
+
+    // the segments that reach it, and their entries that do
+    const auto push = [&](double value, uint32_t at) {
+        const int i = atomicAdd(&sh.candidates, 1);
+        if (i < kRoom<THREADS>) sh.value[i] = value, sh.at[i] = at;
+    };
+    if (mine >= least_key)
+        for (int j = t; j < segments; j += THREADS) {
+            int k = keys[fits ? j : j & (kKeys - 1)];
+            if (k < least_key) continue;
+            const int b = (int)((unsigned)j / (unsigned)row_segments);
+            if (!fits && (k = order(worth_of(tops[j], sh.about[b]))) < least_key) continue;
+            if (sh.beams[b].done) {
+                push(sh.beams[b].score, (uint32_t)b * (uint32_t)p.vocab + (uint32_t)p.end);
+            } else {
+                const int e = atomicAdd(&sh.segments, 1);
+                if (e < kRoom<THREADS>) sh.list[e] = make_uint2(j, k);
+            }
+        }
+    sync<THREADS>();
+    const int listed = sh.segments;
+    if (listed > kRoom<THREADS>) {
+        pick_slowly<T, THREADS>(p, prompt, t, sh);
+        return;
+    }
+    // the bound came from one warp's lanes: the listed segments give a better one, which each warp finds by itself
+    if (!open && listed <= 128 && listed > p.width + p.width / 2) {
+        int k[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) k[i] = i * 32 + lane < listed ? (int)sh.list[i * 32 + lane].y : kClosed;
+        int lo = bound, hi = __reduce_max_sync(~0u, max(max(k[0], k[1]), max(k[2], k[3])));
+        while (lo < hi) {
+            const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) n += __popc(__ballot_sync(~0u, k[i] >= mid));
+            if (n < p.width) {
+                hi = mid - 1;
+            } else {
+                lo = mid;
+                if (n <= p.width + p.width / 4) break;
+            }
+        }
+        if (lo > bound) {
+            bound = lo;
+            set_bound();
+        }
+    }
+    for (int item = t; item < listed << per_log; item += THREADS) {
+        const uint2 e = sh.list[item >> per_log];
+        if ((int)e.y < least_key) continue;
+        const uint32_t b = e.x / (unsigned)row_segments, seg = e.x - b * row_segments;
+        const int i = item & ((1 << per_log) - 1);
+        const T *x = row_of<T>(p, prompt, b);
+        const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab, u = (((seg >> 5) << per_log) + i) * (32 * N) + (seg & 31) * N;
+        if (u >= end) continue;
+        float v[N];
+        unpack(load_run<T, true>(x - off, u, off, end, 0), v, T());
+        const float about = sh.about[b];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            if (!(v[k] + about >= least_f) && !open) continue;
+            const double w = worth(sh.beams[b], v[k], 0, -1);
+            if (open ? w > -INFINITY : w >= least) push(w, b * (uint32_t)p.vocab + (u + k - off));
+        }
     }
     sync<THREADS>();
-    choose<T, THREADS>(p, prompt, t, tops, sums, (int *)tops, VECS, teams[team]);
+    const int n = sh.candidates;
+    if (n > kRoom<THREADS>) {
+        pick_slowly<T, THREADS>(p, prompt, t, sh);
+        return;
+    }
+
+    order_and_write<T, THREADS>(p, prompt, t, n, sh);
+}
+
+// ------------------------------------------------------------------------------------------------ a warp a prompt
+//
+// Many prompts of short rows (16 beams, 2048 entries of 16 bits at most): a warp takes a prompt, and what it costs is instructions. So
+// lanes collect segments and candidates by ballots, and up to 32 candidates are ranked a lane each.
+
+__device__ __forceinline__ float warp_max(float v) {   // NaN left out
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_kernel(const Select p, bool whole) {
+    constexpr int N = kPer<T>;
+    extern __shared__ __align__(16) uint8_t room[];   // for each warp [beams][32] largest entries (then their worth), [beams] sums
+    __shared__ Team<32> teams[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t prompt = (int64_t)blockIdx.x * 8 + warp;
+    if (prompt >= p.prompts) return;
+    Team<32> &sh = teams[warp];
+    float *tops = (float *)(room + warp * p.beams * 136);
+    float2 *sums = (float2 *)(tops + p.beams * 32);
+    const T *first = (const T *)p.logits + prompt * p.prompt_stride;
+    const unsigned done = __ballot_sync(~0u, p.done && lane < p.beams && p.done[prompt * p.beams + lane]);
+    const Pair l = pair(kLog2e, kLog2e);
+    const T *x = first;
+    for (int b = 0; b < p.beams; b++, x += p.beam_stride) {
+        if (done >> b & 1) {
+            tops[b * 32 + lane] = lane ? -INFINITY : 0.0f;
+            continue;
+        }
+        uint4 q[VECS];
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < VECS; i++) q[i] = load_again(x + (i * 32 + lane) * N);
+        } else {
+            const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab;
+#pragma unroll
+            for (int i = 0; i < VECS; i++) q[i] = load_run<T, true>(x - off, i * 32 * N, off, end, lane);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) top = fmaxf(top, largest(q[i], T()));   // NaN left out
+        const float m = warp_max(top), ref = m == -INFINITY ? 0.0f : m;
+        const Pair minus = pair(-ref, -ref);
+        Pair t[2] = {};
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+            for (int k = 0; k < N / 2; k++) t[k & 1] = add(t[k & 1], exp2_approx(mul(add(pair_of(q[i], k, T()), minus), l)));
+        const float2 f = split(add(t[0], t[1]));
+        float s = f.x + f.y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+        tops[b * 32 + lane] = top;
+        if (lane == 0) sums[b] = make_float2(m, s);
+    }
+    __syncwarp();
+    float about = -INFINITY;
+    if (lane < p.beams) {
+        const bool over = done >> lane & 1;
+        const float2 f = over ? make_float2(0.0f, 1.0f) : sums[lane];
+        const Beam beam = beam_of(p, prompt * p.beams + lane, over, f.x, f.y);
+        sh.beams[lane] = beam;
+        about = about_of(beam);
+        sh.about[lane] = about;
+    }
+    const float far = warp_max(fabsf(about) < INFINITY ? fabsf(about) : 0.0f);
+    __syncwarp();
+    float best = -INFINITY;
+    for (int b = 0; b < p.beams; b++) {
+        const float w = worth_of(tops[b * 32 + lane], sh.about[b]);
+        tops[b * 32 + lane] = w;
+        best = fmaxf(best, w);   // NaN is left out
+    }
+    // the W-th largest of the lanes
+    float f = -INFINITY, left = best;
+    if (p.width <= 8) {
+        for (int n = 0;;) {
+            const float m = warp_max(left);
+            if (m == -INFINITY) break;   // too few lanes have something open
+            const unsigned eq = __ballot_sync(~0u, left == m);
+            if ((n += __popc(eq)) >= p.width) {
+                f = m;
+                break;
+            }
+            if (left == m) left = -INFINITY;
+        }
+    } else {
+        f = unorder(bound_of_lanes(order(best), p.width));
+    }
+    const bool open = f < -1e38f;   // no bound: all that is not closed
+    const float slack = 0x1p-22f * (far + fabsf(f)) + (float)kNear * 1.01f;
+    const double least = open ? -INFINITY : f == INFINITY ? INFINITY : (double)f - (double)slack;
+    const float least_f = open ? -3.402823466e38f : f == INFINITY ? INFINITY : f - 2.1f * slack;
+    // the segments that reach it, then their entries that do
+    const unsigned below = (1u << lane) - 1;
+    int listed = 0, n = 0;
+    for (int b = 0; b < p.beams; b++) {
+        const bool take = tops[b * 32 + lane] >= least_f;
+        const unsigned who = __ballot_sync(~0u, take);
+        if (!who) continue;
+        if (done >> b & 1) {
+            if (lane == 0) sh.value[n] = sh.beams[b].score, sh.at[n] = (uint32_t)b * (uint32_t)p.vocab + (uint32_t)p.end;
+            n++;
+            continue;
+        }
+        const int to = listed + __popc(who & below);
+        if (take && to < kRoom<32>) sh.list[to].x = b << 8 | lane;
+        listed += __popc(who);
+    }
+    __syncwarp();
+    if (listed > kRoom<32>) {
+        pick_slowly<T, 32>(p, prompt, lane, sh);
+        return;
+    }
+    for (int turn = 0; turn < listed * VECS; turn += 32) {
+        const int item = turn + lane;
+        float v[N];
+        uint32_t at = 0, mask = 0;
+        int b = 0;
+        if (item < listed * VECS) {
+            const uint32_t e = sh.list[item / VECS].x, u0 = (item % VECS * 32 + (e & 31)) * N;
+            b = e >> 8;
+            const T *x = first + b * p.beam_stride;
+            const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab;
+            at = (uint32_t)b * (uint32_t)p.vocab + u0 - off;
+            const float about = sh.about[b];
+            if (u0 < end) {
+                unpack(load_run<T, true>(x - off, u0, off, end, 0), v, T());
+#pragma unroll
+                for (int k = 0; k < N; k++) mask |= (uint32_t)((open ? worth_of(v[k], about) : v[k] + about) >= least_f) << k;
+            }
+        }
+        while (__any_sync(~0u, mask)) {
+            const int k = __ffs(mask) - 1;
+            float e = v[0];
+#pragma unroll
+            for (int i = 1; i < N; i++) e = k == i ? v[i] : e;
+            const double w = mask ? worth(sh.beams[b], e, 0, -1) : -INFINITY;
+            const bool take = w >= least && w > -INFINITY;
+            const unsigned who = __ballot_sync(~0u, take);
+            const int to = n + __popc(who & below);
+            if (take && to < kRoom<32>) sh.value[to] = w, sh.at[to] = at + k;
+            n += __popc(who);
+            mask &= mask - 1;
+        }
+    }
+    __syncwarp();
+    if (n > kRoom<32>) {
+        pick_slowly<T, 32>(p, prompt, lane, sh);
+        return;
+    }
+    if (n >= p.width && n <= 32 && !p.wide) {
+        double value = -INFINITY;
+        uint32_t at = ~0u;
+        if (lane < n) value = sh.value[lane], at = sh.at[lane];
+        int rank = 0;
+        for (int i = 0; i < n; i++) rank += better(sh.value[i], sh.at[i], value, at);
+        if (lane < n) sh.list[rank].x = lane;
+        __syncwarp();
+        const int own = lane < n ? (int)sh.list[lane].x : 0, before = lane < n ? (int)sh.list[max(min(lane, p.width) - 1, 0)].x : 0;
+        const uint32_t mine = sh.at[own], other = sh.at[before];
+        const int b = (int)(mine / (uint32_t)p.vocab);
+        value = sh.value[own];
+        const bool near = lane && lane < n && sh.value[before] - value < kNear && b != (int)(other / (uint32_t)p.vocab);
+        if (!__any_sync(~0u, near)) {
+            if (lane < p.width) {
+                const int64_t to = prompt * p.width + lane;
+                const bool done = sh.beams[b].done;
+                const int token = done ? p.end : (int)(mine - (uint32_t)b * (uint32_t)p.vocab);
+                ((float *)p.out_scores)[to] = (float)value;
+                p.tokens[to] = token;
+                p.parents[to] = b;
+                if (p.out_done) p.out_done[to] = done || token == p.end;
+            }
+            return;
+        }
+    }
+    if (lane == 0) sh.candidates = n;
+    __syncwarp();
+    order_and_write<T, 32>(p, prompt, lane, n, sh);
+}
+
+// A prompt to a block, in one launch; its warps share its rows' pieces. Dynamic shared memory: [beams][pieces][32] largest entries
+// (then their keys) and [beams][pieces] sums.
+constexpr int kSmallThreads = 256;
+template <typename T, int VECS> __global__ void __launch_bounds__(kSmallThreads) small_kernel(const Select p) {
+    extern __shared__ __align__(16) uint8_t room[];
+    __shared__ Team<kSmallThreads> team;
+    const int lane = threadIdx.x & 31, all = p.beams * p.pieces;
+    const int64_t prompt = blockIdx.x;
+    float *tops = (float *)room;
+    float2 *sums = (float2 *)(tops + all * 32);
+    for (int i = threadIdx.x >> 5; i < all; i += kSmallThreads / 32) {
+        const int b = i / p.pieces;
+        float top = lane || i > b * p.pieces ? -INFINITY : 0.0f;
+        if (!(p.done && p.done[prompt * p.beams + b])) {
+            const float2 s = sum_piece<T, VECS>(row_of<T>(p, prompt, b), p.vocab, i - b * p.pieces, 1, lane, top);
+            if (lane == 0) sums[i] = s;
+        }
+        tops[i * 32 + lane] = top;
+    }
+    __syncthreads();
+    choose<T, kSmallThreads>(p, prompt, threadIdx.x, tops, sums, (int *)tops, VECS == 1 ? 0 : VECS == 2 ? 1 : VECS == 4 ? 2 : 3, team);
 }
 
 // Pieces of rows over the whole GPU, then a block a prompt.
@@ -422,11 +729,14 @@ template <typename T> __global__ void __launch_bounds__(256) pieces_kernel(const
     let_next_begin();
     const int lane = threadIdx.x & 31;
     const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), row = id / p.pieces, prompt = row / p.beams;
-    if (row >= p.prompts * p.beams || (p.done && p.done[row])) return;
-    float top;
-    const float2 s = sum_piece<T, 8>(row_of<T>(p, prompt, (int)(row - prompt * p.beams)), p.vocab, (int)(id - row * p.pieces), p.batches, lane, top);
+    if (row >= p.prompts * p.beams) return;
+    const int piece = (int)(id - row * p.pieces);
+    float top = lane || piece ? -INFINITY : 0.0f;
+    if (!(p.done && p.done[row])) {
+        const float2 s = sum_piece<T, 8>(row_of<T>(p, prompt, (int)(row - prompt * p.beams)), p.vocab, piece, p.batches, lane, top);
+        if (lane == 0) p.sums[id] = s;
+    }
     p.tops[id * 32 + lane] = top;
-    if (lane == 0) p.sums[id] = s;
 }
 constexpr int kChooseThreads = 512;
 template <typename T> __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const Select p) {
@@ -435,12 +745,12 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads) choose_k
     wait_for_previous();
     const int64_t prompt = blockIdx.x, rows = prompt * p.beams;
     choose<T, kChooseThreads>(p, prompt, threadIdx.x, p.tops + rows * p.pieces * 32, p.sums + rows * p.pieces, (int *)room,
-                              8 * p.batches, team);
+                              p.batches == 1 ? 3 : p.batches == 2 ? 4 : 5, team);
 }
 
 // How a call is cut, by its sizes alone (aligned: every row begins on a 16-byte boundary).
 struct Plan {
-    int vecs, pieces, batches, team;   // team: threads of small_kernel's, or 0: two launches
+    int vecs, pieces, batches, team;   // team: a warp's (warp_kernel) or a block's (small_kernel) threads, or 0: two launches
 };
 constexpr int kSms = 148;
 Plan plan_of(int size, bool aligned, int64_t prompts, int beams, int vocab, int width) {
@@ -450,8 +760,8 @@ Plan plan_of(int size, bool aligned, int64_t prompts, int beams, int vocab, int 
     Plan r{lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : 8, 1, 1, 0};
     r.pieces = (lanes + r.vecs - 1) / r.vecs;
     const int all = beams * std::min(r.pieces, 1 << 20);
-    if (all <= 16 && width <= 16 && prompts >= 4 * kSms) r.team = 32;
-    else if (all <= 16 || (all <= 64 && prompts >= kSms)) r.team = 256;
+    if (r.pieces == 1 && beams <= 16 && width <= 16 && prompts >= 4 * kSms) r.team = 32;
+    else if (all <= 16 || (all <= 64 && prompts >= kSms)) r.team = kSmallThreads;
     if (r.team) return r;
     r.vecs = 8;
     const int whole = (lanes + 7) / 8;
@@ -461,24 +771,25 @@ Plan plan_of(int size, bool aligned, int64_t prompts, int beams, int vocab, int 
 }
 size_t room_of(const Plan &r, int64_t rows) { return r.team ? 0 : (size_t)rows * r.pieces * 136; }
 
-template <typename T, int VECS, int THREADS> cudaError_t launch_small(const Select &p, cudaStream_t st) {
-    static SmemLimits limits;
-    const size_t smem = (size_t)(256 / THREADS) * p.beams * p.pieces * 136;
-    const cudaError_t e = raise_smem_limit((const void *)small_kernel<T, VECS, THREADS>, smem, limits);
+template <typename T, int VECS> cudaError_t launch_team(const Select &p, int team, bool aligned, cudaStream_t st) {
+    static SmemLimits warp_limits, limits;
+    const size_t each = (size_t)p.beams * p.pieces * 136, smem = team == 32 ? 8 * each : each;
+    const cudaError_t e = team == 32 ? raise_smem_limit((const void *)warp_kernel<T, VECS>, smem, warp_limits)
+                                     : raise_smem_limit((const void *)small_kernel<T, VECS>, smem, limits);
     if (e != cudaSuccess) return e;
-    small_kernel<T, VECS, THREADS><<<(unsigned)((p.prompts + 256 / THREADS - 1) / (256 / THREADS)), 256, smem, st>>>(p);
+    if (team == 32) warp_kernel<T, VECS><<<(unsigned)((p.prompts + 7) / 8), 256, smem, st>>>(p, aligned && p.vocab == VECS * 32 * kPer<T>);
+    else small_kernel<T, VECS><<<(unsigned)p.prompts, kSmallThreads, smem, st>>>(p);
     return cudaGetLastError();
-}
-template <typename T, int VECS> cudaError_t launch_team(const Select &p, int team, cudaStream_t st) {
-    return team == 32 ? launch_small<T, VECS, 32>(p, st) : launch_small<T, VECS, 256>(p, st);
 }
 template <typename T> cudaError_t launch_select(Select p, bool aligned, void *room, cudaStream_t st) {
     const Plan r = plan_of(sizeof(T), aligned, p.prompts, p.beams, p.vocab, p.width);
     p.pieces = r.pieces;
     p.batches = r.batches;
     if (r.team)
-        return r.vecs == 1 ? launch_team<T, 1>(p, r.team, st) : r.vecs == 2 ? launch_team<T, 2>(p, r.team, st)
-               : r.vecs == 4 ? launch_team<T, 4>(p, r.team, st) : launch_team<T, 8>(p, r.team, st);
+        return r.vecs == 1   ? launch_team<T, 1>(p, r.team, aligned, st)
+               : r.vecs == 2 ? launch_team<T, 2>(p, r.team, aligned, st)
+               : r.vecs == 4 ? launch_team<T, 4>(p, r.team, aligned, st)
+                             : launch_team<T, 8>(p, r.team, aligned, st);
     const int64_t pieces = p.prompts * p.beams * p.pieces;
     p.tops = (float *)room;
     p.sums = (float2 *)(p.tops + pieces * 32);
