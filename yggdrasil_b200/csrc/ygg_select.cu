@@ -41,9 +41,9 @@ struct Select {
 };
 
 // Twice what an lse is off, at most: a term by 2^-22 of exp2 and 2^-23 |y| of its argument (y = x - m, rounded, times log2 e,
-// rounded; weighted by e^y at most log V, 12: 1.4e-6); a chain of 8 + 3 + 4 + 5 + 6 additions by 2^-24 each (1.6e-6); four new references by
-// 2^-22 and their argument (1.6e-6); log2 by 2^-22.
-constexpr double kNear = 1.2e-5;
+// rounded; weighted by e^y at most log V, 12: 1.4e-6); a chain of 8 + 3 + 8 + 5 + 6 additions by 2^-24 each (1.8e-6); eight new references by
+// 2^-22 each (1.9e-6); the join of the pieces by 2^-22, log2 by 2^-22.
+constexpr double kNear = 1.3e-5;
 
 // What a beam's continuations are worth: score + (x - lse). m: the row's largest entry.
 struct Beam {
@@ -76,43 +76,86 @@ __device__ __forceinline__ void write_pick(const Select &p, int64_t prompt, int 
 
 // ---------------------------------------------------------------------------------------------------- pieces of rows
 
+__device__ __forceinline__ float warp_max(float v) {   // NaN left out
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Running sums of a warp: m the largest entry so far (the same in every lane), s the lane's sum of e^(x - m), top its largest entry.
+struct Running { float m, s, top; };
+
+template <typename T, int VECS> __device__ __forceinline__ void add_vectors(Running &a, const uint4 (&q)[VECS]) {
+    constexpr int N = kPer<T>;
+    const Pair l = pair(kLog2e, kLog2e);
+    float mine = largest(q[0], T());
+#pragma unroll
+    for (int r = 1; r < VECS; r++) mine = fmaxf(mine, largest(q[r], T()));
+    a.top = fmaxf(a.top, mine);   // (NaN left out)
+    const float most = warp_max(mine);
+    if (most > a.m) {
+        a.s *= a.m == -INFINITY ? 0.0f : exp2_approx((a.m - most) * kLog2e);
+        a.m = most;
+    }
+    const float ref = a.m == -INFINITY ? 0.0f : a.m;
+    const Pair minus = pair(-ref, -ref);
+    Pair s[4] = {};
+#pragma unroll
+    for (int r = 0; r < VECS; r++)
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) s[(r * N / 2 + i) & 3] = add(s[(r * N / 2 + i) & 3], exp2_approx(mul(add(pair_of(q[r], i, T()), minus), l)));
+    const float2 f = split(add(add(s[0], s[1]), add(s[2], s[3])));
+    a.s += f.x + f.y;
+}
+__device__ __forceinline__ float2 sums_of(Running a) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) a.s += __shfl_xor_sync(~0u, a.s, d);
+    return make_float2(a.m, a.s);
+}
+
 // A warp's piece of a row: m and the sum of e^(x - m) over it (the same in every lane), and the largest entry of the lane's own.
 template <typename T, int VECS>
-__device__ __forceinline__ float2 sum_piece(const T *x, int vocab, int piece, int batches, int lane, float &top) {
+__device__ __forceinline__ float2 sum_piece(const T *x, int vocab, int piece, int lane, float &top) {
     constexpr int N = kPer<T>;
     const uint32_t off = offset_of(x), end = off + (uint32_t)vocab;
+    uint4 q[VECS];
+#pragma unroll
+    for (int r = 0; r < VECS; r++) q[r] = load_run<T, true>(x - off, (piece * VECS + r) * (32 * N), off, end, lane);
+    Running a{-INFINITY, 0.0f, -INFINITY};
+    add_vectors<T>(a, q);
+    top = a.top;
+    return sums_of(a);
+}
+
+// The same of a long row, `turns` times four vectors a lane, the next on their way while it adds.
+template <typename T> __device__ __forceinline__ float2 sum_long(const T *x, int vocab, int piece, int turns, int lane, float &top) {
+    constexpr int N = kPer<T>, kTurn = 4 * 32 * N;
+    const uint32_t off = offset_of(x), end = off + (uint32_t)vocab, u0 = (uint32_t)(piece * turns) * kTurn;
     const T *from = x - off;
-    const Pair l = pair(kLog2e, kLog2e);
-    float m = -INFINITY, sum = 0.0f;
-    top = -INFINITY;
-    for (int b = 0; b < batches; b++) {
-        const uint32_t u0 = (uint32_t)(piece * batches + b) * (VECS * 32 * N);
-        if (u0 >= end) break;
-        uint4 q[VECS];
-        float mine = -INFINITY;
+    const int last = min(turns, (int)((end - u0 + kTurn - 1) / kTurn));
+    const auto load = [&](uint4 (&q)[4], int turn) {
+        const uint32_t u = u0 + (uint32_t)turn * kTurn;
+        if (turn >= last) return;
+        if (u >= off && u + kTurn <= end) {
+            const T *at = from + u + lane * N;
 #pragma unroll
-        for (int r = 0; r < VECS; r++) q[r] = load_run<T, true>(from, u0 + r * 32 * N, off, end, lane);
+            for (int r = 0; r < 4; r++) q[r] = load_again(at + r * (32 * N));
+        } else {
 #pragma unroll
-        for (int r = 0; r < VECS; r++) mine = fmaxf(mine, largest(q[r], T()));
-        top = fmaxf(top, mine);
-        const float most = unorder(__reduce_max_sync(~0u, order(mine)));
-        if (most > m) {
-            sum *= m == -INFINITY ? 0.0f : exp2_approx((m - most) * kLog2e);
-            m = most;
+            for (int r = 0; r < 4; r++) q[r] = load_run<T, true>(from, u + r * (32 * N), off, end, lane);
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const Pair minus = pair(-ref, -ref);
-        Pair s[4] = {};
-#pragma unroll
-        for (int r = 0; r < VECS; r++)
-#pragma unroll
-            for (int i = 0; i < N / 2; i++) s[(r * N / 2 + i) & 3] = add(s[(r * N / 2 + i) & 3], exp2_approx(mul(add(pair_of(q[r], i, T()), minus), l)));
-        const float2 f = split(add(add(s[0], s[1]), add(s[2], s[3])));
-        sum += f.x + f.y;
+    };
+    Running a{-INFINITY, 0.0f, -INFINITY};
+    uint4 q[4], next[4];
+    load(q, 0);
+    for (int turn = 0; turn < last; turn += 2) {
+        load(next, turn + 1);
+        add_vectors<T>(a, q);
+        load(q, turn + 2);
+        if (turn + 1 < last) add_vectors<T>(a, next);
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    return make_float2(m, sum);
+    top = a.top;
+    return sums_of(a);
 }
 
 // --------------------------------------------------------------------------------------------------------- the choice
@@ -126,10 +169,10 @@ template <int THREADS> struct Team {
     float about[kBeams<THREADS>];   // score - lse
     double value[kRoom<THREADS>];
     uint32_t at[kRoom<THREADS>];
-    uint2 list[kRoom<THREADS>];     // segments and their keys; then, in x, the candidates' order
+    uint32_t list[kRoom<THREADS>];  // segments; then the candidates' order
     double part[THREADS / 32];
     uint32_t part_at[THREADS / 32];
-    int bound[THREADS / 32], count[3], candidates, segments;
+    int most[THREADS], count[3], candidates, segments;
     unsigned long long near;        // rows whose lse is wanted in 64 bits
 };
 
@@ -209,10 +252,47 @@ template <typename T, int THREADS> __device__ __noinline__ void pick_slowly(cons
     }
 }
 
+// Up to 32 candidates, as many as are picked at least, by one warp; false where some are too near to each other.
+template <int THREADS> __device__ __forceinline__ bool write_few(const Select &p, int64_t prompt, int lane, int n, Team<THREADS> &sh) {
+    double value = -INFINITY;
+    uint32_t at = ~0u;
+    if (lane < n) value = sh.value[lane], at = sh.at[lane];
+    int rank = 0;
+    for (int i = 0; i < n; i++) rank += better(sh.value[i], sh.at[i], value, at);
+    if (lane < n) sh.list[rank] = lane;
+    __syncwarp();
+    const int own = lane < n ? (int)sh.list[lane] : 0, before = lane < n ? (int)sh.list[max(min(lane, p.width) - 1, 0)] : 0;
+    const uint32_t mine = sh.at[own], other = sh.at[before];
+    const int b = (int)(mine / (uint32_t)p.vocab);
+    value = sh.value[own];
+    const bool near = lane && lane < n && sh.value[before] - value < kNear && b != (int)(other / (uint32_t)p.vocab);
+    if (__any_sync(~0u, near)) return false;
+    if (lane < p.width) {
+        const int64_t to = prompt * p.width + lane;
+        const bool done = sh.beams[b].done;
+        const int token = done ? p.end : (int)(mine - (uint32_t)b * (uint32_t)p.vocab);
+        ((float *)p.out_scores)[to] = (float)value;
+        p.tokens[to] = token;
+        p.parents[to] = b;
+        if (p.out_done) p.out_done[to] = done || token == p.end;
+    }
+    return true;
+}
+
 // The candidates' order and the picks.
 template <typename T, int THREADS>
 __device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt, int t, int n, Team<THREADS> &sh) {
     const int lane = t & 31;
+    if (THREADS > 32 && n >= p.width && n <= 32 && !p.wide) {
+        if (t < 32) {
+            const bool ready = write_few<THREADS>(p, prompt, lane, n, sh);
+            if (lane == 0) sh.near = ready;
+        }
+        __syncthreads();
+        const bool ready = sh.near;
+        __syncthreads();
+        if (ready) return;
+    }
     // A few of them are a warp's work, and the others wait for whether rows are wanted in 64 bits.
     const auto rank = [&](int first, int step) {
         for (int c = first; c < n; c += step) {
@@ -221,7 +301,7 @@ __device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt,
             int r = 0;
 #pragma unroll 4
             for (int i = 0; i < n; i++) r += better(sh.value[i], sh.at[i], v, at);
-            sh.list[r].x = c;
+            sh.list[r] = c;
         }
     };
     const bool few = THREADS == 32 || n <= 64;
@@ -231,7 +311,7 @@ __device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt,
     if (t < 32) {
         unsigned long long near = 0;
         for (int r = lane; r < n; r += 32) {   // with the one before, or, past the last pick, with that
-            const int q = max(min(r, p.width) - 1, 0), cq = sh.list[q].x, cr = sh.list[r].x;
+            const int q = max(min(r, p.width) - 1, 0), cq = sh.list[q], cr = sh.list[r];
             const uint32_t a = sh.at[cq] / (uint32_t)p.vocab, b = sh.at[cr] / (uint32_t)p.vocab;
             if (p.wide || (a != b && sh.value[cq] - sh.value[cr] < kNear)) near |= (1ull << a) | (1ull << b);
         }
@@ -239,7 +319,7 @@ __device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt,
         if (THREADS > 32 && t == 0) sh.near = near;
         if (THREADS == 32) sh.near = near;
         if (!near)
-            for (int k = lane; k < min(n, p.width); k += 32) write_pick(p, prompt, k, sh.at[sh.list[k].x], sh.value[sh.list[k].x], sh.beams);
+            for (int k = lane; k < min(n, p.width); k += 32) write_pick(p, prompt, k, sh.at[sh.list[k]], sh.value[sh.list[k]], sh.beams);
     }
     sync<THREADS>();
     const unsigned long long near = sh.near;
@@ -252,7 +332,7 @@ __device__ __forceinline__ void order_and_write(const Select &p, int64_t prompt,
         sync<THREADS>();
         rank(t, THREADS);
         sync<THREADS>();
-        for (int k = t; k < min(n, p.width); k += THREADS) write_pick(p, prompt, k, sh.at[sh.list[k].x], sh.value[sh.list[k].x], sh.beams);
+        for (int k = t; k < min(n, p.width); k += THREADS) write_pick(p, prompt, k, sh.at[sh.list[k]], sh.value[sh.list[k]], sh.beams);
     }
     if (n >= p.width || t >= 32) return;
     // fewer are open than are wanted: closed ones in their order
@@ -295,20 +375,31 @@ __device__ __forceinline__ float worth_of(float top, float about) {
     return top == -INFINITY ? top : v == -INFINITY && about > -INFINITY ? -3.402823466e38f : v;
 }
 
-// The largest bound that `width` lanes (at least; a quarter more at most, where the search finds one) reach; kClosed if there is none.
-__device__ __forceinline__ int bound_of_lanes(int mine, int width) {
-    const int most = __reduce_max_sync(~0u, mine);
-    if (width > 32 || __popc(__ballot_sync(~0u, mine > kClosed)) < width) return kClosed;
-    int lo = __reduce_min_sync(~0u, mine), hi = most;   // lo: all lanes reach it, or it is kClosed
-    lo = max(lo, kClosed + 1);
-    const int guess = order(unorder(most) - 32.0f);
+// The largest bound that `width` of a warp's K values a lane reach (at least; a quarter more at most, where the search finds one);
+// kClosed if there is none.
+template <int K> __device__ __forceinline__ int bound_of(const int (&v)[K], int width) {
+    const auto reach = [&](int bound) {
+        [[maybe_unused]] int n = 0;
+        if constexpr (K == 1) {
+            return __popc(__ballot_sync(~0u, v[0] >= bound));
+        } else {
+#pragma unroll
+            for (int i = 0; i < K; i++) n += v[i] >= bound;
+            return (int)__reduce_add_sync(~0u, n);
+        }
+    };
+    int hi = v[0], lo = kClosed + 1;
+#pragma unroll
+    for (int i = 1; i < K; i++) hi = max(hi, v[i]);
+    hi = __reduce_max_sync(~0u, hi);
+    if (reach(lo) < width) return kClosed;
+    const int guess = order(unorder(hi) - 16.0f);
     if (guess > lo && guess < hi) {
-        if (__popc(__ballot_sync(~0u, mine >= guess)) >= width) lo = guess;
+        if (reach(guess) >= width) lo = guess;
         else hi = guess - 1;
     }
     while (lo < hi) {
-        const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
-        const int n = __popc(__ballot_sync(~0u, mine >= mid));
+        const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u), n = reach(mid);
         if (n < width) {
             hi = mid - 1;
         } else {
@@ -328,7 +419,7 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
     const int lane = t & 31, row_segments = p.pieces * 32, segments = p.beams * row_segments;
     const bool fits = segments <= kKeys;
     // each row's lse: a thread a row, or a warp where a row has more pieces
-    if (THREADS == 32 || p.pieces <= 4) {
+    if (p.pieces <= 4) {
         if (t < p.beams) {
             const int64_t row = prompt * p.beams + t;
             const bool done = p.done && p.done[row];
@@ -367,7 +458,7 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
         }
     }
     if (t == 0) sh.candidates = sh.segments = 0, sh.count[0] = sh.count[1] = sh.count[2] = 0, sh.near = 0;
-    sync<THREADS>();
+    __syncthreads();
 
     // A bound that at least `width` segments reach, in floats: a segment's key is its largest entry's worth, off by two roundings.
     int mine = kClosed;
@@ -391,22 +482,19 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
         }
     }
     const int held = min(segments, kKeys);
-    int bound = bound_of_lanes(mine, p.width);
-    if (THREADS > 32) {
-        if (lane == 0) sh.bound[t >> 5] = bound;
-        __syncthreads();
-        for (int w = 0; w < THREADS / 32; w++) bound = max(bound, sh.bound[w]);
-    } else {
-        __syncwarp();
-    }
+    sh.most[t] = mine;
+    __syncthreads();
+    int each[THREADS / 32];
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; i++) each[i] = sh.most[i * 32 + lane];
+    int bound = bound_of(each, p.width);   // each warp by itself
     bool open = false;   // no bound: all that is not closed
-    if (bound == kClosed) {   // too few threads have something open, or the picks are more than a warp's lanes
+    if (bound == kClosed) {   // too few threads have something open
         int round = 0;
         const auto reach = [&](int bound) {   // how many keys are at least the bound
             int n = 0;
             for (int j = t; j < held; j += THREADS) n += keys[j] >= bound;
             n = __reduce_add_sync(~0u, n);
-            if (THREADS == 32) return n;
             if (lane == 0 && n) atomicAdd(&sh.count[round], n);
             if (t == 0) sh.count[round == 2 ? 0 : round + 1] = 0;
             __syncthreads();
@@ -432,16 +520,10 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
         }
     }
     open |= unorder(bound) < -1e38f;   // beyond what keys tell apart
-    double least;
-    float least_f;
-    int least_key;
-    const auto set_bound = [&] {
-        const float f = unorder(bound), slack = 0x1p-22f * (far + fabsf(f)) + (float)kNear * 1.01f;
-        least = open ? -INFINITY : f == INFINITY ? INFINITY : (double)f - (double)slack;
-        least_f = open ? -3.402823466e38f : f == INFINITY ? INFINITY : __double2float_rd(least - (double)slack);
-        least_key = open ? kClosed + 1 : order(least_f);
-    };
-    set_bound();
+    const float f = unorder(bound), slack = 0x1p-22f * (far + fabsf(f)) + (float)kNear * 1.01f;
+    const double least = open ? -INFINITY : f == INFINITY ? INFINITY : (double)f - (double)slack;
+    const float least_f = open ? -3.402823466e38f : f == INFINITY ? INFINITY : f - 2.1f * slack;
+    const int least_key = open ? kClosed + 1 : order(least_f);
 
     // the segments that reach it, and their entries that do
     const auto push = [&](double value, uint32_t at) {
@@ -458,42 +540,18 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
                 push(sh.beams[b].score, (uint32_t)b * (uint32_t)p.vocab + (uint32_t)p.end);
             } else {
                 const int e = atomicAdd(&sh.segments, 1);
-                if (e < kRoom<THREADS>) sh.list[e] = make_uint2(j, k);
+                if (e < kRoom<THREADS>) sh.list[e] = j;
             }
         }
-    sync<THREADS>();
+    __syncthreads();
     const int listed = sh.segments;
     if (listed > kRoom<THREADS>) {
         pick_slowly<T, THREADS>(p, prompt, t, sh);
         return;
     }
-    // the bound came from one warp's lanes: the listed segments give a better one, which each warp finds by itself
-    if (!open && listed <= 128 && listed > p.width + p.width / 2) {
-        int k[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) k[i] = i * 32 + lane < listed ? (int)sh.list[i * 32 + lane].y : kClosed;
-        int lo = bound, hi = __reduce_max_sync(~0u, max(max(k[0], k[1]), max(k[2], k[3])));
-        while (lo < hi) {
-            const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) n += __popc(__ballot_sync(~0u, k[i] >= mid));
-            if (n < p.width) {
-                hi = mid - 1;
-            } else {
-                lo = mid;
-                if (n <= p.width + p.width / 4) break;
-            }
-        }
-        if (lo > bound) {
-            bound = lo;
-            set_bound();
-        }
-    }
     for (int item = t; item < listed << per_log; item += THREADS) {
-        const uint2 e = sh.list[item >> per_log];
-        if ((int)e.y < least_key) continue;
-        const uint32_t b = e.x / (unsigned)row_segments, seg = e.x - b * row_segments;
+        const uint32_t e = sh.list[item >> per_log];
+        const uint32_t b = e / (unsigned)row_segments, seg = e - b * row_segments;
         const int i = item & ((1 << per_log) - 1);
         const T *x = row_of<T>(p, prompt, b);
         const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab, u = (((seg >> 5) << per_log) + i) * (32 * N) + (seg & 31) * N;
@@ -501,14 +559,19 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
         float v[N];
         unpack(load_run<T, true>(x - off, u, off, end, 0), v, T());
         const float about = sh.about[b];
+        uint32_t mask = 0;
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            if (!(v[k] + about >= least_f) && !open) continue;
-            const double w = worth(sh.beams[b], v[k], 0, -1);
-            if (open ? w > -INFINITY : w >= least) push(w, b * (uint32_t)p.vocab + (u + k - off));
+        for (int k = 0; k < N; k++) mask |= (uint32_t)((open ? worth_of(v[k], about) : v[k] + about) >= least_f) << k;
+        for (; mask; mask &= mask - 1) {
+            const int k = __ffs(mask) - 1;
+            float e = v[0];
+#pragma unroll
+            for (int i = 1; i < N; i++) e = k == i ? v[i] : e;
+            const double w = worth(sh.beams[b], e, 0, -1);
+            if (w >= least && w > -INFINITY) push(w, b * (uint32_t)p.vocab + (u + k - off));
         }
     }
-    sync<THREADS>();
+    __syncthreads();
     const int n = sh.candidates;
     if (n > kRoom<THREADS>) {
         pick_slowly<T, THREADS>(p, prompt, t, sh);
@@ -522,12 +585,6 @@ __device__ __forceinline__ void choose(const Select &p, int64_t prompt, int t, c
 //
 // Many prompts of short rows (16 beams, 2048 entries of 16 bits at most): a warp takes a prompt, and what it costs is instructions. So
 // lanes collect segments and candidates by ballots, and up to 32 candidates are ranked a lane each.
-
-__device__ __forceinline__ float warp_max(float v) {   // NaN left out
-    float r;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
 
 template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_kernel(const Select p, bool whole) {
     constexpr int N = kPer<T>;
@@ -606,7 +663,8 @@ template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_k
             if (left == m) left = -INFINITY;
         }
     } else {
-        f = unorder(bound_of_lanes(order(best), p.width));
+        const int only[1] = {order(best)};
+        f = unorder(bound_of(only, p.width));
     }
     const bool open = f < -1e38f;   // no bound: all that is not closed
     const float slack = 0x1p-22f * (far + fabsf(f)) + (float)kNear * 1.01f;
@@ -625,7 +683,7 @@ template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_k
             continue;
         }
         const int to = listed + __popc(who & below);
-        if (take && to < kRoom<32>) sh.list[to].x = b << 8 | lane;
+        if (take && to < kRoom<32>) sh.list[to] = b << 8 | lane;
         listed += __popc(who);
     }
     __syncwarp();
@@ -639,7 +697,7 @@ template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_k
         uint32_t at = 0, mask = 0;
         int b = 0;
         if (item < listed * VECS) {
-            const uint32_t e = sh.list[item / VECS].x, u0 = (item % VECS * 32 + (e & 31)) * N;
+            const uint32_t e = sh.list[item / VECS], u0 = (item % VECS * 32 + (e & 31)) * N;
             b = e >> 8;
             const T *x = first + b * p.beam_stride;
             const uint32_t off = offset_of(x), end = off + (uint32_t)p.vocab;
@@ -670,32 +728,7 @@ template <typename T, int VECS> __global__ void __launch_bounds__(256, 4) warp_k
         pick_slowly<T, 32>(p, prompt, lane, sh);
         return;
     }
-    if (n >= p.width && n <= 32 && !p.wide) {
-        double value = -INFINITY;
-        uint32_t at = ~0u;
-        if (lane < n) value = sh.value[lane], at = sh.at[lane];
-        int rank = 0;
-        for (int i = 0; i < n; i++) rank += better(sh.value[i], sh.at[i], value, at);
-        if (lane < n) sh.list[rank].x = lane;
-        __syncwarp();
-        const int own = lane < n ? (int)sh.list[lane].x : 0, before = lane < n ? (int)sh.list[max(min(lane, p.width) - 1, 0)].x : 0;
-        const uint32_t mine = sh.at[own], other = sh.at[before];
-        const int b = (int)(mine / (uint32_t)p.vocab);
-        value = sh.value[own];
-        const bool near = lane && lane < n && sh.value[before] - value < kNear && b != (int)(other / (uint32_t)p.vocab);
-        if (!__any_sync(~0u, near)) {
-            if (lane < p.width) {
-                const int64_t to = prompt * p.width + lane;
-                const bool done = sh.beams[b].done;
-                const int token = done ? p.end : (int)(mine - (uint32_t)b * (uint32_t)p.vocab);
-                ((float *)p.out_scores)[to] = (float)value;
-                p.tokens[to] = token;
-                p.parents[to] = b;
-                if (p.out_done) p.out_done[to] = done || token == p.end;
-            }
-            return;
-        }
-    }
+    if (n >= p.width && n <= 32 && !p.wide && write_few<32>(p, prompt, lane, n, sh)) return;
     if (lane == 0) sh.candidates = n;
     __syncwarp();
     order_and_write<T, 32>(p, prompt, lane, n, sh);
@@ -715,7 +748,7 @@ template <typename T, int VECS> __global__ void __launch_bounds__(kSmallThreads)
         const int b = i / p.pieces;
         float top = lane || i > b * p.pieces ? -INFINITY : 0.0f;
         if (!(p.done && p.done[prompt * p.beams + b])) {
-            const float2 s = sum_piece<T, VECS>(row_of<T>(p, prompt, b), p.vocab, i - b * p.pieces, 1, lane, top);
+            const float2 s = sum_piece<T, VECS>(row_of<T>(p, prompt, b), p.vocab, i - b * p.pieces, lane, top);
             if (lane == 0) sums[i] = s;
         }
         tops[i * 32 + lane] = top;
@@ -733,7 +766,7 @@ template <typename T> __global__ void __launch_bounds__(256) pieces_kernel(const
     const int piece = (int)(id - row * p.pieces);
     float top = lane || piece ? -INFINITY : 0.0f;
     if (!(p.done && p.done[row])) {
-        const float2 s = sum_piece<T, 8>(row_of<T>(p, prompt, (int)(row - prompt * p.beams)), p.vocab, piece, p.batches, lane, top);
+        const float2 s = sum_long<T>(row_of<T>(p, prompt, (int)(row - prompt * p.beams)), p.vocab, piece, 2 * p.batches, lane, top);
         if (lane == 0) p.sums[id] = s;
     }
     p.tops[id * 32 + lane] = top;
