@@ -83,7 +83,7 @@ def check_gradients(grads, types, x, w, b, g, eps):
 
 SIZES = [(1, 1), (1, 2), (3, 5), (2, 31), (5, 32), (4, 33), (7, 100), (1, 1280), (33, 256), (65, 255), (9, 1000), (130, 1024), (17, 1025),
          (3, 4096), (200, 2048), (5, 4099), (2, 8192), (3, 12000), (1, 16384), (2, 20001), (1, 100003), (1003, 96), (4097, 8), (600, 513),
-         (20000, 3), (300, 4096)]
+         (20000, 3), (300, 4096), (700, 4095), (3000, 505), (2500, 1002), (400, 8189), (40, 16379)]
 
 
 @pytest.mark.gpu
@@ -184,24 +184,23 @@ def test_strides_shapes_and_no_rows(dim, dtype):
     x, w, b, g = make(6, dim, dtype, seed=5)
     want = f(x, w, b)
     leaf = x.clone().requires_grad_()
-    want_dx, = torch.autograd.grad(f(leaf, w, b), leaf, g)
     wide = torch.full((6, dim + 20), math.nan, dtype=dtype, device="cuda")
     for off in (0, 1, 3, 8):
         part = wide[:, off:off + dim]
         part.copy_(x)
-        assert torch.equal(f(part, w, b), want)
-        part = part.detach().requires_grad_()
-        arriving = torch.zeros(6, dim + 9, dtype=dtype, device="cuda")[:, off:off + dim].copy_(g)
-        got, = torch.autograd.grad(f(part, w, b), part, arriving)
-        assert torch.equal(got, want_dx)
+        check_values(f(part, w, b), x, w, b, 1e-5)   # (where rows begin, sums may take another order)
+        leaves = [part.detach().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+        for arriving in (g, torch.full((6, dim + 9), math.nan, dtype=dtype, device="cuda")[:, off:off + dim].copy_(g)):
+            grads = torch.autograd.grad(f(*leaves), leaves, arriving)
+            check_gradients(grads, (dtype, torch.float32, torch.float32), x, w, b, g, 1e-5)
     assert torch.equal(f(x.T.contiguous().T, w, b), want)
     assert torch.equal(f(x.view(2, 3, dim), w, b), want.view(2, 3, dim))
-    assert torch.equal(f(x.view(2, 3, dim).transpose(0, 1), w, b), want.view(2, 3, dim).transpose(0, 1))
+    check_values(f(x.view(2, 3, dim).transpose(0, 1), w, b).transpose(0, 1), x.view(2, 3, dim), w, b, 1e-5)
     assert torch.equal(f(x[0], w, b), want[0])
     assert torch.equal(f(x, torch.stack([w, w], 1)[:, 0], b), want)
     turned = leaf.view(2, 3, dim).transpose(0, 1)
     got, = torch.autograd.grad(f(turned, w, b).transpose(0, 1), leaf, g.view(2, 3, dim))
-    assert torch.equal(got, want_dx)
+    check_gradients((got,), (dtype,), x, w, b, g, 1e-5)
     one = x.clone().requires_grad_()
     a, = torch.autograd.grad(f(one, w, b).sum(), one)   # an expanded gradient arrives
     one = x.clone().requires_grad_()
@@ -213,7 +212,7 @@ def test_strides_shapes_and_no_rows(dim, dtype):
     dx, dw = torch.autograd.grad(y, [none, weight], g[:0])
     assert y.shape == dx.shape == (0, dim) and not dw.any()
     same = x[:1].expand(6, dim)
-    assert torch.equal(f(same, w, b), want[:1].expand(6, dim))
+    check_values(f(same, w, b), same, w, b, 1e-5)
 
 
 @pytest.mark.gpu

@@ -5,12 +5,23 @@
 //   dx = r (g w - sum(g w) / D - h sum(g w h) / D),   dw = sum over rows of g h,   db = sum over rows of g.
 // All sums are held in 32 bits; the variance is that of the differences, so that a large mean does not cancel it. The sums
 // over rows are cut by the number of rows and columns alone and joined in one order: results repeat bit for bit.
+//
+// Both passes are bound by HBM where what they do around a row's entries (addresses, sums over warps) is shared by many entries of a thread. A team
+// of 32 to 1024 threads takes a row, in units of 16 bytes as they lie in memory, and goes from row to row with the next ones on their way: in
+// registers in the forward pass, in shared memory in the backward pass (cp.async; a thread reads what it copied), where the sums over rows
+// stay in a thread's registers until the end, so that x and g are read once for all three gradients. Rows of a length that is no multiple of 16
+// bytes begin anywhere: a team then takes rows that begin at one place in their first unit, so that a thread's columns stay the same. (Rows that
+// lie differently in x and its gradients are taken entry by entry.)
 #include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
 
 #include "ygg_ops.cuh"
+#include "ygg_rows.cuh"
+#include "ygg_smem.h"
 
 namespace {
 
@@ -36,6 +47,7 @@ struct NormGrad {
     Affine weight;
     const float2 *stats;
     void *dx;            // rows dim entries apart, or null
+    float *dw, *db;      // [blocks][dim] sums over rows, each may be null
 };
 struct Columns {
     const void *x, *g;
@@ -51,6 +63,351 @@ __device__ __forceinline__ float at(const Affine &a, int i, float none) {
     if (a.dtype == YGG_DTYPE_HALF) return __half2float(((const __half *)a.v)[i]);
     return __bfloat162float(((const __nv_bfloat16 *)a.v)[i]);
 }
+__device__ __forceinline__ int own_type(float) { return YGG_DTYPE_FLOAT; }
+__device__ __forceinline__ int own_type(__half) { return YGG_DTYPE_HALF; }
+__device__ __forceinline__ int own_type(__nv_bfloat16) { return YGG_DTYPE_BFLOAT; }
+
+// How a row is taken: in units of 16 bytes that all rows leave whole, in those of memory, or entry by entry.
+enum Mode { kWhole, kShifted, kSingle };
+
+// A thread's places in its team's rows: `kPer` entries of its k-th unit.
+template <typename T, Mode M, int TEAM> struct Places {
+    static constexpr int N = kPer<T>;
+    int first, off, dim;   // first: the column of its first unit's first entry (kSingle: of its first entry); off: entries of the row's first unit before it
+    __device__ __forceinline__ Places(int t, const void *row, int dim)
+        : off(M == kShifted ? (int)((uintptr_t)row & 15) / (int)sizeof(T) : 0), dim(dim) {
+        first = M == kSingle ? t : t * N - off;
+    }
+    __device__ __forceinline__ int column(int k, int e) const { return first + (M == kSingle ? (k * N + e) * TEAM : k * TEAM * N + e); }
+    __device__ __forceinline__ bool live(int k) const { return column(k, 0) < dim; }
+    __device__ __forceinline__ bool cut(int k) const { return M != kWhole && ((M == kShifted && k == 0 && first < 0) || column(k, N - 1) >= dim); }
+    __device__ __forceinline__ bool in(int k, int e) const { return (unsigned)column(k, e) < (unsigned)dim; }
+    // A unit of the row whose place `first` is at `row`.
+    __device__ __forceinline__ uint4 load(const T *row, int k) const {
+        if (M != kSingle) return __ldg((const uint4 *)row + k * TEAM);
+        uint4 q = make_uint4(0, 0, 0, 0);
+        T *v = (T *)&q;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (in(k, e)) v[e] = row[(k * N + e) * TEAM];
+        return q;
+    }
+    __device__ __forceinline__ void copy(const T *row, int k, uint4 *to) const {
+        if (M != kSingle)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"((const uint4 *)row + k * TEAM)
+                         : "memory");
+        else *to = load(row, k);
+    }
+    // What lies outside the row as zeros.
+    __device__ __forceinline__ void trim(uint4 &q, int k) const {
+        if (M != kShifted || !cut(k)) return;
+        uint32_t *w = (uint32_t *)&q;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (!in(k, e)) w[e * 4 / N] &= N == 4 ? 0u : 0xFFFFu << (e & 1 ? 0 : 16);
+    }
+    __device__ __forceinline__ void store(T *row, int k, const float (&f)[N]) const {
+        if (M == kSingle || cut(k)) {
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (in(k, e)) from_f(f[e], row[M == kSingle ? (k * N + e) * TEAM : k * TEAM * N + e]);
+        } else {
+            ((uint4 *)row)[k * TEAM] = pack(f, T());
+        }
+    }
+    // A weight or a bias from memory, `none` where it is absent; 0 outside the row. Their usual types are x's and float.
+    __device__ __forceinline__ void affine(const Affine &a, int k, float none, float (&v)[N]) const {
+        if (M == kWhole && a.v && ((uintptr_t)a.v & 15) == 0) {
+            const int i = column(k, 0);
+            if (a.dtype == own_type(T())) {
+                unpack(__ldg((const uint4 *)((const T *)a.v + i)), v, T());
+                return;
+            }
+            if (a.dtype == YGG_DTYPE_FLOAT) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) {
+                    const float4 f = __ldg((const float4 *)((const float *)a.v + i + e));
+                    v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = in(k, e) ? at(a, column(k, e), none) : 0.0f;
+    }
+};
+
+__host__ __device__ constexpr int threads_of(int team) { return team < 256 ? 256 : team; }
+
+// Sums over a team, the same in each thread. Its warps meet in shared memory, in `turn`, which the caller counts: one barrier a sum.
+template <int TEAM, int VALUES> struct TeamSum {
+    alignas(16) float part[2][threads_of(TEAM) / 32 * VALUES];
+    __device__ __forceinline__ void operator()(float (&v)[VALUES], int &turn) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < VALUES; i++) v[i] += __shfl_xor_sync(~0u, v[i], d);
+        if constexpr (TEAM > 32) {
+            constexpr int kAll = TEAM / 32 * VALUES;
+            if ((threadIdx.x & 31) == 0)
+#pragma unroll
+                for (int i = 0; i < VALUES; i++) part[turn][(threadIdx.x >> 5) * VALUES + i] = v[i];
+            if (TEAM < 256) asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / TEAM), "n"(TEAM) : "memory");
+            else __syncthreads();
+#pragma unroll
+            for (int i = 0; i < VALUES; i++) v[i] = 0.0f;
+            const float *from = part[turn] + threadIdx.x / TEAM * kAll;
+            if constexpr (kAll % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < kAll / 4; i++) {
+                    const float4 f = ((const float4 *)from)[i];
+                    v[0] += f.x, v[1 % VALUES] += f.y, v[0] += f.z, v[1 % VALUES] += f.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kAll; i++) v[i % VALUES] += from[i];
+            }
+            turn ^= 1;
+        }
+    }
+};
+
+// UNITS: of 16 bytes a thread. Teams of 1024 threads have no registers for weight and bias: they are read with each row, from shared memory (floats
+// in the order of its units) where rows begin anywhere.
+template <typename T> __host__ __device__ constexpr int norm_blocks(int team, int units) { return units * kPer<T> <= 16 && team <= 256 ? 3 : team <= 512 ? 512 / threads_of(team) : 1; }
+template <typename T, Mode M, int UNITS, int TEAM>
+__global__ void __launch_bounds__(threads_of(TEAM), norm_blocks<T>(TEAM, UNITS)) norm_kernel(const Norm p) {
+    constexpr int N = kPer<T>, kThreads = threads_of(TEAM), kTeams = kThreads / TEAM;
+    __shared__ TeamSum<TEAM, 1> sum;
+    extern __shared__ __align__(16) float4 staged[];   // [unit][w, b][N / 4][threads]
+    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / TEAM;
+    const int64_t step = (int64_t)gridDim.x * kTeams;
+    if (row >= p.rows) return;   // a whole team, before any of its sums
+    const T *x = (const T *)p.x + row * p.stride;
+    const Places<T, M, TEAM> place(threadIdx.x % TEAM, x, p.dim);
+    T *y = (T *)p.y + row * p.dim + place.first;
+    x += place.first;
+    const float over = 1.0f / (float)p.dim;
+    int turn = 0;
+    uint4 next[UNITS];
+#pragma unroll
+    for (int k = 0; k < UNITS; k++)
+        if (place.live(k)) next[k] = place.load(x, k);
+    constexpr bool kKeep = TEAM <= 512;   // weight and bias in registers
+    float4 *own = staged + threadIdx.x;
+    float w[kKeep ? UNITS : 1][N], b[kKeep ? UNITS : 1][N];
+    if (kKeep) {
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                place.affine(p.weight, k, 1.0f, w[k]);
+                place.affine(p.bias, k, 0.0f, b[k]);
+            }
+    } else if (M != kWhole) {
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                place.affine(p.weight, k, 1.0f, w[0]);
+                place.affine(p.bias, k, 0.0f, b[0]);
+#pragma unroll
+                for (int i = 0; i < N / 4; i++) {
+                    own[((2 * k) * (N / 4) + i) * kThreads] = make_float4(w[0][4 * i], w[0][4 * i + 1], w[0][4 * i + 2], w[0][4 * i + 3]);
+                    own[((2 * k + 1) * (N / 4) + i) * kThreads] = make_float4(b[0][4 * i], b[0][4 * i + 1], b[0][4 * i + 2], b[0][4 * i + 3]);
+                }
+            }
+    }
+    for (; row < p.rows; row += step) {
+        float v[UNITS][N], s[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                place.trim(next[k], k);
+                unpack(next[k], v[k], T());
+#pragma unroll
+                for (int e = 0; e < N; e++) s[0] += v[k][e];
+            }
+        x += step * p.stride;
+        if (row + step < p.rows)
+#pragma unroll
+            for (int k = 0; k < UNITS; k++)
+                if (place.live(k)) next[k] = place.load(x, k);
+        sum(s, turn);
+        const float mu = s[0] * over;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k][e] -= mu;
+                if (place.cut(k))
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[k][e] = place.in(k, e) ? v[k][e] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < N; e++) s[0] = fmaf(v[k][e], v[k][e], s[0]);
+            }
+        sum(s, turn);
+        const float r = rsqrtf(s[0] * over + p.eps);   // off by 2^-22 at most
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                float (&wk)[N] = w[kKeep ? k : 0], (&bk)[N] = b[kKeep ? k : 0];
+                if (!kKeep && M == kWhole) {
+                    place.affine(p.weight, k, 1.0f, wk);
+                    place.affine(p.bias, k, 0.0f, bk);
+                } else if (!kKeep) {
+#pragma unroll
+                    for (int i = 0; i < N / 4; i++) {
+                        const float4 a = own[((2 * k) * (N / 4) + i) * kThreads], c = own[((2 * k + 1) * (N / 4) + i) * kThreads];
+                        wk[4 * i] = a.x, wk[4 * i + 1] = a.y, wk[4 * i + 2] = a.z, wk[4 * i + 3] = a.w;
+                        bk[4 * i] = c.x, bk[4 * i + 1] = c.y, bk[4 * i + 2] = c.z, bk[4 * i + 3] = c.w;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k][e] = fmaf(v[k][e] * r, wk[e], bk[e]);
+                place.store(y, k, v[k]);
+            }
+        y += step * p.dim;
+        if (p.stats && threadIdx.x % TEAM == 0) p.stats[row] = make_float2(mu, r);
+    }
+}
+
+// Rows that a team has in shared memory or on their way there: two blocks of 256 threads an SM (three, with 80 registers a thread:
+// 96 us against 85 for 16384 x 4096 bf16).
+template <typename T> constexpr int kStages = sizeof(T) == 4 ? 2 : 3;
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// SUMS: the sums over rows too; each block writes its own.
+__host__ __device__ constexpr int grad_blocks(int team) { return team <= 256 ? 2 : 1; }
+template <typename T, Mode M, int UNITS, bool SUMS, int TEAM>
+__global__ void __launch_bounds__(threads_of(TEAM), grad_blocks(TEAM)) grad_kernel(const NormGrad p) {
+    constexpr int N = kPer<T>, H = UNITS * N, kThreads = threads_of(TEAM), kTeams = kThreads / TEAM, kStage = UNITS * 2 * kThreads, kRing = kStages<T>;
+    extern __shared__ __align__(16) uint4 room[];   // [kRing][UNITS][x, g][threads]; at the end [2][dim] sums, where teams share a block
+    __shared__ TeamSum<TEAM, 2> sum;
+    let_next_begin();
+    const int mine = threadIdx.x / TEAM;
+    int64_t row = (int64_t)blockIdx.x * kTeams + mine;
+    const int64_t step = (int64_t)gridDim.x * kTeams;
+    const T *x_row = (const T *)p.x + row * p.stride, *g_row = (const T *)p.g + row * p.g_stride;
+    const Places<T, M, TEAM> place(threadIdx.x % TEAM, x_row, p.dim);
+    T *dx = (T *)p.dx + row * p.dim + place.first;
+    x_row += place.first;
+    g_row += place.first;
+    const float over = 1.0f / (float)p.dim;
+    int turn = 0;
+    uint4 *own = room + threadIdx.x;
+    int64_t ahead = row;
+    const auto fetch = [&](int at) {
+        if (ahead < p.rows)
+#pragma unroll
+            for (int k = 0; k < UNITS; k++)
+                if (place.live(k)) {
+                    place.copy(x_row, k, own + at + 2 * k * kThreads);
+                    place.copy(g_row, k, own + at + (2 * k + 1) * kThreads);
+                }
+        copies_end();
+        ahead += step;
+        x_row += step * p.stride;
+        g_row += step * p.g_stride;
+    };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; i++) fetch(i * kStage);
+    float2 next = row < p.rows ? p.stats[row] : make_float2(0.0f, 0.0f);
+    float w[SUMS ? H : 1], dw[SUMS ? H : 1], db[SUMS ? H : 1];   // without the sums the weight is read with each row
+    const auto weight = [&](int k, float (&v)[N]) {
+        if constexpr (SUMS) {
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = w[k * N + e];
+        } else {
+            place.affine(p.weight, k, 1.0f, v);
+        }
+    };
+    if constexpr (SUMS) {
+#pragma unroll
+        for (int i = 0; i < H; i++) dw[i] = db[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                float v[N];
+                place.affine(p.weight, k, 1.0f, v);
+#pragma unroll
+                for (int e = 0; e < N; e++) w[k * N + e] = v[e];
+            }
+    }
+    int at = 0, to = (kRing - 1) * kStage;   // the stage that is read, and the one that is filled
+    for (; row < p.rows; row += step) {
+        const float2 s = next;
+        if (row + step < p.rows) next = p.stats[row + step];
+        copies_wait<kRing - 2>();
+        fetch(to);
+        to = at;
+        const float minus = -s.x * s.y;   // h = x r - mu r
+        float v[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < UNITS; k++)
+            if (place.live(k)) {
+                uint4 qx = own[at + 2 * k * kThreads], qg = own[at + (2 * k + 1) * kThreads];
+                place.trim(qx, k);   // (an infinity or NaN beside the row is not its own)
+                place.trim(qg, k);
+                float x[N], g[N], wk[N];
+                unpack(qx, x, T());
+                unpack(qg, g, T());
+                weight(k, wk);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float h = fmaf(x[e], s.y, minus), gw = g[e] * wk[e];
+                    v[0] += gw;
+                    v[1] = fmaf(gw, h, v[1]);
+                    if constexpr (SUMS) {
+                        dw[k * N + e] = fmaf(g[e], h, dw[k * N + e]);
+                        db[k * N + e] += g[e];
+                    }
+                }
+            }
+        if (p.dx) {
+            sum(v, turn);
+            const float a = -s.y * (v[0] * over), c = -s.y * (v[1] * over);
+#pragma unroll
+            for (int k = 0; k < UNITS; k++)
+                if (place.live(k)) {
+                    float x[N], g[N], wk[N];
+                    unpack(own[at + 2 * k * kThreads], x, T());
+                    unpack(own[at + (2 * k + 1) * kThreads], g, T());
+                    weight(k, wk);
+#pragma unroll
+                    for (int e = 0; e < N; e++) x[e] = fmaf(fmaf(x[e], s.y, minus), c, fmaf(g[e], wk[e] * s.y, a));
+                    place.store(dx, k, x);
+                }
+            dx += step * p.dim;
+        }
+        at = at == (kRing - 1) * kStage ? 0 : at + kStage;
+    }
+    if constexpr (SUMS) {
+        float *rows_sum = (float *)room;
+        const int64_t part = (int64_t)blockIdx.x * p.dim;
+        if (kTeams > 1) __syncthreads();   // the rows in it are done with
+        for (int i = 0; i < kTeams; i++) {
+            if (mine == i)
+#pragma unroll
+                for (int k = 0; k < UNITS; k++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        if (!place.in(k, e)) continue;
+                        const int j = place.column(k, e);
+                        float a = dw[k * N + e], c = db[k * N + e];
+                        if (kTeams > 1) {
+                            if (i) a += rows_sum[j], c += rows_sum[p.dim + j];
+                            rows_sum[j] = a, rows_sum[p.dim + j] = c;
+                        }
+                        if (i == kTeams - 1) {
+                            if (p.dw) p.dw[part + j] = a;
+                            if (p.db) p.db[part + j] = c;
+                        }
+                    }
+            if (kTeams > 1) __syncthreads();
+        }
+    }
+}
 
 // The sum over the block's 256 threads, the same in each.
 __device__ __forceinline__ float block_sum(float v, float *part) {
@@ -65,30 +422,34 @@ __device__ __forceinline__ float block_sum(float v, float *part) {
     return v;
 }
 
-template <typename T> __global__ void __launch_bounds__(256) norm_kernel(const Norm p) {
+// Rows of any length, read three times.
+template <typename T> __global__ void __launch_bounds__(256) long_norm_kernel(const Norm p) {
     __shared__ float part[8];
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = (const T *)p.x + row * p.stride;
         float sum = 0.0f, sq = 0.0f;
+#pragma unroll 8
         for (int j = threadIdx.x; j < p.dim; j += 256) sum += to_f(x[j]);
         const float mu = block_sum(sum, part) / (float)p.dim;
+#pragma unroll 8
         for (int j = threadIdx.x; j < p.dim; j += 256) {
             const float d = to_f(x[j]) - mu;
             sq = fmaf(d, d, sq);
         }
         const float r = 1.0f / sqrtf(block_sum(sq, part) / (float)p.dim + p.eps);
         T *y = (T *)p.y + row * p.dim;
+#pragma unroll 4
         for (int j = threadIdx.x; j < p.dim; j += 256) from_f(fmaf((to_f(x[j]) - mu) * r, at(p.weight, j, 1.0f), at(p.bias, j, 0.0f)), y[j]);
         if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mu, r);
     }
 }
-
-template <typename T> __global__ void __launch_bounds__(256) grad_kernel(const NormGrad p) {
+template <typename T> __global__ void __launch_bounds__(256) long_grad_kernel(const NormGrad p) {
     __shared__ float part[8];
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = (const T *)p.x + row * p.stride, *g = (const T *)p.g + row * p.g_stride;
         const float2 s = p.stats[row];
         float a = 0.0f, c = 0.0f;
+#pragma unroll 4
         for (int j = threadIdx.x; j < p.dim; j += 256) {
             const float gw = to_f(g[j]) * at(p.weight, j, 1.0f);
             a += gw;
@@ -97,18 +458,20 @@ template <typename T> __global__ void __launch_bounds__(256) grad_kernel(const N
         a = block_sum(a, part) / (float)p.dim;
         c = block_sum(c, part) / (float)p.dim;
         T *dx = (T *)p.dx + row * p.dim;
+#pragma unroll 4
         for (int j = threadIdx.x; j < p.dim; j += 256) {
             const float h = (to_f(x[j]) - s.x) * s.y;
-            from_f(s.y * (to_f(g[j]) * at(p.weight, j, 1.0f) - a - h * c), dx[j]);
+            from_f(s.y * (fmaf(-h, c, fmaf(to_f(g[j]), at(p.weight, j, 1.0f), -a))), dx[j]);
         }
     }
 }
-
+// The sums over rows of rows too long for grad_kernel's registers: a thread a column.
 template <typename T> __global__ void __launch_bounds__(128) columns_kernel(const Columns p) {
     const int j = blockIdx.x * 128 + threadIdx.x;
     if (j >= p.dim) return;
     const int64_t first = (int64_t)blockIdx.y * p.each, end = min(first + p.each, p.rows);
     float w = 0.0f, b = 0.0f;
+#pragma unroll 8
     for (int64_t row = first; row < end; row++) {
         const float2 s = p.stats[row];
         const float g = to_f(((const T *)p.g)[row * p.g_stride + j]);
@@ -120,17 +483,129 @@ template <typename T> __global__ void __launch_bounds__(128) columns_kernel(cons
     if (p.db) p.db[to] = b;
 }
 
-template <typename T> __global__ void __launch_bounds__(128) join_kernel(const float *part, int parts, int dim, T *out) {
-    const int j = blockIdx.x * 128 + threadIdx.x;
-    if (j >= dim) return;
+// The parts' sums: a block 32 columns, eight warps a part each in turn, joined in one order.
+struct Join {
+    const float *part[2];
+    void *out[2];        // null for none
+    int dtype[2], parts, dim;
+};
+__global__ void __launch_bounds__(256) join_kernel(const Join p) {
+    __shared__ float sums[8][33];
+    wait_for_previous();
+    const int which = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    if (!p.out[which]) return;
     float v = 0.0f;
-    for (int i = 0; i < parts; i++) v += part[(int64_t)i * dim + j];
-    from_f(v, out[j]);
+    if (j < p.dim)
+#pragma unroll 8
+        for (int i = warp; i < p.parts; i += 8) v += p.part[which][(int64_t)i * p.dim + j];
+    sums[warp][lane] = v;
+    __syncthreads();
+    if (warp || j >= p.dim) return;
+#pragma unroll
+    for (int w = 1; w < 8; w++) v += sums[w][lane];
+    if (p.dtype[which] == YGG_DTYPE_FLOAT) ((float *)p.out[which])[j] = v;
+    else if (p.dtype[which] == YGG_DTYPE_HALF) ((__half *)p.out[which])[j] = __float2half_rn(v);
+    else ((__nv_bfloat16 *)p.out[which])[j] = __float2bfloat16_rn(v);
 }
 
-int parts_of(int64_t rows) { return (int)std::min<int64_t>((rows + 31) / 32, 256); }
+// How a call is cut, by its sizes alone: threads of a team that take `entries` each (0: rows too long for a block), and blocks (of the backward pass: parts
+// of the sums over rows). Where teams take more than a row, there is a multiple of 8 of them, so that a team's rows begin at one place in their
+// units.
+constexpr int kSms = 148;
+int team_of(int64_t dim, int entries, int most) {
+    if (dim % 8) dim += 7;   // a row that may begin anywhere in its first unit
+    for (int team = 32; team <= most; team *= 2)
+        if (dim <= (int64_t)team * entries) return team;
+    return 0;
+}
+int64_t blocks_of(int64_t rows, int team, int resident) {
+    const int teams = threads_of(team) / team, most = resident * kSms * teams / 8 * 8 / teams;
+    return std::min<int64_t>((rows + teams - 1) / teams, most);
+}
+constexpr int kNormEntries = 16, kGradEntries = 16, kSumsMost = 512;
+int parts_of(int64_t rows, int64_t dim) {
+    const int team = team_of(dim, kGradEntries, kSumsMost);
+    return (int)(team ? blocks_of(rows, team, grad_blocks(team)) : std::min<int64_t>((rows + 31) / 32, 256));
+}
 
-unsigned grid_of(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
+// Rows by their first entry and the distance between them; a single row has none.
+struct RowsOf {
+    const void *first;
+    int64_t stride;
+};
+template <typename T> Mode mode_of(int64_t rows, int64_t dim, std::initializer_list<RowsOf> all) {
+    constexpr int N = kPer<T>;
+    const RowsOf &x = *all.begin();
+    bool whole = dim % N == 0, same = dim % N != 0;
+    for (const RowsOf &r : all) {
+        if (!r.first) continue;
+        whole &= ((uintptr_t)r.first & 15) == 0 && (rows == 1 || r.stride % N == 0);
+        same &= (((uintptr_t)r.first ^ (uintptr_t)x.first) & 15) == 0 && (rows == 1 || (r.stride - x.stride) % N == 0);
+    }
+    return whole ? kWhole : same ? kShifted : kSingle;
+}
+template <typename F> void by_mode(Mode m, F f) {
+    if (m == kWhole) f(std::integral_constant<Mode, kWhole>());
+    else if (m == kShifted) f(std::integral_constant<Mode, kShifted>());
+    else f(std::integral_constant<Mode, kSingle>());
+}
+template <typename F> void by_team(int team, F f) {
+    switch (team) {
+        case 32: f(std::integral_constant<int, 32>()); break;
+        case 64: f(std::integral_constant<int, 64>()); break;
+        case 128: f(std::integral_constant<int, 128>()); break;
+        case 256: f(std::integral_constant<int, 256>()); break;
+        case 512: f(std::integral_constant<int, 512>()); break;
+        default: f(std::integral_constant<int, 1024>());
+    }
+}
+
+template <typename T> cudaError_t launch_norm(const Norm &p, cudaStream_t st) {
+    const int team = team_of(p.dim, kNormEntries, 1024);
+    cudaError_t e = cudaSuccess;
+    if (!team) long_norm_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 1 << 20), 256, 0, st>>>(p);
+    else
+        by_mode(mode_of<T>(p.rows, p.dim, {{p.x, p.stride}, {p.y, p.dim}}), [&](auto m) {
+            by_team(team, [&](auto n) {
+                constexpr Mode M = decltype(m)::value;
+                constexpr int TEAM = decltype(n)::value, UNITS = kNormEntries / kPer<T>, THREADS = threads_of(TEAM);
+                static SmemLimits limits;
+                const auto kernel = norm_kernel<T, M, UNITS, TEAM>;
+                const size_t smem = M == kWhole || TEAM <= 512 ? 0 : THREADS * kNormEntries * 2 * sizeof(float);
+                e = raise_smem_limit((const void *)kernel, smem, limits);
+                if (e == cudaSuccess) kernel<<<(unsigned)blocks_of(p.rows, TEAM, norm_blocks<T>(TEAM, UNITS)), THREADS, smem, st>>>(p);
+            });
+        });
+    return e;
+}
+template <typename T, bool SUMS> cudaError_t launch_grad_as(const NormGrad &p, int team, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
+    by_mode(mode_of<T>(p.rows, p.dim, {{p.x, p.stride}, {p.g, p.g_stride}, {p.dx, p.dim}}), [&](auto m) {
+        by_team(team, [&](auto n) {
+            constexpr int TEAM = decltype(n)::value, UNITS = kGradEntries / kPer<T>, THREADS = threads_of(TEAM);
+            if constexpr (!SUMS || TEAM <= kSumsMost) {
+                static SmemLimits limits;
+                const auto kernel = grad_kernel<T, decltype(m)::value, UNITS, SUMS, TEAM>;
+                const size_t smem = std::max<size_t>(THREADS * UNITS * kStages<T> * 32, SUMS && TEAM < 256 ? 2 * sizeof(float) * p.dim : 0);
+                e = raise_smem_limit((const void *)kernel, smem, limits);
+                if (e == cudaSuccess) kernel<<<(unsigned)blocks_of(p.rows, TEAM, grad_blocks(TEAM)), THREADS, smem, st>>>(p);
+            }
+        });
+    });
+    return e;
+}
+template <typename T> cudaError_t launch_grad(const NormGrad &p, int parts, cudaStream_t st) {
+    const int team = team_of(p.dim, kGradEntries, kSumsMost), wide = team_of(p.dim, kGradEntries, 1024);
+    const bool sums = p.dw || p.db;
+    if (sums && team) return launch_grad_as<T, true>(p, team, st);
+    if (sums)
+        columns_kernel<T><<<dim3((unsigned)((p.dim + 127) / 128), parts), 128, 0, st>>>(
+            {p.x, p.g, p.rows, p.stride, p.g_stride, (p.rows + parts - 1) / parts, p.dim, parts, p.stats, p.dw, p.db});
+    if (!p.dx) return cudaGetLastError();
+    if (wide && kGradEntries / kPer<T> * kStages<T> * 32 * threads_of(wide) <= 224 * 1024) return launch_grad_as<T, false>(p, wide, st);
+    long_grad_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 1 << 20), 256, 0, st>>>(p);
+    return cudaGetLastError();
+}
 
 bool type_ok(int t) { return t >= YGG_DTYPE_FLOAT && t <= YGG_DTYPE_BFLOAT; }
 size_t size_of(int t) { return t == YGG_DTYPE_FLOAT ? 4 : 2; }
@@ -149,13 +624,14 @@ int ygg_layer_norm(int device, int dtype, int64_t rows, int64_t dim, const void 
     OnDevice on(device);
     if (!on.ok) return YGG_E_DEVICE;
     const Norm p{d_x, rows, row_stride, (int)dim, {weight_dtype, d_weight}, {bias_dtype, d_bias}, eps, d_y, (float2 *)d_stats};
-    const int rc = by_type(dtype, [&](auto t) { norm_kernel<decltype(t)><<<grid_of(rows), 256, 0, (cudaStream_t)stream>>>(p); });
-    return rc != YGG_OK ? rc : cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    cudaError_t e = cudaSuccess;
+    const int rc = by_type(dtype, [&](auto t) { e = launch_norm<decltype(t)>(p, (cudaStream_t)stream); });
+    return rc != YGG_OK ? rc : e == cudaSuccess && cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 size_t ygg_layer_norm_workspace(int64_t rows, int64_t dim) {
     if (rows < 0 || dim < 1 || dim > INT32_MAX / 2) return 0;
-    return 2 * sizeof(float) * (size_t)parts_of(rows) * (size_t)dim + 16;
+    return 2 * sizeof(float) * (size_t)parts_of(rows, dim) * (size_t)dim + 16;
 }
 
 int ygg_layer_norm_backward(int device, int dtype, int64_t rows, int64_t dim, const void *d_x, int64_t row_stride,
@@ -176,21 +652,26 @@ int ygg_layer_norm_backward(int device, int dtype, int64_t rows, int64_t dim, co
     if (!d_x || !d_stats || !d_grad) return YGG_E_ARG;
     if ((d_dweight || d_dbias) && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < ygg_layer_norm_workspace(rows, dim)))
         return YGG_E_ARG;
-    const int parts = parts_of(rows);
+    const int parts = parts_of(rows, dim);
     float *dw = (float *)d_workspace, *db = dw + (size_t)parts * dim;
-    const NormGrad p{d_x, d_grad, rows, row_stride, grad_stride, (int)dim, {weight_dtype, d_weight}, (const float2 *)d_stats, d_dx};
-    const Columns c{d_x, d_grad, rows, row_stride, grad_stride, (rows + parts - 1) / parts, (int)dim, parts,
-                    (const float2 *)d_stats, d_dweight ? dw : nullptr, d_dbias ? db : nullptr};
-    const unsigned wide = (unsigned)((dim + 127) / 128);
-    by_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (d_dx) grad_kernel<T><<<grid_of(rows), 256, 0, st>>>(p);
-        if (d_dweight || d_dbias) columns_kernel<T><<<dim3(wide, parts), 128, 0, st>>>(c);
-    });
-    if (d_dweight)
-        by_type(weight_dtype, [&](auto t) { join_kernel<decltype(t)><<<wide, 128, 0, st>>>(dw, parts, (int)dim, (decltype(t) *)d_dweight); });
-    if (d_dbias)
-        by_type(bias_dtype, [&](auto t) { join_kernel<decltype(t)><<<wide, 128, 0, st>>>(db, parts, (int)dim, (decltype(t) *)d_dbias); });
+    const NormGrad p{d_x, d_grad, rows, row_stride, grad_stride, (int)dim, {weight_dtype, d_weight}, (const float2 *)d_stats, d_dx,
+                     d_dweight ? dw : nullptr, d_dbias ? db : nullptr};
+    cudaError_t e = cudaSuccess;
+    by_type(dtype, [&](auto t) { e = launch_grad<decltype(t)>(p, parts, st); });
+    if (e != cudaSuccess) return YGG_E_CUDA;
+    if (d_dweight || d_dbias) {   // it may be launched under the kernel before it, whose sums it waits for
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)((dim + 31) / 32), 2);
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const Join join{{dw, db}, {d_dweight, d_dbias}, {weight_dtype, bias_dtype}, parts, (int)dim};
+        if (cudaLaunchKernelEx(&cfg, join_kernel, join) != cudaSuccess) return YGG_E_CUDA;
+    }
     return cudaGetLastError() == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
