@@ -329,10 +329,15 @@ YGG_API int ygg_fourbit_quantize(int device, int dtype, int64_t n, int64_t k, in
 YGG_API int ygg_fourbit_pack(int device, int64_t n, int64_t k, const int8_t *d_in, int64_t row_stride, uint8_t *d_codes,
                              void *stream);
 
-/* The product. d_bias: float [n], or NULL. */
+/* Bytes of device workspace that ygg_fourbit_linear may need, 16-byte aligned (rows of 16-bit types on 16-byte boundaries need none); it may
+ * be 0. */
+YGG_API size_t ygg_fourbit_workspace(int dtype, int64_t rows, int64_t k);
+
+/* The product. d_bias: float [n], or NULL. Bounded waits that gave up are reported by ygg_linear_status. */
 YGG_API int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, int64_t group, const void *d_x,
                                int64_t row_stride, const uint8_t *d_codes, int scale_dtype, const void *d_scale,
-                               const float *d_bias, int out_dtype, void *d_out, int64_t out_stride, void *stream);
+                               const float *d_bias, int out_dtype, void *d_out, int64_t out_stride, void *d_workspace,
+                               size_t workspace_bytes, void *stream);
 
 /* ---- the choice over beams and vocabulary, and rows in its order ---------------------------------------------------
  * Beam b of a prompt has scores[prompt][b] and the row of logits at prompt_stride and beam_stride entries. With lse its

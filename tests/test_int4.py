@@ -244,8 +244,10 @@ def test_outputs_stay_in_their_rows():
         w = pack(codes, scale, 32)
         frame = torch.full((rows + 2, n + 9), -5.0, device="cuda")
         out = frame[1:-1, 4:4 + n]
+        ws = torch.empty(max(16, lib.ygg_fourbit_workspace(0, rows, k)), dtype=torch.uint8, device="cuda")
         rc = lib.ygg_fourbit_linear(0, 0, rows, k, n, 32, x.data_ptr(), x.stride(0), w.codes.data_ptr(), 0, scale.data_ptr(),
-                                    b.data_ptr(), 0, out.data_ptr(), out.stride(0), torch.cuda.current_stream().cuda_stream)
+                                    b.data_ptr(), 0, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+                                    torch.cuda.current_stream().cuda_stream)
         assert rc == _native.YGG_OK
         assert torch.equal(out, f(x, w, b))
         keep = frame.clone()
@@ -291,13 +293,15 @@ def test_refusals():
 def test_c_entry_refuses_bad_arguments():
     lib = _native.ops()
     linear = lambda rows=1, k=64, n=4, group=32, dtype=0, sd=0, od=0, x=16, codes=16, s=16, out=16: lib.ygg_fourbit_linear(  # noqa: E731
-        0, dtype, rows, k, n, group, x, k, codes, sd, s, None, od, out, n, None)
+        0, dtype, rows, k, n, group, x, k, codes, sd, s, None, od, out, n, None, 0, None)
     for kw in (dict(rows=-1), dict(k=0), dict(n=0), dict(group=31), dict(group=96), dict(x=None), dict(codes=None), dict(s=None),
                dict(out=None), dict(codes=24)):
         assert linear(**kw) == _native.YGG_E_ARG, kw
     for kw in (dict(k=131073), dict(group=1 << 18), dict(sd=3), dict(od=-1)):
         assert linear(**kw) == _native.YGG_E_UNSUPPORTED, kw
     assert linear(rows=0, x=None) == _native.YGG_OK
+    assert lib.ygg_fourbit_workspace(0, 500, 64) > 0 and linear(rows=500) == _native.YGG_E_ARG   # no workspace
+    assert lib.ygg_fourbit_workspace(0, 1, 64) == lib.ygg_fourbit_workspace(0, -1, 64) == lib.ygg_fourbit_workspace(3, 500, 64) == 0
     assert lib.ygg_fourbit_quantize(0, 0, 1, 1, 32, None, 1, 16, 16, None) == _native.YGG_E_ARG
     assert lib.ygg_fourbit_quantize(0, 0, 1, 131073, 32, 16, 1, 16, 16, None) == _native.YGG_E_UNSUPPORTED
     assert lib.ygg_fourbit_pack(0, 1, 1, None, 1, 16, None) == _native.YGG_E_ARG

@@ -16,7 +16,7 @@ EXPORTS = ("ygg_load", "ygg_info", "ygg_step", "ygg_step_debug", "ygg_score", "y
            "ygg_token_logprobs", "ygg_token_logprobs_backward", "ygg_quantize_rows", "ygg_linear_workspace",
            "ygg_linear_quantized", "ygg_linear", "ygg_linear_status", "ygg_cache_workspace", "ygg_cache_fork", "ygg_cache_free",
            "ygg_cache_compact", "ygg_cache_read", "ygg_cache_write", "ygg_cache_copy", "ygg_fourbit_quantize",
-           "ygg_fourbit_pack", "ygg_fourbit_linear", "ygg_beam_workspace", "ygg_beam_select", "ygg_reorder", "ygg_layer_norm",
+           "ygg_fourbit_pack", "ygg_fourbit_workspace", "ygg_fourbit_linear", "ygg_beam_workspace", "ygg_beam_select", "ygg_reorder", "ygg_layer_norm",
            "ygg_layer_norm_workspace", "ygg_layer_norm_backward")
 
 YGG_OK = 0
@@ -130,7 +130,9 @@ def ops() -> ctypes.CDLL:
         l.ygg_cache_copy.argtypes = [i32, cache, i64, vp, vp, vp]
         l.ygg_fourbit_quantize.argtypes = [i32, i32, i64, i64, i64, vp, i64, vp, vp, vp]
         l.ygg_fourbit_pack.argtypes = [i32, i64, i64, vp, i64, vp, vp]
-        l.ygg_fourbit_linear.argtypes = [i32, i32, i64, i64, i64, i64, vp, i64, vp, i32, vp, vp, i32, vp, i64, vp]
+        l.ygg_fourbit_workspace.argtypes = [i32, i64, i64]
+        l.ygg_fourbit_workspace.restype = ctypes.c_size_t
+        l.ygg_fourbit_linear.argtypes = [i32, i32, i64, i64, i64, i64, vp, i64, vp, i32, vp, vp, i32, vp, i64, vp, ctypes.c_size_t, vp]
         l.ygg_beam_select.argtypes = [i32, i32, i64, i64, i64, vp, i64, i64, i32, vp, vp, i64, i64] + [vp] * 5 + [size, vp]
         l.ygg_beam_workspace.argtypes = [i32, i64, i64, i64, i64]
         l.ygg_beam_workspace.restype = size

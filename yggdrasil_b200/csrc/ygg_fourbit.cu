@@ -17,6 +17,7 @@
 
 #include "ygg_ops.cuh"
 #include "ygg_smem.h"
+#include "ygg_tensor.cuh"
 
 namespace {
 
@@ -105,46 +106,6 @@ template <typename T> cudaError_t launch_codes(const Codes &p, cudaStream_t st) 
 }
 
 // ----------------------------------------------------------------------------------------------------- products
-
-// A warp a channel and up to 8 rows; a lane takes a word at a time.
-template <typename T> __global__ void __launch_bounds__(256) plain_kernel(const FourBit p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t ch = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (ch >= p.n) return;
-    const uint32_t *codes = (const uint32_t *)p.codes + ch * p.blocks * 16;
-    for (int64_t m0 = (int64_t)blockIdx.y * 8; m0 < p.rows; m0 += (int64_t)gridDim.y * 8) {
-        const int rows = (int)min((int64_t)8, p.rows - m0);
-        float acc[8] = {};
-        for (int word = lane; word < p.blocks * 16; word += 32) {
-            const int k0 = first_of(word);
-            if (k0 >= p.k) continue;
-            const uint32_t v = codes[word];
-            const float s = load_as(p.scale_dtype, p.scale, ch * p.groups + k0 / p.group);
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                if (r >= rows) break;
-                const T *x = (const T *)p.x + (m0 + r) * p.x_stride;
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (k0 + e < p.k) sum = fmaf(to_f(x[k0 + e]), (float)((int)(v >> field_of(e) & 15u) - 8), sum);
-                acc[r] = fmaf(s, sum, acc[r]);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 8; r++) {
-            float sum = acc[r];
-#pragma unroll
-            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-            if (lane == 0 && r < rows) store_as(p.out_dtype, p.out, (m0 + r) * p.out_stride + ch, sum + (p.bias ? p.bias[ch] : 0.0f));
-        }
-    }
-}
-
-template <typename T> cudaError_t launch_plain(const FourBit &p, cudaStream_t st) {
-    plain_kernel<T><<<dim3((unsigned)((p.n + 7) / 8), (unsigned)std::min<int64_t>((p.rows + 7) / 8, 65535)), 256, 0, st>>>(p);
-    return cudaGetLastError();
-}
 
 // ---------------------------------------------------------------------------------------------------- few rows
 //
@@ -418,6 +379,315 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
     return p.cols <= 8 ? launch_few_cols<T, 1>(p, st) : p.cols <= 16 ? launch_few_cols<T, 2>(p, st) : launch_few_cols<T, 3>(p, st);
 }
 
+// --------------------------------------------------------------------------------------------------- many rows
+//
+// D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N, blocks of 128 inputs. TMA brings a block's codes and
+// the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; eight warps turn the codes into 16-bit
+// integers, K-major and swizzled as the products read them; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
+// longer one) lie in tensor memory, twice, so that eight warps multiply one turn's by the scales and add them up in registers while the next
+// one is summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
+//
+// Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
+// leaves.
+constexpr int kTile = 128, kTurn = 512, kMaxStages = 6, kRing = 216 * 1024;   // three stages of 128 rows
+constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
+
+__device__ int g_fault;   // a bounded wait ran out
+
+struct Many {
+    int64_t rows, n;
+    int blocks, groups, group_log, scale_dtype;   // blocks: of 128 inputs
+    int tn, pieces, stages, channel_blocks, row_blocks, tmem_cols, turn;   // turn: steps of 16 inputs
+    const void *scale;
+    const float *bias;
+    int out_dtype;
+    void *out;
+    int64_t out_stride;
+};
+struct ManyShared {   // at the end of dynamic shared memory
+    uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages], done[2], drained[2];
+    uint32_t tmem;
+};
+
+// E: the type of the products' operands. P: pieces of an entry of x.
+template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
+    many_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap x_map, const Many p) {
+    extern __shared__ __align__(1024) uint8_t ring[];
+    ManyShared &sh = *(ManyShared *)(ring + kRing);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = p.channel_blocks * p.row_blocks;
+    // a stage: the operand of 128 channels (two parts of 64 inputs), the rows of x (pieces, two parts each), the codes
+    const int x_part = p.tn * 128, stage_bytes = 2 * kTile * 128 + P * 2 * x_part + kTile * 64;
+    const auto operand = [&](int s) { return ring + s * stage_bytes; };
+    const auto rows_of = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128; };
+    const auto codes_at = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128 + P * 2 * x_part; };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_addr(&sh.full[s]), 1);
+            mbar_init(smem_addr(&sh.ready[s]), kCodeWarps);
+            mbar_init(smem_addr(&sh.empty[s]), 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(smem_addr(&sh.done[s]), 1);
+            mbar_init(smem_addr(&sh.drained[s]), kSumWarps);
+        }
+        fence_mbar_init();
+    }
+    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), p.tmem_cols);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    bool ok = true;
+
+    if (warp == kSumWarps + kCodeWarps) {          // copies
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 1;
+            wait_for_previous();   // the pieces of x
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const int cb = t % p.channel_blocks, row = t / p.channel_blocks * p.tn;
+                for (int kb = 0; kb < p.blocks; kb++) {
+                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.empty[s]), phase))) break;
+                    const uint32_t bar = smem_addr(&sh.full[s]);
+                    mbar_expect_tx(bar, P * 2 * x_part + kTile * 64);
+                    tma_load<1>(smem_addr(codes_at(s)), &codes_map, kb * 64, cb * kTile, bar);
+                    for (int i = 0; i < 2 * P; i++)
+                        tma_load<1>(smem_addr(rows_of(s)) + i * x_part, &x_map, kb * 128 + (i & 1) * 64, (i >> 1) * (int)p.rows + row, bar);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
+        if (lane == 0) {
+            const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
+            const int every = p.turn / 8;   // blocks of a turn; 0 where a block has several
+            int s = 0, turn = 0;
+            uint32_t phase = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                uint32_t d = 0;
+                int in_turn = 0;
+                for (int kb = 0; kb < p.blocks; kb++) {
+                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.full[s]), phase) && mbar_wait_bounded(smem_addr(&sh.ready[s]), phase))) break;
+                    tmem_fence_after();
+                    const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
+                    const uint64_t part = x_part >> 4;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
+                        if (j % 2 == 0 && start) {
+                            if (!(ok = mbar_wait_bounded(smem_addr(&sh.drained[turn & 1]), ((turn >> 1) & 1) ^ 1))) break;
+                            tmem_fence_after();
+                            d = tmem + (turn & 1) * (p.tmem_cols / 2);
+                        }
+#pragma unroll
+                        for (int i = 0; i < P; i++)
+                            mma_f16(d, a + (j >> 2) * (kTile * 128 / 16) + 2 * (j & 3), b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape,
+                                    !(start && i == 0));
+                        const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
+                        if (j % 2 == 1 && end) {
+                            mma_commit<1>(smem_addr(&sh.done[turn & 1]));
+                            turn++;
+                        }
+                    }
+                    if (!ok) break;
+                    if (++in_turn == every) in_turn = 0;
+                    mma_commit<1>(smem_addr(&sh.empty[s]));
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+            }
+        }
+    } else if (warp >= kSumWarps) {                // codes
+        // a thread: two pieces (of 8 inputs) of each run of a channel's block
+        const int id = threadIdx.x - kSumWarps * 32, r = id & 127, half = id >> 7;
+        int s = 0;
+        uint32_t phase = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int kb = 0; kb < p.blocks; kb++) {
+                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.full[s]), phase)))) break;
+                const uint8_t *from = codes_at(s) + r * 64;
+                uint8_t *to = operand(s) + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int t4 = half * 2 + i;
+                    const uint4 q = *(const uint4 *)(from + ((t4 ^ ((r >> 1) & 3)) << 4));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int run = 0; run < 4; run++) {
+                        const uint4 v = make_uint4(codes_of<E>(w[run], 0), codes_of<E>(w[run], 1), codes_of<E>(w[run], 2), codes_of<E>(w[run], 3));
+                        const int chunk = (run & 1) * 4 + t4;
+                        *(uint4 *)(to + (run >> 1) * (kTile * 128) + ((chunk ^ (r & 7)) << 4)) = v;
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.ready[s]));
+                if (++s == p.stages) s = 0, phase ^= 1;
+            }
+        }
+    } else {                                       // sums
+        const int quad = warp & 3, half = warp >> 2;   // lanes of tensor memory; columns in chunks of 16, every other one
+        int turn = 0;
+        const int turns = (p.blocks * 8 + p.turn - 1) / p.turn;
+        const bool wide = p.scale_dtype == YGG_DTYPE_FLOAT;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            const int64_t row0 = (int64_t)(t / p.channel_blocks) * p.tn, ch = (int64_t)(t % p.channel_blocks) * kTile + quad * 32 + lane;
+            const bool live = ch < p.n;
+            const int64_t scales = (live ? ch : 0) * p.groups;
+            const auto scale_at = [&](int turn) {
+                const int g = min(turn * p.turn * 16 >> p.group_log, p.groups - 1);   // (past k: on zeros)
+                return wide ? ((const uint32_t *)p.scale)[scales + g] : (uint32_t)((const uint16_t *)p.scale)[scales + g];
+            };
+            float acc[4][16];
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) acc[c][j] = 0.0f;
+            uint32_t next = scale_at(0);
+            for (int i = 0; i < turns; i++, turn++) {
+                const float sn = scale_of(next, p.scale_dtype);
+                if (i + 1 < turns) next = scale_at(i + 1);
+                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn & 1]), (turn >> 1) & 1)))) break;
+                tmem_fence_after();
+                const uint32_t d = tmem + (turn & 1) * (p.tmem_cols / 2) + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int column = (2 * c + half) * 16;
+                    if (column >= p.tn) break;
+                    uint32_t v[16];
+                    __syncwarp();
+                    tmem_load16(d + column, v);
+                    tmem_loaded();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) acc[c][j] = fmaf(sn, __uint_as_float(v[j]), acc[c][j]);
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn & 1]));
+            }
+            if (ok && live) {
+                const float bias = p.bias ? p.bias[ch] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int column = (2 * c + half) * 16;
+                    const int rows = (int)min(p.rows - row0 - column, (int64_t)(column < p.tn ? 16 : 0));
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (j < rows) store_as(p.out_dtype, p.out, (row0 + column + j) * p.out_stride + ch, acc[c][j] + bias);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    if (!ok) {
+        *(volatile int *)&g_fault = 1;
+        const long long t0 = clock64();
+        while (clock64() - t0 < 50000000LL) {}
+    }
+    __syncwarp();
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, p.tmem_cols);
+}
+
+// The rows of x as the products read them, 16-byte aligned: pieces of floats, or a copy of 16-bit rows that lie otherwise. [piece][row][padded].
+template <typename T> __global__ void __launch_bounds__(256) pieces_kernel(const FourBit p, uint16_t *out, int padded) {
+    wait_for_previous();
+    let_next_begin();   // (the next launch may read its codes now: whoever wrote them is done)
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T *x = (const T *)p.x + row * p.x_stride;
+#pragma unroll 4
+        for (int j = threadIdx.x; j < padded; j += 256) {
+            T v;
+            from_f(0.0f, v);
+            if (j < p.k) v = x[j];
+            if constexpr (kPieces<T> == 1) {
+                out[row * padded + j] = *(const uint16_t *)&v;
+            } else {
+                const Pieces c = pieces_of(v);
+#pragma unroll
+                for (int i = 0; i < 3; i++) out[((int64_t)i * p.rows + row) * padded + j] = c.v[i];
+            }
+        }
+    }
+}
+
+// Rows of `width` entries of `size` bytes, `stride` bytes apart, in tiles of `box` of them by `box_rows`.
+bool map_tiles(CUtensorMap *map, CUtensorMapDataType type, const void *base, int64_t width, int64_t rows, int64_t stride, int box, int box_rows,
+               CUtensorMapSwizzle swizzle) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t tile[2] = {(cuuint32_t)box, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    return encode(map, type, 2, (void *)base, dims, strides, tile, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int padded_of(int64_t k) { return (int)((k + 7) / 8 * 8); }
+// Whether many_kernel reads the rows of x where they are.
+template <typename T> bool in_place(const void *x, int64_t rows, int64_t stride, int64_t k) {
+    return sizeof(T) == 2 && ((uintptr_t)x & 15) == 0 && (rows == 1 || (stride % 8 == 0 && stride >= k));
+}
+
+template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t st) {
+    using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+    constexpr int P = kPieces<T>;
+    static SmemLimits limits;
+    const size_t smem = kRing + sizeof(ManyShared);
+    if (raise_smem_limit((const void *)many_kernel<E, P>, smem, limits) != cudaSuccess) return YGG_E_CUDA;
+    const bool copied = !in_place<T>(q.x, q.rows, q.x_stride, q.k);
+    const int padded = padded_of(q.k);
+    if (copied) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)std::min<int64_t>(q.rows, 8 * sm_count()));
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        if (cudaLaunchKernelEx(&cfg, pieces_kernel<T>, q, (uint16_t *)room, padded) != cudaSuccess) return YGG_E_CUDA;
+    }
+    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, P, 0, (int)((q.n + kTile - 1) / kTile), 0, 32, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
+    while (1 << p.group_log < q.group) p.group_log++;
+    p.turn = std::min(q.group, kTurn) / 16;
+    // rows of a tile: equal parts of up to 128 (64 of floats, whose pieces take three times the room)
+    const int most = P == 1 ? 128 : 64;
+    const int64_t parts = (q.rows + most - 1) / most;
+    p.tn = (int)(((q.rows + parts - 1) / parts + 15) / 16 * 16);
+    p.row_blocks = (int)((q.rows + p.tn - 1) / p.tn);
+    while (p.tmem_cols < 2 * p.tn) p.tmem_cols *= 2;
+    const int stage = 2 * kTile * 128 + P * 2 * p.tn * 128 + kTile * 64;
+    p.stages = std::min(kMaxStages, kRing / stage);
+    CUtensorMap codes_map, x_map;
+    if (!map_tiles(&codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, q.blocks * 64, q.n, q.blocks * 64, 64, kTile, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !map_tiles(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT16, copied ? room : q.x, copied ? padded : q.k, P * q.rows,
+                   copied ? padded * 2 : (q.rows == 1 ? padded : q.x_stride) * 2, 64, p.tn, CU_TENSOR_MAP_SWIZZLE_128B))
+        return YGG_E_CUDA;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)p.channel_blocks * p.row_blocks, sm_count()));
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = copied ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, many_kernel<E, P>, codes_map, x_map, p) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+}
+
+// Rows beyond what one launch counts its tiles over take several.
+template <typename T> int launch_linear(const FourBit &p, void *room, cudaStream_t st) {
+    if (is_few<T>(p.rows, p.blocks)) return launch_few<T>(p, st) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    const int64_t step = (int64_t)1 << 20;
+    for (int64_t m = 0; m < p.rows; m += step) {
+        FourBit q = p;
+        q.rows = std::min(step, p.rows - m);
+        q.x = (const T *)p.x + m * p.x_stride;
+        q.out = (char *)p.out + m * p.out_stride * (p.out_dtype == YGG_DTYPE_FLOAT ? 4 : 2);
+        const int rc = launch_many<T>(q, room, st);
+        if (rc != YGG_OK) return rc;
+    }
+    return YGG_OK;
+}
+
 bool shape_ok(int64_t n, int64_t k, int64_t group) {
     return n >= 1 && n <= INT32_MAX && k >= 1 && group >= 32 && (group & (group - 1)) == 0;
 }
@@ -425,6 +695,19 @@ int blocks_of(int64_t k) { return (int)((k + 127) / 128); }
 int groups_of(int64_t k, int64_t group) { return (int)((k + group - 1) / group); }
 
 }  // namespace
+
+namespace ygg {
+
+// Whether a bounded wait of many_kernel gave up since the last call; waits for the stream.
+cudaError_t take_fourbit_fault(cudaStream_t st, int *fault) {
+    const int none = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(fault, g_fault, sizeof none, 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && *fault) e = cudaMemcpyToSymbolAsync(g_fault, &none, sizeof none, 0, cudaMemcpyHostToDevice, st);
+    return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
+}
+
+}  // namespace ygg
 
 extern "C" {
 
@@ -454,9 +737,17 @@ int ygg_fourbit_pack(int device, int64_t n, int64_t k, const int8_t *d_in, int64
                                 (cudaStream_t)stream) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
+size_t ygg_fourbit_workspace(int dtype, int64_t rows, int64_t k) {
+    if (rows < 0 || k < 1 || k > YGG_LINEAR_MAX_K || dtype < YGG_DTYPE_FLOAT || dtype > YGG_DTYPE_BFLOAT) return 0;
+    const int pieces = dtype == YGG_DTYPE_FLOAT ? 3 : 1;
+    if (pieces == 3 ? is_few<float>(rows, blocks_of(k)) : is_few<__half>(rows, blocks_of(k))) return 0;
+    return (size_t)std::min<int64_t>(rows, (int64_t)1 << 20) * padded_of(k) * pieces * 2;
+}
+
 int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n, int64_t group, const void *d_x,
                        int64_t row_stride, const uint8_t *d_codes, int scale_dtype, const void *d_scale,
-                       const float *d_bias, int out_dtype, void *d_out, int64_t out_stride, void *stream) {
+                       const float *d_bias, int out_dtype, void *d_out, int64_t out_stride, void *d_workspace,
+                       size_t workspace_bytes, void *stream) {
     if (rows < 0 || rows >= ((int64_t)1 << 40) || !shape_ok(n, k, group)) return YGG_E_ARG;
     if (k > YGG_LINEAR_MAX_K || group > YGG_LINEAR_MAX_K || out_dtype < YGG_DTYPE_FLOAT || out_dtype > YGG_DTYPE_BFLOAT ||
         scale_dtype < YGG_DTYPE_FLOAT || scale_dtype > YGG_DTYPE_BFLOAT)
@@ -467,12 +758,14 @@ int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n
     if (!on.ok) return YGG_E_DEVICE;
     const FourBit p{d_x, rows, row_stride, n, (int)k, blocks_of(k), (int)group, groups_of(k, group), d_codes, scale_dtype,
                     d_scale, d_bias, out_dtype, d_out, out_stride};
-    cudaError_t e = cudaSuccess;
+    int done = YGG_OK;
     const int rc = by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        e = is_few<T>(rows, p.blocks) ? launch_few<T>(p, (cudaStream_t)stream) : launch_plain<T>(p, (cudaStream_t)stream);
+        const size_t room = is_few<T>(rows, p.blocks) || in_place<T>(d_x, rows, row_stride, k) ? 0 : ygg_fourbit_workspace(dtype, rows, k);
+        if (room && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < room)) done = YGG_E_ARG;
+        else done = launch_linear<T>(p, d_workspace, (cudaStream_t)stream);
     });
-    return rc != YGG_OK ? rc : e == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    return rc != YGG_OK ? rc : done;
 }
 
 }  // extern "C"

@@ -17,6 +17,10 @@
 #include "ygg_ops.cuh"
 #include "ygg_tensor.cuh"
 
+namespace ygg {
+cudaError_t take_fourbit_fault(cudaStream_t st, int *fault);   // ygg_fourbit.cu
+}
+
 namespace {
 
 using namespace ygg;
@@ -517,22 +521,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == kEpilogueWarps) tmem_free<1>(tmem, p.tmem_cols);
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return (EncodeTiled)f;
-    }();
-    return fn;
-}
-
 // Rows of k bytes, `stride` apart, in tiles of 128 bytes by `box` rows.
 bool map_rows(CUtensorMap *map, const int8_t *base, int64_t rows, int64_t stride, int k, int box) {
     const EncodeTiled encode = encode_tiled();
@@ -888,8 +876,10 @@ int ygg_linear_status(int device, void *stream, int *status_out) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e == cudaSuccess && v) e = cudaMemcpyToSymbolAsync(g_fault, &none, sizeof none, 0, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    int other = 0;
+    if (e == cudaSuccess) e = take_fourbit_fault(st, &other);
     if (e != cudaSuccess) return YGG_E_CUDA;
-    *status_out = v ? YGG_E_TIMEOUT : YGG_OK;
+    *status_out = v || other ? YGG_E_TIMEOUT : YGG_OK;
     return YGG_OK;
 }
 

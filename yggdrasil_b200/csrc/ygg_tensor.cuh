@@ -2,6 +2,7 @@
 // or a pair, accumulators in tensor memory. CTAS is 1 or 2: the CTAs that share one product.
 #pragma once
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "ygg_device.cuh"
@@ -69,6 +70,17 @@ __device__ __forceinline__ void mma_s8(uint32_t d, uint64_t a, uint64_t b, uint3
             "r"(add ? 1u : 0u)
             : "memory");
 }
+// 16-bit operands of one type, 32-bit float sums, m x n.
+__device__ __forceinline__ uint32_t product_f16(int m, int n, bool bfloat) {
+    return (1u << 4) | ((uint32_t)bfloat << 7) | ((uint32_t)bfloat << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
+        "r"(add ? 1u : 0u)
+        : "memory");
+}
 // One arrival on `bar` (of both CTAs of a pair) when the products issued so far are done.
 template <int CTAS> __device__ __forceinline__ void mma_commit(uint32_t bar) {
     if constexpr (CTAS == 2)
@@ -106,5 +118,22 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
         : "r"(addr));
 }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// The driver's call that describes a tiled copy, or null.
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return (EncodeTiled)f;
+    }();
+    return fn;
+}
 
 }  // namespace ygg

@@ -501,11 +501,14 @@ PyObject *py_int4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int out_dtype = type_asked(args[3], x->scalar_type(), type);
     if (out_dtype < 0) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard on(device);
-    Tensor out = empty({rows, channels}, type, device);
+    Tensor out = empty({rows, channels}, type, device), room;
+    const int64_t bytes = (int64_t)ygg_fourbit_workspace(dtype_of(x->scalar_type()), rows, w->k);
+    if (bytes) room = empty({bytes}, at::kByte, device);
     raise_for(ygg_fourbit_linear(device.index(), dtype_of(x->scalar_type()), rows, w->k, channels, w->group, x->data_ptr(),
                                  x->stride(0), (const uint8_t *)w->codes.data_ptr(), dtype_of(w->scale.scalar_type()),
                                  w->scale.data_ptr(), bias ? (const float *)bias->data_ptr() : nullptr, out_dtype,
-                                 out.data_ptr(), channels, stream_of(device.index())),
+                                 out.data_ptr(), channels, bytes ? room.data_ptr() : nullptr, (size_t)bytes,
+                                 stream_of(device.index())),
               "ygg_fourbit_linear");
     return wrap(out);
     END_HANDLE_TH_ERRORS
