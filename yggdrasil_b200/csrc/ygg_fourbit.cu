@@ -414,7 +414,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap x_map, const Many p) {
     extern __shared__ __align__(1024) uint8_t ring[];
     ManyShared &sh = *(ManyShared *)(ring + kRing);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (a value that the whole warp shares)
     const int tiles = p.channel_blocks * p.row_blocks;
     // a stage: the operand of 128 channels (two parts of 64 inputs), the rows of x (pieces, two parts each), the codes
     const int x_part = p.tn * 128, stage_bytes = 2 * kTile * 128 + P * 2 * x_part + kTile * 64;
@@ -459,42 +459,42 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             }
         }
     } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
-        if (lane == 0) {
-            const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
-            const int every = p.turn / 8;   // blocks of a turn; 0 where a block has several
-            int s = 0, turn = 0;
-            uint32_t phase = 0;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                uint32_t d = 0;
-                int in_turn = 0;
-                for (int kb = 0; kb < p.blocks; kb++) {
-                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.full[s]), phase) && mbar_wait_bounded(smem_addr(&sh.ready[s]), phase))) break;
-                    tmem_fence_after();
-                    const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
-                    const uint64_t part = x_part >> 4;
+        const bool leader = lane == 0;
+        const auto wait = [&](uint64_t &bar, uint32_t phase) { return __all_sync(~0u, mbar_wait_bounded(smem_addr(&bar), phase)) != 0; };
+        const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
+        const int every = p.turn / 8;   // blocks of a turn; 0 where a block has several
+        int s = 0, turn = 0;
+        uint32_t phase = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            uint32_t d = 0;
+            int in_turn = 0;
+            for (int kb = 0; kb < p.blocks; kb++) {
+                if (!(ok = wait(sh.full[s], phase) && wait(sh.ready[s], phase))) break;
+                tmem_fence_after();
+                const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
+                const uint64_t part = x_part >> 4;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
-                        if (j % 2 == 0 && start) {
-                            if (!(ok = mbar_wait_bounded(smem_addr(&sh.drained[turn & 1]), ((turn >> 1) & 1) ^ 1))) break;
-                            tmem_fence_after();
-                            d = tmem + (turn & 1) * (p.tmem_cols / 2);
-                        }
-#pragma unroll
-                        for (int i = 0; i < P; i++)
-                            mma_f16(d, a + (j >> 2) * (kTile * 128 / 16) + 2 * (j & 3), b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape,
-                                    !(start && i == 0));
-                        const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
-                        if (j % 2 == 1 && end) {
-                            mma_commit<1>(smem_addr(&sh.done[turn & 1]));
-                            turn++;
-                        }
+                for (int j = 0; j < 8; j++) {
+                    const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
+                    if (j % 2 == 0 && start) {
+                        if (!(ok = wait(sh.drained[turn & 1], ((turn >> 1) & 1) ^ 1))) break;
+                        tmem_fence_after();
+                        d = tmem + (turn & 1) * (p.tmem_cols / 2);
                     }
-                    if (!ok) break;
-                    if (++in_turn == every) in_turn = 0;
-                    mma_commit<1>(smem_addr(&sh.empty[s]));
-                    if (++s == p.stages) s = 0, phase ^= 1;
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+                        mma_f16(d, a + (j >> 2) * (kTile * 128 / 16) + 2 * (j & 3), b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape, !(start && i == 0),
+                                leader);
+                    const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
+                    if (j % 2 == 1 && end) {
+                        mma_commit_by(smem_addr(&sh.done[turn & 1]), leader);
+                        turn++;
+                    }
                 }
+                if (!ok) break;
+                if (++in_turn == every) in_turn = 0;
+                mma_commit_by(smem_addr(&sh.empty[s]), leader);
+                if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
     } else if (warp >= kSumWarps) {                // codes

@@ -74,11 +74,19 @@ __device__ __forceinline__ void mma_s8(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ uint32_t product_f16(int m, int n, bool bfloat) {
     return (1u << 4) | ((uint32_t)bfloat << 7) | ((uint32_t)bfloat << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+// Issued by the lane where `leader` is set, in control flow that the whole warp shares: its operands then stay in uniform registers. (A lane by
+// itself paid 110 to 240 cycles a product for moving them there.)
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add, bool leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
-        "r"(add ? 1u : 0u)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
+        "r"(add ? 1u : 0u), "r"(leader ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_by(uint32_t bar, bool leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader ? 1u : 0u)
         : "memory");
 }
 // One arrival on `bar` (of both CTAs of a pair) when the products issued so far are done.
