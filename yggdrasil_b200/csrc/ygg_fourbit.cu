@@ -381,26 +381,23 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 
 // --------------------------------------------------------------------------------------------------- many rows
 //
-// D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N. TMA brings codes (blocks of 128 inputs) and the rows of x
-// (64 inputs a stage; for floats the three pieces that a launch before this one wrote) into rings; eight warps turn the codes into 16-bit integers,
-// K-major and swizzled as the products read them, in a ring that goes with that of x; one warp issues the products. The sums of a turn (a group,
-// or 512 inputs of a longer one) lie in tensor memory, in one of four places, and eight warps multiply them by the scales and add them up in
-// registers while the next turns are summed: the scale is applied to float sums, as in the other kernel. A block is persistent over tiles.
-// A round through a ring's barriers takes over a microsecond whatever is in it, so that the rings' number of stages sets the rate: @RINGS@
+// D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N, blocks of 128 inputs. TMA brings a block's codes and
+// the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; eight warps turn the codes into 16-bit
+// integers, K-major and swizzled as the products read them; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
+// longer one) lie in tensor memory, twice, so that eight warps multiply one turn's by the scales and add them up in registers while the next
+// one is summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
 //
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
 // leaves.
-constexpr int kTile = 128, kTurn = 512, kSumPlaces = 4;
-constexpr int kCodeBytes = kTile * 64, kOperandBytes = kTile * 128;   // a block's codes; 64 inputs of 128 channels
-constexpr int kMaxStages = 8, kRing = 216 * 1024;
-constexpr int kSumWarps = 8, kCodeWarps = 8, kProducts = kSumWarps + kCodeWarps, kManyThreads = (kProducts + 3) * 32;
+constexpr int kTile = 128, kTurn = 512, kMaxStages = 6, kRing = 216 * 1024;   // three stages of 128 rows
+constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
 
 __device__ int g_fault;   // a bounded wait ran out
 
 struct Many {
     int64_t rows, n;
     int blocks, groups, group_log, scale_dtype;   // blocks: of 128 inputs
-    int tn, stages, code_stages, channel_blocks, row_blocks, turn;   // turn: steps of 16 inputs
+    int tn, pieces, stages, channel_blocks, row_blocks, tmem_cols, turn;   // turn: steps of 16 inputs
     const void *scale;
     const float *bias;
     int out_dtype;
@@ -408,17 +405,8 @@ struct Many {
     int64_t out_stride;
 };
 struct ManyShared {   // at the end of dynamic shared memory
-    uint64_t codes_full[kMaxStages], codes_empty[kMaxStages], rows_full[kMaxStages], ready[kMaxStages], empty[kMaxStages];
-    uint64_t done[kSumPlaces], drained[kSumPlaces];
+    uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages], done[2], drained[2];
     uint32_t tmem;
-};
-// A place in a ring, and the phase of its barriers.
-struct Ring {
-    int s = 0;
-    uint32_t phase = 0;
-    __device__ __forceinline__ void next(int stages) {
-        if (++s == stages) s = 0, phase ^= 1;
-    }
 };
 
 // E: the type of the products' operands. P: pieces of an entry of x.
@@ -428,125 +416,113 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     ManyShared &sh = *(ManyShared *)(ring + kRing);
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (a value that the whole warp shares)
     const int tiles = p.channel_blocks * p.row_blocks;
-    const int x_part = p.tn * 128, stage_bytes = kOperandBytes + P * x_part;   // a stage: the channels' operand, then the pieces of x
-    uint8_t *codes = ring + p.stages * stage_bytes;
+    // a stage: the operand of 128 channels (two parts of 64 inputs), the rows of x (pieces, two parts each), the codes
+    const int x_part = p.tn * 128, stage_bytes = 2 * kTile * 128 + P * 2 * x_part + kTile * 64;
+    const auto operand = [&](int s) { return ring + s * stage_bytes; };
+    const auto rows_of = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128; };
+    const auto codes_at = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128 + P * 2 * x_part; };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kMaxStages; s++) {
-            mbar_init(smem_addr(&sh.codes_full[s]), 1);
-            mbar_init(smem_addr(&sh.codes_empty[s]), kCodeWarps);
-            mbar_init(smem_addr(&sh.rows_full[s]), 1);
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_addr(&sh.full[s]), 1);
             mbar_init(smem_addr(&sh.ready[s]), kCodeWarps);
             mbar_init(smem_addr(&sh.empty[s]), 1);
         }
-        for (int s = 0; s < kSumPlaces; s++) {
+        for (int s = 0; s < 2; s++) {
             mbar_init(smem_addr(&sh.done[s]), 1);
             mbar_init(smem_addr(&sh.drained[s]), kSumWarps);
         }
         fence_mbar_init();
     }
-    if (warp == kProducts) tmem_alloc<1>(smem_addr(&sh.tmem), kSumPlaces * kTile);
+    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), p.tmem_cols);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     bool ok = true;
 
-    if (warp == kProducts + 1) {          // copies of codes
+    if (warp == kSumWarps + kCodeWarps) {          // copies
         if (lane == 0) {
-            Ring at;
-            wait_for_previous();
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-                for (int kb = 0; kb < p.blocks; kb++, at.next(p.code_stages)) {
-                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.codes_empty[at.s]), at.phase ^ 1))) break;
-                    const uint32_t bar = smem_addr(&sh.codes_full[at.s]);
-                    mbar_expect_tx(bar, kCodeBytes);
-                    tma_load<1>(smem_addr(codes + at.s * kCodeBytes), &codes_map, kb * 64, t % p.channel_blocks * kTile, bar);
-                }
-        }
-    } else if (warp == kProducts + 2) {   // copies of the rows of x
-        if (lane == 0) {
-            Ring at;
+            int s = 0;
+            uint32_t phase = 1;
             wait_for_previous();   // the pieces of x
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-                for (int kh = 0; kh < 2 * p.blocks; kh++, at.next(p.stages)) {
-                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.empty[at.s]), at.phase ^ 1))) break;
-                    const uint32_t bar = smem_addr(&sh.rows_full[at.s]), to = smem_addr(ring + at.s * stage_bytes + kOperandBytes);
-                    mbar_expect_tx(bar, P * x_part);
-#pragma unroll
-                    for (int i = 0; i < P; i++) tma_load<1>(to + i * x_part, &x_map, kh * 64, i * (int)p.rows + t / p.channel_blocks * p.tn, bar);
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const int cb = t % p.channel_blocks, row = t / p.channel_blocks * p.tn;
+                for (int kb = 0; kb < p.blocks; kb++) {
+                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.empty[s]), phase))) break;
+                    const uint32_t bar = smem_addr(&sh.full[s]);
+                    mbar_expect_tx(bar, P * 2 * x_part + kTile * 64);
+                    tma_load<1>(smem_addr(codes_at(s)), &codes_map, kb * 64, cb * kTile, bar);
+                    for (int i = 0; i < 2 * P; i++)
+                        tma_load<1>(smem_addr(rows_of(s)) + i * x_part, &x_map, kb * 128 + (i & 1) * 64, (i >> 1) * (int)p.rows + row, bar);
+                    if (++s == p.stages) s = 0, phase ^= 1;
                 }
+            }
         }
-    } else if (warp == kProducts) {       // products
+    } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
         const bool leader = lane == 0;
         const auto wait = [&](uint64_t &bar, uint32_t phase) { return __all_sync(~0u, mbar_wait_bounded(smem_addr(&bar), phase)) != 0; };
         const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
-        const int every = p.turn / 4;   // stages of a turn; 0 where a stage has two turns
-        int turn = 0;
-        Ring at;
+        const int every = p.turn / 8;   // blocks of a turn; 0 where a block has several
+        int s = 0, turn = 0;
+        uint32_t phase = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
             uint32_t d = 0;
             int in_turn = 0;
-            for (int kh = 0; kh < 2 * p.blocks; kh++, at.next(p.stages)) {
-                if (!(ok = wait(sh.rows_full[at.s], at.phase) && wait(sh.ready[at.s], at.phase))) break;
+            for (int kb = 0; kb < p.blocks; kb++) {
+                if (!(ok = wait(sh.full[s], phase) && wait(sh.ready[s], phase))) break;
                 tmem_fence_after();
-                const uint64_t a = operand_128b(smem_addr(ring + at.s * stage_bytes)), b = a + (kOperandBytes >> 4);
+                const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
+                const uint64_t part = x_part >> 4;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bool start = every ? j == 0 && in_turn == 0 : j % 2 == 0;
+                for (int j = 0; j < 8; j++) {
+                    const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
                     if (j % 2 == 0 && start) {
-                        const int place = turn % kSumPlaces;
-                        if (!(ok = wait(sh.drained[place], (turn / kSumPlaces & 1) ^ 1))) break;
+                        if (!(ok = wait(sh.drained[turn & 1], ((turn >> 1) & 1) ^ 1))) break;
                         tmem_fence_after();
-                        d = tmem + place * kTile;
+                        d = tmem + (turn & 1) * (p.tmem_cols / 2);
                     }
 #pragma unroll
-                    for (int i = 0; i < P; i++) mma_f16(d, a + 2 * j, b + i * (x_part >> 4) + 2 * j, shape, !(start && i == 0), leader);
-                    const bool end = every ? j == 3 && (in_turn + 1 == every || kh + 1 == 2 * p.blocks) : j % 2 == 1;
+                    for (int i = 0; i < P; i++)
+                        mma_f16(d, a + (j >> 2) * (kTile * 128 / 16) + 2 * (j & 3), b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape, !(start && i == 0),
+                                leader);
+                    const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
                     if (j % 2 == 1 && end) {
-                        mma_commit_by(smem_addr(&sh.done[turn % kSumPlaces]), leader);
+                        mma_commit_by(smem_addr(&sh.done[turn & 1]), leader);
                         turn++;
                     }
                 }
                 if (!ok) break;
                 if (++in_turn == every) in_turn = 0;
-                mma_commit_by(smem_addr(&sh.empty[at.s]), leader);
+                mma_commit_by(smem_addr(&sh.empty[s]), leader);
+                if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
     } else if (warp >= kSumWarps) {                // codes
         // a thread: two pieces (of 8 inputs) of each run of a channel's block
         const int id = threadIdx.x - kSumWarps * 32, r = id & 127, half = id >> 7;
-        Ring from, to;
+        int s = 0;
+        uint32_t phase = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int kb = 0; kb < p.blocks && ok; kb++, from.next(p.code_stages)) {
-                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.codes_full[from.s]), from.phase)))) break;
-                const uint8_t *row = codes + from.s * kCodeBytes + r * 64;
-                uint4 q[2];
+            for (int kb = 0; kb < p.blocks; kb++) {
+                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.full[s]), phase)))) break;
+                const uint8_t *from = codes_at(s) + r * 64;
+                uint8_t *to = operand(s) + (r >> 3) * 1024 + (r & 7) * 128;
 #pragma unroll
-                for (int i = 0; i < 2; i++) q[i] = *(const uint4 *)(row + (((half * 2 + i) ^ ((r >> 1) & 3)) << 4));
+                for (int i = 0; i < 2; i++) {
+                    const int t4 = half * 2 + i;
+                    const uint4 q = *(const uint4 *)(from + ((t4 ^ ((r >> 1) & 3)) << 4));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int part = 0; part < 2; part++, to.next(p.stages)) {   // 64 inputs: two runs
-                    uint4 v[2][2];
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int run = 0; run < 2; run++) {
-                            const uint32_t w = part ? (run ? q[i].w : q[i].z) : (run ? q[i].y : q[i].x);
-                            v[i][run] = make_uint4(codes_of<E>(w, 0), codes_of<E>(w, 1), codes_of<E>(w, 2), codes_of<E>(w, 3));
-                        }
-                    if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.empty[to.s]), to.phase ^ 1)))) break;
-                    uint8_t *operand = ring + to.s * stage_bytes + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int run = 0; run < 2; run++) *(uint4 *)(operand + (((run * 4 + half * 2 + i) ^ (r & 7)) << 4)) = v[i][run];
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_addr(&sh.ready[to.s]));
-                        // not before what was read has been used: an arrival alone does not wait for loads that are under way
-                        if (part == 0) mbar_arrive(smem_addr(&sh.codes_empty[from.s]));
+                    for (int run = 0; run < 4; run++) {
+                        const uint4 v = make_uint4(codes_of<E>(w[run], 0), codes_of<E>(w[run], 1), codes_of<E>(w[run], 2), codes_of<E>(w[run], 3));
+                        const int chunk = (run & 1) * 4 + t4;
+                        *(uint4 *)(to + (run >> 1) * (kTile * 128) + ((chunk ^ (r & 7)) << 4)) = v;
                     }
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.ready[s]));
+                if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
     } else {                                       // sums
@@ -571,9 +547,9 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             for (int i = 0; i < turns; i++, turn++) {
                 const float sn = scale_of(next, p.scale_dtype);
                 if (i + 1 < turns) next = scale_at(i + 1);
-                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn % kSumPlaces]), turn / kSumPlaces & 1)))) break;
+                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn & 1]), (turn >> 1) & 1)))) break;
                 tmem_fence_after();
-                const uint32_t d = tmem + turn % kSumPlaces * kTile + ((uint32_t)(quad * 32) << 16);
+                const uint32_t d = tmem + (turn & 1) * (p.tmem_cols / 2) + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int column = (2 * c + half) * 16;
@@ -587,7 +563,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn % kSumPlaces]));
+                if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn & 1]));
             }
             if (ok && live) {
                 const float bias = p.bias ? p.bias[ch] : 0.0f;
@@ -611,7 +587,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     __syncwarp();
     tmem_fence_before();
     __syncthreads();
-    if (warp == kProducts) tmem_free<1>(tmem, kSumPlaces * kTile);
+    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, p.tmem_cols);
 }
 
 // The rows of x as the products read them, 16-byte aligned: pieces of floats, or a copy of 16-bit rows that lie otherwise. [piece][row][padded].
@@ -668,7 +644,7 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
         cfg.stream = st;
         if (cudaLaunchKernelEx(&cfg, pieces_kernel<T>, q, (uint16_t *)room, padded) != cudaSuccess) return YGG_E_CUDA;
     }
-    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, 0, 0, (int)((q.n + kTile - 1) / kTile), 0, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
+    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, P, 0, (int)((q.n + kTile - 1) / kTile), 0, 32, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
     while (1 << p.group_log < q.group) p.group_log++;
     p.turn = std::min(q.group, kTurn) / 16;
     // rows of a tile: equal parts of up to 128 (64 of floats, whose pieces take three times the room)
@@ -676,9 +652,9 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
     const int64_t parts = (q.rows + most - 1) / most;
     p.tn = (int)(((q.rows + parts - 1) / parts + 15) / 16 * 16);
     p.row_blocks = (int)((q.rows + p.tn - 1) / p.tn);
-    const int stage = kOperandBytes + P * p.tn * 128;   // as many stages as leave three blocks of codes, or more of these
-    p.stages = std::min(kMaxStages, (kRing - 3 * kCodeBytes) / stage);
-    p.code_stages = std::min(kMaxStages, (kRing - p.stages * stage) / kCodeBytes);
+    while (p.tmem_cols < 2 * p.tn) p.tmem_cols *= 2;
+    const int stage = 2 * kTile * 128 + P * 2 * p.tn * 128 + kTile * 64;
+    p.stages = std::min(kMaxStages, kRing / stage);
     CUtensorMap codes_map, x_map;
     if (!map_tiles(&codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, q.blocks * 64, q.n, q.blocks * 64, 64, kTile, CU_TENSOR_MAP_SWIZZLE_64B) ||
         !map_tiles(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT16, copied ? room : q.x, copied ? padded : q.k, P * q.rows,
