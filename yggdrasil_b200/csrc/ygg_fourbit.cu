@@ -437,7 +437,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    const uint32_t tmem = __shfl_sync(~0u, *(volatile uint32_t *)&sh.tmem, 0);
     bool ok = true;
 
     if (warp == kSumWarps + kCodeWarps) {          // copies
@@ -469,7 +469,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             uint32_t d = 0;
             int in_turn = 0;
             for (int kb = 0; kb < p.blocks; kb++) {
-                if (!(ok = wait(sh.full[s], phase) && wait(sh.ready[s], phase))) break;
+                if (!(ok = wait(sh.ready[s], phase))) break;   // (who makes the codes ready has waited for the stage's copies)
                 tmem_fence_after();
                 const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
                 const uint64_t part = x_part >> 4;
