@@ -384,12 +384,13 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 // D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N, blocks of 128 inputs. TMA brings a block's codes and
 // the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; eight warps turn the codes into 16-bit
 // integers, K-major and swizzled as the products read them; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
-// longer one) lie in tensor memory, twice, so that eight warps multiply one turn's by the scales and add them up in registers while the next
-// one is summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
+// longer one) lie in tensor memory, in one of four places, and eight warps multiply them by the scales and add them up in registers while the
+// next turns are summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
 //
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
 // leaves.
 constexpr int kTile = 128, kTurn = 512, kMaxStages = 6, kRing = 216 * 1024;   // three stages of 128 rows
+constexpr int kSumPlaces = 4;   // a turn's sums wait to be read for longer than a turn takes: with two places @P2@ us for 256 x 4096 x 16384, @P4@ so
 constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
 
 __device__ int g_fault;   // a bounded wait ran out
@@ -397,7 +398,7 @@ __device__ int g_fault;   // a bounded wait ran out
 struct Many {
     int64_t rows, n;
     int blocks, groups, group_log, scale_dtype;   // blocks: of 128 inputs
-    int tn, pieces, stages, channel_blocks, row_blocks, tmem_cols, turn;   // turn: steps of 16 inputs
+    int tn, pieces, stages, channel_blocks, row_blocks, turn;   // turn: steps of 16 inputs
     const void *scale;
     const float *bias;
     int out_dtype;
@@ -405,7 +406,7 @@ struct Many {
     int64_t out_stride;
 };
 struct ManyShared {   // at the end of dynamic shared memory
-    uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages], done[2], drained[2];
+    uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages], done[kSumPlaces], drained[kSumPlaces];
     uint32_t tmem;
 };
 
@@ -427,13 +428,13 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_init(smem_addr(&sh.ready[s]), kCodeWarps);
             mbar_init(smem_addr(&sh.empty[s]), 1);
         }
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < kSumPlaces; s++) {
             mbar_init(smem_addr(&sh.done[s]), 1);
             mbar_init(smem_addr(&sh.drained[s]), kSumWarps);
         }
         fence_mbar_init();
     }
-    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), p.tmem_cols);
+    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), kSumPlaces * kTile);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -477,9 +478,9 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                 for (int j = 0; j < 8; j++) {
                     const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
                     if (j % 2 == 0 && start) {
-                        if (!(ok = wait(sh.drained[turn & 1], ((turn >> 1) & 1) ^ 1))) break;
+                        if (!(ok = wait(sh.drained[turn % kSumPlaces], (turn / kSumPlaces & 1) ^ 1))) break;
                         tmem_fence_after();
-                        d = tmem + (turn & 1) * (p.tmem_cols / 2);
+                        d = tmem + turn % kSumPlaces * kTile;
                     }
 #pragma unroll
                     for (int i = 0; i < P; i++)
@@ -487,7 +488,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                                 leader);
                     const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
                     if (j % 2 == 1 && end) {
-                        mma_commit_by(smem_addr(&sh.done[turn & 1]), leader);
+                        mma_commit_by(smem_addr(&sh.done[turn % kSumPlaces]), leader);
                         turn++;
                     }
                 }
@@ -543,27 +544,39 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             for (int c = 0; c < 4; c++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) acc[c][j] = 0.0f;
-            uint32_t next = scale_at(0);
-            for (int i = 0; i < turns; i++, turn++) {
-                const float sn = scale_of(next, p.scale_dtype);
-                if (i + 1 < turns) next = scale_at(i + 1);
-                if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn & 1]), (turn >> 1) & 1)))) break;
-                tmem_fence_after();
-                const uint32_t d = tmem + (turn & 1) * (p.tmem_cols / 2) + ((uint32_t)(quad * 32) << 16);
+            // scales four turns ahead: one turn is less than such a load takes
+            uint32_t next[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int column = (2 * c + half) * 16;
-                    if (column >= p.tn) break;
-                    uint32_t v[16];
-                    __syncwarp();
-                    tmem_load16(d + column, v);
-                    tmem_loaded();
+            for (int u = 0; u < 4; u++) next[u] = scale_at(u);
+            for (int first = 0; first < turns && ok; first += 4) {
+                float sn[4];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) acc[c][j] = fmaf(sn, __uint_as_float(v[j]), acc[c][j]);
+                for (int u = 0; u < 4; u++) {
+                    sn[u] = scale_of(next[u], p.scale_dtype);
+                    if (first + 4 < turns) next[u] = scale_at(first + 4 + u);
                 }
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn & 1]));
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if (first + u >= turns) break;
+                    if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn % kSumPlaces]), turn / kSumPlaces & 1)))) break;
+                    tmem_fence_after();
+                    const uint32_t d = tmem + turn % kSumPlaces * kTile + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int column = (2 * c + half) * 16;
+                        if (column >= p.tn) break;
+                        uint32_t v[16];
+                        __syncwarp();
+                        tmem_load16(d + column, v);
+                        tmem_loaded();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) acc[c][j] = fmaf(sn[u], __uint_as_float(v[j]), acc[c][j]);
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn % kSumPlaces]));
+                    turn++;
+                }
             }
             if (ok && live) {
                 const float bias = p.bias ? p.bias[ch] : 0.0f;
@@ -587,7 +600,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     __syncwarp();
     tmem_fence_before();
     __syncthreads();
-    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, p.tmem_cols);
+    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, kSumPlaces * kTile);
 }
 
 // The rows of x as the products read them, 16-byte aligned: pieces of floats, or a copy of 16-bit rows that lie otherwise. [piece][row][padded].
@@ -644,7 +657,7 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
         cfg.stream = st;
         if (cudaLaunchKernelEx(&cfg, pieces_kernel<T>, q, (uint16_t *)room, padded) != cudaSuccess) return YGG_E_CUDA;
     }
-    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, P, 0, (int)((q.n + kTile - 1) / kTile), 0, 32, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
+    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, P, 0, (int)((q.n + kTile - 1) / kTile), 0, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
     while (1 << p.group_log < q.group) p.group_log++;
     p.turn = std::min(q.group, kTurn) / 16;
     // rows of a tile: equal parts of up to 128 (64 of floats, whose pieces take three times the room)
@@ -652,7 +665,6 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
     const int64_t parts = (q.rows + most - 1) / most;
     p.tn = (int)(((q.rows + parts - 1) / parts + 15) / 16 * 16);
     p.row_blocks = (int)((q.rows + p.tn - 1) / p.tn);
-    while (p.tmem_cols < 2 * p.tn) p.tmem_cols *= 2;
     const int stage = 2 * kTile * 128 + P * 2 * p.tn * 128 + kTile * 64;
     p.stages = std::min(kMaxStages, kRing / stage);
     CUtensorMap codes_map, x_map;
