@@ -123,3 +123,59 @@ def test_a_head_whose_product_gave_up_is_reported(models, monkeypatch):
             beam_search(model, [1, 2, 3], n, 2, head=head)
         assert e.value.code == _native.YGG_E_TIMEOUT
     beam_search(model, [1, 2, 3], 3, 2)   # no product of the operators in it
+
+
+@pytest.mark.parametrize("which", ["int8", "float"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_with_a_normalised_head_of_few_bits(models, which, bits):
+    """Layer norm, a product with 4-bit (8-bit) weights, the choice and the reordering of states, run together."""
+    from yggdrasil_b200 import quantize_int4, quantize_rows
+    from yggdrasil_b200.beam import beam_search, state_head
+    model = models[which]
+    k = model.layers * model.n
+    g = torch.Generator().manual_seed(2)
+    w = (torch.randn(model.vocab, k, generator=g) * 0.2).cuda()
+    norm = (1 + 0.1 * torch.randn(k, generator=g)).cuda(), torch.randn(k, generator=g).cuda()
+    b = torch.randn(model.vocab, generator=g).cuda()
+    head = state_head(quantize_int4(w, 32), bias=b, norm=norm) if bits == 4 else state_head(*quantize_rows(w), b, norm)
+    x = np.random.default_rng(4).integers(0, model.vocab, (3, 3))
+    for end in (None, 5):
+        tokens, scores = beam_search(model, x, 8, 4, head=head, end=end)
+        want, best = plain(model, x, 8, 4, head=head, end=end)
+        assert np.array_equal(tokens, want)
+        np.testing.assert_allclose(scores, best, rtol=0, atol=1e-5)
+
+
+def test_a_head_of_4_bits_alone(models):
+    from yggdrasil_b200 import int4_linear, quantize_int4
+    from yggdrasil_b200.beam import state_head
+    model = models["int8"]
+    w = quantize_int4(torch.randn(model.vocab, model.layers * model.n).cuda(), 64)
+    state = torch.randint(-127, 128, (5, model.layers, model.n), dtype=torch.int8).cuda()
+    want = int4_linear(state.float().view(5, -1), w)
+    torch.testing.assert_close(state_head(w)(state), want, rtol=1e-6, atol=1e-4)
+    with pytest.raises(ValueError):
+        state_head(w, torch.ones(model.vocab).cuda())
+
+
+def test_a_norm_is_trained_on_a_steps_states(models):
+    """The loss of a head on normalised states: its gradients through token_logprobs, the product and layer_norm are those of the same
+    formula in 64 bits, within what 32-bit sums leave."""
+    from yggdrasil_b200 import layer_norm, token_logprobs
+    model = models["float"]
+    _, state = model.step(np.arange(6) % model.vocab, model.init_state(6))
+    x = state.reshape(6, -1).float()
+    g = torch.Generator().manual_seed(3)
+    k = x.shape[1]
+    leaves = [torch.ones(k), torch.zeros(k), torch.randn(model.vocab, k, generator=g) / k ** 0.5]
+    targets = torch.arange(6) * 3 % model.vocab
+    own = [v.cuda().requires_grad_() for v in leaves]
+    loss = -token_logprobs(layer_norm(x, own[0], own[1]) @ own[2].T, targets.int().cuda()).logprob.sum()
+    grads = torch.autograd.grad(loss, own)
+    wide = [v.cuda().double().requires_grad_() for v in leaves]
+    h = x.double()
+    h = (h - h.mean(-1, keepdim=True)) / ((h - h.mean(-1, keepdim=True)).square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    logits = (h * wide[0] + wide[1]) @ wide[2].T
+    want = torch.autograd.grad(-torch.log_softmax(logits, -1)[torch.arange(6), targets].sum(), wide)
+    for a, c in zip(grads, want):
+        assert (a - c).norm() <= 1e-5 * c.norm()

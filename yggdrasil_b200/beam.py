@@ -1,22 +1,22 @@
-"""Beam search: a step's alternatives, the states of the streams that go on from them, and, if asked for, an int8 output
-head of one's own, run together.
+"""Beam search: the choice over beams and alternatives, the states of the streams that go on in its order, and, if asked for, an
+output head of one's own with 8-bit or 4-bit weights on the (normalised) states, run together.
 
     from yggdrasil_b200 import Yggdrasil
     from yggdrasil_b200.beam import beam_search
     model = Yggdrasil.load("model.bin", backend="b200")
     tokens, scores = beam_search(model, prompt, n=32, width=4)   # (B, 4, L + 32), (B, 4) nats, best first
 
-Every step: model.step (or the head on the new states) -> token_logprobs with `width` alternatives -> the best `width`
-of the beams' alternatives -> StateCache.fork of the beams that go on, free of the others, compact -> the next step.
+Every step: model.step (or the head on the new states) -> beam_select over the beams' continuations -> reorder_states of the
+states and the tokens so far -> the next step.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
 
-from .cache import StateCache
-from .linear import QuantizedRows, int8_linear, linear_status
-from .logprobs import token_logprobs
+from .linear import Int4Weights, QuantizedRows, int4_linear, int8_linear, linear_status
+from .norm import layer_norm
+from .select import beam_select, reorder_states
 
 
 def state_features(state):
@@ -28,10 +28,26 @@ def state_features(state):
     return rows
 
 
-def state_head(weight, scale, bias=None):
-    """An output head on the states: weight int8 (classes, layers n) and scale (classes,) as quantize_rows gives them.
-    Returns a function state -> logits (B, classes) float32."""
-    return lambda state: int8_linear(state_features(state), weight, scale, bias, out_dtype=torch.float32)
+def state_head(weight, scale=None, bias=None, norm=None):
+    """An output head on the states: weight int8 (classes, layers n) and scale (classes,) as quantize_rows gives them, or
+    Int4Weights of as many inputs (and no scale); norm: a weight and a bias (layers n,) of a layer norm that the states go
+    through first. Returns a function state -> logits (B, classes) float32."""
+    if isinstance(weight, Int4Weights) and scale is not None:
+        raise ValueError("Int4Weights hold their scales")
+
+    def head(state):
+        if norm is None and not isinstance(weight, Int4Weights):
+            return int8_linear(state_features(state), weight, scale, bias, out_dtype=torch.float32)
+        x = state.reshape(state.shape[0], -1)
+        if x.dtype == torch.int8:   # codes up to 127 are exact in either
+            x = x.to(torch.bfloat16 if norm is None else torch.float32)
+        if norm is not None:
+            x = layer_norm(x, *norm)
+        if isinstance(weight, Int4Weights):
+            return int4_linear(x, weight, bias, out_dtype=torch.float32)
+        return int8_linear(x, weight, scale, bias, out_dtype=torch.float32)
+
+    return head
 
 
 def beam_search(model, prompt, n, width=4, head=None, end=None):
@@ -61,51 +77,23 @@ def beam_search(model, prompt, n, width=4, head=None, end=None):
             raise ValueError(f"width {width}: at most {min(classes, 64)}")
         if end is not None and not 0 <= end < classes:
             raise ValueError(f"end {end}: a token below {classes}")
-        # two banks of beams: a step forks one into the other. A step's new pages are taken before the old ones are free.
-        beams = rows * width
-        cache = StateCache.empty(2 * beams + rows, 2 * beams + rows, like=model.init_state(1))
-        first = torch.arange(rows, dtype=torch.int32, device=dev) + 2 * beams
-        cache.grow(first)
-        cache.write(first, state)
-        banks = [torch.arange(beams, dtype=torch.int32, device=dev) + k * beams for k in range(2)]
-        none = torch.full((beams,), -1, dtype=torch.int32, device=dev)
+        end = None if end is None else int(end)
         scores = torch.zeros(rows, 1, dtype=torch.float64, device=dev)
-        done = torch.zeros(rows, 1, dtype=torch.bool, device=dev)
-        tokens = torch.as_tensor(x, device=dev)[:, None]
-        parents_of = first.view(rows, 1)
+        done = None if end is None else torch.zeros(rows, 1, dtype=torch.bool, device=dev)
+        tokens = torch.as_tensor(x, device=dev)   # a row for each beam
         for i in range(n):
-            held = parents_of.shape[1]
-            out = token_logprobs(logits, none[:rows * held], top=width)
-            more = out.top_logprobs.view(rows, held, width).double()
-            ids = out.top_ids.view(rows, held, width)
-            if end is not None:   # a beam that is done goes on with `end` alone, at no cost
-                only = torch.full_like(more, -torch.inf)
-                only[:, :, 0] = 0.0
-                more = torch.where(done[:, :, None], only, more)
-                ids = torch.where(done[:, :, None], end, ids)
-            total = (scores[:, :, None] + more).reshape(rows, -1)
-            total, pick = total.sort(dim=1, descending=True, stable=True)
-            scores, pick = total[:, :width], pick[:, :width]
-            beam, new = pick // width, ids.reshape(rows, -1).gather(1, pick)
-            tokens = torch.cat([tokens.gather(1, beam[:, :, None].expand(-1, -1, tokens.shape[2])),
-                                new[:, :, None].long()], 2)
-            if end is not None:
-                done = done.gather(1, beam) | (new == end)
+            best = beam_select(logits.reshape(rows, -1, classes), scores, width, done=done, end=end)
+            scores, done = best.scores, best.done
+            new = best.tokens.reshape(-1)
             if i + 1 == n:
-                break
-            children = banks[i % 2].view(rows, -1)[:, :width]
-            cache.fork(parents_of.gather(1, beam).reshape(-1), children.reshape(-1))
-            cache.free(parents_of.reshape(-1))
-            cache.compact()   # the beams' states are pages[:beams] now: one contiguous batch, in the order of `page`
-            parents_of = children
-            page = cache.table[children.reshape(-1).long(), 0].long()
-            batch = cache.pages[:beams]
-            order = torch.empty_like(new.reshape(-1))
-            order[page] = new.reshape(-1)
-            logits, state = model.step(order, batch)
-            batch.copy_(state)
-            logits = head_of(logits, state)[page]
-        cache.status()
+                tokens = reorder_states(best.parents, tokens)
+            else:
+                tokens, state = reorder_states(best.parents, tokens, state)
+            tokens = torch.cat([tokens, new[:, None].long()], 1)
+            if i + 1 < n:
+                logits, state = model.step(new, state)
+                logits = head_of(logits, state)
+        tokens = tokens.view(rows, -1, tokens.shape[1])
         if hasattr(model, "status"):
             model.status()
         if head is not None:   # its products may have given up a wait: then the logits are not to be used
