@@ -36,19 +36,13 @@ struct FourBit {
     int64_t out_stride;
 };
 
-__device__ __forceinline__ float load_as(int dtype, const void *p, int64_t at) {
-    if (dtype == YGG_DTYPE_FLOAT) return ((const float *)p)[at];
-    if (dtype == YGG_DTYPE_HALF) return __half2float(((const __half *)p)[at]);
-    return __bfloat162float(((const __nv_bfloat16 *)p)[at]);
-}
 __device__ __forceinline__ void store_as(int dtype, void *p, int64_t at, float v) {
     if (dtype == YGG_DTYPE_FLOAT) ((float *)p)[at] = v;
     else if (dtype == YGG_DTYPE_HALF) ((__half *)p)[at] = __float2half_rn(v);
     else ((__nv_bfloat16 *)p)[at] = __float2bfloat16_rn(v);
 }
 
-// The first input of a word of a row, and where an input of a piece stands in its word.
-__device__ __forceinline__ int first_of(int word) { return (word >> 4) * 128 + (word & 3) * 32 + (word >> 2 & 3) * 8; }
+// Where an input of a piece stands in its word.
 __device__ __forceinline__ int field_of(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
 
 // ------------------------------------------------------------------------------------------------------ weights
@@ -112,7 +106,8 @@ template <typename T> cudaError_t launch_codes(const Codes &p, cudaStream_t st) 
 // Up to 24 columns of 16-bit entries: the rows of x, or three for a row of floats (its bits cut in three pieces of 8, which are
 // exact and add up to it). A warp multiplies 16 channels by 8 columns and 16 inputs at a time (mma.sync, float sums): lane
 // (g, t) holds channels g and g + 8, and 16 bytes of each bring its piece t of four runs of 32 inputs. The columns lie in
-// shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory.
+// shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory. What
+// bounds a row or two is the unpacking of the codes (11 instructions for 8 of them): 1 x 4096 x 32768 21.0 us, half the copy rate.
 constexpr int kFewCols = 24, kFewWarps = 8, kColStride = 20;
 // Blocks an SM: a warp's next 2 KB of codes are on their way while it multiplies nothing, so that the SM's warps cover for each other.
 constexpr int few_blocks(int nt) { return nt == 1 ? 4 : 3; }
@@ -390,7 +385,8 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
 // leaves.
 constexpr int kTile = 128, kTurn = 512, kMaxStages = 6, kRing = 216 * 1024;   // three stages of 128 rows
-constexpr int kSumPlaces = 4;   // a turn's sums wait to be read for longer than a turn takes: with two places @P2@ us for 256 x 4096 x 16384, @P4@ so
+// A turn's sums wait to be read for longer than a turn takes: two places 62.6 us for 256 x 4096 x 16384, four 60.6.
+constexpr int kSumPlaces = 4;
 constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
 
 __device__ int g_fault;   // a bounded wait ran out
@@ -766,16 +762,18 @@ int ygg_fourbit_linear(int device, int dtype, int64_t rows, int64_t k, int64_t n
         return YGG_E_UNSUPPORTED;
     if (rows == 0) return YGG_OK;
     if (!d_x || !d_codes || !d_scale || !d_out || ((uintptr_t)d_codes & 15)) return YGG_E_ARG;
-    OnDevice on(device);
-    if (!on.ok) return YGG_E_DEVICE;
     const FourBit p{d_x, rows, row_stride, n, (int)k, blocks_of(k), (int)group, groups_of(k, group), d_codes, scale_dtype,
                     d_scale, d_bias, out_dtype, d_out, out_stride};
     int done = YGG_OK;
     const int rc = by_type(dtype, [&](auto t) {
         using T = decltype(t);
         const size_t room = is_few<T>(rows, p.blocks) || in_place<T>(d_x, rows, row_stride, k) ? 0 : ygg_fourbit_workspace(dtype, rows, k);
-        if (room && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < room)) done = YGG_E_ARG;
-        else done = launch_linear<T>(p, d_workspace, (cudaStream_t)stream);
+        if (room && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < room)) {
+            done = YGG_E_ARG;
+            return;
+        }
+        OnDevice on(device);
+        done = on.ok ? launch_linear<T>(p, d_workspace, (cudaStream_t)stream) : YGG_E_DEVICE;
     });
     return rc != YGG_OK ? rc : done;
 }
