@@ -100,6 +100,18 @@ def test_every_combination_of_types(rows, dtype, scale_dtype, out_dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,n,group", [(2, 9000, 33, 64), (3, 16385, 4100, 128), (5, 4097, 5003, 32), (8, 4096, 9000, 128),
+                                            (9, 4200, 40, 512), (13, 5000, 4000, 64), (16, 4095, 300, 32)])
+def test_blocks_of_more_warps(rows, k, n, group, dtype):
+    """Rows whose columns fill an SM's shared memory before its warps."""
+    f, _, pack = ops()
+    x = inputs(rows, k, dtype, seed=k) / 16
+    codes, scale, b = weights(n, k, group, dtype, seed=n)
+    check(f(x, pack(codes, scale, group), b), x, codes, scale, group, b, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,k,n", [(1, 131072, 40), (3, 131072, 5), (20, 100003, 300), (130, 65552, 130)])
 def test_long_rows_with_the_largest_codes(rows, k, n):
     f, _, pack = ops()

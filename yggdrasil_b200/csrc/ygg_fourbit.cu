@@ -108,9 +108,9 @@ template <typename T> cudaError_t launch_codes(const Codes &p, cudaStream_t st) 
 // (g, t) holds channels g and g + 8, and 16 bytes of each bring its piece t of four runs of 32 inputs. The columns lie in
 // shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory. What
 // bounds a row or two is the unpacking of the codes (11 instructions for 8 of them): 1 x 4096 x 32768 21.0 us, half the copy rate.
-constexpr int kFewCols = 24, kFewWarps = 8, kColStride = 20;
+constexpr int kFewCols = 24, kFewWarps = 8, kColStride = 20;   // (or twice as many warps)
 // Blocks an SM: a warp's next 2 KB of codes are on their way while it multiplies nothing, so that the SM's warps cover for each other.
-constexpr int few_blocks(int nt) { return nt == 1 ? 4 : 3; }
+constexpr int few_blocks(int nt, int warps) { return (nt == 1 ? 4 : 3) * kFewWarps / warps; }
 
 template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
 
@@ -169,16 +169,16 @@ __device__ __forceinline__ float scale_of(uint32_t raw, int dtype) {
     if (dtype == YGG_DTYPE_HALF) return __half2float(__ushort_as_half((unsigned short)raw));
     return __uint_as_float(dtype == YGG_DTYPE_FLOAT ? raw : raw << 16);
 }
-// RUNS: runs of 32 inputs that share a scale (4: groups of 128 and more).
-template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWarps * 32, few_blocks(NT)) few_kernel(const Few p) {
+// RUNS: runs of 32 inputs that share a scale (4: groups of 128 and more). W: warps of a block.
+template <typename T, int NT, int RUNS, int W> __global__ void __launch_bounds__(W * 32, few_blocks(NT, W)) few_kernel(const Few p) {
     using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
     constexpr int P = kPieces<T>;
     extern __shared__ __align__(16) uint8_t room[];   // [cols][col_bytes] entries, then the sums that warps exchange
     const FourBit &q = p.q;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int units = (q.blocks + 1) / 2, stride = col_bytes(units);
-    float *sums = (float *)(room + p.cols * stride);   // [2][kFewWarps][NT 8][kColStride]
-    const int teams = kFewWarps / p.split, team = warp / p.split, part = warp - team * p.split;
+    float *sums = (float *)(room + p.cols * stride);   // [2][W][NT 8][kColStride]
+    const int teams = W / p.split, team = warp / p.split, part = warp - team * p.split;
     const int64_t tiles = (q.n + 15) / 16, all = (int64_t)gridDim.x * teams, id = (int64_t)blockIdx.x * teams + team;
     const int64_t first = tiles * id / all, last = tiles * (id + 1) / all;
 
@@ -230,7 +230,7 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
         const int vecs = padded / N;
         for (int r = 0; r < rows; r++)
 #pragma unroll 4
-            for (int v = threadIdx.x; v < vecs; v += kFewWarps * 32) {
+            for (int v = threadIdx.x; v < vecs; v += W * 32) {
                 uint4 e = make_uint4(0, 0, 0, 0);
                 if (v * N < q.k) e = load_again(x + r * q.x_stride + v * N);
                 if (v * N < q.k && v * N + N > q.k) {   // the vector that holds the row's end
@@ -255,7 +255,7 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
     } else {
         for (int r = 0; r < rows; r++)
 #pragma unroll 4
-            for (int j = threadIdx.x; j < padded; j += kFewWarps * 32) {
+            for (int j = threadIdx.x; j < padded; j += W * 32) {
                 T e;
                 from_f(0.0f, e);
                 if (j < q.k) e = x[r * q.x_stride + j];
@@ -313,7 +313,7 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
         unit += p.split;
         if (unit < units) continue;
         unit = part;
-        float *mine = sums + (turn * kFewWarps + warp) * (NT * 8 * kColStride);
+        float *mine = sums + (turn * W + warp) * (NT * 8 * kColStride);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             float *to = mine + (j * 8 + 2 * t) * kColStride + g;
@@ -322,7 +322,7 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
         }
         if (p.split == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.split * 32) : "memory");
-        const float *from = sums + (turn * kFewWarps + team * p.split) * (NT * 8 * kColStride);
+        const float *from = sums + (turn * W + team * p.split) * (NT * 8 * kColStride);
         for (int o = part * 32 + lane; o < rows * 16; o += p.split * 32) {
             const int r = o >> 4;
             const int64_t ch = tile * 16 + (o & 15);
@@ -338,32 +338,45 @@ template <typename T, int NT, int RUNS> __global__ void __launch_bounds__(kFewWa
     }
 }
 
-int few_bytes(int cols, int blocks) {
-    return cols * col_bytes((blocks + 1) / 2) + 2 * kFewWarps * ((cols + 7) / 8 * 8) * kColStride * 4;
+int few_bytes(int cols, int blocks, int warps = kFewWarps) {
+    return cols * col_bytes((blocks + 1) / 2) + 2 * warps * ((cols + 7) / 8 * 8) * kColStride * 4;
 }
 template <typename T> bool is_few(int64_t rows, int blocks) {
     return rows <= kFewCols / kPieces<T> && few_bytes((int)rows * kPieces<T>, blocks) <= 220 * 1024;
 }
 
-template <typename T, int NT, int RUNS> cudaError_t launch_few_as(Few p, cudaStream_t st) {
+// Blocks that an SM holds.
+int few_resident(int nt, int warps, size_t smem) { return std::max(1, std::min<int>(few_blocks(nt, warps), 227 * 1024 / (smem + 1024))); }
+
+template <typename T, int NT, int RUNS, int W> cudaError_t launch_few_with(Few p, cudaStream_t st) {
     static SmemLimits limits;
-    const size_t smem = few_bytes(p.cols, p.q.blocks);
-    const cudaError_t e = raise_smem_limit((const void *)few_kernel<T, NT, RUNS>, smem, limits);
+    const size_t smem = few_bytes(p.cols, p.q.blocks, W);
+    const cudaError_t e = raise_smem_limit((const void *)few_kernel<T, NT, RUNS, W>, smem, limits);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = (p.q.n + 15) / 16, units = (p.q.blocks + 1) / 2, resident = std::max<int64_t>(1, std::min<int64_t>(few_blocks(NT), 227 * 1024 / (smem + 1024)));
+    const int64_t tiles = (p.q.n + 15) / 16, units = (p.q.blocks + 1) / 2, resident = few_resident(NT, W, smem);
     // Warps a tile: as few as keep the SMs' warps busy over whole rounds of tiles, since the exchange costs each of them. 1 x 4096
     // x 32768 (0.86 of the warps for two or more): two 21.0 us, four 21.8, eight 22.9, one (0.43) 25.5; 1 x 4096 x 4096: eight
-    // 5.7, four 6.8; 16 x 4096 x 32768 (one block an SM): four 51.4, one and two 57.
-    const int64_t warps = resident * sm_count() * kFewWarps;
+    // 5.7, four 6.8.
+    const int64_t warps = resident * sm_count() * W;
     double most = 0.0;
-    for (int split = 1; split <= kFewWarps && split <= units; split *= 2) {
+    for (int split = 1; split <= W && split <= units; split *= 2) {
         const int64_t busy = tiles * split, rounds = (busy + warps - 1) / warps;
         const double share = (double)busy / (double)(rounds * warps);
         if (share > most * 1.02) most = share, p.split = split;
     }
-    const int64_t grid = std::min<int64_t>((tiles * p.split + kFewWarps - 1) / kFewWarps, resident * sm_count());
-    few_kernel<T, NT, RUNS><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p);
+    const int64_t grid = std::min<int64_t>((tiles * p.split + W - 1) / W, resident * sm_count());
+    few_kernel<T, NT, RUNS, W><<<(unsigned)grid, W * 32, smem, st>>>(p);
     return cudaGetLastError();
+}
+// Blocks of 8 warps, or of 16 that share their columns where an SM holds more warps so: 16 x 4096 x 32768 (the columns take 131 KB) 33.2 us,
+// 51.6 with 8 warps; 8 rows 26.7 and 32.3; 12 x 4096 x 4096 9.6 and 13.9.
+template <typename T, int NT, int RUNS> cudaError_t launch_few_as(const Few &p, cudaStream_t st) {
+    if constexpr (NT < 3) {
+        const size_t wide = few_bytes(p.cols, p.q.blocks, 2 * kFewWarps);
+        if (wide <= 220 * 1024 && 2 * few_resident(NT, 2 * kFewWarps, wide) > few_resident(NT, kFewWarps, few_bytes(p.cols, p.q.blocks)))
+            return launch_few_with<T, NT, RUNS, 2 * kFewWarps>(p, st);
+    }
+    return launch_few_with<T, NT, RUNS, kFewWarps>(p, st);
 }
 template <typename T, int NT> cudaError_t launch_few_cols(const Few &p, cudaStream_t st) {
     return p.q.group == 32 ? launch_few_as<T, NT, 1>(p, st) : p.q.group == 64 ? launch_few_as<T, NT, 2>(p, st) : launch_few_as<T, NT, 4>(p, st);

@@ -213,14 +213,14 @@ def _bias(bias, n, device):
 
 
 def linear_status(device="cuda"):
-    """Raise YggError if a bounded wait of an int8 product on the device gave up since the last call: outputs since then
+    """Raise YggError if a bounded wait of a product on the device gave up since the last call: outputs since then
     are not to be used. Waits for the current stream. The record is one for the device and all of its callers: the first
     that asks is told, and clears it."""
     device = torch.device(device)
     index = device.index if device.index is not None else torch.cuda.current_device()
     out = ctypes.c_int(0)
     check(ops().ygg_linear_status(index, _raw_stream(index), ctypes.byref(out)), "ygg_linear_status")
-    check(out.value, "int8 product")
+    check(out.value, "int8 or 4-bit product")
 
 
 def _laid_out(codes):
