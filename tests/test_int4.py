@@ -268,6 +268,18 @@ def test_outputs_stay_in_their_rows():
 
 
 @pytest.mark.gpu
+def test_views_that_negate():
+    f, quantize, _ = ops()
+    v = torch.randn(5, 1, dtype=torch.complex64, device="cuda").conj().imag
+    plain = v.clone()
+    assert v.is_neg() and not plain.is_neg()
+    w = quantize(plain, 32)
+    got = quantize(v, 32)
+    assert torch.equal(got.codes, w.codes) and torch.equal(got.scale, w.scale)
+    assert torch.equal(f(v, w, v[:, 0]), f(plain, w, plain[:, 0]))
+
+
+@pytest.mark.gpu
 def test_refusals():
     f, quantize, pack = ops()
     x = inputs(4, 64, torch.float32)

@@ -264,6 +264,18 @@ def test_other_streams_and_graphs(rows, dim):
 
 
 @pytest.mark.gpu
+def test_views_that_negate():
+    f = op()
+    v = torch.randn(1, 1, dtype=torch.complex64, device="cuda").conj().imag
+    plain = v.clone()
+    x = torch.randn(3, 1, device="cuda")
+    assert v.is_neg() and v.is_contiguous() and torch.equal(f(x, v[0], v[0]), f(x, plain[0], plain[0]))
+    leaf = plain[0].clone().requires_grad_()   # the gradient that arrives is such a view
+    (db,) = torch.autograd.grad(f(x[:1], None, leaf), leaf, v)
+    assert torch.equal(db, plain[0])
+
+
+@pytest.mark.gpu
 def test_refusals():
     import torch.autograd.forward_ad as fw
     f = op()

@@ -259,6 +259,19 @@ def test_padding_and_layouts_of_reordered_rows():
 
 
 @pytest.mark.gpu
+def test_views_that_conjugate_or_negate():
+    choose, f = ops()
+    z = torch.randn(8, 1, dtype=torch.complex64, device="cuda").conj()
+    parents = torch.tensor([[2, 0], [3, 3]], dtype=torch.int32, device="cuda")
+    rows = [2, 0, 7, 7]
+    assert torch.equal(f(parents, z), z.resolve_conj()[rows])
+    assert z[:1].imag.is_contiguous() and z[:1].imag.is_neg()
+    assert torch.equal(f(parents[:1, :1] * 0, z[:1].imag), z[:1].imag.clone())
+    got = choose(torch.zeros(1, 1, 3, device="cuda"), z[:1].imag, 1)
+    torch.testing.assert_close(got.scores, z[:1].imag.clone() - math.log(3), rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.gpu
 def test_refusals():
     f, reorder = ops()
     x, s = make(2, 4, 50, torch.float32)
@@ -287,7 +300,7 @@ def test_refusals():
         f(x.clone().requires_grad_(), s, 2)
     parents = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
     for bad in ((parents.float(), x[0]), (parents[0], x[0]), (parents.cpu(), x[0]), (parents,), (parents, x[0, :3]), (parents, x[0].cpu()),
-                (parents, x[0], x[0, :2]), (parents, *[x[0]] * 9), (parents, torch.tensor(1.0, device="cuda")), (parents[:0], x[0])):
+                (parents, x[0], x[0, :2]), (parents, *[x[0]] * 9), (parents, x[0, :0]), (parents, torch.tensor(1.0, device="cuda")), (parents[:0], x[0])):
         with pytest.raises(ValueError):
             reorder(*bad)
     with pytest.raises(NotImplementedError):

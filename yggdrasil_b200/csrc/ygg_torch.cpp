@@ -63,6 +63,12 @@ const Tensor *cuda_tensor(PyObject *o) {
     return t.is_cuda() ? &t : nullptr;
 }
 
+// The same, with its values as they lie in memory: no view that conjugates or negates them.
+const Tensor *plain_tensor(PyObject *o) {
+    const Tensor *t = cuda_tensor(o);
+    return t && !t->is_neg() && !t->is_conj() ? t : nullptr;
+}
+
 // A contiguous row of n values of a type on a device (n < 0: any number).
 bool is_row(const Tensor &t, at::ScalarType type, int64_t n, const at::Device &device) {
     return t.scalar_type() == type && t.dim() == 1 && (n < 0 || t.size(0) == n) && t.is_contiguous() &&
@@ -469,7 +475,7 @@ struct FourBit {
 // Int4Weights as the kernels read them.
 std::optional<FourBit> fourbit_of(PyObject *o) {
     if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return std::nullopt;
-    const Tensor *c = cuda_tensor(PyTuple_GET_ITEM(o, 0)), *s = cuda_tensor(PyTuple_GET_ITEM(o, 1));
+    const Tensor *c = plain_tensor(PyTuple_GET_ITEM(o, 0)), *s = plain_tensor(PyTuple_GET_ITEM(o, 1));
     PyObject *k = PyTuple_GET_ITEM(o, 2), *group = PyTuple_GET_ITEM(o, 3);
     if (!c || !s || !PyLong_CheckExact(k) || !PyLong_CheckExact(group)) return std::nullopt;
     FourBit r{*c, *s, PyLong_AsLongLong(k), PyLong_AsLongLong(group)};
@@ -489,13 +495,13 @@ std::optional<FourBit> fourbit_of(PyObject *o) {
 // (x, Int4Weights, bias or None, out_dtype or None) -> y, or None
 PyObject *py_int4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *x = n == 4 ? cuda_tensor(args[0]) : nullptr;
+    const Tensor *x = n == 4 ? plain_tensor(args[0]) : nullptr;
     if (!x || !rows_ok(*x)) Py_RETURN_NONE;
     const auto w = fourbit_of(args[1]);
     const at::Device device = x->device();
     if (!w || x->size(1) != w->k || w->codes.device() != device) Py_RETURN_NONE;
     const int64_t rows = x->size(0), channels = w->codes.size(0);
-    const Tensor *bias = args[2] == Py_None ? nullptr : cuda_tensor(args[2]);
+    const Tensor *bias = args[2] == Py_None ? nullptr : plain_tensor(args[2]);
     if (args[2] != Py_None && (!bias || !is_row(*bias, at::kFloat, channels, device) || tracked(*bias))) Py_RETURN_NONE;
     at::ScalarType type = at::kFloat;
     const int out_dtype = type_asked(args[3], x->scalar_type(), type);
@@ -517,7 +523,7 @@ PyObject *py_int4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // (weight, group) -> (codes, scale), or None
 PyObject *py_quantize_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *w = n == 2 ? cuda_tensor(args[0]) : nullptr;
+    const Tensor *w = n == 2 ? plain_tensor(args[0]) : nullptr;
     if (!w || !rows_ok(*w) || w->size(0) < 1 || !PyLong_Check(args[1])) Py_RETURN_NONE;
     const int64_t group = PyLong_AsLongLong(args[1]), channels = w->size(0), k = w->size(1);
     if (group == -1 && PyErr_Occurred()) throw python_error();
@@ -539,7 +545,7 @@ PyObject *py_quantize_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // (codes int8 (n, k),) -> codes as they are laid out, or None
 PyObject *py_pack_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *c = n == 1 ? cuda_tensor(args[0]) : nullptr;
+    const Tensor *c = n == 1 ? plain_tensor(args[0]) : nullptr;
     if (!c || c->scalar_type() != at::kChar || c->dim() != 2 || c->size(0) < 1 || c->size(1) < 1 ||
         c->size(1) > YGG_LINEAR_MAX_K || (c->size(1) > 1 && c->stride(1) != 1))
         Py_RETURN_NONE;
@@ -558,14 +564,14 @@ PyObject *py_pack_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // (logits, scores, width, done or None, end or None) -> (scores, tokens, parents, done or None), or None
 PyObject *py_beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *x = n == 5 ? cuda_tensor(args[0]) : nullptr, *s = n == 5 ? cuda_tensor(args[1]) : nullptr;
+    const Tensor *x = n == 5 ? plain_tensor(args[0]) : nullptr, *s = n == 5 ? plain_tensor(args[1]) : nullptr;
     if (!x || !s || !PyLong_Check(args[2]) || (args[4] != Py_None && !PyLong_Check(args[4]))) Py_RETURN_NONE;
     const int64_t width = PyLong_AsLongLong(args[2]), end = args[4] == Py_None ? -1 : PyLong_AsLongLong(args[4]);
     if (PyErr_Occurred()) {
         PyErr_Clear();
         Py_RETURN_NONE;
     }
-    const Tensor *done = args[3] == Py_None ? nullptr : cuda_tensor(args[3]);
+    const Tensor *done = args[3] == Py_None ? nullptr : plain_tensor(args[3]);
     if (dtype_of(x->scalar_type()) < 0 || x->dim() != 3 || x->size(1) < 1 || x->size(1) > YGG_BEAMS_MAX || x->size(2) < 1 ||
         x->size(2) > INT32_MAX / x->size(1) || x->size(0) > INT32_MAX || (x->size(2) > 1 && x->stride(2) != 1) ||
         (s->scalar_type() != at::kFloat && s->scalar_type() != at::kDouble) || s->dim() != 2 || s->size(0) != x->size(0) ||
@@ -605,7 +611,7 @@ PyObject *py_beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *py_reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const int count = (int)n - 1;
-    const Tensor *p = n >= 2 ? cuda_tensor(args[0]) : nullptr;
+    const Tensor *p = n >= 2 ? plain_tensor(args[0]) : nullptr;
     if (!p || count > YGG_REORDER_MAX || (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong) || p->dim() != 2 ||
         p->size(0) < 1 || !p->is_contiguous())
         Py_RETURN_NONE;
@@ -613,8 +619,8 @@ PyObject *py_reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::Device device = p->device();
     const Tensor *from[YGG_REORDER_MAX];
     for (int i = 0; i < count; i++) {
-        from[i] = cuda_tensor(args[i + 1]);
-        if (!from[i] || from[i]->dim() < 1 || from[i]->size(0) != (i ? from[0] : from[i])->size(0) ||
+        from[i] = plain_tensor(args[i + 1]);
+        if (!from[i] || from[i]->dim() < 1 || from[i]->size(0) < 1 || from[i]->size(0) != (i ? from[0] : from[i])->size(0) ||
             from[i]->size(0) % prompts || !from[i]->is_contiguous() || from[i]->device() != device || tracked(*from[i]))
             Py_RETURN_NONE;
     }
@@ -685,6 +691,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
         const at::Device device = x.device();
         const c10::cuda::CUDAGuard on(device);
         Tensor g = arriving[0].scalar_type() == x.scalar_type() ? arriving[0] : arriving[0].to(x.scalar_type());
+        g = g.resolve_neg();
         if (!plain_rows(g)) g = g.contiguous();
         const bool has_weight = weight.defined(), has_bias = bias >= 0;
         const auto bias_type = has_bias ? (at::ScalarType)bias : at::kFloat;
@@ -711,7 +718,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 // (x, weight or None, bias or None, eps) -> y, or None
 PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *x = n == 4 ? cuda_tensor(args[0]) : nullptr;
+    const Tensor *x = n == 4 ? plain_tensor(args[0]) : nullptr;
     if (!x || dtype_of(x->scalar_type()) < 0 || x->dim() < 1 || x->size(-1) < 1 || !plain_rows(*x) || !PyFloat_CheckExact(args[3]))
         Py_RETURN_NONE;
     const double eps = PyFloat_AS_DOUBLE(args[3]);
@@ -720,7 +727,7 @@ PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     bool wanted = x->requires_grad(), tangent = has_tangent(*x);
     for (int i = 0; i < 2; i++) {
         if (args[i + 1] == Py_None) continue;
-        const Tensor *t = cuda_tensor(args[i + 1]);
+        const Tensor *t = plain_tensor(args[i + 1]);
         if (!t || dtype_of(t->scalar_type()) < 0 || !is_row(*t, t->scalar_type(), x->size(-1), x->device())) Py_RETURN_NONE;
         a[i] = *t;
         wanted |= t->requires_grad();

@@ -139,7 +139,7 @@ def quantize_int4(weight, group=128):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] < 1:
         raise ValueError("weight must be a float32, float16 or bfloat16 CUDA tensor (N, K)")
     group = _group(group)
-    codes, scale = _ops.quantize_int4(_rows(weight), group)
+    codes, scale = _ops.quantize_int4(_rows(weight).resolve_neg(), group)
     return Int4Weights(codes, scale, weight.shape[1], group)
 
 
@@ -157,7 +157,8 @@ def pack_int4(codes, scale, group=128):
             or scale.device != codes.device:
         raise ValueError(f"scale must be a float tensor {(n, -(-k // group))} on {codes.device}")
     _frozen(scale)
-    return Int4Weights(_ops.pack_int4(codes if k == 1 or codes.stride(1) == 1 else codes.contiguous()), scale.contiguous(), k, group)
+    return Int4Weights(_ops.pack_int4(codes if k == 1 or codes.stride(1) == 1 else codes.contiguous()), scale.resolve_neg().contiguous(), k,
+                       group)
 
 
 def int4_linear(x, weight, bias=None, out_dtype=None):
@@ -191,8 +192,8 @@ def _prepared_int4(x, weight, bias, out_dtype):
         codes = codes.contiguous()
         if codes.data_ptr() % 16:
             codes = codes.clone()
-        weight = Int4Weights(codes, scale.contiguous(), int(k), group)
-        out = _ops.int4_linear(rows, weight, bias, out_dtype)
+        weight = Int4Weights(codes, scale.resolve_neg().contiguous(), int(k), group)
+        out = _ops.int4_linear(rows.resolve_neg(), weight, bias, out_dtype)
     return out.view(*x.shape[:-1], n)
 
 
@@ -209,7 +210,7 @@ def _bias(bias, n, device):
     if not isinstance(bias, torch.Tensor) or bias.shape != (n,) or bias.device != device or bias.dtype not in DTYPES:
         raise ValueError(f"bias must be a float tensor ({n},) on {device}")
     _frozen(bias)
-    return bias.detach().float().contiguous()
+    return bias.detach().resolve_neg().float().contiguous()
 
 
 def linear_status(device="cuda"):

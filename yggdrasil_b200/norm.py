@@ -34,5 +34,5 @@ def _prepared(x, weight, bias, eps):
             raise ValueError(f"{name} must be a float tensor ({x.shape[-1]},) on {x.device}")
     if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0 <= eps < math.inf:
         raise ValueError(f"eps {eps}: a finite number, 0 or more")
-    weight, bias = (v if v is None else v.contiguous() for v in (weight, bias))
-    return _ops.layer_norm(x.contiguous(), weight, bias, float(eps))
+    weight, bias = (v if v is None else v.resolve_neg().contiguous() for v in (weight, bias))
+    return _ops.layer_norm(x.resolve_neg().contiguous(), weight, bias, float(eps))

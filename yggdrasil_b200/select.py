@@ -67,6 +67,7 @@ def _prepared(logits, scores, width, done, end):
             raise ValueError(f"done must be a bool tensor {(prompts, beams)} on {logits.device}")
         done = done.contiguous()
     _no_gradient(logits, scores)
+    logits, scores = logits.resolve_neg(), scores.resolve_neg()
     return _ops.beam_select(logits if vocab == 1 or logits.stride(2) == 1 else logits.contiguous(), scores.contiguous(), int(width),
                             done, None if end is None else int(end))
 
@@ -91,12 +92,12 @@ def _prepared_reorder(parents, tensors):
     for t in tensors:
         if not isinstance(t, torch.Tensor) or t.device != parents.device or t.dim() < 1:
             raise ValueError(f"tensors must be (prompts beams, ...) on {parents.device}")
-        if t.shape[0] != tensors[0].shape[0] or (t.shape[0] % prompts if prompts else t.shape[0]):
-            raise ValueError(f"{t.shape[0]} rows for {prompts} prompts: as many for each, in every tensor")
+        if t.shape[0] != tensors[0].shape[0] or (t.shape[0] % prompts or not t.shape[0] if prompts else t.shape[0]):
+            raise ValueError(f"{t.shape[0]} rows for {prompts} prompts: as many for each, one or more, in every tensor")
     _no_gradient(*tensors)
     if prompts == 0:
         return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors)
-    return _ops.reorder_states(parents.contiguous(), *(t.contiguous() for t in tensors))
+    return _ops.reorder_states(parents.contiguous(), *(t.resolve_conj().resolve_neg().contiguous() for t in tensors))
 
 
 def _no_gradient(*tensors):
