@@ -391,15 +391,17 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 //
 // D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N, blocks of 128 inputs. TMA brings a block's codes and
 // the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; eight warps turn the codes into 16-bit
-// integers, K-major and swizzled as the products read them; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
-// longer one) lie in tensor memory, in one of four places, and eight warps multiply them by the scales and add them up in registers while the
-// next turns are summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
+// integers in tensor memory, the products' other operand; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
+// longer one) lie in tensor memory too, in one of two places (four of up to 64 rows), and eight warps multiply them by the scales and add them
+// up in registers while the next turns are summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
+// Shared memory's bandwidth bounds it (the rows of x are written and read once a product, the codes once): with the integers in shared memory
+// too, written and read there, 256 x 4096 x 16384 took 60.6 us, @A@ so.
 //
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
 // leaves.
-constexpr int kTile = 128, kTurn = 512, kMaxStages = 6, kRing = 216 * 1024;   // three stages of 128 rows
-// A turn's sums wait to be read for longer than a turn takes: two places 62.6 us for 256 x 4096 x 16384, four 60.6.
-constexpr int kSumPlaces = 4;
+constexpr int kTile = 128, kTurn = 512, kMaxStages = 4, kRing = 216 * 1024;
+// Columns of tensor memory: sums, then each stage's integers.
+constexpr int kSumCols = 256, kStageCols = 64, kSumPlaces = 4, kTmemCols = kSumCols + kMaxStages * kStageCols;
 constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
 
 __device__ int g_fault;   // a bounded wait ran out
@@ -426,11 +428,13 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     ManyShared &sh = *(ManyShared *)(ring + kRing);
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (a value that the whole warp shares)
     const int tiles = p.channel_blocks * p.row_blocks;
-    // a stage: the operand of 128 channels (two parts of 64 inputs), the rows of x (pieces, two parts each), the codes
-    const int x_part = p.tn * 128, stage_bytes = 2 * kTile * 128 + P * 2 * x_part + kTile * 64;
-    const auto operand = [&](int s) { return ring + s * stage_bytes; };
-    const auto rows_of = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128; };
-    const auto codes_at = [&](int s) { return ring + s * stage_bytes + 2 * kTile * 128 + P * 2 * x_part; };
+    // a stage: the rows of x (pieces, two parts of 64 inputs each), the codes
+    const int x_part = p.tn * 128, stage_bytes = P * 2 * x_part + kTile * 64;
+    const auto rows_of = [&](int s) { return ring + s * stage_bytes; };
+    const auto codes_at = [&](int s) { return ring + s * stage_bytes + P * 2 * x_part; };
+    // places of sums: two of 128 columns, or four of 64
+    const int place_log = p.tn > 64 ? 1 : 2, place = kSumCols >> place_log;
+    const auto place_of = [&](int turn) { return turn & ((1 << place_log) - 1); };
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_addr(&sh.full[s]), 1);
@@ -443,7 +447,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
         }
         fence_mbar_init();
     }
-    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), kSumPlaces * kTile);
+    if (warp == kSumWarps + kCodeWarps) tmem_alloc<1>(smem_addr(&sh.tmem), kTmemCols);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -469,46 +473,47 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             }
         }
     } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
-        const bool leader = lane == 0;
         const auto wait = [&](uint64_t &bar, uint32_t phase) { return __all_sync(~0u, mbar_wait_bounded(smem_addr(&bar), phase)) != 0; };
         const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
-        const int every = p.turn / 8;   // blocks of a turn; 0 where a block has several
-        int s = 0, turn = 0;
+        const int every = p.turn / 8, run = min(8, p.turn);   // blocks of a turn, 0 where a block has several; steps in a row
+        const uint64_t part = x_part >> 4;
+        int s = 0, turn = 0, in_turn = 0;
         uint32_t phase = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            uint32_t d = 0;
-            int in_turn = 0;
             for (int kb = 0; kb < p.blocks; kb++) {
-                if (!(ok = wait(sh.ready[s], phase))) break;   // (who makes the codes ready has waited for the stage's copies)
+                if (!(ok = wait(sh.full[s], phase) && wait(sh.ready[s], phase))) break;
                 tmem_fence_after();
-                const uint64_t a = operand_128b(smem_addr(operand(s))), b = operand_128b(smem_addr(rows_of(s)));
-                const uint64_t part = x_part >> 4;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool start = every ? j == 0 && in_turn == 0 : (j & (p.turn - 1)) == 0;
-                    if (j % 2 == 0 && start) {
-                        if (!(ok = wait(sh.drained[turn % kSumPlaces], (turn / kSumPlaces & 1) ^ 1))) break;
+                const uint64_t b = operand_128b(smem_addr(rows_of(s)));
+                const uint32_t a = tmem + kSumCols + s * kStageCols;
+                for (int first = 0; first < 8; first += run) {
+                    const bool end = !every || in_turn + 1 == every || kb + 1 == p.blocks;
+                    if (in_turn == 0) {
+                        if (!(ok = wait(sh.drained[place_of(turn)], (turn >> place_log & 1) ^ 1))) break;
                         tmem_fence_after();
-                        d = tmem + turn % kSumPlaces * kTile;
                     }
+                    const uint32_t d = tmem + place_of(turn) * place;
+                    if (elected()) {
+                        for (int j = first; j < first + run; j += 2)
 #pragma unroll
-                    for (int i = 0; i < P; i++)
-                        mma_f16(d, a + (j >> 2) * (kTile * 128 / 16) + 2 * (j & 3), b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape, !(start && i == 0),
-                                leader);
-                    const bool end = every ? j == 7 && (in_turn + 1 == every || kb + 1 == p.blocks) : ((j + 1) & (p.turn - 1)) == 0;
-                    if (j % 2 == 1 && end) {
-                        mma_commit_by(smem_addr(&sh.done[turn % kSumPlaces]), leader);
-                        turn++;
+                            for (int u = 0; u < 2; u++)
+#pragma unroll
+                                for (int i = 0; i < P; i++)
+                                    mma_f16(d, a + 8 * (j + u), b + (2 * i + (j >> 2)) * part + 2 * ((j & 3) + u), shape,
+                                            in_turn > 0 || j > first || u + i > 0);
+                        if (end) mma_commit<1>(smem_addr(&sh.done[place_of(turn)]));
+                        if (first + run == 8) mma_commit<1>(smem_addr(&sh.empty[s]));
                     }
+                    __syncwarp();
+                    if (end) turn++;
+                    in_turn = end ? 0 : in_turn + 1;
                 }
                 if (!ok) break;
-                if (++in_turn == every) in_turn = 0;
-                mma_commit_by(smem_addr(&sh.empty[s]), leader);
                 if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
     } else if (warp >= kSumWarps) {                // codes
-        // a thread: two pieces (of 8 inputs) of each run of a channel's block
+        // a thread: two pieces (of 8 inputs) of each run of a channel's block. (A stage is filled again when its products are done: its integers,
+        // too, are not read any more.)
         const int id = threadIdx.x - kSumWarps * 32, r = id & 127, half = id >> 7;
         int s = 0;
         uint32_t phase = 0;
@@ -516,20 +521,23 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             for (int kb = 0; kb < p.blocks; kb++) {
                 if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.full[s]), phase)))) break;
                 const uint8_t *from = codes_at(s) + r * 64;
-                uint8_t *to = operand(s) + (r >> 3) * 1024 + (r & 7) * 128;
+                const uint32_t to = tmem + kSumCols + s * kStageCols + half * 8 + ((uint32_t)(r & 96) << 16);
+                uint32_t w[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int t4 = half * 2 + i;
-                    const uint4 q = *(const uint4 *)(from + ((t4 ^ ((r >> 1) & 3)) << 4));
-                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int run = 0; run < 4; run++) {
-                        const uint4 v = make_uint4(codes_of<E>(w[run], 0), codes_of<E>(w[run], 1), codes_of<E>(w[run], 2), codes_of<E>(w[run], 3));
-                        const int chunk = (run & 1) * 4 + t4;
-                        *(uint4 *)(to + (run >> 1) * (kTile * 128) + ((chunk ^ (r & 7)) << 4)) = v;
-                    }
+                    const uint4 q = *(const uint4 *)(from + (((half * 2 + i) ^ ((r >> 1) & 3)) << 4));
+                    w[i][0] = q.x, w[i][1] = q.y, w[i][2] = q.z, w[i][3] = q.w;
                 }
-                fence_proxy_async();
+                tmem_fence_after();
+#pragma unroll
+                for (int run = 0; run < 4; run++) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = codes_of<E>(w[j >> 2][run], j & 3);
+                    tmem_store8(to + run * 16, v);
+                }
+                tmem_stored();
+                tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&sh.ready[s]));
                 if (++s == p.stages) s = 0, phase ^= 1;
@@ -567,9 +575,9 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     if (first + u >= turns) break;
-                    if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[turn % kSumPlaces]), turn / kSumPlaces & 1)))) break;
+                    if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.done[place_of(turn)]), turn >> place_log & 1)))) break;
                     tmem_fence_after();
-                    const uint32_t d = tmem + turn % kSumPlaces * kTile + ((uint32_t)(quad * 32) << 16);
+                    const uint32_t d = tmem + place_of(turn) * place + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         const int column = (2 * c + half) * 16;
@@ -583,7 +591,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                     tmem_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_addr(&sh.drained[turn % kSumPlaces]));
+                    if (lane == 0) mbar_arrive(smem_addr(&sh.drained[place_of(turn)]));
                     turn++;
                 }
             }
@@ -609,7 +617,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     __syncwarp();
     tmem_fence_before();
     __syncthreads();
-    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, kSumPlaces * kTile);
+    if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, kTmemCols);
 }
 
 // The rows of x as the products read them, 16-byte aligned: pieces of floats, or a copy of 16-bit rows that lie otherwise. [piece][row][padded].
@@ -674,7 +682,7 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
     const int64_t parts = (q.rows + most - 1) / most;
     p.tn = (int)(((q.rows + parts - 1) / parts + 15) / 16 * 16);
     p.row_blocks = (int)((q.rows + p.tn - 1) / p.tn);
-    const int stage = 2 * kTile * 128 + P * 2 * p.tn * 128 + kTile * 64;
+    const int stage = P * 2 * p.tn * 128 + kTile * 64;
     p.stages = std::min(kMaxStages, kRing / stage);
     CUtensorMap codes_map, x_map;
     if (!map_tiles(&codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, q.blocks * 64, q.n, q.blocks * 64, 64, kTile, CU_TENSOR_MAP_SWIZZLE_64B) ||

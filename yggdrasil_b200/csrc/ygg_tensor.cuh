@@ -74,19 +74,18 @@ __device__ __forceinline__ void mma_s8(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ uint32_t product_f16(int m, int n, bool bfloat) {
     return (1u << 4) | ((uint32_t)bfloat << 7) | ((uint32_t)bfloat << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// Issued by the lane where `leader` is set, in control flow that the whole warp shares: its operands then stay in uniform registers. (A lane by
-// itself paid 110 to 240 cycles a product for moving them there.)
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add, bool leader) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
-        "r"(add ? 1u : 0u), "r"(leader ? 1u : 0u)
-        : "memory");
+// True in one lane of a warp that is here as a whole, always the same one. Products are issued once a warp, their operands in uniform
+// registers: under `if (elected())` that is plain, while under a condition on the lane each product of 128 x n x 16 took 140 cycles.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
-__device__ __forceinline__ void mma_commit_by(uint32_t bar, bool leader) {
+// a: in tensor memory, a row along M a lane, two entries along K a column.
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader ? 1u : 0u)
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"(add ? 1u : 0u)
         : "memory");
 }
 // One arrival on `bar` (of both CTAs of a pair) when the products issued so far are done.
@@ -125,6 +124,13 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr));
 }
+// 8 columns of this warp's 32 lanes; they are written after tmem_stored().
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // The driver's call that describes a tiled copy, or null.
