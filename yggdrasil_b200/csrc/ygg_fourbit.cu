@@ -473,26 +473,22 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             }
         }
     } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
-        const auto wait = [&](uint64_t &bar, uint32_t phase) { return __all_sync(~0u, mbar_wait_bounded(smem_addr(&bar), phase)) != 0; };
-        const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
-        const int every = p.turn / 8, run = min(8, p.turn);   // blocks of a turn, 0 where a block has several; steps in a row
-        const uint64_t part = x_part >> 4;
-        int s = 0, turn = 0, in_turn = 0;
-        uint32_t phase = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int kb = 0; kb < p.blocks; kb++) {
-                if (!(ok = wait(sh.full[s], phase) && wait(sh.ready[s], phase))) break;
-                tmem_fence_after();
-                const uint64_t b = operand_128b(smem_addr(rows_of(s)));
-                const uint32_t a = tmem + kSumCols + s * kStageCols;
-                for (int first = 0; first < 8; first += run) {
-                    const bool end = !every || in_turn + 1 == every || kb + 1 == p.blocks;
-                    if (in_turn == 0) {
-                        if (!(ok = wait(sh.drained[place_of(turn)], (turn >> place_log & 1) ^ 1))) break;
+        if (elected()) {
+            const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
+            const int every = p.turn / 8, run = min(8, p.turn);   // blocks of a turn, 0 where a block has several; steps in a row
+            const uint64_t part = x_part >> 4;
+            int s = 0, turn = 0, in_turn = 0;
+            uint32_t phase = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                for (int kb = 0; kb < p.blocks; kb++) {
+                    if (!(ok = mbar_wait_bounded(smem_addr(&sh.ready[s]), phase))) break;   // (who makes the codes ready has waited for the stage's copies)
+                    const uint64_t b = operand_128b(smem_addr(rows_of(s)));
+                    const uint32_t a = tmem + kSumCols + s * kStageCols;
+                    for (int first = 0; first < 8; first += run) {
+                        const bool end = !every || in_turn + 1 == every || kb + 1 == p.blocks;
+                        if (in_turn == 0 && !(ok = mbar_wait_bounded(smem_addr(&sh.drained[place_of(turn)]), (turn >> place_log & 1) ^ 1))) break;
                         tmem_fence_after();
-                    }
-                    const uint32_t d = tmem + place_of(turn) * place;
-                    if (elected()) {
+                        const uint32_t d = tmem + place_of(turn) * place;
                         for (int j = first; j < first + run; j += 2)
 #pragma unroll
                             for (int u = 0; u < 2; u++)
@@ -501,16 +497,16 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                                     mma_f16(d, a + 8 * (j + u), b + (2 * i + (j >> 2)) * part + 2 * ((j & 3) + u), shape,
                                             in_turn > 0 || j > first || u + i > 0);
                         if (end) mma_commit<1>(smem_addr(&sh.done[place_of(turn)]));
-                        if (first + run == 8) mma_commit<1>(smem_addr(&sh.empty[s]));
+                        if (end) turn++;
+                        in_turn = end ? 0 : in_turn + 1;
                     }
-                    __syncwarp();
-                    if (end) turn++;
-                    in_turn = end ? 0 : in_turn + 1;
+                    if (!ok) break;
+                    mma_commit<1>(smem_addr(&sh.empty[s]));
+                    if (++s == p.stages) s = 0, phase ^= 1;
                 }
-                if (!ok) break;
-                if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
+        __syncwarp();
     } else if (warp >= kSumWarps) {                // codes
         // a thread: two pieces (of 8 inputs) of each run of a channel's block. (A stage is filled again when its products are done: its integers,
         // too, are not read any more.)
