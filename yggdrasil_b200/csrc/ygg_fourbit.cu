@@ -475,34 +475,56 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     } else if (warp == kSumWarps + kCodeWarps + 1) {   // products
         if (elected()) {
             const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
-            const int every = p.turn / 8, run = min(8, p.turn);   // blocks of a turn, 0 where a block has several; steps in a row
-            const uint64_t part = x_part >> 4;
-            int s = 0, turn = 0, in_turn = 0;
+            const uint64_t part = x_part >> 4, b0 = operand_128b(smem_addr(rows_of(0)));
+            const uint32_t places = (1u << place_log) - 1;
+            const int blocks = p.blocks, stages = p.stages;
+            int s = 0, turn = 0;
             uint32_t phase = 0;
+            // the products of steps first .. first + count - 1 of a stage
+            const auto products = [&](uint32_t d, int first, auto count, bool fresh) {
+                const uint64_t b = b0 + (uint64_t)(s * (stage_bytes >> 4));
+                const uint32_t a = tmem + kSumCols + s * kStageCols;
+#pragma unroll
+                for (int u = 0; u < decltype(count)::value; u++) {
+                    const int j = first + u;
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+                        mma_f16(d, a + 8 * j, b + (2 * i + (j >> 2)) * part + 2 * (j & 3), shape, u + i > 0 || !fresh);
+                }
+            };
+            const auto drained = [&] {
+                return mbar_wait_bounded(smem_addr(&sh.drained[turn & places]), (turn >> place_log & 1) ^ 1);
+            };
             for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                for (int kb = 0; kb < p.blocks; kb++) {
+                int left = p.turn / 8;   // blocks that the turn still has
+                for (int kb = 0; kb < blocks; kb++) {
                     if (!(ok = mbar_wait_bounded(smem_addr(&sh.ready[s]), phase))) break;   // (who makes the codes ready has waited for the stage's copies)
-                    const uint64_t b = operand_128b(smem_addr(rows_of(s)));
-                    const uint32_t a = tmem + kSumCols + s * kStageCols;
-                    for (int first = 0; first < 8; first += run) {
-                        const bool end = !every || in_turn + 1 == every || kb + 1 == p.blocks;
-                        if (in_turn == 0 && !(ok = mbar_wait_bounded(smem_addr(&sh.drained[place_of(turn)]), (turn >> place_log & 1) ^ 1))) break;
+                    if (p.turn >= 8) {
+                        const bool fresh = left == p.turn / 8;
+                        if (fresh && !(ok = drained())) break;
                         tmem_fence_after();
-                        const uint32_t d = tmem + place_of(turn) * place;
-                        for (int j = first; j < first + run; j += 2)
+                        products(tmem + (turn & places) * place, 0, std::integral_constant<int, 8>(), fresh);
+                        if (--left == 0 || kb + 1 == blocks) {
+                            mma_commit<1>(smem_addr(&sh.done[turn & places]));
+                            turn++;
+                            left = p.turn / 8;
+                        }
+                    } else {
 #pragma unroll
-                            for (int u = 0; u < 2; u++)
-#pragma unroll
-                                for (int i = 0; i < P; i++)
-                                    mma_f16(d, a + 8 * (j + u), b + (2 * i + (j >> 2)) * part + 2 * ((j & 3) + u), shape,
-                                            in_turn > 0 || j > first || u + i > 0);
-                        if (end) mma_commit<1>(smem_addr(&sh.done[place_of(turn)]));
-                        if (end) turn++;
-                        in_turn = end ? 0 : in_turn + 1;
+                        for (int first = 0; first < 8; first += 2) {
+                            const bool fresh = (first & (p.turn - 1)) == 0;
+                            if (fresh && !(ok = drained())) break;
+                            tmem_fence_after();
+                            products(tmem + (turn & places) * place, first, std::integral_constant<int, 2>(), fresh);
+                            if (((first + 2) & (p.turn - 1)) == 0) {
+                                mma_commit<1>(smem_addr(&sh.done[turn & places]));
+                                turn++;
+                            }
+                        }
+                        if (!ok) break;
                     }
-                    if (!ok) break;
                     mma_commit<1>(smem_addr(&sh.empty[s]));
-                    if (++s == p.stages) s = 0, phase ^= 1;
+                    if (++s == stages) s = 0, phase ^= 1;
                 }
             }
         }
