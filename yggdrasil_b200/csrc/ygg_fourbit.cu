@@ -402,7 +402,7 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 constexpr int kTile = 128, kTurn = 512, kMaxStages = 4, kRing = 216 * 1024;
 // Columns of tensor memory: sums, then each stage's integers.
 constexpr int kSumCols = 256, kStageCols = 64, kSumPlaces = 4, kTmemCols = kSumCols + kMaxStages * kStageCols;
-constexpr int kSumWarps = 8, kCodeWarps = 8, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
+constexpr int kSumWarps = 8, kCodeWarps = 4, kManyThreads = (kSumWarps + kCodeWarps + 2) * 32;
 
 __device__ int g_fault;   // a bounded wait ran out
 
@@ -530,29 +530,28 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
         }
         __syncwarp();
     } else if (warp >= kSumWarps) {                // codes
-        // a thread: two pieces (of 8 inputs) of each run of a channel's block. (A stage is filled again when its products are done: its integers,
-        // too, are not read any more.)
-        const int id = threadIdx.x - kSumWarps * 32, r = id & 127, half = id >> 7;
+        // a thread: a channel's block. (A stage is filled again when its products are done: its integers, too, are not read any more.)
+        const int r = threadIdx.x - kSumWarps * 32;
         int s = 0;
         uint32_t phase = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
             for (int kb = 0; kb < p.blocks; kb++) {
                 if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.full[s]), phase)))) break;
                 const uint8_t *from = codes_at(s) + r * 64;
-                const uint32_t to = tmem + kSumCols + s * kStageCols + half * 8 + ((uint32_t)(r & 96) << 16);
-                uint32_t w[2][4];
+                const uint32_t to = tmem + kSumCols + s * kStageCols + ((uint32_t)(r & 96) << 16);
+                uint4 w[4];   // the pieces t of the four runs
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint4 q = *(const uint4 *)(from + (((half * 2 + i) ^ ((r >> 1) & 3)) << 4));
-                    w[i][0] = q.x, w[i][1] = q.y, w[i][2] = q.z, w[i][3] = q.w;
-                }
+                for (int i = 0; i < 4; i++) w[i] = *(const uint4 *)(from + ((i ^ ((r >> 1) & 3)) << 4));
                 tmem_fence_after();
 #pragma unroll
                 for (int run = 0; run < 4; run++) {
-                    uint32_t v[8];
+                    uint32_t v[16];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = codes_of<E>(w[j >> 2][run], j & 3);
-                    tmem_store8(to + run * 16, v);
+                    for (int j = 0; j < 16; j++) {
+                        const uint4 q = w[j >> 2];
+                        v[j] = codes_of<E>(run == 0 ? q.x : run == 1 ? q.y : run == 2 ? q.z : q.w, j & 3);
+                    }
+                    tmem_store16(to + run * 16, v);
                 }
                 tmem_stored();
                 tmem_fence_before();
@@ -562,7 +561,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             }
         }
     } else {                                       // sums
-        const int quad = warp & 3, half = warp >> 2;   // lanes of tensor memory; columns in chunks of 16, every other one
+        const int quad = warp & 3, half = warp >> 2;   // lanes of tensor memory; columns in chunks of 32, every other one
         int turn = 0;
         const int turns = (p.blocks * 8 + p.turn - 1) / p.turn;
         const bool wide = p.scale_dtype == YGG_DTYPE_FLOAT;
@@ -574,11 +573,11 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                 const int g = min(turn * p.turn * 16 >> p.group_log, p.groups - 1);   // (past k: on zeros)
                 return wide ? ((const uint32_t *)p.scale)[scales + g] : (uint32_t)((const uint16_t *)p.scale)[scales + g];
             };
-            float acc[4][16];
+            float acc[2][32];
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 2; c++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) acc[c][j] = 0.0f;
+                for (int j = 0; j < 32; j++) acc[c][j] = 0.0f;
             // scales four turns ahead: one turn is less than such a load takes
             uint32_t next[4];
 #pragma unroll
@@ -597,15 +596,15 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_fence_after();
                     const uint32_t d = tmem + place_of(turn) * place + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int column = (2 * c + half) * 16;
+                    for (int c = 0; c < 2; c++) {
+                        const int column = (2 * c + half) * 32;
                         if (column >= p.tn) break;
-                        uint32_t v[16];
+                        uint32_t v[32];
                         __syncwarp();
-                        tmem_load16(d + column, v);
+                        tmem_load32(d + column, v);
                         tmem_loaded();
 #pragma unroll
-                        for (int j = 0; j < 16; j++) acc[c][j] = fmaf(sn[u], __uint_as_float(v[j]), acc[c][j]);
+                        for (int j = 0; j < 32; j++) acc[c][j] = fmaf(sn[u], __uint_as_float(v[j]), acc[c][j]);
                     }
                     tmem_fence_before();
                     __syncwarp();
@@ -616,11 +615,11 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             if (ok && live) {
                 const float bias = p.bias ? p.bias[ch] : 0.0f;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int column = (2 * c + half) * 16;
-                    const int rows = (int)min(p.rows - row0 - column, (int64_t)(column < p.tn ? 16 : 0));
+                for (int c = 0; c < 2; c++) {
+                    const int column = (2 * c + half) * 32;
+                    const int rows = (int)min(p.rows - row0 - column, (int64_t)(column < p.tn ? p.tn - column : 0));
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
+                    for (int j = 0; j < 32; j++)
                         if (j < rows) store_as(p.out_dtype, p.out, (row0 + column + j) * p.out_stride + ch, acc[c][j] + bias);
                 }
             }
