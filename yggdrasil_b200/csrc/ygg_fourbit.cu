@@ -103,12 +103,12 @@ template <typename T> cudaError_t launch_codes(const Codes &p, cudaStream_t st) 
 
 // ---------------------------------------------------------------------------------------------------- few rows
 //
-// Up to 24 columns of 16-bit entries: the rows of x, or three for a row of floats (its bits cut in three pieces of 8, which are
+// Up to 16 columns of 16-bit entries, the rows of x, or 24, three for a row of floats (its bits cut in three pieces of 8, which are
 // exact and add up to it). A warp multiplies 16 channels by 8 columns and 16 inputs at a time (mma.sync, float sums): lane
 // (g, t) holds channels g and g + 8, and 16 bytes of each bring its piece t of four runs of 32 inputs. The columns lie in
 // shared memory. Warps share a tile's blocks of 128 inputs where there are few tiles, and add up through shared memory. What
 // bounds a row or two is the unpacking of the codes (11 instructions for 8 of them): 1 x 4096 x 32768 21.0 us, half the copy rate.
-constexpr int kFewCols = 24, kFewWarps = 8, kColStride = 20;   // (or twice as many warps)
+constexpr int kFewWarps = 8, kColStride = 20;   // (or twice as many warps)
 // Blocks an SM: a warp's next 2 KB of codes are on their way while it multiplies nothing, so that the SM's warps cover for each other.
 constexpr int few_blocks(int nt, int warps) { return (nt == 1 ? 4 : 3) * kFewWarps / warps; }
 
@@ -341,8 +341,10 @@ template <typename T, int NT, int RUNS, int W> __global__ void __launch_bounds__
 int few_bytes(int cols, int blocks, int warps = kFewWarps) {
     return cols * col_bytes((blocks + 1) / 2) + 2 * warps * ((cols + 7) / 8 * 8) * kColStride * 4;
 }
+// More rows are faster in many_kernel: 20 x 1000 x 5003 of 16-bit rows 10.9 us here, 9.4 there; but floats take a launch more there: 8 rows of them
+// 8.2 us here, 11.2 there.
 template <typename T> bool is_few(int64_t rows, int blocks) {
-    return rows <= kFewCols / kPieces<T> && few_bytes((int)rows * kPieces<T>, blocks) <= 220 * 1024;
+    return rows <= (kPieces<T> == 1 ? 16 : 8) && few_bytes((int)rows * kPieces<T>, blocks) <= 220 * 1024;
 }
 
 // Blocks that an SM holds.
@@ -371,11 +373,9 @@ template <typename T, int NT, int RUNS, int W> cudaError_t launch_few_with(Few p
 // Blocks of 8 warps, or of 16 that share their columns where an SM holds more warps so: 16 x 4096 x 32768 (the columns take 131 KB) 33.2 us,
 // 51.6 with 8 warps; 8 rows 26.7 and 32.3; 12 x 4096 x 4096 9.6 and 13.9.
 template <typename T, int NT, int RUNS> cudaError_t launch_few_as(const Few &p, cudaStream_t st) {
-    if constexpr (NT < 3) {
-        const size_t wide = few_bytes(p.cols, p.q.blocks, 2 * kFewWarps);
-        if (wide <= 220 * 1024 && 2 * few_resident(NT, 2 * kFewWarps, wide) > few_resident(NT, kFewWarps, few_bytes(p.cols, p.q.blocks)))
-            return launch_few_with<T, NT, RUNS, 2 * kFewWarps>(p, st);
-    }
+    const size_t wide = few_bytes(p.cols, p.q.blocks, 2 * kFewWarps);
+    if (wide <= 220 * 1024 && 2 * few_resident(NT, 2 * kFewWarps, wide) > few_resident(NT, kFewWarps, few_bytes(p.cols, p.q.blocks)))
+        return launch_few_with<T, NT, RUNS, 2 * kFewWarps>(p, st);
     return launch_few_with<T, NT, RUNS, kFewWarps>(p, st);
 }
 template <typename T, int NT> cudaError_t launch_few_cols(const Few &p, cudaStream_t st) {
@@ -384,7 +384,9 @@ template <typename T, int NT> cudaError_t launch_few_cols(const Few &p, cudaStre
 template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) {
     Few p{q, (int)q.rows * kPieces<T>, 1, 0};
     while (128 << p.shift < q.group) p.shift++;
-    return p.cols <= 8 ? launch_few_cols<T, 1>(p, st) : p.cols <= 16 ? launch_few_cols<T, 2>(p, st) : launch_few_cols<T, 3>(p, st);
+    if constexpr (kPieces<T> > 1)
+        if (p.cols > 16) return launch_few_cols<T, 3>(p, st);
+    return p.cols <= 8 ? launch_few_cols<T, 1>(p, st) : launch_few_cols<T, 2>(p, st);
 }
 
 // --------------------------------------------------------------------------------------------------- many rows
