@@ -112,6 +112,21 @@ def test_blocks_of_more_warps(rows, k, n, group, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,n,group", [(17, 1024, 300, 128), (20, 16384, 130, 32), (33, 4097, 1000, 512), (50, 16300, 7, 2048),
+                                            (100, 2500, 2000, 64), (128, 9000, 129, 128), (130, 6000, 128, 131072), (200, 3000, 513, 32),
+                                            (64, 1100, 64, 1024)])
+def test_clusters_that_share_the_inputs(rows, k, n, group, dtype):
+    f, _, pack = ops()
+    x = inputs(rows, k, dtype, seed=k) / 16
+    codes, scale, b = weights(n, k, group, dtype, seed=n)
+    w = pack(codes, scale, group)
+    y = f(x, w, b)
+    check(y, x, codes, scale, group, b, dtype)
+    assert torch.equal(y, f(x, w, b))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,k,n", [(1, 131072, 40), (3, 131072, 5), (20, 100003, 300), (130, 65552, 130)])
 def test_long_rows_with_the_largest_codes(rows, k, n):
     f, _, pack = ops()

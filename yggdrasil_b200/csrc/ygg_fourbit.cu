@@ -392,12 +392,15 @@ template <typename T> cudaError_t launch_few(const FourBit &q, cudaStream_t st) 
 // --------------------------------------------------------------------------------------------------- many rows
 //
 // D[channel][row] on tcgen05 (kind::f16): 128 channels along M, up to 128 rows of x along N, blocks of 128 inputs. TMA brings a block's codes and
-// the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; eight warps turn the codes into 16-bit
-// integers in tensor memory, the products' other operand; one warp issues the products. The sums of a turn (a group, or 512 inputs of a
-// longer one) lie in tensor memory too, in one of two places (four of up to 64 rows), and eight warps multiply them by the scales and add them
-// up in registers while the next turns are summed: the scale is applied to float sums, as in the other kernels. A block is persistent over tiles.
-// Shared memory's bandwidth bounds it (the rows of x are written and read once a product, the codes once): with the integers in shared memory
-// too, written and read there, 256 x 4096 x 16384 took 60.6 us, @A@ so.
+// the rows of x (for floats the three pieces that a launch before this one wrote) into a ring of stages; four warps turn the codes into 16-bit
+// integers in tensor memory, the products' other operand (in shared memory they would be written and read there, and only three stages fit); one
+// lane issues the products. The sums of a turn (a group, or 512 inputs of a longer one) lie in tensor memory too, in one of two places (four of up
+// to 64 rows), and eight warps multiply them by the scales and add them up in registers while the next turns are summed: the scale is applied to
+// float sums, as in the other kernels. A block is persistent over tiles; few tiles are shared by clusters, which join their parts over shared memory.
+//
+// 256 x 4096 x 16384: 42 us, half the tensor rate (256 tiles on 148 processors take two rounds, 0.86); 2048 rows 266 us, 0.63. A stage of
+// 128 rows takes 1 050 cycles, its products 512, turning the codes and reading the sums 600 each, and their waits for each other the rest. Of few rows
+// (32 x 4096 x 32768: 33.5 us) the codes are the longest. With the products under a condition on the lane, each took 140 cycles to issue: 61 us.
 //
 // Every wait is bounded: one that runs out raises the library's fault word (ygg_linear_status), gives its copies in flight time to land and
 // leaves.
@@ -411,7 +414,8 @@ __device__ int g_fault;   // a bounded wait ran out
 struct Many {
     int64_t rows, n;
     int blocks, groups, group_log, scale_dtype;   // blocks: of 128 inputs
-    int tn, pieces, stages, channel_blocks, row_blocks, turn;   // turn: steps of 16 inputs
+    int tn, stages, channel_blocks, row_blocks, turn;   // turn: steps of 16 inputs
+    int split, per;   // blocks that share a tile's inputs (a cluster), and the blocks of inputs of each
     const void *scale;
     const float *bias;
     int out_dtype;
@@ -423,13 +427,16 @@ struct ManyShared {   // at the end of dynamic shared memory
     uint32_t tmem;
 };
 
-// E: the type of the products' operands. P: pieces of an entry of x.
-template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
+// E: the type of the products' operands. P: pieces of an entry of x. SHARED: a cluster shares a tile's inputs.
+template <typename E, int P, bool SHARED> __global__ void __launch_bounds__(kManyThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap x_map, const Many p) {
     extern __shared__ __align__(1024) uint8_t ring[];
     ManyShared &sh = *(ManyShared *)(ring + kRing);
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (a value that the whole warp shares)
     const int tiles = p.channel_blocks * p.row_blocks;
+    // this block's tiles and its part of their inputs
+    const int mine = SHARED ? blockIdx.x / p.split : blockIdx.x, rank = SHARED ? blockIdx.x - mine * p.split : 0, step = SHARED ? tiles : gridDim.x;
+    const int kb0 = SHARED ? rank * p.per : 0, blocks = SHARED ? min(p.blocks - kb0, p.per) : p.blocks;
     // a stage: the rows of x (pieces, two parts of 64 inputs each), the codes
     const int x_part = p.tn * 128, stage_bytes = P * 2 * x_part + kTile * 64;
     const auto rows_of = [&](int s) { return ring + s * stage_bytes; };
@@ -461,15 +468,15 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             int s = 0;
             uint32_t phase = 1;
             wait_for_previous();   // the pieces of x
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int t = mine; t < tiles && ok; t += step) {
                 const int cb = t % p.channel_blocks, row = t / p.channel_blocks * p.tn;
-                for (int kb = 0; kb < p.blocks; kb++) {
+                for (int kb = 0; kb < blocks; kb++) {
                     if (!(ok = mbar_wait_bounded(smem_addr(&sh.empty[s]), phase))) break;
                     const uint32_t bar = smem_addr(&sh.full[s]);
                     mbar_expect_tx(bar, P * 2 * x_part + kTile * 64);
-                    tma_load<1>(smem_addr(codes_at(s)), &codes_map, kb * 64, cb * kTile, bar);
+                    tma_load<1>(smem_addr(codes_at(s)), &codes_map, (kb0 + kb) * 64, cb * kTile, bar);
                     for (int i = 0; i < 2 * P; i++)
-                        tma_load<1>(smem_addr(rows_of(s)) + i * x_part, &x_map, kb * 128 + (i & 1) * 64, (i >> 1) * (int)p.rows + row, bar);
+                        tma_load<1>(smem_addr(rows_of(s)) + i * x_part, &x_map, (kb0 + kb) * 128 + (i & 1) * 64, (i >> 1) * (int)p.rows + row, bar);
                     if (++s == p.stages) s = 0, phase ^= 1;
                 }
             }
@@ -479,7 +486,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             const uint32_t shape = product_f16(kTile, p.tn, std::is_same<E, __nv_bfloat16>::value);
             const uint64_t part = x_part >> 4, b0 = operand_128b(smem_addr(rows_of(0)));
             const uint32_t places = (1u << place_log) - 1;
-            const int blocks = p.blocks, stages = p.stages;
+            const int stages = p.stages;
             int s = 0, turn = 0;
             uint32_t phase = 0;
             // the products of steps first .. first + count - 1 of a stage
@@ -497,7 +504,7 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
             const auto drained = [&] {
                 return mbar_wait_bounded(smem_addr(&sh.drained[turn & places]), (turn >> place_log & 1) ^ 1);
             };
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int t = mine; t < tiles && ok; t += step) {
                 int left = p.turn / 8;   // blocks that the turn still has
                 for (int kb = 0; kb < blocks; kb++) {
                     if (!(ok = mbar_wait_bounded(smem_addr(&sh.ready[s]), phase))) break;   // (who makes the codes ready has waited for the stage's copies)
@@ -536,8 +543,8 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
         const int r = threadIdx.x - kSumWarps * 32;
         int s = 0;
         uint32_t phase = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int kb = 0; kb < p.blocks; kb++) {
+        for (int t = mine; t < tiles && ok; t += step) {
+            for (int kb = 0; kb < blocks; kb++) {
                 if (!(ok = __all_sync(~0u, mbar_wait_bounded(smem_addr(&sh.full[s]), phase)))) break;
                 const uint8_t *from = codes_at(s) + r * 64;
                 const uint32_t to = tmem + kSumCols + s * kStageCols + ((uint32_t)(r & 96) << 16);
@@ -565,14 +572,14 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
     } else {                                       // sums
         const int quad = warp & 3, half = warp >> 2;   // lanes of tensor memory; columns in chunks of 32, every other one
         int turn = 0;
-        const int turns = (p.blocks * 8 + p.turn - 1) / p.turn;
+        const int turns = (blocks * 8 + p.turn - 1) / p.turn;
         const bool wide = p.scale_dtype == YGG_DTYPE_FLOAT;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (int t = mine; t < tiles && ok; t += step) {
             const int64_t row0 = (int64_t)(t / p.channel_blocks) * p.tn, ch = (int64_t)(t % p.channel_blocks) * kTile + quad * 32 + lane;
             const bool live = ch < p.n;
             const int64_t scales = (live ? ch : 0) * p.groups;
             const auto scale_at = [&](int turn) {
-                const int g = min(turn * p.turn * 16 >> p.group_log, p.groups - 1);   // (past k: on zeros)
+                const int g = min((kb0 * 8 + turn * p.turn) * 16 >> p.group_log, p.groups - 1);   // (past k: on zeros)
                 return wide ? ((const uint32_t *)p.scale)[scales + g] : (uint32_t)((const uint16_t *)p.scale)[scales + g];
             };
             float acc[2][32];
@@ -614,7 +621,13 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
                     turn++;
                 }
             }
-            if (ok && live) {
+            if constexpr (SHARED) {   // what its part adds, where the copies were: [row][channel]
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if ((2 * c + half) * 32 + j < p.tn) ((float *)ring)[((2 * c + half) * 32 + j) * kTile + quad * 32 + lane] = acc[c][j];
+            } else if (ok && live) {
                 const float bias = p.bias ? p.bias[ch] : 0.0f;
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
@@ -634,6 +647,20 @@ template <typename E, int P> __global__ void __launch_bounds__(kManyThreads, 1)
         while (clock64() - t0 < 50000000LL) {}
     }
     __syncwarp();
+    if constexpr (SHARED) {   // a block adds up some of the tile's rows, over the parts in their order
+        cluster_sync();
+        const int64_t row0 = (int64_t)(mine / p.channel_blocks) * p.tn, ch = (int64_t)(mine % p.channel_blocks) * kTile + (threadIdx.x & 127);
+        const int rows = (int)min(p.rows - row0, (int64_t)p.tn), end = rows * (rank + 1) / p.split;
+        if (ch < p.n && threadIdx.x < kManyThreads / 128 * 128)
+            for (int r = rows * rank / p.split + threadIdx.x / 128; r < end; r += kManyThreads / 128) {
+                const uint32_t at = smem_addr(ring) + (r * kTile + (threadIdx.x & 127)) * 4;
+                float v = 0.0f;
+                for (int i = 0; i < p.split; i++) v += load_at_rank(at, i);
+                store_as(p.out_dtype, p.out, (row0 + r) * p.out_stride + ch, v + (p.bias ? p.bias[ch] : 0.0f));
+            }
+        __syncwarp();
+        cluster_sync();
+    }
     tmem_fence_before();
     __syncthreads();
     if (warp == kSumWarps + kCodeWarps) tmem_free<1>(tmem, kTmemCols);
@@ -681,9 +708,7 @@ template <typename T> bool in_place(const void *x, int64_t rows, int64_t stride,
 template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t st) {
     using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
     constexpr int P = kPieces<T>;
-    static SmemLimits limits;
     const size_t smem = kRing + sizeof(ManyShared);
-    if (raise_smem_limit((const void *)many_kernel<E, P>, smem, limits) != cudaSuccess) return YGG_E_CUDA;
     const bool copied = !in_place<T>(q.x, q.rows, q.x_stride, q.k);
     const int padded = padded_of(q.k);
     if (copied) {
@@ -693,7 +718,7 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
         cfg.stream = st;
         if (cudaLaunchKernelEx(&cfg, pieces_kernel<T>, q, (uint16_t *)room, padded) != cudaSuccess) return YGG_E_CUDA;
     }
-    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, P, 0, (int)((q.n + kTile - 1) / kTile), 0, 0, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
+    Many p{q.rows, q.n, q.blocks, q.groups, 0, q.scale_dtype, 0, 0, (int)((q.n + kTile - 1) / kTile), 0, 0, 1, q.blocks, q.scale, q.bias, q.out_dtype, q.out, q.out_stride};
     while (1 << p.group_log < q.group) p.group_log++;
     p.turn = std::min(q.group, kTurn) / 16;
     // rows of a tile: equal parts of up to 128 (64 of floats, whose pieces take three times the room)
@@ -708,17 +733,38 @@ template <typename T> int launch_many(const FourBit &q, void *room, cudaStream_t
         !map_tiles(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT16, copied ? room : q.x, copied ? padded : q.k, P * q.rows,
                    copied ? padded * 2 : (q.rows == 1 ? padded : q.x_stride) * 2, 64, p.tn, CU_TENSOR_MAP_SWIZZLE_128B))
         return YGG_E_CUDA;
+    // Few tiles: a cluster shares the inputs of each, in whole turns. A block of inputs takes about half a microsecond, the join one to three, more of
+    // more rows: 20 x 16384 x 1000 in eight parts 12.2 us, 57.1 in one; 20 x 1000 x 5003 in two 8.0 and 9.4; but 128 x 512 x 4096 in two 12.7 and 8.0.
+    // (Clusters of eight do not fill the processors: 16 of them took two rounds.)
+    const int64_t tiles = (int64_t)p.channel_blocks * p.row_blocks;
+    const int unit = std::max(1, p.turn / 8);
+    while (p.split < 8 && tiles * p.split * 2 <= (p.split < 4 ? sm_count() : sm_count() * 3 / 4) &&
+           p.blocks / (2 * p.split) >= (p.split == 1 ? 3 + p.tn / 32 : 2 + p.tn / 64))
+        p.split *= 2;
+    p.per = ((p.blocks + p.split - 1) / p.split + unit - 1) / unit * unit;
+    while (p.per * (p.split - 1) >= p.blocks) p.split /= 2, p.per = ((p.blocks + p.split - 1) / p.split + unit - 1) / unit * unit;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)p.channel_blocks * p.row_blocks, sm_count()));
+    cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sm_count())));
     cfg.blockDim = dim3(kManyThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = copied ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, many_kernel<E, P>, codes_map, x_map, p) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
+    if (p.split > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)p.split;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+    }
+    if (copied) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs++;
+    }
+    static SmemLimits limits[2];
+    const auto kernel = p.split > 1 ? many_kernel<E, P, true> : many_kernel<E, P, false>;
+    if (raise_smem_limit((const void *)kernel, smem, limits[p.split > 1]) != cudaSuccess) return YGG_E_CUDA;
+    return cudaLaunchKernelEx(&cfg, kernel, codes_map, x_map, p) == cudaSuccess ? YGG_OK : YGG_E_CUDA;
 }
 
 // Rows beyond what one launch counts its tiles over take several.
